@@ -469,6 +469,134 @@ extern "C" {
         d_dx: *mut c_void,
         accumulate: c_int,
     ) -> c_int;
+    pub fn fg_layer_norm(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_x: *const c_void,
+        ldx: c_int,
+        d_gamma: *const c_void,
+        d_beta: *const c_void,
+        eps: f32,
+        R: c_int,
+        C: c_int,
+        d_y: *mut c_void,
+        ldy: c_int,
+        d_mean: *mut f32,
+        d_rstd: *mut f32,
+    ) -> c_int;
+    pub fn fg_layer_norm_bwd(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_x: *const c_void,
+        ldx: c_int,
+        d_dy: *const c_void,
+        lddy: c_int,
+        d_gamma: *const c_void,
+        d_mean: *const f32,
+        d_rstd: *const f32,
+        R: c_int,
+        C: c_int,
+        d_dx: *mut c_void,
+        lddx: c_int,
+        accumulate: c_int,
+        d_dgamma: *mut c_void,
+        dgamma_accumulate: c_int,
+        d_dbeta: *mut c_void,
+        dbeta_accumulate: c_int,
+    ) -> c_int;
+    pub fn fg_embedding(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_tokens: *const u32,
+        T: c_int,
+        V: c_int,
+        C: c_int,
+        d_table: *const c_void,
+        ldt: c_int,
+        scale: f32,
+        d_out: *mut c_void,
+        ldo: c_int,
+    ) -> c_int;
+    pub fn fg_embedding_bwd(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_tokens: *const u32,
+        T: c_int,
+        V: c_int,
+        C: c_int,
+        d_dout: *const c_void,
+        lddo: c_int,
+        scale: f32,
+        d_dtable: *mut c_void,
+        lddt: c_int,
+        accumulate: c_int,
+    ) -> c_int;
+    pub fn fg_ckpt8_save(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_x: *const c_void,
+        ldx: c_int,
+        R: c_int,
+        C: c_int,
+        d_q: *mut i8,
+        ldq: c_int,
+        d_e: *mut u8,
+        lde: c_int,
+    ) -> c_int;
+    pub fn fg_ckpt8_load(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        act: c_int,
+        d_q: *const i8,
+        ldq: c_int,
+        d_e: *const u8,
+        lde: c_int,
+        R: c_int,
+        C: c_int,
+        d_z: *mut c_void,
+        ldz: c_int,
+        d_h: *mut c_void,
+        ldh: c_int,
+    ) -> c_int;
+    pub fn fg_act_bwd_ckpt8(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        act: c_int,
+        d_dH: *const c_void,
+        lddh: c_int,
+        d_q: *const i8,
+        ldq: c_int,
+        d_e: *const u8,
+        lde: c_int,
+        R: c_int,
+        C: c_int,
+        d_dZ: *mut c_void,
+        lddz: c_int,
+    ) -> c_int;
+    pub fn fg_matmul_bwd_ckpt8(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        M: c_int,
+        N: c_int,
+        K: c_int,
+        act: c_int,
+        d_q: *const i8,
+        ldq: c_int,
+        d_e: *const u8,
+        lde: c_int,
+        d_W: *const c_void,
+        ldw: c_int,
+        d_dZ: *const c_void,
+        lddz: c_int,
+        d_Zr: *mut c_void,
+        d_Xr: *mut c_void,
+        d_dX: *mut c_void,
+        lddx: c_int,
+        d_dW: *mut c_void,
+        lddw: c_int,
+        d_dbias: *mut c_void,
+        accumulate: c_int,
+    ) -> c_int;
     pub fn fg_mt_create(
         ctx: *mut fg_ctx,
         n: c_int,

@@ -190,6 +190,66 @@ class Context:
         call("fg_softmax_bwd", self.handle, dtype, _ptr(y), _ptr(dy), R, C, _ptr(dx),
              int(accumulate))
 
+    def layer_norm(self, x, ldx: int, R: int, C: int, y, ldy: int, gamma=None, beta=None,
+                   eps: float = 1e-5, mean=None, rstd=None, dtype: int = DTYPE_F32) -> None:
+        """y = (x - mean) * rstd * gamma + beta per row; mean and rstd (fp32,
+        one per row) are kept when given."""
+        call("fg_layer_norm", self.handle, dtype, _ptr(x), ldx, _ptr(gamma), _ptr(beta), eps, R, C,
+             _ptr(y), ldy, _ptr(mean), _ptr(rstd))
+
+    def layer_norm_bwd(self, x, ldx: int, dy, lddy: int, mean, rstd, R: int, C: int, gamma=None,
+                       dx=None, lddx: int = 0, dgamma=None, dbeta=None, accumulate: bool = False,
+                       dgamma_accumulate: bool = False, dbeta_accumulate: bool = False,
+                       dtype: int = DTYPE_F32) -> None:
+        """dx, dgamma and dbeta (any may be None) from x, dy and the forward's
+        mean and rstd."""
+        call("fg_layer_norm_bwd", self.handle, dtype, _ptr(x), ldx, _ptr(dy), lddy, _ptr(gamma),
+             _ptr(mean), _ptr(rstd), R, C, _ptr(dx), lddx or C, int(accumulate), _ptr(dgamma),
+             int(dgamma_accumulate), _ptr(dbeta), int(dbeta_accumulate))
+
+    def embedding(self, tokens, T: int, V: int, C: int, table, ldt: int, out, ldo: int,
+                  scale: float = 1.0, dtype: int = DTYPE_F32) -> None:
+        """out[t] = scale * table[tokens[t]] (u32 tokens; a row of NaN for a
+        token outside the table)."""
+        call("fg_embedding", self.handle, dtype, _ptr(tokens), T, V, C, _ptr(table), ldt, scale,
+             _ptr(out), ldo)
+
+    def embedding_bwd(self, tokens, T: int, V: int, C: int, dout, lddo: int, dtable, lddt: int,
+                      scale: float = 1.0, accumulate: bool = False,
+                      dtype: int = DTYPE_F32) -> None:
+        """dtable[v] (=|+=) scale * sum of dout[t] over the t with tokens[t] = v."""
+        call("fg_embedding_bwd", self.handle, dtype, _ptr(tokens), T, V, C, _ptr(dout), lddo,
+             scale, _ptr(dtable), lddt, int(accumulate))
+
+    def ckpt8_save(self, x, ldx: int, R: int, C: int, q, ldq: int, e, lde: int,
+                   dtype: int = DTYPE_F32) -> None:
+        """x in 8 bits: int8 q[R][C] and a uint8 exponent e[R][ceil(C / 32)]
+        per 32 columns of a row."""
+        call("fg_ckpt8_save", self.handle, dtype, _ptr(x), ldx, R, C, _ptr(q), ldq, _ptr(e), lde)
+
+    def ckpt8_load(self, q, ldq: int, e, lde: int, R: int, C: int, z=None, ldz: int = 0, h=None,
+                   ldh: int = 0, act: int = ACT_NONE, dtype: int = DTYPE_F32) -> None:
+        """z = the values kept by ckpt8_save, h = act(z) (either may be None)."""
+        call("fg_ckpt8_load", self.handle, dtype, act, _ptr(q), ldq, _ptr(e), lde, R, C, _ptr(z),
+             ldz or C, _ptr(h), ldh or C)
+
+    def act_bwd_ckpt8(self, act: int, dH, lddh: int, q, ldq: int, e, lde: int, R: int, C: int, dZ,
+                      lddz: int, dtype: int = DTYPE_F32) -> None:
+        """dZ = dH * act'(z) with the pre-activation z kept by ckpt8_save."""
+        call("fg_act_bwd_ckpt8", self.handle, dtype, act, _ptr(dH), lddh, _ptr(q), ldq, _ptr(e),
+             lde, R, C, _ptr(dZ), lddz)
+
+    def matmul_bwd_ckpt8(self, M: int, N: int, K: int, q, ldq: int, e, lde: int, W, ldw: int, dZ,
+                         lddz: int, Xr, dX, lddx: int, dW, lddw: int, Zr=None, dbias=None,
+                         act: int = ACT_NONE, accumulate: bool = False,
+                         dtype: int = DTYPE_F32) -> None:
+        """matmul_bwd of X.W with X = act(z) and z[M][K] kept by ckpt8_save:
+        dW = act(z)^T.dZ (+ dbias = colsum(dZ)), dX = (dZ.W^T) * act'(z).  Xr
+        and (with an activation) Zr are scratch of M x K elements."""
+        call("fg_matmul_bwd_ckpt8", self.handle, dtype, M, N, K, act, _ptr(q), ldq, _ptr(e), lde,
+             _ptr(W), ldw, _ptr(dZ), lddz, _ptr(Zr), _ptr(Xr), _ptr(dX), lddx, _ptr(dW), lddw,
+             _ptr(dbias), int(accumulate))
+
     def fill_u32(self, dst, value: int, count: int) -> None:
         call("fg_fill_u32", self.handle, _ptr(dst), value, count)
 

@@ -37,6 +37,9 @@ SOURCES = [
     "k_gemm16_f16.hip",
     "k_eltwise_prog.hip",
     "k_noalloc.hip",
+    "k_layer_norm.hip",
+    "k_embedding.hip",
+    "k_ckpt8.hip",
     "fg_graph.cpp",
     "fg_bpat.cpp",
     "fg_telemetry.cpp",

@@ -86,6 +86,16 @@ SIGNATURES = {
     "fg_softmax_ce_f32": (i32, [vp, vp, i32, vp, i32, i32, f32, vp, vp, vp, i32, vp]),
     "fg_softmax_f32": (i32, [vp, vp, i32, i32, vp]),
     "fg_softmax_bwd_f32": (i32, [vp, vp, vp, i32, i32, vp, i32]),
+    "fg_layer_norm": (i32, [vp, i32, vp, i32, vp, vp, f32, i32, i32, vp, i32, vp, vp]),
+    "fg_layer_norm_bwd": (i32, [vp, i32, vp, i32, vp, i32, vp, vp, vp, i32, i32, vp, i32, i32, vp,
+                                i32, vp, i32]),
+    "fg_embedding": (i32, [vp, i32, vp, i32, i32, i32, vp, i32, f32, vp, i32]),
+    "fg_embedding_bwd": (i32, [vp, i32, vp, i32, i32, i32, vp, i32, f32, vp, i32, i32]),
+    "fg_ckpt8_save": (i32, [vp, i32, vp, i32, i32, i32, vp, i32, vp, i32]),
+    "fg_ckpt8_load": (i32, [vp, i32, i32, vp, i32, vp, i32, i32, i32, vp, i32, vp, i32]),
+    "fg_act_bwd_ckpt8": (i32, [vp, i32, i32, vp, i32, vp, i32, vp, i32, i32, i32, vp, i32]),
+    "fg_matmul_bwd_ckpt8": (i32, [vp, i32, i32, i32, i32, i32, vp, i32, vp, i32, vp, i32, vp, i32,
+                                  vp, vp, vp, i32, vp, i32, vp, i32]),
     "fg_mt_create": (i32, [vp, i32, vp, vp, vp, vp, vp, pvp]),
     "fg_mt_destroy": (i32, [vp]),
     "fg_sgd_step": (i32, [vp, vp, f32, i32]),

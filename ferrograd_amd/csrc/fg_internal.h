@@ -133,6 +133,11 @@ int gemm16_dw_dx_dispatches(fg_ctx *ctx, int M1, int N1, int K1, const void *A1,
                             const void *B1, int ldb1, int M2, int N2, int K2, const void *A2,
                             int lda2, const void *B2, int ldb2);
 
+// Workspace bytes of fg_layer_norm_bwd with weight gradients on a device with
+// `cus` compute units, and of fg_embedding_bwd.
+uint64_t layer_norm_bwd_ws_bytes(int cus, int R, int C);
+uint64_t embedding_bwd_ws_bytes(int T, int V, int C);
+
 // Adam with device-resident step counter / bias-correction scalars
 // (k_optim.hip).  d_state points at adam_dev_state_bytes() zeroed bytes.
 uint64_t adam_dev_state_bytes();

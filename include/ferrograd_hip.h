@@ -299,6 +299,82 @@ int fg_softmax(fg_ctx *ctx, int dtype, const void *d_x, int R, int C, void *d_y)
 int fg_softmax_bwd(fg_ctx *ctx, int dtype, const void *d_y, const void *d_dy, int R,
                    int C, void *d_dx, int accumulate);
 
+/* -------------------------------------------------- token-model operators */
+/* Layer norm over the last dimension (no reference counterpart; the row
+ * operator next to the softmax node, op/softmax.rs:14-759).  Per row r:
+ *   mean = sum(x_r) / C ; var = sum((x_r - mean)^2) / C ; rstd = 1/sqrt(var + eps)
+ *   y_r = (x_r - mean) * rstd * gamma + beta
+ * x, y, gamma[C], beta[C] of element type dtype, statistics and sums fp32, y
+ * rounded once.  gamma (1) and beta (0) may be NULL; d_mean / d_rstd [R]
+ * (fp32, what the backward needs) may be NULL.  y may be x (ldy = ldx).
+ * eps > 0. */
+int fg_layer_norm(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const void *d_gamma,
+                  const void *d_beta, float eps, int R, int C, void *d_y, int ldy,
+                  float *d_mean, float *d_rstd);
+/* Its backward from x, dy and the saved statistics, xh = (x - mean) * rstd,
+ * g = dy * gamma:
+ *   dx (=|+=) rstd * (g - mean(g) - xh * mean(g * xh))
+ *   dgamma (=|+=) sum over rows of dy * xh ;  dbeta (=|+=) sum over rows of dy
+ * Any output may be NULL; gamma may be NULL (1).  dx may be x or dy (equal
+ * leading dimensions) unless it accumulates.  The rows' partial sums of
+ * dgamma and dbeta go to the workspace, 8 bytes a column for each of at most
+ * 1024 row splits, and are added in a fixed order.  R = 0 writes zeros to
+ * dgamma and dbeta (or adds nothing). */
+int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const void *d_dy,
+                      int lddy, const void *d_gamma, const float *d_mean, const float *d_rstd,
+                      int R, int C, void *d_dx, int lddx, int accumulate, void *d_dgamma,
+                      int dgamma_accumulate, void *d_dbeta, int dbeta_accumulate);
+
+/* Embedding lookup (no reference counterpart): out[t][c] = scale *
+ * table[tokens[t]][c] for T tokens and a table of V rows of C elements of
+ * type dtype, rounded once.  A token outside [0, V) gives a row of NaN, as a
+ * label outside its classes does in fg_softmax_ce. */
+int fg_embedding(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T, int V, int C,
+                 const void *d_table, int ldt, float scale, void *d_out, int ldo);
+/* The table's gradient by sorted tokens:
+ *   dtable[v][c] (=|+=) scale * sum of dout[t][c] over t with tokens[t] = v
+ * Sums in fp32 in an order fixed by the tokens (no atomics), rounded once.
+ * Without accumulate every row of dtable is written (rows of no token: 0),
+ * with it rows of no token are left as they are.  Tokens outside [0, V) add
+ * to nothing.  The sort and the partial sums use the workspace. */
+int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T, int V, int C,
+                     const void *d_dout, int lddo, float scale, void *d_dtable, int lddt,
+                     int accumulate);
+
+/* Activation checkpoints in 8 bits (no reference counterpart: its forward_saved
+ * tensors keep their type, dispatch/mod.rs:509-575).  A matrix x[R][C] of
+ * type dtype becomes int8 elements q[R][C] (ld ldq) and one exponent byte
+ * e[R][ceil(C / 32)] (ld lde) per 32 columns of a row.  With b = max(1, exponent
+ * field of the block's largest |x| as fp32), stored in e:
+ *   q = clamp(rint(x * 2^(133 - b)), -127, 127) ;  restored z = q * 2^(b - 133)
+ * (the OCP MX format with INT8 elements and E8M0 scales).  The restored value
+ * is exact in every dtype; it is off by at most 2^(b - 134), half of
+ * 1/64 of the power of two below the block's largest |x|, except that values
+ * above 127.5 steps restore as 127.  A block with an infinity or NaN gets
+ * b = 255 and restores as NaN. */
+int fg_ckpt8_save(fg_ctx *ctx, int dtype, const void *d_x, int ldx, int R, int C, int8_t *d_q,
+                  int ldq, uint8_t *d_e, int lde);
+/* z = the restored values, h = act(z) rounded once; either may be NULL. */
+int fg_ckpt8_load(fg_ctx *ctx, int dtype, int act, const int8_t *d_q, int ldq,
+                  const uint8_t *d_e, int lde, int R, int C, void *d_z, int ldz, void *d_h,
+                  int ldh);
+/* fg_act_bwd_f32 for any dtype with the pre-activation in 8 bits:
+ * dZ = dH * act'(z), rounded once.  dZ may be dH (lddz = lddh). */
+int fg_act_bwd_ckpt8(fg_ctx *ctx, int dtype, int act, const void *d_dH, int lddh,
+                     const int8_t *d_q, int ldq, const uint8_t *d_e, int lde, int R, int C,
+                     void *d_dZ, int lddz);
+/* fg_matmul_bwd_f32 / _x16 for C = X.W with X = act(z) and z[M][K], the
+ * pre-activation of X's producer, kept in 8 bits:
+ *   dW (=|+=) act(z)^T.dZ [K][N], dbias (=|+=) colsum(dZ) (or NULL)
+ *   dX (=|+=) (dZ.W^T) * act'(z) [M][K]
+ * d_Xr and (with an activation) d_Zr are the caller's scratch, M x K elements
+ * of dtype each, overwritten with act(z) and z as the products read them. */
+int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int act,
+                        const int8_t *d_q, int ldq, const uint8_t *d_e, int lde,
+                        const void *d_W, int ldw, const void *d_dZ, int lddz, void *d_Zr,
+                        void *d_Xr, void *d_dX, int lddx, void *d_dW, int lddw, void *d_dbias,
+                        int accumulate);
+
 /* ----------------------------------------- multi-tensor optimiser lists */
 /* One launch updates every tensor of the list.  Replaces the per-tensor
  * optimiser kernels captured one launch per input tensor
