@@ -8,84 +8,632 @@
 // The gradient's sums run in fp32 in an order fixed by the tokens alone, so
 // equal calls give equal bits (no atomics).  Tokens outside the table add to
 // nothing.
+//
+// Both are bound by HBM (the rows they read and write once).  The gradient:
+//  * the positions in (token, position) order: by counting, for each position, the
+//    ones before it (up to kRankMax tokens, one launch: T^2 / 64 two-instruction
+//    steps spread over all CUs), by a stable radix sort above;
+//  * the sorted positions in units of equal length, so that a token that fills half
+//    the batch is spread over the GPU as evenly as any other: a unit adds its runs
+//    of equal tokens, writes the rows of runs that it holds whole, and leaves the
+//    runs that cross its ends as fp32 partial sums; workgroups of the same launch
+//    zero the rows of no token;
+//  * the crossing runs' partial sums are joined in order.
+// A few tokens (kDirectMax) take one launch: every workgroup owns some table rows
+// and lists the tokens that are its own.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 
 #include "fg_half.h"
 #include "fg_internal.h"
+#include "fg_rows.h"
 
 namespace {
 
-constexpr int kNT = 256;
+using fg::rows::Io;
+using fg::rows::u32x4;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-__global__ __launch_bounds__(kNT) void emb_fwd(int dt, const uint32_t *tokens, int V, int C,
-                                               const void *table, int ldt, float scale, void *out,
-                                               int ldo) {
-    const uint64_t t = blockIdx.x;
+constexpr int kNT = 256;
+constexpr int kDirectMax = 256;
+constexpr int kRankMax = 16384;
+
+// A row's chunk j where j is below its whole chunks nb, or (j == nb) its last,
+// partial one, one element after the other.
+template <int DT>
+struct Chunk {
+    using IO = Io<DT>;
+    static constexpr int E = IO::E;
+    static __device__ __forceinline__ u32x4 load(const typename IO::T *row, int j, int nb, int C) {
+        if (j < nb) return fg::rows::load<DT>(row, j);
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = j * E + e < C ? IO::load1(row, j * E + e) : 0.0f;
+        return IO::pack(v);
+    }
+    static __device__ __forceinline__ void store(typename IO::T *row, int j, int nb, int C,
+                                                 const float (&v)[E]) {
+        if (j < nb) {
+            fg::rows::store<DT>(row, j, IO::pack(v));
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (j * E + e < C) IO::store1(row, j * E + e, v[e]);
+    }
+};
+
+// ------------------------------------------------------------------- lookup
+// 2^lshift lanes take a row, UNR chunks in flight a lane.
+template <int DT>
+__global__ __launch_bounds__(kNT) void emb_fwd(const uint32_t *__restrict__ tokens, int T, int V,
+                                               int C, const typename Io<DT>::T *__restrict__ table,
+                                               int ldt, float scale, typename Io<DT>::T *out,
+                                               int ldo, int lshift) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E, UNR = 4;
+    const int lanes = 1 << lshift, lane = threadIdx.x & (lanes - 1);
+    const int64_t t = ((int64_t)blockIdx.x << (8 - lshift)) + (threadIdx.x >> lshift);
+    if (t >= T) return;
     const uint32_t v = tokens[t];
     const bool in = v < (uint32_t)V;
-    for (int c = threadIdx.x; c < C; c += kNT)
-        fg::store_from_f(out, dt, t * ldo + c,
-                         in ? scale * fg::load_as_f(table, dt, (uint64_t)v * ldt + c)
-                            : __builtin_nanf(""));
-}
-
-// order[k] = the k-th token position in (token, position) order, sorted[k] its
-// token.  A thread counts the positions before its own.
-__global__ __launch_bounds__(kNT) void emb_rank(const uint32_t *tokens, int T, uint32_t *order,
-                                                uint32_t *sorted) {
-    const int i = blockIdx.x * kNT + threadIdx.x;
-    if (i >= T) return;
-    const uint32_t mine = tokens[i];
-    int before = 0;
-    for (int j = 0; j < T; ++j) {
-        const uint32_t o = tokens[j];
-        before += (o < mine || (o == mine && j < i)) ? 1 : 0;
+    const auto *row = table + (size_t)(in ? v : 0) * ldt;
+    auto *to = out + (size_t)t * ldo;
+    const float k = in ? scale : __builtin_nanf("");
+    const int nb = C / E, chunks = (C - 1) / E + 1;
+    auto put = [&](int j, u32x4 w) {
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = in ? k * IO::get(w, e) : k;
+        Chunk<DT>::store(to, j, nb, C, o);
+    };
+    int j = lane;
+    for (; j + (UNR - 1) * lanes < nb; j += UNR * lanes) {
+        u32x4 w[UNR];
+#pragma unroll
+        for (int u = 0; u < UNR; ++u) w[u] = fg::rows::load<DT>(row, j + u * lanes);
+#pragma unroll
+        for (int u = 0; u < UNR; ++u) put(j + u * lanes, w[u]);
     }
-    order[before] = (uint32_t)i;
-    sorted[before] = mine;
+    for (; j < chunks; j += lanes) put(j, Chunk<DT>::load(row, j, nb, C));
 }
 
-// First position of `sorted` that holds a value >= v.
-__device__ __forceinline__ int lower_bound(const uint32_t *sorted, int T, uint32_t v) {
-    int lo = 0, n = T;
-    while (n > 0) {
-        const int h = n >> 1;
-        if (sorted[lo + h] < v) {
-            lo += h + 1;
-            n -= h + 1;
-        } else {
-            n = h;
+// --------------------------------------------------- few tokens: one launch
+// A workgroup owns `rows` table rows from blockIdx.x * rows on: it lists the
+// positions of their tokens in order, then each group of 2^lshift lanes adds the
+// rows of its own tokens.
+template <int DT>
+__global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ tokens, int T,
+                                                   int V, int C,
+                                                   const typename Io<DT>::T *__restrict__ dout,
+                                                   int lddo, float scale,
+                                                   typename Io<DT>::T *dtable, int lddt,
+                                                   int accumulate, int rows, int lshift) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E;
+    static_assert(kDirectMax <= kNT, "one token a thread");
+    __shared__ uint32_t tok[kDirectMax + 8], at[kDirectMax + 8];  // (+ 8: read ahead)
+    __shared__ int count[kNT / 64];
+    const int lanes = 1 << lshift, lane = threadIdx.x & (lanes - 1);
+    const int64_t v0 = (int64_t)blockIdx.x * rows;
+    const int nrows = (int)min((int64_t)rows, V - v0);
+    const uint32_t mine = threadIdx.x < (unsigned)T ? tokens[threadIdx.x] : 0xffffffffu;
+    const bool hit = threadIdx.x < (unsigned)T && mine >= v0 && mine < v0 + nrows;
+    const uint64_t mask = __ballot(hit);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) count[wave] = __popcll(mask);
+    __syncthreads();
+    int base = 0, n = 0;
+#pragma unroll
+    for (int w = 0; w < kNT / 64; ++w) {
+        base += w < wave ? count[w] : 0;
+        n += count[w];
+    }
+    if (hit) {
+        const int k = base + __popcll(mask & ((1ull << (threadIdx.x & 63)) - 1));
+        tok[k] = mine;
+        at[k] = threadIdx.x;
+    }
+    __syncthreads();
+    const int nb = C / E, chunks = (C - 1) / E + 1;
+    for (int r = threadIdx.x >> lshift; r < nrows; r += kNT >> lshift) {
+        const uint32_t v = (uint32_t)(v0 + r);
+        auto *to = dtable + (size_t)v * lddt;
+        int first = n, last = -1;
+        for (int k = 0; k < n; ++k)
+            if (tok[k] == v) {
+                first = min(first, k);
+                last = k;
+            }
+        if (last < 0 && accumulate) continue;
+        for (int j = lane; j < chunks; j += lanes) {
+            float a[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) a[e] = 0.0f;
+            for (int k = first; k <= last; ++k) {
+                if (tok[k] != v) continue;
+                const u32x4 w = Chunk<DT>::load(dout + (size_t)at[k] * lddo, j, nb, C);
+#pragma unroll
+                for (int e = 0; e < E; ++e) a[e] += IO::get(w, e);
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) a[e] *= scale;
+            if (accumulate) {
+                const u32x4 was = Chunk<DT>::load(to, j, nb, C);
+#pragma unroll
+                for (int e = 0; e < E; ++e) a[e] += IO::get(was, e);
+            }
+            Chunk<DT>::store(to, j, nb, C, a);
         }
+    }
+}
+
+// ------------------------------------------------------------------- sorting
+// order[k] = the k-th position in (token, position) order, sorted[k] its token: a
+// lane counts the positions before its own, 16 waves a share of the tokens each.
+__global__ __launch_bounds__(1024) void emb_rank(const uint32_t *__restrict__ tokens, int T,
+                                                 uint32_t *__restrict__ order,
+                                                 uint32_t *__restrict__ sorted) {
+    __shared__ int sum[16][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g0 = blockIdx.x * 64, i = g0 + lane;
+    const uint32_t mine = i < T ? tokens[i] : 0xffffffffu;
+    const int per = (T + 15) / 16, j0 = wave * per, j1 = min(T, j0 + per);
+    int before = 0;
+    // Positions before the workgroup's 64, the 64, and those after them.
+    int j = j0;
+#pragma unroll 8
+    for (; j < min(j1, g0); ++j) before += tokens[j] <= mine;
+    for (; j < min(j1, g0 + 64); ++j) {
+        const uint32_t o = tokens[j];
+        before += o < mine || (o == mine && j < i);
+    }
+#pragma unroll 8
+    for (; j < j1; ++j) before += tokens[j] < mine;
+    sum[wave][lane] = before;
+    __syncthreads();
+    if (wave == 0 && i < T) {
+        before = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) before += sum[w][lane];
+        order[before] = (uint32_t)i;
+        sorted[before] = mine;
+    }
+}
+
+// Stable radix sort, least significant digit first, of (token, position) pairs:
+// tile b of the input counts its digits (radix_count: hist[digit][tile]), then
+// places its pairs behind those of smaller digits and of earlier tiles
+// (radix_place).  Tokens outside the table sort as V.
+constexpr int kMaxBits = 11, kBins = 1 << kMaxBits;
+constexpr int kTiles = 64;  // at most
+constexpr int kSortNT = 1024;
+
+__device__ __forceinline__ uint32_t key_of(uint32_t token, uint32_t V) { return min(token, V); }
+
+__global__ __launch_bounds__(kSortNT) void radix_count(const uint32_t *__restrict__ keys, int T,
+                                                       uint32_t V, int per, int shift, int bits,
+                                                       uint32_t *__restrict__ hist) {
+    __shared__ uint32_t h[kBins];
+    const int bins = 1 << bits;
+    for (int d = threadIdx.x; d < bins; d += kSortNT) h[d] = 0;
+    __syncthreads();
+    const int64_t i0 = (int64_t)blockIdx.x * per, i1 = min((int64_t)T, i0 + per);
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += kSortNT)
+        atomicAdd(&h[(key_of(keys[i], V) >> shift) & (bins - 1)], 1u);  // (counts: any order)
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += kSortNT)
+        hist[(size_t)d * gridDim.x + blockIdx.x] = h[d];
+}
+
+// pos NULL: the pairs' positions are their own indices (the first pass).
+__global__ __launch_bounds__(kSortNT) void radix_place(const uint32_t *__restrict__ keys,
+                                                       const uint32_t *__restrict__ pos, int T,
+                                                       uint32_t V, int per, int shift, int bits,
+                                                       const uint32_t *__restrict__ hist,
+                                                       uint32_t *__restrict__ keys_out,
+                                                       uint32_t *__restrict__ pos_out) {
+    constexpr int kWaves = kSortNT / 64;
+    // Pairs of digit d in the tile's wave w; then where they go.
+    __shared__ uint32_t cnt[kWaves][kBins];
+    __shared__ uint32_t base[kBins];
+    __shared__ uint32_t wsum[kWaves];
+    const int bins = 1 << bits, tiles = gridDim.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int k = threadIdx.x; k < kWaves * bins; k += kSortNT) cnt[k >> bits][k & (bins - 1)] = 0;
+    // base[d] = pairs of digit d in earlier tiles, and of smaller digits: a digit's
+    // tiles by consecutive threads' loads, then a scan over the digits.
+    constexpr int kOwn = kBins / kSortNT;  // digits of a thread
+    uint32_t total[kOwn], mine = 0;
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+        const int d = threadIdx.x * kOwn + u;
+        uint32_t before = 0, all = 0;
+        if (d < bins) {
+            const uint32_t *h = hist + (size_t)d * tiles;
+#pragma unroll 8
+            for (int b = 0; b < tiles; ++b) {
+                const uint32_t c = h[b];
+                all += c;
+                before += b < (int)blockIdx.x ? c : 0u;
+            }
+            base[d] = before;
+        }
+        total[u] = all;
+        mine += all;
+    }
+    uint32_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = __shfl_up(incl, o);
+        if (lane >= o) incl += up;
+    }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    uint32_t excl = incl - mine;
+    for (int w = 0; w < wave; ++w) excl += wsum[w];
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+        const int d = threadIdx.x * kOwn + u;
+        if (d < bins) base[d] += excl;
+        excl += total[u];
+    }
+    // Each wave takes a run of the tile, 64 pairs at a time.
+    const int64_t t0 = (int64_t)blockIdx.x * per, t1 = min((int64_t)T, t0 + per);
+    const int run = (per + kWaves - 1) / kWaves;
+    const int64_t i0 = t0 + (int64_t)wave * run, i1 = min(t1, i0 + run);
+    // Lanes of a round with the lane's digit.
+    auto same = [&](uint32_t d, bool in) {
+        uint64_t m = __ballot(in);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t s = __ballot((d >> b) & 1u);
+            m &= (d >> b) & 1u ? s : ~s;
+        }
+        return m;
+    };
+    for (int64_t i = i0; i < i1; i += 64) {
+        const bool in = i + lane < i1;
+        const uint32_t d = in ? (key_of(keys[i + lane], V) >> shift) & (bins - 1) : 0u;
+        const uint64_t m = same(d, in);
+        if (in && lane == __ffsll((long long)m) - 1) cnt[wave][d] += (uint32_t)__popcll(m);
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += kSortNT) {
+        uint32_t at = base[d];
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const uint32_t c = cnt[w][d];
+            cnt[w][d] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    for (int64_t i = i0; i < i1; i += 64) {
+        const bool in = i + lane < i1;
+        const uint32_t key = in ? key_of(keys[i + lane], V) : 0u;
+        const uint32_t p = in && pos ? pos[i + lane] : (uint32_t)(i + lane);
+        const uint32_t d = (key >> shift) & (bins - 1);
+        const uint64_t m = same(d, in);
+        uint32_t to = 0;
+        if (in) to = cnt[wave][d] + (uint32_t)__popcll(m & ((1ull << lane) - 1));
+        // (A wave's LDS accesses run in order: the next round reads what this one wrote.)
+        __builtin_amdgcn_wave_barrier();
+        if (in && lane == __ffsll((long long)m) - 1) cnt[wave][d] += (uint32_t)__popcll(m);
+        __builtin_amdgcn_wave_barrier();
+        if (in) {
+            keys_out[to] = key;
+            pos_out[to] = p;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------- sums
+// First of sorted[lo, hi) that is not below v.
+__device__ __forceinline__ int lower_bound(const uint32_t *sorted, int lo, int hi, uint32_t v) {
+    while (lo < hi) {
+        const int mid = lo + ((hi - lo) >> 1);
+        if (sorted[mid] < v) lo = mid + 1;
+        else hi = mid;
     }
     return lo;
 }
-
-__global__ __launch_bounds__(kNT) void emb_bwd_row(int dt, const uint32_t *order,
-                                                   const uint32_t *sorted, int T, int C,
-                                                   const void *dout, int ldo, float scale,
-                                                   void *dtable, int ldt, int accumulate) {
-    const uint32_t v = blockIdx.x;
-    const int k0 = lower_bound(sorted, T, v);
-    if (accumulate && (k0 >= T || sorted[k0] != v)) return;
-    for (int c = threadIdx.x; c < C; c += kNT) {
-        float s = 0.0f;
-        for (int k = k0; k < T && sorted[k] == v; ++k)
-            s += fg::load_as_f(dout, dt, (uint64_t)order[k] * ldo + c);
-        s *= scale;
-        const uint64_t at = (uint64_t)v * ldt + c;
-        fg::store_from_f(dtable, dt, at, accumulate ? fg::load_as_f(dtable, dt, at) + s : s);
+// The same by a whole wave, 64 probes at a time (all lanes; the same in each).
+__device__ __forceinline__ int wave_lower_bound(const uint32_t *sorted, int T, uint32_t v) {
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0, hi = T;  // the answer is in [lo, hi]
+    while (lo < hi) {
+        const int64_t step = (hi - lo + 63) / 64, at = lo + lane * step;
+        const uint64_t below = __ballot(at < hi && sorted[at < hi ? at : lo] < v);
+        const int n = __popcll(below);  // probes below v: the first n
+        if (n == 0) return (int)lo;
+        const int64_t last = lo + (int64_t)(n - 1) * step;  // is below
+        hi = min(hi, last + step);
+        lo = last + 1;
     }
+    return (int)lo;
+}
+
+struct Sums {
+    const uint32_t *order, *sorted;
+    int T, V, C, lddo, lddt, accumulate;
+    float scale;
+    int P;            // sorted positions of a unit
+    int units;        // units in all
+    int lshift;       // log2 of a unit's lanes
+    int unit_blocks;  // workgroups of units; those after them zero `zrows` rows each
+    int zrows;
+    int64_t Cp;       // columns of a partial sum (rounded up to chunks)
+    float *partial;   // [units][2][Cp]: the run that began before, the one that goes on
+};
+
+template <int DT>
+__global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
+                                                const typename Io<DT>::T *__restrict__ dout,
+                                                typename Io<DT>::T *dtable) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E, UNR = 8;
+    const int nb = p.C / E, chunks = (p.C - 1) / E + 1;
+    if ((int)blockIdx.x >= p.unit_blocks) {
+        // Rows of no token.
+        if (blockIdx.y > 0) return;
+        __shared__ int used[kNT];
+        __shared__ int range[2];
+        const int64_t v0 = (int64_t)(blockIdx.x - p.unit_blocks) * p.zrows;
+        const int n = (int)min((int64_t)p.zrows, p.V - v0), wave = threadIdx.x >> 6;
+        if (wave < 2) {
+            const int at = wave_lower_bound(p.sorted, p.T, (uint32_t)(v0 + (wave ? n : 0)));
+            if ((threadIdx.x & 63) == 0) range[wave] = at;
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < n) {
+            const uint32_t v = (uint32_t)(v0 + threadIdx.x);
+            const int k = lower_bound(p.sorted, range[0], range[1], v);
+            used[threadIdx.x] = k < range[1] && p.sorted[k] == v;
+        }
+        __syncthreads();
+        const float z[E] = {};
+        for (int r = 0; r < n; ++r) {
+            if (used[r]) continue;
+            auto *to = dtable + (size_t)(v0 + r) * p.lddt;
+            for (int j = threadIdx.x; j < chunks; j += kNT) Chunk<DT>::store(to, j, nb, p.C, z);
+        }
+        return;
+    }
+    const int lanes = 1 << p.lshift;
+    const int unit = (int)(blockIdx.x << (8 - p.lshift)) + (int)(threadIdx.x >> p.lshift);
+    const int j = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
+    if (unit >= p.units || j >= chunks) return;
+    const int k0 = unit * p.P, k1 = min(p.T, k0 + p.P);
+    // A run that began before the unit, or goes on after it, is a partial sum.
+    const uint32_t V = (uint32_t)p.V;
+    bool head = k0 > 0 && p.sorted[k0 - 1] == p.sorted[k0];
+    float a[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) a[e] = 0.0f;
+    for (int k = k0; k < k1; k += UNR) {
+        uint32_t tok[UNR + 1];
+        u32x4 w[UNR];
+#pragma unroll
+        for (int u = 0; u < UNR; ++u) {
+            const int at = min(k + u, k1 - 1);
+            tok[u] = p.sorted[at];
+            w[u] = Chunk<DT>::load(dout + (size_t)p.order[at] * p.lddo, j, nb, p.C);
+        }
+        tok[UNR] = p.sorted[min(k + UNR, p.T - 1)];
+#pragma unroll
+        for (int u = 0; u < UNR; ++u) {
+            if (k + u >= k1) break;
+#pragma unroll
+            for (int e = 0; e < E; ++e) a[e] += IO::get(w[u], e);
+            const bool last = k + u + 1 == p.T;
+            const uint32_t next =
+                k + u + 1 < k1 || last ? tok[u + 1] : p.sorted[k1];  // (k1 < T there)
+            if (!last && next == tok[u] && k + u + 1 < k1) continue;
+            const bool on = !last && next == tok[u];  // goes on in the next unit
+            if (tok[u] < V) {
+                if (head || on) {
+                    float *to = p.partial + ((size_t)unit * 2 + (head ? 0 : 1)) * p.Cp +
+                                (size_t)j * E;
+#pragma unroll
+                    for (int q = 0; q < E / 4; ++q)
+                        *reinterpret_cast<f32x4 *>(to + 4 * q) =
+                            f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+                } else {
+                    auto *to = dtable + (size_t)tok[u] * p.lddt;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) a[e] *= p.scale;
+                    if (p.accumulate) {
+                        const u32x4 was = Chunk<DT>::load(to, j, nb, p.C);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) a[e] += IO::get(was, e);
+                    }
+                    Chunk<DT>::store(to, j, nb, p.C, a);
+                }
+            }
+            head = false;
+#pragma unroll
+            for (int e = 0; e < E; ++e) a[e] = 0.0f;
+        }
+    }
+}
+
+// Joins the partial sums of the run that begins in unit blockIdx.x and goes on after
+// it (if one does), 4 columns a lane, a share of the units a wave.
+constexpr int kJoinCols = 256;
+template <int DT>
+__global__ __launch_bounds__(kNT) void emb_join(const Sums p, typename Io<DT>::T *dtable) {
+    using IO = Io<DT>;
+    constexpr int kWaves = kNT / 64;
+    __shared__ f32x4 sh[kWaves][64];
+    const int u0 = blockIdx.x, k1 = (u0 + 1) * p.P, k0 = u0 * p.P;  // (the last unit joins nothing)
+    const uint32_t v = p.sorted[k1 - 1];
+    if (v >= (uint32_t)p.V || p.sorted[k1] != v) return;
+    if (p.sorted[k0] == v && k0 > 0 && p.sorted[k0 - 1] == v) return;  // began earlier
+    const int end = wave_lower_bound(p.sorted, p.T, v + 1);  // (v + 1 <= V: no overflow)
+    const int u1 = (end - 1) / p.P;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.y * kJoinCols + lane * 4;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    const int n = u1 - u0 + 1, per = (n + kWaves - 1) / kWaves;
+    const int b0 = wave * per, b1 = min(n, b0 + per);
+    if (col < p.Cp) {
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b)
+            a += *reinterpret_cast<const f32x4 *>(
+                p.partial + ((size_t)(u0 + b) * 2 + (b == 0 ? 1 : 0)) * p.Cp + col);
+    }
+    sh[wave][lane] = a;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) a += sh[w][lane];
+    auto *to = dtable + (size_t)v * p.lddt;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (col + e >= p.C) continue;
+        float o = a[e] * p.scale;
+        if (p.accumulate) o += IO::load1(to, (int)col + e);
+        IO::store1(to, (int)col + e, o);
+    }
+}
+
+int log2_up(int64_t n) {
+    int s = 0;
+    while ((int64_t(1) << s) < n) ++s;
+    return s;
+}
+// Lanes that take a row of `chunks` chunks: a power of two, at most a workgroup.
+int lane_shift(int chunks) { return std::min(8, log2_up(chunks)); }
+
+// How a gradient of T tokens over rows of C columns is laid out.
+struct Plan {
+    int P, units, lshift;
+    int64_t Cp;
+    int passes, bits, tiles, per;  // of the radix sort (passes 0: by counting)
+    uint64_t sort_words, hist_words, partial_floats;
+    uint64_t bytes() const {
+        return 4 * (sort_words + hist_words) + 16 + 4 * partial_floats;
+    }
+};
+Plan plan_of(int dtype, int T, int V, int C) {
+    Plan p{};
+    if (T <= kDirectMax) return p;
+    const int E = dtype == FG_DTYPE_F32 ? 4 : 8, chunks = (C - 1) / E + 1;
+    p.lshift = lane_shift(chunks);
+    p.Cp = (int64_t)chunks * E;
+    // About 2048 workgroups of units of 8 to 128 positions.
+    const int64_t tiles = (chunks - 1) / (1 << p.lshift) + 1;
+    const int64_t lanes = ((int64_t)T << p.lshift) * tiles;  // with one position a unit
+    p.P = 8;
+    while (p.P < 128 && lanes / p.P > 2048 * kNT) p.P *= 2;
+    p.units = (T - 1) / p.P + 1;
+    p.partial_floats = (uint64_t)p.units * 2 * (uint64_t)p.Cp;
+    p.sort_words = 2 * (uint64_t)T;
+    if (T > kRankMax) {
+        const int need = std::max(1, log2_up((int64_t)V + 1));  // of keys 0 .. V
+        p.passes = (need - 1) / kMaxBits + 1;
+        p.bits = (need - 1) / p.passes + 1;
+        p.tiles = std::min(kTiles, (T - 1) / kSortNT + 1);
+        p.per = (T - 1) / p.tiles + 1;
+        p.sort_words *= 2;
+        p.hist_words = ((uint64_t)p.tiles << p.bits);
+    }
+    return p;
+}
+
+template <int DT>
+int launch_fwd(fg_ctx *ctx, const uint32_t *tokens, int T, int V, int C, const void *table, int ldt,
+               float scale, void *out, int ldo) {
+    using Ty = typename Io<DT>::T;
+    const int lshift = lane_shift((C - 1) / Io<DT>::E + 1), rows = kNT >> lshift;
+    emb_fwd<DT><<<(T - 1) / rows + 1, kNT, 0, ctx->stream>>>(
+        tokens, T, V, C, static_cast<const Ty *>(table), ldt, scale, static_cast<Ty *>(out), ldo,
+        lshift);
+    FG_LAUNCH_CHECK("emb_fwd");
+    return FG_OK;
+}
+
+template <int DT>
+int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, int T, int V, int C,
+               const void *dout, int lddo, float scale, void *dtable, int lddt, int accumulate) {
+    using Ty = typename Io<DT>::T;
+    const Ty *d = static_cast<const Ty *>(dout);
+    Ty *g = static_cast<Ty *>(dtable);
+    hipStream_t st = ctx->stream;
+    const int chunks = (C - 1) / Io<DT>::E + 1;
+    if (T <= kDirectMax) {
+        const int lshift = lane_shift(chunks), at_once = kNT >> lshift;
+        // Table rows of a workgroup: those it takes at once, more where the table is long.
+        const int rows = (int)std::max<int64_t>(at_once, (V - 1) / (16 * ctx->cu_count) + 1);
+        emb_bwd_few<DT><<<(V - 1) / rows + 1, kNT, 0, st>>>(tokens, T, V, C, d, lddo, scale, g, lddt,
+                                                           accumulate, rows, lshift);
+        FG_LAUNCH_CHECK("emb_bwd_few");
+        return FG_OK;
+    }
+    uint32_t *order = (uint32_t *)ws, *sorted = order + T;
+    if (pl.passes == 0) {
+        emb_rank<<<(T - 1) / 64 + 1, 1024, 0, st>>>(tokens, T, order, sorted);
+        FG_LAUNCH_CHECK("emb_rank");
+    } else {
+        // The passes go back and forth between two pairs of arrays and end in the first.
+        uint32_t *pos[2] = {order, order + 2 * (size_t)T};
+        uint32_t *key[2] = {sorted, sorted + 2 * (size_t)T};
+        uint32_t *hist = order + 4 * (size_t)T;
+        const uint32_t *kin = tokens, *pin = nullptr;
+        for (int n = 0; n < pl.passes; ++n) {
+            const int to = (pl.passes - 1 - n) & 1;
+            radix_count<<<pl.tiles, kSortNT, 0, st>>>(kin, T, (uint32_t)V, pl.per, n * pl.bits,
+                                                      pl.bits, hist);
+            FG_LAUNCH_CHECK("radix_count");
+            radix_place<<<pl.tiles, kSortNT, 0, st>>>(kin, pin, T, (uint32_t)V, pl.per,
+                                                      n * pl.bits, pl.bits, hist, key[to],
+                                                      pos[to]);
+            FG_LAUNCH_CHECK("radix_place");
+            kin = key[to];
+            pin = pos[to];
+        }
+    }
+    Sums s{};
+    s.order = order;
+    s.sorted = sorted;
+    s.T = T;
+    s.V = V;
+    s.C = C;
+    s.lddo = lddo;
+    s.lddt = lddt;
+    s.accumulate = accumulate;
+    s.scale = scale;
+    s.P = pl.P;
+    s.units = pl.units;
+    s.lshift = pl.lshift;
+    s.Cp = pl.Cp;
+    s.partial = (float *)ws + ((pl.sort_words + pl.hist_words + 3) & ~uint64_t(3));
+    s.unit_blocks = ((pl.units - 1) >> (8 - pl.lshift)) + 1;
+    int blocks = s.unit_blocks;
+    s.zrows = 1;
+    if (!accumulate) {
+        // Rows a workgroup zeroes: about 2048 workgroups, at most one row a thread.
+        while (s.zrows < kNT && V / s.zrows > 2048) s.zrows *= 2;
+        blocks += (V - 1) / s.zrows + 1;
+    }
+    const int tiles = (chunks - 1) / (1 << pl.lshift) + 1;
+    emb_sums<DT><<<dim3(blocks, tiles), kNT, 0, st>>>(s, d, g);
+    FG_LAUNCH_CHECK("emb_sums");
+    if (pl.units > 1) {
+        emb_join<DT><<<dim3(pl.units - 1, (unsigned)((pl.Cp - 1) / kJoinCols + 1)), kNT, 0, st>>>(s,
+                                                                                                g);
+        FG_LAUNCH_CHECK("emb_join");
+    }
+    return FG_OK;
 }
 
 }  // namespace
 
 namespace fg {
-uint64_t embedding_bwd_ws_bytes(int T, int V, int C) {
-    (void)V;
-    (void)C;
-    return std::max<uint64_t>(1, (uint64_t)T) * 8;
+uint64_t embedding_bwd_ws_bytes(int dtype, int T, int V, int C) {
+    return plan_of(dtype, T, V, C).bytes();
 }
 }  // namespace fg
 
@@ -103,9 +651,10 @@ FG_API int fg_embedding(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T,
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     if (T == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
-    emb_fwd<<<T, kNT, 0, ctx->stream>>>(dtype, d_tokens, V, C, d_table, ldt, scale, d_out, ldo);
-    FG_LAUNCH_CHECK("emb_fwd");
-    return FG_OK;
+    auto launch = dtype == FG_DTYPE_F32    ? launch_fwd<fg::kF32>
+                  : dtype == FG_DTYPE_BF16 ? launch_fwd<fg::kBF16>
+                                           : launch_fwd<fg::kF16>;
+    return launch(ctx, d_tokens, T, V, C, d_table, ldt, scale, d_out, ldo);
 }
 
 FG_API int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T, int V, int C,
@@ -122,15 +671,11 @@ FG_API int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, in
                "%s: tokens, dout and dtable are required", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     FG_HIP(hipSetDevice(ctx->device));
-    uint32_t *order = (uint32_t *)fg::workspace(ctx, fg::embedding_bwd_ws_bytes(T, V, C));
-    if (!order) return FG_ERR_OUT_OF_MEMORY;
-    uint32_t *sorted = order + T;
-    if (T > 0) {
-        emb_rank<<<(T + kNT - 1) / kNT, kNT, 0, ctx->stream>>>(d_tokens, T, order, sorted);
-        FG_LAUNCH_CHECK("emb_rank");
-    }
-    emb_bwd_row<<<V, kNT, 0, ctx->stream>>>(dtype, order, sorted, T, C, d_dout, lddo, scale,
-                                            d_dtable, lddt, accumulate);
-    FG_LAUNCH_CHECK("emb_bwd_row");
-    return FG_OK;
+    const Plan pl = plan_of(dtype, T, V, C);
+    void *ws = nullptr;
+    if (T > kDirectMax && !(ws = fg::workspace(ctx, pl.bytes()))) return FG_ERR_OUT_OF_MEMORY;
+    auto launch = dtype == FG_DTYPE_F32    ? launch_bwd<fg::kF32>
+                  : dtype == FG_DTYPE_BF16 ? launch_bwd<fg::kBF16>
+                                           : launch_bwd<fg::kF16>;
+    return launch(ctx, pl, ws, d_tokens, T, V, C, d_dout, lddo, scale, d_dtable, lddt, accumulate);
 }

@@ -23,57 +23,82 @@ namespace {
 
 using fg::rows::Io;
 using fg::rows::u32x4;
-using fg::rows::wave_sum;
 
-// The sum over a row's NW waves of v (its own waves' sums in turn), the same in
-// every lane.  One barrier; sm: NW floats that nothing of the last two sums uses.
-template <int NW>
-__device__ __forceinline__ float row_sum(float v, float *sm, int wave) {
-    v = wave_sum(v);
-    if constexpr (NW > 1) {
-        if ((threadIdx.x & 63) == 0) sm[wave] = v;
+// How a row lies on its L lanes (fg_rows.h): lane t holds whole chunks t, t + L, ...
+// below nb, and column `single` where it is below C.
+template <int DT>
+struct Lanes {
+    int nb, single;
+    __device__ __forceinline__ Lanes(int C, int t) {
+        constexpr int E = Io<DT>::E;
+        nb = C / E;
+        single = t < C - nb * E ? nb * E + t : C;
+    }
+};
+
+// The sum over a row's L lanes, the same in every lane: 16 lanes of a wave, or its
+// L / 64 waves' sums in turn.  Waves wait at one barrier; sm: a float per wave of
+// the row, which nothing of the sum before the last uses.
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float *sm, int t) {
+    if constexpr (L == 16) return fg::smrow::row16_sum(v);
+    v = fg::rows::wave_sum(v);
+    if constexpr (L > 64) {
+        if ((t & 63) == 0) sm[t >> 6] = v;
         __syncthreads();
         v = sm[0];
 #pragma unroll
-        for (int k = 1; k < NW; ++k) v += sm[k];
+        for (int k = 1; k < L / 64; ++k) v += sm[k];
     }
     return v;
 }
 
 // ------------------------------------------------------------------ forward
-// A row is held in registers by NW waves, NV chunks a lane, NG rows at once in a
+// A row is held in registers by L lanes, NV chunks a lane, NG rows at once in a
 // workgroup; the workgroup walks the rows with gamma and beta held, and the next
-// rows' loads go out before this one's sums.
-template <int DT, int NV, int NW, int NG>
-__global__ __launch_bounds__(64 * NW * NG) void ln_fwd(
+// rows' loads go out before this one's sums.  The variance is summed from x - mean
+// (a difference of squares would lose a row far from zero), and sums are divided by
+// C, so that the mean of a constant row is exact.
+template <int DT, int NV, int L, int NG>
+__global__ __launch_bounds__(L *NG) void ln_fwd(
     const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *gamma,
     const typename Io<DT>::T *beta, float eps, int R, int C, typename Io<DT>::T *y, int ldy,
     float *mean, float *rstd) {
     using IO = Io<DT>;
-    constexpr int E = IO::E, NT = 64 * NW;
-    __shared__ float sm[2][2][NG][NW];
-    const int grp = threadIdx.x / NT, t = threadIdx.x % NT, wave = t >> 6;
+    constexpr int E = IO::E, NS = (L + 63) / 64;
+    __shared__ float sm[2][2][NG][NS];
+    const int grp = threadIdx.x / L, t = threadIdx.x % L;
+    const Lanes<DT> ln(C, t);
+    const bool one = ln.single < C;
+    const float n = (float)C;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
     u32x4 g[NV], b[NV], w[NV];
+    float g1 = 1.0f, b1 = 0.0f, w1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int col = (t + i * NT) * E;
-        if (gamma) g[i] = fg::rows::load<DT>(gamma, col, C - col);
-        if (beta) b[i] = fg::rows::load<DT>(beta, col, C - col);
+        const int j = t + i * L;
+        g[i] = gamma && j < ln.nb ? fg::rows::load<DT>(gamma, j) : zero;
+        b[i] = beta && j < ln.nb ? fg::rows::load<DT>(beta, j) : zero;
     }
-    const float n = (float)C;  // (sums are divided: a constant row's mean is then exact)
+    if (gamma && one) g1 = IO::load1(gamma, ln.single);
+    if (beta && one) b1 = IO::load1(beta, ln.single);
     uint32_t r = blockIdx.x * NG + grp;  // (unsigned: past R by less than a step)
     const uint32_t rows = R, step = gridDim.x * NG;
     auto fetch = [&](uint32_t row) {
+        const auto *xr = x + (size_t)row * ldx;
+        const bool in = row < rows;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (t + i * NT) * E;
-            w[i] = fg::rows::load<DT>(x + (size_t)row * ldx, col, row < rows ? C - col : 0);
+            const int j = t + i * L;
+            w[i] = in && j < ln.nb ? fg::rows::load<DT>(xr, j) : zero;
         }
+        w1 = in && one ? IO::load1(xr, ln.single) : 0.0f;
     };
     fetch(r);
     for (uint32_t r0 = blockIdx.x * NG, it = 0; r0 < rows; r0 += step, ++it) {
         u32x4 v[NV];
-        float s = 0.0f;
+        const float v1 = w1;
+        float s = v1;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             v[i] = w[i];
@@ -83,22 +108,25 @@ __global__ __launch_bounds__(64 * NW * NG) void ln_fwd(
         const uint32_t row = r;
         r += step;
         if (r0 + step < rows) fetch(r);
-        const float mu = row_sum<NW>(s, sm[it & 1][0][grp], wave) / n;
-        float q = 0.0f;
+        const float mu = row_sum<L>(s, sm[it & 1][0][grp], t) / n;
+        float q = one ? (v1 - mu) * (v1 - mu) : 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int left = C - (t + i * NT) * E;
+            float p = 0.0f;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float d = IO::get(v[i], e) - mu;
-                q += e < left ? d * d : 0.0f;
+                p += d * d;
             }
+            q += t + i * L < ln.nb ? p : 0.0f;
         }
-        const float rs = 1.0f / sqrtf(row_sum<NW>(q, sm[it & 1][1][grp], wave) / n + eps);
+        const float rs = 1.0f / sqrtf(row_sum<L>(q, sm[it & 1][1][grp], t) / n + eps);
         if (row < rows) {
+            auto *yr = y + (size_t)row * ldy;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int col = (t + i * NT) * E;
+                const int j = t + i * L;
+                if (j >= ln.nb) continue;
                 float o[E];
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
@@ -106,8 +134,9 @@ __global__ __launch_bounds__(64 * NW * NG) void ln_fwd(
                     if (gamma) o[e] *= IO::get(g[i], e);
                     if (beta) o[e] += IO::get(b[i], e);
                 }
-                fg::rows::store<DT>(y + (size_t)row * ldy, col, C - col, IO::pack(o));
+                fg::rows::store<DT>(yr, j, IO::pack(o));
             }
+            if (one) IO::store1(yr, ln.single, (v1 - mu) * rs * g1 + b1);
             if (t == 0) {
                 if (mean) mean[row] = mu;
                 if (rstd) rstd[row] = rs;
@@ -116,250 +145,604 @@ __global__ __launch_bounds__(64 * NW * NG) void ln_fwd(
     }
 }
 
+// A row per workgroup and nothing else held (gamma and beta come from the caches
+// where the output needs them), so that two or more rows share a CU and their loads
+// overlap one another's sums.
+template <int DT, int NV, int L>
+__global__ __launch_bounds__(L) __attribute__((amdgpu_waves_per_eu(8))) void ln_fwd_wide(
+    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *__restrict__ gamma,
+    const typename Io<DT>::T *__restrict__ beta, float eps, int C, typename Io<DT>::T *y, int ldy,
+    float *mean, float *rstd) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E;
+    __shared__ float sm[2][L / 64];
+    const auto *xr = x + (size_t)blockIdx.x * ldx;
+    auto *yr = y + (size_t)blockIdx.x * ldy;
+    const int t = threadIdx.x;
+    const Lanes<DT> ln(C, t);
+    const bool one = ln.single < C;
+    const float n = (float)C;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    u32x4 w[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = t + i * L < ln.nb ? fg::rows::load<DT>(xr, t + i * L) : zero;
+    float v1 = one ? IO::load1(xr, ln.single) : 0.0f;
+    float s = v1;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float p = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) p += IO::get(w[i], e);
+        s += p;
+    }
+    const float mu = row_sum<L>(s, sm[0], t) / n;
+    fg::smany::repack(w);
+    float q = one ? (v1 - mu) * (v1 - mu) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float p = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float d = IO::get(w[i], e) - mu;
+            p += d * d;
+        }
+        q += t + i * L < ln.nb ? p : 0.0f;
+    }
+    const float rs = 1.0f / sqrtf(row_sum<L>(q, sm[1], t) / n + eps);
+    fg::smany::repack(w);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = t + i * L;
+        if (j >= ln.nb) continue;
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = (IO::get(w[i], e) - mu) * rs;
+        if (gamma) {
+            const u32x4 g = fg::rows::load<DT>(gamma, j);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= IO::get(g, e);
+        }
+        if (beta) {
+            const u32x4 b = fg::rows::load<DT>(beta, j);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += IO::get(b, e);
+        }
+        fg::rows::store<DT>(yr, j, IO::pack(o));
+    }
+    if (one) {
+        v1 = (v1 - mu) * rs;
+        if (gamma) v1 *= IO::load1(gamma, ln.single);
+        if (beta) v1 += IO::load1(beta, ln.single);
+        IO::store1(yr, ln.single, v1);
+    }
+    if (t == 0) {
+        if (mean) mean[blockIdx.x] = mu;
+        if (rstd) rstd[blockIdx.x] = rs;
+    }
+}
+
 // Rows longer than registers hold: three passes over the row, the second and third
 // from the caches where they hold it.
-constexpr int kLongNW = 16;
+constexpr int kLongL = 1024;
 template <int DT>
-__global__ __launch_bounds__(64 * kLongNW) void ln_fwd_long(
+__global__ __launch_bounds__(kLongL) void ln_fwd_long(
     const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *gamma,
     const typename Io<DT>::T *beta, float eps, int C, typename Io<DT>::T *y, int ldy, float *mean,
     float *rstd) {
     using IO = Io<DT>;
-    constexpr int E = IO::E, NT = 64 * kLongNW;
-    __shared__ float sm[2][kLongNW];
+    constexpr int E = IO::E;
+    __shared__ float sm[2][kLongL / 64];
     const auto *xr = x + (size_t)blockIdx.x * ldx;
     auto *yr = y + (size_t)blockIdx.x * ldy;
-    const int wave = threadIdx.x >> 6;
-    const float n = (float)C;  // (sums are divided: a constant row's mean is then exact)
-    float s = 0.0f;
-    for (int64_t col = threadIdx.x * E; col < C; col += NT * E) {
-        const u32x4 w = fg::rows::load<DT>(xr, (int)col, C - (int)col);
+    const int t = threadIdx.x;
+    const Lanes<DT> ln(C, t);
+    const bool one = ln.single < C;
+    const float n = (float)C;
+    float v1 = one ? IO::load1(xr, ln.single) : 0.0f;
+    float s = v1;
+#pragma unroll 4
+    for (int j = t; j < ln.nb; j += kLongL) {
+        const u32x4 w = fg::rows::load<DT>(xr, j);
         float p = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) p += IO::get(w, e);
         s += p;
     }
-    const float mu = row_sum<kLongNW>(s, sm[0], wave) / n;
-    float q = 0.0f;
-    for (int64_t col = threadIdx.x * E; col < C; col += NT * E) {
-        const int left = C - (int)col;
-        const u32x4 w = fg::rows::load<DT>(xr, (int)col, left);
+    const float mu = row_sum<kLongL>(s, sm[0], t) / n;
+    float q = one ? (v1 - mu) * (v1 - mu) : 0.0f;
+#pragma unroll 4
+    for (int j = t; j < ln.nb; j += kLongL) {
+        const u32x4 w = fg::rows::load<DT>(xr, j);
         float p = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const float d = IO::get(w, e) - mu;
-            p += e < left ? d * d : 0.0f;
+            p += d * d;
         }
         q += p;
     }
-    const float rs = 1.0f / sqrtf(row_sum<kLongNW>(q, sm[1], wave) / n + eps);
-    for (int64_t c64 = threadIdx.x * E; c64 < C; c64 += NT * E) {
-        const int col = (int)c64, left = C - col;
-        const u32x4 w = fg::rows::load<DT>(xr, col, left);
-        u32x4 g, b;
-        if (gamma) g = fg::rows::load<DT>(gamma, col, left);
-        if (beta) b = fg::rows::load<DT>(beta, col, left);
+    const float rs = 1.0f / sqrtf(row_sum<kLongL>(q, sm[1], t) / n + eps);
+#pragma unroll 2
+    for (int j = t; j < ln.nb; j += kLongL) {
+        const u32x4 w = fg::rows::load<DT>(xr, j);
         float o[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            o[e] = (IO::get(w, e) - mu) * rs;
-            if (gamma) o[e] *= IO::get(g, e);
-            if (beta) o[e] += IO::get(b, e);
+        for (int e = 0; e < E; ++e) o[e] = (IO::get(w, e) - mu) * rs;
+        if (gamma) {
+            const u32x4 g = fg::rows::load<DT>(gamma, j);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] *= IO::get(g, e);
         }
-        fg::rows::store<DT>(yr, col, left, IO::pack(o));
+        if (beta) {
+            const u32x4 b = fg::rows::load<DT>(beta, j);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += IO::get(b, e);
+        }
+        fg::rows::store<DT>(yr, j, IO::pack(o));
     }
-    if (threadIdx.x == 0) {
+    if (one) {
+        v1 = (v1 - mu) * rs;
+        if (gamma) v1 *= IO::load1(gamma, ln.single);
+        if (beta) v1 += IO::load1(beta, ln.single);
+        IO::store1(yr, ln.single, v1);
+    }
+    if (t == 0) {
         if (mean) mean[blockIdx.x] = mu;
         if (rstd) rstd[blockIdx.x] = rs;
     }
 }
 
 // ----------------------------------------------------------------- backward
-// The row in registers as above (one sum phase a row: mean and rstd are given),
-// with the weights' gradients of a lane's columns summed in its registers over the
+// With c = x - mean and gd = dy * gamma, a row needs the sums of gd and gd * c:
+//   dx = rstd * (gd - sum(gd) / C - c * rstd * (rstd * sum(gd * c) / C))
+// The row in registers as above (one sum phase: mean and rstd are given), with the
+// weights' gradients of a lane's columns summed in its registers over the
 // workgroup's rows, over its NG rows at once in LDS, and written once per workgroup
-// as partial[workgroup][2][C].
-template <int DT, int NV, int NW, int NG, bool WEIGHTS>
-__global__ __launch_bounds__(64 * NW * NG) void ln_bwd(
+// as partial[workgroup][2][Cp] (Cp: C rounded up to 4).
+__host__ __device__ constexpr int64_t padded(int64_t C) { return (C + 3) & ~int64_t(3); }
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <int DT, int NV, int L, int NG, bool WEIGHTS>
+__global__ __launch_bounds__(L *NG) void ln_bwd(
     const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
     const typename Io<DT>::T *gamma, const float *mean, const float *rstd, int R, int C,
     typename Io<DT>::T *dx, int lddx, int accumulate, float *partial) {
     using IO = Io<DT>;
-    constexpr int E = IO::E, NT = 64 * NW;
-    __shared__ float sm[2][2][NG][NW];
-    extern __shared__ float cols[];  // [2][C]
-    const int grp = threadIdx.x / NT, t = threadIdx.x % NT, wave = t >> 6;
-    u32x4 g[NV], wx[NV], wd[NV];
-    float ag[WEIGHTS ? NV : 1][E], ab[WEIGHTS ? NV : 1][E];
+    constexpr int E = IO::E, NS = (L + 63) / 64;
+    __shared__ float sm[2][2][NG][NS];
+    extern __shared__ f32x4 cols[];  // [2][Cp]
+    const int grp = threadIdx.x / L, t = threadIdx.x % L;
+    const Lanes<DT> ln(C, t);
+    const bool one = ln.single < C;
+    const float n = (float)C;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    u32x4 wx[NV], wd[NV];
+    float g[NV][E], ag[NV][E], ab[NV][E];
+    float g1 = 1.0f, ag1 = 0.0f, ab1 = 0.0f, wx1 = 0.0f, wd1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int col = (t + i * NT) * E;
-        if (gamma) g[i] = fg::rows::load<DT>(gamma, col, C - col);
-        if constexpr (WEIGHTS) {
+        const int j = t + i * L;
+        const u32x4 v = gamma && j < ln.nb ? fg::rows::load<DT>(gamma, j) : zero;
 #pragma unroll
-            for (int e = 0; e < E; ++e) ag[i][e] = ab[i][e] = 0.0f;
+        for (int e = 0; e < E; ++e) {
+            g[i][e] = gamma ? IO::get(v, e) : 1.0f;
+            ag[i][e] = ab[i][e] = 0.0f;
         }
     }
-    const float n = (float)C;  // (sums are divided: a constant row's mean is then exact)
+    if (gamma && one) g1 = IO::load1(gamma, ln.single);
     uint32_t r = blockIdx.x * NG + grp;  // (unsigned: past R by less than a step)
     const uint32_t rows = R, step = gridDim.x * NG;
     float mu = 0.0f, rs = 0.0f;
     auto fetch = [&](uint32_t row) {
         const bool in = row < rows;
+        const auto *xr = x + (size_t)row * ldx, *dr = dy + (size_t)row * lddy;
         mu = in ? mean[row] : 0.0f;
         rs = in ? rstd[row] : 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int col = (t + i * NT) * E;
-            wx[i] = fg::rows::load<DT>(x + (size_t)row * ldx, col, in ? C - col : 0);
-            wd[i] = fg::rows::load<DT>(dy + (size_t)row * lddy, col, in ? C - col : 0);
+            const int j = t + i * L;
+            const bool mine = in && j < ln.nb;
+            wx[i] = mine ? fg::rows::load<DT>(xr, j) : zero;
+            wd[i] = mine ? fg::rows::load<DT>(dr, j) : zero;
         }
+        wx1 = in && one ? IO::load1(xr, ln.single) : 0.0f;
+        wd1 = in && one ? IO::load1(dr, ln.single) : 0.0f;
     };
     fetch(r);
     for (uint32_t r0 = blockIdx.x * NG, it = 0; r0 < rows; r0 += step, ++it) {
-        u32x4 vx[NV], vd[NV];
+        float c[NV][E], gd[NV][E];
         const float m = mu, k = rs;
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            vx[i] = wx[i];
-            vd[i] = wd[i];
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float d = IO::get(vd[i], e), xh = (IO::get(vx[i], e) - m) * k;
-                const float gd = gamma ? d * IO::get(g[i], e) : d;
-                s1 += gd;
-                s2 += gd * xh;
+                const float d = IO::get(wd[i], e);
+                c[i][e] = IO::get(wx[i], e) - m;
+                gd[i][e] = d * g[i][e];
+                s1 += gd[i][e];
+                s2 += gd[i][e] * c[i][e];
                 if constexpr (WEIGHTS) {
-                    ag[i][e] += d * xh;
+                    ag[i][e] += d * k * c[i][e];
                     ab[i][e] += d;
                 }
             }
+        const float c1 = wx1 - m, gd1 = wd1 * g1;
+        s1 += gd1;
+        s2 += gd1 * c1;
+        if constexpr (WEIGHTS) {
+            ag1 += wd1 * k * c1;
+            ab1 += wd1;
         }
         const uint32_t row = r;
         r += step;
         if (r0 + step < rows) fetch(r);
-        if (dx) {
-            s1 = wave_sum(s1);
-            s2 = wave_sum(s2);
-            if constexpr (NW > 1) {
-                float(*p)[NW] = sm[it & 1][0] + grp, (*q)[NW] = sm[it & 1][1] + grp;
-                if ((threadIdx.x & 63) == 0) {
-                    (*p)[wave] = s1;
-                    (*q)[wave] = s2;
-                }
-                __syncthreads();
-                s1 = (*p)[0];
-                s2 = (*q)[0];
-#pragma unroll
-                for (int h = 1; h < NW; ++h) {
-                    s1 += (*p)[h];
-                    s2 += (*q)[h];
-                }
+        if (!dx) continue;
+        if constexpr (L == 16) {
+            s1 = fg::smrow::row16_sum(s1);
+            s2 = fg::smrow::row16_sum(s2);
+        } else {
+            s1 = fg::rows::wave_sum(s1);
+            s2 = fg::rows::wave_sum(s2);
+        }
+        if constexpr (L > 64) {
+            float *p = sm[it & 1][0][grp], *q = sm[it & 1][1][grp];
+            if ((t & 63) == 0) {
+                p[t >> 6] = s1;
+                q[t >> 6] = s2;
             }
-            const float m1 = s1 / n, m2 = s2 / n;
-            if (row < rows) {
-                auto *out = dx + (size_t)row * lddx;
+            __syncthreads();
+            s1 = p[0];
+            s2 = q[0];
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int col = (t + i * NT) * E;
-                    float o[E];
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const float d = IO::get(vd[i], e), xh = (IO::get(vx[i], e) - m) * k;
-                        o[e] = k * ((gamma ? d * IO::get(g[i], e) : d) - m1 - xh * m2);
-                    }
-                    if (accumulate) {
-                        const u32x4 was = fg::rows::load<DT>(out, col, C - col);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) o[e] += IO::get(was, e);
-                    }
-                    fg::rows::store<DT>(out, col, C - col, IO::pack(o));
-                }
+            for (int h = 1; h < NS; ++h) {
+                s1 += p[h];
+                s2 += q[h];
             }
+        }
+        const float m1 = s1 / n, m2 = k * (k * s2 / n);
+        if (row >= rows) continue;  // (the last rows of a group; no barrier follows but the next row's)
+        auto *out = dx + (size_t)row * lddx;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = t + i * L;
+            if (j >= ln.nb) continue;
+            float o[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = k * (gd[i][e] - m1 - c[i][e] * m2);
+            if (accumulate) {
+                const u32x4 was = fg::rows::load<DT>(out, j);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] += IO::get(was, e);
+            }
+            fg::rows::store<DT>(out, j, IO::pack(o));
+        }
+        if (one) {
+            float o = k * (gd1 - m1 - c1 * m2);
+            if (accumulate) o += IO::load1(out, ln.single);
+            IO::store1(out, ln.single, o);
         }
     }
     if constexpr (WEIGHTS) {
-        for (int h = 0; h < NG; ++h) {  // the row groups in turn
-            if (grp == h) {
+        const int64_t Cp = padded(C);
+        if constexpr (L == 16) {  // the wave's four rows
+            auto over4 = [](float v) {
+                v += __shfl_xor(v, 16);
+                return v + __shfl_xor(v, 32);
+            };
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const int col = (t + i * NT) * E + e;
-                        if (col >= C) continue;
-                        float a = ag[i][e], c = ab[i][e];
-                        if (h > 0) {
-                            a += cols[col];
-                            c += cols[C + col];
-                        }
-                        if (h + 1 < NG) {
-                            cols[col] = a;
-                            cols[C + col] = c;
-                        } else {
-                            partial[(size_t)blockIdx.x * 2 * C + col] = a;
-                            partial[(size_t)blockIdx.x * 2 * C + C + col] = c;
+                for (int e = 0; e < E; ++e) {
+                    ag[i][e] = over4(ag[i][e]);
+                    ab[i][e] = over4(ab[i][e]);
+                }
+            ag1 = over4(ag1);
+            ab1 = over4(ab1);
+        }
+        // Then the workgroup's row groups (waves of rows) in turn.
+        constexpr int kTurns = L == 16 ? NG / 4 : NG;
+        const int turn = L == 16 ? threadIdx.x >> 6 : grp;
+        float *lds = reinterpret_cast<float *>(cols);
+        float *part = partial + (size_t)blockIdx.x * 2 * Cp;
+        for (int h = 0; h < kTurns; ++h) {
+            if (turn == h && (L != 16 || (threadIdx.x & 63) < 16)) {
+                const bool last = h + 1 == kTurns;
+                auto pass = [&](float (&a)[NV][E], float a1, int64_t at) {
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        const int j = t + i * L;
+                        if (j >= ln.nb) continue;
+#pragma unroll
+                        for (int q = 0; q < E / 4; ++q) {
+                            const int64_t to = at + (int64_t)j * E + 4 * q;
+                            f32x4 v = {a[i][4 * q], a[i][4 * q + 1], a[i][4 * q + 2],
+                                       a[i][4 * q + 3]};
+                            if (h > 0) v += *reinterpret_cast<f32x4 *>(lds + to);
+                            *reinterpret_cast<f32x4 *>((last ? part : lds) + to) = v;
                         }
                     }
+                    if (one) {
+                        if (h > 0) a1 += lds[at + ln.single];
+                        (last ? part : lds)[at + ln.single] = a1;
+                    }
+                };
+                pass(ag, ag1, 0);
+                pass(ab, ab1, Cp);
             }
-            if (h + 1 < NG) __syncthreads();
+            if (h + 1 < kTurns) __syncthreads();
         }
     }
 }
 
-// Rows longer than that: the row twice for dx ...
-template <int DT>
-__global__ __launch_bounds__(64 * kLongNW) void ln_bwd_long(
+// The same for rows whose weight gradients leave no room for a second row's loads:
+// x and dy stay packed, gamma comes from the caches.
+template <int DT, int NV>
+__global__ __launch_bounds__(1024) void ln_bwd_wide(
     const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
-    const typename Io<DT>::T *gamma, const float *mean, const float *rstd, int C,
+    const typename Io<DT>::T *__restrict__ gamma, const float *mean, const float *rstd, int R,
+    int C, typename Io<DT>::T *dx, int lddx, int accumulate, float *partial) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E, L = 1024;
+    __shared__ float sm[2][2][L / 64];
+    const int t = threadIdx.x;
+    const Lanes<DT> ln(C, t);
+    const bool one = ln.single < C;
+    const float n = (float)C;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    float ag[NV][E], ab[NV][E], ag1 = 0.0f, ab1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) ag[i][e] = ab[i][e] = 0.0f;
+    const float g1 = gamma && one ? IO::load1(gamma, ln.single) : 1.0f;
+    const uint32_t rows = R;
+    for (uint32_t row = blockIdx.x, it = 0; row < rows; row += gridDim.x, ++it) {
+        const auto *xr = x + (size_t)row * ldx, *dr = dy + (size_t)row * lddy;
+        u32x4 wx[NV], wd[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const bool mine = t + i * L < ln.nb;
+            wx[i] = mine ? fg::rows::load<DT>(xr, t + i * L) : zero;
+            wd[i] = mine ? fg::rows::load<DT>(dr, t + i * L) : zero;
+        }
+        const float m = mean[row], k = rstd[row];
+        const float c1 = (one ? IO::load1(xr, ln.single) : 0.0f) - m;
+        const float d1 = one ? IO::load1(dr, ln.single) : 0.0f, gd1 = d1 * g1;
+        float s1 = gd1, s2 = gd1 * c1;
+        ag1 += d1 * k * c1;
+        ab1 += d1;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            u32x4 g = zero;
+            if (gamma && t + i * L < ln.nb) g = fg::rows::load<DT>(gamma, t + i * L);
+            float p1 = 0.0f, p2 = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float d = IO::get(wd[i], e), c = IO::get(wx[i], e) - m;
+                const float gd = gamma ? d * IO::get(g, e) : d;
+                p1 += gd;
+                p2 += gd * c;
+                ag[i][e] += d * k * c;
+                ab[i][e] += d;
+            }
+            s1 += p1;
+            s2 += p2;
+        }
+        if (!dx) continue;
+        fg::smany::repack(wx);
+        fg::smany::repack(wd);
+        s1 = fg::rows::wave_sum(s1);
+        s2 = fg::rows::wave_sum(s2);
+        float *p = sm[it & 1][0], *q = sm[it & 1][1];
+        if ((t & 63) == 0) {
+            p[t >> 6] = s1;
+            q[t >> 6] = s2;
+        }
+        __syncthreads();
+        s1 = p[0];
+        s2 = q[0];
+#pragma unroll
+        for (int h = 1; h < L / 64; ++h) {
+            s1 += p[h];
+            s2 += q[h];
+        }
+        const float m1 = s1 / n, m2 = k * (k * s2 / n);
+        auto *out = dx + (size_t)row * lddx;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = t + i * L;
+            if (j >= ln.nb) continue;
+            u32x4 g = zero;
+            if (gamma) g = fg::rows::load<DT>(gamma, j);
+            float o[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float d = IO::get(wd[i], e), c = IO::get(wx[i], e) - m;
+                o[e] = k * ((gamma ? d * IO::get(g, e) : d) - m1 - c * m2);
+            }
+            if (accumulate) {
+                const u32x4 was = fg::rows::load<DT>(out, j);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] += IO::get(was, e);
+            }
+            fg::rows::store<DT>(out, j, IO::pack(o));
+        }
+        if (one) {
+            float o = k * (gd1 - m1 - c1 * m2);
+            if (accumulate) o += IO::load1(out, ln.single);
+            IO::store1(out, ln.single, o);
+        }
+    }
+    const int64_t Cp = padded(C);
+    float *part = partial + (size_t)blockIdx.x * 2 * Cp;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = t + i * L;
+        if (j >= ln.nb) continue;
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q) {
+            float *to = part + (size_t)j * E + 4 * q;
+            *reinterpret_cast<f32x4 *>(to) =
+                f32x4{ag[i][4 * q], ag[i][4 * q + 1], ag[i][4 * q + 2], ag[i][4 * q + 3]};
+            *reinterpret_cast<f32x4 *>(to + Cp) =
+                f32x4{ab[i][4 * q], ab[i][4 * q + 1], ab[i][4 * q + 2], ab[i][4 * q + 3]};
+        }
+    }
+    if (one) {
+        part[ln.single] = ag1;
+        part[Cp + ln.single] = ab1;
+    }
+}
+
+// Rows longer than that: dx from a row held packed, a workgroup a row, as ln_fwd_wide
+// (longer still: the row twice) ...
+template <int DT, int NV>
+__global__ __launch_bounds__(1024) void ln_bwd_dx(
+    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
+    const typename Io<DT>::T *__restrict__ gamma, const float *mean, const float *rstd, int C,
     typename Io<DT>::T *dx, int lddx, int accumulate) {
     using IO = Io<DT>;
-    constexpr int E = IO::E, NT = 64 * kLongNW;
-    __shared__ float sm[2][kLongNW];
-    const size_t r = blockIdx.x;
-    const auto *xr = x + r * ldx, *dr = dy + r * lddy;
-    auto *out = dx + r * lddx;
-    const int wave = threadIdx.x >> 6;
-    const float n = (float)C, m = mean[r], k = rstd[r];
-    float s1 = 0.0f, s2 = 0.0f;
-    for (int64_t c64 = threadIdx.x * E; c64 < C; c64 += NT * E) {
-        const int col = (int)c64, left = C - col;
-        const u32x4 wx = fg::rows::load<DT>(xr, col, left), wd = fg::rows::load<DT>(dr, col, left);
-        u32x4 g;
-        if (gamma) g = fg::rows::load<DT>(gamma, col, left);
+    constexpr int E = IO::E, L = 1024;
+    __shared__ float sm[2][L / 64];
+    const size_t row = blockIdx.x;
+    const auto *xr = x + row * ldx, *dr = dy + row * lddy;
+    auto *out = dx + row * lddx;
+    const int t = threadIdx.x;
+    const Lanes<DT> ln(C, t);
+    const bool one = ln.single < C;
+    const float n = (float)C, m = mean[row], k = rstd[row];
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    u32x4 wx[NV], wd[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const bool mine = t + i * L < ln.nb;
+        wx[i] = mine ? fg::rows::load<DT>(xr, t + i * L) : zero;
+        wd[i] = mine ? fg::rows::load<DT>(dr, t + i * L) : zero;
+    }
+    float c1 = 0.0f, gd1 = 0.0f;
+    if (one) {
+        c1 = IO::load1(xr, ln.single) - m;
+        gd1 = IO::load1(dr, ln.single);
+        if (gamma) gd1 *= IO::load1(gamma, ln.single);
+    }
+    float s1 = gd1, s2 = gd1 * c1;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (t + i * L >= ln.nb) continue;
+        u32x4 g = zero;
+        if (gamma) g = fg::rows::load<DT>(gamma, t + i * L);
         float p1 = 0.0f, p2 = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float d = IO::get(wd, e), gd = gamma ? d * IO::get(g, e) : d;
+            const float d = IO::get(wd[i], e), gd = gamma ? d * IO::get(g, e) : d;
             p1 += gd;
-            p2 += gd * ((IO::get(wx, e) - m) * k);
+            p2 += gd * (IO::get(wx[i], e) - m);
         }
         s1 += p1;
         s2 += p2;
     }
-    const float m1 = row_sum<kLongNW>(s1, sm[0], wave) / n;
-    const float m2 = row_sum<kLongNW>(s2, sm[1], wave) / n;
-    for (int64_t c64 = threadIdx.x * E; c64 < C; c64 += NT * E) {
-        const int col = (int)c64, left = C - col;
-        const u32x4 wx = fg::rows::load<DT>(xr, col, left), wd = fg::rows::load<DT>(dr, col, left);
-        u32x4 g;
-        if (gamma) g = fg::rows::load<DT>(gamma, col, left);
+    const float m1 = row_sum<L>(s1, sm[0], t) / n;
+    const float m2 = k * (k * row_sum<L>(s2, sm[1], t) / n);
+    fg::smany::repack(wx);
+    fg::smany::repack(wd);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int j = t + i * L;
+        if (j >= ln.nb) continue;
+        u32x4 g = zero;
+        if (gamma) g = fg::rows::load<DT>(gamma, j);
         float o[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float d = IO::get(wd, e), xh = (IO::get(wx, e) - m) * k;
-            o[e] = k * ((gamma ? d * IO::get(g, e) : d) - m1 - xh * m2);
+            const float d = IO::get(wd[i], e), c = IO::get(wx[i], e) - m;
+            o[e] = k * ((gamma ? d * IO::get(g, e) : d) - m1 - c * m2);
         }
         if (accumulate) {
-            const u32x4 was = fg::rows::load<DT>(out, col, left);
+            const u32x4 was = fg::rows::load<DT>(out, j);
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] += IO::get(was, e);
         }
-        fg::rows::store<DT>(out, col, left, IO::pack(o));
+        fg::rows::store<DT>(out, j, IO::pack(o));
+    }
+    if (one) {
+        float o = k * (gd1 - m1 - c1 * m2);
+        if (accumulate) o += IO::load1(out, ln.single);
+        IO::store1(out, ln.single, o);
     }
 }
 
-// ... and the columns of a strip over a split of the rows, a chunk a lane.
+template <int DT>
+__global__ __launch_bounds__(kLongL) void ln_bwd_long(
+    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
+    const typename Io<DT>::T *gamma, const float *mean, const float *rstd, int C,
+    typename Io<DT>::T *dx, int lddx, int accumulate) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E;
+    __shared__ float sm[2][kLongL / 64];
+    const size_t r = blockIdx.x;
+    const auto *xr = x + r * ldx, *dr = dy + r * lddy;
+    auto *out = dx + r * lddx;
+    const int t = threadIdx.x;
+    const Lanes<DT> ln(C, t);
+    const bool one = ln.single < C;
+    const float n = (float)C, m = mean[r], k = rstd[r];
+    float c1 = 0.0f, gd1 = 0.0f;
+    if (one) {
+        c1 = IO::load1(xr, ln.single) - m;
+        gd1 = IO::load1(dr, ln.single);
+        if (gamma) gd1 *= IO::load1(gamma, ln.single);
+    }
+    float s1 = gd1, s2 = gd1 * c1;
+    auto chunk = [&](int j, float (&c)[E], float (&gd)[E]) {
+        const u32x4 wx = fg::rows::load<DT>(xr, j), wd = fg::rows::load<DT>(dr, j);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            c[e] = IO::get(wx, e) - m;
+            gd[e] = IO::get(wd, e);
+        }
+        if (gamma) {
+            const u32x4 g = fg::rows::load<DT>(gamma, j);
+#pragma unroll
+            for (int e = 0; e < E; ++e) gd[e] *= IO::get(g, e);
+        }
+    };
+#pragma unroll 4
+    for (int j = t; j < ln.nb; j += kLongL) {
+        float c[E], gd[E], p1 = 0.0f, p2 = 0.0f;
+        chunk(j, c, gd);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            p1 += gd[e];
+            p2 += gd[e] * c[e];
+        }
+        s1 += p1;
+        s2 += p2;
+    }
+    const float m1 = row_sum<kLongL>(s1, sm[0], t) / n;
+    const float m2 = k * (k * row_sum<kLongL>(s2, sm[1], t) / n);
+#pragma unroll 2
+    for (int j = t; j < ln.nb; j += kLongL) {
+        float c[E], o[E];
+        chunk(j, c, o);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = k * (o[e] - m1 - c[e] * m2);
+        if (accumulate) {
+            const u32x4 was = fg::rows::load<DT>(out, j);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] += IO::get(was, e);
+        }
+        fg::rows::store<DT>(out, j, IO::pack(o));
+    }
+    if (one) {
+        float o = k * (gd1 - m1 - c1 * m2);
+        if (accumulate) o += IO::load1(out, ln.single);
+        IO::store1(out, ln.single, o);
+    }
+}
+
+// ... and the columns of a strip over a split of the rows, a chunk a lane (the
+// columns past the last whole chunk, one to a lane, in the strip after it).
 constexpr int kColsNT = 256;
 template <int DT>
 __global__ __launch_bounds__(kColsNT) void ln_bwd_cols(const typename Io<DT>::T *x, int ldx,
@@ -368,32 +751,43 @@ __global__ __launch_bounds__(kColsNT) void ln_bwd_cols(const typename Io<DT>::T 
                                                        int C, int rows, float *partial) {
     using IO = Io<DT>;
     constexpr int E = IO::E;
-    const int64_t c64 = ((int64_t)blockIdx.x * kColsNT + threadIdx.x) * E;
-    if (c64 >= C) return;
-    const int col = (int)c64, left = C - col;
+    const int nb = C / E, j = blockIdx.x * kColsNT + threadIdx.x;
     const int r0 = blockIdx.y * rows, r1 = min(R, r0 + rows);
-    float ag[E], ab[E];
+    const int64_t Cp = padded(C);
+    float *p = partial + (size_t)blockIdx.y * 2 * Cp;
+    if (j < nb) {
+        float ag[E], ab[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) ag[e] = ab[e] = 0.0f;
+        for (int e = 0; e < E; ++e) ag[e] = ab[e] = 0.0f;
 #pragma unroll 4
-    for (int r = r0; r < r1; ++r) {
-        const u32x4 wx = fg::rows::load<DT>(x + (size_t)r * ldx, col, left);
-        const u32x4 wd = fg::rows::load<DT>(dy + (size_t)r * lddy, col, left);
-        const float m = mean[r], k = rstd[r];
+        for (int r = r0; r < r1; ++r) {
+            const u32x4 wx = fg::rows::load<DT>(x + (size_t)r * ldx, j);
+            const u32x4 wd = fg::rows::load<DT>(dy + (size_t)r * lddy, j);
+            const float m = mean[r], k = rstd[r];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float d = IO::get(wd, e);
+                ag[e] += d * k * (IO::get(wx, e) - m);
+                ab[e] += d;
+            }
+        }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const float d = IO::get(wd, e);
-            ag[e] += d * ((IO::get(wx, e) - m) * k);
-            ab[e] += d;
+            p[(size_t)j * E + e] = ag[e];
+            p[Cp + (size_t)j * E + e] = ab[e];
         }
+    } else if (nb * E + (j - nb) < C) {
+        const int col = nb * E + (j - nb);
+        float ag = 0.0f, ab = 0.0f;
+#pragma unroll 4
+        for (int r = r0; r < r1; ++r) {
+            const float d = IO::load1(dy + (size_t)r * lddy, col);
+            ag += d * rstd[r] * (IO::load1(x + (size_t)r * ldx, col) - mean[r]);
+            ab += d;
+        }
+        p[col] = ag;
+        p[Cp + col] = ab;
     }
-    float *p = partial + (size_t)blockIdx.y * 2 * C;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (e < left) {
-            p[col + e] = ag[e];
-            p[(size_t)C + col + e] = ab[e];
-        }
 }
 
 // Adds the partial sums of each column: 16 threads a column, each a run of them in
@@ -404,13 +798,15 @@ __global__ __launch_bounds__(kFinalCols *kFinalGroups) void ln_bwd_final(
     void *dbeta, int acc_b) {
     __shared__ float sh[kFinalGroups][kFinalCols];
     const int c = threadIdx.x % kFinalCols, q = threadIdx.x / kFinalCols;
-    const int64_t at = (int64_t)blockIdx.x * kFinalCols + c;  // of the 2 C columns
+    const int64_t Cp = padded(C), N = 2 * Cp;
+    const int64_t at = (int64_t)blockIdx.x * kFinalCols + c;
+    const int64_t i = at < Cp ? at : at - Cp;
     const int per = (splits + kFinalGroups - 1) / kFinalGroups;
     int k = q * per;
     const int end = min(splits, k + per);
-    const int64_t N = 2 * (int64_t)C;
+    const bool mine = at < N && i < C;
     float s = 0.0f;
-    if (at < N) {
+    if (mine) {
         for (; k + 8 <= end; k += 8) {
             float v[8];
 #pragma unroll
@@ -422,57 +818,53 @@ __global__ __launch_bounds__(kFinalCols *kFinalGroups) void ln_bwd_final(
     }
     sh[q][c] = s;
     __syncthreads();
-    if (q != 0 || at >= N) return;
+    if (q != 0 || !mine) return;
 #pragma unroll
-    for (int n = 1; n < kFinalGroups; ++n) s += sh[n][c];
-    void *out = at < C ? dgamma : dbeta;
+    for (int h = 1; h < kFinalGroups; ++h) s += sh[h][c];
+    void *out = at < Cp ? dgamma : dbeta;
     if (!out) return;
-    const int64_t i = at < C ? at : at - C;
-    fg::store_from_f(out, dt, i, (at < C ? acc_g : acc_b) ? fg::load_as_f(out, dt, i) + s : s);
+    fg::store_from_f(out, dt, i, (at < Cp ? acc_g : acc_b) ? fg::load_as_f(out, dt, i) + s : s);
 }
 
 // ------------------------------------------------------------------ choices
-// Runs f<NV, NW, NG>() for a row of `chunks` 16-byte chunks; false: longer than
-// any holds.
+// Runs f<NV, L, NG>() for a row of `chunks` whole 16-byte chunks; false: longer
+// than any holds.
+#define FG_LN_KIND(NV, L, NG)                                         \
+    if (chunks <= NV * L) {                                           \
+        f(integral_constant<int, NV>{}, integral_constant<int, L>{},  \
+          integral_constant<int, NG>{});                              \
+        return true;                                                  \
+    }
 template <class F>
 bool fwd_kind(int chunks, bool few, F f) {
     using std::integral_constant;
-#define FG_LN_KIND(NV, NW, NG)                                              \
-    if (chunks <= NV * NW * 64) {                                           \
-        f(integral_constant<int, NV>{}, integral_constant<int, NW>{},       \
-          integral_constant<int, NG>{});                                    \
-        return true;                                                        \
-    }
     if (few) {
-        FG_LN_KIND(1, 1, 1)
-        FG_LN_KIND(1, 4, 1)
-        FG_LN_KIND(1, 16, 1)
+        FG_LN_KIND(1, 64, 1)
+        FG_LN_KIND(1, 256, 1)
+        FG_LN_KIND(1, 1024, 1)
     }
-    FG_LN_KIND(1, 1, 4)
-    FG_LN_KIND(2, 1, 4)
-    FG_LN_KIND(4, 1, 4)
-    FG_LN_KIND(2, 4, 1)
-    FG_LN_KIND(4, 4, 1)
-    FG_LN_KIND(4, 8, 1)
-    FG_LN_KIND(4, 16, 1)
+    FG_LN_KIND(1, 16, 16)
+    FG_LN_KIND(2, 16, 16)
+    FG_LN_KIND(1, 64, 4)
+    FG_LN_KIND(2, 64, 4)
+    FG_LN_KIND(4, 64, 4)
+    FG_LN_KIND(2, 256, 1)
+    FG_LN_KIND(4, 256, 1)
     return false;
 }
-
 template <int DT, class F>
 bool bwd_kind(int chunks, F f) {
     using std::integral_constant;
-    FG_LN_KIND(1, 1, 8)
-    FG_LN_KIND(2, 1, 8)
-    FG_LN_KIND(2, 2, 4)
-    FG_LN_KIND(2, 4, 2)
-    FG_LN_KIND(2, 8, 1)
-    FG_LN_KIND(2, 16, 1)
-    if constexpr (DT == fg::kF32) {
-        FG_LN_KIND(4, 16, 1)
-    }
-#undef FG_LN_KIND
+    FG_LN_KIND(1, 16, 32)
+    FG_LN_KIND(2, 16, 32)
+    FG_LN_KIND(1, 64, 8)
+    FG_LN_KIND(2, 64, 8)
+    FG_LN_KIND(2, 128, 4)
+    FG_LN_KIND(2, 256, 2)
+    FG_LN_KIND(2, 512, 1)
     return false;
 }
+#undef FG_LN_KIND
 
 template <int DT>
 void launch_fwd(fg_ctx *ctx, const void *x, int ldx, const void *gamma, const void *beta,
@@ -481,34 +873,49 @@ void launch_fwd(fg_ctx *ctx, const void *x, int ldx, const void *gamma, const vo
     const T *xt = static_cast<const T *>(x), *gt = static_cast<const T *>(gamma),
             *bt = static_cast<const T *>(beta);
     T *yt = static_cast<T *>(y);
-    const int chunks = (C - 1) / Io<DT>::E + 1;
     const bool few = R < 2 * ctx->cu_count;
-    const bool held = fwd_kind(chunks, few, [&](auto nv, auto nw, auto ng) {
-        const int per_cu = 32 / (nw() * ng());
+    const bool held = fwd_kind(C / Io<DT>::E, few, [&](auto nv, auto l, auto ng) {
+        const int per_cu = (nv() == 1 ? 32 : 12) * 64 / (l() * ng());
         const int grid = std::min((R - 1) / ng() + 1, ctx->cu_count * std::max(1, per_cu));
-        ln_fwd<DT, nv(), nw(), ng()><<<grid, 64 * nw() * ng(), 0, ctx->stream>>>(
+        ln_fwd<DT, nv(), l(), ng()><<<grid, l() * ng(), 0, ctx->stream>>>(
             xt, ldx, gt, bt, eps, R, C, yt, ldy, mean, rstd);
     });
-    if (!held)
-        ln_fwd_long<DT><<<R, 64 * kLongNW, 0, ctx->stream>>>(xt, ldx, gt, bt, eps, C, yt, ldy, mean,
-                                                             rstd);
+    const int chunks = C / Io<DT>::E;
+    if (held) return;
+#define FG_LN_WIDE(NV, L)                                                                       \
+    if (chunks <= NV * L) {                                                                     \
+        ln_fwd_wide<DT, NV, L><<<R, L, 0, ctx->stream>>>(xt, ldx, gt, bt, eps, C, yt, ldy, mean, \
+                                                         rstd);                                 \
+        return;                                                                                 \
+    }
+    FG_LN_WIDE(4, 256)
+    FG_LN_WIDE(4, 512)
+    FG_LN_WIDE(4, 1024)
+    FG_LN_WIDE(8, 1024)
+#undef FG_LN_WIDE
+    ln_fwd_long<DT><<<R, kLongL, 0, ctx->stream>>>(xt, ldx, gt, bt, eps, C, yt, ldy, mean, rstd);
 }
 
 // How a backward call's rows are shared out: workgroups of the held rows, or the
 // row splits of the long ones.
 struct Split {
     int splits = 0, rows = 0, strips = 0;
-    bool held = false;
+    bool held = false, wide = false;
 };
 Split split_of(int cus, int dtype, int R, int C) {
     Split s;
-    const int E = dtype == FG_DTYPE_F32 ? 4 : 8, chunks = (C - 1) / E + 1;
+    const int E = dtype == FG_DTYPE_F32 ? 4 : 8, chunks = C / E;
     auto held = [&](auto, auto, auto ng) {
-        s.splits = std::min(R > 0 ? (R - 1) / ng() + 1 : 0, 2 * cus);
+        s.splits = std::min(R > 0 ? (R - 1) / ng() + 1 : 0, cus);
     };
     s.held = E == 4 ? bwd_kind<fg::kF32>(chunks, held) : bwd_kind<fg::kBF16>(chunks, held);
     if (s.held) return s;
-    s.strips = (chunks - 1) / kColsNT + 1;
+    s.wide = chunks <= (E == 4 ? 4 : 2) * 1024;
+    if (s.wide) {
+        s.splits = std::min(R, cus);
+        return s;
+    }
+    s.strips = (chunks + C % E - 1) / kColsNT + 1;
     const int want = std::max(1, std::min((4 * cus - 1) / s.strips + 1, (R + 15) / 16));
     s.rows = R > 0 ? (R - 1) / want + 1 : 1;
     s.splits = R > 0 ? (R - 1) / s.rows + 1 : 0;
@@ -525,16 +932,26 @@ int launch_bwd(fg_ctx *ctx, const Split &s, const void *x, int ldx, const void *
     T *ot = static_cast<T *>(dx);
     hipStream_t st = ctx->stream;
     if (s.held) {
-        bwd_kind<DT>((C - 1) / Io<DT>::E + 1, [&](auto nv, auto nw, auto ng) {
-            const size_t lds = ng() > 1 ? 2 * (size_t)C * sizeof(float) : 0;
+        bwd_kind<DT>(C / Io<DT>::E, [&](auto nv, auto l, auto ng) {
+            const size_t lds = ng() > 1 ? 2 * (size_t)padded(C) * sizeof(float) : 0;
             if (partial)
-                ln_bwd<DT, nv(), nw(), ng(), true><<<s.splits, 64 * nw() * ng(), lds, st>>>(
+                ln_bwd<DT, nv(), l(), ng(), true><<<s.splits, l() * ng(), lds, st>>>(
                     xt, ldx, dt, lddy, gt, mean, rstd, R, C, ot, lddx, accumulate, partial);
             else
-                ln_bwd<DT, nv(), nw(), ng(), false><<<s.splits, 64 * nw() * ng(), 0, st>>>(
+                ln_bwd<DT, nv(), l(), ng(), false><<<s.splits, l() * ng(), 0, st>>>(
                     xt, ldx, dt, lddy, gt, mean, rstd, R, C, ot, lddx, accumulate, partial);
         });
         FG_LAUNCH_CHECK("ln_bwd");
+        return FG_OK;
+    }
+    if (s.wide && partial) {
+        const int chunks = C / Io<DT>::E;
+        auto kernel = ln_bwd_wide<DT, 2>;
+        if constexpr (DT == fg::kF32)
+            if (chunks > 2 * 1024) kernel = ln_bwd_wide<DT, 4>;
+        kernel<<<s.splits, 1024, 0, st>>>(xt, ldx, dt, lddy, gt, mean, rstd, R, C, ot, lddx,
+                                          accumulate, partial);
+        FG_LAUNCH_CHECK("ln_bwd_wide");
         return FG_OK;
     }
     // The weights' gradients first: dx may be written over x or dy.
@@ -543,9 +960,16 @@ int launch_bwd(fg_ctx *ctx, const Split &s, const void *x, int ldx, const void *
                                                                      R, C, s.rows, partial);
         FG_LAUNCH_CHECK("ln_bwd_cols");
     }
-    if (dx) {
-        ln_bwd_long<DT><<<R, 64 * kLongNW, 0, st>>>(xt, ldx, dt, lddy, gt, mean, rstd, C, ot, lddx,
-                                                    accumulate);
+    if (dx && C / Io<DT>::E <= 8 * 1024) {
+        const int chunks = C / Io<DT>::E;
+        auto kernel = chunks <= 2 * 1024   ? ln_bwd_dx<DT, 2>
+                      : chunks <= 4 * 1024 ? ln_bwd_dx<DT, 4>
+                                           : ln_bwd_dx<DT, 8>;
+        kernel<<<R, 1024, 0, st>>>(xt, ldx, dt, lddy, gt, mean, rstd, C, ot, lddx, accumulate);
+        FG_LAUNCH_CHECK("ln_bwd_dx");
+    } else if (dx) {
+        ln_bwd_long<DT><<<R, kLongL, 0, st>>>(xt, ldx, dt, lddy, gt, mean, rstd, C, ot, lddx,
+                                              accumulate);
         FG_LAUNCH_CHECK("ln_bwd_long");
     }
     return FG_OK;
@@ -556,7 +980,7 @@ int launch_bwd(fg_ctx *ctx, const Split &s, const void *x, int ldx, const void *
 namespace fg {
 uint64_t layer_norm_bwd_ws_bytes(int cus, int dtype, int R, int C) {
     const Split s = split_of(cus > 0 ? cus : 256, dtype, R, C);
-    return (uint64_t)std::max(s.splits, 1) * 2 * (uint64_t)C * sizeof(float);
+    return (uint64_t)std::max(s.splits, 1) * 2 * (uint64_t)padded(C) * sizeof(float);
 }
 }  // namespace fg
 
@@ -616,7 +1040,7 @@ FG_API int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, c
             return rc;
     }
     if (partial) {
-        ln_bwd_final<<<(unsigned)((2 * (int64_t)C - 1) / kFinalCols + 1), kFinalCols * kFinalGroups,
+        ln_bwd_final<<<(unsigned)((2 * padded(C) - 1) / kFinalCols + 1), kFinalCols * kFinalGroups,
                        0, ctx->stream>>>(dtype, partial, s.splits, C, d_dgamma, dgamma_accumulate,
                                          d_dbeta, dbeta_accumulate);
         FG_LAUNCH_CHECK("ln_bwd_final");
