@@ -38,6 +38,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kNT = 256;
 constexpr int kDirectMax = 256;
 constexpr int kRankMax = 16384;
+#ifndef UB
+#define UB 1024
+#endif
+constexpr int kUnitBlocks = UB;
 
 // A row's chunk j where j is below its whole chunks nb, or (j == nb) its last,
 // partial one, one element after the other.
@@ -151,11 +155,18 @@ __global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ 
             float a[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) a[e] = 0.0f;
-            for (int k = first; k <= last; ++k) {
-                if (tok[k] != v) continue;
-                const u32x4 w = Chunk<DT>::load(dout + (size_t)at[k] * lddo, j, nb, C);
+            for (int k = first; k <= last; k += 8) {
+                u32x4 w[8];
 #pragma unroll
-                for (int e = 0; e < E; ++e) a[e] += IO::get(w, e);
+                for (int u = 0; u < 8; ++u) {
+                    const bool own = k + u <= last && tok[k + u] == v;
+                    w[u] = u32x4{0u, 0u, 0u, 0u};
+                    if (own) w[u] = Chunk<DT>::load(dout + (size_t)at[k + u] * lddo, j, nb, C);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) a[e] += IO::get(w[u], e);
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) a[e] *= scale;
@@ -171,7 +182,11 @@ __global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ 
 
 // ------------------------------------------------------------------- sorting
 // order[k] = the k-th position in (token, position) order, sorted[k] its token: a
-// lane counts the positions before its own, 16 waves a share of the tokens each.
+// lane counts the positions before its own; 16 waves take a share of the tokens
+// each, 64 at a time in scalar registers, so that a comparison and an addition with
+// carry are all a lane does for a token.
+typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
+typedef u32x16 u32x16_any __attribute__((aligned(4)));
 __global__ __launch_bounds__(1024) void emb_rank(const uint32_t *__restrict__ tokens, int T,
                                                  uint32_t *__restrict__ order,
                                                  uint32_t *__restrict__ sorted) {
@@ -179,18 +194,31 @@ __global__ __launch_bounds__(1024) void emb_rank(const uint32_t *__restrict__ to
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g0 = blockIdx.x * 64, i = g0 + lane;
     const uint32_t mine = i < T ? tokens[i] : 0xffffffffu;
-    const int per = (T + 15) / 16, j0 = wave * per, j1 = min(T, j0 + per);
-    int before = 0;
-    // Positions before the workgroup's 64, the 64, and those after them.
-    int j = j0;
-#pragma unroll 8
-    for (; j < min(j1, g0); ++j) before += tokens[j] <= mine;
-    for (; j < min(j1, g0 + 64); ++j) {
-        const uint32_t o = tokens[j];
-        before += o < mine || (o == mine && j < i);
+    const int per = ((T + 15) / 16 + 63) & ~63, j0 = wave * per, j1 = min(T, j0 + per);
+    int before = 0, j = j0;
+    // Equal tokens count where they lie before the workgroup's 64 positions, and not
+    // after them; the 64 themselves are in wave 0's lanes.
+    auto count = [&](int end, auto counts) {
+        for (; j + 64 <= end; j += 64) {
+            u32x16 o[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                o[q] = *reinterpret_cast<const u32x16_any *>(tokens + j + 16 * q);
+#pragma unroll
+            for (int e = 0; e < 64; ++e) before += counts(o[e / 16][e % 16]);
+        }
+        for (; j < end; ++j) before += counts(tokens[j]);
+    };
+    count(min(j1, g0), [&](uint32_t o) { return o <= mine; });
+    j = max(j, g0 + 64);
+    count(j1, [&](uint32_t o) { return o < mine; });
+    if (wave == 0) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) {
+            const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)mine, e);
+            before += o < mine || (o == mine && e < lane);
+        }
     }
-#pragma unroll 8
-    for (; j < j1; ++j) before += tokens[j] < mine;
     sum[wave][lane] = before;
     __syncthreads();
     if (wave == 0 && i < T) {
@@ -203,7 +231,7 @@ __global__ __launch_bounds__(1024) void emb_rank(const uint32_t *__restrict__ to
 }
 
 // Stable radix sort, least significant digit first, of (token, position) pairs:
-// tile b of the input counts its digits (radix_count: hist[digit][tile]), then
+// tile b of the input counts its digits (radix_count: hist[tile][digit]), then
 // places its pairs behind those of smaller digits and of earlier tiles
 // (radix_place).  Tokens outside the table sort as V.
 constexpr int kMaxBits = 11, kBins = 1 << kMaxBits;
@@ -224,7 +252,7 @@ __global__ __launch_bounds__(kSortNT) void radix_count(const uint32_t *__restric
         atomicAdd(&h[(key_of(keys[i], V) >> shift) & (bins - 1)], 1u);  // (counts: any order)
     __syncthreads();
     for (int d = threadIdx.x; d < bins; d += kSortNT)
-        hist[(size_t)d * gridDim.x + blockIdx.x] = h[d];
+        hist[((size_t)blockIdx.x << bits) + d] = h[d];
 }
 
 // pos NULL: the pairs' positions are their own indices (the first pass).
@@ -241,22 +269,51 @@ __global__ __launch_bounds__(kSortNT) void radix_place(const uint32_t *__restric
     __shared__ uint32_t wsum[kWaves];
     const int bins = 1 << bits, tiles = gridDim.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int k = threadIdx.x; k < kWaves * bins; k += kSortNT) cnt[k >> bits][k & (bins - 1)] = 0;
-    // base[d] = pairs of digit d in earlier tiles, and of smaller digits: a digit's
-    // tiles by consecutive threads' loads, then a scan over the digits.
-    constexpr int kOwn = kBins / kSortNT;  // digits of a thread
+    // Each wave takes a run of the tile, 64 pairs at a time; the first kHeld rounds'
+    // pairs are loaded here and stay in registers.
+    constexpr int kHeld = 4;
+    const int64_t t0 = (int64_t)blockIdx.x * per, t1 = min((int64_t)T, t0 + per);
+    const int run = (per + kWaves - 1) / kWaves;
+    const int64_t i0 = t0 + (int64_t)wave * run, i1 = min(t1, i0 + run);
+    auto key_at = [&](int64_t i) { return i + lane < i1 ? key_of(keys[i + lane], V) : 0u; };
+    auto pos_at = [&](int64_t i) {
+        return pos && i + lane < i1 ? pos[i + lane] : (uint32_t)(i + lane);
+    };
+    uint32_t hkey[kHeld], hpos[kHeld];
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+        hkey[u] = key_at(i0 + 64 * u);
+        hpos[u] = pos_at(i0 + 64 * u);
+    }
+    // base[d] = pairs of digit d in earlier tiles, and of smaller digits: thread
+    // (g, d) adds the digit's counts of every G-th tile, the threads of a digit are
+    // added in LDS (in cnt, which is cleared after), then a scan over the digits.
+    constexpr int kOwn = kBins / kSortNT;  // digits of a thread in the scan
+    const int G = max(1, kSortNT >> bits);
+    for (int d0 = threadIdx.x; d0 < max(bins, kSortNT); d0 += kSortNT) {
+        const int d = d0 & (bins - 1), g = d0 >> bits;
+        uint32_t before = 0, all = 0;
+        if (g < G) {
+#pragma unroll 16
+            for (int b = g; b < tiles; b += G) {
+                const uint32_t c = hist[((size_t)b << bits) + d];
+                all += c;
+                before += b < (int)blockIdx.x ? c : 0u;
+            }
+            cnt[0][d0] = all;  // (G * bins <= 2 kSortNT = kBins values each)
+            cnt[1][d0] = before;
+        }
+    }
+    __syncthreads();
     uint32_t total[kOwn], mine = 0;
 #pragma unroll
     for (int u = 0; u < kOwn; ++u) {
         const int d = threadIdx.x * kOwn + u;
         uint32_t before = 0, all = 0;
         if (d < bins) {
-            const uint32_t *h = hist + (size_t)d * tiles;
-#pragma unroll 8
-            for (int b = 0; b < tiles; ++b) {
-                const uint32_t c = h[b];
-                all += c;
-                before += b < (int)blockIdx.x ? c : 0u;
+            for (int g = 0; g < G; ++g) {
+                all += cnt[0][(g << bits) + d];
+                before += cnt[1][(g << bits) + d];
             }
             base[d] = before;
         }
@@ -279,10 +336,9 @@ __global__ __launch_bounds__(kSortNT) void radix_place(const uint32_t *__restric
         if (d < bins) base[d] += excl;
         excl += total[u];
     }
-    // Each wave takes a run of the tile, 64 pairs at a time.
-    const int64_t t0 = (int64_t)blockIdx.x * per, t1 = min((int64_t)T, t0 + per);
-    const int run = (per + kWaves - 1) / kWaves;
-    const int64_t i0 = t0 + (int64_t)wave * run, i1 = min(t1, i0 + run);
+    __syncthreads();
+    for (int k = threadIdx.x; k < kWaves * bins; k += kSortNT) cnt[k >> bits][k & (bins - 1)] = 0;
+    __syncthreads();
     // Lanes of a round with the lane's digit.
     auto same = [&](uint32_t d, bool in) {
         uint64_t m = __ballot(in);
@@ -292,13 +348,18 @@ __global__ __launch_bounds__(kSortNT) void radix_place(const uint32_t *__restric
         }
         return m;
     };
-    for (int64_t i = i0; i < i1; i += 64) {
+    auto count = [&](int64_t i, uint32_t key) {
         const bool in = i + lane < i1;
-        const uint32_t d = in ? (key_of(keys[i + lane], V) >> shift) & (bins - 1) : 0u;
+        const uint32_t d = (key >> shift) & (bins - 1);
         const uint64_t m = same(d, in);
+        // (A wave's LDS accesses run in order: a round reads what the last one wrote.)
         if (in && lane == __ffsll((long long)m) - 1) cnt[wave][d] += (uint32_t)__popcll(m);
         __builtin_amdgcn_wave_barrier();
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+        if (i0 + 64 * u < i1) count(i0 + 64 * u, hkey[u]);
+    for (int64_t i = i0 + 64 * kHeld; i < i1; i += 64) count(i, key_at(i));
     __syncthreads();
     for (int d = threadIdx.x; d < bins; d += kSortNT) {
         uint32_t at = base[d];
@@ -310,15 +371,12 @@ __global__ __launch_bounds__(kSortNT) void radix_place(const uint32_t *__restric
         }
     }
     __syncthreads();
-    for (int64_t i = i0; i < i1; i += 64) {
+    auto place = [&](int64_t i, uint32_t key, uint32_t p) {
         const bool in = i + lane < i1;
-        const uint32_t key = in ? key_of(keys[i + lane], V) : 0u;
-        const uint32_t p = in && pos ? pos[i + lane] : (uint32_t)(i + lane);
         const uint32_t d = (key >> shift) & (bins - 1);
         const uint64_t m = same(d, in);
         uint32_t to = 0;
         if (in) to = cnt[wave][d] + (uint32_t)__popcll(m & ((1ull << lane) - 1));
-        // (A wave's LDS accesses run in order: the next round reads what this one wrote.)
         __builtin_amdgcn_wave_barrier();
         if (in && lane == __ffsll((long long)m) - 1) cnt[wave][d] += (uint32_t)__popcll(m);
         __builtin_amdgcn_wave_barrier();
@@ -326,7 +384,11 @@ __global__ __launch_bounds__(kSortNT) void radix_place(const uint32_t *__restric
             keys_out[to] = key;
             pos_out[to] = p;
         }
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+        if (i0 + 64 * u < i1) place(i0 + 64 * u, hkey[u], hpos[u]);
+    for (int64_t i = i0 + 64 * kHeld; i < i1; i += 64) place(i, key_at(i), pos_at(i));
 }
 
 // ---------------------------------------------------------------------- sums
@@ -394,10 +456,12 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
         }
         __syncthreads();
         const float z[E] = {};
-        for (int r = 0; r < n; ++r) {
+        const int lanes = 1 << p.lshift;
+        for (int r = threadIdx.x >> p.lshift; r < n; r += kNT >> p.lshift) {
             if (used[r]) continue;
             auto *to = dtable + (size_t)(v0 + r) * p.lddt;
-            for (int j = threadIdx.x; j < chunks; j += kNT) Chunk<DT>::store(to, j, nb, p.C, z);
+            for (int j = threadIdx.x & (lanes - 1); j < chunks; j += lanes)
+                Chunk<DT>::store(to, j, nb, p.C, z);
         }
         return;
     }
@@ -460,35 +524,48 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
 }
 
 // Joins the partial sums of the run that begins in unit blockIdx.x and goes on after
-// it (if one does), 4 columns a lane, a share of the units a wave.
-constexpr int kJoinCols = 256;
+// it (if one does): 4 columns a lane, 2^jshift lanes across the columns, and the
+// workgroup's other lanes and waves a share of the run's units each.
+constexpr int kJoinNT = 256;
 template <int DT>
-__global__ __launch_bounds__(kNT) void emb_join(const Sums p, typename Io<DT>::T *dtable) {
+__global__ __launch_bounds__(kJoinNT) void emb_join(const Sums p, typename Io<DT>::T *dtable,
+                                                    int jshift) {
     using IO = Io<DT>;
-    constexpr int kWaves = kNT / 64;
-    __shared__ f32x4 sh[kWaves][64];
-    const int u0 = blockIdx.x, k1 = (u0 + 1) * p.P, k0 = u0 * p.P;  // (the last unit joins nothing)
-    const uint32_t v = p.sorted[k1 - 1];
-    if (v >= (uint32_t)p.V || p.sorted[k1] != v) return;
-    if (p.sorted[k0] == v && k0 > 0 && p.sorted[k0 - 1] == v) return;  // began earlier
-    const int end = wave_lower_bound(p.sorted, p.T, v + 1);  // (v + 1 <= V: no overflow)
-    const int u1 = (end - 1) / p.P;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.y * kJoinCols + lane * 4;
-    f32x4 a = {0.f, 0.f, 0.f, 0.f};
-    const int n = u1 - u0 + 1, per = (n + kWaves - 1) / kWaves;
-    const int b0 = wave * per, b1 = min(n, b0 + per);
-    if (col < p.Cp) {
-#pragma unroll 8
-        for (int b = b0; b < b1; ++b)
-            a += *reinterpret_cast<const f32x4 *>(
-                p.partial + ((size_t)(u0 + b) * 2 + (b == 0 ? 1 : 0)) * p.Cp + col);
+    __shared__ f32x4 sh[kJoinNT];
+    const int u0 = blockIdx.x, k0 = u0 * p.P, k1 = k0 + p.P;  // (k1 < T: the last unit joins nothing)
+    const int lane = threadIdx.x & 63;
+    const uint32_t v = p.sorted[k1 - 1], first = p.sorted[k0], prev = p.sorted[max(k0 - 1, 0)];
+    // Units after u0 that begin with v, 64 at a time (the first of them beside the
+    // loads above).
+    int n = 1;
+    for (;;) {
+        const int64_t at = (int64_t)(u0 + n + lane) * p.P;
+        const uint64_t on = __ballot(at < p.T && p.sorted[at < p.T ? at : 0] == v);
+        const int c = on == ~0ull ? 64 : __ffsll((long long)~on) - 1;
+        n += c;
+        if (n == 1 || v >= (uint32_t)p.V || (k0 > 0 && first == v && prev == v)) return;
+        if (c < 64) break;
     }
-    sh[wave][lane] = a;
+    const int lanes = 1 << jshift, splits = kJoinNT >> jshift;
+    const int64_t col = ((int64_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * 4;
+    const int split = threadIdx.x >> jshift, per = (n + splits - 1) / splits;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    if (col < p.Cp) {
+        int b = split * per;
+        const int end = min(n, b + per);
+        const float *at = p.partial + ((size_t)u0 * 2) * p.Cp + col;
+        if (b == 0) {
+            a = *reinterpret_cast<const f32x4 *>(at + p.Cp);
+            ++b;
+        }
+#pragma unroll 16
+        for (; b < end; ++b) a += *reinterpret_cast<const f32x4 *>(at + (size_t)b * 2 * p.Cp);
+    }
+    sh[threadIdx.x] = a;
     __syncthreads();
-    if (wave != 0) return;
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) a += sh[w][lane];
+    if (split != 0 || col >= p.Cp) return;
+    const int used = min(splits, (n - 1) / per + 1);
+    for (int w = 1; w < used; ++w) a += sh[threadIdx.x + (w << jshift)];
     auto *to = dtable + (size_t)v * p.lddt;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -523,11 +600,12 @@ Plan plan_of(int dtype, int T, int V, int C) {
     const int E = dtype == FG_DTYPE_F32 ? 4 : 8, chunks = (C - 1) / E + 1;
     p.lshift = lane_shift(chunks);
     p.Cp = (int64_t)chunks * E;
-    // About 2048 workgroups of units of 8 to 128 positions.
+    // About 1024 workgroups of units of 8 to 512 positions, and at most 4096 units (the
+    // longest run joins as many).
     const int64_t tiles = (chunks - 1) / (1 << p.lshift) + 1;
     const int64_t lanes = ((int64_t)T << p.lshift) * tiles;  // with one position a unit
     p.P = 8;
-    while (p.P < 128 && lanes / p.P > 2048 * kNT) p.P *= 2;
+    while (p.P < 512 && (lanes / p.P > kUnitBlocks * kNT || T / p.P > 4096)) p.P *= 2;
     p.units = (T - 1) / p.P + 1;
     p.partial_floats = (uint64_t)p.units * 2 * (uint64_t)p.Cp;
     p.sort_words = 2 * (uint64_t)T;
@@ -622,8 +700,9 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
     emb_sums<DT><<<dim3(blocks, tiles), kNT, 0, st>>>(s, d, g);
     FG_LAUNCH_CHECK("emb_sums");
     if (pl.units > 1) {
-        emb_join<DT><<<dim3(pl.units - 1, (unsigned)((pl.Cp - 1) / kJoinCols + 1)), kNT, 0, st>>>(s,
-                                                                                                g);
+        const int jshift = std::min(6, log2_up(pl.Cp / 4));
+        emb_join<DT><<<dim3(pl.units - 1, (unsigned)(((pl.Cp / 4 - 1) >> jshift) + 1)), kJoinNT, 0,
+                       st>>>(s, g, jshift);
         FG_LAUNCH_CHECK("emb_join");
     }
     return FG_OK;
