@@ -245,7 +245,7 @@ class Context:
                          dtype: int = DTYPE_F32) -> None:
         """matmul_bwd of X.W with X = act(z) and z[M][K] kept by ckpt8_save:
         dW = act(z)^T.dZ (+ dbias = colsum(dZ)), dX = (dZ.W^T) * act'(z).  Xr
-        and (with an activation) Zr are scratch of M x K elements."""
+        and (for GELU) Zr are scratch of M x K elements."""
         call("fg_matmul_bwd_ckpt8", self.handle, dtype, M, N, K, act, _ptr(q), ldq, _ptr(e), lde,
              _ptr(W), ldw, _ptr(dZ), lddz, _ptr(Zr), _ptr(Xr), _ptr(dX), lddx, _ptr(dW), lddw,
              _ptr(dbias), int(accumulate))

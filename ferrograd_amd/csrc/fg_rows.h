@@ -40,6 +40,31 @@ __device__ __forceinline__ void store(typename Io<DT>::T *row, int j, u32x4 w) {
         w, reinterpret_cast<u32x4_any *>(reinterpret_cast<char *>(row) + (uint32_t)j * 16u));
 }
 
+// A row's chunk j where j is below its whole chunks nb, else what the row has of it,
+// one element after the other (zeros past the row's end).
+template <int DT>
+struct Chunk {
+    using IO = Io<DT>;
+    static constexpr int E = IO::E;
+    static __device__ __forceinline__ u32x4 load(const typename IO::T *row, int j, int nb, int C) {
+        if (j < nb) return rows::load<DT>(row, j);
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = j * E + e < C ? IO::load1(row, j * E + e) : 0.0f;
+        return IO::pack(v);
+    }
+    static __device__ __forceinline__ void store(typename IO::T *row, int j, int nb, int C,
+                                                 const float (&v)[E]) {
+        if (j < nb) {
+            rows::store<DT>(row, j, IO::pack(v));
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (j * E + e < C) IO::store1(row, j * E + e, v[e]);
+    }
+};
+
 // Sum over a wave's 64 lanes (all active), the same in every lane: the 16-lane
 // rows by DPP, then the four rows' sums.
 __device__ __forceinline__ float wave_sum(float s) {

@@ -13,66 +13,243 @@
 // restored value has at most 7 significant bits and no bit below what its type
 // can hold: it is exact in fp32, fp16 and bf16.  A block that holds an infinity
 // or NaN gets b = 255 and is restored as NaN.
+//
+// All three passes are bound by HBM.  A lane takes a 16-byte chunk of a row (a block
+// is four lanes, eight in fp32) and, of the 8-bit form, the chunk's 8 or 4 bytes, so
+// that every access of a wave is one stretch of memory: with 16 columns a lane, each
+// store of a wave left gaps, and 2048 x 4096 fp32 there and back took 64 us.  Rows may
+// start anywhere.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fg_act.h"
 #include "fg_half.h"
 #include "fg_internal.h"
+#include "fg_rows.h"
 
 namespace {
 
+using fg::rows::Chunk;
+using fg::rows::Io;
+using fg::rows::u32x2;
+using fg::rows::u32x4;
+
 constexpr int kNT = 256;
 constexpr int kBlock = 32;  // columns per exponent byte
+constexpr int kDeep = 4;    // chunks of a lane, loaded together
+typedef u32x2 u32x2_byte __attribute__((aligned(1)));
+typedef uint32_t u32_byte __attribute__((aligned(1)));
 
-__device__ __forceinline__ float restore(int q, int b) {
-    return b == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf((float)q, b - 133);
-}
+// Where a lane's chunks lie: 2^lshift lanes take kDeep chunks each of a row, and
+// blockIdx.y the row's next 2^lshift * kDeep.
+struct Tile {
+    size_t row;
+    int first, step;
+    bool in;
+    __device__ __forceinline__ Tile(int R, int lshift) {
+        const int64_t r = ((int64_t)blockIdx.x << (8 - lshift)) + (threadIdx.x >> lshift);
+        in = r < R;
+        row = in ? (size_t)r : 0;
+        step = 1 << lshift;
+        first = (blockIdx.y << lshift) * kDeep + (threadIdx.x & (step - 1));
+    }
+};
 
-// 32 lanes per block of columns; blockIdx.x walks (row, block) pairs.
-__global__ __launch_bounds__(kNT) void ckpt8_save_k(int dt, const void *x, int ldx, uint64_t pairs,
-                                                    int nb, int C, int8_t *q, int ldq, uint8_t *e,
-                                                    int lde) {
-    const int lane = threadIdx.x & 31;
-    for (uint64_t p = (uint64_t)blockIdx.x * (kNT / 32) + (threadIdx.x >> 5); p < pairs;
-         p += (uint64_t)gridDim.x * (kNT / 32)) {
-        const uint64_t r = p / nb;
-        const int blk = (int)(p % nb), c = blk * kBlock + lane;
-        const float v = c < C ? fg::load_as_f(x, dt, r * ldx + c) : 0.0f;
-        uint32_t m = __float_as_uint(v) & 0x7fffffffu;
+// E signed bytes in one access; the bytes of the row's last, partial chunk in turn.
+template <int E>
+struct Bytes {
+    uint32_t w[E / 4];
+    __device__ __forceinline__ void load(const int8_t *row, int j, int nb, int C) {
+        const int8_t *p = row + (size_t)j * E;
+        if (j < nb) {
+            if constexpr (E == 8) {
+                const u32x2 v = *reinterpret_cast<const u32x2_byte *>(p);
+                w[0] = v[0];
+                w[1] = v[1];
+            } else {
+                w[0] = *reinterpret_cast<const u32_byte *>(p);
+            }
+            return;
+        }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+        for (int k = 0; k < E / 4; ++k) w[k] = 0;
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+            if (j * E + k < C) w[k / 4] |= (uint32_t)(uint8_t)p[k] << (8 * (k & 3));
+    }
+    __device__ __forceinline__ void store(int8_t *row, int j, int nb, int C) const {
+        int8_t *p = row + (size_t)j * E;
+        if (j < nb) {
+            if constexpr (E == 8) *reinterpret_cast<u32x2_byte *>(p) = u32x2{w[0], w[1]};
+            else *reinterpret_cast<u32_byte *>(p) = w[0];
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < E; ++k)
+            if (j * E + k < C) p[k] = (int8_t)(w[k / 4] >> (8 * (k & 3)));
+    }
+    __device__ __forceinline__ int get(int k) const {
+        return (int)(int8_t)(w[k / 4] >> (8 * (k & 3)));
+    }
+};
+
+template <int DT>
+__global__ __launch_bounds__(kNT) void ckpt8_save_k(const typename Io<DT>::T *__restrict__ x,
+                                                    int ldx, int R, int C, int8_t *__restrict__ q,
+                                                    int ldq, uint8_t *__restrict__ e, int lde,
+                                                    int lshift) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E, kLanes = kBlock / E;  // lanes of a block
+    const Tile t(R, lshift);
+    if (!t.in) return;
+    const auto *xr = x + t.row * ldx;
+    const int nb = C / E, chunks = ((C - 1) / kBlock + 1) * kLanes;  // whole blocks of lanes
+    u32x4 w[kDeep];
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+        const int j = t.first + u * t.step;
+        if (j < chunks) w[u] = Chunk<DT>::load(xr, j, nb, C);
+    }
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+        const int j = t.first + u * t.step;
+        if (j >= chunks) break;
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < E; ++k) m = max(m, __float_as_uint(IO::get(w[u], k)) & 0x7fffffffu);
+        // The block's other lanes (all here: chunks come in whole blocks).
+        m = max(m, (uint32_t)fg::smrow::dpp_i<fg::smrow::kDppSwap1>((int)m));
+        m = max(m, (uint32_t)fg::smrow::dpp_i<fg::smrow::kDppSwap2>((int)m));
+        if constexpr (kLanes == 8)
+            m = max(m, (uint32_t)fg::smrow::dpp_i<fg::smrow::kDppHalfMirror>((int)m));
         const int b = max(1, (int)(m >> 23));
-        const float s = __builtin_rintf(__builtin_amdgcn_ldexpf(v, 133 - b));
-        if (c < C)
-            q[r * ldq + c] = b == 255 ? (int8_t)0 : (int8_t)fminf(fmaxf(s, -127.0f), 127.0f);
-        if (lane == 0) e[r * lde + blk] = (uint8_t)b;
+        Bytes<E> o;
+#pragma unroll
+        for (int k = 0; k < E; k += 4) {
+            uint32_t p = 0;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float s =
+                    __builtin_rintf(__builtin_amdgcn_ldexpf(IO::get(w[u], k + n), 133 - b));
+                const int c = (int)__builtin_amdgcn_fmed3f(s, -127.0f, 127.0f);
+                p |= ((uint32_t)c & 255u) << (8 * n);
+            }
+            o.w[k / 4] = b == 255 ? 0u : p;
+        }
+        o.store(q + t.row * ldq, j, nb, C);
+        if (j % kLanes == 0) e[t.row * lde + j / kLanes] = (uint8_t)b;
     }
 }
 
-// What: 0 restores z and / or h = act(z), 1 writes dz = dh * act'(z) to z.
-template <int WHAT>
-__global__ __launch_bounds__(kNT) void ckpt8_load_k(int dt, int act, const int8_t *q, int ldq,
-                                                    const uint8_t *e, int lde, uint64_t n, int C,
-                                                    void *z, int ldz, void *h, int ldh) {
-    for (uint64_t i = (uint64_t)blockIdx.x * kNT + threadIdx.x; i < n;
-         i += (uint64_t)gridDim.x * kNT) {
-        const uint64_t r = i / C;
-        const int c = (int)(i % C);
-        const float v = restore(q[r * ldq + c], e[r * lde + c / kBlock]);
-        if constexpr (WHAT == 0) {
-            if (z) fg::store_from_f(z, dt, r * ldz + c, v);
-            if (h) fg::store_from_f(h, dt, r * ldh + c, fg::act_fwd(act, v));
-        } else {
-            const float d = fg::load_as_f(h, dt, r * ldh + c);
-            fg::store_from_f(z, dt, r * ldz + c, d * fg::act_grad(act, v));
+// Restored values: bytes and exponents of a lane's chunks, loaded together.
+template <int E>
+struct Kept {
+    static constexpr int kLanes = kBlock / E;
+    Bytes<E> q[kDeep];
+    int b[kDeep];
+    __device__ __forceinline__ Kept(const Tile &t, const int8_t *qr, const uint8_t *er, int nb,
+                                    int chunks, int C) {
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+            const int j = t.first + u * t.step;
+            if (j >= chunks) continue;
+            q[u].load(qr, j, nb, C);
+            b[u] = er[j / kLanes];
+        }
+    }
+    __device__ __forceinline__ void values(int u, float (&v)[E]) const {
+        // 2^(b - 133), exact (down to 2^-132; fp32 denormals are on).
+        const float s =
+            b[u] == 255 ? __builtin_nanf("") : __builtin_amdgcn_ldexpf(1.0f, b[u] - 133);
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[k] = (float)q[u].get(k) * s;
+    }
+};
+
+template <int DT, int ACT>
+__global__ __launch_bounds__(kNT) void ckpt8_load_k(const int8_t *__restrict__ q, int ldq,
+                                                    const uint8_t *__restrict__ e, int lde, int R,
+                                                    int C, typename Io<DT>::T *z, int ldz,
+                                                    typename Io<DT>::T *h, int ldh, int lshift) {
+    constexpr int E = Io<DT>::E;
+    const Tile t(R, lshift);
+    if (!t.in) return;
+    const int nb = C / E, chunks = (C - 1) / E + 1;
+    const Kept<E> kept(t, q + t.row * ldq, e + t.row * lde, nb, chunks, C);
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+        const int j = t.first + u * t.step;
+        if (j >= chunks) break;
+        float v[E];
+        kept.values(u, v);
+        if (z) Chunk<DT>::store(z + t.row * ldz, j, nb, C, v);
+        if (h) {
+#pragma unroll
+            for (int k = 0; k < E; ++k) v[k] = fg::act_fwd(ACT, v[k]);
+            Chunk<DT>::store(h + t.row * ldh, j, nb, C, v);
         }
     }
 }
 
-unsigned grid_of(uint64_t work) {
-    return (unsigned)std::min<uint64_t>((work + kNT - 1) / kNT, 1u << 20);
+template <int DT, int ACT>
+__global__ __launch_bounds__(kNT) void act_bwd_ckpt8_k(const typename Io<DT>::T *dh, int lddh,
+                                                       const int8_t *__restrict__ q, int ldq,
+                                                       const uint8_t *__restrict__ e, int lde,
+                                                       int R, int C, typename Io<DT>::T *dz,
+                                                       int lddz, int lshift) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E;
+    const Tile t(R, lshift);
+    if (!t.in) return;
+    const int nb = C / E, chunks = (C - 1) / E + 1;
+    u32x4 w[kDeep];
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+        const int j = t.first + u * t.step;
+        if (j < chunks) w[u] = Chunk<DT>::load(dh + t.row * lddh, j, nb, C);
+    }
+    const Kept<E> kept(t, q + t.row * ldq, e + t.row * lde, nb, chunks, C);
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+        const int j = t.first + u * t.step;
+        if (j >= chunks) break;
+        float v[E];
+        kept.values(u, v);
+#pragma unroll
+        for (int k = 0; k < E; ++k) v[k] = IO::get(w[u], k) * fg::act_grad(ACT, v[k]);
+        Chunk<DT>::store(dz + t.row * lddz, j, nb, C, v);
+    }
+}
+
+struct Shape {
+    dim3 grid;
+    int lshift;
+};
+Shape shape_of(int dtype, int R, int C) {
+    Shape s;
+    const int E = dtype == FG_DTYPE_F32 ? 4 : 8;
+    const int chunks = ((C - 1) / kBlock + 1) * (kBlock / E);  // whole blocks
+    s.lshift = 3;  // (at least a block's lanes)
+    while (s.lshift < 8 && (kDeep << s.lshift) < chunks) ++s.lshift;
+    const int rows = kNT >> s.lshift;
+    s.grid = dim3((R - 1) / rows + 1, (chunks - 1) / (kDeep << s.lshift) + 1);
+    return s;
+}
+
+// f<DT, ACT>() for run-time codes.
+template <class F>
+void with_types(int dtype, int act, F f) {
+    using std::integral_constant;
+    auto with_act = [&](auto dt) {
+        if (act == FG_ACT_RELU) f(dt, integral_constant<int, fg::kActRelu>{});
+        else if (act == FG_ACT_GELU) f(dt, integral_constant<int, fg::kActGelu>{});
+        else f(dt, integral_constant<int, fg::kActNone>{});
+    };
+    if (dtype == FG_DTYPE_F32) with_act(integral_constant<int, fg::kF32>{});
+    else if (dtype == FG_DTYPE_BF16) with_act(integral_constant<int, fg::kBF16>{});
+    else with_act(integral_constant<int, fg::kF16>{});
 }
 
 int check_q(const char *who, int dtype, int R, int C, const void *q, int ldq, const void *e,
@@ -98,10 +275,13 @@ FG_API int fg_ckpt8_save(fg_ctx *ctx, int dtype, const void *d_x, int ldx, int R
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
-    const int nb = (C - 1) / kBlock + 1;
-    const uint64_t pairs = (uint64_t)R * nb;
-    ckpt8_save_k<<<grid_of(pairs * 32), kNT, 0, ctx->stream>>>(dtype, d_x, ldx, pairs, nb, C, d_q,
-                                                               ldq, d_e, lde);
+    const Shape s = shape_of(dtype, R, C);
+    auto launch = [&](auto dt) {
+        using T = typename Io<dt()>::T;
+        ckpt8_save_k<dt()><<<s.grid, kNT, 0, ctx->stream>>>(static_cast<const T *>(d_x), ldx, R, C,
+                                                            d_q, ldq, d_e, lde, s.lshift);
+    };
+    with_types(dtype, FG_ACT_NONE, [&](auto dt, auto) { launch(dt); });
     FG_LAUNCH_CHECK("ckpt8_save");
     return FG_OK;
 }
@@ -119,9 +299,13 @@ FG_API int fg_ckpt8_load(fg_ctx *ctx, int dtype, int act, const int8_t *d_q, int
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
-    const uint64_t n = (uint64_t)R * C;
-    ckpt8_load_k<0><<<grid_of(n), kNT, 0, ctx->stream>>>(dtype, act, d_q, ldq, d_e, lde, n, C, d_z,
-                                                         ldz, d_h, ldh);
+    const Shape s = shape_of(dtype, R, C);
+    with_types(dtype, act, [&](auto dt, auto a) {
+        using T = typename Io<dt()>::T;
+        ckpt8_load_k<dt(), a()><<<s.grid, kNT, 0, ctx->stream>>>(
+            d_q, ldq, d_e, lde, R, C, static_cast<T *>(d_z), ldz, static_cast<T *>(d_h), ldh,
+            s.lshift);
+    });
     FG_LAUNCH_CHECK("ckpt8_load");
     return FG_OK;
 }
@@ -139,9 +323,13 @@ FG_API int fg_act_bwd_ckpt8(fg_ctx *ctx, int dtype, int act, const void *d_dH, i
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
-    const uint64_t n = (uint64_t)R * C;
-    ckpt8_load_k<1><<<grid_of(n), kNT, 0, ctx->stream>>>(dtype, act, d_q, ldq, d_e, lde, n, C, d_dZ,
-                                                         lddz, const_cast<void *>(d_dH), lddh);
+    const Shape s = shape_of(dtype, R, C);
+    with_types(dtype, act, [&](auto dt, auto a) {
+        using T = typename Io<dt()>::T;
+        act_bwd_ckpt8_k<dt(), a()><<<s.grid, kNT, 0, ctx->stream>>>(
+            static_cast<const T *>(d_dH), lddh, d_q, ldq, d_e, lde, R, C, static_cast<T *>(d_dZ),
+            lddz, s.lshift);
+    });
     FG_LAUNCH_CHECK("act_bwd_ckpt8");
     return FG_OK;
 }
@@ -160,19 +348,21 @@ FG_API int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int 
                "%s: a leading dimension is below its row length", who);
     FG_REQUIRE(d_W && d_dZ && d_dX && d_dW, FG_ERR_INVALID_ARGUMENT, "%s: NULL operand or output",
                who);
-    FG_REQUIRE(d_Xr && (act == FG_ACT_NONE || d_Zr), FG_ERR_INVALID_ARGUMENT,
-               "%s: Xr, and with an activation Zr, is required", who);
+    FG_REQUIRE(d_Xr && (act != FG_ACT_GELU || d_Zr), FG_ERR_INVALID_ARGUMENT,
+               "%s: Xr, and for GELU Zr, is required", who);
     FG_REQUIRE(d_Xr != d_Zr && d_Xr != d_dX, FG_ERR_INVALID_ARGUMENT,
                "%s: Xr must not be Zr or dX", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
-    void *zr = act == FG_ACT_NONE ? nullptr : d_Zr;
+    // [act(z) > 0] == [z > 0] for ReLU, whose derivative then reads Xr.
+    void *zr = act == FG_ACT_GELU ? d_Zr : nullptr;
     if (int rc = fg_ckpt8_load(ctx, dtype, act, d_q, ldq, d_e, lde, M, K, zr, K, d_Xr, K))
         return rc;
+    const void *zs = act == FG_ACT_RELU ? d_Xr : zr;
     if (dtype == FG_DTYPE_F32)
         return fg_matmul_bwd_f32(ctx, M, N, K, (const float *)d_Xr, K, (const float *)d_W, ldw,
-                                 (const float *)d_dZ, lddz, act, (const float *)zr, K,
+                                 (const float *)d_dZ, lddz, act, (const float *)zs, K,
                                  (float *)d_dX, lddx, (float *)d_dW, lddw, (float *)d_dbias,
                                  accumulate);
-    return fg_matmul_bwd_x16(ctx, dtype, M, N, K, d_Xr, K, d_W, ldw, d_dZ, lddz, act, zr, K, d_dX,
+    return fg_matmul_bwd_x16(ctx, dtype, M, N, K, d_Xr, K, d_W, ldw, d_dZ, lddz, act, zs, K, d_dX,
                              lddx, d_dW, lddw, d_dbias, accumulate);
 }

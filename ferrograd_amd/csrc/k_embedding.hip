@@ -31,6 +31,7 @@
 
 namespace {
 
+using fg::rows::Chunk;
 using fg::rows::Io;
 using fg::rows::u32x4;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -42,31 +43,6 @@ constexpr int kRankMax = 16384;
 #define UB 1024
 #endif
 constexpr int kUnitBlocks = UB;
-
-// A row's chunk j where j is below its whole chunks nb, or (j == nb) its last,
-// partial one, one element after the other.
-template <int DT>
-struct Chunk {
-    using IO = Io<DT>;
-    static constexpr int E = IO::E;
-    static __device__ __forceinline__ u32x4 load(const typename IO::T *row, int j, int nb, int C) {
-        if (j < nb) return fg::rows::load<DT>(row, j);
-        float v[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = j * E + e < C ? IO::load1(row, j * E + e) : 0.0f;
-        return IO::pack(v);
-    }
-    static __device__ __forceinline__ void store(typename IO::T *row, int j, int nb, int C,
-                                                 const float (&v)[E]) {
-        if (j < nb) {
-            fg::rows::store<DT>(row, j, IO::pack(v));
-            return;
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (j * E + e < C) IO::store1(row, j * E + e, v[e]);
-    }
-};
 
 // ------------------------------------------------------------------- lookup
 // 2^lshift lanes take a row, UNR chunks in flight a lane.

@@ -367,8 +367,9 @@ int fg_act_bwd_ckpt8(fg_ctx *ctx, int dtype, int act, const void *d_dH, int lddh
  * pre-activation of X's producer, kept in 8 bits:
  *   dW (=|+=) act(z)^T.dZ [K][N], dbias (=|+=) colsum(dZ) (or NULL)
  *   dX (=|+=) (dZ.W^T) * act'(z) [M][K]
- * d_Xr and (with an activation) d_Zr are the caller's scratch, M x K elements
- * of dtype each, overwritten with act(z) and z as the products read them. */
+ * d_Xr and (for GELU; else it may be NULL) d_Zr are the caller's scratch, M x K
+ * elements of dtype each, overwritten with act(z) and z as the products read
+ * them: act(z) is rounded to dtype, as the forward's stored activation is. */
 int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int act,
                         const int8_t *d_q, int ldq, const uint8_t *d_e, int lde,
                         const void *d_W, int ldw, const void *d_dZ, int lddz, void *d_Zr,
