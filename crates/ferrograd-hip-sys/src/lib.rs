@@ -106,6 +106,7 @@ pub const FG_ACT_GELU: c_int = 2;
 pub const FG_DTYPE_F32: c_int = 0;
 pub const FG_DTYPE_F16: c_int = 1;
 pub const FG_DTYPE_BF16: c_int = 2;
+pub const FG_DTYPE_U32: c_int = 3;
 // fg_bpat_header (BpatHeader declaration order)
 pub const FG_BPAT_V0: c_int = 0;
 pub const FG_BPAT_V1: c_int = 1;
@@ -142,6 +143,8 @@ pub const FG_OP_ABS: c_int = 13;
 pub const FG_OP_NEG: c_int = 14;
 pub const FG_OP_SOFTMAX: c_int = 15;
 pub const FG_OP_BIAS_ADD: c_int = 16;
+pub const FG_OP_LAYER_NORM: c_int = 17;
+pub const FG_OP_EMBEDDING: c_int = 18;
 // input flags
 pub const FG_INPUT_NO_GRAD: u32 = 0x1;
 pub const FG_INPUT_FROZEN: u32 = 0x2;
@@ -728,6 +731,22 @@ extern "C" {
         n_inputs: c_int,
         node: *mut u32,
     ) -> c_int;
+    pub fn fg_graph_layer_norm(
+        g: *mut fg_graph,
+        x: u32,
+        gamma: u32,
+        beta: u32,
+        eps: f32,
+        node: *mut u32,
+    ) -> c_int;
+    pub fn fg_graph_embedding(
+        g: *mut fg_graph,
+        table: u32,
+        tokens: u32,
+        scale: f32,
+        node: *mut u32,
+    ) -> c_int;
+    pub fn fg_graph_set_ckpt8(g: *mut fg_graph, node: u32, on: c_int) -> c_int;
     pub fn fg_graph_set_input_flags(g: *mut fg_graph, node: u32, flags: u32) -> c_int;
     pub fn fg_graph_num_nodes(g: *const fg_graph, n: *mut u32) -> c_int;
     pub fn fg_graph_validate(g: *const fg_graph, meta: *const u32, n_meta: c_int) -> c_int;

@@ -254,6 +254,25 @@ impl Graph {
         Ok(id)
     }
 
+    /// Layer norm of `x[..., N]` over its last dimension with `gamma[N]`, `beta[N]`.
+    pub fn layer_norm(&mut self, x: u32, gamma: u32, beta: u32, eps: f32) -> Result<u32, Error> {
+        let mut id = 0u32;
+        check(unsafe { sys::fg_graph_layer_norm(self.raw, x, gamma, beta, eps, &mut id) })?;
+        Ok(id)
+    }
+
+    /// `scale * table[tokens]`, `tokens` an input of type `FG_DTYPE_U32`.
+    pub fn embedding(&mut self, table: u32, tokens: u32, scale: f32) -> Result<u32, Error> {
+        let mut id = 0u32;
+        check(unsafe { sys::fg_graph_embedding(self.raw, table, tokens, scale, &mut id) })?;
+        Ok(id)
+    }
+
+    /// Keep what the backward needs of a relu / gelu node in 8 bits.
+    pub fn set_ckpt8(&mut self, node: u32, on: bool) -> Result<(), Error> {
+        check(unsafe { sys::fg_graph_set_ckpt8(self.raw, node, on as c_int) })
+    }
+
     pub fn set_input_flags(&mut self, node: u32, flags: u32) -> Result<(), Error> {
         check(unsafe { sys::fg_graph_set_input_flags(self.raw, node, flags) })
     }

@@ -111,6 +111,9 @@ SIGNATURES = {
     "fg_graph_input": (i32, [vp, vp, i32, ctypes.POINTER(u32)]),
     "fg_graph_constant_f32": (i32, [vp, f32, ctypes.POINTER(u32)]),
     "fg_graph_op": (i32, [vp, i32, vp, i32, ctypes.POINTER(u32)]),
+    "fg_graph_layer_norm": (i32, [vp, u32, u32, u32, f32, ctypes.POINTER(u32)]),
+    "fg_graph_embedding": (i32, [vp, u32, u32, f32, ctypes.POINTER(u32)]),
+    "fg_graph_set_ckpt8": (i32, [vp, u32, i32]),
     "fg_graph_set_input_flags": (i32, [vp, u32, u32]),
     "fg_graph_num_nodes": (i32, [vp, ctypes.POINTER(u32)]),
     "fg_graph_validate": (i32, [vp, vp, i32]),

@@ -20,6 +20,9 @@
 //     every node value;
 //   * softmax followed by the CE loss becomes ONE fused softmax+CE launch
 //     writing dlogits = p - onehot directly;
+//   * layer norm and embedding nodes become their own launches; an activation
+//     marked by fg_graph_set_ckpt8 keeps its pre-activation in 8 bits, its GEMM
+//     writing Z and the activation into memory that such layers share;
 //   * backward is planned statically in reverse node order; the activation
 //     derivative of a layer is fused into the epilogue of the dA GEMM of the
 //     layer above (dZ_prev = (dZ W^T) * act'(Z_prev)), bias gradients are
@@ -63,14 +66,15 @@ bool is_elementwise(int op) { return is_unary(op) || is_binary_elt(op); }
 int arity(int op) {
     if (op == FG_OP_INPUT || op == FG_OP_CONST) return 0;
     if (is_unary(op) || op == FG_OP_SOFTMAX) return 1;
-    return 2;
+    return op == FG_OP_LAYER_NORM ? 3 : 2;
 }
 
 const char *op_name(int op) {
     static const char *names[] = {"input", "const", "add",  "sub", "mul",  "div",
                                   "matmul", "relu", "gelu", "elu", "tanh", "exp",
-                                  "log",   "abs",   "neg",  "softmax", "bias_add"};
-    return (op >= 0 && op <= FG_OP_BIAS_ADD) ? names[op] : "?";
+                                  "log",   "abs",   "neg",  "softmax", "bias_add",
+                                  "layer_norm", "embedding"};
+    return (op >= 0 && op <= FG_OP_EMBEDDING) ? names[op] : "?";
 }
 
 // SaveIndicator flags (kernel/mod.rs:41-93).
@@ -80,14 +84,19 @@ struct GNode {
     int op = FG_OP_INPUT;
     std::vector<uint32_t> in;
     std::vector<uint32_t> fields;  // Input: meta field per dim
-    float value = 0.0f;            // Const (already rounded to dtype)
+    float value = 0.0f;            // Const (already rounded to dtype); layer norm: eps;
+                                   // embedding: scale
     uint32_t flags = 0;            // Input flags
+    bool ckpt8 = false;            // pre-activation kept in 8 bits (fg_graph_set_ckpt8)
     int dtype = FG_DTYPE_F32;      // Input / Const: declared; operations: of their first input
 };
 
-int esize(int dt) { return dt == FG_DTYPE_F32 ? 4 : 2; }
+int esize(int dt) { return dt == FG_DTYPE_F32 || dt == FG_DTYPE_U32 ? 4 : 2; }
 const char *dtype_name(int dt) {
-    return dt == FG_DTYPE_F16 ? "f16" : dt == FG_DTYPE_BF16 ? "bf16" : "f32";
+    return dt == FG_DTYPE_F16    ? "f16"
+           : dt == FG_DTYPE_BF16 ? "bf16"
+           : dt == FG_DTYPE_U32  ? "u32"
+                                 : "f32";
 }
 
 // Host rounding of an fp32 value to a 16-bit type and back (graph constants
@@ -141,6 +150,13 @@ int infer_shapes(const fg_graph &g, const uint32_t *meta, int n_meta, std::vecto
     for (size_t i = 0; i < n; ++i) {
         const GNode &nd = g.nodes[i];
         Shape s;
+        for (size_t k = 0; k < nd.in.size(); ++k) {
+            const GNode &x = g.nodes[nd.in[k]];
+            const bool tokens = x.op == FG_OP_INPUT && x.dtype == FG_DTYPE_U32;
+            FG_REQUIRE(tokens == (nd.op == FG_OP_EMBEDDING && k == 1), FG_ERR_UNSUPPORTED,
+                       "%s %zu: u32 inputs are the tokens of embeddings and nothing else",
+                       op_name(nd.op), i);
+        }
         switch (nd.op) {
             case FG_OP_INPUT: {
                 FG_REQUIRE(!nd.fields.empty(), FG_ERR_GRAPH, "input %zu has rank 0", i);
@@ -175,6 +191,24 @@ int infer_shapes(const fg_graph &g, const uint32_t *meta, int n_meta, std::vecto
                 const Shape &a = sh[nd.in[0]];
                 FG_REQUIRE(!a.scalar, FG_ERR_SHAPE, "softmax %zu of a scalar", i);
                 s = a;
+                break;
+            }
+            case FG_OP_LAYER_NORM: {
+                const Shape &a = sh[nd.in[0]], &ga = sh[nd.in[1]], &be = sh[nd.in[2]];
+                FG_REQUIRE(!a.scalar && ga.vector && be.vector && ga.cols == a.cols &&
+                               be.cols == a.cols,
+                           FG_ERR_SHAPE, "layer_norm %zu: needs x[..., N], gamma[N], beta[N]", i);
+                s = a;
+                break;
+            }
+            case FG_OP_EMBEDDING: {
+                const Shape &a = sh[nd.in[0]], &t = sh[nd.in[1]];
+                FG_REQUIRE(!a.scalar && !a.vector, FG_ERR_SHAPE,
+                           "embedding %zu: the table must be a matrix", i);
+                s.rows = t.numel();
+                s.cols = a.cols;
+                FG_REQUIRE(s.rows <= INT32_MAX && a.rows <= INT32_MAX, FG_ERR_SHAPE,
+                           "embedding %zu: more than 2^31 - 1 tokens or table rows", i);
                 break;
             }
             default: {
@@ -227,6 +261,12 @@ enum LaunchKind {
     LK_ELT,
     LK_SMCE,
     LK_FILL0,
+    LK_LN,
+    LK_LN_BWD,
+    LK_EMB,
+    LK_EMB_BWD,
+    LK_CKPT_SAVE,
+    LK_CKPT_LOAD,
 };
 
 struct Launch {
@@ -236,6 +276,13 @@ struct Launch {
     int act = FG_ACT_NONE, accumulate = 0;
     int accumulate2 = 0;  // TN GEMM with fused bias gradient: accumulate into sExtra
     int sA = kNone, sB = kNone, sC = kNone, sZ = kNone, sBias = kNone, sExtra = kNone;
+    // Layer norm: sA x, sB dy, sC y / dx, sZ gamma, sBias beta, sMean / sRstd the
+    // statistics, sG / sH dgamma / dbeta (accumulate2 / accumulate3).  Embedding: sA
+    // the table (forward), sB tokens, sZ dout, sC out / dtable; K the table's rows.
+    // Checkpoints: sA the pre-activation, sB the bytes, sZ the exponents, sC the
+    // activation.
+    int sMean = kNone, sRstd = kNone, sG = kNone, sH = kNone, accumulate3 = 0;
+    float value = 0.0f;  // eps, scale
     fg::EltProgram prog{};
     int src_slot[fg::kEltMaxSrc];
     int dst_slot[fg::kEltMaxDst];
@@ -269,6 +316,7 @@ struct Slot {
     bool external = false;
     void *ext = nullptr;
     int dtype = FG_DTYPE_F32;  // element type (u32 labels count as 4-byte elements)
+    int base = kNone;          // the slot whose memory this one shares
 };
 
 struct Group {
@@ -288,6 +336,10 @@ struct fg_plan {
     std::vector<uint32_t> save;
     std::vector<char> needs_grad;
     std::vector<int> val_slot, grad_slot, group_of;
+    std::vector<int> mean_of, rstd_of;  // layer norm statistics, per node
+    // Activations whose pre-activation is kept in 8 bits: its bytes and exponents,
+    // and the shared memory that a backward restores z and act(z) into.
+    std::vector<int> ck_q, ck_e, ck_z, ck_h;
     std::vector<Group> groups;
     std::vector<Slot> slots;
     char *arena = nullptr;
@@ -331,6 +383,7 @@ struct fg_plan {
     void *ptr(int slot) const {
         if (slot == kNone) return nullptr;
         const Slot &s = slots[slot];
+        if (s.base != kNone) return (void *)(arena + slots[s.base].offset);
         return s.external ? s.ext : (void *)(arena + s.offset);
     }
     // Slot of `elems` elements of type dt (bytes rounded up to whole words
@@ -350,6 +403,13 @@ struct fg_plan {
         s.external = true;
         slots.push_back(s);
         return (int)slots.size() - 1;
+    }
+    // A slot in the memory of `base` (which grows to hold it).
+    int new_shared(int base, uint64_t elems, int dt) {
+        const int s = new_slot(elems, dt);
+        slots[s].base = base;
+        slots[base].bytes = std::max(slots[base].bytes, slots[s].bytes);
+        return s;
     }
     int sdt(int slot) const { return slot == kNone ? FG_DTYPE_F32 : slots[slot].dtype; }
     int vslot(uint32_t n) const { return val_slot[n]; }
@@ -400,6 +460,12 @@ void compute_saved(const fg_graph &g, const std::vector<std::vector<uint32_t>> &
                 }
                 for (uint32_t u : users[i]) save[u] |= kDefBwd;
                 break;
+            case FG_OP_LAYER_NORM:
+                save[i] |= kDefFwd | kDefBwd;
+                for (uint32_t x : nd.in)
+                    if (nonleaf(x)) save[x] |= kDefFwd;
+                break;
+            case FG_OP_EMBEDDING: save[i] |= kDefFwd | kDefBwd; break;
             case FG_OP_MUL:
             case FG_OP_DIV:
                 for (uint32_t x : nd.in)
@@ -569,6 +635,55 @@ int lower_forward(fg_plan &P) {
                      (L.sBias != kNone ? " +bias" : "") +
                      (L.act == FG_ACT_RELU ? " +relu" : L.act == FG_ACT_GELU ? " +gelu" : "") +
                      " -> node " + std::to_string(G.fin);
+            P.fwd.push_back(L);
+            if (P.ck_q[n] != kNone) {
+                Launch S;
+                S.kind = LK_CKPT_SAVE;
+                S.dtype = L.dtype;
+                S.M = L.M;
+                S.N = L.N;
+                S.sA = L.sZ;
+                S.sB = P.ck_q[n];
+                S.sZ = P.ck_e[n];
+                S.desc = "forward ckpt8 save " + std::to_string(L.M) + "x" + std::to_string(L.N) +
+                         " of node " + std::to_string(G.pre);
+                P.fwd.push_back(S);
+            }
+            continue;
+        }
+        if (nd.op == FG_OP_LAYER_NORM) {
+            eb.flush(P.fwd, "forward");
+            Launch L;
+            L.kind = LK_LN;
+            L.dtype = P.dtype[n];
+            L.M = (int)P.shape[n].rows;
+            L.N = (int)P.shape[n].cols;
+            L.sA = P.vslot(nd.in[0]);
+            L.sZ = P.vslot(nd.in[1]);
+            L.sBias = P.vslot(nd.in[2]);
+            L.sC = P.vslot(n);
+            L.sMean = P.mean_of[n];
+            L.sRstd = P.rstd_of[n];
+            L.value = nd.value;
+            L.desc = "forward layer_norm " + std::to_string(L.M) + "x" + std::to_string(L.N) +
+                     dt_suffix(L.dtype) + " -> node " + std::to_string(n);
+            P.fwd.push_back(L);
+            continue;
+        }
+        if (nd.op == FG_OP_EMBEDDING) {
+            eb.flush(P.fwd, "forward");
+            Launch L;
+            L.kind = LK_EMB;
+            L.dtype = P.dtype[n];
+            L.M = (int)P.shape[n].rows;
+            L.N = (int)P.shape[n].cols;
+            L.K = (int)P.shape[nd.in[0]].rows;
+            L.sA = P.vslot(nd.in[0]);
+            L.sB = P.vslot(nd.in[1]);
+            L.sC = P.vslot(n);
+            L.value = nd.value;
+            L.desc = "forward embedding " + dims_str(L.M, L.N, L.K) + dt_suffix(L.dtype) +
+                     " -> node " + std::to_string(n);
             P.fwd.push_back(L);
             continue;
         }
@@ -922,6 +1037,25 @@ int lower_backward(fg_plan &P, bool fused, std::vector<Launch> &out) {
                 ginit[G.bias_src] = 1;
                 out.push_back(L);
             }
+            // An A operand kept in 8 bits: restored for the two products.
+            const bool kept = P.ck_q[a] != kNone;
+            if (kept) {
+                const bool relu = g.nodes[a].op == FG_OP_RELU;
+                Launch L;
+                L.kind = LK_CKPT_LOAD;
+                L.dtype = P.dtype[a];
+                L.M = M;
+                L.N = K;
+                L.act = relu ? FG_ACT_RELU : FG_ACT_GELU;
+                L.sB = P.ck_q[a];
+                L.sZ = P.ck_e[a];
+                // (ReLU's derivative reads the activation.)
+                if (P.needs_grad[a] && !relu) L.sA = P.ck_z[a];
+                if (P.needs_grad[b] || relu) L.sC = P.ck_h[a];
+                L.desc = "backward ckpt8 load " + std::to_string(M) + "x" + std::to_string(K) +
+                         (relu ? " +relu" : " +gelu") + " for node " + std::to_string(a);
+                if (L.sA != kNone || L.sC != kNone) out.push_back(L);
+            }
             int idx_db = kNone;
             if (P.needs_grad[b]) {  // dB = A^T dZ
                 idx_db = (int)out.size();
@@ -932,7 +1066,7 @@ int lower_backward(fg_plan &P, bool fused, std::vector<Launch> &out) {
                 L.M = K;
                 L.N = N;
                 L.K = M;
-                L.sA = P.vslot(a);
+                L.sA = kept ? P.ck_h[a] : P.vslot(a);
                 L.lda = K;
                 L.sB = gs(pre);
                 L.ldb = N;
@@ -969,7 +1103,7 @@ int lower_backward(fg_plan &P, bool fused, std::vector<Launch> &out) {
                 if (fuse) {
                     const Group &G2 = P.groups[ga];
                     L.act = g.nodes[a].op == FG_OP_RELU ? FG_ACT_RELU : FG_ACT_GELU;
-                    L.sZ = P.vslot(G2.pre);
+                    L.sZ = !kept ? P.vslot(G2.pre) : L.act == FG_ACT_RELU ? P.ck_h[a] : P.ck_z[a];
                     L.ldz = K;
                     L.sC = gs(G2.pre);
                     L.accumulate = ginit[G2.pre];
@@ -994,6 +1128,53 @@ int lower_backward(fg_plan &P, bool fused, std::vector<Launch> &out) {
             continue;
         }
         if (!ginit[n]) continue;  // no gradient reaches this node
+        if (nd.op == FG_OP_LAYER_NORM) {
+            const uint32_t x = nd.in[0], ga = nd.in[1], be = nd.in[2];
+            Launch L;
+            L.kind = LK_LN_BWD;
+            L.dtype = P.dtype[n];
+            L.M = (int)P.shape[n].rows;
+            L.N = (int)P.shape[n].cols;
+            L.sA = P.vslot(x);
+            L.sB = gs(n);
+            L.sZ = P.vslot(ga);
+            L.sMean = P.mean_of[n];
+            L.sRstd = P.rstd_of[n];
+            L.desc = "backward layer_norm " + std::to_string(L.M) + "x" + std::to_string(L.N) +
+                     " -> grad of node";
+            auto to = [&](uint32_t t, int &slot, int &acc) {
+                if (!P.needs_grad[t]) return;
+                slot = gs(t);
+                acc = ginit[t];
+                ginit[t] = 1;
+                L.desc += " " + std::to_string(t);
+            };
+            to(x, L.sC, L.accumulate);
+            to(ga, L.sG, L.accumulate2);
+            to(be, L.sH, L.accumulate3);
+            out.push_back(L);
+            continue;
+        }
+        if (nd.op == FG_OP_EMBEDDING) {
+            const uint32_t x = nd.in[0];
+            if (!P.needs_grad[x]) continue;
+            Launch L;
+            L.kind = LK_EMB_BWD;
+            L.dtype = P.dtype[n];
+            L.M = (int)P.shape[n].rows;
+            L.N = (int)P.shape[n].cols;
+            L.K = (int)P.shape[x].rows;
+            L.sB = P.vslot(nd.in[1]);
+            L.sZ = gs(n);
+            L.sC = gs(x);
+            L.accumulate = ginit[x];
+            L.value = nd.value;
+            ginit[x] = 1;
+            L.desc = "backward embedding " + dims_str(L.M, L.N, L.K) + " -> grad of node " +
+                     std::to_string(x);
+            out.push_back(L);
+            continue;
+        }
         if (nd.op == FG_OP_SOFTMAX) {
             const uint32_t x = nd.in[0];
             if (!P.needs_grad[x]) continue;
@@ -1078,6 +1259,35 @@ int check_launch(const fg_plan &P, const Launch &L) {
             break;
         case LK_FILL0:
             chk(L.sC, L.count, "fill");
+            break;
+        case LK_LN:
+        case LK_LN_BWD:
+            chk(L.sA, M * N, "x");
+            chk(L.sB, M * N, "dy");
+            chk(L.sC, M * N, "y");
+            chk(L.sZ, N, "gamma");
+            chk(L.sBias, N, "beta");
+            chk(L.sMean, M, "mean");
+            chk(L.sRstd, M, "rstd");
+            chk(L.sG, N, "dgamma");
+            chk(L.sH, N, "dbeta");
+            break;
+        case LK_EMB:
+            chk(L.sA, K * N, "table");
+            chk(L.sB, M, "tokens");
+            chk(L.sC, M * N, "out");
+            break;
+        case LK_EMB_BWD:
+            chk(L.sB, M, "tokens");
+            chk(L.sZ, M * N, "dout");
+            chk(L.sC, K * N, "dtable");
+            break;
+        case LK_CKPT_SAVE:
+        case LK_CKPT_LOAD:
+            chk(L.sA, M * N, "pre-activation");
+            chk(L.sC, M * N, "activation");
+            if (rc == FG_OK) rc = check_slot(P, L, L.sB, M * N, "bytes");
+            if (rc == FG_OK) rc = check_slot(P, L, L.sZ, M * ((N - 1) / 32 + 1), "exponents");
             break;
         case LK_ELT: {
             const fg::EltProgram &p = L.prog;
@@ -1371,6 +1581,36 @@ int run(fg_plan &P, const std::vector<Launch> &list, bool step = false, bool def
             case LK_FILL0:
                 rc = fg_fill_u32(ctx, P.ptr(L.sC), 0u, L.count);
                 break;
+            case LK_LN:
+                rc = fg_layer_norm(ctx, L.dtype, P.ptr(L.sA), L.N, P.ptr(L.sZ), P.ptr(L.sBias),
+                                   L.value, L.M, L.N, P.ptr(L.sC), L.N, (float *)P.ptr(L.sMean),
+                                   (float *)P.ptr(L.sRstd));
+                break;
+            case LK_LN_BWD:
+                rc = fg_layer_norm_bwd(ctx, L.dtype, P.ptr(L.sA), L.N, P.ptr(L.sB), L.N,
+                                       P.ptr(L.sZ), (const float *)P.ptr(L.sMean),
+                                       (const float *)P.ptr(L.sRstd), L.M, L.N, P.ptr(L.sC), L.N,
+                                       L.accumulate, P.ptr(L.sG), L.accumulate2, P.ptr(L.sH),
+                                       L.accumulate3);
+                break;
+            case LK_EMB:
+                rc = fg_embedding(ctx, L.dtype, (const uint32_t *)P.ptr(L.sB), L.M, L.K, L.N,
+                                  P.ptr(L.sA), L.N, L.value, P.ptr(L.sC), L.N);
+                break;
+            case LK_EMB_BWD:
+                rc = fg_embedding_bwd(ctx, L.dtype, (const uint32_t *)P.ptr(L.sB), L.M, L.K, L.N,
+                                      P.ptr(L.sZ), L.N, L.value, P.ptr(L.sC), L.N, L.accumulate);
+                break;
+            case LK_CKPT_SAVE:
+                rc = fg_ckpt8_save(ctx, L.dtype, P.ptr(L.sA), L.N, L.M, L.N,
+                                   (int8_t *)P.ptr(L.sB), L.N, (uint8_t *)P.ptr(L.sZ),
+                                   (L.N - 1) / 32 + 1);
+                break;
+            case LK_CKPT_LOAD:
+                rc = fg_ckpt8_load(ctx, L.dtype, L.act, (const int8_t *)P.ptr(L.sB), L.N,
+                                   (const uint8_t *)P.ptr(L.sZ), (L.N - 1) / 32 + 1, L.M, L.N,
+                                   P.ptr(L.sA), L.N, P.ptr(L.sC), L.N);
+                break;
             default:
                 fg::set_error("plan: unknown launch kind %d", L.kind);
                 return FG_ERR_INTERNAL;
@@ -1390,7 +1630,8 @@ const std::vector<Launch> &captured_bwd(const fg_plan &P) {
 
 // Byte ranges a launch reads or writes (its slots, whole).
 std::vector<fg::ByteRange> launch_ranges(const fg_plan &P, const Launch &L) {
-    std::vector<int> sl = {L.sA, L.sB, L.sC, L.sZ, L.sBias, L.sExtra, L.sProbs, L.label_slot};
+    std::vector<int> sl = {L.sA,     L.sB,     L.sC,         L.sZ,    L.sBias, L.sExtra,
+                           L.sProbs, L.sMean,  L.sRstd,      L.sG,    L.sH,    L.label_slot};
     for (int k = 0; k < fg::kEltMaxSrc; ++k) sl.push_back(L.src_slot[k]);
     for (int k = 0; k < fg::kEltMaxDst; ++k) sl.push_back(L.dst_slot[k]);
     std::vector<fg::ByteRange> r;
@@ -1739,11 +1980,56 @@ FG_API int fg_graph_input(fg_graph *g, const uint32_t *fields, int rank, uint32_
 
 FG_API int fg_graph_input_x(fg_graph *g, const uint32_t *fields, int rank, int dtype,
                            uint32_t *node) {
-    FG_REQUIRE(dtype >= FG_DTYPE_F32 && dtype <= FG_DTYPE_BF16, FG_ERR_UNSUPPORTED,
-               "fg_graph_input_x: element type %d is not F32 / F16 / BF16", dtype);
+    FG_REQUIRE(dtype >= FG_DTYPE_F32 && dtype <= FG_DTYPE_U32, FG_ERR_UNSUPPORTED,
+               "fg_graph_input_x: element type %d is not F32 / F16 / BF16 / U32", dtype);
     int rc = fg_graph_input(g, fields, rank, node);
     if (rc == FG_OK) g->nodes[*node].dtype = dtype;
     return rc;
+}
+
+FG_API int fg_graph_layer_norm(fg_graph *g, uint32_t x, uint32_t gamma, uint32_t beta, float eps,
+                               uint32_t *node) {
+    FG_REQUIRE(g && node, FG_ERR_INVALID_ARGUMENT, "fg_graph_layer_norm: NULL argument");
+    FG_REQUIRE(eps > 0.0f && eps < INFINITY, FG_ERR_INVALID_ARGUMENT,
+               "fg_graph_layer_norm: eps must be positive and finite");
+    for (uint32_t k : {x, gamma, beta})
+        FG_REQUIRE(k < g->nodes.size(), FG_ERR_GRAPH,
+                   "fg_graph_layer_norm: input node %u does not exist", k);
+    FG_REQUIRE(x != gamma && x != beta && gamma != beta, FG_ERR_UNSUPPORTED,
+               "fg_graph_layer_norm: x, gamma and beta must be different nodes");
+    GNode nd;
+    nd.op = FG_OP_LAYER_NORM;
+    nd.in = {x, gamma, beta};
+    nd.value = eps;
+    g->nodes.push_back(nd);
+    *node = (uint32_t)g->nodes.size() - 1;
+    return FG_OK;
+}
+
+FG_API int fg_graph_embedding(fg_graph *g, uint32_t table, uint32_t tokens, float scale,
+                              uint32_t *node) {
+    FG_REQUIRE(g && node, FG_ERR_INVALID_ARGUMENT, "fg_graph_embedding: NULL argument");
+    for (uint32_t k : {table, tokens})
+        FG_REQUIRE(k < g->nodes.size(), FG_ERR_GRAPH,
+                   "fg_graph_embedding: input node %u does not exist", k);
+    FG_REQUIRE(g->nodes[tokens].op == FG_OP_INPUT && g->nodes[tokens].dtype == FG_DTYPE_U32,
+               FG_ERR_UNSUPPORTED, "fg_graph_embedding: node %u is not a u32 input", tokens);
+    GNode nd;
+    nd.op = FG_OP_EMBEDDING;
+    nd.in = {table, tokens};
+    nd.value = scale;
+    g->nodes.push_back(nd);
+    *node = (uint32_t)g->nodes.size() - 1;
+    return FG_OK;
+}
+
+FG_API int fg_graph_set_ckpt8(fg_graph *g, uint32_t node, int on) {
+    FG_REQUIRE(g && node < g->nodes.size(), FG_ERR_INVALID_ARGUMENT,
+               "fg_graph_set_ckpt8: NULL graph or no node %u", node);
+    FG_REQUIRE(g->nodes[node].op == FG_OP_RELU || g->nodes[node].op == FG_OP_GELU,
+               FG_ERR_INVALID_ARGUMENT, "fg_graph_set_ckpt8: node %u is not a relu or gelu", node);
+    g->nodes[node].ckpt8 = on != 0;
+    return FG_OK;
 }
 
 FG_API int fg_graph_constant(fg_graph *g, int dtype, float value, uint32_t *node) {
@@ -1839,7 +2125,7 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
     for (uint32_t i = 0; i < nn; ++i) {
         const GNode &nd = G.nodes[i];
         if (nd.op == FG_OP_INPUT) {
-            P->needs_grad[i] = !(nd.flags & FG_INPUT_NO_GRAD);
+            P->needs_grad[i] = !(nd.flags & FG_INPUT_NO_GRAD) && nd.dtype != FG_DTYPE_U32;
             P->inputs.push_back(i);
         } else if (nd.op != FG_OP_CONST) {
             for (uint32_t x : nd.in) P->needs_grad[i] |= P->needs_grad[x];
@@ -1857,6 +2143,14 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
                        "%s %u: gradient of a row-broadcast operand is not supported",
                        op_name(nd.op), i);
         }
+    }
+    for (uint32_t i = 0; i < nn; ++i) {
+        const GNode &nd = G.nodes[i];
+        if (nd.op == FG_OP_LAYER_NORM)
+            FG_REQUIRE(P->dtype[nd.in[1]] == P->dtype[i] && P->dtype[nd.in[2]] == P->dtype[i] &&
+                           G.nodes[nd.in[1]].op != FG_OP_CONST && G.nodes[nd.in[2]].op != FG_OP_CONST,
+                       FG_ERR_UNSUPPORTED,
+                       "layer_norm %u: x, gamma and beta of different element types", i);
     }
     P->ce_fused_possible = G.loss == FG_LOSS_CE && G.nodes.back().op == FG_OP_SOFTMAX;
 
@@ -1911,10 +2205,57 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
     for (uint32_t i = 0; i < nn; ++i) {
         const int op = G.nodes[i].op;
         if (op == FG_OP_INPUT || op == FG_OP_CONST) continue;
+        const int gi = P->group_of[i];
+        const int act = gi == kNone ? kNone : P->groups[gi].act_node;
+        if (act != kNone && G.nodes[act].ckpt8) continue;  // below
         P->val_slot[i] = P->new_slot((uint64_t)P->shape[i].numel(), P->dtype[i]);
+    }
+    // Activations kept in 8 bits: their GEMM writes z into one slot that all of them
+    // share and the activation into one of few, taken in turn by the layers whose
+    // forward no longer reads it; a backward restores both there.
+    P->ck_q.assign(nn, kNone);
+    P->ck_e = P->ck_z = P->ck_h = P->ck_q;
+    std::vector<char> scratch(nn, 0);
+    {
+        int z_base = kNone;
+        std::vector<std::pair<int, uint32_t>> pool;  // slot, the last node that reads it
+        for (uint32_t i = 0; i < nn; ++i) {
+            if (!G.nodes[i].ckpt8) continue;
+            const int gi = P->group_of[i];
+            const bool fits = gi != kNone && P->groups[gi].act_node == (int)i &&
+                              (int)i != P->last && P->users[i].size() == 1 &&
+                              G.nodes[P->users[i][0]].op == FG_OP_MATMUL &&
+                              G.nodes[P->users[i][0]].in[0] == i;
+            FG_REQUIRE(fits, FG_ERR_UNSUPPORTED,
+                       "fg_graph_set_ckpt8: node %u must be the activation of a matmul (and bias) "
+                       "and the first operand of one other matmul, its only user", i);
+            const Group &gr = P->groups[gi];
+            const uint32_t reader = (uint32_t)P->groups[P->group_of[P->users[i][0]]].fin;
+            const uint64_t n = (uint64_t)P->shape[i].numel(), rows = (uint64_t)P->shape[i].rows;
+            const uint64_t blocks = (uint64_t)((P->shape[i].cols - 1) / 32 + 1);
+            if (z_base == kNone) z_base = P->new_slot(0);
+            size_t k = 0;
+            while (k < pool.size() && pool[k].second >= i) ++k;
+            if (k == pool.size()) pool.push_back({P->new_slot(0), 0});
+            pool[k].second = reader;
+            P->ck_z[i] = P->val_slot[gr.pre] = P->new_shared(z_base, n, P->dtype[i]);
+            P->val_slot[i] = P->new_shared(pool[k].first, n, P->dtype[i]);
+            P->ck_h[i] = P->new_shared(pool[0].first, n, P->dtype[i]);
+            P->ck_q[i] = P->new_slot((n + 3) / 4);
+            P->ck_e[i] = P->new_slot((rows * blocks + 3) / 4);
+            for (int m : {gr.mm, gr.bias_node, gr.act_node})
+                if (m != kNone) scratch[m] = 1;
+        }
     }
     for (const Group &gr : P->groups)  // the pre-bias product is not materialised
         if (gr.bias_node != kNone) P->val_slot[gr.mm] = P->val_slot[gr.bias_node];
+    P->mean_of.assign(nn, kNone);
+    P->rstd_of.assign(nn, kNone);
+    for (uint32_t i = 0; i < nn; ++i)
+        if (G.nodes[i].op == FG_OP_LAYER_NORM) {
+            P->mean_of[i] = P->new_slot((uint64_t)P->shape[i].rows);
+            P->rstd_of[i] = P->new_slot((uint64_t)P->shape[i].rows);
+        }
     for (uint32_t i = 0; i < nn; ++i) {
         if (G.nodes[i].op == FG_OP_CONST) continue;
         if (P->needs_grad[i] || (int)i == P->last)
@@ -1942,7 +2283,8 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
     // Optimiser.
     for (size_t k = 0; k < P->inputs.size(); ++k) {
         const GNode &nd = G.nodes[P->inputs[k]];
-        if (!(nd.flags & (FG_INPUT_NO_GRAD | FG_INPUT_FROZEN))) P->opt_inputs.push_back((uint32_t)k);
+        if (!(nd.flags & (FG_INPUT_NO_GRAD | FG_INPUT_FROZEN)) && nd.dtype != FG_DTYPE_U32)
+            P->opt_inputs.push_back((uint32_t)k);
     }
     P->m_slot.assign(P->inputs.size(), kNone);
     P->v_slot.assign(P->inputs.size(), kNone);
@@ -1956,7 +2298,7 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
     }
     // Exposed lists in SaveIndicator order.
     for (uint32_t i = 0; i < nn; ++i) {
-        if (P->save[i] & kDefFwd) P->saved_nodes.push_back(i);
+        if ((P->save[i] & kDefFwd) && !scratch[i]) P->saved_nodes.push_back(i);
         if ((P->save[i] & kDefBwd) && P->grad_slot[i] != kNone) P->grad_nodes.push_back(i);
     }
 
@@ -1983,6 +2325,12 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
             for (const Launch &L : *list)
                 if (L.kind == LK_BIAS_GRAD)
                     ws = std::max<uint64_t>(ws, fg::bias_grad_ws_bytes(cus, L.M, L.N));
+                else if (L.kind == LK_LN_BWD && (L.sG != kNone || L.sH != kNone))
+                    ws = std::max<uint64_t>(ws,
+                                            fg::layer_norm_bwd_ws_bytes(cus, L.dtype, L.M, L.N));
+                else if (L.kind == LK_EMB_BWD)
+                    ws = std::max<uint64_t>(
+                        ws, fg::embedding_bwd_ws_bytes(L.dtype, L.M, L.K, L.N));
         for (auto *list : {&P->fwd, &P->bwd_seed, &P->bwd_fused})
             for (const Launch &L : *list)
                 if ((L.kind == LK_GEMM || L.kind == LK_GEMM_BWD) && L.dtype != FG_DTYPE_F32) {
@@ -2005,7 +2353,7 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
     uint64_t off = 0;
     int k = 0;
     for (Slot &s : P->slots) {
-        if (s.external) continue;
+        if (s.external || s.base != kNone) continue;
         constexpr uint64_t kWin = 64 * 1024, kStep = 4 * 1024;
         const uint64_t want = kStep * (1 + (uint64_t)(k++ % 15));
         off += (want + kWin - off % kWin) % kWin;
@@ -2301,7 +2649,8 @@ FG_API int fg_plan_launch_step(fg_plan *p) {
 }
 
 // ------------------------------------------------------------ checkpoints
-// A checkpoint is a bpat file holding every Input in input order, then for
+// A checkpoint is a bpat file holding every Input in input order (but u32
+// tokens, which are data and have no bpat type), then for
 // Adam the m and v state of each updated input and a one-element tensor
 // with the step count (the reference's io::save_tensors covers the tensors
 // a caller passes; optimiser state has no counterpart there).
@@ -2326,7 +2675,8 @@ int plan_ckpt_tensors(const fg_plan *p, std::vector<fg_bpat_tensor> &ts) {
         return FG_OK;
     };
     for (size_t k = 0; k < p->inputs.size(); ++k)
-        if (int rc = add(p->input_slot[k], p->inputs[k])) return rc;
+        if (p->dtype[p->inputs[k]] != FG_DTYPE_U32)
+            if (int rc = add(p->input_slot[k], p->inputs[k])) return rc;
     if (p->g.optim == FG_OPTIM_ADAM) {
         for (uint32_t k : p->opt_inputs) {
             if (int rc = add(p->m_slot[k], p->inputs[k])) return rc;
@@ -2500,6 +2850,11 @@ FG_API int fg_plan_describe(const fg_plan *p, char *buf, size_t len, size_t *nee
                 n += fg::softmax_ce_dispatches(L.M, L.N, L.sBias != kNone);
             else if (L.kind == LK_BIAS_GRAD)
                 n += 2;
+            else if (L.kind == LK_LN_BWD)
+                n += fg::layer_norm_bwd_dispatches(wc ? wc->cu_count : 0, L.dtype, L.M, L.N,
+                                                   L.sC != kNone, L.sG != kNone || L.sH != kNone);
+            else if (L.kind == LK_EMB_BWD)
+                n += fg::embedding_bwd_dispatches(L.dtype, L.M, L.K, L.N);
             else
                 n += gemm_dispatches(L);
         }

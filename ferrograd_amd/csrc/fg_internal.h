@@ -137,6 +137,9 @@ int gemm16_dw_dx_dispatches(fg_ctx *ctx, int M1, int N1, int K1, const void *A1,
 // `cus` compute units, and of fg_embedding_bwd.
 uint64_t layer_norm_bwd_ws_bytes(int cus, int dtype, int R, int C);
 uint64_t embedding_bwd_ws_bytes(int dtype, int T, int V, int C);
+// Dispatches of those calls.
+int layer_norm_bwd_dispatches(int cus, int dtype, int R, int C, bool dx, bool weights);
+int embedding_bwd_dispatches(int dtype, int T, int V, int C);
 
 // Adam with device-resident step counter / bias-correction scalars
 // (k_optim.hip).  d_state points at adam_dev_state_bytes() zeroed bytes.

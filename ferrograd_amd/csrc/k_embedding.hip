@@ -690,6 +690,11 @@ namespace fg {
 uint64_t embedding_bwd_ws_bytes(int dtype, int T, int V, int C) {
     return plan_of(dtype, T, V, C).bytes();
 }
+int embedding_bwd_dispatches(int dtype, int T, int V, int C) {
+    if (T <= kDirectMax) return 1;
+    const Plan p = plan_of(dtype, T, V, C);
+    return (p.passes ? 2 * p.passes : 1) + 1 + (p.units > 1 ? 1 : 0);
+}
 }  // namespace fg
 
 FG_API int fg_embedding(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T, int V, int C,

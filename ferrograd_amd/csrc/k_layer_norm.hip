@@ -982,6 +982,11 @@ uint64_t layer_norm_bwd_ws_bytes(int cus, int dtype, int R, int C) {
     const Split s = split_of(cus > 0 ? cus : 256, dtype, R, C);
     return (uint64_t)std::max(s.splits, 1) * 2 * (uint64_t)padded(C) * sizeof(float);
 }
+int layer_norm_bwd_dispatches(int cus, int dtype, int R, int C, bool dx, bool weights) {
+    const Split s = split_of(cus > 0 ? cus : 256, dtype, R, C);
+    const bool one = s.held || (s.wide && weights);
+    return (one ? (dx || weights) : (int)dx + (int)weights) + (int)weights;
+}
 }  // namespace fg
 
 FG_API int fg_layer_norm(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const void *d_gamma,

@@ -26,8 +26,11 @@ Differences, all deliberate:
   * dims need not be multiples of 16 (the reference asserts they are,
     backend/mod.rs:617-619);
   * `bias_add` (and broadcast in add / sub) exist;
-  * `Optim.adam()` exists; `SimpleDType` covers F32, F16 and BF16 (F64 and
-    the integer types have no op on this path);
+  * `Optim.adam()` exists; `SimpleDType` covers F32, F16 and BF16, and U32 for
+    the tokens of `embedding` (F64 and the other integer types have no op on
+    this path);
+  * `layer_norm`, `embedding` and `ckpt8` (an activation kept in 8 bits for the
+    backward) exist;
   * after `dispatch_loss` with CROSS_ENTROPY on a final softmax the next
     `dispatch_backward` starts from dlogits = p - onehot (the reference
     pushes that gradient through the softmax Jacobian a second time);
@@ -49,7 +52,7 @@ from ._lib import FgError, call
 # fg_op
 OP_INPUT, OP_CONST, OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_MATMUL = 0, 1, 2, 3, 4, 5, 6
 OP_RELU, OP_GELU, OP_ELU, OP_TANH, OP_EXP, OP_LOG, OP_ABS, OP_NEG = 7, 8, 9, 10, 11, 12, 13, 14
-OP_SOFTMAX, OP_BIAS_ADD = 15, 16
+OP_SOFTMAX, OP_BIAS_ADD, OP_LAYER_NORM, OP_EMBEDDING = 15, 16, 17, 18
 # fg_role
 ROLE_FORWARD_OUT, ROLE_SEED, ROLE_LOSS, ROLE_FORWARD_SAVED, ROLE_GRAD = 0, 1, 2, 3, 4
 ROLE_INPUT, ROLE_STATE, ROLE_MEAN_LOSS, ROLE_TARGET = 5, 6, 7, 8
@@ -75,10 +78,11 @@ class SimpleDType:
     F32 = "f32"
     F16 = "f16"
     BF16 = "bf16"
+    U32 = "u32"  # token inputs only
 
 
-DTYPE_CODE = {SimpleDType.F32: 0, SimpleDType.F16: 1, SimpleDType.BF16: 2}
-_CODE_NP = {0: np.float32, 1: np.float16, 2: np.uint16}
+DTYPE_CODE = {SimpleDType.F32: 0, SimpleDType.F16: 1, SimpleDType.BF16: 2, SimpleDType.U32: 3}
+_CODE_NP = {0: np.float32, 1: np.float16, 2: np.uint16, 3: np.uint32}
 
 
 def bf16_from_f32(x) -> np.ndarray:
@@ -153,9 +157,10 @@ class _Node:
     op: int
     inputs: List[int] = field(default_factory=list)
     fields: List[int] = field(default_factory=list)
-    value: float = 0.0
+    value: float = 0.0  # constant; layer norm: eps; embedding: scale
     flags: int = 0
     dtype: int = 0  # DTYPE_CODE of an input / constant
+    ckpt8: bool = False
 
 
 class _DefineOps:
@@ -181,6 +186,8 @@ class _DefineOps:
               trainable: bool = True, requires_grad: bool = True) -> int:
         if dtype not in DTYPE_CODE:
             raise FgError(3, f"element type {dtype!r} is not supported on this path")
+        if dtype == SimpleDType.U32:
+            requires_grad = False
         flags = (0 if requires_grad else INPUT_NO_GRAD) | (0 if trainable else INPUT_FROZEN)
         return self._push(_Node(OP_INPUT, fields=[f.index for f in shape], flags=flags,
                                 dtype=DTYPE_CODE[dtype]))
@@ -212,6 +219,23 @@ class _DefineOps:
     def abs(self, x): return self._op(OP_ABS, x)
     def neg(self, x): return self._op(OP_NEG, x)
     def softmax(self, x): return self._op(OP_SOFTMAX, x)
+
+    def layer_norm(self, x, gamma, beta, eps: float = 1e-5) -> int:
+        """(x - mean) * rstd * gamma + beta over the last dimension; gamma and
+        beta are vectors of its length."""
+        return self._push(_Node(OP_LAYER_NORM, inputs=[x, gamma, beta], value=float(eps)))
+
+    def embedding(self, table, tokens, scale: float = 1.0) -> int:
+        """scale * table[tokens]: one row per token of a U32 input."""
+        return self._push(_Node(OP_EMBEDDING, inputs=[table, tokens], value=float(scale)))
+
+    def ckpt8(self, x) -> int:
+        """Keep what the backward needs of the activation node x in 8 bits
+        (fg_graph_set_ckpt8); returns x."""
+        if not 0 <= x < len(self.g.nodes):
+            raise FgError(6, f"input node {x} does not exist")
+        self.g.nodes[x].ckpt8 = True
+        return x
 
 
 class Graph:
@@ -251,7 +275,11 @@ class Graph:
                         save[x] |= 3
                 for u in users[i]:
                     save[u] |= 2
-            elif nd.op in (OP_MUL, OP_DIV):
+            elif nd.op == OP_EMBEDDING:
+                save[i] |= 3
+            elif nd.op in (OP_MUL, OP_DIV, OP_LAYER_NORM):
+                if nd.op == OP_LAYER_NORM:
+                    save[i] |= 3
                 for x in nd.inputs:
                     if nonleaf[x]:
                         save[x] |= 1
@@ -275,9 +303,15 @@ class Graph:
                         call("fg_graph_set_input_flags", h, out.value, nd.flags)
                 elif nd.op == OP_CONST:
                     call("fg_graph_constant", h, nd.dtype, nd.value, ctypes.byref(out))
+                elif nd.op == OP_LAYER_NORM:
+                    call("fg_graph_layer_norm", h, *nd.inputs, nd.value, ctypes.byref(out))
+                elif nd.op == OP_EMBEDDING:
+                    call("fg_graph_embedding", h, *nd.inputs, nd.value, ctypes.byref(out))
                 else:
                     arr = (ctypes.c_uint32 * len(nd.inputs))(*nd.inputs)
                     call("fg_graph_op", h, nd.op, arr, len(nd.inputs), ctypes.byref(out))
+                if nd.ckpt8:
+                    call("fg_graph_set_ckpt8", h, out.value, 1)
         except Exception:
             call("fg_graph_destroy", h)
             raise
@@ -501,6 +535,13 @@ class GpuContext:
         a = (a.astype(np.uint16) if a.dtype == np.uint16 else bf16_from_f32(a)).reshape(-1)
         if a.size != int(np.prod(shape)):
             raise FgError(5, f"init_tensor_bf16: {a.size} values for shape {tuple(shape)}")
+        return self._alloc(a, shape)
+
+    def init_tensor_u32(self, shape: Sequence[int], data) -> Tensor:
+        """Tokens of a U32 input."""
+        a = np.asarray(data, dtype=np.uint32).reshape(-1)
+        if a.size != int(np.prod(shape)):
+            raise FgError(5, f"init_tensor_u32: {a.size} values for shape {tuple(shape)}")
         return self._alloc(a, shape)
 
     def new_onehot_init(self, labels: Sequence[int]) -> Tensor:

@@ -192,7 +192,12 @@ int fg_matmul_bwd_f32(fg_ctx *ctx, int M, int N, int K,
  * (crates/fused_gpu/src/dispatch/backend/mod.rs:335-427). 16-bit tensors are
  * stored as 16-bit words; kernels compute in fp32 and round to the storage
  * type (nearest even) wherever a node value is stored. */
-typedef enum fg_dtype { FG_DTYPE_F32 = 0, FG_DTYPE_F16 = 1, FG_DTYPE_BF16 = 2 } fg_dtype;
+typedef enum fg_dtype {
+    FG_DTYPE_F32 = 0,
+    FG_DTYPE_F16 = 1,
+    FG_DTYPE_BF16 = 2,
+    FG_DTYPE_U32 = 3 /* token inputs of a graph only (fg_graph_embedding) */
+} fg_dtype;
 
 /* 16-bit GEMMs (dtype FG_DTYPE_F16 or FG_DTYPE_BF16 for every operand and
  * output): the same contract as fg_gemm_f32 / fg_gemm_bwd_f32, with the
@@ -528,7 +533,9 @@ typedef enum fg_op {
     FG_OP_ABS = 13,
     FG_OP_NEG = 14,
     FG_OP_SOFTMAX = 15,
-    FG_OP_BIAS_ADD = 16
+    FG_OP_BIAS_ADD = 16,
+    FG_OP_LAYER_NORM = 17, /* built by fg_graph_layer_norm */
+    FG_OP_EMBEDDING = 18   /* built by fg_graph_embedding  */
 } fg_op;
 
 /* Input flags (extension): every Input is trainable in ferrograd
@@ -546,8 +553,9 @@ int fg_graph_new_field(fg_graph *g, uint32_t *field);
  * meta fields. */
 int fg_graph_input(fg_graph *g, const uint32_t *fields, int rank, uint32_t *node);
 /* DefineOps::input(&[fields], SimpleDType) (graph.rs:111, backend/mod.rs:
- * 335-427): an input of element type dtype (FG_DTYPE_F32 / F16 / BF16).
- * Operations take the type of their first input. */
+ * 335-427): an input of element type dtype (FG_DTYPE_F32 / F16 / BF16, or U32
+ * for tokens, which take no gradient and no update).  Operations take the type
+ * of their first input. */
 int fg_graph_input_x(fg_graph *g, const uint32_t *fields, int rank, int dtype,
                      uint32_t *node);
 /* DefineOps::constant_f32 (graph.rs:106-159): a scalar constant. */
@@ -558,6 +566,26 @@ int fg_graph_constant(fg_graph *g, int dtype, float value, uint32_t *node);
 /* DefineOps::{add,sub,mul,div,matmul,relu,...,softmax}: node from op and
  * inputs (ids must exist already). */
 int fg_graph_op(fg_graph *g, int op, const uint32_t *inputs, int n_inputs, uint32_t *node);
+/* Layer norm over the last dimension of x[..., N] with gamma[N] and beta[N] (three
+ * different nodes of one element type; no reference counterpart): the forward
+ * is fg_layer_norm, the backward fg_layer_norm_bwd. */
+int fg_graph_layer_norm(fg_graph *g, uint32_t x, uint32_t gamma, uint32_t beta, float eps,
+                        uint32_t *node);
+/* The lookup scale * table[tokens] of a u32 input in a table[V][N] (no reference
+ * counterpart): a matrix of one row per token.  fg_embedding, and for the
+ * table's gradient fg_embedding_bwd.  A table may also feed other nodes (a tied
+ * output layer): its gradients add. */
+int fg_graph_embedding(fg_graph *g, uint32_t table, uint32_t tokens, float scale,
+                       uint32_t *node);
+/* Keep what the backward needs of a relu or gelu node in 8 bits (on != 0; see
+ * fg_ckpt8_save): the node's matmul writes its pre-activation and activation
+ * into memory that all such layers of a plan share, and the backward of the
+ * matmul that reads the activation restores both there.  The forward's values
+ * are unchanged; the gradients come from the restored ones.  The node must be the
+ * activation of a matmul (with or without bias) and the first operand of one
+ * other matmul, its only user (checked by fg_plan_create).  Its values are not
+ * among FG_ROLE_FORWARD_SAVED. */
+int fg_graph_set_ckpt8(fg_graph *g, uint32_t node, int on);
 int fg_graph_set_input_flags(fg_graph *g, uint32_t node, uint32_t flags);
 int fg_graph_num_nodes(const fg_graph *g, uint32_t *n);
 /* Graph::validate (backend/mod.rs:853-975, 1172-1185) against a meta
@@ -624,7 +652,7 @@ int fg_plan_single_optim(fg_plan *p, int input_index);
 int fg_plan_capture_step(fg_plan *p);
 int fg_plan_launch_step(fg_plan *p);
 /* Checkpoint of a plan to / from a bpat file (format header as for
- * fg_bpat_save): every Input in input order, then for Adam the m and v of
+ * fg_bpat_save): every Input but u32 tokens in input order, then for Adam the m and v of
  * each updated input and a one-element tensor holding the step count.
  * Loading checks the tensor count and sizes and restores all of them into
  * the plan's bound inputs and state.  (The reference saves only the tensors
