@@ -38,11 +38,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNT = 256;
 constexpr int kDirectMax = 256;
-constexpr int kRankMax = 16384;
-#ifndef UB
-#define UB 1024
-#endif
-constexpr int kUnitBlocks = UB;
+constexpr int kRankMax = 14336;
+constexpr int kUnitBlocks = 1024;
 
 // ------------------------------------------------------------------- lookup
 // 2^lshift lanes take a row, UNR chunks in flight a lane.
@@ -160,7 +157,10 @@ __global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ 
 // order[k] = the k-th position in (token, position) order, sorted[k] its token: a
 // lane counts the positions before its own; 16 waves take a share of the tokens
 // each, 64 at a time in scalar registers, so that a comparison and an addition with
-// carry are all a lane does for a token.
+// carry are all a lane does for a token: bound by the vector unit, 8192 tokens 11.7 us,
+// 16384 21.3 (the radix sort about 24 from there to 65536).  [a < b] as a subtraction
+// that stops at 0, bounded by 1 and added two at a time, which waits for no result in
+// a scalar register, took as long.
 typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
 typedef u32x16 u32x16_any __attribute__((aligned(4)));
 __global__ __launch_bounds__(1024) void emb_rank(const uint32_t *__restrict__ tokens, int T,
@@ -406,7 +406,9 @@ struct Sums {
     float *partial;   // [units][2][Cp]: the run that began before, the one that goes on
 };
 
-template <int DT>
+// WAVE: a unit's lanes fill whole waves, so that positions, tokens and rows' addresses
+// are scalar.
+template <int DT, bool WAVE>
 __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
                                                 const typename Io<DT>::T *__restrict__ dout,
                                                 typename Io<DT>::T *dtable) {
@@ -425,10 +427,17 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
             if ((threadIdx.x & 63) == 0) range[wave] = at;
         }
         __syncthreads();
-        if ((int)threadIdx.x < n) {
+        // The rows' tokens are sorted[lo, hi): marked from there where a thread takes
+        // one each, else (a frequent token is among them) searched for.
+        const int lo = range[0], hi = range[1];
+        if (hi - lo <= kNT) {
+            used[threadIdx.x] = 0;
+            __syncthreads();
+            if (lo + (int)threadIdx.x < hi) used[p.sorted[lo + threadIdx.x] - (uint32_t)v0] = 1;
+        } else if ((int)threadIdx.x < n) {
             const uint32_t v = (uint32_t)(v0 + threadIdx.x);
-            const int k = lower_bound(p.sorted, range[0], range[1], v);
-            used[threadIdx.x] = k < range[1] && p.sorted[k] == v;
+            const int k = lower_bound(p.sorted, lo, hi, v);
+            used[threadIdx.x] = k < hi && p.sorted[k] == v;
         }
         __syncthreads();
         const float z[E] = {};
@@ -442,38 +451,48 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
         return;
     }
     const int lanes = 1 << p.lshift;
-    const int unit = (int)(blockIdx.x << (8 - p.lshift)) + (int)(threadIdx.x >> p.lshift);
+    int unit = (int)(blockIdx.x << (8 - p.lshift)) + (int)(threadIdx.x >> p.lshift);
+    if constexpr (WAVE) unit = __builtin_amdgcn_readfirstlane(unit);
     const int j = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
     if (unit >= p.units || j >= chunks) return;
     const int k0 = unit * p.P, k1 = min(p.T, k0 + p.P);
-    // A run that began before the unit, or goes on after it, is a partial sum.
     const uint32_t V = (uint32_t)p.V;
-    bool head = k0 > 0 && p.sorted[k0 - 1] == p.sorted[k0];
+    const uint32_t *__restrict__ sorted = p.sorted, *__restrict__ order = p.order;
+    // A run that began before the unit, or goes on after it, is a partial sum.
+    bool head = k0 > 0 && sorted[k0 - 1] == sorted[k0];
     float a[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) a[e] = 0.0f;
-    for (int k = k0; k < k1; k += UNR) {
-        uint32_t tok[UNR + 1];
-        u32x4 w[UNR];
+    // Positions and tokens of the next UNR rows are loaded before this batch's rows
+    // are added.
+    uint32_t pos[UNR], tok[UNR + 1];
+    auto index = [&](int k) {
 #pragma unroll
         for (int u = 0; u < UNR; ++u) {
-            const int at = min(k + u, k1 - 1);
-            tok[u] = p.sorted[at];
-            w[u] = Chunk<DT>::load(dout + (size_t)p.order[at] * p.lddo, j, nb, p.C);
+            pos[u] = order[min(k + u, k1 - 1)];
+            tok[u] = sorted[min(k + u, p.T - 1)];
         }
-        tok[UNR] = p.sorted[min(k + UNR, p.T - 1)];
+        tok[UNR] = sorted[min(k + UNR, p.T - 1)];
+    };
+    index(k0);
+    for (int k = k0; k < k1; k += UNR) {
+        u32x4 w[UNR];
+        uint32_t t[UNR + 1];
+#pragma unroll
+        for (int u = 0; u < UNR; ++u)
+            w[u] = Chunk<DT>::load(dout + (size_t)pos[u] * p.lddo, j, nb, p.C);
+#pragma unroll
+        for (int u = 0; u <= UNR; ++u) t[u] = tok[u];
+        if (k + UNR < k1) index(k + UNR);
 #pragma unroll
         for (int u = 0; u < UNR; ++u) {
             if (k + u >= k1) break;
 #pragma unroll
             for (int e = 0; e < E; ++e) a[e] += IO::get(w[u], e);
-            const bool last = k + u + 1 == p.T;
-            const uint32_t next =
-                k + u + 1 < k1 || last ? tok[u + 1] : p.sorted[k1];  // (k1 < T there)
-            if (!last && next == tok[u] && k + u + 1 < k1) continue;
-            const bool on = !last && next == tok[u];  // goes on in the next unit
-            if (tok[u] < V) {
-                if (head || on) {
+            const bool same = k + u + 1 < p.T && t[u + 1] == t[u];
+            if (same && k + u + 1 < k1) continue;
+            if (t[u] < V) {
+                if (head || same) {  // (same: the run goes on in the next unit)
                     float *to = p.partial + ((size_t)unit * 2 + (head ? 0 : 1)) * p.Cp +
                                 (size_t)j * E;
 #pragma unroll
@@ -481,7 +500,7 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
                         *reinterpret_cast<f32x4 *>(to + 4 * q) =
                             f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
                 } else {
-                    auto *to = dtable + (size_t)tok[u] * p.lddt;
+                    auto *to = dtable + (size_t)t[u] * p.lddt;
 #pragma unroll
                     for (int e = 0; e < E; ++e) a[e] *= p.scale;
                     if (p.accumulate) {
@@ -641,6 +660,8 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
             radix_count<<<pl.tiles, kSortNT, 0, st>>>(kin, T, (uint32_t)V, pl.per, n * pl.bits,
                                                       pl.bits, hist);
             FG_LAUNCH_CHECK("radix_count");
+            // (The next pass's counts added up here by atomics, one launch fewer, took the
+            // first pass from 8.5 to 21 us for 65536 tokens.)
             radix_place<<<pl.tiles, kSortNT, 0, st>>>(kin, pin, T, (uint32_t)V, pl.per,
                                                       n * pl.bits, pl.bits, hist, key[to],
                                                       pos[to]);
@@ -673,7 +694,8 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
         blocks += (V - 1) / s.zrows + 1;
     }
     const int tiles = (chunks - 1) / (1 << pl.lshift) + 1;
-    emb_sums<DT><<<dim3(blocks, tiles), kNT, 0, st>>>(s, d, g);
+    auto sums = pl.lshift >= 6 ? emb_sums<DT, true> : emb_sums<DT, false>;
+    sums<<<dim3(blocks, tiles), kNT, 0, st>>>(s, d, g);
     FG_LAUNCH_CHECK("emb_sums");
     if (pl.units > 1) {
         const int jshift = std::min(6, log2_up(pl.Cp / 4));
