@@ -153,6 +153,30 @@ __global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ 
     }
 }
 
+// -------------------------------------------------------------------- zeros
+// Table rows that a launch zeroes beside its own work (whether tokens have them or
+// not; what tokens do have is written by later launches).
+struct Zero {
+    char *base;
+    uint64_t stride;           // bytes between rows
+    int64_t row_bytes;         // even
+    int first, count, lshift;  // rows; log2 of a row's lanes
+};
+__device__ __forceinline__ void zero_rows(const Zero &z, int block, int blocks) {
+    const int lanes = 1 << z.lshift, lane = threadIdx.x & (lanes - 1);
+    const int groups = blockDim.x >> z.lshift;
+    const int64_t end = z.row_bytes & ~int64_t(15);
+    for (int64_t r = (int64_t)block * groups + (threadIdx.x >> z.lshift); r < z.count;
+         r += (int64_t)blocks * groups) {
+        char *to = z.base + (uint64_t)(z.first + r) * z.stride;
+        for (int64_t at = lane * 16; at < end; at += lanes * 16)
+            __builtin_nontemporal_store(u32x4{0u, 0u, 0u, 0u},
+                                        reinterpret_cast<fg::rows::u32x4_any *>(to + at));
+        for (int64_t at = end + lane * 2; at < z.row_bytes; at += lanes * 2)
+            *reinterpret_cast<uint16_t *>(to + at) = 0;
+    }
+}
+
 // ------------------------------------------------------------------- sorting
 // order[k] = the k-th position in (token, position) order, sorted[k] its token: a
 // lane counts the positions before its own; 16 waves take a share of the tokens
@@ -165,8 +189,13 @@ typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
 typedef u32x16 u32x16_any __attribute__((aligned(4)));
 __global__ __launch_bounds__(1024) void emb_rank(const uint32_t *__restrict__ tokens, int T,
                                                  uint32_t *__restrict__ order,
-                                                 uint32_t *__restrict__ sorted) {
+                                                 uint32_t *__restrict__ sorted, int blocks,
+                                                 const Zero z) {
     __shared__ int sum[16][64];
+    if ((int)blockIdx.x >= blocks) {
+        zero_rows(z, blockIdx.x - blocks, gridDim.x - blocks);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g0 = blockIdx.x * 64, i = g0 + lane;
     const uint32_t mine = i < T ? tokens[i] : 0xffffffffu;
@@ -218,8 +247,13 @@ __device__ __forceinline__ uint32_t key_of(uint32_t token, uint32_t V) { return 
 
 __global__ __launch_bounds__(kSortNT) void radix_count(const uint32_t *__restrict__ keys, int T,
                                                        uint32_t V, int per, int shift, int bits,
-                                                       uint32_t *__restrict__ hist) {
+                                                       uint32_t *__restrict__ hist, int tiles,
+                                                       const Zero z) {
     __shared__ uint32_t h[kBins];
+    if ((int)blockIdx.x >= tiles) {
+        zero_rows(z, blockIdx.x - tiles, gridDim.x - tiles);
+        return;
+    }
     const int bins = 1 << bits;
     for (int d = threadIdx.x; d < bins; d += kSortNT) h[d] = 0;
     __syncthreads();
@@ -237,13 +271,18 @@ __global__ __launch_bounds__(kSortNT) void radix_place(const uint32_t *__restric
                                                        uint32_t V, int per, int shift, int bits,
                                                        const uint32_t *__restrict__ hist,
                                                        uint32_t *__restrict__ keys_out,
-                                                       uint32_t *__restrict__ pos_out) {
+                                                       uint32_t *__restrict__ pos_out, int tiles,
+                                                       const Zero z) {
+    if ((int)blockIdx.x >= tiles) {
+        zero_rows(z, blockIdx.x - tiles, gridDim.x - tiles);
+        return;
+    }
     constexpr int kWaves = kSortNT / 64;
     // Pairs of digit d in the tile's wave w; then where they go.
     __shared__ uint32_t cnt[kWaves][kBins];
     __shared__ uint32_t base[kBins];
     __shared__ uint32_t wsum[kWaves];
-    const int bins = 1 << bits, tiles = gridDim.x;
+    const int bins = 1 << bits;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     // Each wave takes a run of the tile, 64 pairs at a time; the first kHeld rounds'
     // pairs are loaded here and stay in registers.
@@ -400,8 +439,9 @@ struct Sums {
     int P;            // sorted positions of a unit
     int units;        // units in all
     int lshift;       // log2 of a unit's lanes
-    int unit_blocks;  // workgroups of units; those after them zero `zrows` rows each
-    int zrows;
+    int unit_blocks;  // workgroups of units; those after them zero `zrows` rows each,
+    int zrows;        // from zfirst on
+    int zfirst;
     int64_t Cp;       // columns of a partial sum (rounded up to chunks)
     float *partial;   // [units][2][Cp]: the run that began before, the one that goes on
 };
@@ -420,7 +460,7 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
         if (blockIdx.y > 0) return;
         __shared__ int used[kNT];
         __shared__ int range[2];
-        const int64_t v0 = (int64_t)(blockIdx.x - p.unit_blocks) * p.zrows;
+        const int64_t v0 = p.zfirst + (int64_t)(blockIdx.x - p.unit_blocks) * p.zrows;
         const int n = (int)min((int64_t)p.zrows, p.V - v0), wave = threadIdx.x >> 6;
         if (wave < 2) {
             const int at = wave_lower_bound(p.sorted, p.T, (uint32_t)(v0 + (wave ? n : 0)));
@@ -646,8 +686,31 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
         return FG_OK;
     }
     uint32_t *order = (uint32_t *)ws, *sorted = order + T;
+    // Zeroed beside the sort, which leaves the memory idle: what its launches have time
+    // for; the whole table where that is most of it, or where few of its rows are
+    // written again.  The rest goes beside the sums, without the rows of tokens.
+    constexpr double kMB = 1 << 20;
+    const double row_mb = (double)C * sizeof(Ty) / kMB, q = T / 8192.0;
+    const double count_mb = 20.0, place_mb = 44.0, rank_mb = 12.0 + 40.0 * q * q;
+    const double sort_mb = pl.passes ? pl.passes * (count_mb + place_mb) : rank_mb;
+    int early = 0, done = 0;  // rows zeroed beside the sort; by the launches so far
+    if (!accumulate) {
+        const bool all = V * row_mb < 1.25 * sort_mb || T <= V / 8;
+        early = all ? V : (int)(sort_mb / row_mb);
+    }
+    Zero z{(char *)dtable, (uint64_t)lddt * sizeof(Ty), (int64_t)C * (int64_t)sizeof(Ty), 0, 0,
+           std::min(6, log2_up(std::max<int64_t>(1, (int64_t)C * (int64_t)sizeof(Ty) / 16)))};
+    // Workgroups (1024 threads) of the next launch's share of them.
+    auto share = [&](double mb) {
+        z.first = done;
+        z.count = std::min(early - done, (int)(early * (mb / sort_mb)) + 1);
+        done += z.count;
+        const int per = 1024 >> z.lshift;  // rows at once
+        return z.count ? std::min(2 * ctx->cu_count, (z.count - 1) / per + 1) : 0;
+    };
     if (pl.passes == 0) {
-        emb_rank<<<(T - 1) / 64 + 1, 1024, 0, st>>>(tokens, T, order, sorted);
+        const int blocks = (T - 1) / 64 + 1, zeros = share(rank_mb);
+        emb_rank<<<blocks + zeros, 1024, 0, st>>>(tokens, T, order, sorted, blocks, z);
         FG_LAUNCH_CHECK("emb_rank");
     } else {
         // The passes go back and forth between two pairs of arrays and end in the first.
@@ -657,14 +720,16 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
         const uint32_t *kin = tokens, *pin = nullptr;
         for (int n = 0; n < pl.passes; ++n) {
             const int to = (pl.passes - 1 - n) & 1;
-            radix_count<<<pl.tiles, kSortNT, 0, st>>>(kin, T, (uint32_t)V, pl.per, n * pl.bits,
-                                                      pl.bits, hist);
+            int zeros = share(count_mb);
+            radix_count<<<pl.tiles + zeros, kSortNT, 0, st>>>(
+                kin, T, (uint32_t)V, pl.per, n * pl.bits, pl.bits, hist, pl.tiles, z);
             FG_LAUNCH_CHECK("radix_count");
             // (The next pass's counts added up here by atomics, one launch fewer, took the
             // first pass from 8.5 to 21 us for 65536 tokens.)
-            radix_place<<<pl.tiles, kSortNT, 0, st>>>(kin, pin, T, (uint32_t)V, pl.per,
-                                                      n * pl.bits, pl.bits, hist, key[to],
-                                                      pos[to]);
+            zeros = share(place_mb);
+            radix_place<<<pl.tiles + zeros, kSortNT, 0, st>>>(kin, pin, T, (uint32_t)V, pl.per,
+                                                              n * pl.bits, pl.bits, hist, key[to],
+                                                              pos[to], pl.tiles, z);
             FG_LAUNCH_CHECK("radix_place");
             kin = key[to];
             pin = pos[to];
@@ -688,10 +753,11 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
     s.unit_blocks = ((pl.units - 1) >> (8 - pl.lshift)) + 1;
     int blocks = s.unit_blocks;
     s.zrows = 1;
-    if (!accumulate) {
+    s.zfirst = done;
+    if (!accumulate && done < V) {
         // Rows a workgroup zeroes: about 2048 workgroups, at most one row a thread.
-        while (s.zrows < kNT && V / s.zrows > 2048) s.zrows *= 2;
-        blocks += (V - 1) / s.zrows + 1;
+        while (s.zrows < kNT && (V - done) / s.zrows > 2048) s.zrows *= 2;
+        blocks += (V - done - 1) / s.zrows + 1;
     }
     const int tiles = (chunks - 1) / (1 << pl.lshift) + 1;
     auto sums = pl.lshift >= 6 ? emb_sums<DT, true> : emb_sums<DT, false>;
