@@ -706,7 +706,7 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
         z.count = std::min(early - done, (int)(early * (mb / sort_mb)) + 1);
         done += z.count;
         const int per = 1024 >> z.lshift;  // rows at once
-        return z.count ? std::min(2 * ctx->cu_count, (z.count - 1) / per + 1) : 0;
+        return z.count ? std::min(64 * ctx->cu_count, (z.count - 1) / per + 1) : 0;
     };
     if (pl.passes == 0) {
         const int blocks = (T - 1) / 64 + 1, zeros = share(rank_mb);
