@@ -20,6 +20,10 @@
 namespace fg {
 namespace rows {
 
+// Longest row, in columns: counts of columns are then exact in fp32, byte offsets
+// within a row fit 32 bits, and a grid's y dimension holds a row's workgroups.
+constexpr int kMaxCols = 1 << 24;
+
 using smany::Io;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));  // at any element

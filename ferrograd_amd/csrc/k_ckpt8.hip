@@ -257,6 +257,8 @@ int check_q(const char *who, int dtype, int R, int C, const void *q, int ldq, co
     FG_REQUIRE(dtype >= FG_DTYPE_F32 && dtype <= FG_DTYPE_BF16, FG_ERR_INVALID_ARGUMENT,
                "%s: bad dtype %d", who, dtype);
     FG_REQUIRE(R >= 0 && C > 0, FG_ERR_SHAPE, "%s: bad shape %d x %d", who, R, C);
+    FG_REQUIRE(C <= fg::rows::kMaxCols, FG_ERR_OUT_OF_BOUNDS, "%s: %d columns, at most %d", who, C,
+               fg::rows::kMaxCols);
     FG_REQUIRE(ldq >= C, FG_ERR_SHAPE, "%s: ldq=%d < %d columns", who, ldq, C);
     FG_REQUIRE(lde >= (C - 1) / kBlock + 1, FG_ERR_SHAPE,
                "%s: lde=%d < %d exponents (one per 32 columns)", who, lde, (C - 1) / kBlock + 1);

@@ -691,7 +691,7 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
     // written again.  The rest goes beside the sums, without the rows of tokens.
     constexpr double kMB = 1 << 20;
     const double row_mb = (double)C * sizeof(Ty) / kMB, q = T / 8192.0;
-    const double count_mb = 20.0, place_mb = 44.0, rank_mb = 12.0 + 40.0 * q * q;
+    const double count_mb = 16.0, place_mb = 60.0, rank_mb = 12.0 + 40.0 * q * q;
     const double sort_mb = pl.passes ? pl.passes * (count_mb + place_mb) : rank_mb;
     int early = 0, done = 0;  // rows zeroed beside the sort; by the launches so far
     if (!accumulate) {
@@ -792,6 +792,8 @@ FG_API int fg_embedding(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T,
                "%s: bad dtype %d", who, dtype);
     FG_REQUIRE(T >= 0 && V > 0 && C > 0, FG_ERR_SHAPE, "%s: bad shape T=%d V=%d C=%d", who, T, V,
                C);
+    FG_REQUIRE(C <= fg::rows::kMaxCols, FG_ERR_OUT_OF_BOUNDS, "%s: %d columns, at most %d", who, C,
+               fg::rows::kMaxCols);
     FG_REQUIRE(ldt >= C && ldo >= C, FG_ERR_SHAPE, "%s: ldt=%d or ldo=%d < C=%d", who, ldt, ldo,
                C);
     FG_REQUIRE(T == 0 || (d_tokens && d_table && d_out), FG_ERR_INVALID_ARGUMENT,
@@ -813,6 +815,8 @@ FG_API int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, in
                "%s: bad dtype %d", who, dtype);
     FG_REQUIRE(T >= 0 && V > 0 && C > 0, FG_ERR_SHAPE, "%s: bad shape T=%d V=%d C=%d", who, T, V,
                C);
+    FG_REQUIRE(C <= fg::rows::kMaxCols, FG_ERR_OUT_OF_BOUNDS, "%s: %d columns, at most %d", who, C,
+               fg::rows::kMaxCols);
     FG_REQUIRE(lddo >= C && lddt >= C, FG_ERR_SHAPE, "%s: lddo=%d or lddt=%d < C=%d", who, lddo,
                lddt, C);
     FG_REQUIRE(d_dtable && (T == 0 || (d_tokens && d_dout)), FG_ERR_INVALID_ARGUMENT,

@@ -1085,6 +1085,8 @@ FG_API int fg_layer_norm(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const
     FG_REQUIRE(dtype >= FG_DTYPE_F32 && dtype <= FG_DTYPE_BF16, FG_ERR_INVALID_ARGUMENT,
                "%s: bad dtype %d", who, dtype);
     FG_REQUIRE(R >= 0 && C > 0, FG_ERR_SHAPE, "%s: bad shape R=%d C=%d", who, R, C);
+    FG_REQUIRE(C <= fg::rows::kMaxCols, FG_ERR_OUT_OF_BOUNDS, "%s: %d columns, at most %d", who, C,
+               fg::rows::kMaxCols);
     FG_REQUIRE(ldx >= C && ldy >= C, FG_ERR_SHAPE, "%s: ldx=%d or ldy=%d < C=%d", who, ldx, ldy,
                C);
     FG_REQUIRE(eps > 0.0f && eps < INFINITY, FG_ERR_INVALID_ARGUMENT,
@@ -1112,6 +1114,8 @@ FG_API int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, c
     FG_REQUIRE(dtype >= FG_DTYPE_F32 && dtype <= FG_DTYPE_BF16, FG_ERR_INVALID_ARGUMENT,
                "%s: bad dtype %d", who, dtype);
     FG_REQUIRE(R >= 0 && C > 0, FG_ERR_SHAPE, "%s: bad shape R=%d C=%d", who, R, C);
+    FG_REQUIRE(C <= fg::rows::kMaxCols, FG_ERR_OUT_OF_BOUNDS, "%s: %d columns, at most %d", who, C,
+               fg::rows::kMaxCols);
     FG_REQUIRE(ldx >= C && lddy >= C && (!d_dx || lddx >= C), FG_ERR_SHAPE,
                "%s: ldx=%d, lddy=%d or lddx=%d < C=%d", who, ldx, lddy, lddx, C);
     FG_REQUIRE(d_x && d_dy && d_mean && d_rstd, FG_ERR_INVALID_ARGUMENT,

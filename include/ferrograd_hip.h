@@ -305,6 +305,10 @@ int fg_softmax_bwd(fg_ctx *ctx, int dtype, const void *d_y, const void *d_dy, in
                    int C, void *d_dx, int accumulate);
 
 /* -------------------------------------------------- token-model operators */
+/* The following take rows of any alignment and of up to 2^24 columns.  Calls
+ * that use the workspace share it with the context's other direct calls, in
+ * the stream's order: graphs captured on one context must not run at the same
+ * time. */
 /* Layer norm over the last dimension (no reference counterpart; the row
  * operator next to the softmax node, op/softmax.rs:14-759).  Per row r:
  *   mean = sum(x_r) / C ; var = sum((x_r - mean)^2) / C ; rstd = 1/sqrt(var + eps)

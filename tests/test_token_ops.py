@@ -7,7 +7,8 @@ import ferrograd_amd as fa
 from ferrograd_amd import _lib
 
 P = 4096  # a non-NULL pointer; nothing may read it
-INVALID, SHAPE = 1, 5
+INVALID, SHAPE, BOUNDS = 1, 5, 9
+BIG = (1 << 24) + 1  # columns: one more than any of these takes
 NAN, INF = float("nan"), float("inf")
 
 # name -> (argument names, a call that only lacks its context)
@@ -32,6 +33,12 @@ CALLS = {
 }
 
 REFUSED = [
+    ("fg_layer_norm", dict(C=BIG, ldx=BIG, ldy=BIG), BOUNDS),
+    ("fg_layer_norm_bwd", dict(C=BIG, ldx=BIG, lddy=BIG, lddx=BIG), BOUNDS),
+    ("fg_embedding", dict(C=BIG, ldt=BIG, ldo=BIG), BOUNDS),
+    ("fg_embedding_bwd", dict(C=BIG, lddo=BIG, lddt=BIG), BOUNDS),
+    ("fg_ckpt8_save", dict(C=BIG, ldx=BIG, ldq=BIG, lde=BIG), BOUNDS),
+    ("fg_matmul_bwd_ckpt8", dict(K=BIG, ldq=BIG, lde=BIG, lddx=BIG), BOUNDS),
     ("fg_layer_norm", dict(dtype=3), INVALID), ("fg_layer_norm", dict(dtype=-1), INVALID),
     ("fg_layer_norm", dict(R=-1), SHAPE), ("fg_layer_norm", dict(C=0), SHAPE),
     ("fg_layer_norm", dict(ldx=63), SHAPE), ("fg_layer_norm", dict(ldy=63), SHAPE),
