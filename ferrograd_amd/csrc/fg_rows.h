@@ -22,7 +22,11 @@ namespace rows {
 
 // Longest row, in columns: counts of columns are then exact in fp32, byte offsets
 // within a row fit 32 bits, and a grid's y dimension holds a row's workgroups.
-constexpr int kMaxCols = 1 << 24;
+constexpr int kMaxCols = 1 << 23;
+// Whether a grid's x dimension holds `blocks` workgroups: fewer than 2^32 threads.
+inline bool grid_holds(int64_t blocks, int threads) {
+    return blocks * threads < int64_t(1) << 32;
+}
 
 using smany::Io;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -263,6 +263,8 @@ int check_q(const char *who, int dtype, int R, int C, const void *q, int ldq, co
     FG_REQUIRE(lde >= (C - 1) / kBlock + 1, FG_ERR_SHAPE,
                "%s: lde=%d < %d exponents (one per 32 columns)", who, lde, (C - 1) / kBlock + 1);
     FG_REQUIRE(q && e, FG_ERR_INVALID_ARGUMENT, "%s: q and e are required", who);
+    FG_REQUIRE(R == 0 || fg::rows::grid_holds(shape_of(dtype, R, C).grid.x, kNT),
+               FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns", who, R, C);
     return FG_OK;
 }
 

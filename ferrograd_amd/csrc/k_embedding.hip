@@ -40,6 +40,7 @@ constexpr int kNT = 256;
 constexpr int kDirectMax = 256;
 constexpr int kRankMax = 14336;
 constexpr int kUnitBlocks = 1024;
+constexpr int kMaxTokens = 1 << 30;  // (positions a little past the last are 32-bit too)
 
 // ------------------------------------------------------------------- lookup
 // 2^lshift lanes take a row, UNR chunks in flight a lane.
@@ -656,12 +657,17 @@ Plan plan_of(int dtype, int T, int V, int C) {
     return p;
 }
 
+int64_t fwd_blocks(int dtype, int T, int C) {
+    const int rows = kNT >> lane_shift((C - 1) / (dtype == FG_DTYPE_F32 ? 4 : 8) + 1);
+    return ((int64_t)T + rows - 1) / rows;
+}
+
 template <int DT>
 int launch_fwd(fg_ctx *ctx, const uint32_t *tokens, int T, int V, int C, const void *table, int ldt,
                float scale, void *out, int ldo) {
     using Ty = typename Io<DT>::T;
-    const int lshift = lane_shift((C - 1) / Io<DT>::E + 1), rows = kNT >> lshift;
-    emb_fwd<DT><<<(T - 1) / rows + 1, kNT, 0, ctx->stream>>>(
+    const int lshift = lane_shift((C - 1) / Io<DT>::E + 1);
+    emb_fwd<DT><<<(unsigned)fwd_blocks(DT, T, C), kNT, 0, ctx->stream>>>(
         tokens, T, V, C, static_cast<const Ty *>(table), ldt, scale, static_cast<Ty *>(out), ldo,
         lshift);
     FG_LAUNCH_CHECK("emb_fwd");
@@ -798,6 +804,8 @@ FG_API int fg_embedding(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T,
                C);
     FG_REQUIRE(T == 0 || (d_tokens && d_table && d_out), FG_ERR_INVALID_ARGUMENT,
                "%s: tokens, table and out are required", who);
+    FG_REQUIRE(fg::rows::grid_holds(fwd_blocks(dtype, T, C), kNT), FG_ERR_OUT_OF_BOUNDS,
+               "%s: %d rows of %d columns", who, T, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     if (T == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
@@ -817,6 +825,8 @@ FG_API int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, in
                C);
     FG_REQUIRE(C <= fg::rows::kMaxCols, FG_ERR_OUT_OF_BOUNDS, "%s: %d columns, at most %d", who, C,
                fg::rows::kMaxCols);
+    FG_REQUIRE(T <= kMaxTokens, FG_ERR_OUT_OF_BOUNDS, "%s: %d tokens, at most %d", who, T,
+               kMaxTokens);
     FG_REQUIRE(lddo >= C && lddt >= C, FG_ERR_SHAPE, "%s: lddo=%d or lddt=%d < C=%d", who, lddo,
                lddt, C);
     FG_REQUIRE(d_dtable && (T == 0 || (d_tokens && d_dout)), FG_ERR_INVALID_ARGUMENT,

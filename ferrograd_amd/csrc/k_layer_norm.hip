@@ -1063,6 +1063,11 @@ int launch_bwd_few(fg_ctx *ctx, const void *x, int ldx, const void *dy, int lddy
     return FG_OK;
 }
 
+// Rows that registers do not hold two of take a workgroup each, of 1024 threads at most.
+bool rows_fit(int dtype, int R, int C) {
+    return C / (dtype == FG_DTYPE_F32 ? 4 : 8) <= 1024 || fg::rows::grid_holds(R, 1024);
+}
+
 }  // namespace
 
 namespace fg {
@@ -1092,6 +1097,7 @@ FG_API int fg_layer_norm(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const
     FG_REQUIRE(eps > 0.0f && eps < INFINITY, FG_ERR_INVALID_ARGUMENT,
                "%s: eps must be positive and finite", who);
     FG_REQUIRE(d_x && d_y, FG_ERR_INVALID_ARGUMENT, "%s: x and y are required", who);
+    FG_REQUIRE(rows_fit(dtype, R, C), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns", who, R, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
@@ -1120,6 +1126,7 @@ FG_API int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, c
                "%s: ldx=%d, lddy=%d or lddx=%d < C=%d", who, ldx, lddy, lddx, C);
     FG_REQUIRE(d_x && d_dy && d_mean && d_rstd, FG_ERR_INVALID_ARGUMENT,
                "%s: x, dy, mean and rstd are required", who);
+    FG_REQUIRE(rows_fit(dtype, R, C), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns", who, R, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     FG_HIP(hipSetDevice(ctx->device));
     if (R > 0 && R <= kFewRows) {

@@ -305,7 +305,8 @@ int fg_softmax_bwd(fg_ctx *ctx, int dtype, const void *d_y, const void *d_dy, in
                    int C, void *d_dx, int accumulate);
 
 /* -------------------------------------------------- token-model operators */
-/* The following take rows of any alignment and of up to 2^24 columns.  Calls
+/* The following take rows of any alignment and of up to 2^23 columns; rows so
+ * many and so long that a grid cannot hold them (2^32 threads) are out of bounds.  Calls
  * that use the workspace share it with the context's other direct calls, in
  * the stream's order: graphs captured on one context must not run at the same
  * time. */

@@ -8,7 +8,7 @@ from ferrograd_amd import _lib
 
 P = 4096  # a non-NULL pointer; nothing may read it
 INVALID, SHAPE, BOUNDS = 1, 5, 9
-BIG = (1 << 24) + 1  # columns: one more than any of these takes
+BIG = (1 << 23) + 1  # columns: one more than any of these takes
 NAN, INF = float("nan"), float("inf")
 
 # name -> (argument names, a call that only lacks its context)
@@ -32,7 +32,14 @@ CALLS = {
                                 lddw=8, dbias=P, acc=0),
 }
 
+MANY = (1 << 31) - 1  # rows
+
 REFUSED = [
+    ("fg_layer_norm", dict(R=MANY, C=8200, ldx=8200, ldy=8200), BOUNDS),
+    ("fg_layer_norm_bwd", dict(R=MANY, C=8200, ldx=8200, lddy=8200, lddx=8200), BOUNDS),
+    ("fg_embedding", dict(T=MANY, C=2048, ldt=2048, ldo=2048), BOUNDS),
+    ("fg_embedding_bwd", dict(T=(1 << 30) + 1), BOUNDS),
+    ("fg_ckpt8_load", dict(R=MANY, C=4096, ldq=4096, lde=128, ldz=4096, ldh=4096), BOUNDS),
     ("fg_layer_norm", dict(C=BIG, ldx=BIG, ldy=BIG), BOUNDS),
     ("fg_layer_norm_bwd", dict(C=BIG, ldx=BIG, lddy=BIG, lddx=BIG), BOUNDS),
     ("fg_embedding", dict(C=BIG, ldt=BIG, ldo=BIG), BOUNDS),
