@@ -39,11 +39,9 @@ __all__ = [
 
 def _ptr(x) -> Optional[int]:
     """Device address of x: None, an int address, or an object with data_ptr()."""
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or isinstance(x, int):
         return x
-    return int(x.data_ptr())
+    return x.data_ptr()
 
 
 class Context:

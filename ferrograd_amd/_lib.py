@@ -194,4 +194,6 @@ def check(rc: int) -> None:
 
 def call(name: str, *args):
     """Call ``name`` and raise FgError on a non-zero status."""
-    check(getattr(load(), name)(*args))
+    rc = getattr(_lib or load(), name)(*args)
+    if rc:
+        check(rc)
