@@ -38,7 +38,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNT = 256;
 constexpr int kDirectMax = 256;
-constexpr int kRankMax = 14336;
+constexpr int64_t kOrderReads = 10 << 20;
 constexpr int kUnitBlocks = 1024;
 constexpr int kMaxTokens = 1 << 30;  // (positions a little past the last are 32-bit too)
 
@@ -179,61 +179,115 @@ __device__ __forceinline__ void zero_rows(const Zero &z, int block, int blocks) 
 }
 
 // ------------------------------------------------------------------- sorting
-// order[k] = the k-th position in (token, position) order, sorted[k] its token: a
-// lane counts the positions before its own; 16 waves take a share of the tokens
-// each, 64 at a time in scalar registers, so that a comparison and an addition with
-// carry are all a lane does for a token: bound by the vector unit, 8192 tokens 11.7 us,
-// 16384 21.3 (the radix sort about 24 from there to 65536).  [a < b] as a subtraction
-// that stops at 0, bounded by 1 and added two at a time, which waits for no result in
-// a scalar register, took as long.
-typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
-typedef u32x16 u32x16_any __attribute__((aligned(4)));
-__global__ __launch_bounds__(1024) void emb_rank(const uint32_t *__restrict__ tokens, int T,
-                                                 uint32_t *__restrict__ order,
-                                                 uint32_t *__restrict__ sorted, int blocks,
-                                                 const Zero z) {
-    __shared__ int sum[16][64];
+// order[k] = the k-th position in (token, position) order, sorted[k] its token: each
+// workgroup owns `bins` tokens and reads all of the batch.  Its waves take a run of
+// positions each and count the tokens below the workgroup's and each of its own; the
+// counts' prefix sums, by token and then by wave, are where a second reading places
+// the workgroup's positions.  64 positions that hold none of its tokens, as most do,
+// cost two comparisons.  Tokens outside the table sort as V.
+constexpr int kOrderNT = 1024, kOrderWaves = kOrderNT / 64;
+constexpr int kOrderBlocks = 256, kOrderBins = 1024;  // at least; at most
+__global__ __launch_bounds__(kOrderNT) void emb_order(const uint32_t *__restrict__ tokens, int T,
+                                                      uint32_t V, int bins,
+                                                      uint32_t *__restrict__ order,
+                                                      uint32_t *__restrict__ sorted, int blocks,
+                                                      const Zero z) {
+    __shared__ uint32_t cnt[kOrderWaves * kOrderBins];  // [wave][bins]
+    __shared__ uint32_t wbelow[kOrderWaves], wsum[kOrderWaves];
     if ((int)blockIdx.x >= blocks) {
         zero_rows(z, blockIdx.x - blocks, gridDim.x - blocks);
         return;
     }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g0 = blockIdx.x * 64, i = g0 + lane;
-    const uint32_t mine = i < T ? tokens[i] : 0xffffffffu;
-    const int per = ((T + 15) / 16 + 63) & ~63, j0 = wave * per, j1 = min(T, j0 + per);
-    int before = 0, j = j0;
-    // Equal tokens count where they lie before the workgroup's 64 positions, and not
-    // after them; the 64 themselves are in wave 0's lanes.
-    auto count = [&](int end, auto counts) {
-        for (; j + 64 <= end; j += 64) {
-            u32x16 o[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                o[q] = *reinterpret_cast<const u32x16_any *>(tokens + j + 16 * q);
-#pragma unroll
-            for (int e = 0; e < 64; ++e) before += counts(o[e / 16][e % 16]);
+    const uint32_t v0 = blockIdx.x * (uint32_t)bins, n = min((uint32_t)bins, V + 1 - v0);
+    const int per = (((T - 1) / kOrderNT + 1) | 1) * 64, i0 = wave * per, i1 = min(T, i0 + per);
+    constexpr int kBatch = 8;  // loads of a lane in flight
+    uint32_t *mine = cnt + wave * bins;
+    // f(its bin, its lanes) for each of the workgroup's tokens of 64 positions, in some
+    // order.
+    auto each = [&](uint32_t d, auto f) {
+        uint64_t hits = __ballot(d < n);
+        while (hits) {
+            const uint32_t at =
+                (uint32_t)__builtin_amdgcn_readlane((int)d, __ffsll((long long)hits) - 1);
+            const uint64_t m = __ballot(d == at);
+            f(at, m);
+            hits &= ~m;
         }
-        for (; j < end; ++j) before += counts(tokens[j]);
     };
-    count(min(j1, g0), [&](uint32_t o) { return o <= mine; });
-    j = max(j, g0 + 64);
-    count(j1, [&](uint32_t o) { return o < mine; });
-    if (wave == 0) {
+    auto scan = [&](auto f) {
+        uint32_t next[kBatch];
+        auto load = [&](int i) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e) {
-            const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)mine, e);
-            before += o < mine || (o == mine && e < lane);
+            for (int u = 0; u < kBatch; ++u) next[u] = tokens[min(i + 64 * u + lane, T - 1)];
+        };
+        load(i0);
+        int i = i0;
+        for (; i + 64 * kBatch <= i1; i += 64 * kBatch) {
+            uint32_t key[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) key[u] = min(next[u], V);
+            load(i + 64 * kBatch);
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) f(key[u], i + 64 * u + lane);
         }
-    }
-    sum[wave][lane] = before;
-    __syncthreads();
-    if (wave == 0 && i < T) {
-        before = 0;
 #pragma unroll
-        for (int w = 0; w < 16; ++w) before += sum[w][lane];
-        order[before] = (uint32_t)i;
-        sorted[before] = mine;
+        for (int u = 0; u < kBatch; ++u) {
+            const int at = i + 64 * u + lane;
+            if (i + 64 * u < i1) f(at < i1 ? min(next[u], V) : 0xffffffffu, at);
+        }
+    };
+    for (int d = threadIdx.x; d < kOrderWaves * bins; d += kOrderNT) cnt[d] = 0;
+    __syncthreads();
+    uint32_t below = 0;
+    scan([&](uint32_t key, int) {
+        below += (uint32_t)__popcll(__ballot(key < v0));
+        each(key - v0, [&](uint32_t own, uint64_t m) {
+            if (key - v0 == own && !(m & ((1ull << lane) - 1)))  // (one lane)
+                atomicAdd(&mine[own], (uint32_t)__popcll(m));
+        });
+    });
+    if (lane == 0) wbelow[wave] = below;
+    __syncthreads();
+    // A thread a bin.
+    uint32_t total = 0;
+    const uint32_t bin = threadIdx.x;
+    if (bin < n)
+        for (int w = 0; w < kOrderWaves; ++w) total += cnt[w * bins + bin];
+    uint32_t incl = total;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = __shfl_up(incl, o);
+        if (lane >= o) incl += up;
     }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    uint32_t at = incl - total, all = 0;
+    for (int w = 0; w < kOrderWaves; ++w) {
+        at += wbelow[w] + (w < wave ? wsum[w] : 0u);
+        all += wsum[w];
+    }
+    if (all == 0) return;
+    if (bin < n)
+        for (int w = 0; w < kOrderWaves; ++w) {
+            const uint32_t c = cnt[w * bins + bin];
+            cnt[w * bins + bin] = at;
+            at += c;
+        }
+    __syncthreads();
+    scan([&](uint32_t key, int i) {
+        const uint32_t d = key - v0;
+        each(d, [&](uint32_t own, uint64_t m) {
+            uint32_t to = 0;
+            if (lane == 0) to = atomicAdd(&mine[own], (uint32_t)__popcll(m));
+            to = (uint32_t)__builtin_amdgcn_readfirstlane((int)to);
+            if (d == own) {
+                to += (uint32_t)__popcll(m & ((1ull << lane) - 1));
+                order[to] = (uint32_t)i;
+                sorted[to] = key;
+            }
+        });
+    });
 }
 
 // Stable radix sort, least significant digit first, of (token, position) pairs:
@@ -559,49 +613,54 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
     }
 }
 
-// Joins the partial sums of the run that begins in unit blockIdx.x and goes on after
-// it (if one does): 4 columns a lane, 2^jshift lanes across the columns, and the
-// workgroup's other lanes and waves a share of the run's units each.
-constexpr int kJoinNT = 256;
+// Joins the partial sums of a run that crosses units, 4 columns a lane.  Of a run of n
+// units, the first S take a share of the columns each (S = 1 up to 16 units, so that a
+// lane has one batch of loads), and in them S groups of lanes a share of the units each,
+// added in order.  blockIdx.x: a unit but the last, blockIdx.y: 1024 columns.
+constexpr int kJoinNT = 256, kJoinShare = 16;
 template <int DT>
-__global__ __launch_bounds__(kJoinNT) void emb_join(const Sums p, typename Io<DT>::T *dtable,
-                                                    int jshift) {
+__global__ __launch_bounds__(kJoinNT) void emb_join(const Sums p, typename Io<DT>::T *dtable) {
     using IO = Io<DT>;
     __shared__ f32x4 sh[kJoinNT];
-    const int u0 = blockIdx.x, k0 = u0 * p.P, k1 = k0 + p.P;  // (k1 < T: the last unit joins nothing)
-    const int lane = threadIdx.x & 63;
-    const uint32_t v = p.sorted[k1 - 1], first = p.sorted[k0], prev = p.sorted[max(k0 - 1, 0)];
-    // Units after u0 that begin with v, 64 at a time (the first of them beside the
-    // loads above).
-    int n = 1;
-    for (;;) {
-        const int64_t at = (int64_t)(u0 + n + lane) * p.P;
-        const uint64_t on = __ballot(at < p.T && p.sorted[at < p.T ? at : 0] == v);
-        const int c = on == ~0ull ? 64 : __ffsll((long long)~on) - 1;
-        n += c;
-        if (n == 1 || v >= (uint32_t)p.V || (k0 > 0 && first == v && prev == v)) return;
-        if (c < 64) break;
-    }
-    const int lanes = 1 << jshift, splits = kJoinNT >> jshift;
-    const int64_t col = ((int64_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1))) * 4;
-    const int split = threadIdx.x >> jshift, per = (n + splits - 1) / splits;
+    const int u = blockIdx.x, lane = threadIdx.x & 63;
+    const int64_t after = (int64_t)(u + 1 + lane) * p.P, before = (int64_t)(u - lane) * p.P - 1;
+    const uint32_t v = p.sorted[(u + 1) * p.P - 1];
+    // Units after u, and before it, that hold v as well: u's row of them, up to 64.
+    auto ones = [](uint64_t m) { return m == ~0ull ? 64 : __ffsll((long long)~m) - 1; };
+    const uint64_t on = __ballot(p.sorted[after < p.T ? after : 0] == v && after < p.T);
+    const uint64_t back = __ballot(p.sorted[before > 0 ? before : 0] == v && before >= 0);
+    int c = ones(on);
+    const int b = ones(back);
+    if (c == 0 || v >= (uint32_t)p.V || b == 64) return;
+    if (c == 64) c = (wave_lower_bound(p.sorted, p.T, v + 1) - 1) / p.P - u;
+    const int u0 = u - b, n = b + 1 + c;
+    int sshift = 0;
+    while (sshift < 6 && (kJoinShare << sshift) < n) ++sshift;
+    if (b >> sshift) return;
+    const int lshift = 8 - sshift, split = threadIdx.x >> lshift;
+    const int per = (n + (1 << sshift) - 1) >> sshift;
+    const int64_t col = ((int64_t)blockIdx.y * kJoinNT + (b << lshift) +
+                         (threadIdx.x & ((1 << lshift) - 1))) * 4;
     f32x4 a = {0.f, 0.f, 0.f, 0.f};
     if (col < p.Cp) {
-        int b = split * per;
-        const int end = min(n, b + per);
-        const float *at = p.partial + ((size_t)u0 * 2) * p.Cp + col;
-        if (b == 0) {
+        int k = split * per;
+        const int end = min(n, k + per);
+        const float *at = p.partial + (size_t)u0 * 2 * p.Cp + col;
+        if (k == 0) {
             a = *reinterpret_cast<const f32x4 *>(at + p.Cp);
-            ++b;
+            ++k;
         }
 #pragma unroll 16
-        for (; b < end; ++b) a += *reinterpret_cast<const f32x4 *>(at + (size_t)b * 2 * p.Cp);
+        for (; k < end; ++k) a += *reinterpret_cast<const f32x4 *>(at + (size_t)k * 2 * p.Cp);
     }
-    sh[threadIdx.x] = a;
-    __syncthreads();
-    if (split != 0 || col >= p.Cp) return;
-    const int used = min(splits, (n - 1) / per + 1);
-    for (int w = 1; w < used; ++w) a += sh[threadIdx.x + (w << jshift)];
+    if (sshift) {
+        sh[threadIdx.x] = a;
+        __syncthreads();
+        if (split != 0) return;
+        const int used = (n - 1) / per + 1;
+        for (int w = 1; w < used; ++w) a += sh[threadIdx.x + (w << lshift)];
+    }
+    if (col >= p.Cp) return;
     auto *to = dtable + (size_t)v * p.lddt;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -624,7 +683,8 @@ int lane_shift(int chunks) { return std::min(8, log2_up(chunks)); }
 struct Plan {
     int P, units, lshift;
     int64_t Cp;
-    int passes, bits, tiles, per;  // of the radix sort (passes 0: by counting)
+    int bins, blocks;              // of emb_order
+    int passes, bits, tiles, per;  // of the radix sort (passes 0: emb_order)
     uint64_t sort_words, hist_words, partial_floats;
     uint64_t bytes() const {
         return 4 * (sort_words + hist_words) + 16 + 4 * partial_floats;
@@ -645,7 +705,9 @@ Plan plan_of(int dtype, int T, int V, int C) {
     p.units = (T - 1) / p.P + 1;
     p.partial_floats = (uint64_t)p.units * 2 * (uint64_t)p.Cp;
     p.sort_words = 2 * (uint64_t)T;
-    if (T > kRankMax) {
+    p.bins = std::min(kOrderBins, V / kOrderBlocks + 1);  // (of keys 0 .. V)
+    p.blocks = V / p.bins + 1;
+    if ((int64_t)p.blocks * T > kOrderReads) {
         const int need = std::max(1, log2_up((int64_t)V + 1));  // of keys 0 .. V
         p.passes = (need - 1) / kMaxBits + 1;
         p.bits = (need - 1) / p.passes + 1;
@@ -697,8 +759,8 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
     // written again.  The rest goes beside the sums, without the rows of tokens.
     constexpr double kMB = 1 << 20;
     const double row_mb = (double)C * sizeof(Ty) / kMB, q = T / 8192.0;
-    const double count_mb = 16.0, place_mb = 60.0, rank_mb = 12.0 + 40.0 * q * q;
-    const double sort_mb = pl.passes ? pl.passes * (count_mb + place_mb) : rank_mb;
+    const double count_mb = 16.0, place_mb = 60.0, order_mb = 20.0 + 30.0 * q;
+    const double sort_mb = pl.passes ? pl.passes * (count_mb + place_mb) : order_mb;
     int early = 0, done = 0;  // rows zeroed beside the sort; by the launches so far
     if (!accumulate) {
         const bool all = V * row_mb < 1.25 * sort_mb || T <= V / 8;
@@ -715,9 +777,10 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
         return z.count ? std::min(64 * ctx->cu_count, (z.count - 1) / per + 1) : 0;
     };
     if (pl.passes == 0) {
-        const int blocks = (T - 1) / 64 + 1, zeros = share(rank_mb);
-        emb_rank<<<blocks + zeros, 1024, 0, st>>>(tokens, T, order, sorted, blocks, z);
-        FG_LAUNCH_CHECK("emb_rank");
+        const int zeros = share(order_mb);
+        emb_order<<<pl.blocks + zeros, kOrderNT, 0, st>>>(tokens, T, (uint32_t)V, pl.bins, order,
+                                                          sorted, pl.blocks, z);
+        FG_LAUNCH_CHECK("emb_order");
     } else {
         // The passes go back and forth between two pairs of arrays and end in the first.
         uint32_t *pos[2] = {order, order + 2 * (size_t)T};
@@ -770,9 +833,8 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
     sums<<<dim3(blocks, tiles), kNT, 0, st>>>(s, d, g);
     FG_LAUNCH_CHECK("emb_sums");
     if (pl.units > 1) {
-        const int jshift = std::min(6, log2_up(pl.Cp / 4));
-        emb_join<DT><<<dim3(pl.units - 1, (unsigned)(((pl.Cp / 4 - 1) >> jshift) + 1)), kJoinNT, 0,
-                       st>>>(s, g, jshift);
+        emb_join<DT><<<dim3(pl.units - 1, (unsigned)((pl.Cp / 4 - 1) / kJoinNT + 1)), kJoinNT, 0,
+                       st>>>(s, g);
         FG_LAUNCH_CHECK("emb_join");
     }
     return FG_OK;
