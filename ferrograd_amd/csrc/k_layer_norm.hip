@@ -21,7 +21,6 @@
 
 namespace {
 
-using fg::rows::Chunk;
 using fg::rows::Io;
 using fg::rows::u32x4;
 
@@ -750,10 +749,11 @@ __global__ __launch_bounds__(kLongL) void ln_bwd_long(
 }
 
 // Few rows (kFewRows), where launches count: one for everything, workgroups of one
-// row for dx, and behind them workgroups of 64 chunks of columns for the weights,
-// whose waves take every 16th row and are added in order.  64 x 4096 bf16 10.4 us in
-// two launches, now 7.3.
-constexpr int kFewRows = 128;
+// row for dx, and behind them workgroups of 16 chunks of columns for the weights,
+// whose 64 groups of lanes take every 64th row and are added in order.  bf16, in two
+// launches as below and in this one: 64 x 4096 9.1 us and 6.2, 256 x 16384 22.5 and
+// 12.2; with 512 rows fp32 of 4096 12.1 and 14.9, 512 x 512 8.9 and 9.2.
+constexpr int kFewRows = 256, kFewLanes = 16, kFewGroups = kLongL / kFewLanes;
 template <int DT>
 __global__ __launch_bounds__(kLongL) void ln_bwd_few(
     const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
@@ -761,25 +761,25 @@ __global__ __launch_bounds__(kLongL) void ln_bwd_few(
     typename Io<DT>::T *dx, int lddx, int accumulate, void *dgamma, int acc_g, void *dbeta,
     int acc_b, int row_blocks) {
     using IO = Io<DT>;
-    constexpr int E = IO::E, kWaves = kLongL / 64;
-    __shared__ float sm[2][kWaves];
-    __shared__ float sh[kWaves][64 * E];
+    constexpr int E = IO::E, kCols = kFewLanes * E;
+    __shared__ float sm[2][kLongL / 64];
+    __shared__ float sh[kFewGroups][kCols];
     if ((int)blockIdx.x < row_blocks) {
         bwd_long_row<DT>(blockIdx.x, x, ldx, dy, lddy, gamma, mean, rstd, C, dx, lddx, accumulate,
                          sm);
         return;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int j = ((int)blockIdx.x - row_blocks) * 64 + lane;
-    const int nb = C / E, chunks = (C - 1) / E + 1;
+    const int lane = threadIdx.x % kFewLanes, group = threadIdx.x / kFewLanes;
+    const int strip = (int)blockIdx.x - row_blocks, j = strip * kFewLanes + lane;
+    const int nb = C / E;  // (the columns past the last whole chunk, one to a lane after it)
     float ag[E], ab[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) ag[e] = ab[e] = 0.0f;
-    if (j < chunks) {
+    if (j < nb) {
 #pragma unroll 4
-        for (int r = wave; r < R; r += kWaves) {
-            const u32x4 wx = Chunk<DT>::load(x + (size_t)r * ldx, j, nb, C);
-            const u32x4 wd = Chunk<DT>::load(dy + (size_t)r * lddy, j, nb, C);
+        for (int r = group; r < R; r += kFewGroups) {
+            const u32x4 wx = fg::rows::load<DT>(x + (size_t)r * ldx, j);
+            const u32x4 wd = fg::rows::load<DT>(dy + (size_t)r * lddy, j);
             const float m = mean[r], k = rstd[r];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -788,17 +788,27 @@ __global__ __launch_bounds__(kLongL) void ln_bwd_few(
                 ab[e] += d;
             }
         }
+    } else if (nb * E + (j - nb) < C) {
+        const int col = nb * E + (j - nb);
+#pragma unroll 4
+        for (int r = group; r < R; r += kFewGroups) {
+            const float d = IO::load1(dy + (size_t)r * lddy, col);
+            ag[0] += d * rstd[r] * (IO::load1(x + (size_t)r * ldx, col) - mean[r]);
+            ab[0] += d;
+        }
     }
-    // The waves' sums in order, a column a thread.
+    // The groups' sums in order, a column a thread.
     auto add = [&](const float (&a)[E], void *out, int acc) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) sh[wave][lane * E + e] = a[e];
+        for (int e = 0; e < E; ++e) sh[group][lane * E + e] = a[e];
         __syncthreads();
-        const int64_t col = (int64_t)((int)blockIdx.x - row_blocks) * 64 * E + threadIdx.x;
-        if ((int)threadIdx.x < 64 * E && col < C && out) {
+        const int at = strip * kFewLanes + (int)threadIdx.x / E, e = threadIdx.x % E;
+        const int col = at < nb ? at * E + e : e == 0 ? nb * E + (at - nb) : C;
+        if ((int)threadIdx.x < kCols && col < C && out) {
             float s = sh[0][threadIdx.x];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) s += sh[w][threadIdx.x];
+            const int used = min(kFewGroups, R);
+#pragma unroll 8
+            for (int g = 1; g < used; ++g) s += sh[g][threadIdx.x];
             fg::store_from_f(out, DT, col, acc ? fg::load_as_f(out, DT, col) + s : s);
         }
         __syncthreads();
@@ -856,9 +866,10 @@ __global__ __launch_bounds__(kColsNT) void ln_bwd_cols(const typename Io<DT>::T 
     }
 }
 
-// Adds the partial sums of each column: 16 threads a column, each a run of them in
-// order, then the 16 in order.
-constexpr int kFinalCols = 64, kFinalGroups = 16;
+// Adds the partial sums of each column: 32 threads a column, each a run of them in
+// order, then the 32 in order (64 columns of 16 threads: half the workgroups, 0.2 to
+// 0.5 us longer).
+constexpr int kFinalCols = 32, kFinalGroups = 32;
 __global__ __launch_bounds__(kFinalCols *kFinalGroups) void ln_bwd_final(
     int dt, const float *__restrict__ partial, int splits, int C, void *dgamma, int acc_g,
     void *dbeta, int acc_b) {
@@ -1047,7 +1058,7 @@ int launch_bwd_few(fg_ctx *ctx, const void *x, int ldx, const void *dy, int lddy
                    int lddx, int accumulate, void *dgamma, int acc_g, void *dbeta, int acc_b) {
     using T = typename Io<DT>::T;
     const int row_blocks = dx ? R : 0;
-    const int strips = dgamma || dbeta ? ((C - 1) / Io<DT>::E) / 64 + 1 : 0;
+    const int strips = dgamma || dbeta ? (C / Io<DT>::E + C % Io<DT>::E - 1) / kFewLanes + 1 : 0;
     auto launch = [&](int rows, int cols) {
         if (rows + cols == 0) return;
         ln_bwd_few<DT><<<rows + cols, kLongL, 0, ctx->stream>>>(
