@@ -475,40 +475,56 @@ __global__ __launch_bounds__(L *NG) void ln_bwd(
     }
 }
 
-// The same for rows whose weight gradients leave no room for a second row's loads:
-// x and dy stay packed, gamma comes from the caches.
+// The same for rows whose weight gradients leave no registers for a second row's loads:
+// their sums are in LDS, 16 bytes a lane in each access, x and dy stay packed, gamma
+// comes from the caches.
 template <int DT, int NV>
 __global__ __launch_bounds__(1024) void ln_bwd_wide(
     const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
     const typename Io<DT>::T *__restrict__ gamma, const float *mean, const float *rstd, int R,
     int C, typename Io<DT>::T *dx, int lddx, int accumulate, float *partial) {
     using IO = Io<DT>;
-    constexpr int E = IO::E, L = 1024;
+    constexpr int E = IO::E, L = 1024, Q = E / 4;
     __shared__ float sm[2][2][L / 64];
+    __shared__ f32x4 acc[NV][2][Q][L];  // a lane's own
     const int t = threadIdx.x;
     const Lanes<DT> ln(C, t);
     const bool one = ln.single < C;
     const float n = (float)C;
     const u32x4 zero = {0u, 0u, 0u, 0u};
-    float ag[NV][E], ab[NV][E], ag1 = 0.0f, ab1 = 0.0f;
+    float ag1 = 0.0f, ab1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < E; ++e) ag[i][e] = ab[i][e] = 0.0f;
+        for (int q = 0; q < Q; ++q) acc[i][0][q][t] = acc[i][1][q][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float g1 = gamma && one ? IO::load1(gamma, ln.single) : 1.0f;
     const uint32_t rows = R;
-    for (uint32_t row = blockIdx.x, it = 0; row < rows; row += gridDim.x, ++it) {
+    u32x4 nx[NV], nd[NV];
+    float nx1, nd1, nm, nk;
+    auto fetch = [&](uint32_t row) {
         const auto *xr = x + (size_t)row * ldx, *dr = dy + (size_t)row * lddy;
-        u32x4 wx[NV], wd[NV];
+        nm = mean[row];
+        nk = rstd[row];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const bool mine = t + i * L < ln.nb;
-            wx[i] = mine ? fg::rows::load<DT>(xr, t + i * L) : zero;
-            wd[i] = mine ? fg::rows::load<DT>(dr, t + i * L) : zero;
+            nx[i] = mine ? fg::rows::load<DT>(xr, t + i * L) : zero;
+            nd[i] = mine ? fg::rows::load<DT>(dr, t + i * L) : zero;
         }
-        const float m = mean[row], k = rstd[row];
-        const float c1 = (one ? IO::load1(xr, ln.single) : 0.0f) - m;
-        const float d1 = one ? IO::load1(dr, ln.single) : 0.0f, gd1 = d1 * g1;
+        nx1 = one ? IO::load1(xr, ln.single) : 0.0f;
+        nd1 = one ? IO::load1(dr, ln.single) : 0.0f;
+    };
+    uint32_t row = blockIdx.x;
+    fetch(row);  // (no workgroup without a row)
+    for (uint32_t it = 0; row < rows; row += gridDim.x, ++it) {
+        u32x4 wx[NV], wd[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            wx[i] = nx[i];
+            wd[i] = nd[i];
+        }
+        const float m = nm, k = nk, c1 = nx1 - m, d1 = nd1, gd1 = d1 * g1;
+        if (row + gridDim.x < rows) fetch(row + gridDim.x);
         float s1 = gd1, s2 = gd1 * c1;
         ag1 += d1 * k * c1;
         ab1 += d1;
@@ -518,13 +534,20 @@ __global__ __launch_bounds__(1024) void ln_bwd_wide(
             if (gamma && t + i * L < ln.nb) g = fg::rows::load<DT>(gamma, t + i * L);
             float p1 = 0.0f, p2 = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float d = IO::get(wd[i], e), c = IO::get(wx[i], e) - m;
-                const float gd = gamma ? d * IO::get(g, e) : d;
-                p1 += gd;
-                p2 += gd * c;
-                ag[i][e] += d * k * c;
-                ab[i][e] += d;
+            for (int q = 0; q < Q; ++q) {
+                f32x4 ag = acc[i][0][q][t], ab = acc[i][1][q][t];
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const int e = 4 * q + h;
+                    const float d = IO::get(wd[i], e), c = IO::get(wx[i], e) - m;
+                    const float gd = gamma ? d * IO::get(g, e) : d;
+                    p1 += gd;
+                    p2 += gd * c;
+                    ag[h] += d * k * c;
+                    ab[h] += d;
+                }
+                acc[i][0][q][t] = ag;
+                acc[i][1][q][t] = ab;
             }
             s1 += p1;
             s2 += p2;
@@ -581,12 +604,10 @@ __global__ __launch_bounds__(1024) void ln_bwd_wide(
         const int j = t + i * L;
         if (j >= ln.nb) continue;
 #pragma unroll
-        for (int q = 0; q < E / 4; ++q) {
+        for (int q = 0; q < Q; ++q) {
             float *to = part + (size_t)j * E + 4 * q;
-            *reinterpret_cast<f32x4 *>(to) =
-                f32x4{ag[i][4 * q], ag[i][4 * q + 1], ag[i][4 * q + 2], ag[i][4 * q + 3]};
-            *reinterpret_cast<f32x4 *>(to + Cp) =
-                f32x4{ab[i][4 * q], ab[i][4 * q + 1], ab[i][4 * q + 2], ab[i][4 * q + 3]};
+            *reinterpret_cast<f32x4 *>(to) = acc[i][0][q][t];
+            *reinterpret_cast<f32x4 *>(to + Cp) = acc[i][1][q][t];
         }
     }
     if (one) {
@@ -848,9 +869,10 @@ __global__ __launch_bounds__(kColsNT) void ln_bwd_cols(const typename Io<DT>::T 
             }
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            p[(size_t)j * E + e] = ag[e];
-            p[Cp + (size_t)j * E + e] = ab[e];
+        for (int q = 0; q < E; q += 4) {
+            float *to = p + (size_t)j * E + q;
+            *reinterpret_cast<f32x4 *>(to) = f32x4{ag[q], ag[q + 1], ag[q + 2], ag[q + 3]};
+            *reinterpret_cast<f32x4 *>(to + Cp) = f32x4{ab[q], ab[q + 1], ab[q + 2], ab[q + 3]};
         }
     } else if (nb * E + (j - nb) < C) {
         const int col = nb * E + (j - nb);
@@ -866,19 +888,18 @@ __global__ __launch_bounds__(kColsNT) void ln_bwd_cols(const typename Io<DT>::T 
     }
 }
 
-// Adds the partial sums of each column: 32 threads a column, each a run of them in
-// order, then the 32 in order (64 columns of 16 threads: half the workgroups, 0.2 to
-// 0.5 us longer).
-constexpr int kFinalCols = 32, kFinalGroups = 32;
-__global__ __launch_bounds__(kFinalCols *kFinalGroups) void ln_bwd_final(
+// Adds the partial sums of each column: GROUPS threads a column, each a run of them in
+// order, then the groups' sums in order.
+template <int COLS, int GROUPS>
+__global__ __launch_bounds__(COLS *GROUPS) void ln_bwd_final(
     int dt, const float *__restrict__ partial, int splits, int C, void *dgamma, int acc_g,
     void *dbeta, int acc_b) {
-    __shared__ float sh[kFinalGroups][kFinalCols];
-    const int c = threadIdx.x % kFinalCols, q = threadIdx.x / kFinalCols;
+    __shared__ float sh[GROUPS][COLS];
+    const int c = threadIdx.x % COLS, q = threadIdx.x / COLS;
     const int64_t Cp = padded(C), N = 2 * Cp;
-    const int64_t at = (int64_t)blockIdx.x * kFinalCols + c;
+    const int64_t at = (int64_t)blockIdx.x * COLS + c;
     const int64_t i = at < Cp ? at : at - Cp;
-    const int per = (splits + kFinalGroups - 1) / kFinalGroups;
+    const int per = (splits + GROUPS - 1) / GROUPS;
     int k = q * per;
     const int end = min(splits, k + per);
     const bool mine = at < N && i < C;
@@ -897,11 +918,13 @@ __global__ __launch_bounds__(kFinalCols *kFinalGroups) void ln_bwd_final(
     __syncthreads();
     if (q != 0 || !mine) return;
 #pragma unroll
-    for (int h = 1; h < kFinalGroups; ++h) s += sh[h][c];
+    for (int h = 1; h < GROUPS; ++h) s += sh[h][c];
     void *out = at < Cp ? dgamma : dbeta;
     if (!out) return;
     fg::store_from_f(out, dt, i, (at < Cp ? acc_g : acc_b) ? fg::load_as_f(out, dt, i) + s : s);
 }
+
+constexpr int kFewSums = 64;
 
 // ------------------------------------------------------------------ choices
 // Runs f<NV, L, NG>() for a row of `chunks` whole 16-byte chunks; false: longer
@@ -1163,9 +1186,16 @@ FG_API int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, c
             return rc;
     }
     if (partial) {
-        ln_bwd_final<<<(unsigned)((2 * padded(C) - 1) / kFinalCols + 1), kFinalCols * kFinalGroups,
-                       0, ctx->stream>>>(dtype, partial, s.splits, C, d_dgamma, dgamma_accumulate,
-                                         d_dbeta, dbeta_accumulate);
+        // 32 threads a column (half of them: 0.2 to 0.5 us longer), or 4 for few sums.
+        auto final = [&](auto cols, auto groups) {
+            ln_bwd_final<cols(), groups()>
+                <<<(unsigned)((2 * padded(C) - 1) / cols() + 1), cols() * groups(), 0,
+                   ctx->stream>>>(dtype, partial, s.splits, C, d_dgamma, dgamma_accumulate, d_dbeta,
+                                  dbeta_accumulate);
+        };
+        using std::integral_constant;
+        if (s.splits > kFewSums) final(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+        else final(integral_constant<int, 64>{}, integral_constant<int, 4>{});
         FG_LAUNCH_CHECK("ln_bwd_final");
     }
     return FG_OK;
