@@ -9,18 +9,22 @@
 // equal calls give equal bits (no atomics).  Tokens outside the table add to
 // nothing.
 //
-// Both are bound by HBM (the rows they read and write once).  The gradient:
-//  * the positions in (token, position) order: by counting, for each position, the
-//    ones before it (up to kRankMax tokens, one launch: T^2 / 64 two-instruction
-//    steps spread over all CUs), by a stable radix sort above;
+// Both are bound by HBM (the rows they read and write once): the lookup of 16384 rows
+// of 4096 in bf16 takes 32.5 us, 5.6 TB/s.  The gradient:
+//  * the positions in (token, position) order: one launch of workgroups that own
+//    tokens (up to kOrderReads reads), a stable radix sort above; table rows are zeroed
+//    beside either, which leave the memory idle;
 //  * the sorted positions in units of equal length, so that a token that fills half
 //    the batch is spread over the GPU as evenly as any other: a unit adds its runs
 //    of equal tokens, writes the rows of runs that it holds whole, and leaves the
 //    runs that cross its ends as fp32 partial sums; workgroups of the same launch
-//    zero the rows of no token;
+//    zero the rows of no token that are left;
 //  * the crossing runs' partial sums are joined in order.
+// 65536 tokens over 131072 rows of 2048 in bf16 (805 MB): sort 32 us, sums 137 at
+// 4.7 TB/s, joins 8.  20011 tokens, four in ten of them one, over 50257 rows of 777 in
+// fp32 (218 MB): order 25 with 93 MB of zeros, sums 25, joins 7.6.
 // A few tokens (kDirectMax) take one launch: every workgroup owns some table rows
-// and lists the tokens that are its own.
+// and lists the tokens that are its own (256 tokens over 1000 rows of 256: 3.8 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -37,8 +41,15 @@ using fg::rows::u32x4;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNT = 256;
-constexpr int kDirectMax = 256;
+constexpr int kDirectMax = 256;  // (a token a thread)
+// Tokens that all of emb_order's workgroups read: 40960 a workgroup where there are 256.
+// It takes 8.6 us for 8192 tokens, 15 for 16384, 22 for 32768 (as much again where zeros
+// share the CUs); the radix sort's launches 24 or more for any of these.  All of the
+// gradient, bf16, 32000 rows of 1024: 8192 tokens 25.7 us (radix sort 36.7), 16384 34.2
+// (45.0), 32768 47.9 (54.6); 40900 tokens over 131072 rows 73.7 (75.9).
 constexpr int64_t kOrderReads = 10 << 20;
+// Workgroups of units (with 512 and 2048: 65536 tokens, 131072 rows of 2048 in bf16 177.5
+// and 180.4 us, 177.1 with 1024; 20011 tokens, rows of 777 in fp32 67.4 and 60.6, 58.0).
 constexpr int kUnitBlocks = 1024;
 constexpr int kMaxTokens = 1 << 30;  // (positions a little past the last are 32-bit too)
 
@@ -757,6 +768,8 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
     // Zeroed beside the sort, which leaves the memory idle: what its launches have time
     // for; the whole table where that is most of it, or where few of its rows are
     // written again.  The rest goes beside the sums, without the rows of tokens.
+    // (emb_order, MB for 20011 and 32768 tokens: 34 and 50 68.3 and 86.3 us in all, 59
+    // and 90 60.0 and 79.7, 95 and 150 61.0 and 72.0, 142 and 220 70.0 and 77.0.)
     constexpr double kMB = 1 << 20;
     const double row_mb = (double)C * sizeof(Ty) / kMB, q = T / 8192.0;
     const double count_mb = 16.0, place_mb = 60.0, order_mb = 20.0 + 30.0 * q;

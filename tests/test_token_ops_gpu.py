@@ -198,7 +198,9 @@ def ln_bwd_reference(x, dy, gamma, mean, rstd):
 
 
 LN_BWD_SHAPES = LN_SHAPES + [(300, 1, 0, 0), (1031, 72, 0, 0), (2048, 520, 0, 0),
-                             (4099, 131, 5, 0), (515, 4096, 0, 0), (600, 9000, 0, 0)]
+                             (4099, 131, 5, 0), (515, 4096, 0, 0), (600, 9000, 0, 0),
+                             (129, 1000, 0, 0), (256, 4100, 4, 1), (257, 6001, 1, 0),
+                             (300, 16384, 0, 0), (1100, 17001, 0, 0)]
 
 
 @pytest.mark.parametrize("dt", DTS)
@@ -315,7 +317,8 @@ EMB_SHAPES = [  # T, V, C, pad, start
     (255, 50, 777, 0, 0), (256, 4096, 64, 0, 0), (1000, 17, 1024, 0, 0), (1024, 70000, 8, 0, 0),
     (3001, 1009, 130, 3, 0), (4096, 64, 512, 8, 0), (4097, 300, 2051, 0, 1), (9000, 32000, 96, 0, 0),
     (20011, 257, 48, 0, 0), (40000, 5000, 24, 0, 0), (70000, 131072, 16, 0, 0),
-    (131072, 3, 40, 0, 0), (300, 9, 8192, 0, 0), (50, 9, 20000, 0, 0)]
+    (131072, 3, 40, 0, 0), (300, 9, 8192, 0, 0), (50, 9, 20000, 0, 0), (257, 1, 24, 0, 0),
+    (2000, 255, 16, 0, 0), (2000, 256, 16, 0, 0), (3000, 262144, 8, 0, 0)]
 
 
 @pytest.mark.parametrize("dt", DTS)
