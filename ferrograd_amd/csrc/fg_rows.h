@@ -73,6 +73,57 @@ struct Chunk {
     }
 };
 
+// The same where a partial chunk may take columns of the one before it too: it is then
+// the row's last E columns, in one access, and both lanes that have a column must make
+// the same of it.  Rows of fewer than E columns go element by element.
+template <int DT>
+struct Tail {
+    using IO = Io<DT>;
+    static constexpr int E = IO::E;
+    int C, first;  // the lane's first column
+    bool whole;
+    __device__ __forceinline__ Tail(int j, int cols)
+        : C(cols), first(cols < E ? j * E : min(j * E, cols - E)), whole(cols >= E) {}
+    __device__ __forceinline__ uint32_t bytes() const {
+        return (uint32_t)first * (uint32_t)sizeof(typename IO::T);
+    }
+    __device__ __forceinline__ u32x4 load(const typename IO::T *row) const {
+        if (whole)
+            return *reinterpret_cast<const u32x4_any *>(reinterpret_cast<const char *>(row) +
+                                                        bytes());
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = e < C ? IO::load1(row, e) : 0.0f;
+        return IO::pack(v);
+    }
+    __device__ __forceinline__ void store(typename IO::T *row, const float (&v)[E]) const {
+        if (whole) {
+            __builtin_nontemporal_store(
+                IO::pack(v),
+                reinterpret_cast<u32x4_any *>(reinterpret_cast<char *>(row) + bytes()));
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (e < C) IO::store1(row, e, v[e]);
+    }
+    // Adds v to the row: columns of the chunk before j's are its lane's.
+    __device__ __forceinline__ void add(typename IO::T *row, int j, const float (&v)[E]) const {
+        if (first == j * E && whole) {
+            const u32x4 was = load(row);
+            float o[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[e] = v[e] + IO::get(was, e);
+            store(row, o);
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (first + e >= j * E && first + e < C)
+                IO::store1(row, first + e, v[e] + IO::load1(row, first + e));
+    }
+};
+
 // Sum over a wave's 64 lanes (all active), the same in every lane: the 16-lane
 // rows by DPP, then the four rows' sums.
 __device__ __forceinline__ float wave_sum(float s) {

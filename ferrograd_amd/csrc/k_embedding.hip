@@ -35,10 +35,11 @@
 
 namespace {
 
-using fg::rows::Chunk;
 using fg::rows::Io;
+using fg::rows::Tail;
 using fg::rows::u32x4;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
 constexpr int kNT = 256;
 constexpr int kDirectMax = 256;  // (a token a thread)
@@ -71,21 +72,33 @@ __global__ __launch_bounds__(kNT) void emb_fwd(const uint32_t *__restrict__ toke
     auto *to = out + (size_t)t * ldo;
     const float k = in ? scale : __builtin_nanf("");
     const int nb = C / E, chunks = (C - 1) / E + 1;
-    auto put = [&](int j, u32x4 w) {
-        float o[E];
+    // (The product is rounded to fp32 and then to the type, here and in the oracle: kept
+    // apart, or the compiler makes one rounding of both in one of the loops, and lanes
+    // that share a column could differ.)
+    auto out_of = [&](u32x4 w, float (&o)[E]) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = in ? k * IO::get(w, e) : k;
-        Chunk<DT>::store(to, j, nb, C, o);
+        for (int e = 0; e < E; ++e) {
+            o[e] = in ? k * IO::get(w, e) : k;
+            asm("" : "+v"(o[e]));
+        }
     };
     int j = lane;
+    float o[E];
     for (; j + (UNR - 1) * lanes < nb; j += UNR * lanes) {
         u32x4 w[UNR];
 #pragma unroll
         for (int u = 0; u < UNR; ++u) w[u] = fg::rows::load<DT>(row, j + u * lanes);
 #pragma unroll
-        for (int u = 0; u < UNR; ++u) put(j + u * lanes, w[u]);
+        for (int u = 0; u < UNR; ++u) {
+            out_of(w[u], o);
+            fg::rows::store<DT>(to, j + u * lanes, IO::pack(o));
+        }
     }
-    for (; j < chunks; j += lanes) put(j, Chunk<DT>::load(row, j, nb, C));
+    for (; j < chunks; j += lanes) {
+        const Tail<DT> tail(j, C);
+        out_of(tail.load(row), o);
+        tail.store(to, o);
+    }
 }
 
 // --------------------------------------------------- few tokens: one launch
@@ -125,7 +138,7 @@ __global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ 
         at[k] = threadIdx.x;
     }
     __syncthreads();
-    const int nb = C / E, chunks = (C - 1) / E + 1;
+    const int chunks = (C - 1) / E + 1;
     for (int r = threadIdx.x >> lshift; r < nrows; r += kNT >> lshift) {
         const uint32_t v = (uint32_t)(v0 + r);
         auto *to = dtable + (size_t)v * lddt;
@@ -137,6 +150,7 @@ __global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ 
             }
         if (last < 0 && accumulate) continue;
         for (int j = lane; j < chunks; j += lanes) {
+            const Tail<DT> at_j(j, C);
             float a[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) a[e] = 0.0f;
@@ -146,7 +160,7 @@ __global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ 
                 for (int u = 0; u < 8; ++u) {
                     const bool own = k + u <= last && tok[k + u] == v;
                     w[u] = u32x4{0u, 0u, 0u, 0u};
-                    if (own) w[u] = Chunk<DT>::load(dout + (size_t)at[k + u] * lddo, j, nb, C);
+                    if (own) w[u] = at_j.load(dout + (size_t)at[k + u] * lddo);
                 }
 #pragma unroll
                 for (int u = 0; u < 8; ++u)
@@ -155,12 +169,8 @@ __global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ 
             }
 #pragma unroll
             for (int e = 0; e < E; ++e) a[e] *= scale;
-            if (accumulate) {
-                const u32x4 was = Chunk<DT>::load(to, j, nb, C);
-#pragma unroll
-                for (int e = 0; e < E; ++e) a[e] += IO::get(was, e);
-            }
-            Chunk<DT>::store(to, j, nb, C, a);
+            if (accumulate) at_j.add(to, j, a);
+            else at_j.store(to, a);
         }
     }
 }
@@ -520,7 +530,7 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
                                                 typename Io<DT>::T *dtable) {
     using IO = Io<DT>;
     constexpr int E = IO::E, UNR = 8;
-    const int nb = p.C / E, chunks = (p.C - 1) / E + 1;
+    const int chunks = (p.C - 1) / E + 1;
     if ((int)blockIdx.x >= p.unit_blocks) {
         // Rows of no token.
         if (blockIdx.y > 0) return;
@@ -552,7 +562,7 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
             if (used[r]) continue;
             auto *to = dtable + (size_t)(v0 + r) * p.lddt;
             for (int j = threadIdx.x & (lanes - 1); j < chunks; j += lanes)
-                Chunk<DT>::store(to, j, nb, p.C, z);
+                Tail<DT>(j, p.C).store(to, z);
         }
         return;
     }
@@ -561,6 +571,7 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
     if constexpr (WAVE) unit = __builtin_amdgcn_readfirstlane(unit);
     const int j = blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
     if (unit >= p.units || j >= chunks) return;
+    const Tail<DT> at_j(j, p.C);
     const int k0 = unit * p.P, k1 = min(p.T, k0 + p.P);
     const uint32_t V = (uint32_t)p.V;
     const uint32_t *__restrict__ sorted = p.sorted, *__restrict__ order = p.order;
@@ -586,7 +597,7 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
         uint32_t t[UNR + 1];
 #pragma unroll
         for (int u = 0; u < UNR; ++u)
-            w[u] = Chunk<DT>::load(dout + (size_t)pos[u] * p.lddo, j, nb, p.C);
+            w[u] = at_j.load(dout + (size_t)pos[u] * p.lddo);
 #pragma unroll
         for (int u = 0; u <= UNR; ++u) t[u] = tok[u];
         if (k + UNR < k1) index(k + UNR);
@@ -600,21 +611,17 @@ __global__ __launch_bounds__(kNT) void emb_sums(const Sums p,
             if (t[u] < V) {
                 if (head || same) {  // (same: the run goes on in the next unit)
                     float *to = p.partial + ((size_t)unit * 2 + (head ? 0 : 1)) * p.Cp +
-                                (size_t)j * E;
+                                at_j.first;
 #pragma unroll
                     for (int q = 0; q < E / 4; ++q)
-                        *reinterpret_cast<f32x4 *>(to + 4 * q) =
+                        *reinterpret_cast<f32x4_any *>(to + 4 * q) =
                             f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
                 } else {
                     auto *to = dtable + (size_t)t[u] * p.lddt;
 #pragma unroll
                     for (int e = 0; e < E; ++e) a[e] *= p.scale;
-                    if (p.accumulate) {
-                        const u32x4 was = Chunk<DT>::load(to, j, nb, p.C);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) a[e] += IO::get(was, e);
-                    }
-                    Chunk<DT>::store(to, j, nb, p.C, a);
+                    if (p.accumulate) at_j.add(to, j, a);
+                    else at_j.store(to, a);
                 }
             }
             head = false;
