@@ -18,7 +18,8 @@
 // is four lanes, eight in fp32) and, of the 8-bit form, the chunk's 8 or 4 bytes, so
 // that every access of a wave is one stretch of memory: with 16 columns a lane, each
 // store of a wave left gaps, and 2048 x 4096 fp32 there and back took 64 us.  Rows may
-// start anywhere.
+// start anywhere.  bf16 16384 x 4096: save 37 us, load of z and gelu(z) 48 us
+// (6.9 TB/s), act_bwd 60 us (5.6 TB/s); 2048 x 4096 there and back 13.4 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -357,6 +358,11 @@ FG_API int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int 
     FG_REQUIRE(d_Xr != d_Zr && d_Xr != d_dX, FG_ERR_INVALID_ARGUMENT,
                "%s: Xr must not be Zr or dX", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    // One pass restores z and act(z), 6 % of the call at bf16 2048 x 4096 x 4096 (8.6 us of
+    // 147), then the products as from kept activations, with their roundings: act(z) to
+    // the type (what the matrix instructions take), dX's product to the type before it is
+    // multiplied by act'(z), so that a layer's gradients are the same bits whichever form
+    // its input was kept in, where that form is exact.
     // [act(z) > 0] == [z > 0] for ReLU, whose derivative then reads Xr.
     void *zr = act == FG_ACT_GELU ? d_Zr : nullptr;
     if (int rc = fg_ckpt8_load(ctx, dtype, act, d_q, ldq, d_e, lde, M, K, zr, K, d_Xr, K))
