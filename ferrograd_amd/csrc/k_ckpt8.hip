@@ -325,6 +325,8 @@ FG_API int fg_act_bwd_ckpt8(fg_ctx *ctx, int dtype, int act, const void *d_dH, i
     FG_REQUIRE(lddh >= C && lddz >= C, FG_ERR_SHAPE, "%s: lddh=%d or lddz=%d < C=%d", who, lddh,
                lddz, C);
     FG_REQUIRE(d_dH && d_dZ, FG_ERR_INVALID_ARGUMENT, "%s: dH and dZ are required", who);
+    FG_REQUIRE(d_dZ != d_dH || lddz == lddh, FG_ERR_INVALID_ARGUMENT,
+               "%s: dZ is dH, but lddz=%d, lddh=%d", who, lddz, lddh);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
@@ -355,8 +357,11 @@ FG_API int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int 
                who);
     FG_REQUIRE(d_Xr && (act != FG_ACT_GELU || d_Zr), FG_ERR_INVALID_ARGUMENT,
                "%s: Xr, and for GELU Zr, is required", who);
-    FG_REQUIRE(d_Xr != d_Zr && d_Xr != d_dX, FG_ERR_INVALID_ARGUMENT,
-               "%s: Xr must not be Zr or dX", who);
+    auto apart = [&](const void *r) {
+        return !r || (r != d_W && r != d_dZ && r != d_dX && r != d_dW && r != d_dbias);
+    };
+    FG_REQUIRE(d_Xr != d_Zr && apart(d_Xr) && apart(d_Zr), FG_ERR_INVALID_ARGUMENT,
+               "%s: Xr and Zr must not be an operand, an output or each other", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     // One pass restores z and act(z), 6 % of the call at bf16 2048 x 4096 x 4096 (8.6 us of
     // 147), then the products as from kept activations, with their roundings: act(z) to

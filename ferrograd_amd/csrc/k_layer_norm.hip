@@ -1149,6 +1149,8 @@ FG_API int fg_layer_norm(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const
     FG_REQUIRE(eps > 0.0f && eps < INFINITY, FG_ERR_INVALID_ARGUMENT,
                "%s: eps must be positive and finite", who);
     FG_REQUIRE(d_x && d_y, FG_ERR_INVALID_ARGUMENT, "%s: x and y are required", who);
+    FG_REQUIRE(d_y != d_x || ldy == ldx, FG_ERR_INVALID_ARGUMENT, "%s: y is x, but ldy=%d, ldx=%d",
+               who, ldy, ldx);
     FG_REQUIRE(rows_fit(dtype, R, C), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns", who, R, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     if (R == 0) return FG_OK;
@@ -1178,6 +1180,10 @@ FG_API int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, c
                "%s: ldx=%d, lddy=%d or lddx=%d < C=%d", who, ldx, lddy, lddx, C);
     FG_REQUIRE(d_x && d_dy && d_mean && d_rstd, FG_ERR_INVALID_ARGUMENT,
                "%s: x, dy, mean and rstd are required", who);
+    FG_REQUIRE((d_dx != d_x || lddx == ldx) && (d_dx != d_dy || lddx == lddy),
+               FG_ERR_INVALID_ARGUMENT, "%s: dx is x or dy, but of another leading dimension", who);
+    FG_REQUIRE(!accumulate || (d_dx != d_x && d_dx != d_dy), FG_ERR_INVALID_ARGUMENT,
+               "%s: dx is x or dy and adds to itself", who);
     FG_REQUIRE(rows_fit(dtype, R, C), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns", who, R, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     FG_HIP(hipSetDevice(ctx->device));

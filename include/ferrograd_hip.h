@@ -326,8 +326,8 @@ int fg_layer_norm(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const void *
  *   dx (=|+=) rstd * (g - mean(g) - xh * mean(g * xh))
  *   dgamma (=|+=) sum over rows of dy * xh ;  dbeta (=|+=) sum over rows of dy
  * Any output may be NULL; gamma may be NULL (1).  dx may be x or dy (equal
- * leading dimensions) unless it accumulates.  The rows' partial sums of
- * dgamma and dbeta go to the workspace, 8 bytes a column for each of at most
+ * leading dimensions) unless it accumulates.  Above 256 rows, their partial sums
+ * of dgamma and dbeta go to the workspace, 8 bytes a column for each of at most
  * 1024 row splits, and are added in a fixed order.  R = 0 writes zeros to
  * dgamma and dbeta (or adds nothing). */
 int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const void *d_dy,
@@ -379,7 +379,9 @@ int fg_act_bwd_ckpt8(fg_ctx *ctx, int dtype, int act, const void *d_dH, int lddh
  *   dX (=|+=) (dZ.W^T) * act'(z) [M][K]
  * d_Xr and (for GELU; else it may be NULL) d_Zr are the caller's scratch, M x K
  * elements of dtype each, overwritten with act(z) and z as the products read
- * them: act(z) is rounded to dtype, as the forward's stored activation is. */
+ * them (no operand or output may be there): act(z) is rounded to dtype, as the
+ * forward's stored activation is, and so is dX's product before act'(z)
+ * multiplies it, as in fg_matmul_bwd_x16. */
 int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int act,
                         const int8_t *d_q, int ldq, const uint8_t *d_e, int lde,
                         const void *d_W, int ldw, const void *d_dZ, int lddz, void *d_Zr,

@@ -28,7 +28,7 @@ CALLS = {
     "fg_act_bwd_ckpt8": dict(ctx=None, dtype=0, act=2, dH=P, lddh=65, q=P, ldq=65, e=P, lde=3, R=4,
                              C=65, dZ=P, lddz=65),
     "fg_matmul_bwd_ckpt8": dict(ctx=None, dtype=2, M=4, N=8, K=65, act=2, q=P, ldq=65, e=P, lde=3,
-                                W=P, ldw=8, dZ=P, lddz=8, Zr=P, Xr=2 * P, dX=3 * P, lddx=65, dW=P,
+                                W=P, ldw=8, dZ=P, lddz=8, Zr=4 * P, Xr=2 * P, dX=3 * P, lddx=65, dW=P,
                                 lddw=8, dbias=P, acc=0),
 }
 
@@ -40,6 +40,14 @@ REFUSED = [
     ("fg_embedding", dict(T=MANY, C=2048, ldt=2048, ldo=2048), BOUNDS),
     ("fg_embedding_bwd", dict(T=(1 << 30) + 1), BOUNDS),
     ("fg_ckpt8_load", dict(R=MANY, C=4096, ldq=4096, lde=128, ldz=4096, ldh=4096), BOUNDS),
+    # Outputs that are inputs, of another leading dimension or added to.
+    ("fg_layer_norm", dict(ldx=65), INVALID), ("fg_layer_norm_bwd", dict(ldx=65), INVALID),
+    ("fg_layer_norm_bwd", dict(lddy=65, x=2 * P), INVALID),
+    ("fg_layer_norm_bwd", dict(acc=1), INVALID),
+    ("fg_layer_norm_bwd", dict(acc=1, dy=2 * P), INVALID),
+    ("fg_act_bwd_ckpt8", dict(lddh=66), INVALID),
+    ("fg_matmul_bwd_ckpt8", dict(Zr=3 * P), INVALID),
+    ("fg_matmul_bwd_ckpt8", dict(Xr=P), INVALID), ("fg_matmul_bwd_ckpt8", dict(Zr=P), INVALID),
     ("fg_layer_norm", dict(C=BIG, ldx=BIG, ldy=BIG), BOUNDS),
     ("fg_layer_norm_bwd", dict(C=BIG, ldx=BIG, lddy=BIG, lddx=BIG), BOUNDS),
     ("fg_embedding", dict(C=BIG, ldt=BIG, ldo=BIG), BOUNDS),
