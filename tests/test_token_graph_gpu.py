@@ -288,6 +288,26 @@ def test_captured_steps_give_the_eager_bits(gctx, dt, optim):
         m.close()
 
 
+@pytest.mark.parametrize("ckpt", [(), (0,), (1,), (0, 1)])
+def test_captured_small_layers_beside_kept_ones(gctx, ckpt):
+    """A long first product, a small hidden layer and a head of few classes, as a captured
+    SGD step runs them (split, chained, the loss in the head's product), with each layer
+    kept in 8 bits or not: the eager parameters after each of three steps."""
+    size = (64, 40, 784, 64, 10)
+    make = lambda: Model(gctx, "f32", *size, ckpt=ckpt, optim=G.Optim.sgd(), norm=False)
+    a, b = make(), make()
+    gctx.capture_step(b.sch, b.target)
+    for k in range(3):
+        a.step()
+        gctx.dispatch_optim(a.sch)
+        gctx.launch_step(b.sch)
+        gctx.sync()
+        for x, y, n in zip(a.ins[1:], b.ins[1:], a.names):
+            assert np.array_equal(gctx.download(x), gctx.download(y)), (k, n)
+    a.close()
+    b.close()
+
+
 def test_tied_table_and_shared_gamma_add_their_gradients(gctx):
     """A table read by two lookups and a gamma by two layer norms: gradients add."""
     T, V, C = 130, 40, 24
