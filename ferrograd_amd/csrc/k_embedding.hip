@@ -54,13 +54,26 @@ constexpr int64_t kOrderReads = 10 << 20;
 constexpr int kUnitBlocks = 1024;
 constexpr int kMaxTokens = 1 << 30;  // (positions a little past the last are 32-bit too)
 
+// A kernel's arguments are one or two structs: with a dozen arguments the runtime takes
+// up to 0.9 us more for a launch (layer norm backward of 64 rows, a call 5.4 us and 4.9).
+
 // ------------------------------------------------------------------- lookup
+template <class T>
+struct Lookup {
+    const uint32_t *tokens;
+    const T *table;
+    T *out;
+    int count, V, C, ldt, ldo, lshift;
+    float scale;
+};
 // 2^lshift lanes take a row, UNR chunks in flight a lane.
 template <int DT>
-__global__ __launch_bounds__(kNT) void emb_fwd(const uint32_t *__restrict__ tokens, int T, int V,
-                                               int C, const typename Io<DT>::T *__restrict__ table,
-                                               int ldt, float scale, typename Io<DT>::T *out,
-                                               int ldo, int lshift) {
+__global__ __launch_bounds__(kNT) void emb_fwd(const Lookup<typename Io<DT>::T> a) {
+    const uint32_t *__restrict__ tokens = a.tokens;
+    const auto *__restrict__ table = a.table;
+    auto *out = a.out;
+    const int T = a.count, V = a.V, C = a.C, ldt = a.ldt, ldo = a.ldo, lshift = a.lshift;
+    const float scale = a.scale;
     using IO = Io<DT>;
     constexpr int E = IO::E, UNR = 4;
     const int lanes = 1 << lshift, lane = threadIdx.x & (lanes - 1);
@@ -105,13 +118,22 @@ __global__ __launch_bounds__(kNT) void emb_fwd(const uint32_t *__restrict__ toke
 // A workgroup owns `rows` table rows from blockIdx.x * rows on: it lists the
 // positions of their tokens in order, then each group of 2^lshift lanes adds the
 // rows of its own tokens.
+template <class T>
+struct Few {
+    const uint32_t *tokens;
+    const T *dout;
+    T *dtable;
+    int count, V, C, lddo, lddt, accumulate, rows, lshift;
+    float scale;
+};
 template <int DT>
-__global__ __launch_bounds__(kNT) void emb_bwd_few(const uint32_t *__restrict__ tokens, int T,
-                                                   int V, int C,
-                                                   const typename Io<DT>::T *__restrict__ dout,
-                                                   int lddo, float scale,
-                                                   typename Io<DT>::T *dtable, int lddt,
-                                                   int accumulate, int rows, int lshift) {
+__global__ __launch_bounds__(kNT) void emb_bwd_few(const Few<typename Io<DT>::T> p) {
+    const uint32_t *__restrict__ tokens = p.tokens;
+    const auto *__restrict__ dout = p.dout;
+    auto *dtable = p.dtable;
+    const int T = p.count, V = p.V, C = p.C, lddo = p.lddo, lddt = p.lddt;
+    const int accumulate = p.accumulate, rows = p.rows, lshift = p.lshift;
+    const float scale = p.scale;
     using IO = Io<DT>;
     constexpr int E = IO::E;
     static_assert(kDirectMax <= kNT, "one token a thread");
@@ -208,11 +230,17 @@ __device__ __forceinline__ void zero_rows(const Zero &z, int block, int blocks) 
 // cost two comparisons.  Tokens outside the table sort as V.
 constexpr int kOrderNT = 1024, kOrderWaves = kOrderNT / 64;
 constexpr int kOrderBlocks = 256, kOrderBins = 1024;  // at least; at most
-__global__ __launch_bounds__(kOrderNT) void emb_order(const uint32_t *__restrict__ tokens, int T,
-                                                      uint32_t V, int bins,
-                                                      uint32_t *__restrict__ order,
-                                                      uint32_t *__restrict__ sorted, int blocks,
-                                                      const Zero z) {
+struct Order {
+    const uint32_t *tokens;
+    uint32_t *order, *sorted;
+    int count, bins, blocks;
+    uint32_t V;
+};
+__global__ __launch_bounds__(kOrderNT) void emb_order(const Order p, const Zero z) {
+    const uint32_t *__restrict__ tokens = p.tokens;
+    uint32_t *__restrict__ order = p.order, *__restrict__ sorted = p.sorted;
+    const int T = p.count, bins = p.bins, blocks = p.blocks;
+    const uint32_t V = p.V;
     __shared__ uint32_t cnt[kOrderWaves * kOrderBins];  // [wave][bins]
     __shared__ uint32_t wbelow[kOrderWaves], wsum[kOrderWaves];
     if ((int)blockIdx.x >= blocks) {
@@ -318,13 +346,20 @@ __global__ __launch_bounds__(kOrderNT) void emb_order(const uint32_t *__restrict
 constexpr int kMaxBits = 11, kBins = 1 << kMaxBits;
 constexpr int kTiles = 64;  // at most
 constexpr int kSortNT = 1024;
+struct Radix {
+    const uint32_t *keys, *pos;
+    uint32_t *hist, *keys_out, *pos_out;
+    int count, per, shift, bits, tiles;
+    uint32_t V;
+};
 
 __device__ __forceinline__ uint32_t key_of(uint32_t token, uint32_t V) { return min(token, V); }
 
-__global__ __launch_bounds__(kSortNT) void radix_count(const uint32_t *__restrict__ keys, int T,
-                                                       uint32_t V, int per, int shift, int bits,
-                                                       uint32_t *__restrict__ hist, int tiles,
-                                                       const Zero z) {
+__global__ __launch_bounds__(kSortNT) void radix_count(const Radix p, const Zero z) {
+    const uint32_t *__restrict__ keys = p.keys;
+    uint32_t *__restrict__ hist = p.hist;
+    const int T = p.count, per = p.per, shift = p.shift, bits = p.bits, tiles = p.tiles;
+    const uint32_t V = p.V;
     __shared__ uint32_t h[kBins];
     if ((int)blockIdx.x >= tiles) {
         zero_rows(z, blockIdx.x - tiles, gridDim.x - tiles);
@@ -342,13 +377,12 @@ __global__ __launch_bounds__(kSortNT) void radix_count(const uint32_t *__restric
 }
 
 // pos NULL: the pairs' positions are their own indices (the first pass).
-__global__ __launch_bounds__(kSortNT) void radix_place(const uint32_t *__restrict__ keys,
-                                                       const uint32_t *__restrict__ pos, int T,
-                                                       uint32_t V, int per, int shift, int bits,
-                                                       const uint32_t *__restrict__ hist,
-                                                       uint32_t *__restrict__ keys_out,
-                                                       uint32_t *__restrict__ pos_out, int tiles,
-                                                       const Zero z) {
+__global__ __launch_bounds__(kSortNT) void radix_place(const Radix p, const Zero z) {
+    const uint32_t *__restrict__ keys = p.keys, *__restrict__ pos = p.pos;
+    const uint32_t *__restrict__ hist = p.hist;
+    uint32_t *__restrict__ keys_out = p.keys_out, *__restrict__ pos_out = p.pos_out;
+    const int T = p.count, per = p.per, shift = p.shift, bits = p.bits, tiles = p.tiles;
+    const uint32_t V = p.V;
     if ((int)blockIdx.x >= tiles) {
         zero_rows(z, blockIdx.x - tiles, gridDim.x - tiles);
         return;
@@ -746,10 +780,9 @@ template <int DT>
 int launch_fwd(fg_ctx *ctx, const uint32_t *tokens, int T, int V, int C, const void *table, int ldt,
                float scale, void *out, int ldo) {
     using Ty = typename Io<DT>::T;
-    const int lshift = lane_shift((C - 1) / Io<DT>::E + 1);
     emb_fwd<DT><<<(unsigned)fwd_blocks(DT, T, C), kNT, 0, ctx->stream>>>(
-        tokens, T, V, C, static_cast<const Ty *>(table), ldt, scale, static_cast<Ty *>(out), ldo,
-        lshift);
+        {tokens, static_cast<const Ty *>(table), static_cast<Ty *>(out), T, V, C, ldt, ldo,
+         lane_shift((C - 1) / Io<DT>::E + 1), scale});
     FG_LAUNCH_CHECK("emb_fwd");
     return FG_OK;
 }
@@ -766,8 +799,8 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
         const int lshift = lane_shift(chunks), at_once = kNT >> lshift;
         // Table rows of a workgroup: those it takes at once, more where the table is long.
         const int rows = (int)std::max<int64_t>(at_once, (V - 1) / (16 * ctx->cu_count) + 1);
-        emb_bwd_few<DT><<<(V - 1) / rows + 1, kNT, 0, st>>>(tokens, T, V, C, d, lddo, scale, g, lddt,
-                                                           accumulate, rows, lshift);
+        emb_bwd_few<DT><<<(V - 1) / rows + 1, kNT, 0, st>>>(
+            {tokens, d, g, T, V, C, lddo, lddt, accumulate, rows, lshift, scale});
         FG_LAUNCH_CHECK("emb_bwd_few");
         return FG_OK;
     }
@@ -798,8 +831,8 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
     };
     if (pl.passes == 0) {
         const int zeros = share(order_mb);
-        emb_order<<<pl.blocks + zeros, kOrderNT, 0, st>>>(tokens, T, (uint32_t)V, pl.bins, order,
-                                                          sorted, pl.blocks, z);
+        emb_order<<<pl.blocks + zeros, kOrderNT, 0, st>>>(
+            {tokens, order, sorted, T, pl.bins, pl.blocks, (uint32_t)V}, z);
         FG_LAUNCH_CHECK("emb_order");
     } else {
         // The passes go back and forth between two pairs of arrays and end in the first.
@@ -809,16 +842,15 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
         const uint32_t *kin = tokens, *pin = nullptr;
         for (int n = 0; n < pl.passes; ++n) {
             const int to = (pl.passes - 1 - n) & 1;
+            const Radix r{kin, pin, hist, key[to], pos[to], T, pl.per, n * pl.bits, pl.bits,
+                          pl.tiles, (uint32_t)V};
             int zeros = share(count_mb);
-            radix_count<<<pl.tiles + zeros, kSortNT, 0, st>>>(
-                kin, T, (uint32_t)V, pl.per, n * pl.bits, pl.bits, hist, pl.tiles, z);
+            radix_count<<<pl.tiles + zeros, kSortNT, 0, st>>>(r, z);
             FG_LAUNCH_CHECK("radix_count");
             // (The next pass's counts added up here by atomics, one launch fewer, took the
             // first pass from 8.5 to 21 us for 65536 tokens.)
             zeros = share(place_mb);
-            radix_place<<<pl.tiles + zeros, kSortNT, 0, st>>>(kin, pin, T, (uint32_t)V, pl.per,
-                                                              n * pl.bits, pl.bits, hist, key[to],
-                                                              pos[to], pl.tiles, z);
+            radix_place<<<pl.tiles + zeros, kSortNT, 0, st>>>(r, z);
             FG_LAUNCH_CHECK("radix_place");
             kin = key[to];
             pin = pos[to];

@@ -60,6 +60,28 @@ __device__ __forceinline__ float row_sum(float v, float *sm, int t) {
     return v;
 }
 
+// A kernel's arguments are one or two structs: with a dozen arguments the runtime takes
+// up to 0.9 us more for a launch (layer norm backward of 64 rows, a call 5.4 us and 4.9).
+template <class T>
+struct Fwd {
+    const T *x, *gamma, *beta;
+    T *y;
+    float *mean, *rstd, eps;
+    int ldx, ldy, R, C;
+};
+template <class T>
+struct Bwd {
+    const T *x, *dy, *gamma;
+    const float *mean, *rstd;
+    T *dx;
+    float *partial;
+    int ldx, lddy, lddx, R, C, accumulate;
+    int rows;           // ln_bwd_cols: of a split
+    int row_blocks;     // ln_bwd_few
+    void *dgamma, *dbeta;
+    int acc_g, acc_b;
+};
+
 // ------------------------------------------------------------------ forward
 // A row is held in registers by L lanes, NV chunks a lane, NG rows at once in a
 // workgroup; the workgroup walks the rows with gamma and beta held, and the next
@@ -67,10 +89,13 @@ __device__ __forceinline__ float row_sum(float v, float *sm, int t) {
 // (a difference of squares would lose a row far from zero), and sums are divided by
 // C, so that the mean of a constant row is exact.
 template <int DT, int NV, int L, int NG>
-__global__ __launch_bounds__(L *NG) void ln_fwd(
-    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *gamma,
-    const typename Io<DT>::T *beta, float eps, int R, int C, typename Io<DT>::T *y, int ldy,
-    float *mean, float *rstd) {
+__global__ __launch_bounds__(L *NG) void ln_fwd(const Fwd<typename Io<DT>::T> a) {
+    const auto *x = a.x;
+    const auto *gamma = a.gamma, *beta = a.beta;
+    auto *y = a.y;
+    float *mean = a.mean, *rstd = a.rstd;
+    const float eps = a.eps;
+    const int ldx = a.ldx, ldy = a.ldy, R = a.R, C = a.C;
     using IO = Io<DT>;
     constexpr int E = IO::E, NS = (L + 63) / 64;
     __shared__ float sm[2][2][NG][NS];
@@ -157,10 +182,13 @@ __global__ __launch_bounds__(L *NG) void ln_fwd(
 // overlap one another's sums: bf16 4096 x 12000 40.1 us in workgroups of 512, 46.0 in
 // ones of 1024; 2048 x 16384 23.2 us, 5.8 TB/s.
 template <int DT, int NV, int L>
-__global__ __launch_bounds__(L) __attribute__((amdgpu_waves_per_eu(8))) void ln_fwd_wide(
-    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *__restrict__ gamma,
-    const typename Io<DT>::T *__restrict__ beta, float eps, int C, typename Io<DT>::T *y, int ldy,
-    float *mean, float *rstd) {
+__global__ __launch_bounds__(L) __attribute__((amdgpu_waves_per_eu(8))) void ln_fwd_wide(const Fwd<typename Io<DT>::T> a) {
+    const auto *x = a.x;
+    const auto *__restrict__ gamma = a.gamma, *__restrict__ beta = a.beta;
+    auto *y = a.y;
+    float *mean = a.mean, *rstd = a.rstd;
+    const float eps = a.eps;
+    const int ldx = a.ldx, ldy = a.ldy, C = a.C;
     using IO = Io<DT>;
     constexpr int E = IO::E;
     __shared__ float sm[2][L / 64];
@@ -233,10 +261,13 @@ __global__ __launch_bounds__(L) __attribute__((amdgpu_waves_per_eu(8))) void ln_
 // from the caches where they hold it.
 constexpr int kLongL = 1024;
 template <int DT>
-__global__ __launch_bounds__(kLongL) void ln_fwd_long(
-    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *gamma,
-    const typename Io<DT>::T *beta, float eps, int C, typename Io<DT>::T *y, int ldy, float *mean,
-    float *rstd) {
+__global__ __launch_bounds__(kLongL) void ln_fwd_long(const Fwd<typename Io<DT>::T> a) {
+    const auto *x = a.x;
+    const auto *gamma = a.gamma, *beta = a.beta;
+    auto *y = a.y;
+    float *mean = a.mean, *rstd = a.rstd;
+    const float eps = a.eps;
+    const int ldx = a.ldx, ldy = a.ldy, C = a.C;
     using IO = Io<DT>;
     constexpr int E = IO::E;
     __shared__ float sm[2][kLongL / 64];
@@ -313,10 +344,14 @@ __host__ __device__ constexpr int64_t padded(int64_t C) { return (C + 3) & ~int6
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 template <int DT, int NV, int L, int NG, bool WEIGHTS>
-__global__ __launch_bounds__(L *NG) void ln_bwd(
-    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
-    const typename Io<DT>::T *gamma, const float *mean, const float *rstd, int R, int C,
-    typename Io<DT>::T *dx, int lddx, int accumulate, float *partial) {
+__global__ __launch_bounds__(L *NG) void ln_bwd(const Bwd<typename Io<DT>::T> a) {
+    const auto *x = a.x, *dy = a.dy;
+    const auto *gamma = a.gamma;
+    const float *mean = a.mean, *rstd = a.rstd;
+    auto *dx = a.dx;
+    const int ldx = a.ldx, lddy = a.lddy, lddx = a.lddx, C = a.C, accumulate = a.accumulate;
+    const int R = a.R;
+    float *partial = a.partial;
     using IO = Io<DT>;
     constexpr int E = IO::E, NS = (L + 63) / 64;
     __shared__ float sm[2][2][NG][NS];
@@ -491,10 +526,14 @@ __global__ __launch_bounds__(L *NG) void ln_bwd(
 // loads at a time 44.2), a quarter of it the partial sums, as large as two rows a
 // workgroup are.
 template <int DT, int NV>
-__global__ __launch_bounds__(1024) void ln_bwd_wide(
-    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
-    const typename Io<DT>::T *__restrict__ gamma, const float *mean, const float *rstd, int R,
-    int C, typename Io<DT>::T *dx, int lddx, int accumulate, float *partial) {
+__global__ __launch_bounds__(1024) void ln_bwd_wide(const Bwd<typename Io<DT>::T> a) {
+    const auto *x = a.x, *dy = a.dy;
+    const auto *__restrict__ gamma = a.gamma;
+    const float *mean = a.mean, *rstd = a.rstd;
+    auto *dx = a.dx;
+    const int ldx = a.ldx, lddy = a.lddy, lddx = a.lddx, C = a.C, accumulate = a.accumulate;
+    const int R = a.R;
+    float *partial = a.partial;
     using IO = Io<DT>;
     constexpr int E = IO::E, L = 1024, Q = E / 4;
     __shared__ float sm[2][2][L / 64];
@@ -631,10 +670,12 @@ __global__ __launch_bounds__(1024) void ln_bwd_wide(
 // Rows longer than that: dx from a row held packed, a workgroup a row, as ln_fwd_wide
 // (longer still: the row twice) ...
 template <int DT, int NV>
-__global__ __launch_bounds__(1024) void ln_bwd_dx(
-    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
-    const typename Io<DT>::T *__restrict__ gamma, const float *mean, const float *rstd, int C,
-    typename Io<DT>::T *dx, int lddx, int accumulate) {
+__global__ __launch_bounds__(1024) void ln_bwd_dx(const Bwd<typename Io<DT>::T> a) {
+    const auto *x = a.x, *dy = a.dy;
+    const auto *__restrict__ gamma = a.gamma;
+    const float *mean = a.mean, *rstd = a.rstd;
+    auto *dx = a.dx;
+    const int ldx = a.ldx, lddy = a.lddy, lddx = a.lddx, C = a.C, accumulate = a.accumulate;
     using IO = Io<DT>;
     constexpr int E = IO::E, L = 1024;
     __shared__ float sm[2][L / 64];
@@ -706,10 +747,13 @@ __global__ __launch_bounds__(1024) void ln_bwd_dx(
 }
 
 template <int DT>
-__device__ __forceinline__ void bwd_long_row(
-    size_t r, const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
-    const typename Io<DT>::T *gamma, const float *mean, const float *rstd, int C,
-    typename Io<DT>::T *dx, int lddx, int accumulate, float (*sm)[kLongL / 64]) {
+__device__ __forceinline__ void bwd_long_row(size_t r, const Bwd<typename Io<DT>::T> &a,
+                                             float (*sm)[kLongL / 64]) {
+    const auto *x = a.x, *dy = a.dy;
+    const auto *gamma = a.gamma;
+    const float *mean = a.mean, *rstd = a.rstd;
+    auto *dx = a.dx;
+    const int ldx = a.ldx, lddy = a.lddy, lddx = a.lddx, C = a.C, accumulate = a.accumulate;
     using IO = Io<DT>;
     constexpr int E = IO::E;
     const auto *xr = x + r * ldx, *dr = dy + r * lddy;
@@ -773,12 +817,9 @@ __device__ __forceinline__ void bwd_long_row(
 }
 
 template <int DT>
-__global__ __launch_bounds__(kLongL) void ln_bwd_long(
-    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
-    const typename Io<DT>::T *gamma, const float *mean, const float *rstd, int C,
-    typename Io<DT>::T *dx, int lddx, int accumulate) {
+__global__ __launch_bounds__(kLongL) void ln_bwd_long(const Bwd<typename Io<DT>::T> a) {
     __shared__ float sm[2][kLongL / 64];
-    bwd_long_row<DT>(blockIdx.x, x, ldx, dy, lddy, gamma, mean, rstd, C, dx, lddx, accumulate, sm);
+    bwd_long_row<DT>(blockIdx.x, a, sm);
 }
 
 // Few rows (kFewRows), where launches count: one for everything, workgroups of one
@@ -788,18 +829,16 @@ __global__ __launch_bounds__(kLongL) void ln_bwd_long(
 // 12.2; with 512 rows fp32 of 4096 12.1 and 14.9, 512 x 512 8.9 and 9.2.
 constexpr int kFewRows = 256, kFewLanes = 16, kFewGroups = kLongL / kFewLanes;
 template <int DT>
-__global__ __launch_bounds__(kLongL) void ln_bwd_few(
-    const typename Io<DT>::T *x, int ldx, const typename Io<DT>::T *dy, int lddy,
-    const typename Io<DT>::T *gamma, const float *mean, const float *rstd, int R, int C,
-    typename Io<DT>::T *dx, int lddx, int accumulate, void *dgamma, int acc_g, void *dbeta,
-    int acc_b, int row_blocks) {
+__global__ __launch_bounds__(kLongL) void ln_bwd_few(const Bwd<typename Io<DT>::T> a) {
+    const auto *x = a.x, *dy = a.dy;
+    const float *mean = a.mean, *rstd = a.rstd;
+    const int ldx = a.ldx, lddy = a.lddy, R = a.R, C = a.C, row_blocks = a.row_blocks;
     using IO = Io<DT>;
     constexpr int E = IO::E, kCols = kFewLanes * E;
     __shared__ float sm[2][kLongL / 64];
     __shared__ float sh[kFewGroups][kCols];
     if ((int)blockIdx.x < row_blocks) {
-        bwd_long_row<DT>(blockIdx.x, x, ldx, dy, lddy, gamma, mean, rstd, C, dx, lddx, accumulate,
-                         sm);
+        bwd_long_row<DT>(blockIdx.x, a, sm);
         return;
     }
     const int lane = threadIdx.x % kFewLanes, group = threadIdx.x / kFewLanes;
@@ -831,9 +870,9 @@ __global__ __launch_bounds__(kLongL) void ln_bwd_few(
         }
     }
     // The groups' sums in order, a column a thread.
-    auto add = [&](const float (&a)[E], void *out, int acc) {
+    auto add = [&](const float (&v)[E], void *out, int acc) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) sh[group][lane * E + e] = a[e];
+        for (int e = 0; e < E; ++e) sh[group][lane * E + e] = v[e];
         __syncthreads();
         const int at = strip * kFewLanes + (int)threadIdx.x / E, e = threadIdx.x % E;
         const int col = at < nb ? at * E + e : e == 0 ? nb * E + (at - nb) : C;
@@ -846,8 +885,8 @@ __global__ __launch_bounds__(kLongL) void ln_bwd_few(
         }
         __syncthreads();
     };
-    add(ag, dgamma, acc_g);
-    add(ab, dbeta, acc_b);
+    add(ag, a.dgamma, a.acc_g);
+    add(ab, a.dbeta, a.acc_b);
 }
 
 // ... and the columns of a strip over a split of the rows, a chunk a lane (the
@@ -855,10 +894,11 @@ __global__ __launch_bounds__(kLongL) void ln_bwd_few(
 // are read twice: bf16 512 x 65536 72 us, 4.6 TB/s of what both read and write.
 constexpr int kColsNT = 256;
 template <int DT>
-__global__ __launch_bounds__(kColsNT) void ln_bwd_cols(const typename Io<DT>::T *x, int ldx,
-                                                       const typename Io<DT>::T *dy, int lddy,
-                                                       const float *mean, const float *rstd, int R,
-                                                       int C, int rows, float *partial) {
+__global__ __launch_bounds__(kColsNT) void ln_bwd_cols(const Bwd<typename Io<DT>::T> a) {
+    const auto *x = a.x, *dy = a.dy;
+    const float *mean = a.mean, *rstd = a.rstd;
+    const int ldx = a.ldx, lddy = a.lddy, R = a.R, C = a.C, rows = a.rows;
+    float *partial = a.partial;
     using IO = Io<DT>;
     constexpr int E = IO::E;
     const int nb = C / E, j = blockIdx.x * kColsNT + threadIdx.x;
@@ -903,10 +943,15 @@ __global__ __launch_bounds__(kColsNT) void ln_bwd_cols(const typename Io<DT>::T 
 
 // Adds the partial sums of each column: GROUPS threads a column, each a run of them in
 // order, then the groups' sums in order.
+struct Final {
+    const float *partial;
+    void *dgamma, *dbeta;
+    int dt, splits, C, acc_g, acc_b;
+};
 template <int COLS, int GROUPS>
-__global__ __launch_bounds__(COLS *GROUPS) void ln_bwd_final(
-    int dt, const float *__restrict__ partial, int splits, int C, void *dgamma, int acc_g,
-    void *dbeta, int acc_b) {
+__global__ __launch_bounds__(COLS *GROUPS) void ln_bwd_final(const Final a) {
+    const float *__restrict__ partial = a.partial;
+    const int splits = a.splits, C = a.C, dt = a.dt;
     __shared__ float sh[GROUPS][COLS];
     const int c = threadIdx.x % COLS, q = threadIdx.x / COLS;
     const int64_t Cp = padded(C), N = 2 * Cp;
@@ -932,9 +977,10 @@ __global__ __launch_bounds__(COLS *GROUPS) void ln_bwd_final(
     if (q != 0 || !mine) return;
 #pragma unroll
     for (int h = 1; h < GROUPS; ++h) s += sh[h][c];
-    void *out = at < Cp ? dgamma : dbeta;
+    void *out = at < Cp ? a.dgamma : a.dbeta;
     if (!out) return;
-    fg::store_from_f(out, dt, i, (at < Cp ? acc_g : acc_b) ? fg::load_as_f(out, dt, i) + s : s);
+    const int acc = at < Cp ? a.acc_g : a.acc_b;
+    fg::store_from_f(out, dt, i, acc ? fg::load_as_f(out, dt, i) + s : s);
 }
 
 constexpr int kFewSums = 64;  // (bf16 512 x 65536: 32 sums a column 12 us, by 4 threads 5)
@@ -986,32 +1032,30 @@ template <int DT>
 void launch_fwd(fg_ctx *ctx, const void *x, int ldx, const void *gamma, const void *beta,
                 float eps, int R, int C, void *y, int ldy, float *mean, float *rstd) {
     using T = typename Io<DT>::T;
-    const T *xt = static_cast<const T *>(x), *gt = static_cast<const T *>(gamma),
-            *bt = static_cast<const T *>(beta);
-    T *yt = static_cast<T *>(y);
+    const Fwd<T> a{static_cast<const T *>(x), static_cast<const T *>(gamma),
+                   static_cast<const T *>(beta), static_cast<T *>(y), mean, rstd, eps, ldx, ldy, R,
+                   C};
     const bool few = R < 2 * ctx->cu_count;
     const bool held = fwd_kind(C / Io<DT>::E, few, [&](auto nv, auto l, auto ng) {
         // Waves a CU walking the rows: all it holds, or 12 where a lane holds more than a
         // chunk (bf16 16384 x 512 7.6 us, with 12 8.8; 8192 x 1024 7.5, with 32 8.3).
         const int per_cu = (nv() == 1 ? 32 : 12) * 64 / (l() * ng());
         const int grid = std::min((R - 1) / ng() + 1, ctx->cu_count * std::max(1, per_cu));
-        ln_fwd<DT, nv(), l(), ng()><<<grid, l() * ng(), 0, ctx->stream>>>(
-            xt, ldx, gt, bt, eps, R, C, yt, ldy, mean, rstd);
+        ln_fwd<DT, nv(), l(), ng()><<<grid, l() * ng(), 0, ctx->stream>>>(a);
     });
     const int chunks = C / Io<DT>::E;
     if (held) return;
-#define FG_LN_WIDE(NV, L)                                                                       \
-    if (chunks <= NV * L) {                                                                     \
-        ln_fwd_wide<DT, NV, L><<<R, L, 0, ctx->stream>>>(xt, ldx, gt, bt, eps, C, yt, ldy, mean, \
-                                                         rstd);                                 \
-        return;                                                                                 \
+#define FG_LN_WIDE(NV, L)                                 \
+    if (chunks <= NV * L) {                               \
+        ln_fwd_wide<DT, NV, L><<<R, L, 0, ctx->stream>>>(a); \
+        return;                                           \
     }
     FG_LN_WIDE(4, 256)
     FG_LN_WIDE(4, 512)
     FG_LN_WIDE(4, 1024)
     FG_LN_WIDE(8, 1024)
 #undef FG_LN_WIDE
-    ln_fwd_long<DT><<<R, kLongL, 0, ctx->stream>>>(xt, ldx, gt, bt, eps, C, yt, ldy, mean, rstd);
+    ln_fwd_long<DT><<<R, kLongL, 0, ctx->stream>>>(a);
 }
 
 // How a backward call's rows are shared out: workgroups of the held rows, or the
@@ -1041,78 +1085,90 @@ Split split_of(int cus, int dtype, int R, int C) {
 }
 
 template <int DT>
-int launch_bwd(fg_ctx *ctx, const Split &s, const void *x, int ldx, const void *dy, int lddy,
-               const void *gamma, const float *mean, const float *rstd, int R, int C, void *dx,
-               int lddx, int accumulate, float *partial) {
-    using T = typename Io<DT>::T;
-    const T *xt = static_cast<const T *>(x), *dt = static_cast<const T *>(dy),
-            *gt = static_cast<const T *>(gamma);
-    T *ot = static_cast<T *>(dx);
+int launch_bwd(fg_ctx *ctx, const Split &s, const Bwd<typename Io<DT>::T> &a) {
     hipStream_t st = ctx->stream;
+    const int chunks = a.C / Io<DT>::E;
     if (s.held) {
-        bwd_kind<DT>(C / Io<DT>::E, [&](auto nv, auto l, auto ng) {
-            const size_t lds = ng() > 1 ? 2 * (size_t)padded(C) * sizeof(float) : 0;
-            if (partial)
-                ln_bwd<DT, nv(), l(), ng(), true><<<s.splits, l() * ng(), lds, st>>>(
-                    xt, ldx, dt, lddy, gt, mean, rstd, R, C, ot, lddx, accumulate, partial);
+        bwd_kind<DT>(chunks, [&](auto nv, auto l, auto ng) {
+            const size_t lds = ng() > 1 ? 2 * (size_t)padded(a.C) * sizeof(float) : 0;
+            if (a.partial)
+                ln_bwd<DT, nv(), l(), ng(), true><<<s.splits, l() * ng(), lds, st>>>(a);
             else
-                ln_bwd<DT, nv(), l(), ng(), false><<<s.splits, l() * ng(), 0, st>>>(
-                    xt, ldx, dt, lddy, gt, mean, rstd, R, C, ot, lddx, accumulate, partial);
+                ln_bwd<DT, nv(), l(), ng(), false><<<s.splits, l() * ng(), 0, st>>>(a);
         });
         FG_LAUNCH_CHECK("ln_bwd");
         return FG_OK;
     }
-    if (s.wide && partial) {
-        const int chunks = C / Io<DT>::E;
+    if (s.wide && a.partial) {
         auto kernel = ln_bwd_wide<DT, 2>;
         if constexpr (DT == fg::kF32)
             if (chunks > 2 * 1024) kernel = ln_bwd_wide<DT, 4>;
-        kernel<<<s.splits, 1024, 0, st>>>(xt, ldx, dt, lddy, gt, mean, rstd, R, C, ot, lddx,
-                                          accumulate, partial);
+        kernel<<<s.splits, 1024, 0, st>>>(a);
         FG_LAUNCH_CHECK("ln_bwd_wide");
         return FG_OK;
     }
     // The weights' gradients first: dx may be written over x or dy.
-    if (partial) {
-        ln_bwd_cols<DT><<<dim3(s.strips, s.splits), kColsNT, 0, st>>>(xt, ldx, dt, lddy, mean, rstd,
-                                                                     R, C, s.rows, partial);
+    if (a.partial) {
+        ln_bwd_cols<DT><<<dim3(s.strips, s.splits), kColsNT, 0, st>>>(a);
         FG_LAUNCH_CHECK("ln_bwd_cols");
     }
-    if (dx && C / Io<DT>::E <= 8 * 1024) {
-        const int chunks = C / Io<DT>::E;
+    if (a.dx && chunks <= 8 * 1024) {
         auto kernel = chunks <= 2 * 1024   ? ln_bwd_dx<DT, 2>
                       : chunks <= 4 * 1024 ? ln_bwd_dx<DT, 4>
                                            : ln_bwd_dx<DT, 8>;
-        kernel<<<R, 1024, 0, st>>>(xt, ldx, dt, lddy, gt, mean, rstd, C, ot, lddx, accumulate);
+        kernel<<<a.R, 1024, 0, st>>>(a);
         FG_LAUNCH_CHECK("ln_bwd_dx");
-    } else if (dx) {
-        ln_bwd_long<DT><<<R, kLongL, 0, st>>>(xt, ldx, dt, lddy, gt, mean, rstd, C, ot, lddx,
-                                              accumulate);
+    } else if (a.dx) {
+        ln_bwd_long<DT><<<a.R, kLongL, 0, st>>>(a);
         FG_LAUNCH_CHECK("ln_bwd_long");
     }
     return FG_OK;
 }
 
 template <int DT>
-int launch_bwd_few(fg_ctx *ctx, const void *x, int ldx, const void *dy, int lddy,
-                   const void *gamma, const float *mean, const float *rstd, int R, int C, void *dx,
-                   int lddx, int accumulate, void *dgamma, int acc_g, void *dbeta, int acc_b) {
-    using T = typename Io<DT>::T;
-    const int row_blocks = dx ? R : 0;
-    const int strips = dgamma || dbeta ? (C / Io<DT>::E + C % Io<DT>::E - 1) / kFewLanes + 1 : 0;
+int launch_bwd_few(fg_ctx *ctx, Bwd<typename Io<DT>::T> a) {
+    constexpr int E = Io<DT>::E;
+    const int strips = a.dgamma || a.dbeta ? (a.C / E + a.C % E - 1) / kFewLanes + 1 : 0;
     auto launch = [&](int rows, int cols) {
         if (rows + cols == 0) return;
-        ln_bwd_few<DT><<<rows + cols, kLongL, 0, ctx->stream>>>(
-            static_cast<const T *>(x), ldx, static_cast<const T *>(dy), lddy,
-            static_cast<const T *>(gamma), mean, rstd, R, C, static_cast<T *>(dx), lddx,
-            accumulate, dgamma, acc_g, dbeta, acc_b, rows);
+        a.row_blocks = rows;
+        ln_bwd_few<DT><<<rows + cols, kLongL, 0, ctx->stream>>>(a);
     };
     // The columns first where dx replaces what they read.
-    const bool in_place = dx && (dx == x || dx == dy);
+    const bool in_place = a.dx && (a.dx == a.x || a.dx == a.dy);
     if (in_place) launch(0, strips);
-    launch(row_blocks, in_place ? 0 : strips);
+    launch(a.dx ? a.R : 0, in_place ? 0 : strips);
     FG_LAUNCH_CHECK("ln_bwd_few");
     return FG_OK;
+}
+
+// The rows' launches: all of a few rows' backward, else dx and the partial sums.
+template <int DT>
+int launch_rows(fg_ctx *ctx, const Split &s, const void *x, int ldx, const void *dy, int lddy,
+                const void *gamma, const float *mean, const float *rstd, int R, int C, void *dx,
+                int lddx, int accumulate, void *dgamma, int acc_g, void *dbeta, int acc_b,
+                float *partial) {
+    using T = typename Io<DT>::T;
+    Bwd<T> a{};
+    a.x = static_cast<const T *>(x);
+    a.dy = static_cast<const T *>(dy);
+    a.gamma = static_cast<const T *>(gamma);
+    a.mean = mean;
+    a.rstd = rstd;
+    a.dx = static_cast<T *>(dx);
+    a.partial = partial;
+    a.ldx = ldx;
+    a.lddy = lddy;
+    a.lddx = lddx;
+    a.R = R;
+    a.C = C;
+    a.accumulate = accumulate;
+    a.rows = s.rows;
+    a.dgamma = dgamma;
+    a.acc_g = acc_g;
+    a.dbeta = dbeta;
+    a.acc_b = acc_b;
+    return R <= kFewRows ? launch_bwd_few<DT>(ctx, a) : launch_bwd<DT>(ctx, s, a);
 }
 
 // Rows that registers do not hold two of take a workgroup each, of 1024 threads at most.
@@ -1187,35 +1243,31 @@ FG_API int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, c
     FG_REQUIRE(rows_fit(dtype, R, C), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns", who, R, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     FG_HIP(hipSetDevice(ctx->device));
-    if (R > 0 && R <= kFewRows) {
-        auto launch = dtype == FG_DTYPE_F32    ? launch_bwd_few<fg::kF32>
-                      : dtype == FG_DTYPE_BF16 ? launch_bwd_few<fg::kBF16>
-                                               : launch_bwd_few<fg::kF16>;
-        return launch(ctx, d_x, ldx, d_dy, lddy, d_gamma, d_mean, d_rstd, R, C, d_dx, lddx,
-                      accumulate, d_dgamma, dgamma_accumulate, d_dbeta, dbeta_accumulate);
-    }
     const Split s = split_of(ctx->cu_count, dtype, R, C);
+    const bool few = R > 0 && R <= kFewRows;
     float *partial = nullptr;
-    if (d_dgamma || d_dbeta) {
+    if ((d_dgamma || d_dbeta) && !few) {
         partial =
             (float *)fg::workspace(ctx, fg::layer_norm_bwd_ws_bytes(ctx->cu_count, dtype, R, C));
         if (!partial) return FG_ERR_OUT_OF_MEMORY;
     }
-    if (R > 0 && (d_dx || partial)) {
-        auto launch = dtype == FG_DTYPE_F32    ? launch_bwd<fg::kF32>
-                      : dtype == FG_DTYPE_BF16 ? launch_bwd<fg::kBF16>
-                                               : launch_bwd<fg::kF16>;
+    if (R > 0 && (d_dx || d_dgamma || d_dbeta)) {
+        auto launch = dtype == FG_DTYPE_F32    ? launch_rows<fg::kF32>
+                      : dtype == FG_DTYPE_BF16 ? launch_rows<fg::kBF16>
+                                               : launch_rows<fg::kF16>;
         if (int rc = launch(ctx, s, d_x, ldx, d_dy, lddy, d_gamma, d_mean, d_rstd, R, C, d_dx, lddx,
-                            accumulate, partial))
+                            accumulate, d_dgamma, dgamma_accumulate, d_dbeta, dbeta_accumulate,
+                            partial))
             return rc;
     }
     if (partial) {
         // 32 threads a column (half of them: 0.2 to 0.5 us longer), or 4 for few sums.
+        const Final f{partial, d_dgamma, d_dbeta, dtype, s.splits, C, dgamma_accumulate,
+                      dbeta_accumulate};
         auto final = [&](auto cols, auto groups) {
             ln_bwd_final<cols(), groups()>
                 <<<(unsigned)((2 * padded(C) - 1) / cols() + 1), cols() * groups(), 0,
-                   ctx->stream>>>(dtype, partial, s.splits, C, d_dgamma, dgamma_accumulate, d_dbeta,
-                                  dbeta_accumulate);
+                   ctx->stream>>>(f);
         };
         using std::integral_constant;
         if (s.splits > kFewSums) final(integral_constant<int, 32>{}, integral_constant<int, 32>{});
