@@ -23,8 +23,9 @@
 // 65536 tokens over 131072 rows of 2048 in bf16 (805 MB): sort 32 us, sums 137 at
 // 4.7 TB/s, joins 8.  20011 tokens, four in ten of them one, over 50257 rows of 777 in
 // fp32 (218 MB): order 25 with 93 MB of zeros, sums 25, joins 7.6.
-// A few tokens (kDirectMax) take one launch: every workgroup owns some table rows
-// and lists the tokens that are its own (256 tokens over 1000 rows of 256: 3.8 us).
+// Small batches (own_launch) take one launch, whose workgroups own table rows and order
+// their positions in LDS; the fewest tokens (kDirectMax) one of smaller workgroups, which
+// only list theirs.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -42,7 +43,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
 constexpr int kNT = 256;
-constexpr int kDirectMax = 256;  // (a token a thread)
+constexpr int kDirectMax = 32;
 // Tokens that all of emb_order's workgroups read: 40960 a workgroup where there are 256.
 // It takes 8.6 us for 8192 tokens, 15 for 16384, 22 for 32768 (as much again where zeros
 // share the CUs); the radix sort's launches 24 or more for any of these.  All of the
@@ -115,6 +116,9 @@ __global__ __launch_bounds__(kNT) void emb_fwd(const Lookup<typename Io<DT>::T> 
 }
 
 // --------------------------------------------------- few tokens: one launch
+// (Zeros of 65 MB beside 64 tokens 13.9 us, as emb_bwd_own 16.8; but 64 tokens of 10 rows
+// of 256 10.2 and 6.3, and 256 of which four in ten are one 33.7 and 16.3: a row's lanes
+// walk the list from its first token to its last.)
 // A workgroup owns `rows` table rows from blockIdx.x * rows on: it lists the
 // positions of their tokens in order, then each group of 2^lshift lanes adds the
 // rows of its own tokens.
@@ -222,33 +226,24 @@ __device__ __forceinline__ void zero_rows(const Zero &z, int block, int blocks) 
 }
 
 // ------------------------------------------------------------------- sorting
-// order[k] = the k-th position in (token, position) order, sorted[k] its token: each
-// workgroup owns `bins` tokens and reads all of the batch.  Its waves take a run of
-// positions each and count the tokens below the workgroup's and each of its own; the
-// counts' prefix sums, by token and then by wave, are where a second reading places
-// the workgroup's positions.  64 positions that hold none of its tokens, as most do,
-// cost two comparisons.  Tokens outside the table sort as V.
+// The positions of a workgroup's own tokens, `n` of them from v0 on, in (token, position)
+// order.  Its waves take a run of the batch each and count the tokens below the
+// workgroup's (where BELOW) and each of its own; the counts' prefix sums, by token and
+// then by wave, are where a second reading places its positions: start(token, where,
+// count) by a thread for each token, then place(where, position, key).  64 positions
+// that hold none of its tokens, as most do, cost two comparisons.  Tokens outside the
+// table count as V.
 constexpr int kOrderNT = 1024, kOrderWaves = kOrderNT / 64;
-constexpr int kOrderBlocks = 256, kOrderBins = 1024;  // at least; at most
-struct Order {
-    const uint32_t *tokens;
-    uint32_t *order, *sorted;
-    int count, bins, blocks;
-    uint32_t V;
+constexpr int kOrderBlocks = 256, kOrderBins = 1024;  // workgroups at least; tokens at most
+struct OrderLds {
+    uint32_t wbelow[kOrderWaves], wsum[kOrderWaves];
 };
-__global__ __launch_bounds__(kOrderNT) void emb_order(const Order p, const Zero z) {
-    const uint32_t *__restrict__ tokens = p.tokens;
-    uint32_t *__restrict__ order = p.order, *__restrict__ sorted = p.sorted;
-    const int T = p.count, bins = p.bins, blocks = p.blocks;
-    const uint32_t V = p.V;
-    __shared__ uint32_t cnt[kOrderWaves * kOrderBins];  // [wave][bins]
-    __shared__ uint32_t wbelow[kOrderWaves], wsum[kOrderWaves];
-    if ((int)blockIdx.x >= blocks) {
-        zero_rows(z, blockIdx.x - blocks, gridDim.x - blocks);
-        return;
-    }
+template <bool BELOW, class S, class P>
+__device__ __forceinline__ void order_own(const uint32_t *__restrict__ tokens, int T, uint32_t V,
+                                          uint32_t v0, uint32_t n, int bins, OrderLds &lds,
+                                          uint32_t *cnt, S start, P place) {  // cnt[wave][bins]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t v0 = blockIdx.x * (uint32_t)bins, n = min((uint32_t)bins, V + 1 - v0);
+    // (An odd number of 64s: the waves' runs then begin in different memory channels.)
     const int per = (((T - 1) / kOrderNT + 1) | 1) * 64, i0 = wave * per, i1 = min(T, i0 + per);
     constexpr int kBatch = 8;  // loads of a lane in flight
     uint32_t *mine = cnt + wave * bins;
@@ -290,13 +285,13 @@ __global__ __launch_bounds__(kOrderNT) void emb_order(const Order p, const Zero 
     __syncthreads();
     uint32_t below = 0;
     scan([&](uint32_t key, int) {
-        below += (uint32_t)__popcll(__ballot(key < v0));
+        if constexpr (BELOW) below += (uint32_t)__popcll(__ballot(key < v0));
         each(key - v0, [&](uint32_t own, uint64_t m) {
             if (key - v0 == own && !(m & ((1ull << lane) - 1)))  // (one lane)
                 atomicAdd(&mine[own], (uint32_t)__popcll(m));
         });
     });
-    if (lane == 0) wbelow[wave] = below;
+    if (lane == 0) lds.wbelow[wave] = below;
     __syncthreads();
     // A thread a bin.
     uint32_t total = 0;
@@ -309,13 +304,14 @@ __global__ __launch_bounds__(kOrderNT) void emb_order(const Order p, const Zero 
         const uint32_t up = __shfl_up(incl, o);
         if (lane >= o) incl += up;
     }
-    if (lane == 63) wsum[wave] = incl;
+    if (lane == 63) lds.wsum[wave] = incl;
     __syncthreads();
     uint32_t at = incl - total, all = 0;
     for (int w = 0; w < kOrderWaves; ++w) {
-        at += wbelow[w] + (w < wave ? wsum[w] : 0u);
-        all += wsum[w];
+        at += lds.wbelow[w] + (w < wave ? lds.wsum[w] : 0u);
+        all += lds.wsum[w];
     }
+    if (bin < n) start(bin, at, total);
     if (all == 0) return;
     if (bin < n)
         for (int w = 0; w < kOrderWaves; ++w) {
@@ -330,13 +326,121 @@ __global__ __launch_bounds__(kOrderNT) void emb_order(const Order p, const Zero 
             uint32_t to = 0;
             if (lane == 0) to = atomicAdd(&mine[own], (uint32_t)__popcll(m));
             to = (uint32_t)__builtin_amdgcn_readfirstlane((int)to);
-            if (d == own) {
-                to += (uint32_t)__popcll(m & ((1ull << lane) - 1));
-                order[to] = (uint32_t)i;
-                sorted[to] = key;
-            }
+            if (d == own) place(to + (uint32_t)__popcll(m & ((1ull << lane) - 1)), i, key);
         });
     });
+}
+
+// order[k] = the k-th position in (token, position) order, sorted[k] its token.
+struct Order {
+    const uint32_t *tokens;
+    uint32_t *order, *sorted;
+    int count, bins, blocks;
+    uint32_t V;
+};
+__global__ __launch_bounds__(kOrderNT) void emb_order(const Order p, const Zero z) {
+    __shared__ OrderLds lds;
+    extern __shared__ uint32_t cnt[];
+    if ((int)blockIdx.x >= p.blocks) {
+        zero_rows(z, blockIdx.x - p.blocks, gridDim.x - p.blocks);
+        return;
+    }
+    const uint32_t v0 = blockIdx.x * (uint32_t)p.bins, n = min((uint32_t)p.bins, p.V + 1 - v0);
+    uint32_t *__restrict__ order = p.order, *__restrict__ sorted = p.sorted;
+    order_own<true>(p.tokens, p.count, p.V, v0, n, p.bins, lds, cnt,
+                    [](uint32_t, uint32_t, uint32_t) {},
+                    [&](uint32_t to, int i, uint32_t key) {
+                        order[to] = (uint32_t)i;
+                        sorted[to] = key;
+                    });
+}
+
+// All of a small batch's gradient in one launch: a workgroup zeroes its own table rows,
+// which overlaps the ordering of their positions in LDS, then 2^lshift lanes take a row
+// with tokens each, or all of them a share of a row of many tokens (kOwnMany), whose
+// sums are added in order.
+// (kOwnBlocks: with 512, fp32 448 tokens over 2568 rows of 42 8.8 us, 256 6.2.)
+constexpr int kOwnMax = 4096, kOwnMany = 32, kOwnBlocks = 256;
+template <int DT>
+__global__ __launch_bounds__(kOrderNT) void emb_bwd_own(const Few<typename Io<DT>::T> p) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E;
+    __shared__ OrderLds lds;
+    __shared__ uint32_t many[kOwnMax / kOwnMany], nfew, nmany;
+    extern __shared__ uint32_t cnt[];
+    uint32_t *first = cnt + kOrderWaves * p.rows, *few = first + p.rows + 1;
+    uint32_t *list = few + p.rows;  // (few, many: rows, in any order)
+    __shared__ f32x4 part[E / 4][kOrderNT];
+    const auto *__restrict__ dout = p.dout;
+    const uint32_t v0 = blockIdx.x * (uint32_t)p.rows, n = min((uint32_t)p.rows, p.V - v0);
+    const int chunks = (p.C - 1) / E + 1, lanes = 1 << p.lshift, groups = kOrderNT >> p.lshift;
+    const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> p.lshift;
+    const int j = blockIdx.y * lanes + lane;
+    const Tail<DT> at_j(min(j, chunks - 1), p.C);
+    if (threadIdx.x == 0) nfew = nmany = 0;
+    float a[E] = {};
+    if (!p.accumulate && j < chunks)
+        for (uint32_t r = group; r < n; r += groups)
+            at_j.store(p.dtable + (size_t)(v0 + r) * p.lddt, a);
+    order_own<false>(p.tokens, p.count, (uint32_t)p.V, v0, n, p.rows, lds, cnt,
+                     [&](uint32_t bin, uint32_t at, uint32_t count) {
+                         first[bin] = at;
+                         if (bin + 1 == n) first[n] = at + count;
+                         if (count > kOwnMany) many[atomicAdd(&nmany, 1u)] = bin;
+                         else if (count) few[atomicAdd(&nfew, 1u)] = bin;
+                     },
+                     [&](uint32_t to, int i, uint32_t) { list[to] = (uint32_t)i; });
+    // (The zeros of a row are written before its sum, by whichever wave.)
+    __threadfence_block();
+    __syncthreads();
+    // list[k0, k1) in order.
+    auto sum = [&](uint32_t k0, uint32_t k1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) a[e] = 0.0f;
+        for (uint32_t k = k0; k < k1; k += 8) {
+            u32x4 w[8];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) {
+                w[u] = u32x4{0u, 0u, 0u, 0u};
+                if (k + u < k1) w[u] = at_j.load(dout + (size_t)list[k + u] * p.lddo);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < E; ++e) a[e] += IO::get(w[u], e);
+        }
+    };
+    auto put = [&](uint32_t bin) {
+        auto *to = p.dtable + (size_t)(v0 + bin) * p.lddt;
+#pragma unroll
+        for (int e = 0; e < E; ++e) a[e] *= p.scale;
+        if (p.accumulate) at_j.add(to, j, a);
+        else at_j.store(to, a);
+    };
+    if (j < chunks)
+        for (uint32_t h = group; h < nfew; h += groups) {
+            const uint32_t bin = few[h];
+            sum(first[bin], first[bin + 1]);
+            put(bin);
+        }
+    for (uint32_t h = 0; h < nmany; ++h) {
+        const uint32_t bin = many[h], k0 = first[bin], k1 = first[bin + 1];
+        const uint32_t per = max(8u, (k1 - k0 - 1) / groups + 1), k = k0 + group * per;
+        sum(min(k, k1), min(k + per, k1));
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q)
+            part[q][threadIdx.x] = f32x4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+        __syncthreads();
+        if (group == 0 && j < chunks) {
+            const int used = (int)((k1 - k0 - 1) / per + 1);
+#pragma unroll 4
+            for (int g = 1; g < used; ++g)
+#pragma unroll
+                for (int e = 0; e < E; ++e) a[e] += part[e / 4][(g << p.lshift) + lane][e % 4];
+            put(bin);
+        }
+        __syncthreads();
+    }
 }
 
 // Stable radix sort, least significant digit first, of (token, position) pairs:
@@ -731,6 +835,16 @@ int log2_up(int64_t n) {
 // Lanes that take a row of `chunks` chunks: a power of two, at most a workgroup.
 int lane_shift(int chunks) { return std::min(8, log2_up(chunks)); }
 
+// Whether emb_bwd_own takes the batch: one workgroup reads all of a token's rows, 1 KB of
+// each, so at most 1 MB; and at most 1024 workgroups order the batch each.  bf16, four
+// tokens in ten one, 32000 rows of 1024: 1024 tokens 20.2 us (three launches 23.5), 2048
+// 25.6 (25.0), 4096 37.2 (24.0); fp32 448 tokens, 2568 rows of 42 6.2 (12.7); 512 tokens,
+// 2000000 rows of 16 37.8 (33.4).
+bool own_launch(int dtype, int T, int V, int C) {
+    const int64_t row = (int64_t)C * (dtype == FG_DTYPE_F32 ? 4 : 2);
+    return T <= kOwnMax && V <= 1024 * kOrderBins && T * std::min<int64_t>(row, 1024) <= 1 << 20;
+}
+
 // How a gradient of T tokens over rows of C columns is laid out.
 struct Plan {
     int P, units, lshift;
@@ -744,7 +858,7 @@ struct Plan {
 };
 Plan plan_of(int dtype, int T, int V, int C) {
     Plan p{};
-    if (T <= kDirectMax) return p;
+    if (T <= kDirectMax || own_launch(dtype, T, V, C)) return p;
     const int E = dtype == FG_DTYPE_F32 ? 4 : 8, chunks = (C - 1) / E + 1;
     p.lshift = lane_shift(chunks);
     p.Cp = (int64_t)chunks * E;
@@ -805,6 +919,16 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
         return FG_OK;
     }
     uint32_t *order = (uint32_t *)ws, *sorted = order + T;
+    if (own_launch(DT, T, V, C)) {
+        const int lshift = std::min(6, log2_up(chunks)), tiles = ((chunks - 1) >> lshift) + 1;
+        const int blocks = std::max(1, kOwnBlocks / tiles);
+        const int rows = std::min(kOrderBins, (V - 1) / blocks + 1);
+        const size_t lds = 4 * ((size_t)(kOrderWaves + 2) * rows + 1 + T);
+        emb_bwd_own<DT><<<dim3((V - 1) / rows + 1, tiles), kOrderNT, lds, st>>>(
+            {tokens, d, g, T, V, C, lddo, lddt, accumulate, rows, lshift, scale});
+        FG_LAUNCH_CHECK("emb_bwd_own");
+        return FG_OK;
+    }
     // Zeroed beside the sort, which leaves the memory idle: what its launches have time
     // for; the whole table where that is most of it, or where few of its rows are
     // written again.  The rest goes beside the sums, without the rows of tokens.
@@ -831,7 +955,7 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
     };
     if (pl.passes == 0) {
         const int zeros = share(order_mb);
-        emb_order<<<pl.blocks + zeros, kOrderNT, 0, st>>>(
+        emb_order<<<pl.blocks + zeros, kOrderNT, 4 * kOrderWaves * pl.bins, st>>>(
             {tokens, order, sorted, T, pl.bins, pl.blocks, (uint32_t)V}, z);
         FG_LAUNCH_CHECK("emb_order");
     } else {
@@ -899,8 +1023,8 @@ uint64_t embedding_bwd_ws_bytes(int dtype, int T, int V, int C) {
     return plan_of(dtype, T, V, C).bytes();
 }
 int embedding_bwd_dispatches(int dtype, int T, int V, int C) {
-    if (T <= kDirectMax) return 1;
     const Plan p = plan_of(dtype, T, V, C);
+    if (p.units == 0) return 1;
     return (p.passes ? 2 * p.passes : 1) + 1 + (p.units > 1 ? 1 : 0);
 }
 }  // namespace fg
@@ -949,7 +1073,7 @@ FG_API int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, in
     FG_HIP(hipSetDevice(ctx->device));
     const Plan pl = plan_of(dtype, T, V, C);
     void *ws = nullptr;
-    if (T > kDirectMax && !(ws = fg::workspace(ctx, pl.bytes()))) return FG_ERR_OUT_OF_MEMORY;
+    if (pl.units > 0 && !(ws = fg::workspace(ctx, pl.bytes()))) return FG_ERR_OUT_OF_MEMORY;
     auto launch = dtype == FG_DTYPE_F32    ? launch_bwd<fg::kF32>
                   : dtype == FG_DTYPE_BF16 ? launch_bwd<fg::kBF16>
                                            : launch_bwd<fg::kF16>;

@@ -318,7 +318,8 @@ EMB_SHAPES = [  # T, V, C, pad, start
     (3001, 1009, 130, 3, 0), (4096, 64, 512, 8, 0), (4097, 300, 2051, 0, 1), (9000, 32000, 96, 0, 0),
     (20011, 257, 48, 0, 0), (40000, 5000, 24, 0, 0), (70000, 131072, 16, 0, 0),
     (131072, 3, 40, 0, 0), (300, 9, 8192, 0, 0), (50, 9, 20000, 0, 0), (257, 1, 24, 0, 0),
-    (2000, 255, 16, 0, 0), (2000, 256, 16, 0, 0), (3000, 262144, 8, 0, 0)]
+    (2000, 255, 16, 0, 0), (2000, 256, 16, 0, 0), (3000, 262144, 8, 0, 0),
+    (32, 40, 72, 0, 0), (33, 40, 1100, 2, 1), (1025, 77, 600, 0, 0), (4096, 1000, 120, 1, 1)]
 
 
 @pytest.mark.parametrize("dt", DTS)
