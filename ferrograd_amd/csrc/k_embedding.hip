@@ -41,6 +41,8 @@ using fg::rows::Tail;
 using fg::rows::u32x4;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
+using fg::rows::u32x2;
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
 
 constexpr int kNT = 256;
 constexpr int kDirectMax = 32;
@@ -817,13 +819,36 @@ __global__ __launch_bounds__(kJoinNT) void emb_join(const Sums p, typename Io<DT
         for (int w = 1; w < used; ++w) a += sh[threadIdx.x + (w << lshift)];
     }
     if (col >= p.Cp) return;
-    auto *to = dtable + (size_t)v * p.lddt;
+    // The 4 columns in one access, or the row's last ones one by one.
+    auto *to = dtable + (size_t)v * p.lddt + col;
+    float o[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (col + e >= p.C) continue;
-        float o = a[e] * p.scale;
-        if (p.accumulate) o += IO::load1(to, (int)col + e);
-        IO::store1(to, (int)col + e, o);
+    for (int e = 0; e < 4; ++e) o[e] = a[e] * p.scale;
+    const bool whole = col + 4 <= p.C;
+    if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (col + e < p.C) IO::store1(to, e, p.accumulate ? o[e] + IO::load1(to, e) : o[e]);
+        return;
+    }
+    if constexpr (DT == fg::kF32) {
+        auto *row = reinterpret_cast<f32x4_any *>(to);
+        f32x4 r = {o[0], o[1], o[2], o[3]};
+        if (p.accumulate) r += *row;
+        *row = r;
+    } else {
+        auto *row = reinterpret_cast<u32x2_any *>(to);
+        u32x4 w = {0u, 0u, 0u, 0u};
+        if (p.accumulate) {
+            const u32x2 was = *row;
+            w[0] = was[0];
+            w[1] = was[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += IO::get(w, e);
+        }
+        const float eight[8] = {o[0], o[1], o[2], o[3]};
+        w = IO::pack(eight);
+        *row = u32x2{w[0], w[1]};
     }
 }
 
