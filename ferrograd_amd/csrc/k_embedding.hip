@@ -22,7 +22,7 @@
 //  * the crossing runs' partial sums are joined in order.
 // 65536 tokens over 131072 rows of 2048 in bf16 (805 MB): sort 32 us, sums 137 at
 // 4.7 TB/s, joins 8.  20011 tokens, four in ten of them one, over 50257 rows of 777 in
-// fp32 (218 MB): order 25 with 93 MB of zeros, sums 25, joins 7.6.
+// fp32 (218 MB): order 25 with 93 MB of zeros, sums 25, joins 7.4.
 // Small batches (own_launch) take one launch, whose workgroups own table rows and order
 // their positions in LDS; the fewest tokens (kDirectMax) one of smaller workgroups, which
 // only list theirs.
@@ -46,6 +46,7 @@ typedef u32x2 u32x2_any __attribute__((aligned(2)));
 
 constexpr int kNT = 256;
 constexpr int kDirectMax = 32;
+constexpr int kOwnMax = 4096;
 // Tokens that all of emb_order's workgroups read: 40960 a workgroup where there are 256.
 // It takes 8.6 us for 8192 tokens, 15 for 16384, 22 for 32768 (as much again where zeros
 // share the CUs); the radix sort's launches 24 or more for any of these.  All of the
@@ -234,20 +235,24 @@ __device__ __forceinline__ void zero_rows(const Zero &z, int block, int blocks) 
 // then by wave, are where a second reading places its positions: start(token, where,
 // count) by a thread for each token, then place(where, position, key).  64 positions
 // that hold none of its tokens, as most do, cost two comparisons.  Tokens outside the
-// table count as V.
+// table count as V.  A wave's run of up to 512 (without BELOW, all of up to kOwnMax
+// tokens) stays in registers between the readings.  idle() runs after the first, its
+// memory accesses beside what follows.
 constexpr int kOrderNT = 1024, kOrderWaves = kOrderNT / 64;
 constexpr int kOrderBlocks = 256, kOrderBins = 1024;  // workgroups at least; tokens at most
 struct OrderLds {
     uint32_t wbelow[kOrderWaves], wsum[kOrderWaves];
 };
-template <bool BELOW, class S, class P>
+template <bool BELOW, class I, class S, class P>
 __device__ __forceinline__ void order_own(const uint32_t *__restrict__ tokens, int T, uint32_t V,
                                           uint32_t v0, uint32_t n, int bins, OrderLds &lds,
-                                          uint32_t *cnt, S start, P place) {  // cnt[wave][bins]
+                                          uint32_t *cnt,  // [wave][bins]
+                                          I idle, S start, P place) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // (An odd number of 64s: the waves' runs then begin in different memory channels.)
     const int per = (((T - 1) / kOrderNT + 1) | 1) * 64, i0 = wave * per, i1 = min(T, i0 + per);
-    constexpr int kBatch = 8;  // loads of a lane in flight
+    // Loads of a lane in flight; of a small batch, all.
+    constexpr int kBatch = BELOW ? 8 : ((kOwnMax - 1) / kOrderNT + 1) | 1;
     uint32_t *mine = cnt + wave * bins;
     // f(its bin, its lanes) for each of the workgroup's tokens of 64 positions, in some
     // order.
@@ -261,15 +266,15 @@ __device__ __forceinline__ void order_own(const uint32_t *__restrict__ tokens, i
             hits &= ~m;
         }
     };
-    auto scan = [&](auto f) {
-        uint32_t next[kBatch];
-        auto load = [&](int i) {
+    uint32_t next[kBatch];
+    auto load = [&](int i) {
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) next[u] = tokens[min(i + 64 * u + lane, T - 1)];
-        };
-        load(i0);
+        for (int u = 0; u < kBatch; ++u) next[u] = tokens[min(i + 64 * u + lane, T - 1)];
+    };
+    load(i0);
+    auto scan = [&](auto f) {  // (next: the run's first)
         int i = i0;
-        for (; i + 64 * kBatch <= i1; i += 64 * kBatch) {
+        for (; BELOW && i + 64 * kBatch <= i1; i += 64 * kBatch) {
             uint32_t key[kBatch];
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) key[u] = min(next[u], V);
@@ -294,6 +299,7 @@ __device__ __forceinline__ void order_own(const uint32_t *__restrict__ tokens, i
         });
     });
     if (lane == 0) lds.wbelow[wave] = below;
+    idle();
     __syncthreads();
     // A thread a bin.
     uint32_t total = 0;
@@ -321,6 +327,7 @@ __device__ __forceinline__ void order_own(const uint32_t *__restrict__ tokens, i
             cnt[w * bins + bin] = at;
             at += c;
         }
+    if (BELOW && per >= 64 * kBatch) load(i0);
     __syncthreads();
     scan([&](uint32_t key, int i) {
         const uint32_t d = key - v0;
@@ -350,19 +357,20 @@ __global__ __launch_bounds__(kOrderNT) void emb_order(const Order p, const Zero 
     const uint32_t v0 = blockIdx.x * (uint32_t)p.bins, n = min((uint32_t)p.bins, p.V + 1 - v0);
     uint32_t *__restrict__ order = p.order, *__restrict__ sorted = p.sorted;
     order_own<true>(p.tokens, p.count, p.V, v0, n, p.bins, lds, cnt,
-                    [](uint32_t, uint32_t, uint32_t) {},
+                    [] {}, [](uint32_t, uint32_t, uint32_t) {},
                     [&](uint32_t to, int i, uint32_t key) {
                         order[to] = (uint32_t)i;
                         sorted[to] = key;
                     });
 }
 
-// All of a small batch's gradient in one launch: a workgroup zeroes its own table rows,
-// which overlaps the ordering of their positions in LDS, then 2^lshift lanes take a row
+// All of a small batch's gradient in one launch: a workgroup zeroes its own table rows
+// beside the ordering of their positions in LDS (whose tokens are in registers by then:
+// loads wait for the stores before them), then 2^lshift lanes take a row
 // with tokens each, or all of them a share of a row of many tokens (kOwnMany), whose
 // sums are added in order.
-// (kOwnBlocks: with 512, fp32 448 tokens over 2568 rows of 42 8.8 us, 256 6.2.)
-constexpr int kOwnMax = 4096, kOwnMany = 32, kOwnBlocks = 256;
+// (kOwnBlocks: fp32 448 tokens over 2568 rows of 42 8.8 us with 512, 6.2 with 256.)
+constexpr int kOwnMany = 32, kOwnBlocks = 256;
 template <int DT>
 __global__ __launch_bounds__(kOrderNT) void emb_bwd_own(const Few<typename Io<DT>::T> p) {
     using IO = Io<DT>;
@@ -381,10 +389,12 @@ __global__ __launch_bounds__(kOrderNT) void emb_bwd_own(const Few<typename Io<DT
     const Tail<DT> at_j(min(j, chunks - 1), p.C);
     if (threadIdx.x == 0) nfew = nmany = 0;
     float a[E] = {};
-    if (!p.accumulate && j < chunks)
-        for (uint32_t r = group; r < n; r += groups)
-            at_j.store(p.dtable + (size_t)(v0 + r) * p.lddt, a);
-    order_own<false>(p.tokens, p.count, (uint32_t)p.V, v0, n, p.rows, lds, cnt,
+    auto zero = [&] {
+        if (!p.accumulate && j < chunks)
+            for (uint32_t r = group; r < n; r += groups)
+                at_j.store(p.dtable + (size_t)(v0 + r) * p.lddt, a);
+    };
+    order_own<false>(p.tokens, p.count, (uint32_t)p.V, v0, n, p.rows, lds, cnt, zero,
                      [&](uint32_t bin, uint32_t at, uint32_t count) {
                          first[bin] = at;
                          if (bin + 1 == n) first[n] = at + count;
@@ -863,7 +873,7 @@ int lane_shift(int chunks) { return std::min(8, log2_up(chunks)); }
 // Whether emb_bwd_own takes the batch: one workgroup reads all of a token's rows, 1 KB of
 // each, so at most 1 MB; and at most 1024 workgroups order the batch each.  bf16, four
 // tokens in ten one, 32000 rows of 1024: 1024 tokens 20.2 us (three launches 23.5), 2048
-// 25.6 (25.0), 4096 37.2 (24.0); fp32 448 tokens, 2568 rows of 42 6.2 (12.7); 512 tokens,
+// 25.6 (25.0), 4096 37.2 (24.0); fp32 448 tokens, 2568 rows of 42 5.8 (12.7); 512 tokens,
 // 2000000 rows of 16 37.8 (33.4).
 bool own_launch(int dtype, int T, int V, int C) {
     const int64_t row = (int64_t)C * (dtype == FG_DTYPE_F32 ? 4 : 2);
