@@ -76,7 +76,7 @@ struct Bwd {
     T *dx;
     float *partial;
     int ldx, lddy, lddx, R, C, accumulate;
-    int rows;           // ln_bwd_cols: of a split
+    int rows;           // ln_bwd_cols: of a split; ln_bwd_few: of a workgroup
     int row_blocks;     // ln_bwd_few
     void *dgamma, *dbeta;
     int acc_g, acc_b;
@@ -746,7 +746,8 @@ __global__ __launch_bounds__(1024) void ln_bwd_dx(const Bwd<typename Io<DT>::T> 
     }
 }
 
-template <int DT>
+// A row by L lanes, twice from memory.
+template <int DT, int L>
 __device__ __forceinline__ void bwd_long_row(size_t r, const Bwd<typename Io<DT>::T> &a,
                                              float (*sm)[kLongL / 64]) {
     const auto *x = a.x, *dy = a.dy;
@@ -758,7 +759,7 @@ __device__ __forceinline__ void bwd_long_row(size_t r, const Bwd<typename Io<DT>
     constexpr int E = IO::E;
     const auto *xr = x + r * ldx, *dr = dy + r * lddy;
     auto *out = dx + r * lddx;
-    const int t = threadIdx.x;
+    const int t = threadIdx.x % L;
     const Lanes<DT> ln(C, t);
     const bool one = ln.single < C;
     const float n = (float)C, m = mean[r], k = rstd[r];
@@ -783,7 +784,7 @@ __device__ __forceinline__ void bwd_long_row(size_t r, const Bwd<typename Io<DT>
         }
     };
 #pragma unroll 4
-    for (int j = t; j < ln.nb; j += kLongL) {
+    for (int j = t; j < ln.nb; j += L) {
         float c[E], gd[E], p1 = 0.0f, p2 = 0.0f;
         chunk(j, c, gd);
 #pragma unroll
@@ -794,10 +795,10 @@ __device__ __forceinline__ void bwd_long_row(size_t r, const Bwd<typename Io<DT>
         s1 += p1;
         s2 += p2;
     }
-    const float m1 = row_sum<kLongL>(s1, sm[0], t) / n;
-    const float m2 = k * (k * row_sum<kLongL>(s2, sm[1], t) / n);
+    const float m1 = row_sum<L>(s1, sm[0], t) / n;
+    const float m2 = k * (k * row_sum<L>(s2, sm[1], t) / n);
 #pragma unroll 2
-    for (int j = t; j < ln.nb; j += kLongL) {
+    for (int j = t; j < ln.nb; j += L) {
         float c[E], o[E];
         chunk(j, c, o);
 #pragma unroll
@@ -819,15 +820,18 @@ __device__ __forceinline__ void bwd_long_row(size_t r, const Bwd<typename Io<DT>
 template <int DT>
 __global__ __launch_bounds__(kLongL) void ln_bwd_long(const Bwd<typename Io<DT>::T> a) {
     __shared__ float sm[2][kLongL / 64];
-    bwd_long_row<DT>(blockIdx.x, a, sm);
+    bwd_long_row<DT, kLongL>(blockIdx.x, a, sm);
 }
 
-// Few rows (kFewRows), where launches count: one for everything, workgroups of one
-// row for dx, and behind them workgroups of 16 chunks of columns for the weights,
-// whose 64 groups of lanes take every 64th row and are added in order.  bf16, in two
+// Few rows (kFewRows, or kFewShort short ones), where launches count: one for everything,
+// workgroups of one row, or of 16 short ones, for dx, and behind them workgroups of 16
+// chunks of columns for the weights, whose 64 groups of lanes take every 64th row and are
+// added in order.  bf16, in two
 // launches as below and in this one: 64 x 4096 9.1 us and 6.2, 256 x 16384 22.5 and
-// 12.2; with 512 rows fp32 of 4096 12.1 and 14.9, 512 x 512 8.9 and 9.2.
-constexpr int kFewRows = 256, kFewLanes = 16, kFewGroups = kLongL / kFewLanes;
+// 12.2; 512 x 512 10.0 and 6.5, 640 x 2048 10.2 and 8.5, but 1024 x 2048 10.5 and 11.4,
+// fp32 512 x 4096 12.1 and 14.9.
+constexpr int kFewWave = 256;  // whole chunks of a row that a wave takes
+constexpr int kFewRows = 256, kFewShort = 640, kFewLanes = 16, kFewGroups = kLongL / kFewLanes;
 template <int DT>
 __global__ __launch_bounds__(kLongL) void ln_bwd_few(const Bwd<typename Io<DT>::T> a) {
     const auto *x = a.x, *dy = a.dy;
@@ -838,7 +842,9 @@ __global__ __launch_bounds__(kLongL) void ln_bwd_few(const Bwd<typename Io<DT>::
     __shared__ float sm[2][kLongL / 64];
     __shared__ float sh[kFewGroups][kCols];
     if ((int)blockIdx.x < row_blocks) {
-        bwd_long_row<DT>(blockIdx.x, a, sm);
+        const int r = (int)blockIdx.x * a.rows + (int)(threadIdx.x >> 6);
+        if (a.rows == 1) bwd_long_row<DT, kLongL>(blockIdx.x, a, sm);
+        else if (r < a.R) bwd_long_row<DT, 64>(r, a, sm);
         return;
     }
     const int lane = threadIdx.x % kFewLanes, group = threadIdx.x / kFewLanes;
@@ -1128,11 +1134,13 @@ int launch_bwd(fg_ctx *ctx, const Split &s, const Bwd<typename Io<DT>::T> &a) {
 template <int DT>
 int launch_bwd_few(fg_ctx *ctx, Bwd<typename Io<DT>::T> a) {
     constexpr int E = Io<DT>::E;
+    const int chunks = a.C / E;
     const int strips = a.dgamma || a.dbeta ? (a.C / E + a.C % E - 1) / kFewLanes + 1 : 0;
     auto launch = [&](int rows, int cols) {
         if (rows + cols == 0) return;
-        a.row_blocks = rows;
-        ln_bwd_few<DT><<<rows + cols, kLongL, 0, ctx->stream>>>(a);
+        a.rows = chunks <= kFewWave ? kLongL / 64 : 1;
+        a.row_blocks = rows ? (rows - 1) / a.rows + 1 : 0;
+        ln_bwd_few<DT><<<a.row_blocks + cols, kLongL, 0, ctx->stream>>>(a);
     };
     // The columns first where dx replaces what they read.
     const bool in_place = a.dx && (a.dx == a.x || a.dx == a.dy);
@@ -1140,6 +1148,11 @@ int launch_bwd_few(fg_ctx *ctx, Bwd<typename Io<DT>::T> a) {
     launch(a.dx ? a.R : 0, in_place ? 0 : strips);
     FG_LAUNCH_CHECK("ln_bwd_few");
     return FG_OK;
+}
+
+// Whether a backward takes ln_bwd_few.
+bool few_rows(int dtype, int R, int C) {
+    return R <= kFewRows || (R <= kFewShort && C / (dtype == FG_DTYPE_F32 ? 4 : 8) <= kFewWave);
 }
 
 // The rows' launches: all of a few rows' backward, else dx and the partial sums.
@@ -1168,7 +1181,7 @@ int launch_rows(fg_ctx *ctx, const Split &s, const void *x, int ldx, const void 
     a.acc_g = acc_g;
     a.dbeta = dbeta;
     a.acc_b = acc_b;
-    return R <= kFewRows ? launch_bwd_few<DT>(ctx, a) : launch_bwd<DT>(ctx, s, a);
+    return few_rows(DT, R, C) ? launch_bwd_few<DT>(ctx, a) : launch_bwd<DT>(ctx, s, a);
 }
 
 // Rows that registers do not hold two of take a workgroup each, of 1024 threads at most.
@@ -1184,7 +1197,7 @@ uint64_t layer_norm_bwd_ws_bytes(int cus, int dtype, int R, int C) {
     return (uint64_t)std::max(s.splits, 1) * 2 * (uint64_t)padded(C) * sizeof(float);
 }
 int layer_norm_bwd_dispatches(int cus, int dtype, int R, int C, bool dx, bool weights) {
-    if (R <= kFewRows) return 1;  // (a plan's dx is a buffer of its own)
+    if (few_rows(dtype, R, C)) return 1;  // (a plan's dx is a buffer of its own)
     const Split s = split_of(cus > 0 ? cus : 256, dtype, R, C);
     const bool one = s.held || (s.wide && weights);
     return (one ? (dx || weights) : (int)dx + (int)weights) + (int)weights;
@@ -1244,7 +1257,7 @@ FG_API int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, c
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     FG_HIP(hipSetDevice(ctx->device));
     const Split s = split_of(ctx->cu_count, dtype, R, C);
-    const bool few = R > 0 && R <= kFewRows;
+    const bool few = R > 0 && few_rows(dtype, R, C);
     float *partial = nullptr;
     if ((d_dgamma || d_dbeta) && !few) {
         partial =

@@ -200,7 +200,8 @@ def ln_bwd_reference(x, dy, gamma, mean, rstd):
 LN_BWD_SHAPES = LN_SHAPES + [(300, 1, 0, 0), (1031, 72, 0, 0), (2048, 520, 0, 0),
                              (4099, 131, 5, 0), (515, 4096, 0, 0), (600, 9000, 0, 0),
                              (129, 1000, 0, 0), (256, 4100, 4, 1), (257, 6001, 1, 0),
-                             (300, 16384, 0, 0), (1100, 17001, 0, 0)]
+                             (300, 16384, 0, 0), (1100, 17001, 0, 0), (600, 2048, 0, 0),
+                             (640, 777, 3, 1), (641, 300, 0, 0), (257, 24, 0, 0)]
 
 
 @pytest.mark.parametrize("dt", DTS)
