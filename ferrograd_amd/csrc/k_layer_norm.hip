@@ -180,9 +180,13 @@ __global__ __launch_bounds__(L *NG) void ln_fwd(const Fwd<typename Io<DT>::T> a)
 // A row per workgroup and nothing else held (gamma and beta come from the caches
 // where the output needs them), so that two or more rows share a CU and their loads
 // overlap one another's sums: bf16 4096 x 12000 40.1 us in workgroups of 512, 46.0 in
-// ones of 1024; 2048 x 16384 23.2 us, 5.8 TB/s.
+// ones of 1024; 2048 x 16384 24.3 us, 5.5 TB/s.  The longest rows a CU holds two of take 16
+// chunks a lane (fp32 1024 x 32768 51.5 us, 66.7 with 8 chunks in registers for two
+// workgroups of 1024, which do not suffice), one a CU where there are no more rows than
+// CUs (bf16 64 x 65536 10.9 us, 15.3).
 template <int DT, int NV, int L>
-__global__ __launch_bounds__(L) __attribute__((amdgpu_waves_per_eu(8))) void ln_fwd_wide(const Fwd<typename Io<DT>::T> a) {
+__global__ __launch_bounds__(L) __attribute__((amdgpu_waves_per_eu(NV > 4 ? 4 : 8))) void ln_fwd_wide(
+    const Fwd<typename Io<DT>::T> a) {
     const auto *x = a.x;
     const auto *__restrict__ gamma = a.gamma, *__restrict__ beta = a.beta;
     auto *y = a.y;
@@ -1059,7 +1063,9 @@ void launch_fwd(fg_ctx *ctx, const void *x, int ldx, const void *gamma, const vo
     FG_LN_WIDE(4, 256)
     FG_LN_WIDE(4, 512)
     FG_LN_WIDE(4, 1024)
-    FG_LN_WIDE(8, 1024)
+    if (R <= ctx->cu_count) FG_LN_WIDE(8, 1024)
+    FG_LN_WIDE(16, 512)
+    FG_LN_WIDE(16, 1024)
 #undef FG_LN_WIDE
     ln_fwd_long<DT><<<R, kLongL, 0, ctx->stream>>>(a);
 }

@@ -5,7 +5,8 @@ Tolerances are error bounds, elementwise.  u = 2^-24 is fp32's rounding, h the
 storage type's (2^-24, 2^-11, 2^-8).  A sum of n fp32 terms taken as chains of
 at most m terms joined by a tree of at most 10 levels is off by at most
 (m + 10) u times the sum of magnitudes; a row of up to 2^17 columns is summed
-in chains of at most 128 (1024 threads), so rows count N_ROW u.  Sums over rows
+in chains of at most 128 (1024 threads; longer rows by chunks of at most 8, whose
+sums' chains are shorter), so rows count N_ROW u.  Sums over rows
 or tokens use the bound of any order, their count.
 """
 import math
@@ -84,7 +85,8 @@ LN_SHAPES = [  # R, C, pad, start
     (1, 1, 0, 0), (3, 2, 0, 1), (1, 7, 0, 0), (5, 33, 2, 0), (4, 64, 0, 0), (17, 255, 1, 3),
     (64, 256, 0, 0), (9, 777, 0, 0), (33, 1000, 8, 0), (130, 1531, 3, 1), (2, 2048, 0, 0),
     (257, 2048, 0, 0), (7, 4096, 0, 8), (12, 4100, 4, 0), (5, 8192, 0, 0), (3, 8200, 0, 2),
-    (3, 16384, 0, 0), (2, 20001, 0, 0), (2, 32768, 0, 0), (2, 65537, 0, 1), (1, 131072, 0, 0)]
+    (3, 16384, 0, 0), (2, 20001, 0, 0), (2, 32768, 0, 0), (2, 65537, 0, 1), (1, 131072, 0, 0),
+    (300, 40000, 0, 0), (1, 140000, 0, 1)]
 
 
 def ln_reference(x, gamma, beta, eps):
