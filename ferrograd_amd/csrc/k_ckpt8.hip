@@ -322,6 +322,7 @@ FG_API int fg_ckpt8_load(fg_ctx *ctx, int dtype, int act, const int8_t *d_q, int
     FG_REQUIRE(act >= FG_ACT_NONE && act <= FG_ACT_GELU, FG_ERR_INVALID_ARGUMENT,
                "%s: bad act %d", who, act);
     FG_REQUIRE(d_z || d_h, FG_ERR_INVALID_ARGUMENT, "%s: z or h is required", who);
+    FG_REQUIRE(d_z != d_h, FG_ERR_INVALID_ARGUMENT, "%s: z is h", who);
     FG_REQUIRE((!d_z || ldz >= C) && (!d_h || ldh >= C), FG_ERR_SHAPE,
                "%s: ldz=%d or ldh=%d < C=%d", who, ldz, ldh, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);

@@ -1077,6 +1077,7 @@ FG_API int fg_embedding(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T,
                C);
     FG_REQUIRE(T == 0 || (d_tokens && d_table && d_out), FG_ERR_INVALID_ARGUMENT,
                "%s: tokens, table and out are required", who);
+    FG_REQUIRE(!d_out || d_out != d_table, FG_ERR_INVALID_ARGUMENT, "%s: out is the table", who);
     FG_REQUIRE(fg::rows::grid_holds(fwd_blocks(dtype, T, C), kNT), FG_ERR_OUT_OF_BOUNDS,
                "%s: %d rows of %d columns", who, T, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
@@ -1104,6 +1105,7 @@ FG_API int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, in
                lddt, C);
     FG_REQUIRE(d_dtable && (T == 0 || (d_tokens && d_dout)), FG_ERR_INVALID_ARGUMENT,
                "%s: tokens, dout and dtable are required", who);
+    FG_REQUIRE(d_dtable != d_dout, FG_ERR_INVALID_ARGUMENT, "%s: dtable is dout", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     FG_HIP(hipSetDevice(ctx->device));
     const Plan pl = plan_of(dtype, T, V, C);

@@ -1257,6 +1257,8 @@ FG_API int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, c
                "%s: x, dy, mean and rstd are required", who);
     FG_REQUIRE((d_dx != d_x || lddx == ldx) && (d_dx != d_dy || lddx == lddy),
                FG_ERR_INVALID_ARGUMENT, "%s: dx is x or dy, but of another leading dimension", who);
+    FG_REQUIRE(!d_dgamma || d_dgamma != d_dbeta, FG_ERR_INVALID_ARGUMENT,
+               "%s: dgamma is dbeta", who);
     FG_REQUIRE(!accumulate || (d_dx != d_x && d_dx != d_dy), FG_ERR_INVALID_ARGUMENT,
                "%s: dx is x or dy and adds to itself", who);
     FG_REQUIRE(rows_fit(dtype, R, C), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns", who, R, C);

@@ -364,7 +364,8 @@ int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T, in
  * b = 255 and restores as NaN. */
 int fg_ckpt8_save(fg_ctx *ctx, int dtype, const void *d_x, int ldx, int R, int C, int8_t *d_q,
                   int ldq, uint8_t *d_e, int lde);
-/* z = the restored values, h = act(z) rounded once; either may be NULL. */
+/* z = the restored values, h = act(z) rounded once (not in one place); either may
+ * be NULL. */
 int fg_ckpt8_load(fg_ctx *ctx, int dtype, int act, const int8_t *d_q, int ldq,
                   const uint8_t *d_e, int lde, int R, int C, void *d_z, int ldz, void *d_h,
                   int ldh);

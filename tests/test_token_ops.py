@@ -16,20 +16,20 @@ CALLS = {
     "fg_layer_norm": dict(ctx=None, dtype=2, x=P, ldx=64, gamma=P, beta=P, eps=1e-5, R=4, C=64,
                           y=P, ldy=64, mean=P, rstd=P),
     "fg_layer_norm_bwd": dict(ctx=None, dtype=2, x=P, ldx=64, dy=P, lddy=64, gamma=P, mean=P,
-                              rstd=P, R=4, C=64, dx=P, lddx=64, acc=0, dgamma=P, acc_g=0, dbeta=P,
-                              acc_b=0),
+                              rstd=P, R=4, C=64, dx=P, lddx=64, acc=0, dgamma=P, acc_g=0,
+                              dbeta=2 * P, acc_b=0),
     "fg_embedding": dict(ctx=None, dtype=1, tokens=P, T=8, V=10, C=64, table=P, ldt=64, scale=1.0,
-                         out=P, ldo=64),
+                         out=2 * P, ldo=64),
     "fg_embedding_bwd": dict(ctx=None, dtype=1, tokens=P, T=8, V=10, C=64, dout=P, lddo=64,
-                             scale=1.0, dtable=P, lddt=64, acc=0),
+                             scale=1.0, dtable=2 * P, lddt=64, acc=0),
     "fg_ckpt8_save": dict(ctx=None, dtype=0, x=P, ldx=65, R=4, C=65, q=P, ldq=65, e=P, lde=3),
     "fg_ckpt8_load": dict(ctx=None, dtype=0, act=2, q=P, ldq=65, e=P, lde=3, R=4, C=65, z=P,
-                          ldz=65, h=P, ldh=65),
+                          ldz=65, h=2 * P, ldh=65),
     "fg_act_bwd_ckpt8": dict(ctx=None, dtype=0, act=2, dH=P, lddh=65, q=P, ldq=65, e=P, lde=3, R=4,
                              C=65, dZ=P, lddz=65),
     "fg_matmul_bwd_ckpt8": dict(ctx=None, dtype=2, M=4, N=8, K=65, act=2, q=P, ldq=65, e=P, lde=3,
-                                W=P, ldw=8, dZ=P, lddz=8, Zr=4 * P, Xr=2 * P, dX=3 * P, lddx=65, dW=P,
-                                lddw=8, dbias=P, acc=0),
+                                W=P, ldw=8, dZ=P, lddz=8, Zr=4 * P, Xr=2 * P, dX=3 * P, lddx=65,
+                                dW=P, lddw=8, dbias=P, acc=0),
 }
 
 MANY = (1 << 31) - 1  # rows
@@ -46,6 +46,8 @@ REFUSED = [
     ("fg_layer_norm_bwd", dict(acc=1), INVALID),
     ("fg_layer_norm_bwd", dict(acc=1, dy=2 * P), INVALID),
     ("fg_act_bwd_ckpt8", dict(lddh=66), INVALID),
+    ("fg_layer_norm_bwd", dict(dbeta=P), INVALID), ("fg_embedding", dict(out=P), INVALID),
+    ("fg_embedding_bwd", dict(dtable=P), INVALID), ("fg_ckpt8_load", dict(h=P), INVALID),
     ("fg_matmul_bwd_ckpt8", dict(Zr=3 * P), INVALID),
     ("fg_matmul_bwd_ckpt8", dict(Xr=P), INVALID), ("fg_matmul_bwd_ckpt8", dict(Zr=P), INVALID),
     ("fg_layer_norm", dict(C=BIG, ldx=BIG, ldy=BIG), BOUNDS),
