@@ -82,7 +82,9 @@ struct Args {
     int M, N, K;
     int lda, ldb, ldc, ldz, ldzs;
     int act;
-    int mode;  // 0 forward epilogue, 1 backward (act-derivative) epilogue
+    // 0 forward epilogue, 1 backward (act-derivative) epilogue, 2 the backward one with
+    // a single rounding, of the stored value
+    int mode;
     int accumulate;
     int tiles_m, tiles_n;
     // TN on the pipelined path only: colsum[n] (=|+=) sum_k B[k][n] --
@@ -236,12 +238,13 @@ __device__ __forceinline__ void tile_of(int bid, int tiles_m, int tiles_n, int &
 
 // Epilogue of one element: v is the fp32 sum; node values are rounded to
 // the storage type as the reference's matmul, bias-add and activation nodes
-// each are.
+// each are, but in mode 2, whose products and sums stay fp32 until the store
+// (opaque: in every epilogue the same ones).
 template <bool BF>
 __device__ __forceinline__ float epi16(const Args &p, float v, const uint16_t *bias, int row,
                                        int col, float *zout) {
     using E = T16<BF>;
-    v = E::to_f(E::from_f(v));
+    if (p.mode != 2) v = E::to_f(E::from_f(v));
     if (p.mode == 0) {
         if (bias) v = E::to_f(E::from_f(v + E::to_f(bias[col])));
         *zout = v;
@@ -250,8 +253,9 @@ __device__ __forceinline__ float epi16(const Args &p, float v, const uint16_t *b
     if (p.act != kActNone) {
         const float z = E::to_f(p.Zs[(size_t)row * p.ldzs + col]);
         // ReLU' masks (a select: +0 where z <= 0); GELU' scales.
-        v = p.act == kActRelu ? (z > 0.0f ? v : 0.0f)
-                              : E::to_f(E::from_f(v * act_grad(p.act, z)));
+        if (p.act == kActRelu) return z > 0.0f ? v : 0.0f;
+        v = opaque(v * act_grad(p.act, z));
+        if (p.mode != 2) v = E::to_f(E::from_f(v));
     }
     return v;
 }
@@ -276,7 +280,7 @@ __device__ __forceinline__ void epi16_x4(const Args &p, f32x4 v, f32x4 bv, int r
         *reinterpret_cast<u32x2_u *>(q) = u32x2{pack2(E::from_f(x[0]), E::from_f(x[1])),
                                               pack2(E::from_f(x[2]), E::from_f(x[3]))};
     };
-    v = rnd(v);
+    if (p.mode != 2) v = rnd(v);
     if (p.mode == 0) {
         if (p.bias) v = rnd(v + bv);
         if (p.Z) st4(p.Z + (size_t)row * p.ldz + col, v);
@@ -293,8 +297,8 @@ __device__ __forceinline__ void epi16_x4(const Args &p, f32x4 v, f32x4 bv, int r
             for (int t = 0; t < 4; ++t) v[t] = z[t] > 0.0f ? v[t] : 0.0f;
         } else {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) v[t] = v[t] * act_grad(p.act, z[t]);
-            v = rnd(v);
+            for (int t = 0; t < 4; ++t) v[t] = opaque(v[t] * act_grad(p.act, z[t]));
+            if (p.mode != 2) v = rnd(v);
         }
     }
     uint16_t *c = p.C + (size_t)row * p.ldc + col;
@@ -398,8 +402,8 @@ __device__ __forceinline__ void store_tile16(const Args &p, const f32x16 (&acc)[
 // 4096^3 NN 116.0 -> 112.9 us, 4096x4096x1024 with bias + GELU + Z 53.4 ->
 // 46.7 us.
 
-// epi16_x4 with the mode (0 forward, 1 act-derivative), the bias and the
-// activation fixed, without the stores: returns the four C values and (MODE
+// epi16_x4 with the mode (0 forward, 1 act-derivative, rounded per node or, by
+// p.mode, once), the bias and the activation fixed, without the stores: returns the four C values and (MODE
 // 0 with Z) the four Z values, packed; z: the four saved pre-activations
 // (MODE 1 with an activation); c_old: C's current four values when
 // accumulating.
@@ -415,7 +419,8 @@ __device__ __forceinline__ u32x2 epi16_x4_k(const Args &p, f32x4 v, f32x4 bv, f3
     auto pk = [](f32x4 x) {
         return u32x2{pack2(E::from_f(x[0]), E::from_f(x[1])), pack2(E::from_f(x[2]), E::from_f(x[3]))};
     };
-    v = rnd(v);
+    const bool once = MODE == 1 && p.mode == 2;
+    if (!once) v = rnd(v);
     if constexpr (MODE == 0) {
         if constexpr (BIAS) v = rnd(v + bv);
         *zpack = pk(v);
@@ -429,8 +434,8 @@ __device__ __forceinline__ u32x2 epi16_x4_k(const Args &p, f32x4 v, f32x4 bv, f3
         for (int t = 0; t < 4; ++t) v[t] = z[t] > 0.0f ? v[t] : 0.0f;
     } else if constexpr (ACT != kActNone) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] = v[t] * act_grad(ACT, z[t]);
-        v = rnd(v);
+        for (int t = 0; t < 4; ++t) v[t] = opaque(v[t] * act_grad(ACT, z[t]));
+        if (!once) v = rnd(v);
     }
     if (p.accumulate) v += c_old;
     return pk(v);

@@ -123,12 +123,14 @@ uint64_t gemm16_split_ws_bytes(int cus, int layout, int M, int N, int K, bool co
 int gemm16_dispatches(fg_ctx *ctx, int layout, int M, int N, int K, const void *A, int lda,
                       const void *B, int ldb, bool colsum);
 // A layer's dW (TN, fused column sums) and dX (NT, act') with 16-bit tensors,
-// in one launch when their kernels pair; its dispatches (no launch).
+// in one launch when their kernels pair; its dispatches (no launch).  once: dX's
+// product stays fp32 until act' has multiplied it, and sums with what was there are
+// rounded once.
 int gemm16_dw_dx(fg_ctx *ctx, int dtype, int M1, int N1, int K1, const void *A1, int lda1,
                  const void *B1, int ldb1, void *C1, int ldc1, int acc1, void *colsum,
                  int colsum_acc, int M2, int N2, int K2, const void *A2, int lda2,
                  const void *B2, int ldb2, int act, const void *Zs, int ldzs, void *C2, int ldc2,
-                 int acc2);
+                 int acc2, bool once = false);
 int gemm16_dw_dx_dispatches(fg_ctx *ctx, int M1, int N1, int K1, const void *A1, int lda1,
                             const void *B1, int ldb1, int M2, int N2, int K2, const void *A2,
                             int lda2, const void *B2, int ldb2);

@@ -388,10 +388,11 @@ FG_API int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int 
                "%s: Xr and Zr must not be an operand, an output or each other", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     // One pass restores z and act(z), 6 % of the call at bf16 2048 x 4096 x 4096 (8.6 us of
-    // 147), then the products as from kept activations, with their roundings: act(z) to
-    // the type (what the matrix instructions take), dX's product to the type before it is
-    // multiplied by act'(z), so that a layer's gradients are the same bits whichever form
-    // its input was kept in, where that form is exact.
+    // 147), then the products as from kept activations: act(z) is rounded to the type,
+    // which is what the matrix instructions take and what the forward multiplied (in bf16
+    // that is half of dW's error, 0.0024 normwise of fp64 where its own rounding makes
+    // 0.0017; without it dW's product would take act(z) in two parts, twice the work).
+    // Nothing else is rounded before it is stored.
     // [act(z) > 0] == [z > 0] for ReLU, whose derivative then reads Xr.
     void *zr = act == FG_ACT_GELU ? d_Zr : nullptr;
     if (int rc = fg_ckpt8_load(ctx, dtype, act, d_q, ldq, d_e, lde, M, K, zr, K, d_Xr, K))
@@ -402,6 +403,8 @@ FG_API int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int 
                                  (const float *)d_dZ, lddz, act, (const float *)zs, K,
                                  (float *)d_dX, lddx, (float *)d_dW, lddw, (float *)d_dbias,
                                  accumulate);
-    return fg_matmul_bwd_x16(ctx, dtype, M, N, K, d_Xr, K, d_W, ldw, d_dZ, lddz, act, zs, K, d_dX,
-                             lddx, d_dW, lddw, d_dbias, accumulate);
+    // dW: TN K x N over M; dX: NT M x K over N.
+    return fg::gemm16_dw_dx(ctx, dtype, K, N, M, d_Xr, K, d_dZ, lddz, d_dW, lddw, accumulate,
+                            d_dbias, accumulate, M, K, N, d_dZ, lddz, d_W, ldw, act, zs, K, d_dX,
+                            lddx, accumulate, true);
 }

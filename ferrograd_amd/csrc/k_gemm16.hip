@@ -320,26 +320,26 @@ bool pairable16(fg_ctx *ctx, Args &w, Args &x) {
 namespace fg {
 // A layer's two gradient GEMMs with 16-bit tensors: one launch
 // (gemm16_pair_big) when both take the large tiles' pipelined kernels
-// unsplit, else fg_gemm_dw_x16 then fg_gemm_bwd_x16.  Each part runs
-// exactly as its own call.
+// unsplit, else one after the other.  Each part runs exactly as its own call
+// (fg_gemm_dw_x16, fg_gemm_bwd_x16), or with once in the epilogue that rounds once.
 int gemm16_dw_dx(fg_ctx *ctx, int dtype, int M1, int N1, int K1, const void *A1, int lda1,
                  const void *B1, int ldb1, void *C1, int ldc1, int acc1, void *colsum,
                  int colsum_acc, int M2, int N2, int K2, const void *A2, int lda2,
                  const void *B2, int ldb2, int act, const void *Zs, int ldzs, void *C2, int ldc2,
-                 int acc2) {
+                 int acc2, bool once) {
     Args w = dw_args16(M1, N1, K1, A1, lda1, B1, ldb1, C1, ldc1, acc1, colsum, colsum_acc);
     Args x = dx_args16(M2, N2, K2, A2, lda2, B2, ldb2, act, Zs, ldzs, C2, ldc2, acc2);
+    if (once) w.mode = x.mode = 2;
     const bool checked = M1 > 0 && N1 > 0 && M2 > 0 && N2 > 0 &&
                          gemm16_check(ctx, dtype, FG_TN, w, "fg_gemm_dw_x16") == FG_OK &&
                          gemm16_check(ctx, dtype, FG_NT, x, "fg_gemm_bwd_x16") == FG_OK &&
                          (act == FG_ACT_NONE || (Zs && ldzs >= N2));
     if (!checked || !pairable16(ctx, w, x)) {
         fg::clear_error();  // the calls below report any error themselves
-        const int rc = fg_gemm_dw_x16(ctx, dtype, M1, N1, K1, A1, lda1, B1, ldb1, C1, ldc1, acc1,
-                                      colsum, colsum_acc);
-        if (rc) return rc;
-        return fg_gemm_bwd_x16(ctx, dtype, FG_NT, M2, N2, K2, A2, lda2, B2, ldb2, act, Zs, ldzs,
-                               C2, ldc2, acc2);
+        if (int rc = gemm16_common(ctx, dtype, FG_TN, w, "fg_gemm_dw_x16")) return rc;
+        FG_REQUIRE(act == FG_ACT_NONE || (Zs && ldzs >= N2), FG_ERR_INVALID_ARGUMENT,
+                   "fg_gemm_bwd_x16: act %d needs Zs with ldzs >= N", act);
+        return gemm16_common(ctx, dtype, FG_NT, x, "fg_gemm_bwd_x16");
     }
     FG_HIP(hipSetDevice(ctx->device));
     if (dtype == FG_DTYPE_BF16)

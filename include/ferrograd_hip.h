@@ -381,8 +381,9 @@ int fg_act_bwd_ckpt8(fg_ctx *ctx, int dtype, int act, const void *d_dH, int lddh
  * d_Xr and (for GELU; else it may be NULL) d_Zr are the caller's scratch, M x K
  * elements of dtype each, overwritten with act(z) and z as the products read
  * them (no operand or output may be there): act(z) is rounded to dtype, as the
- * forward's stored activation is, and so is dX's product before act'(z)
- * multiplies it, as in fg_matmul_bwd_x16. */
+ * forward's stored activation is.  The outputs are rounded once, sums with what
+ * was there too (fg_matmul_bwd_x16 rounds dX's product before act'(z) multiplies
+ * it, and products before they are added). */
 int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int act,
                         const int8_t *d_q, int ldq, const uint8_t *d_e, int lde,
                         const void *d_W, int ldw, const void *d_dZ, int lddz, void *d_Zr,
