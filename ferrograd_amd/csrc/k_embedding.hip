@@ -196,8 +196,9 @@ __global__ __launch_bounds__(kNT) void emb_bwd_few(const Few<typename Io<DT>::T>
 #pragma unroll
                     for (int e = 0; e < E; ++e) a[e] += IO::get(w[u], e);
             }
+            // (A row of no token is +0 whatever the scale.)
 #pragma unroll
-            for (int e = 0; e < E; ++e) a[e] *= scale;
+            for (int e = 0; e < E; ++e) a[e] = last < 0 ? 0.0f : a[e] * scale;
             if (accumulate) at_j.add(to, j, a);
             else at_j.store(to, a);
         }

@@ -1,6 +1,8 @@
-"""Layer norm, embedding and 8-bit checkpoints on paths of their own: in place in every
+"""Layer norm and embedding on paths of their own: in place in every
 layer norm kernel, every form of the token sort, table rows that the summing launch
-zeroes, captured gradients that use the workspace."""
+zeroes, unused rows whatever the scale, captured gradients that use the workspace."""
+import math
+
 import numpy as np
 import pytest
 
@@ -174,6 +176,25 @@ def test_embedding_backward_zeroes_past_32_bits(gpu_ctx):
         got = d[v:v + 6000]
         within(got, ref, bound, "bf16")
         assert (got[~used].view(torch.int16) == 0).all()
+
+
+@pytest.mark.parametrize("dt", DTS)
+@pytest.mark.parametrize("scale", [-0.5, math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("T", [0, 1, 32, 33, 5000])
+def test_rows_of_no_token_are_zero_whatever_the_scale(gpu_ctx, dt, scale, T):
+    V, C = 700, 53
+    note("embedding_bwd scale", dt, scale, T)
+    tok = tokens_of("uniform", max(T, 1), V, 351)
+    dout = rand((max(T, 1), C), dt, 352)
+    d, untouched = blank((V, C), dt, 2)
+    gpu_ctx.embedding_bwd(tok, T, V, C, dout, C, d, ld(d), scale=scale, dtype=DTS[dt][0])
+    torch.cuda.synchronize()
+    used = torch.zeros(V, dtype=torch.bool, device="cuda")
+    used[tok[:T].long()] = True
+    bits = d.contiguous().view({"f32": torch.int32}.get(dt, torch.int16))
+    assert (bits[~used] == 0).all() and untouched()
+    if not math.isfinite(scale):
+        assert not torch.isfinite(d[used]).any()
 
 
 # ------------------------------------------------------------------ graphs
