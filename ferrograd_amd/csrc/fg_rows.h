@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 
 #include "fg_half.h"
 #include "fg_softmax_any.h"  // Io: a chunk's elements
@@ -26,6 +27,13 @@ constexpr int kMaxCols = 1 << 23;
 // Whether a grid's x dimension holds `blocks` workgroups: fewer than 2^32 threads.
 inline bool grid_holds(int64_t blocks, int threads) {
     return blocks * threads < int64_t(1) << 32;
+}
+
+// Whether an output that a call may go without (NULL) is none of its other buffers.
+inline bool apart(const void *out, std::initializer_list<const void *> others) {
+    for (const void *o : others)
+        if (out && out == o) return false;
+    return true;
 }
 
 using smany::Io;

@@ -32,6 +32,7 @@
 
 namespace {
 
+using fg::rows::apart;
 using fg::rows::Chunk;
 using fg::rows::Io;
 using fg::rows::u32x2;
@@ -301,6 +302,8 @@ FG_API int fg_ckpt8_save(fg_ctx *ctx, int dtype, const void *d_x, int ldx, int R
     FG_REQUIRE(ldx >= C, FG_ERR_SHAPE, "%s: ldx=%d < C=%d", who, ldx, C);
     FG_REQUIRE(d_x, FG_ERR_INVALID_ARGUMENT, "%s: x is required", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_q, {d_x, d_e}) && apart(d_e, {d_x}), FG_ERR_INVALID_ARGUMENT,
+               "%s: x, q and e must be apart", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
     const Shape s = shape_of(dtype, R, C);
@@ -326,6 +329,8 @@ FG_API int fg_ckpt8_load(fg_ctx *ctx, int dtype, int act, const int8_t *d_q, int
     FG_REQUIRE((!d_z || ldz >= C) && (!d_h || ldh >= C), FG_ERR_SHAPE,
                "%s: ldz=%d or ldh=%d < C=%d", who, ldz, ldh, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_z, {d_q, d_e}) && apart(d_h, {d_q, d_e}), FG_ERR_INVALID_ARGUMENT,
+               "%s: z or h is q or e", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
     const Shape s = shape_of(dtype, R, C);
@@ -352,6 +357,7 @@ FG_API int fg_act_bwd_ckpt8(fg_ctx *ctx, int dtype, int act, const void *d_dH, i
     FG_REQUIRE(d_dZ != d_dH || lddz == lddh, FG_ERR_INVALID_ARGUMENT,
                "%s: dZ is dH, but lddz=%d, lddh=%d", who, lddz, lddh);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_dZ, {d_q, d_e}), FG_ERR_INVALID_ARGUMENT, "%s: dZ is q or e", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
     const Shape s = shape_of(dtype, R, C);
@@ -381,10 +387,10 @@ FG_API int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int 
                who);
     FG_REQUIRE(d_Xr && (act != FG_ACT_GELU || d_Zr), FG_ERR_INVALID_ARGUMENT,
                "%s: Xr, and for GELU Zr, is required", who);
-    auto apart = [&](const void *r) {
-        return !r || (r != d_W && r != d_dZ && r != d_dX && r != d_dW && r != d_dbias);
+    auto free = [&](const void *r) {
+        return apart(r, {d_q, d_e, d_W, d_dZ, d_dX, d_dW, d_dbias});
     };
-    FG_REQUIRE(d_Xr != d_Zr && apart(d_Xr) && apart(d_Zr), FG_ERR_INVALID_ARGUMENT,
+    FG_REQUIRE(d_Xr != d_Zr && free(d_Xr) && free(d_Zr), FG_ERR_INVALID_ARGUMENT,
                "%s: Xr and Zr must not be an operand, an output or each other", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     // One pass restores z and act(z), 6 % of the call at bf16 2048 x 4096 x 4096 (8.6 us of

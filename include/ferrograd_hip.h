@@ -361,7 +361,8 @@ int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T, in
  * is exact in every dtype; it is off by at most 2^(b - 134), half of
  * 1/64 of the power of two below the block's largest |x|, except that values
  * above 127.5 steps restore as 127.  A block with an infinity or NaN gets
- * b = 255 and restores as NaN. */
+ * b = 255 and restores as NaN.  No output of these calls may be one of the 8-bit
+ * form's buffers, x included. */
 int fg_ckpt8_save(fg_ctx *ctx, int dtype, const void *d_x, int ldx, int R, int C, int8_t *d_q,
                   int ldq, uint8_t *d_e, int lde);
 /* z = the restored values, h = act(z) rounded once (not in one place); either may
