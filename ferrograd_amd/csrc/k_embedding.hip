@@ -36,6 +36,7 @@
 
 namespace {
 
+using fg::rows::apart;
 using fg::rows::Io;
 using fg::rows::Tail;
 using fg::rows::u32x4;
@@ -1082,6 +1083,7 @@ FG_API int fg_embedding(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T,
     FG_REQUIRE(fg::rows::grid_holds(fwd_blocks(dtype, T, C), kNT), FG_ERR_OUT_OF_BOUNDS,
                "%s: %d rows of %d columns", who, T, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_out, {d_tokens}), FG_ERR_INVALID_ARGUMENT, "%s: out is the tokens", who);
     if (T == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
     auto launch = dtype == FG_DTYPE_F32    ? launch_fwd<fg::kF32>
@@ -1108,6 +1110,8 @@ FG_API int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, in
                "%s: tokens, dout and dtable are required", who);
     FG_REQUIRE(d_dtable != d_dout, FG_ERR_INVALID_ARGUMENT, "%s: dtable is dout", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_dtable, {d_tokens}), FG_ERR_INVALID_ARGUMENT, "%s: dtable is the tokens",
+               who);
     FG_HIP(hipSetDevice(ctx->device));
     const Plan pl = plan_of(dtype, T, V, C);
     void *ws = nullptr;

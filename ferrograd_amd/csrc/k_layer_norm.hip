@@ -28,6 +28,7 @@
 
 namespace {
 
+using fg::rows::apart;
 using fg::rows::Io;
 using fg::rows::u32x4;
 
@@ -1228,6 +1229,10 @@ FG_API int fg_layer_norm(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const
                who, ldy, ldx);
     FG_REQUIRE(rows_fit(dtype, R, C), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns", who, R, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_y, {d_gamma, d_beta, d_mean, d_rstd}) &&
+                   apart(d_mean, {d_x, d_gamma, d_beta, d_rstd}) &&
+                   apart(d_rstd, {d_x, d_gamma, d_beta}),
+               FG_ERR_INVALID_ARGUMENT, "%s: an output is another output or an input but x", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
     if (dtype == FG_DTYPE_F32)
@@ -1263,6 +1268,11 @@ FG_API int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, c
                "%s: dx is x or dy and adds to itself", who);
     FG_REQUIRE(rows_fit(dtype, R, C), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns", who, R, C);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_dx, {d_gamma, d_mean, d_rstd}) &&
+                   apart(d_dgamma, {d_x, d_dy, d_gamma, d_mean, d_rstd, d_dx}) &&
+                   apart(d_dbeta, {d_x, d_dy, d_gamma, d_mean, d_rstd, d_dx}),
+               FG_ERR_INVALID_ARGUMENT,
+               "%s: an output is another output or an input (but dx, which may be x or dy)", who);
     FG_HIP(hipSetDevice(ctx->device));
     const Split s = split_of(ctx->cu_count, dtype, R, C);
     const bool few = R > 0 && few_rows(dtype, R, C);

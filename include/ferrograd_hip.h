@@ -306,7 +306,8 @@ int fg_softmax_bwd(fg_ctx *ctx, int dtype, const void *d_y, const void *d_dy, in
 
 /* -------------------------------------------------- token-model operators */
 /* The following take rows of any alignment and of up to 2^23 columns; rows so
- * many and so long that a grid cannot hold them (2^32 threads) are out of bounds.  Calls
+ * many and so long that a grid cannot hold them (2^32 threads) are out of bounds.  An
+ * output is never an input or another output, but where a call says so.  Calls
  * that use the workspace share it with the context's other direct calls, in
  * the stream's order: graphs captured on one context must not run at the same
  * time. */
@@ -361,8 +362,7 @@ int fg_embedding_bwd(fg_ctx *ctx, int dtype, const uint32_t *d_tokens, int T, in
  * is exact in every dtype; it is off by at most 2^(b - 134), half of
  * 1/64 of the power of two below the block's largest |x|, except that values
  * above 127.5 steps restore as 127.  A block with an infinity or NaN gets
- * b = 255 and restores as NaN.  No output of these calls may be one of the 8-bit
- * form's buffers, x included. */
+ * b = 255 and restores as NaN. */
 int fg_ckpt8_save(fg_ctx *ctx, int dtype, const void *d_x, int ldx, int R, int C, int8_t *d_q,
                   int ldq, uint8_t *d_e, int lde);
 /* z = the restored values, h = act(z) rounded once (not in one place); either may
