@@ -41,7 +41,7 @@ def _ptr(x) -> Optional[int]:
     """Device address of x: None, an int address, or an object with data_ptr()."""
     if x is None or isinstance(x, int):
         return x
-    return x.data_ptr()
+    return int(x.data_ptr())
 
 
 class Context:

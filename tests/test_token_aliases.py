@@ -4,6 +4,7 @@ told apart once there is a context; this one has no device, and the calls that a
 through have no rows.)"""
 import ctypes
 
+import numpy as np
 import pytest
 
 import ferrograd_amd as fa
@@ -59,6 +60,18 @@ def test_refuses_an_output_that_is_another_buffer(fn, a, b):
     e = call(fn, **{a: b})
     assert e is not None and e.code == INVALID
     assert f"{fn}: " in str(e) and "ctx is NULL" not in str(e)
+
+
+def test_addresses_that_are_no_python_ints():
+    """An object whose data_ptr() gives another integer type is taken as it was."""
+    class Buffer:
+        def data_ptr(self):
+            return np.uint64(1 << 40)
+
+    with pytest.raises(fa.FgError) as e:
+        _lib.call("fg_softmax_f32", None, fa._ptr(Buffer()), 4, 4, fa._ptr(Buffer()))
+    assert e.value.code == INVALID
+    assert fa._ptr(Buffer()) == 1 << 40 and fa._ptr(None) is None and fa._ptr(7) == 7
 
 
 @pytest.mark.parametrize("fn", [f for f, c in CASES.items() if c[2].get("R", c[2].get("T")) == 0])
