@@ -394,7 +394,7 @@ FG_API int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int 
                "%s: Xr and Zr must not be an operand, an output or each other", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     // One pass restores z and act(z), 6 % of the call at bf16 2048 x 4096 x 4096 (8.6 us of
-    // 147), then the products as from kept activations: act(z) is rounded to the type,
+    // 148; fp32 26 us of 981), then the products as from kept activations: act(z) is rounded to the type,
     // which is what the matrix instructions take and what the forward multiplied (in bf16
     // that is half of dW's error, 0.0024 normwise of fp64 where its own rounding makes
     // 0.0017; without it dW's product would take act(z) in two parts, twice the work).

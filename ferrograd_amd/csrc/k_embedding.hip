@@ -12,7 +12,7 @@
 // Both are bound by HBM (the rows they read and write once): the lookup of 16384 rows
 // of 4096 in bf16 takes 32.5 us, 5.6 TB/s.  The gradient:
 //  * the positions in (token, position) order: one launch of workgroups that own
-//    tokens (up to kOrderReads reads), a stable radix sort above; table rows are zeroed
+//    tokens (up to kOrderReads reads in all), a stable radix sort above; table rows are zeroed
 //    beside either, which leave the memory idle;
 //  * the sorted positions in units of equal length, so that a token that fills half
 //    the batch is spread over the GPU as evenly as any other: a unit adds its runs
@@ -48,7 +48,12 @@ typedef u32x2 u32x2_any __attribute__((aligned(2)));
 constexpr int kNT = 256;
 constexpr int kDirectMax = 32;
 constexpr int kOwnMax = 4096;
-// Tokens that all of emb_order's workgroups read: 40960 a workgroup where there are 256.
+// Tokens that all of emb_order's workgroups read: 40960 a workgroup where there are 256,
+// fewer where there are more (tables above 2^18 rows), more where a small table has fewer
+// workgroups (3 for 2 rows, 51 for 50, 129 for 256), which may then take longer than the
+// radix sort would (all of the gradient, bf16 rows of 256: 131072 tokens over 2 rows 92 us
+// and 44, over 50 rows 81 and 38, over 256 rows 39 and 38; 40960 over 2 rows 41 and 34;
+// 16384 over 2 rows 29 and 32).
 // It takes 8.6 us for 8192 tokens, 15 for 16384, 22 for 32768 (as much again where zeros
 // share the CUs); the radix sort's launches 24 or more for any of these.  All of the
 // gradient, bf16, 32000 rows of 1024: 8192 tokens 25.7 us (radix sort 36.7), 16384 34.2
@@ -969,7 +974,8 @@ int launch_bwd(fg_ctx *ctx, const Plan &pl, void *ws, const uint32_t *tokens, in
     // Zeroed beside the sort, which leaves the memory idle: what its launches have time
     // for; the whole table where that is most of it, or where few of its rows are
     // written again.  The rest goes beside the sums, without the rows of tokens.
-    // (emb_order, MB for 20011 and 32768 tokens: 34 and 50 68.3 and 86.3 us in all, 59
+    // (Measured with 256 workgroups ordering and a frequent token in both batches;
+    // emb_order, MB for 20011 and 32768 tokens: 34 and 50 68.3 and 86.3 us in all, 59
     // and 90 60.0 and 79.7, 95 and 150 61.0 and 72.0, 142 and 220 70.0 and 77.0.)
     constexpr double kMB = 1 << 20;
     const double row_mb = (double)C * sizeof(Ty) / kMB, q = T / 8192.0;

@@ -327,8 +327,9 @@ int fg_layer_norm(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const void *
  *   dx (=|+=) rstd * (g - mean(g) - xh * mean(g * xh))
  *   dgamma (=|+=) sum over rows of dy * xh ;  dbeta (=|+=) sum over rows of dy
  * Any output may be NULL; gamma may be NULL (1).  dx may be x or dy (equal
- * leading dimensions) unless it accumulates.  Above 256 rows, their partial sums
- * of dgamma and dbeta go to the workspace, 8 bytes a column for each of at most
+ * leading dimensions) unless it accumulates.  Above 256 rows (640 where a row is
+ * at most 1024 fp32 or 2048 16-bit columns), the partial sums of dgamma and
+ * dbeta go to the workspace, 8 bytes a column for each of at most
  * 1024 row splits, and are added in a fixed order.  R = 0 writes zeros to
  * dgamma and dbeta (or adds nothing). */
 int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const void *d_dy,
@@ -591,7 +592,10 @@ int fg_graph_embedding(fg_graph *g, uint32_t table, uint32_t tokens, float scale
  * fg_ckpt8_save): the node's matmul writes its pre-activation and activation
  * into memory that all such layers of a plan share, and the backward of the
  * matmul that reads the activation restores both there.  The forward's values
- * are unchanged; the gradients come from the restored ones.  The node must be the
+ * are unchanged; the gradients come from the restored ones: what is below half a
+ * step of its block restores as 0, so a kept relu passes no gradient where the
+ * forward passed such a value.  The gradients' own memory is that of a layer
+ * that is not kept.  The node must be the
  * activation of a matmul (with or without bias) and the first operand of one
  * other matmul, its only user (checked by fg_plan_create).  Its values are not
  * among FG_ROLE_FORWARD_SAVED. */
