@@ -403,10 +403,10 @@ __device__ __forceinline__ void store_tile16(const Args &p, const f32x16 (&acc)[
 // 46.7 us.
 
 // epi16_x4 with the mode (0 forward, 1 act-derivative, rounded per node or, by
-// p.mode, once), the bias and the activation fixed, without the stores: returns the four C values and (MODE
-// 0 with Z) the four Z values, packed; z: the four saved pre-activations
-// (MODE 1 with an activation); c_old: C's current four values when
-// accumulating.
+// p.mode, once), the bias and the activation fixed, without the stores:
+// returns the four C values and (MODE 0 with Z) the four Z values, packed;
+// z: the four saved pre-activations (MODE 1 with an activation); c_old: C's
+// current four values when accumulating.
 template <bool BF, int MODE, bool BIAS, int ACT>
 __device__ __forceinline__ u32x2 epi16_x4_k(const Args &p, f32x4 v, f32x4 bv, f32x4 z,
                                             f32x4 c_old, u32x2 *zpack) {

@@ -394,11 +394,12 @@ FG_API int fg_matmul_bwd_ckpt8(fg_ctx *ctx, int dtype, int M, int N, int K, int 
                "%s: Xr and Zr must not be an operand, an output or each other", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     // One pass restores z and act(z), 6 % of the call at bf16 2048 x 4096 x 4096 (8.6 us of
-    // 148; fp32 26 us of 981), then the products as from kept activations: act(z) is rounded to the type,
-    // which is what the matrix instructions take and what the forward multiplied (in bf16
-    // that is half of dW's error, 0.0024 normwise of fp64 where its own rounding makes
-    // 0.0017; without it dW's product would take act(z) in two parts, twice the work).
-    // Nothing else is rounded before it is stored.
+    // 148; fp32 26 us of 981), then the products as from kept activations: act(z) is
+    // rounded to the type, which is what the matrix instructions take and what the forward
+    // multiplied (in bf16 that is half of dW's error, 0.0024 normwise of fp64 where its
+    // own rounding makes 0.0017; without it dW's product would take act(z) in two parts,
+    // twice the work).  Nothing else is rounded before it is stored: dX 0.0017, with its
+    // product rounded before act'(z) multiplies it 0.0023.
     // [act(z) > 0] == [z > 0] for ReLU, whose derivative then reads Xr.
     void *zr = act == FG_ACT_GELU ? d_Zr : nullptr;
     if (int rc = fg_ckpt8_load(ctx, dtype, act, d_q, ldq, d_e, lde, M, K, zr, K, d_Xr, K))
