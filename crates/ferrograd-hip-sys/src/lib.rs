@@ -600,6 +600,77 @@ extern "C" {
         d_dbias: *mut c_void,
         accumulate: c_int,
     ) -> c_int;
+    pub fn fg_rms_norm(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_x: *const c_void,
+        ldx: c_int,
+        d_r: *const c_void,
+        ldr: c_int,
+        d_gamma: *const c_void,
+        eps: f32,
+        R: c_int,
+        C: c_int,
+        d_s: *mut c_void,
+        lds: c_int,
+        d_y: *mut c_void,
+        ldy: c_int,
+        d_q: *mut i8,
+        ldq: c_int,
+        d_e: *mut u8,
+        lde: c_int,
+        d_rstd: *mut f32,
+    ) -> c_int;
+    pub fn fg_rms_norm_bwd(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_s: *const c_void,
+        lds: c_int,
+        d_dy: *const c_void,
+        lddy: c_int,
+        d_gamma: *const c_void,
+        d_rstd: *const f32,
+        R: c_int,
+        C: c_int,
+        d_ds: *const c_void,
+        ldds: c_int,
+        d_dx: *mut c_void,
+        lddx: c_int,
+        d_dgamma: *mut c_void,
+        dgamma_accumulate: c_int,
+    ) -> c_int;
+    pub fn fg_token_logprobs(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_logits: *const c_void,
+        ldx: c_int,
+        d_tokens: *const u32,
+        R: c_int,
+        C: c_int,
+        scale: f32,
+        d_logp: *mut f32,
+        d_entropy: *mut f32,
+        d_lse: *mut f32,
+        top: c_int,
+        d_top_ids: *mut u32,
+        d_top_logp: *mut f32,
+    ) -> c_int;
+    pub fn fg_token_logprobs_bwd(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_logits: *const c_void,
+        ldx: c_int,
+        d_tokens: *const u32,
+        R: c_int,
+        C: c_int,
+        scale: f32,
+        d_lse: *const f32,
+        d_entropy: *const f32,
+        d_dlogp: *const f32,
+        d_dentropy: *const f32,
+        d_dlogits: *mut c_void,
+        ldd: c_int,
+    ) -> c_int;
     pub fn fg_mt_create(
         ctx: *mut fg_ctx,
         n: c_int,

@@ -205,6 +205,41 @@ class Context:
              _ptr(mean), _ptr(rstd), R, C, _ptr(dx), lddx or C, int(accumulate), _ptr(dgamma),
              int(dgamma_accumulate), _ptr(dbeta), int(dbeta_accumulate))
 
+    def rms_norm(self, x, ldx: int, R: int, C: int, y=None, ldy: int = 0, r=None, ldr: int = 0,
+                 s=None, lds: int = 0, gamma=None, eps: float = 1e-5, q=None, ldq: int = 0, e=None,
+                 lde: int = 0, rstd=None, dtype: int = DTYPE_F32) -> None:
+        """s = x + r (without r: x), y = s * rstd * gamma per row; y in 8 bits
+        too when q and e are given, rstd (fp32, one per row) kept when given."""
+        call("fg_rms_norm", self.handle, dtype, _ptr(x), ldx, _ptr(r), ldr or C, _ptr(gamma), eps,
+             R, C, _ptr(s), lds or C, _ptr(y), ldy or C, _ptr(q), ldq or C, _ptr(e),
+             lde or (C + 31) // 32, _ptr(rstd))
+
+    def rms_norm_bwd(self, s, lds: int, dy, lddy: int, rstd, R: int, C: int, gamma=None, ds=None,
+                     ldds: int = 0, dx=None, lddx: int = 0, dgamma=None,
+                     dgamma_accumulate: bool = False, dtype: int = DTYPE_F32) -> None:
+        """dx (the norm's, plus ds) and dgamma (either may be None) from s, dy
+        and the forward's rstd."""
+        call("fg_rms_norm_bwd", self.handle, dtype, _ptr(s), lds, _ptr(dy), lddy, _ptr(gamma),
+             _ptr(rstd), R, C, _ptr(ds), ldds or C, _ptr(dx), lddx or C, _ptr(dgamma),
+             int(dgamma_accumulate))
+
+    def token_logprobs(self, logits, ldx: int, tokens, R: int, C: int, logp=None, entropy=None,
+                       lse=None, top: int = 0, top_ids=None, top_logp=None, scale: float = 1.0,
+                       dtype: int = DTYPE_F32) -> None:
+        """Per row of softmax(scale * logits): the log probability of its token,
+        the entropy, the log of the sum and the `top` most probable columns with
+        theirs."""
+        call("fg_token_logprobs", self.handle, dtype, _ptr(logits), ldx, _ptr(tokens), R, C, scale,
+             _ptr(logp), _ptr(entropy), _ptr(lse), top, _ptr(top_ids), _ptr(top_logp))
+
+    def token_logprobs_bwd(self, logits, ldx: int, tokens, R: int, C: int, lse, dlogits, ldd: int,
+                           entropy=None, dlogp=None, dentropy=None, scale: float = 1.0,
+                           dtype: int = DTYPE_F32) -> None:
+        """dlogits from the gradients of logp and entropy (either may be None)
+        and the forward's lse and entropy."""
+        call("fg_token_logprobs_bwd", self.handle, dtype, _ptr(logits), ldx, _ptr(tokens), R, C,
+             scale, _ptr(lse), _ptr(entropy), _ptr(dlogp), _ptr(dentropy), _ptr(dlogits), ldd)
+
     def embedding(self, tokens, T: int, V: int, C: int, table, ldt: int, out, ldo: int,
                   scale: float = 1.0, dtype: int = DTYPE_F32) -> None:
         """out[t] = scale * table[tokens[t]] (u32 tokens; a row of NaN for a

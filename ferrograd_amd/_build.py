@@ -40,6 +40,8 @@ SOURCES = [
     "k_layer_norm.hip",
     "k_embedding.hip",
     "k_ckpt8.hip",
+    "k_rms_norm.hip",
+    "k_logprobs.hip",
     "fg_graph.cpp",
     "fg_bpat.cpp",
     "fg_telemetry.cpp",

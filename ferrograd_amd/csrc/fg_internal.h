@@ -142,6 +142,9 @@ uint64_t embedding_bwd_ws_bytes(int dtype, int T, int V, int C);
 // Dispatches of those calls.
 int layer_norm_bwd_dispatches(int cus, int dtype, int R, int C, bool dx, bool weights);
 int embedding_bwd_dispatches(int dtype, int T, int V, int C);
+// The same two of fg_rms_norm_bwd.
+uint64_t rms_norm_bwd_ws_bytes(int cus, int dtype, int R, int C);
+int rms_norm_bwd_dispatches(int cus, int dtype, int R, int C, bool dx, bool weights);
 
 // Adam with device-resident step counter / bias-correction scalars
 // (k_optim.hip).  d_state points at adam_dev_state_bytes() zeroed bytes.

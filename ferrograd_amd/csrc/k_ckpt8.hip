@@ -26,23 +26,22 @@
 #include <type_traits>
 
 #include "fg_act.h"
+#include "fg_bits8.h"
 #include "fg_half.h"
 #include "fg_internal.h"
 #include "fg_rows.h"
 
 namespace {
 
+using fg::bits8::Bytes;
+using fg::bits8::kBlock;
 using fg::rows::apart;
 using fg::rows::Chunk;
 using fg::rows::Io;
-using fg::rows::u32x2;
 using fg::rows::u32x4;
 
 constexpr int kNT = 256;
-constexpr int kBlock = 32;  // columns per exponent byte
 constexpr int kDeep = 4;    // chunks of a lane, loaded together
-typedef u32x2 u32x2_byte __attribute__((aligned(1)));
-typedef uint32_t u32_byte __attribute__((aligned(1)));
 
 // Where a lane's chunks lie: 2^lshift lanes take kDeep chunks each of a row, and
 // blockIdx.y the row's next 2^lshift * kDeep.
@@ -56,44 +55,6 @@ struct Tile {
         row = in ? (size_t)r : 0;
         step = 1 << lshift;
         first = (blockIdx.y << lshift) * kDeep + (threadIdx.x & (step - 1));
-    }
-};
-
-// E signed bytes in one access; the bytes of the row's last, partial chunk in turn.
-template <int E>
-struct Bytes {
-    uint32_t w[E / 4];
-    __device__ __forceinline__ void load(const int8_t *row, int j, int nb, int C) {
-        const int8_t *p = row + (size_t)j * E;
-        if (j < nb) {
-            if constexpr (E == 8) {
-                const u32x2 v = *reinterpret_cast<const u32x2_byte *>(p);
-                w[0] = v[0];
-                w[1] = v[1];
-            } else {
-                w[0] = *reinterpret_cast<const u32_byte *>(p);
-            }
-            return;
-        }
-#pragma unroll
-        for (int k = 0; k < E / 4; ++k) w[k] = 0;
-#pragma unroll
-        for (int k = 0; k < E; ++k)
-            if (j * E + k < C) w[k / 4] |= (uint32_t)(uint8_t)p[k] << (8 * (k & 3));
-    }
-    __device__ __forceinline__ void store(int8_t *row, int j, int nb, int C) const {
-        int8_t *p = row + (size_t)j * E;
-        if (j < nb) {
-            if constexpr (E == 8) *reinterpret_cast<u32x2_byte *>(p) = u32x2{w[0], w[1]};
-            else *reinterpret_cast<u32_byte *>(p) = w[0];
-            return;
-        }
-#pragma unroll
-        for (int k = 0; k < E; ++k)
-            if (j * E + k < C) p[k] = (int8_t)(w[k / 4] >> (8 * (k & 3)));
-    }
-    __device__ __forceinline__ int get(int k) const {
-        return (int)(int8_t)(w[k / 4] >> (8 * (k & 3)));
     }
 };
 
@@ -137,28 +98,12 @@ __global__ __launch_bounds__(kNT) void ckpt8_save_k(const Save<typename Io<DT>::
     for (int u = 0; u < kDeep; ++u) {
         const int j = t.first + u * t.step;
         if (j >= chunks) break;
-        uint32_t m = 0;
+        float v[E];
 #pragma unroll
-        for (int k = 0; k < E; ++k) m = max(m, __float_as_uint(IO::get(w[u], k)) & 0x7fffffffu);
-        // The block's other lanes (all here: chunks come in whole blocks).
-        m = max(m, (uint32_t)fg::smrow::dpp_i<fg::smrow::kDppSwap1>((int)m));
-        m = max(m, (uint32_t)fg::smrow::dpp_i<fg::smrow::kDppSwap2>((int)m));
-        if constexpr (kLanes == 8)
-            m = max(m, (uint32_t)fg::smrow::dpp_i<fg::smrow::kDppHalfMirror>((int)m));
-        const int b = max(1, (int)(m >> 23));
+        for (int k = 0; k < E; ++k) v[k] = IO::get(w[u], k);
         Bytes<E> o;
-#pragma unroll
-        for (int k = 0; k < E; k += 4) {
-            uint32_t p = 0;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const float s =
-                    __builtin_rintf(__builtin_amdgcn_ldexpf(IO::get(w[u], k + n), 133 - b));
-                const int c = (int)__builtin_amdgcn_fmed3f(s, -127.0f, 127.0f);
-                p |= ((uint32_t)c & 255u) << (8 * n);
-            }
-            o.w[k / 4] = b == 255 ? 0u : p;
-        }
+        // (The block's other lanes are all here: chunks come in whole blocks.)
+        const int b = fg::bits8::quantise<E>(v, o);
         o.store(q + t.row * ldq, j, nb, C);
         if (j % kLanes == 0) e[t.row * lde + j / kLanes] = (uint8_t)b;
     }

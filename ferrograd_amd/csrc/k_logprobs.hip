@@ -1,0 +1,412 @@
+// k_logprobs.hip -- log probabilities of given tokens with the entropy and the most
+// probable tokens of each row, and their gradient, for gfx950.  The reference answers
+// with the softmax's values (crates/ferrograd-nn/src/op/softmax.rs:14-446) and its
+// cross entropy (loss/basic_loss.rs:91-133).
+//
+// For a row x of C logits, z = scale * x, m = max z, s = sum exp(z - m):
+//   lse = m + log(s),  logp = (z_token - m) - log(s)
+//   entropy = log(s) + sum exp(z - m) (m - z) / s        (no difference of near values)
+//   alternatives: the K largest x, the lower column first among equals
+// Backward, from the gradients a of logp and b of entropy, p = exp(z - lse):
+//   dx_c = scale * (a ([c = token] - p_c) - b p_c (z_c - lse + entropy))
+// which needs no sum over the row again.
+//
+// Both are bound by HBM, and in 16 bits by the vector unit beside it: the forward reads
+// a row once, with a running maximum and sums a thread that are raised together; the
+// backward reads and writes each logit once.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "fg_half.h"
+#include "fg_internal.h"
+#include "fg_rows.h"
+
+namespace {
+
+using fg::rows::apart;
+using fg::rows::Io;
+using fg::rows::u32x4;
+
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+constexpr int kMaxTop = 32;   // alternatives: at most the 64 groups of threads
+constexpr int kCands = 1024;  // candidates for them kept at once
+
+// A number's place among a row's, as an unsigned integer: -0 as +0, NaN below all.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    if ((b & 0x7fffffffu) > 0x7f800000u) return 0u;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// Running maximum m of x * c (c = scale log2 e) and, of e = 2^(x c - m), the sums
+// s of e and w of e (x c - m).
+struct Stats {
+    float m = -INFINITY, s = 0.0f, w = 0.0f;
+    // To the maximum `to` (m: as it was).
+    __device__ __forceinline__ void raise(float to) {
+        if (!(to > m)) return;
+        const float d = m - to, f = __builtin_amdgcn_exp2f(d);
+        w = s > 0.0f ? f * (w + s * d) : w;  // (s = 0: no number yet, d may be -inf)
+        s *= f;
+        m = to;
+    }
+    __device__ __forceinline__ void join(float m2, float s2, float w2) {
+        Stats o;
+        o.m = m2;
+        o.s = s2;
+        o.w = w2;
+        raise(m2);
+        o.raise(m);
+        s += o.s;
+        w += o.w;
+    }
+    // A value, with from = m (0 before the first number).  exp2 of -inf is 0, and so is
+    // that value's share of w; NaN goes into s.
+    __device__ __forceinline__ void add(float x, float c, float from) {
+        const float d = __builtin_fmaf(x, c, -from), e = __builtin_amdgcn_exp2f(d);
+        s += e;
+        w = __builtin_fmaf(e, fmaxf(d, -1000.0f), w);
+    }
+    __device__ __forceinline__ float from() const { return m == -INFINITY ? 0.0f : m; }
+};
+
+struct Fwd {
+    const void *x;
+    const uint32_t *tokens;
+    float *logp, *entropy, *lse;
+    uint32_t *ids;
+    float *tops;
+    float scale;
+    int ldx, C, K;
+};
+
+// A row a workgroup of NT threads, read once; for the alternatives the threads that
+// hold one (about as many as there are) read their own chunks again.
+//   The K-th largest of the maxima of 64 groups of threads is no more than the row's
+// K-th largest value, so every alternative is among the values from it on: about as
+// many as K where the large values lie anyhow.  Where they are more than fit (rows of
+// few different values), the K are taken one after the other, a pass over the row each.
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void logprobs_fwd(const Fwd a) {
+    using IO = Io<DT>;
+    constexpr int E = IO::E, NW = NT / 64, kDeep = 4;
+    __shared__ float sm[NW][3];
+    __shared__ uint32_t keys[kCands];
+    __shared__ int cols[kCands];
+    __shared__ uint32_t bound_s;
+    __shared__ int count_s;
+    const size_t r = blockIdx.x;
+    const auto *x = static_cast<const typename IO::T *>(a.x) + r * a.ldx;
+    const int t = threadIdx.x, nb = a.C / E;
+    const float c = a.scale * kLog2e;
+    const int single = t < a.C - nb * E ? nb * E + t : -1;
+    const uint32_t token = a.tokens[r];
+    const float xt = token < (uint32_t)a.C ? IO::load1(x, (int)token) : 0.0f;
+    Stats st;
+    float big = -INFINITY;  // the thread's largest value
+    auto take = [&](u32x4 w) {
+        float b = IO::get(w, 0);
+#pragma unroll
+        for (int e = 1; e < E; ++e) b = fmaxf(b, IO::get(w, e));
+        big = fmaxf(big, b);
+        // Raised only by values 2^4 above the maximum, which are few after the first
+        // chunks; the exact one comes at the end.
+        if (__any(b * c > st.m + 4.0f)) st.raise(b * c);
+        const float from = st.from();
+#pragma unroll
+        for (int e = 0; e < E; ++e) st.add(IO::get(w, e), c, from);
+    };
+    int j = t;
+    for (; j + (kDeep - 1) * NT < nb; j += kDeep * NT) {
+        u32x4 w[kDeep];
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) w[u] = fg::rows::load<DT>(x, j + u * NT);
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) take(w[u]);
+    }
+    for (; j < nb; j += NT) take(fg::rows::load<DT>(x, j));
+    if (single >= 0) {
+        const float v = IO::load1(x, single);
+        st.raise(v * c);
+        st.add(v, c, st.from());
+        big = fmaxf(big, v);
+    }
+    st.raise(big * c);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        st.join(__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.w, o));
+    if (NW > 1) {
+        if ((t & 63) == 0) {
+            sm[t >> 6][0] = st.m;
+            sm[t >> 6][1] = st.s;
+            sm[t >> 6][2] = st.w;
+        }
+    }
+    // (0: no number among the thread's values, or nothing above -inf.)
+    const uint32_t mine = big > -INFINITY ? order_key(big) : 0u;
+    if (a.K) {
+        keys[t] = mine;
+        if (t == 0) count_s = 0;
+    }
+    if (NW > 1 || a.K) __syncthreads();
+    if (NW > 1) {
+        st.m = sm[0][0];
+        st.s = sm[0][1];
+        st.w = sm[0][2];
+        for (int k = 1; k < NW; ++k) st.join(sm[k][0], sm[k][1], sm[k][2]);
+    }
+    const float log_s = logf(st.s);
+    if (t == 0) {
+        if (a.logp)
+            a.logp[r] = token < (uint32_t)a.C ? __builtin_fmaf(xt, c, -st.m) * kLn2 - log_s
+                                              : __builtin_nanf("");
+        if (a.entropy) a.entropy[r] = log_s - kLn2 * (st.w / st.s);
+        if (a.lse) a.lse[r] = __builtin_fmaf(st.m, kLn2, log_s);
+    }
+    if (!a.K) return;
+    if (t < 64) {
+        uint32_t g = keys[t];
+        for (int k = 1; k < NW; ++k) g = max(g, keys[k * 64 + t]);
+        int before = 0;
+#pragma unroll 8
+        for (int k = 0; k < 64; ++k) {
+            const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)g, k);
+            before += o > g || (o == g && k < t);
+        }
+        if (before == a.K - 1) bound_s = g;
+    }
+    __syncthreads();
+    const uint32_t bound = bound_s;
+    auto each = [&](auto f) {  // every (key, column, value) of the thread's
+        for (int i = t; i < nb; i += NT) {
+            const u32x4 w = fg::rows::load<DT>(x, i);
+#pragma unroll
+            for (int e = 0; e < E; ++e) f(order_key(IO::get(w, e)), i * E + e);
+        }
+        if (single >= 0) f(order_key(IO::load1(x, single)), single);
+    };
+    auto write = [&](int place, int col) {
+        if (a.ids) a.ids[r * a.K + place] = (uint32_t)col;
+        if (a.tops)
+            a.tops[r * a.K + place] = __builtin_fmaf(IO::load1(x, col), c, -st.m) * kLn2 - log_s;
+    };
+    if (mine >= bound)
+        each([&](uint32_t key, int col) {
+            if (key < bound) return;
+            const int at = atomicAdd(&count_s, 1);
+            if (at < kCands) {
+                keys[at] = key;
+                cols[at] = col;
+            }
+        });
+    __syncthreads();
+    const int n = count_s;
+    if (n >= a.K && n <= kCands) {
+        // Each at the place that as many come before it.
+        for (int i = t; i < n; i += NT) {
+            const uint32_t key = keys[i];
+            const int col = cols[i];
+            int before = 0;
+            for (int k = 0; k < n; ++k)
+                before += keys[k] > key || (keys[k] == key && cols[k] < col);
+            if (before < a.K) write(before, col);
+        }
+        return;
+    }
+    uint64_t last = ~0ull;  // (key, ~column) of the one before
+    for (int k = 0; k < a.K; ++k) {
+        uint64_t best = 0;
+        each([&](uint32_t key, int col) {
+            const uint64_t v = (uint64_t)key << 32 | (uint32_t)~col;
+            if (v < last) best = max(best, v);
+        });
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t other = (uint64_t)__shfl_xor((long long)best, o);
+            best = max(best, other);
+        }
+        __syncthreads();
+        if ((t & 63) == 0) {
+            keys[t >> 6] = (uint32_t)(best >> 32);
+            cols[t >> 6] = (int)(uint32_t)best;
+        }
+        __syncthreads();
+        for (int q = 0; q < NW; ++q) {
+            const uint64_t v = (uint64_t)keys[q] << 32 | (uint32_t)cols[q];
+            best = max(best, v);
+        }
+        last = best;
+        if (t == 0) write(k, (int)~(uint32_t)best);
+    }
+}
+
+struct Bwd {
+    const void *x;
+    const uint32_t *tokens;
+    const float *lse, *entropy, *dlogp, *dentropy;
+    void *dx;
+    float scale;
+    int ldx, lddx, R, C, lshift;
+};
+
+// Elementwise over rows of 2^lshift lanes, kBwdDeep chunks a lane, loaded together.
+// The columns past a row's whole chunks go one to a lane, so that dx may be x.  Rows of
+// no gradient (padding) are written as zeros and not read.
+constexpr int kBwdNT = 256, kBwdDeep = 4;
+template <int DT>
+__global__ __launch_bounds__(kBwdNT) void logprobs_bwd(const Bwd a) {
+    using IO = Io<DT>;
+    using T = typename IO::T;
+    constexpr int E = IO::E;
+    const int64_t row = ((int64_t)blockIdx.x << (8 - a.lshift)) + (threadIdx.x >> a.lshift);
+    if (row >= a.R) return;
+    const int step = 1 << a.lshift;
+    const int lane = threadIdx.x & (step - 1);
+    const int first = (blockIdx.y << a.lshift) * kBwdDeep + lane;
+    const T *x = static_cast<const T *>(a.x) + (size_t)row * a.ldx;
+    T *dx = static_cast<T *>(a.dx) + (size_t)row * a.lddx;
+    const int nb = a.C / E;
+    const int single = blockIdx.y == 0 && lane < a.C - nb * E ? nb * E + lane : -1;
+    const float ga = a.dlogp ? a.dlogp[row] * a.scale : 0.0f;
+    const float gb = a.dentropy ? a.dentropy[row] * a.scale : 0.0f;
+    if (ga == 0.0f && gb == 0.0f) {
+        const float zeros[E] = {};
+#pragma unroll
+        for (int u = 0; u < kBwdDeep; ++u)
+            if (first + u * step < nb) fg::rows::store<DT>(dx, first + u * step, IO::pack(zeros));
+        if (single >= 0) IO::store1(dx, single, 0.0f);
+        return;
+    }
+    const float lse = a.lse[row], h = gb != 0.0f ? a.entropy[row] : 0.0f;
+    const uint32_t token = a.tokens[row];
+    const float c = a.scale * kLog2e, from = lse * kLog2e;
+    const float k1 = -gb * a.scale, k0 = -(ga + gb * (h - lse));
+    auto grad = [&](float v, bool hot) {
+        v = fmaxf(v, -1e30f);  // (a masked logit: -inf times its probability, 0)
+        float o;
+        if constexpr (DT == fg::kF32) {
+            // z - lse rounded once; `from` would be off by 2^-24 of lse itself.
+            const float d = __builtin_fmaf(v, a.scale, -lse);
+            o = -__builtin_amdgcn_exp2f(d * kLog2e) * __builtin_fmaf(gb, d + h, ga);
+        } else {
+            o = __builtin_amdgcn_exp2f(__builtin_fmaf(v, c, -from)) * __builtin_fmaf(v, k1, k0);
+        }
+        return hot ? o + ga : o;
+    };
+    u32x4 w[kBwdDeep];
+#pragma unroll
+    for (int u = 0; u < kBwdDeep; ++u)
+        if (first + u * step < nb) w[u] = fg::rows::load<DT>(x, first + u * step);
+#pragma unroll
+    for (int u = 0; u < kBwdDeep; ++u) {
+        const int j = first + u * step;
+        if (j >= nb) break;
+        const uint32_t hot = token - (uint32_t)(j * E);
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = grad(IO::get(w[u], e), hot == (uint32_t)e);
+        fg::rows::store<DT>(dx, j, IO::pack(o));
+    }
+    if (single >= 0) IO::store1(dx, single, grad(IO::load1(x, single), token == (uint32_t)single));
+}
+
+template <int DT>
+void launch_fwd(hipStream_t st, int R, const Fwd &a) {
+    // A wave a row up to 2 chunks a lane, then four waves, then sixteen.
+    const int chunks = a.C / Io<DT>::E;
+    if (chunks <= 128) logprobs_fwd<DT, 64><<<R, 64, 0, st>>>(a);
+    else if (chunks <= 2048) logprobs_fwd<DT, 256><<<R, 256, 0, st>>>(a);
+    else logprobs_fwd<DT, 1024><<<R, 1024, 0, st>>>(a);
+}
+
+template <int DT>
+void launch_bwd(hipStream_t st, Bwd a) {
+    const int chunks = std::max(1, a.C / Io<DT>::E);
+    a.lshift = 3;  // at least as many lanes as columns past the whole chunks
+    while (a.lshift < 8 && (kBwdDeep << a.lshift) < chunks) ++a.lshift;
+    const dim3 grid(((int64_t)a.R - 1) / (kBwdNT >> a.lshift) + 1,
+                    (chunks - 1) / (kBwdDeep << a.lshift) + 1);
+    logprobs_bwd<DT><<<grid, kBwdNT, 0, st>>>(a);
+}
+
+}  // namespace
+
+FG_API int fg_token_logprobs(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
+                             const uint32_t *d_tokens, int R, int C, float scale, float *d_logp,
+                             float *d_entropy, float *d_lse, int top, uint32_t *d_top_ids,
+                             float *d_top_logp) {
+    const char *who = "fg_token_logprobs";
+    FG_REQUIRE(dtype >= FG_DTYPE_F32 && dtype <= FG_DTYPE_BF16, FG_ERR_INVALID_ARGUMENT,
+               "%s: bad dtype %d", who, dtype);
+    FG_REQUIRE(R >= 0 && C > 0, FG_ERR_SHAPE, "%s: bad shape R=%d C=%d", who, R, C);
+    FG_REQUIRE(C <= fg::rows::kMaxCols, FG_ERR_OUT_OF_BOUNDS, "%s: %d columns, at most %d", who, C,
+               fg::rows::kMaxCols);
+    FG_REQUIRE(ldx >= C, FG_ERR_SHAPE, "%s: ldx=%d < C=%d", who, ldx, C);
+    FG_REQUIRE(top >= 0 && top <= kMaxTop && top <= C, FG_ERR_OUT_OF_BOUNDS,
+               "%s: %d alternatives of %d columns, at most %d", who, top, C, kMaxTop);
+    FG_REQUIRE(scale > 0.0f && scale < INFINITY, FG_ERR_INVALID_ARGUMENT,
+               "%s: scale must be positive and finite", who);
+    FG_REQUIRE(d_logits && d_tokens, FG_ERR_INVALID_ARGUMENT, "%s: logits and tokens are required",
+               who);
+    FG_REQUIRE((top > 0) == (d_top_ids || d_top_logp), FG_ERR_INVALID_ARGUMENT,
+               "%s: %d alternatives, but %s for them", who, top,
+               top > 0 ? "no output" : "an output");
+    FG_REQUIRE(d_logp || d_entropy || d_lse || top, FG_ERR_INVALID_ARGUMENT, "%s: no output", who);
+    FG_REQUIRE(fg::rows::grid_holds(R, 1024), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns",
+               who, R, C);
+    FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_logp, {d_logits, d_tokens, d_entropy, d_lse, d_top_ids, d_top_logp}) &&
+                   apart(d_entropy, {d_logits, d_tokens, d_lse, d_top_ids, d_top_logp}) &&
+                   apart(d_lse, {d_logits, d_tokens, d_top_ids, d_top_logp}) &&
+                   apart(d_top_ids, {d_logits, d_tokens, d_top_logp}) &&
+                   apart(d_top_logp, {d_logits, d_tokens}),
+               FG_ERR_INVALID_ARGUMENT, "%s: an output is another output or an input", who);
+    if (R == 0) return FG_OK;
+    FG_HIP(hipSetDevice(ctx->device));
+    const Fwd a{d_logits, d_tokens, d_logp, d_entropy, d_lse, d_top_ids, d_top_logp, scale,
+                ldx, C, top};
+    if (dtype == FG_DTYPE_F32) launch_fwd<fg::kF32>(ctx->stream, R, a);
+    else if (dtype == FG_DTYPE_BF16) launch_fwd<fg::kBF16>(ctx->stream, R, a);
+    else launch_fwd<fg::kF16>(ctx->stream, R, a);
+    FG_LAUNCH_CHECK("logprobs_fwd");
+    return FG_OK;
+}
+
+FG_API int fg_token_logprobs_bwd(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
+                                 const uint32_t *d_tokens, int R, int C, float scale,
+                                 const float *d_lse, const float *d_entropy, const float *d_dlogp,
+                                 const float *d_dentropy, void *d_dlogits, int ldd) {
+    const char *who = "fg_token_logprobs_bwd";
+    FG_REQUIRE(dtype >= FG_DTYPE_F32 && dtype <= FG_DTYPE_BF16, FG_ERR_INVALID_ARGUMENT,
+               "%s: bad dtype %d", who, dtype);
+    FG_REQUIRE(R >= 0 && C > 0, FG_ERR_SHAPE, "%s: bad shape R=%d C=%d", who, R, C);
+    FG_REQUIRE(C <= fg::rows::kMaxCols, FG_ERR_OUT_OF_BOUNDS, "%s: %d columns, at most %d", who, C,
+               fg::rows::kMaxCols);
+    FG_REQUIRE(ldx >= C && ldd >= C, FG_ERR_SHAPE, "%s: ldx=%d or ldd=%d < C=%d", who, ldx, ldd, C);
+    FG_REQUIRE(scale > 0.0f && scale < INFINITY, FG_ERR_INVALID_ARGUMENT,
+               "%s: scale must be positive and finite", who);
+    FG_REQUIRE(d_logits && d_tokens && d_lse && d_dlogits && (d_dlogp || d_dentropy),
+               FG_ERR_INVALID_ARGUMENT,
+               "%s: logits, tokens, lse, dlogits and a gradient of logp or entropy are required",
+               who);
+    FG_REQUIRE(!d_dentropy || d_entropy, FG_ERR_INVALID_ARGUMENT,
+               "%s: the entropy's gradient needs the entropy", who);
+    FG_REQUIRE(d_dlogits != d_logits || ldd == ldx, FG_ERR_INVALID_ARGUMENT,
+               "%s: dlogits is logits, but ldd=%d, ldx=%d", who, ldd, ldx);
+    FG_REQUIRE(fg::rows::grid_holds(R, kBwdNT), FG_ERR_OUT_OF_BOUNDS, "%s: %d rows of %d columns",
+               who, R, C);
+    FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_dlogits, {d_tokens, d_lse, d_entropy, d_dlogp, d_dentropy}),
+               FG_ERR_INVALID_ARGUMENT, "%s: dlogits is an input but logits", who);
+    if (R == 0) return FG_OK;
+    FG_HIP(hipSetDevice(ctx->device));
+    const Bwd a{d_logits, d_tokens, d_lse, d_entropy, d_dlogp, d_dentropy, d_dlogits, scale,
+                ldx, ldd, R, C, 0};
+    if (dtype == FG_DTYPE_F32) launch_bwd<fg::kF32>(ctx->stream, a);
+    else if (dtype == FG_DTYPE_BF16) launch_bwd<fg::kBF16>(ctx->stream, a);
+    else launch_bwd<fg::kF16>(ctx->stream, a);
+    FG_LAUNCH_CHECK("logprobs_bwd");
+    return FG_OK;
+}

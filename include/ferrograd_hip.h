@@ -337,6 +337,57 @@ int fg_layer_norm_bwd(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const vo
                       int R, int C, void *d_dx, int lddx, int accumulate, void *d_dgamma,
                       int dgamma_accumulate, void *d_dbeta, int dbeta_accumulate);
 
+/* RMS norm over the last dimension with the residual's addition (no reference
+ * counterpart).  Per row:
+ *   s = x + r, rounded to dtype (without r: s = x)
+ *   rstd = 1/sqrt(sum(s^2) / C + eps) ;  y = s * rstd * gamma
+ * x, r, gamma[C], s, y of element type dtype, statistics and sums fp32, y rounded
+ * once.  gamma (1) may be NULL.  r and s (where the sum is kept: the backward reads
+ * it) are given together or not at all.  d_q and d_e: y in 8 bits, as fg_ckpt8_save
+ * would keep its fp32 values (int8 q[R][C], an exponent byte e[R][ceil(C / 32)] per
+ * 32 columns), for fg_matmul_bwd_ckpt8 with FG_ACT_NONE; NULL: none.  y may be NULL
+ * where they are given.  d_rstd [R] (fp32, what the backward needs) may be NULL.
+ * s may be x or r, and y the other of them (equal leading dimensions).  eps > 0. */
+int fg_rms_norm(fg_ctx *ctx, int dtype, const void *d_x, int ldx, const void *d_r, int ldr,
+                const void *d_gamma, float eps, int R, int C, void *d_s, int lds, void *d_y,
+                int ldy, int8_t *d_q, int ldq, uint8_t *d_e, int lde, float *d_rstd);
+/* Its backward from s (x without a residual), dy and rstd, xh = s * rstd,
+ * g = dy * gamma:
+ *   dx = rstd * (g - xh * mean(g * xh)) + ds     (x's gradient, and r's)
+ *   dgamma (=|+=) sum over rows of dy * xh
+ * ds: the gradient that reaches s another way (the residual's path), NULL: none.
+ * dx or dgamma may be NULL, gamma too (1).  dx may be s, dy or ds (equal leading
+ * dimensions).  dgamma's partial sums go to the workspace, 4 bytes a column for each
+ * of at most 4 row splits a CU, and are added in a fixed order.  R = 0 writes zeros to
+ * dgamma (or adds nothing). */
+int fg_rms_norm_bwd(fg_ctx *ctx, int dtype, const void *d_s, int lds, const void *d_dy, int lddy,
+                    const void *d_gamma, const float *d_rstd, int R, int C, const void *d_ds,
+                    int ldds, void *d_dx, int lddx, void *d_dgamma, int dgamma_accumulate);
+
+/* Log probabilities of given tokens (no reference counterpart; the answers next to
+ * fg_softmax_ce's loss).  Per row r of R rows of C logits, z = scale * logits:
+ *   lse[r] = log sum exp(z) ;  logp[r] = z[tokens[r]] - lse[r]
+ *   entropy[r] = -sum p log p, p = softmax(z)
+ *   top_ids[r][k], top_logp[r][k]: the k-th largest logit's column and log
+ *   probability, k < top, the lower column first among equals (NaN below all)
+ * Outputs are fp32 (top_ids u32, both [R][top]); any may be NULL.  top is at most 32
+ * and C.  A token outside [0, C) gives a NaN logp; logits of -inf (masked) have
+ * probability 0.  scale > 0 (an inverse temperature). */
+int fg_token_logprobs(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
+                      const uint32_t *d_tokens, int R, int C, float scale, float *d_logp,
+                      float *d_entropy, float *d_lse, int top, uint32_t *d_top_ids,
+                      float *d_top_logp);
+/* Its backward from lse and entropy [R], with the gradients dlogp and dentropy [R]
+ * (either may be NULL: 0; entropy is read where dentropy is given):
+ *   dlogits[c] = scale * (dlogp * ([c = token] - p_c)
+ *                         - dentropy * p_c * (z_c - lse + entropy))
+ * rounded to dtype once.  dlogits may be logits (ldd = ldx).  A row whose two
+ * gradients are 0 is zeros, whatever its logits; a token outside [0, C) is no column. */
+int fg_token_logprobs_bwd(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
+                          const uint32_t *d_tokens, int R, int C, float scale,
+                          const float *d_lse, const float *d_entropy, const float *d_dlogp,
+                          const float *d_dentropy, void *d_dlogits, int ldd);
+
 /* Embedding lookup (no reference counterpart): out[t][c] = scale *
  * table[tokens[t]][c] for T tokens and a table of V rows of C elements of
  * type dtype, rounded once.  A token outside [0, V) gives a row of NaN, as a
