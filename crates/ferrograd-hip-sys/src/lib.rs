@@ -671,6 +671,62 @@ extern "C" {
         d_dlogits: *mut c_void,
         ldd: c_int,
     ) -> c_int;
+    pub fn fg_attention(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_q: *const c_void,
+        ldq: c_int,
+        d_k: *const c_void,
+        ldk: c_int,
+        d_v: *const c_void,
+        ldv: c_int,
+        d_q_starts: *const u32,
+        d_k_starts: *const u32,
+        d_k_lens: *const u32,
+        n: c_int,
+        Tq: c_int,
+        Tk: c_int,
+        heads: c_int,
+        kv_heads: c_int,
+        D: c_int,
+        scale: f32,
+        causal: c_int,
+        d_out: *mut c_void,
+        ldo: c_int,
+        d_lse: *mut f32,
+    ) -> c_int;
+    pub fn fg_attention_bwd(
+        ctx: *mut fg_ctx,
+        dtype: c_int,
+        d_q: *const c_void,
+        ldq: c_int,
+        d_k: *const c_void,
+        ldk: c_int,
+        d_v: *const c_void,
+        ldv: c_int,
+        d_out: *const c_void,
+        ldo: c_int,
+        d_dout: *const c_void,
+        lddo: c_int,
+        d_lse: *const f32,
+        d_q_starts: *const u32,
+        d_k_starts: *const u32,
+        n: c_int,
+        Tq: c_int,
+        Tk: c_int,
+        heads: c_int,
+        kv_heads: c_int,
+        D: c_int,
+        scale: f32,
+        causal: c_int,
+        d_dq: *mut c_void,
+        lddq: c_int,
+        d_dk: *mut c_void,
+        lddk: c_int,
+        d_dv: *mut c_void,
+        lddv: c_int,
+        accumulate: c_int,
+    ) -> c_int;
     pub fn fg_mt_create(
         ctx: *mut fg_ctx,
         n: c_int,

@@ -223,6 +223,28 @@ class Context:
              _ptr(rstd), R, C, _ptr(ds), ldds or C, _ptr(dx), lddx or C, _ptr(dgamma),
              int(dgamma_accumulate))
 
+    def attention(self, q, ldq: int, k, ldk: int, v, ldv: int, q_starts, k_starts, n: int, Tq: int,
+                  Tk: int, heads: int, kv_heads: int, D: int, out, ldo: int, k_lens=None,
+                  scale: Optional[float] = None, causal: bool = True, lse=None,
+                  dtype: int = DTYPE_F32) -> None:
+        """Attention over n packed sequences (u32 starts of their rows and keys,
+        n + 1 each; k_lens: the keys used of a cache's).  scale None: 1/sqrt(D).
+        lse (fp32, [heads][Tq]) is kept when given."""
+        call("fg_attention", self.handle, dtype, _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv,
+             _ptr(q_starts), _ptr(k_starts), _ptr(k_lens), n, Tq, Tk, heads, kv_heads, D,
+             D ** -0.5 if scale is None else scale, int(causal), _ptr(out), ldo, _ptr(lse))
+
+    def attention_bwd(self, q, ldq: int, k, ldk: int, v, ldv: int, out, ldo: int, dout, lddo: int,
+                      lse, q_starts, k_starts, n: int, Tq: int, Tk: int, heads: int, kv_heads: int,
+                      D: int, dq, lddq: int, dk, lddk: int, dv, lddv: int,
+                      scale: Optional[float] = None, causal: bool = True, accumulate: bool = False,
+                      dtype: int = DTYPE_F32) -> None:
+        """dq, dk and dv from dout and the forward's out and lse."""
+        call("fg_attention_bwd", self.handle, dtype, _ptr(q), ldq, _ptr(k), ldk, _ptr(v), ldv,
+             _ptr(out), ldo, _ptr(dout), lddo, _ptr(lse), _ptr(q_starts), _ptr(k_starts), n, Tq, Tk,
+             heads, kv_heads, D, D ** -0.5 if scale is None else scale, int(causal), _ptr(dq), lddq,
+             _ptr(dk), lddk, _ptr(dv), lddv, int(accumulate))
+
     def token_logprobs(self, logits, ldx: int, tokens, R: int, C: int, logp=None, entropy=None,
                        lse=None, top: int = 0, top_ids=None, top_logp=None, scale: float = 1.0,
                        dtype: int = DTYPE_F32) -> None:

@@ -42,6 +42,10 @@ SOURCES = [
     "k_ckpt8.hip",
     "k_rms_norm.hip",
     "k_logprobs.hip",
+    "k_attention.hip",
+    "k_attention_bf16.hip",
+    "k_attention_f16.hip",
+    "k_attention_f32.hip",
     "fg_graph.cpp",
     "fg_bpat.cpp",
     "fg_telemetry.cpp",

@@ -102,6 +102,11 @@ SIGNATURES = {
                               i32]),
     "fg_token_logprobs": (i32, [vp, i32, vp, i32, vp, i32, i32, f32, vp, vp, vp, i32, vp, vp]),
     "fg_token_logprobs_bwd": (i32, [vp, i32, vp, i32, vp, i32, i32, f32, vp, vp, vp, vp, vp, i32]),
+    "fg_attention": (i32, [vp, i32, vp, i32, vp, i32, vp, i32, vp, vp, vp, i32, i32, i32, i32, i32,
+                           i32, f32, i32, vp, i32, vp]),
+    "fg_attention_bwd": (i32, [vp, i32, vp, i32, vp, i32, vp, i32, vp, i32, vp, i32, vp, vp, vp,
+                               i32, i32, i32, i32, i32, i32, f32, i32, vp, i32, vp, i32, vp, i32,
+                               i32]),
     "fg_mt_create": (i32, [vp, i32, vp, vp, vp, vp, vp, pvp]),
     "fg_mt_destroy": (i32, [vp]),
     "fg_sgd_step": (i32, [vp, vp, f32, i32]),

@@ -1,0 +1,1200 @@
+// fg_attention_kernel.h -- attention over packed sequences, forward and backward, on
+// CDNA4 matrix cores.  Included by k_attention_{bf16,f16,f32}.hip.  The reference has
+// no attention; its nearest operators are the matmul and softmax nodes
+// (crates/ferrograd-nn/src/op/matmul/mod.rs:17-188, op/softmax.rs:14-759).
+//
+//   S = scale Q K^T, -inf where a key is not visible;  P = softmax of S's rows
+//   O = P V,  lse = log sum exp of S's rows
+//   delta = rows' sums of dO O,  dS = P (dO V^T - delta)
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
+// Key j of lk is visible to query i of lq if j < lk and, causal, j <= i + lk - lq.
+//
+// One layout serves every product.  An MFMA's result has its column in the lane and
+// its rows in the lane's registers, rows 8 (r / 4) + 4 h + r % 4 for register r of lane
+// half h; an operand has its row (or column) in the lane and 8 of the summed index in
+// its registers.  So S^T = K Q^T (keys in registers, a query a lane) is, rounded, the
+// second operand of O^T = V^T P^T and dQ^T = K^T dS^T as it stands, and S = Q K^T
+// (queries in registers, a key a lane) that of dV^T = dO^T P and dK^T = Q^T dS -- if the
+// first operand takes its 8 of the summed index in the same order, 4 h + 0..3 and
+// 8 + 4 h + 0..3 of each 16.  Softmax statistics are a lane's own, but for the half of
+// the keys that lane ^ 32 holds.
+//
+// Tiles sit in LDS as rows of DP elements with 16-byte chunk c of row r at c ^ swz(r):
+// read by rows (8 lanes a cycle, the same chunk of 8 rows) and, through the transposing
+// reads, by columns (4 rows of 2 chunks a cycle), both reach distinct banks.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "fg_attention.h"
+#include "fg_half.h"
+#include "fg_sched.h"
+
+namespace fg {
+namespace attn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef short v4i16 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+
+// Bits of a chunk's place that its row sets.
+__device__ __forceinline__ int swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+
+template <int DT>
+struct Type {
+    static constexpr bool kWide = DT == kF32;
+    using T = typename std::conditional<kWide, float, uint16_t>::type;
+    using Frag = typename std::conditional<kWide, f32x8, u32x4>::type;
+    static constexpr int E = kWide ? 4 : 8;  // elements of a 16-byte chunk
+
+    // A 32x32 block's product over 16 of the summed index.  fp32: eight instructions of
+    // two (one of a lane half each), element j of both operands in the j-th.
+    static __device__ __forceinline__ f32x16 mfma(const Frag &a, const Frag &b, f32x16 c) {
+        if constexpr (kWide) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+            return c;
+        } else if constexpr (DT == kBF16) {
+            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                           __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                           0);
+        } else {
+            return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                          __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+        }
+    }
+    // Registers 8 u .. 8 u + 7 of a block of fp32 values, rounded, as an operand.
+    static __device__ __forceinline__ Frag pack(const f32x16 &s, int u) {
+        Frag f;
+        if constexpr (kWide) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = s[8 * u + j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = s[8 * u + 2 * j], y = s[8 * u + 2 * j + 1];
+                if constexpr (DT == kBF16)
+                    f[j] = __builtin_bit_cast(uint32_t,
+                                              __builtin_convertvector((f32x2{x, y}), bf16x2));
+                else f[j] = (uint32_t)f_to_f16(x) | ((uint32_t)f_to_f16(y) << 16);
+            }
+        }
+        return f;
+    }
+    static __device__ __forceinline__ float get(const Frag &f, int j) {
+        if constexpr (kWide) return f[j];
+        else return h16_to_f(DT, (uint16_t)(f[j >> 1] >> (16 * (j & 1))));
+    }
+    static __device__ __forceinline__ float load1(const T *p) {
+        if constexpr (kWide) return *p;
+        else return h16_to_f(DT, *p);
+    }
+    static __device__ __forceinline__ void store1(T *p, float v) {
+        if constexpr (kWide) *p = v;
+        else *p = f_to_h16(DT, v);
+    }
+    // Elements d .. d + 7 of a row of D (zeros past it; row NULL: zeros).
+    static __device__ __forceinline__ Frag load8(const T *row, int d, int D) {
+        Frag f;
+        if (row && d + 8 <= D) {
+            if constexpr (kWide) {
+                const f32x4 x = *reinterpret_cast<const f32x4_any *>(row + d);
+                const f32x4 y = *reinterpret_cast<const f32x4_any *>(row + d + 4);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = j < 4 ? x[j & 3] : y[j & 3];
+            } else {
+                f = *reinterpret_cast<const u32x4_any *>(row + d);
+            }
+            return f;
+        }
+        T e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = row && d + j < D ? row[d + j] : T(0);
+        if constexpr (kWide) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = e[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = (uint32_t)e[2 * j] | ((uint32_t)e[2 * j + 1] << 16);
+        }
+        return f;
+    }
+    // Four values from column d on of a row of D; (=|+=), each rounded once.
+    static __device__ __forceinline__ void store4(T *row, int d, int D, f32x4 v, bool add) {
+        if (d + 4 <= D) {
+            if constexpr (kWide) {
+                f32x4_any *p = reinterpret_cast<f32x4_any *>(row + d);
+                *p = add ? *p + v : v;
+            } else {
+                u32x2_any *p = reinterpret_cast<u32x2_any *>(row + d);
+                if (add) {
+                    const u32x2 w = *p;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        v[e] += h16_to_f(DT, (uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+                }
+                u32x2 w;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (DT == kBF16)
+                        w[j] = __builtin_bit_cast(
+                            uint32_t,
+                            __builtin_convertvector((f32x2{v[2 * j], v[2 * j + 1]}), bf16x2));
+                    else
+                        w[j] = (uint32_t)f_to_f16(v[2 * j]) |
+                               ((uint32_t)f_to_f16(v[2 * j + 1]) << 16);
+                }
+                *p = w;
+            }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < D) store1(row + d + e, add ? v[e] + load1(row + d + e) : v[e]);
+    }
+};
+
+// ------------------------------------------------------------------ LDS tiles
+// ROWS rows of DP elements.
+template <int DT, int DP, int ROWS>
+struct Tile {
+    using Ty = Type<DT>;
+    using T = typename Ty::T;
+    using Frag = typename Ty::Frag;
+    static constexpr int E = Ty::E, CH = DP / E;  // chunks of a row
+    static constexpr int kElems = ROWS * DP;
+    static constexpr int kChunks = ROWS * CH;
+
+    static __device__ __forceinline__ const T *at(const T *t, int row, int chunk) {
+        return t + row * DP + ((chunk ^ swz(row)) * E);
+    }
+    // Row `row`, elements 16 ks + 8 h .. + 7: an operand with the tile's rows in lanes.
+    static __device__ __forceinline__ Frag by_row(const T *t, int row, int ks, int h) {
+        if constexpr (Ty::kWide) {
+            Frag f;
+            const int c = 4 * ks + 2 * h;
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(at(t, row, c));
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(at(t, row, c + 1));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = j < 4 ? x[j & 3] : y[j & 3];
+            return f;
+        } else {
+            return *reinterpret_cast<const u32x4 *>(at(t, row, 2 * ks + h));
+        }
+    }
+    // Column d0 + lane % 32, rows r0 + 4 h + 0..3 and r0 + 8 + 4 h + 0..3: an operand
+    // with the tile's columns in lanes.  16 bits: two transposing reads, in which source
+    // lane 4 e + q of each 16 reads 4 elements of row e, and lane l gets column l's rows.
+    static __device__ __forceinline__ Frag by_column(const T *t, int r0, int d0, int lane) {
+        const int h = lane >> 5;
+        Frag f;
+        if constexpr (Ty::kWide) {
+            const int d = d0 + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = r0 + 8 * (j >> 2) + 4 * h + (j & 3);
+                f[j] = at(t, row, d >> 2)[d & 3];
+            }
+        } else {
+            const int e = (lane >> 2) & 3, q = lane & 3;
+            const int d = d0 + (lane & 16) + 4 * q;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = r0 + 8 * half + 4 * h + e;
+                const v4i16 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) v4i16 *)(at(t, row, d >> 3) + (d & 7)));
+                const u32x2 w = __builtin_bit_cast(u32x2, v);
+                f[2 * half] = w[0];
+                f[2 * half + 1] = w[1];
+            }
+        }
+        return f;
+    }
+    // Whether the whole tile is finite (by one wave).
+    static __device__ __forceinline__ bool finite(const T *t, int lane) {
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        uint32_t top = 0;
+#pragma unroll 4
+        for (int c = lane; c < kChunks; c += 64) {
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(t + c * E);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (Ty::kWide) {
+                    top = max(top, w[e] & 0x7fffffffu);
+                } else {
+                    top = __builtin_bit_cast(
+                        uint32_t,
+                        __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                  __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu)));
+                }
+            }
+        }
+        constexpr uint32_t kInf = DT == kF16 ? 0x7c00u : 0x7f80u;
+        bool bad;
+        if constexpr (Ty::kWide) bad = top >= 0x7f800000u;
+        else bad = (top & 0xffffu) >= kInf || (top >> 16) >= kInf;
+        return !__any(bad);
+    }
+};
+
+// Moves a tile's rows from memory, NT threads together (tid among them; wave of them,
+// lane).  DMA: straight into LDS, lane l of a wave load at its 16 l bytes, the source
+// chosen so that the chunks land swizzled; rows past the last are the last again.
+// Otherwise through registers, zeros past the last row and column.
+template <int DT, int DP, int ROWS, int NT, bool DMA>
+struct Mover {
+    using Tl = Tile<DT, DP, ROWS>;
+    using T = typename Tl::T;
+    static constexpr int E = Tl::E, CH = Tl::CH;
+    static constexpr int kPer = Tl::kChunks / NT;
+    static_assert(Tl::kChunks % NT == 0, "whole chunks a thread");
+    u32x4 v[DMA ? 1 : kPer];
+
+    // row_at(r): row r's first element, of the last row for those past it.
+    template <class F>
+    __device__ __forceinline__ void load(T *lds, int tid, int rows, int D, F row_at) {
+        const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if constexpr (DMA) {
+                const int li = wave * kPer + i, pos = li * 64 + lane;
+                const int row = pos / CH, c = (pos % CH) ^ swz(row);
+                lds_dma16(row_at(row) + c * E, lds + li * 64 * E);
+            } else {
+                const int pos = i * NT + tid, row = pos / CH, d = (pos % CH) * E;
+                const T *p = row_at(row) + d;
+                if (row < rows && d + E <= D) {
+                    v[i] = *reinterpret_cast<const u32x4_any *>(p);
+                } else {
+                    T e[E];
+#pragma unroll
+                    for (int k = 0; k < E; ++k) e[k] = row < rows && d + k < D ? p[k] : T(0);
+                    v[i] = __builtin_bit_cast(u32x4, e);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *lds, int tid) const {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int pos = i * NT + tid, row = pos / CH, c = pos % CH;
+                *reinterpret_cast<u32x4 *>(lds + row * DP + ((c ^ swz(row)) * E)) = v[i];
+            }
+        }
+    }
+};
+
+// The wave's direct loads have landed and its LDS reads are done, and every other
+// wave's.
+__device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// ------------------------------------------------------------------ sequences
+// Sequence of work slot `slot` and its tile there: sequence s has the slots from
+// start(s) = first(s) / per + s on (first: its first row, or key), at least as many as
+// tiles, so that neither a list of tiles nor the lengths on the host are needed.  A wave
+// tries 64 sequences at a time.
+struct Place {
+    int seq, tile;
+};
+template <class F>
+__device__ __forceinline__ Place place_of(int slot, int n, F start) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, len = n;  // the sequence is in [lo, lo + len)
+    while (len > 1) {
+        const int step = (len + 63) >> 6;
+        const int s = lo + lane * step;
+        const bool past = lane * step < len && start(s) <= slot;
+        const int k = max(1, (int)__popcll(__ballot(past))) - 1;
+        lo += k * step;
+        len = min(step, len - k * step);
+        if (step == 1) break;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    return {lo, slot - start(lo)};
+}
+
+// A sequence's rows and keys, whatever its offsets say within the matrices.
+struct Seq {
+    int q0, lq, k0, lk;
+    __device__ __forceinline__ Seq(const Args &a, int s) {
+        q0 = (int)min(a.qs[s], (uint32_t)a.Tq);
+        lq = max(0, (int)min(a.qs[s + 1], (uint32_t)a.Tq) - q0);
+        k0 = (int)min(a.ks[s], (uint32_t)a.Tk);
+        lk = max(0, (int)min(a.ks[s + 1], (uint32_t)a.Tk) - k0);
+        if (a.klens) lk = (int)min((uint32_t)lk, a.klens[s]);
+    }
+};
+
+// Key head and slot of a workgroup.  Consecutive workgroups go to the 8 XCDs in turn:
+// the key heads vary fastest, eight at a time where they come in eights, so that an
+// XCD's L2 keeps few heads' keys.
+struct Work {
+    int kv, slot;
+    __device__ __forceinline__ Work(int bid, int KV, int slots) {
+        const int by = KV % 8 == 0 ? 8 : KV;
+        const int g = bid / (by * slots), in = bid - g * by * slots;
+        slot = in / by;
+        kv = g * by + in - slot * by;
+    }
+};
+
+// acc[b] (columns in lanes, rows d in registers) += sum over the 32 rows k of a tile
+// from r0 on of tile[r0 + k][d] * w[k], only those with lo <= k <= hi of the lane: what
+// the MFMA does where masked rows hold infinities or NaN, which 0 times is NaN.
+// scratch: 32 x 32 floats of the wave.
+template <int DT, int DP, int ROWS, int NB>
+__device__ __forceinline__ void add_careful(f32x16 (&acc)[NB], const f32x16 &w, const void *tile,
+                                            int r0, int lo, int hi, float *scratch, int lane) {
+    using Tl = Tile<DT, DP, ROWS>;
+    using T = typename Tl::T;
+    const T *t = static_cast<const T *>(tile);
+    const int h = lane >> 5, l32 = lane & 31;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < 16; ++r) scratch[(8 * (r >> 2) + 4 * h + (r & 3)) * 32 + l32] = w[r];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int k = 0; k < 32; ++k) {
+        const float x = scratch[k * 32 + l32];
+        const bool on = k >= lo && k <= hi;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int d = 32 * b + 8 * q + 4 * h;
+                const T *p = Tl::at(t, r0 + k, d / Tl::E) + d % Tl::E;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[b][4 * q + e] += on ? x * Type<DT>::load1(p + e) : 0.0f;
+            }
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <int NB>
+__device__ __forceinline__ void clear(f32x16 (&acc)[NB]) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[b][r] = 0.0f;
+}
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+    return z;
+}
+
+// ------------------------------------------------------------------- forward
+// A wave's 32 rows (one a lane, both halves): queries as operands, running statistics
+// and O^T.  m is a score that the exponentials are taken from, raised only by scores far
+// above it (the sums stay far from overflow; the quotient is the same), so that O is
+// seldom rescaled.  fp16 probabilities carry a factor of 2^8: the smallest that count
+// stay above the type's subnormals.
+template <int DT, int DP, int KT>
+struct Rows {
+    using Ty = Type<DT>;
+    using T = typename Ty::T;
+    using Tl = Tile<DT, DP, KT>;
+    static constexpr int NB = DP / 32, NK = DP / 16;
+    static constexpr float kUp = DT == kF16 ? 8.0f : 0.0f, kRaise = DT == kF16 ? 4.0f : 8.0f;
+    typename Ty::Frag q[NK];
+    f32x16 o[NB];
+    float m = -INFINITY, l = 0.0f;
+
+    // Keys key0 .. key0 + KT - 1 in tiles k and v, up to `last` for the lane's row; whole:
+    // every one is visible to every row of the wave.
+    __device__ __forceinline__ void step(const T *k, const T *v, int key0, int last, bool whole,
+                                         float c, float *scratch, int lane) {
+        const int h = lane >> 5, l32 = lane & 31;
+        constexpr int KB = KT / 32;
+        f32x16 s[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            s[b] = zero16();
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks)
+                s[b] = Ty::mfma(Tl::by_row(k, 32 * b + l32, ks, h), q[ks], s[b]);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = key0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
+                    s[b][r] = key <= last ? s[b][r] : -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        if (__any((top - m) * c > kRaise)) {
+            const float to = fmaxf(m, top);
+            const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[b][r] *= f;
+        }
+        const float from = (m == -INFINITY ? 0.0f : m * c) - kUp;
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], c, -from));
+                part[r & 3] += s[b][r];
+            }
+        l += (part[0] + part[1]) + (part[2] + part[3]);
+        if (!whole && !Tl::finite(v, lane)) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+                add_careful<DT, DP, KT>(o, s[b], v, 32 * b, 0, last - key0 - 32 * b, scratch, lane);
+            return;
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const typename Ty::Frag p = Ty::pack(s[b], u);
+#pragma unroll
+                for (int d = 0; d < NB; ++d)
+                    o[d] = Ty::mfma(Tl::by_column(v, 32 * b + 16 * u, 32 * d, lane), p, o[d]);
+            }
+    }
+};
+
+// Where a row's outputs go.  at: its place among the key head's rows.
+template <int DT, int DP>
+__device__ __forceinline__ void write_row(const Args &a, int kv, int split, int row, int token,
+                                          int g, int h, const f32x16 (&o)[DP / 32], float m,
+                                          float l, float c) {
+    using Ty = Type<DT>;
+    using T = typename Ty::T;
+    constexpr float kUp = Rows<DT, DP, 32>::kUp;
+    if (a.splits > 1) {
+        const int64_t rows = (int64_t)a.KV * a.Tq * a.G;
+        const int64_t at = (int64_t)split * rows + (int64_t)kv * a.Tq * a.G + row;
+        if (h == 0) {
+            float *ml = a.part + a.splits * rows * a.D + 2 * at;
+            ml[0] = m;
+            ml[1] = l;
+        }
+        if (l == 0.0f) return;
+        float *p = a.part + at * a.D;
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                Type<kF32>::store4(p, 32 * b + 8 * q + 4 * h, a.D,
+                                   f32x4{o[b][4 * q], o[b][4 * q + 1], o[b][4 * q + 2],
+                                         o[b][4 * q + 3]},
+                                   false);
+        return;
+    }
+    const int head = kv * a.G + g;
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    T *p = static_cast<T *>(a.out) + token * a.ldo + (int64_t)head * a.D;
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            Ty::store4(p, 32 * b + 8 * q + 4 * h, a.D,
+                       f32x4{o[b][4 * q] * f, o[b][4 * q + 1] * f, o[b][4 * q + 2] * f,
+                             o[b][4 * q + 3] * f},
+                       false);
+    if (a.lse && h == 0)
+        a.lse[(int64_t)head * a.Tq + token] =
+            l == 0.0f ? -INFINITY : (m * c + (__log2f(l) - kUp)) * kLn2;
+}
+
+// Four waves of 32 rows, the same keys for all: K and V tiles of KT keys, two stages.
+template <int DT>
+constexpr int keys_of() {
+    return DT == kF32 ? 32 : 64;
+}
+
+template <int DT, int DP, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
+att_fwd(const Args a) {
+    using Ty = Type<DT>;
+    using T = typename Ty::T;
+    constexpr int KT = keys_of<DT>();
+    using Tl = Tile<DT, DP, KT>;
+    __shared__ __attribute__((aligned(16))) T lds[4 * Tl::kElems];
+    __shared__ float scratch[4][32 * 32];
+    const Work w(blockIdx.x, a.KV, a.slots);
+    const Place pl = place_of(a.slots - 1 - w.slot, a.n, [&](int s) {
+        return (int)min(a.qs[s], (uint32_t)a.Tq) * a.G / kRows + s;
+    });
+    const Seq sq(a, pl.seq);
+    const int rows = sq.lq * a.G, m0 = pl.tile * kRows;
+    if (pl.tile < 0 || m0 >= rows) return;  // (a slot of no tile)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, l32 = lane & 31, off = sq.lk - sq.lq;
+    const float c = a.scale * kLog2e;
+    const T *k = static_cast<const T *>(a.k) + sq.k0 * a.ldk + (int64_t)w.kv * a.D;
+    const T *v = static_cast<const T *>(a.v) + sq.k0 * a.ldv + (int64_t)w.kv * a.D;
+    // The last key that a row sees.
+    auto last_of = [&](int row) {
+        return a.causal ? min(sq.lk - 1, a.group.of(row) + off) : sq.lk - 1;
+    };
+    const int w0 = m0 + 32 * wave, row = w0 + l32;
+    const int token = sq.q0 + a.group.of(row), g = row - (token - sq.q0) * a.G;
+    const int last = row < rows ? last_of(row) : -1;
+    const int wave_first = w0 < rows ? last_of(w0) : -1;
+    const int wave_last = w0 < rows ? last_of(min(w0 + 31, rows - 1)) : -1;
+    const int keys = last_of(min(m0 + kRows, rows) - 1) + 1;
+    const int tiles = keys > 0 ? (keys - 1) / KT + 1 : 0;
+    const int t0 = (int)((int64_t)tiles * blockIdx.y / a.splits);
+    const int t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / a.splits);
+
+    Rows<DT, DP, KT> st;
+    const T *qrow = row < rows ? static_cast<const T *>(a.q) + token * a.ldq +
+                                     (int64_t)(w.kv * a.G + g) * a.D
+                               : nullptr;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) st.q[ks] = Ty::load8(qrow, 16 * ks + 8 * h, a.D);
+    clear(st.o);
+
+    Mover<DT, DP, KT, 256, DMA> mk, mv;
+    auto load = [&](int t) {
+        T *to = lds + (t & 1) * 2 * Tl::kElems;
+        const int key0 = t * KT, left = sq.lk - key0;
+        mk.load(to, tid, left, a.D, [&](int r) { return k + min(key0 + r, sq.lk - 1) * a.ldk; });
+        mv.load(to + Tl::kElems, tid, left, a.D,
+                [&](int r) { return v + min(key0 + r, sq.lk - 1) * a.ldv; });
+    };
+    auto store = [&](int t) {
+        T *to = lds + (t & 1) * 2 * Tl::kElems;
+        mk.store(to, tid);
+        mv.store(to + Tl::kElems, tid);
+    };
+    if (t0 < t1) {
+        load(t0);
+        store(t0);
+    }
+    for (int t = t0; t < t1; ++t) {
+        // The tile has landed, and every wave is done with the one before it.
+        if constexpr (DMA) landed();
+        else __syncthreads();
+        if (t + 1 < t1) load(t + 1);
+        const int key0 = t * KT;
+        const T *at = lds + (t & 1) * 2 * Tl::kElems;
+        if (key0 <= wave_last)
+            st.step(at, at + Tl::kElems, key0, last, key0 + KT - 1 <= wave_first, c, scratch[wave],
+                    lane);
+        if (t + 1 < t1) store(t + 1);
+    }
+    st.l += __shfl_xor(st.l, 32);
+    if (row < rows)
+        write_row<DT, DP>(a, w.kv, blockIdx.y, sq.q0 * a.G + row, token, g, h, st.o, st.m, st.l, c);
+}
+
+// Few rows (single tokens: a group's heads): 32 rows a workgroup, whose four waves take
+// key tiles in turn, each through LDS of its own, without barriers; their statistics and
+// sums are joined at the end.
+constexpr int kFewKeys = 32;
+template <int DT, int DP, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void att_fwd_few(
+    const Args a) {
+    using Ty = Type<DT>;
+    using T = typename Ty::T;
+    constexpr int KT = kFewKeys, NB = DP / 32;
+    using Tl = Tile<DT, DP, KT>;
+    // A wave's two stages of K and V; at the end its O^T, 32 x DP floats.
+    constexpr int kStages = DT == kF32 && DP > 64 ? 1 : 2;
+    constexpr int kWave = kStages * 2 * Tl::kElems;
+    static_assert(kWave * sizeof(T) >= 32 * DP * sizeof(float), "room for the sums");
+    __shared__ __attribute__((aligned(16))) T lds[4 * kWave];
+    __shared__ float scratch[4][32 * 32];
+    __shared__ float ml[4][32][2];
+    const Work w(blockIdx.x, a.KV, a.slots);
+    const Place pl = place_of(w.slot, a.n, [&](int s) {
+        return (int)min(a.qs[s], (uint32_t)a.Tq) * a.G / kFewRows + s;
+    });
+    const Seq sq(a, pl.seq);
+    const int rows = sq.lq * a.G, m0 = pl.tile * kFewRows;
+    if (pl.tile < 0 || m0 >= rows) return;  // (a slot of no tile)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, l32 = lane & 31, off = sq.lk - sq.lq;
+    const float c = a.scale * kLog2e;
+    const T *k = static_cast<const T *>(a.k) + sq.k0 * a.ldk + (int64_t)w.kv * a.D;
+    const T *v = static_cast<const T *>(a.v) + sq.k0 * a.ldv + (int64_t)w.kv * a.D;
+    auto last_of = [&](int row) {
+        return a.causal ? min(sq.lk - 1, a.group.of(row) + off) : sq.lk - 1;
+    };
+    const int row = m0 + l32;
+    const int token = sq.q0 + a.group.of(row), g = row - (token - sq.q0) * a.G;
+    const int last = row < rows ? last_of(row) : -1;
+    const int first = last_of(m0);
+    const int keys = last_of(min(m0 + kFewRows, rows) - 1) + 1;
+    const int tiles = keys > 0 ? (keys - 1) / KT + 1 : 0;
+    const int t0 = (int)((int64_t)tiles * blockIdx.y / a.splits) + wave;
+    const int t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / a.splits);
+
+    Rows<DT, DP, KT> st;
+    const T *qrow = row < rows ? static_cast<const T *>(a.q) + token * a.ldq +
+                                     (int64_t)(w.kv * a.G + g) * a.D
+                               : nullptr;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) st.q[ks] = Ty::load8(qrow, 16 * ks + 8 * h, a.D);
+    clear(st.o);
+
+    T *mine = lds + wave * kWave;
+    Mover<DT, DP, KT, 64, DMA> mk, mv;
+    auto load = [&](int t, int stage) {
+        T *to = mine + stage * 2 * Tl::kElems;
+        const int key0 = t * KT, left = sq.lk - key0;
+        mk.load(to, lane, left, a.D, [&](int r) { return k + min(key0 + r, sq.lk - 1) * a.ldk; });
+        mv.load(to + Tl::kElems, lane, left, a.D,
+                [&](int r) { return v + min(key0 + r, sq.lk - 1) * a.ldv; });
+    };
+    auto store = [&](int stage) {
+        T *to = mine + stage * 2 * Tl::kElems;
+        mk.store(to, lane);
+        mv.store(to + Tl::kElems, lane);
+    };
+    int stage = 0;
+    if (t0 < t1) {
+        load(t0, 0);
+        store(0);
+    }
+    for (int t = t0; t < t1; t += 4) {
+        const int next = kStages > 1 ? stage ^ 1 : 0;
+        const bool more = t + 4 < t1;
+        // DMA: this wave's loads of tile t are done when only the next tile's are left.
+        if constexpr (DMA) {
+            // (The reads of the stage that the next loads fill are done first.)
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (more) {
+                load(t + 4, next);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Mover<DT, DP, KT, 64, DMA>::kPer)
+                             : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+        } else {
+            __builtin_amdgcn_wave_barrier();
+            if (more) load(t + 4, next);
+        }
+        const int key0 = t * KT;
+        const T *at = mine + stage * 2 * Tl::kElems;
+        st.step(at, at + Tl::kElems, key0, last, key0 + KT - 1 <= first, c, scratch[wave], lane);
+        if constexpr (!DMA) {
+            __builtin_amdgcn_wave_barrier();
+            if (more) store(next);
+            __builtin_amdgcn_wave_barrier();
+        }
+        stage = next;
+    }
+    st.l += __shfl_xor(st.l, 32);
+    // Join the waves: from their largest m, O scaled by each wave into its own LDS, added
+    // by the first.
+    if (h == 0) {
+        ml[wave][l32][0] = st.m;
+        ml[wave][l32][1] = st.l;
+    }
+    __syncthreads();
+    float m = ml[0][l32][0];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) m = fmaxf(m, ml[k][l32][0]);
+    const float f = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((st.m - m) * c);
+    float l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float mk_ = ml[k][l32][0];
+        l += mk_ == -INFINITY ? ml[k][l32][1]  // (0, or NaN)
+                              : ml[k][l32][1] * __builtin_amdgcn_exp2f((mk_ - m) * c);
+    }
+    float *os = reinterpret_cast<float *>(mine);
+    const bool any = st.l != 0.0f;  // (a wave without keys adds nothing)
+    if (wave > 0) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                os[(16 * b + r) * 64 + lane] = any ? st.o[b][r] * f : 0.0f;
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            float s = any ? st.o[b][r] * f : 0.0f;
+#pragma unroll
+            for (int k = 1; k < 4; ++k)
+                s += reinterpret_cast<const float *>(lds + k * kWave)[(16 * b + r) * 64 + lane];
+            st.o[b][r] = s;
+        }
+    if (row < rows)
+        write_row<DT, DP>(a, w.kv, blockIdx.y, sq.q0 * a.G + row, token, g, h, st.o, m, l, c);
+}
+
+// Joins a row's splits, a wave a row, 4 rows a workgroup; rows of no sequence are left.
+template <int DT>
+__global__ __launch_bounds__(256) void att_combine(const Args a) {
+    using Ty = Type<DT>;
+    using T = typename Ty::T;
+    constexpr float kUp = Rows<DT, 32, 32>::kUp;
+    const int lane = threadIdx.x & 63;
+    const int64_t rows = (int64_t)a.KV * a.Tq * a.G;
+    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= rows) return;
+    const int kv = (int)(at / ((int64_t)a.Tq * a.G));
+    const int row = (int)(at - (int64_t)kv * a.Tq * a.G);
+    const int token = a.group.of(row), g = row - token * a.G;
+    const Place pl = place_of(token, a.n, [&](int s) { return (int)min(a.qs[s], (uint32_t)a.Tq); });
+    const Seq sq(a, pl.seq);
+    if (token < sq.q0 || token >= sq.q0 + sq.lq) return;
+    const float c = a.scale * kLog2e;
+    const float *ml = a.part + a.splits * rows * a.D;
+    // Lane s takes split s's weight.
+    float m = -INFINITY, l = 0.0f;
+    if (lane < a.splits) {
+        m = ml[2 * (lane * rows + at)];
+        l = ml[2 * (lane * rows + at) + 1];
+    }
+    float top = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float f = m == -INFINITY ? (l == l ? 0.0f : l) : __builtin_amdgcn_exp2f((m - top) * c);
+    float sum = l == 0.0f ? 0.0f : l * f;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    const int head = kv * a.G + g;
+    T *p = static_cast<T *>(a.out) + token * a.ldo + (int64_t)head * a.D;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    for (int d = lane; d < ((a.D + 63) & ~63); d += 64) {
+        float s = 0.0f;
+        for (int k = 0; k < a.splits; ++k) {
+            const float fk = __shfl(f, k), lk = __shfl(l, k);
+            if (lk != 0.0f && d < a.D) s += fk * a.part[(k * rows + at) * a.D + d];
+        }
+        if (d < a.D) Ty::store1(p + d, s * inv);
+    }
+    if (a.lse && lane == 0)
+        a.lse[(int64_t)head * a.Tq + token] =
+            sum == 0.0f ? -INFINITY : (top * c + (__log2f(sum) - kUp)) * kLn2;
+}
+
+// ------------------------------------------------------------------ backward
+// dS of fp16 tensors carries a power of two that brings it near 1, whatever dout's size:
+// probabilities of long rows times small gradients would be subnormal.  From a number
+// above the largest |dout| of its rows (their V of order 1: what is summed stays within
+// the type up to |V| of some hundreds).
+__device__ __forceinline__ int exponent_above(float x) {
+    return max((int)((__float_as_uint(x) & 0x7fffffffu) >> 23) - 126, -100);
+}
+__device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
+constexpr float kUpDs = 4.0f;  // its power above 1 / the largest |dout|
+constexpr float kUpP = 8.0f;   // fp16: the probabilities' that dV is summed from
+
+// dQ, a tile of rows a workgroup, in the forward's layout; and for the pass over the
+// keys, in the order of the key head's rows, log2 of their sums, delta and (fp16) their
+// largest |dout|.
+template <int DT, int DP, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
+att_bwd_q(const Args a) {
+    using Ty = Type<DT>;
+    using T = typename Ty::T;
+    constexpr int KT = keys_of<DT>(), NB = DP / 32, NK = DP / 16;
+    using Tl = Tile<DT, DP, KT>;
+    __shared__ __attribute__((aligned(16))) T lds[4 * Tl::kElems];
+    __shared__ float scratch[4][32 * 32];
+    const Work w(blockIdx.x, a.KV, a.slots);
+    const Place pl = place_of(a.slots - 1 - w.slot, a.n, [&](int s) {
+        return (int)min(a.qs[s], (uint32_t)a.Tq) * a.G / kRows + s;
+    });
+    const Seq sq(a, pl.seq);
+    const int rows = sq.lq * a.G, m0 = pl.tile * kRows;
+    if (pl.tile < 0 || m0 >= rows) return;  // (a slot of no tile)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, l32 = lane & 31, off = sq.lk - sq.lq;
+    const float c = a.scale * kLog2e;
+    const T *k = static_cast<const T *>(a.k) + sq.k0 * a.ldk + (int64_t)w.kv * a.D;
+    const T *v = static_cast<const T *>(a.v) + sq.k0 * a.ldv + (int64_t)w.kv * a.D;
+    auto last_of = [&](int row) {
+        return a.causal ? min(sq.lk - 1, a.group.of(row) + off) : sq.lk - 1;
+    };
+    const int w0 = m0 + 32 * wave, row = w0 + l32;
+    const int token = sq.q0 + a.group.of(row), g = row - (token - sq.q0) * a.G;
+    const int head = w.kv * a.G + g;
+    const int last = row < rows ? last_of(row) : -1;
+    const int wave_first = w0 < rows ? last_of(w0) : -1;
+    const int wave_last = w0 < rows ? last_of(min(w0 + 31, rows - 1)) : -1;
+    const int keys = last_of(min(m0 + kRows, rows) - 1) + 1;
+    const int tiles = keys > 0 ? (keys - 1) / KT + 1 : 0;
+
+    typename Ty::Frag q[NK], dout[NK];
+    const T *qrow = nullptr, *drow = nullptr, *orow = nullptr;
+    if (row < rows) {
+        const int64_t col = (int64_t)head * a.D;
+        qrow = static_cast<const T *>(a.q) + token * a.ldq + col;
+        drow = static_cast<const T *>(a.dout) + token * a.lddo + col;
+        orow = static_cast<const T *>(a.out) + token * a.ldo + col;
+    }
+    float delta = 0.0f, big = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) {
+        q[ks] = Ty::load8(qrow, 16 * ks + 8 * h, a.D);
+        dout[ks] = Ty::load8(drow, 16 * ks + 8 * h, a.D);
+        const typename Ty::Frag o = Ty::load8(orow, 16 * ks + 8 * h, a.D);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = Ty::get(dout[ks], j);
+            delta += d * Ty::get(o, j);
+            if constexpr (DT == kF16) big = fmaxf(big, fabsf(d));
+        }
+    }
+    delta += __shfl_xor(delta, 32);
+    if constexpr (DT == kF16) big = fmaxf(big, __shfl_xor(big, 32));
+    // A row of no key (its lse -inf): every probability 0.
+    float lse2 = INFINITY;
+    if (row < rows) {
+        const float x = a.lse[(int64_t)head * a.Tq + token];
+        lse2 = x == -INFINITY ? INFINITY : x * kLog2e;
+        if (x == -INFINITY) delta = 0.0f;
+        if (h == 0) {
+            const int64_t n = (int64_t)a.KV * a.Tq * a.G;
+            const int64_t at = (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G + row;
+            a.rows[at] = lse2;
+            a.rows[n + at] = delta;
+            if constexpr (DT == kF16) a.rows[2 * n + at] = big;
+        }
+    }
+    const int up = DT == kF16 ? (int)kUpDs - exponent_above(big) : 0;
+    const float from = lse2 - (float)up;
+
+    Mover<DT, DP, KT, 256, DMA> mk, mv;
+    auto load = [&](int t) {
+        T *to = lds + (t & 1) * 2 * Tl::kElems;
+        const int key0 = t * KT, left = sq.lk - key0;
+        mk.load(to, tid, left, a.D, [&](int r) { return k + min(key0 + r, sq.lk - 1) * a.ldk; });
+        mv.load(to + Tl::kElems, tid, left, a.D,
+                [&](int r) { return v + min(key0 + r, sq.lk - 1) * a.ldv; });
+    };
+    auto store = [&](int t) {
+        T *to = lds + (t & 1) * 2 * Tl::kElems;
+        mk.store(to, tid);
+        mv.store(to + Tl::kElems, tid);
+    };
+    f32x16 dq[NB];
+    clear(dq);
+    if (tiles > 0) {
+        load(0);
+        store(0);
+    }
+    for (int t = 0; t < tiles; ++t) {
+        if constexpr (DMA) landed();
+        else __syncthreads();
+        if (t + 1 < tiles) load(t + 1);
+        const int key0 = t * KT;
+        const T *kt = lds + (t & 1) * 2 * Tl::kElems, *vt = kt + Tl::kElems;
+        if (key0 <= wave_last) {
+            const bool whole = key0 + KT - 1 <= wave_first;
+            const bool plain = whole || Tl::finite(kt, lane);
+#pragma unroll
+            for (int b = 0; b < KT / 32; ++b) {
+                f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks)
+                    s = Ty::mfma(Tl::by_row(kt, 32 * b + l32, ks, h), q[ks], s);
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks)
+                    dp = Ty::mfma(Tl::by_row(vt, 32 * b + l32, ks, h), dout[ks], dp);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -from));
+                    s[r] = p * (dp[r] - delta);
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int key = key0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
+                        s[r] = key <= last ? s[r] : 0.0f;
+                    }
+                }
+                if (plain) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const typename Ty::Frag ds = Ty::pack(s, u);
+#pragma unroll
+                        for (int d = 0; d < NB; ++d)
+                            dq[d] = Ty::mfma(Tl::by_column(kt, 32 * b + 16 * u, 32 * d, lane), ds,
+                                             dq[d]);
+                    }
+                } else {
+                    add_careful<DT, DP, KT>(dq, s, kt, 32 * b, 0, last - key0 - 32 * b,
+                                            scratch[wave], lane);
+                }
+            }
+        }
+        if (t + 1 < tiles) store(t + 1);
+    }
+    if (row >= rows) return;
+    const float f = a.scale * pow2(-up);
+    T *p = static_cast<T *>(a.dq) + token * a.lddq + (int64_t)head * a.D;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int qd = 0; qd < 4; ++qd)
+            Ty::store4(p, 32 * b + 8 * qd + 4 * h, a.D,
+                       f32x4{dq[b][4 * qd] * f, dq[b][4 * qd + 1] * f, dq[b][4 * qd + 2] * f,
+                             dq[b][4 * qd + 3] * f},
+                       a.accumulate);
+}
+
+// dK and dV, kKeys keys a workgroup, 32 a wave (one a lane, both halves), over the rows
+// that see them: of all the group's heads, so the sum over a key head's queries is one
+// accumulator's.
+template <int DT>
+constexpr int rows_of() {
+    return DT == kF32 ? 32 : 64;
+}
+template <int DT, int DP, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
+att_bwd_kv(const Args a) {
+    using Ty = Type<DT>;
+    using T = typename Ty::T;
+    constexpr int RT = rows_of<DT>(), NB = DP / 32, NK = DP / 16;
+    constexpr float kUpV = DT == kF16 ? kUpP : 0.0f;
+    using Tl = Tile<DT, DP, RT>;
+    __shared__ __attribute__((aligned(16))) T lds[4 * Tl::kElems];
+    __shared__ __attribute__((aligned(16))) float stats[2][3][RT];
+    __shared__ float scratch[4][32 * 32];
+    const Work w(blockIdx.x, a.KV, a.kslots);
+    const Place pl = place_of(w.slot, a.n, [&](int s) {
+        return (int)min(a.ks[s], (uint32_t)a.Tk) / kKeys + s;
+    });
+    const Seq sq(a, pl.seq);
+    const int n0 = pl.tile * kKeys;
+    if (pl.tile < 0 || n0 >= sq.lk) return;  // (a slot of no tile)
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, l32 = lane & 31, off = sq.lk - sq.lq;
+    const float c = a.scale * kLog2e;
+    const int rows = sq.lq * a.G;
+    // The first row that sees a key.
+    auto first_of = [&](int key) { return a.causal ? max(0, key - off) * a.G : 0; };
+    const int kw = n0 + 32 * wave, key = kw + l32;
+    const int first = key < sq.lk ? first_of(key) : rows;
+    const int wave_first = kw < sq.lk ? first_of(kw) : rows;
+    const int wave_last = kw < sq.lk ? first_of(min(kw + 31, sq.lk - 1)) : rows;
+
+    typename Ty::Frag kf[NK], vf[NK];
+    const T *krow = nullptr, *vrow = nullptr;
+    if (key < sq.lk) {
+        krow = static_cast<const T *>(a.k) + (sq.k0 + key) * a.ldk + (int64_t)w.kv * a.D;
+        vrow = static_cast<const T *>(a.v) + (sq.k0 + key) * a.ldv + (int64_t)w.kv * a.D;
+    }
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) {
+        kf[ks] = Ty::load8(krow, 16 * ks + 8 * h, a.D);
+        vf[ks] = Ty::load8(vrow, 16 * ks + 8 * h, a.D);
+    }
+    Mover<DT, DP, RT, 256, DMA> mq, md;
+    const T *qb = static_cast<const T *>(a.q) + sq.q0 * a.ldq + (int64_t)w.kv * a.G * a.D;
+    const T *db = static_cast<const T *>(a.dout) + sq.q0 * a.lddo + (int64_t)w.kv * a.G * a.D;
+    const int64_t n = (int64_t)a.KV * a.Tq * a.G;
+    const float *rs = a.rows + (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G;
+    float sv = 0.0f;
+    auto load = [&](int t) {
+        T *to = lds + (t & 1) * 2 * Tl::kElems;
+        const int r0 = t * RT, left = rows - r0;
+        auto at = [&](const T *base, int64_t ld, int r) {
+            const int x = min(r0 + r, rows - 1), i = a.group.of(x);
+            return base + i * ld + (int64_t)(x - i * a.G) * a.D;
+        };
+        mq.load(to, tid, left, a.D, [&](int r) { return at(qb, a.ldq, r); });
+        md.load(to + Tl::kElems, tid, left, a.D, [&](int r) { return at(db, a.lddo, r); });
+        const int what = tid / RT, r = tid % RT;
+        if (what < (DT == kF16 ? 3 : 2)) {
+            // (Rows past the last: probability 0.)
+            sv = r < left ? rs[what * n + r0 + r] : what == 0 ? INFINITY : 0.0f;
+        }
+    };
+    auto store = [&](int t) {
+        T *to = lds + (t & 1) * 2 * Tl::kElems;
+        mq.store(to, tid);
+        md.store(to + Tl::kElems, tid);
+        const int what = tid / RT;
+        if (what < (DT == kF16 ? 3 : 2)) stats[t & 1][what][tid % RT] = sv;
+    };
+    f32x16 dk[NB], dv[NB];
+    clear(dk);
+    clear(dv);
+    int up = 0;  // fp16: the power of two that dK carries
+    bool any = false;
+    const int t0 = first_of(n0) / RT, t1 = rows > 0 ? (rows - 1) / RT + 1 : 0;
+    if (t0 < t1) {
+        load(t0);
+        store(t0);
+    }
+    for (int t = t0; t < t1; ++t) {
+        if constexpr (DMA) landed();
+        else __syncthreads();
+        if (t + 1 < t1) load(t + 1);
+        const int r0 = t * RT;
+        const T *qt = lds + (t & 1) * 2 * Tl::kElems, *dt = qt + Tl::kElems;
+        const float *st = stats[t & 1][0];
+        if (r0 + RT > wave_first) {
+            const bool whole = r0 >= wave_last && r0 + RT <= rows;
+            const bool plain = whole || (Tl::finite(qt, lane) && Tl::finite(dt, lane));
+            float fs = 1.0f;
+            if constexpr (DT == kF16) {
+                float big = st[2 * RT + lane];
+#pragma unroll
+                for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o));
+                const int e = __builtin_amdgcn_readfirstlane((int)kUpDs - exponent_above(big));
+                if (!any || e < up) {
+                    if (any) {
+                        const float f = pow2(e - up);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) dk[b][r] *= f;
+                    }
+                    up = e;
+                    any = true;
+                }
+                fs = pow2(up - (int)kUpP);
+            }
+#pragma unroll
+            for (int b = 0; b < RT / 32; ++b) {
+                f32x16 p = zero16(), dp = zero16();
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks)
+                    p = Ty::mfma(Tl::by_row(qt, 32 * b + l32, ks, h), kf[ks], p);
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks)
+                    dp = Ty::mfma(Tl::by_row(dt, 32 * b + l32, ks, h), vf[ks], dp);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int at = 32 * b + 8 * q + 4 * h;
+                    const f32x4 lse = *reinterpret_cast<const f32x4 *>(st + at);
+                    const f32x4 delta = *reinterpret_cast<const f32x4 *>(st + RT + at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = 4 * q + e;
+                        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], c, kUpV - lse[e]));
+                        dp[r] = p[r] * (DT == kF16 ? (dp[r] - delta[e]) * fs : dp[r] - delta[e]);
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int x = r0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
+                        const bool on = x >= first && x < rows;
+                        p[r] = on ? p[r] : 0.0f;
+                        dp[r] = on ? dp[r] : 0.0f;
+                    }
+                }
+                if (plain) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const typename Ty::Frag pf = Ty::pack(p, u);
+#pragma unroll
+                        for (int d = 0; d < NB; ++d)
+                            dv[d] = Ty::mfma(Tl::by_column(dt, 32 * b + 16 * u, 32 * d, lane), pf,
+                                             dv[d]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const typename Ty::Frag ds = Ty::pack(dp, u);
+#pragma unroll
+                        for (int d = 0; d < NB; ++d)
+                            dk[d] = Ty::mfma(Tl::by_column(qt, 32 * b + 16 * u, 32 * d, lane), ds,
+                                             dk[d]);
+                    }
+                } else {
+                    const int lo = first - r0 - 32 * b, hi = rows - 1 - r0 - 32 * b;
+                    add_careful<DT, DP, RT>(dv, p, dt, 32 * b, lo, hi, scratch[wave], lane);
+                    add_careful<DT, DP, RT>(dk, dp, qt, 32 * b, lo, hi, scratch[wave], lane);
+                }
+            }
+        }
+        if (t + 1 < t1) store(t + 1);
+    }
+    if (key >= sq.lk) return;
+    const float fk = a.scale * pow2(-up), fv = pow2(-(int)kUpV);
+    const int64_t col = (int64_t)w.kv * a.D;
+    T *pk = static_cast<T *>(a.dk) + (sq.k0 + key) * a.lddk + col;
+    T *pv = static_cast<T *>(a.dv) + (sq.k0 + key) * a.lddv + col;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int d = 32 * b + 8 * q + 4 * h;
+            Ty::store4(pk, d, a.D,
+                       f32x4{dk[b][4 * q] * fk, dk[b][4 * q + 1] * fk, dk[b][4 * q + 2] * fk,
+                             dk[b][4 * q + 3] * fk},
+                       a.accumulate);
+            Ty::store4(pv, d, a.D,
+                       f32x4{dv[b][4 * q] * fv, dv[b][4 * q + 1] * fv, dv[b][4 * q + 2] * fv,
+                             dv[b][4 * q + 3] * fv},
+                       a.accumulate);
+        }
+}
+
+// ------------------------------------------------------------------ launches
+template <int DT, class F>
+void with_width(int D, bool dma, F f) {
+    using std::integral_constant;
+    constexpr bool kDma = DT != kF32;
+    auto with = [&](auto dp) {
+        if (kDma && dma) f(dp, std::integral_constant<bool, kDma>{});
+        else f(dp, std::false_type{});
+    };
+    if (D <= 64) with(integral_constant<int, 64>{});
+    else with(integral_constant<int, 128>{});
+}
+
+template <int DT>
+int forward(hipStream_t st, const Args &a, bool few, bool dma) {
+    const dim3 grid(a.KV * a.slots, a.splits);
+    with_width<DT>(a.D, dma, [&](auto dp, auto d) {
+        if (few) att_fwd_few<DT, dp(), d()><<<grid, 256, 0, st>>>(a);
+        else att_fwd<DT, dp(), d()><<<grid, 256, 0, st>>>(a);
+    });
+    return (int)hipGetLastError();
+}
+template <int DT>
+int combine(hipStream_t st, const Args &a) {
+    att_combine<DT><<<((int64_t)a.KV * a.Tq * a.G - 1) / 4 + 1, 256, 0, st>>>(a);
+    return (int)hipGetLastError();
+}
+template <int DT>
+int backward(hipStream_t st, const Args &a, bool dma) {
+    with_width<DT>(a.D, dma, [&](auto dp, auto d) {
+        att_bwd_q<DT, dp(), d()><<<a.KV * a.slots, 256, 0, st>>>(a);
+        if (a.kslots) att_bwd_kv<DT, dp(), d()><<<a.KV * a.kslots, 256, 0, st>>>(a);
+    });
+    return (int)hipGetLastError();
+}
+
+}  // namespace attn
+}  // namespace fg

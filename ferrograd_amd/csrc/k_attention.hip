@@ -1,0 +1,202 @@
+// k_attention.hip -- entry points of attention over packed sequences with grouped
+// heads, for prompts, single tokens over a cache, and training.  The kernels, and the
+// mathematics, are in fg_attention_kernel.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "fg_attention.h"
+#include "fg_half.h"
+#include "fg_internal.h"
+#include "fg_rows.h"
+
+namespace {
+
+using fg::attn::Args;
+using fg::rows::apart;
+
+constexpr int kMaxD = 128;      // columns of a head
+constexpr int kMaxSplits = 32;  // of a row's keys
+
+// Few rows a sequence (single tokens): the kernel whose waves share out the keys.
+bool few_rows(const Args &a) { return (int64_t)a.Tq * a.G <= (int64_t)a.n * fg::attn::kFewRows; }
+
+// Splits of each sequence's keys, from what the host knows: workgroups for every CU,
+// and no fewer than 512 keys each of a sequence of average length.
+int splits_of(int cus, const Args &a, bool few) {
+    const int per = few ? fg::attn::kFewRows : fg::attn::kRows;
+    const int64_t tiles = std::max<int64_t>(a.n, ((int64_t)a.Tq * a.G + per - 1) / per) * a.KV;
+    const int64_t want = (few ? 8 : 2) * (int64_t)cus / std::max<int64_t>(tiles, 1);
+    const int64_t most = (int64_t)a.Tk / a.n / 512;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
+}
+
+bool whole_chunks(const Args &a, std::initializer_list<std::pair<const void *, int64_t>> rows) {
+    if (a.D != 64 && a.D != 128) return false;
+    for (const auto &r : rows)
+        if (((uintptr_t)r.first & 15) || r.second % 8) return false;
+    return true;
+}
+
+// What both directions ask of their arguments.
+int check(const char *who, int dtype, const Args &a, int heads, int kv_heads) {
+    FG_REQUIRE(dtype >= FG_DTYPE_F32 && dtype <= FG_DTYPE_BF16, FG_ERR_INVALID_ARGUMENT,
+               "%s: bad dtype %d", who, dtype);
+    FG_REQUIRE(a.n >= 0 && a.Tq >= 0 && a.Tk >= 0 && heads > 0 && kv_heads > 0 && a.D > 0,
+               FG_ERR_SHAPE, "%s: bad shape n=%d Tq=%d Tk=%d heads=%d kv_heads=%d D=%d", who, a.n,
+               a.Tq, a.Tk, heads, kv_heads, a.D);
+    FG_REQUIRE(heads % kv_heads == 0, FG_ERR_SHAPE, "%s: %d heads are no multiple of %d key heads",
+               who, heads, kv_heads);
+    FG_REQUIRE(a.D <= kMaxD, FG_ERR_UNSUPPORTED, "%s: heads of %d columns, at most %d", who, a.D,
+               kMaxD);
+    const int64_t wide = (int64_t)heads * a.D, kv_wide = (int64_t)kv_heads * a.D;
+    FG_REQUIRE(wide < INT32_MAX && a.ldq >= wide && a.ldk >= kv_wide && a.ldv >= kv_wide,
+               FG_ERR_SHAPE, "%s: ldq=%lld, ldk=%lld or ldv=%lld too small for %d and %d heads", who,
+               (long long)a.ldq, (long long)a.ldk, (long long)a.ldv, heads, kv_heads);
+    FG_REQUIRE(a.scale > 0.0f && a.scale < INFINITY, FG_ERR_INVALID_ARGUMENT,
+               "%s: scale must be positive and finite", who);
+    // Rows of a key head are counted in 32 bits, and a grid holds the slots.
+    const int64_t slots = (int64_t)a.Tq * (heads / kv_heads) / fg::attn::kFewRows + a.n;
+    const int64_t kslots = (int64_t)a.Tk / fg::attn::kKeys + a.n;
+    FG_REQUIRE((int64_t)a.Tq * (heads / kv_heads) < INT32_MAX - 256 && a.Tk < INT32_MAX - 256 &&
+                   fg::rows::grid_holds(kv_heads * std::max(slots, kslots), 256),
+               FG_ERR_OUT_OF_BOUNDS, "%s: %d sequences of %d rows and %d keys with %d heads", who,
+               a.n, a.Tq, a.Tk, heads);
+    return FG_OK;
+}
+
+}  // namespace
+
+namespace fg {
+uint64_t attention_bwd_ws_bytes(int Tq, int heads) {
+    return 3 * (uint64_t)std::max(Tq, 1) * (uint64_t)heads * sizeof(float);
+}
+}  // namespace fg
+
+FG_API int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k, int ldk,
+                        const void *d_v, int ldv, const uint32_t *d_q_starts,
+                        const uint32_t *d_k_starts, const uint32_t *d_k_lens, int n, int Tq, int Tk,
+                        int heads, int kv_heads, int D, float scale, int causal, void *d_out,
+                        int ldo, float *d_lse) {
+    const char *who = "fg_attention";
+    Args a{};
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.qs = d_q_starts;
+    a.ks = d_k_starts;
+    a.klens = d_k_lens;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.n = n;
+    a.Tq = Tq;
+    a.Tk = Tk;
+    a.D = D;
+    a.scale = scale;
+    if (int rc = check(who, dtype, a, heads, kv_heads)) return rc;
+    a.KV = kv_heads;
+    a.G = heads / kv_heads;
+    a.group = fg::attn::Div((uint32_t)a.G);
+    a.causal = causal != 0;
+    a.out = d_out;
+    a.ldo = ldo;
+    a.lse = d_lse;
+    FG_REQUIRE(ldo >= heads * D, FG_ERR_SHAPE, "%s: ldo=%d < %d heads of %d", who, ldo, heads, D);
+    FG_REQUIRE(d_q && d_k && d_v && d_q_starts && d_k_starts && d_out, FG_ERR_INVALID_ARGUMENT,
+               "%s: q, k, v, the starts and out are required", who);
+    FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    FG_REQUIRE(apart(d_out, {d_q, d_k, d_v, d_q_starts, d_k_starts, d_k_lens, d_lse}) &&
+                   apart(d_lse, {d_q, d_k, d_v, d_q_starts, d_k_starts, d_k_lens}),
+               FG_ERR_INVALID_ARGUMENT, "%s: an output is another output or an input", who);
+    if (n == 0 || Tq == 0) return FG_OK;
+    FG_HIP(hipSetDevice(ctx->device));
+    const bool few = few_rows(a);
+    a.splits = splits_of(ctx->cu_count, a, few);
+    const int64_t rows = (int64_t)Tq * heads;
+    if (a.splits > 1) {
+        a.part = (float *)fg::workspace(ctx, (uint64_t)a.splits * rows * (D + 2) * sizeof(float));
+        if (!a.part) return FG_ERR_OUT_OF_MEMORY;
+    }
+    a.slots = (int)((int64_t)Tq * a.G / (few ? fg::attn::kFewRows : fg::attn::kRows) + n);
+    const bool dma = whole_chunks(a, {{d_k, ldk}, {d_v, ldv}});
+    auto launch = dtype == FG_DTYPE_F32    ? fg::attn::forward<fg::kF32>
+                  : dtype == FG_DTYPE_BF16 ? fg::attn::forward<fg::kBF16>
+                                           : fg::attn::forward<fg::kF16>;
+    FG_HIP((hipError_t)launch(ctx->stream, a, few, dma));
+    if (a.splits > 1) {
+        auto join = dtype == FG_DTYPE_F32    ? fg::attn::combine<fg::kF32>
+                    : dtype == FG_DTYPE_BF16 ? fg::attn::combine<fg::kBF16>
+                                             : fg::attn::combine<fg::kF16>;
+        FG_HIP((hipError_t)join(ctx->stream, a));
+    }
+    return FG_OK;
+}
+
+FG_API int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k,
+                            int ldk, const void *d_v, int ldv, const void *d_out, int ldo,
+                            const void *d_dout, int lddo, const float *d_lse,
+                            const uint32_t *d_q_starts, const uint32_t *d_k_starts, int n, int Tq,
+                            int Tk, int heads, int kv_heads, int D, float scale, int causal,
+                            void *d_dq, int lddq, void *d_dk, int lddk, void *d_dv, int lddv,
+                            int accumulate) {
+    const char *who = "fg_attention_bwd";
+    Args a{};
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.qs = d_q_starts;
+    a.ks = d_k_starts;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.n = n;
+    a.Tq = Tq;
+    a.Tk = Tk;
+    a.D = D;
+    a.scale = scale;
+    if (int rc = check(who, dtype, a, heads, kv_heads)) return rc;
+    a.KV = kv_heads;
+    a.G = heads / kv_heads;
+    a.group = fg::attn::Div((uint32_t)a.G);
+    a.causal = causal != 0;
+    a.out = const_cast<void *>(d_out);
+    a.ldo = ldo;
+    a.lse = const_cast<float *>(d_lse);
+    a.dout = d_dout;
+    a.lddo = lddo;
+    a.dq = d_dq;
+    a.lddq = lddq;
+    a.dk = d_dk;
+    a.lddk = lddk;
+    a.dv = d_dv;
+    a.lddv = lddv;
+    a.accumulate = accumulate != 0;
+    FG_REQUIRE(ldo >= heads * D && lddo >= heads * D && lddq >= heads * D, FG_ERR_SHAPE,
+               "%s: ldo=%d, lddo=%d or lddq=%d < %d heads of %d", who, ldo, lddo, lddq, heads, D);
+    FG_REQUIRE(lddk >= kv_heads * D && lddv >= kv_heads * D, FG_ERR_SHAPE,
+               "%s: lddk=%d or lddv=%d < %d heads of %d", who, lddk, lddv, kv_heads, D);
+    FG_REQUIRE(d_q && d_k && d_v && d_out && d_dout && d_lse && d_q_starts && d_k_starts,
+               FG_ERR_INVALID_ARGUMENT, "%s: q, k, v, out, dout, lse and the starts are required",
+               who);
+    FG_REQUIRE(d_dq && d_dk && d_dv, FG_ERR_INVALID_ARGUMENT, "%s: dq, dk and dv are required", who);
+    FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
+    for (const void *o : {(const void *)d_dq, (const void *)d_dk, (const void *)d_dv})
+        FG_REQUIRE(apart(o, {d_q, d_k, d_v, d_out, d_dout, d_lse, d_q_starts, d_k_starts}),
+                   FG_ERR_INVALID_ARGUMENT, "%s: an output is an input", who);
+    FG_REQUIRE(d_dq != d_dk && d_dq != d_dv && d_dk != d_dv, FG_ERR_INVALID_ARGUMENT,
+               "%s: an output is another output", who);
+    if (n == 0 || (Tq == 0 && Tk == 0)) return FG_OK;
+    FG_HIP(hipSetDevice(ctx->device));
+    a.rows = (float *)fg::workspace(ctx, fg::attention_bwd_ws_bytes(Tq, heads));
+    if (!a.rows) return FG_ERR_OUT_OF_MEMORY;
+    a.splits = 1;
+    a.slots = (int)((int64_t)Tq * a.G / fg::attn::kRows + n);
+    a.kslots = Tk / fg::attn::kKeys + n;
+    const bool dma = whole_chunks(a, {{d_q, ldq}, {d_k, ldk}, {d_v, ldv}, {d_dout, lddo}});
+    auto launch = dtype == FG_DTYPE_F32    ? fg::attn::backward<fg::kF32>
+                  : dtype == FG_DTYPE_BF16 ? fg::attn::backward<fg::kBF16>
+                                           : fg::attn::backward<fg::kF16>;
+    FG_HIP((hipError_t)launch(ctx->stream, a, dma));
+    return FG_OK;
+}

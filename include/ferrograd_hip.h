@@ -364,6 +364,39 @@ int fg_rms_norm_bwd(fg_ctx *ctx, int dtype, const void *d_s, int lds, const void
                     const void *d_gamma, const float *d_rstd, int R, int C, const void *d_ds,
                     int ldds, void *d_dx, int lddx, void *d_dgamma, int dgamma_accumulate);
 
+/* Attention over packed sequences (no reference counterpart).  n sequences: s has
+ * the rows q_starts[s] .. q_starts[s + 1] - 1 of q and out, and the rows from
+ * k_starts[s] on of k and v, up to k_starts[s + 1] or, with d_k_lens (a cache with
+ * room), k_lens[s] of them.  (The starts are n + 1 numbers that do not fall, at most Tq
+ * and Tk; what lies past those is not read.)  q and out are Tq x (heads D), k and v
+ * Tk x (kv_heads D) matrices of element type dtype; query head h, columns h D on, reads
+ * key head h / (heads / kv_heads).  For query i of lq and key j of lk:
+ *   S = scale * q_i . k_j, visible if not causal or j <= i + lk - lq
+ *   out_i = sum over visible j of softmax(S)_j v_j ;  lse = log sum exp(S)
+ * Products and statistics are fp32, probabilities rounded to dtype for the second
+ * product, out rounded once.  d_lse [heads][Tq] (fp32, what the backward needs) may be
+ * NULL.  A row that sees no key is 0, its lse -inf.  Values of keys that a row does not
+ * see do not reach it, infinities and NaN included.  Rows of no sequence are left as
+ * they are.  1 <= D <= 128, scale > 0.  Where rows are few and keys many, the keys'
+ * splits go to the workspace: D + 2 floats for each of at most 32 a row and head. */
+int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k, int ldk,
+                 const void *d_v, int ldv, const uint32_t *d_q_starts, const uint32_t *d_k_starts,
+                 const uint32_t *d_k_lens, int n, int Tq, int Tk, int heads, int kv_heads, int D,
+                 float scale, int causal, void *d_out, int ldo, float *d_lse);
+/* Its backward from out, dout and lse (without k_lens), P = exp(S - lse):
+ *   delta = dout_i . out_i ;  dS = P * (dout_i . v_j - delta)
+ *   dq (=|+=) scale * dS k ;  dk (=|+=) scale * dS^T q ;  dv (=|+=) P^T dout
+ * dk and dv are sums over the group's heads.  P and dS are rounded to dtype for their
+ * products, outputs once; no atomics, the order of every sum is fixed.  Rows of dq, and
+ * of dk and dv, of no sequence are left as they are.  The workspace takes 12 bytes a row
+ * and head. */
+int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k, int ldk,
+                     const void *d_v, int ldv, const void *d_out, int ldo, const void *d_dout,
+                     int lddo, const float *d_lse, const uint32_t *d_q_starts,
+                     const uint32_t *d_k_starts, int n, int Tq, int Tk, int heads, int kv_heads,
+                     int D, float scale, int causal, void *d_dq, int lddq, void *d_dk, int lddk,
+                     void *d_dv, int lddv, int accumulate);
+
 /* Log probabilities of given tokens (no reference counterpart; the answers next to
  * fg_softmax_ce's loss).  Per row r of R rows of C logits, z = scale * logits:
  *   lse[r] = log sum exp(z) ;  logp[r] = z[tokens[r]] - lse[r]
