@@ -170,6 +170,30 @@ struct Type {
 };
 
 // ------------------------------------------------------------------ LDS tiles
+// A lane's places in tiles of rows of DP elements, computed once: what the swizzle makes
+// of the low bits of a chunk; everything else of an address is a constant.
+template <int DT, int DP>
+struct Lanes {
+    static constexpr bool kWide = DT == kF32;
+    int row[4], col[4], lane;
+    __device__ __forceinline__ explicit Lanes(int lane_) : lane(lane_) {
+        const int h = lane >> 5, l32 = lane & 31;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (kWide) {
+                row[i] = l32 * DP + (((4 * (i >> 1) + 2 * h + (i & 1)) ^ swz(l32)) * 4);
+                col[i] = (4 * h + i) * DP + (((l32 >> 2) ^ swz(4 * h + i)) * 4) + (l32 & 3);
+            } else {
+                const int e = (lane >> 2) & 3, q = lane & 3;
+                row[i] = l32 * DP + (((2 * i + h) ^ swz(l32)) * 8);
+                col[i] = (4 * h + e) * DP +
+                         (((4 * (i & 1) + 2 * ((lane >> 4) & 1) + (q >> 1)) ^ swz(4 * h + e)) * 8) +
+                         4 * (q & 1);
+            }
+        }
+    }
+};
+
 // ROWS rows of DP elements.
 template <int DT, int DP, int ROWS>
 struct Tile {
@@ -180,44 +204,40 @@ struct Tile {
     static constexpr int kElems = ROWS * DP;
     static constexpr int kChunks = ROWS * CH;
 
-    static __device__ __forceinline__ const T *at(const T *t, int row, int chunk) {
-        return t + row * DP + ((chunk ^ swz(row)) * E);
-    }
-    // Row `row`, elements 16 ks + 8 h .. + 7: an operand with the tile's rows in lanes.
-    static __device__ __forceinline__ Frag by_row(const T *t, int row, int ks, int h) {
+    // Rows 32 b + lane % 32, elements 16 ks + 8 h .. + 7: an operand with the tile's rows in
+    // lanes.
+    static __device__ __forceinline__ Frag by_row(const T *t, int b, int ks,
+                                                  const Lanes<DT, DP> &L) {
+        t += 32 * b * DP;
         if constexpr (Ty::kWide) {
             Frag f;
-            const int c = 4 * ks + 2 * h;
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(at(t, row, c));
-            const f32x4 y = *reinterpret_cast<const f32x4 *>(at(t, row, c + 1));
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(t + L.row[2 * (ks & 1)] + 32 * (ks >> 1));
+            const f32x4 y =
+                *reinterpret_cast<const f32x4 *>(t + L.row[2 * (ks & 1) + 1] + 32 * (ks >> 1));
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = j < 4 ? x[j & 3] : y[j & 3];
             return f;
         } else {
-            return *reinterpret_cast<const u32x4 *>(at(t, row, 2 * ks + h));
+            return *reinterpret_cast<const u32x4 *>(t + L.row[ks & 3] + 64 * (ks >> 2));
         }
     }
-    // Column d0 + lane % 32, rows r0 + 4 h + 0..3 and r0 + 8 + 4 h + 0..3: an operand
-    // with the tile's columns in lanes.  16 bits: two transposing reads, in which source
-    // lane 4 e + q of each 16 reads 4 elements of row e, and lane l gets column l's rows.
-    static __device__ __forceinline__ Frag by_column(const T *t, int r0, int d0, int lane) {
-        const int h = lane >> 5;
+    // Columns 32 d + lane % 32, rows r0 + 4 h + 0..3 and r0 + 8 + 4 h + 0..3 (r0 a multiple
+    // of 16): an operand with the tile's columns in lanes.  16 bits: two transposing reads,
+    // in which source lane 4 e + q of each 16 reads 4 elements of row e, and lane l gets
+    // column l's rows.
+    static __device__ __forceinline__ Frag by_column(const T *t, int r0, int d,
+                                                     const Lanes<DT, DP> &L) {
+        t += r0 * DP;
         Frag f;
         if constexpr (Ty::kWide) {
-            const int d = d0 + (lane & 31);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int row = r0 + 8 * (j >> 2) + 4 * h + (j & 3);
-                f[j] = at(t, row, d >> 2)[d & 3];
-            }
+            for (int j = 0; j < 8; ++j) f[j] = t[L.col[j & 3] + 8 * (j >> 2) * DP + 32 * d];
         } else {
-            const int e = (lane >> 2) & 3, q = lane & 3;
-            const int d = d0 + (lane & 16) + 4 * q;
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int row = r0 + 8 * half + 4 * h + e;
                 const v4i16 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) v4i16 *)(at(t, row, d >> 3) + (d & 7)));
+                    (__attribute__((address_space(3))) v4i16 *)(t + L.col[d & 1] + 64 * (d >> 1) +
+                                                               8 * half * DP));
                 const u32x2 w = __builtin_bit_cast(u32x2, v);
                 f[2 * half] = w[0];
                 f[2 * half + 1] = w[1];
@@ -356,37 +376,36 @@ struct Work {
     }
 };
 
-// acc[b] (columns in lanes, rows d in registers) += sum over the 32 rows k of a tile
-// from r0 on of tile[r0 + k][d] * w[k], only those with lo <= k <= hi of the lane: what
-// the MFMA does where masked rows hold infinities or NaN, which 0 times is NaN.
-// scratch: 32 x 32 floats of the wave.
-template <int DT, int DP, int ROWS, int NB>
-__device__ __forceinline__ void add_careful(f32x16 (&acc)[NB], const f32x16 &w, const void *tile,
-                                            int r0, int lo, int hi, float *scratch, int lane) {
-    using Tl = Tile<DT, DP, ROWS>;
-    using T = typename Tl::T;
-    const T *t = static_cast<const T *>(tile);
-    const int h = lane >> 5, l32 = lane & 31;
-    __builtin_amdgcn_wave_barrier();
+// Where a tile in which not every key is visible to every row holds an infinity or NaN,
+// the matrix instructions would bring it, times 0, to rows that do not see it.  A
+// workgroup that meets such a tile does its work over, a wave an output row, lanes over
+// 64 of the summed index and then over the row's columns, what is not visible left out.
+// Sum over a row's D columns of x y, x the wave's row, y the lane's (lanes that are on).
+template <int DT>
+__device__ __forceinline__ float dot(const typename Type<DT>::T *x, const typename Type<DT>::T *y,
+                                     int D, bool on) {
+    float s = 0.0f;
+    if (on)
+        for (int d = 0; d < D; ++d) s += Type<DT>::load1(x + d) * Type<DT>::load1(y + d);
+    return s;
+}
+// acc[i] (column lane + 64 i) += w times the row's.
+template <int DT>
+__device__ __forceinline__ void add_row(float (&acc)[2], float w, const typename Type<DT>::T *row,
+                                        int D, int lane) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) scratch[(8 * (r >> 2) + 4 * h + (r & 3)) * 32 + l32] = w[r];
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-    for (int k = 0; k < 32; ++k) {
-        const float x = scratch[k * 32 + l32];
-        const bool on = k >= lo && k <= hi;
+    for (int i = 0; i < 2; ++i)
+        if (lane + 64 * i < D) acc[i] += w * Type<DT>::load1(row + lane + 64 * i);
+}
+template <int DT>
+__device__ __forceinline__ void put_row(typename Type<DT>::T *row, const float (&acc)[2], float f,
+                                        int D, int lane, bool add) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int d = 32 * b + 8 * q + 4 * h;
-                const T *p = Tl::at(t, r0 + k, d / Tl::E) + d % Tl::E;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    acc[b][4 * q + e] += on ? x * Type<DT>::load1(p + e) : 0.0f;
-            }
+    for (int i = 0; i < 2; ++i) {
+        const int d = lane + 64 * i;
+        if (d < D)
+            Type<DT>::store1(row + d, acc[i] * f + (add ? Type<DT>::load1(row + d) : 0.0f));
     }
-    __builtin_amdgcn_wave_barrier();
 }
 
 template <int NB>
@@ -419,12 +438,13 @@ struct Rows {
     typename Ty::Frag q[NK];
     f32x16 o[NB];
     float m = -INFINITY, l = 0.0f;
+    bool bad = false;  // a tile of keys not all visible held an infinity or NaN
 
     // Keys key0 .. key0 + KT - 1 in tiles k and v, up to `last` for the lane's row; whole:
     // every one is visible to every row of the wave.
     __device__ __forceinline__ void step(const T *k, const T *v, int key0, int last, bool whole,
-                                         float c, float *scratch, int lane) {
-        const int h = lane >> 5, l32 = lane & 31;
+                                         float c, const Lanes<DT, DP> &L) {
+        const int h = L.lane >> 5;
         constexpr int KB = KT / 32;
         f32x16 s[KB];
 #pragma unroll
@@ -432,7 +452,7 @@ struct Rows {
             s[b] = zero16();
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks)
-                s[b] = Ty::mfma(Tl::by_row(k, 32 * b + l32, ks, h), q[ks], s[b]);
+                s[b] = Ty::mfma(Tl::by_row(k, b, ks, L), q[ks], s[b]);
         }
         if (!whole) {
 #pragma unroll
@@ -469,12 +489,7 @@ struct Rows {
                 part[r & 3] += s[b][r];
             }
         l += (part[0] + part[1]) + (part[2] + part[3]);
-        if (!whole && !Tl::finite(v, lane)) {
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-                add_careful<DT, DP, KT>(o, s[b], v, 32 * b, 0, last - key0 - 32 * b, scratch, lane);
-            return;
-        }
+        if (!whole) bad |= !Tl::finite(v, L.lane);
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -482,7 +497,7 @@ struct Rows {
                 const typename Ty::Frag p = Ty::pack(s[b], u);
 #pragma unroll
                 for (int d = 0; d < NB; ++d)
-                    o[d] = Ty::mfma(Tl::by_column(v, 32 * b + 16 * u, 32 * d, lane), p, o[d]);
+                    o[d] = Ty::mfma(Tl::by_column(v, 32 * b + 16 * u, d, L), p, o[d]);
             }
     }
 };
@@ -531,6 +546,66 @@ __device__ __forceinline__ void write_row(const Args &a, int kv, int split, int 
             l == 0.0f ? -INFINITY : (m * c + (__log2f(l) - kUp)) * kLn2;
 }
 
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Rows row0 .. row1 - 1 of a sequence over its keys key0 .. key1 - 1, carefully.
+template <int DT>
+__device__ void careful_fwd(const Args &a, const Seq &sq, int kv, int split, int row0, int row1,
+                            int key0, int key1, int wave, int lane) {
+    using T = typename Type<DT>::T;
+    constexpr float kUp = Rows<DT, 32, 32>::kUp;
+    const float c = a.scale * kLog2e;
+    const T *k = static_cast<const T *>(a.k) + sq.k0 * a.ldk + (int64_t)kv * a.D;
+    const T *v = static_cast<const T *>(a.v) + sq.k0 * a.ldv + (int64_t)kv * a.D;
+    for (int row = row0 + wave; row < row1; row += 4) {
+        const int i = a.group.of(row), head = kv * a.G + row - i * a.G, token = sq.q0 + i;
+        const int end = min(min(key1, sq.lk), a.causal ? i + sq.lk - sq.lq + 1 : sq.lk);
+        const T *q = static_cast<const T *>(a.q) + token * a.ldq + (int64_t)head * a.D;
+        float m = -INFINITY, l = 0.0f, acc[2] = {0.0f, 0.0f};
+        for (int j0 = key0; j0 < end; j0 += 64) {
+            const int j = j0 + lane;
+            const float x = dot<DT>(q, k + j * a.ldk, a.D, j < end);
+            const float to = fmaxf(m, wave_max(j < end ? x : -INFINITY));
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - to) * c);
+            m = to;
+            const float from = (m == -INFINITY ? 0.0f : m * c) - kUp;
+            const float p =
+                j < end ? __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -from)) : 0.0f;
+            l = (l == 0.0f ? 0.0f : l * f) + wave_add(p);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) acc[e] = acc[e] == 0.0f ? 0.0f : acc[e] * f;
+            for (int n = 0; n < min(64, end - j0); ++n)
+                add_row<DT>(acc, __shfl(p, n), v + (j0 + n) * a.ldv, a.D, lane);
+        }
+        if (a.splits > 1) {
+            const int64_t rows = (int64_t)a.KV * a.Tq * a.G;
+            const int64_t at =
+                (int64_t)split * rows + (int64_t)kv * a.Tq * a.G + sq.q0 * a.G + row;
+            if (lane == 0) {
+                float *ml = a.part + a.splits * rows * a.D + 2 * at;
+                ml[0] = m;
+                ml[1] = l;
+            }
+            put_row<kF32>(a.part + at * a.D, acc, 1.0f, a.D, lane, false);
+            continue;
+        }
+        put_row<DT>(static_cast<T *>(a.out) + token * a.ldo + (int64_t)head * a.D, acc,
+                    l == 0.0f ? 0.0f : 1.0f / l, a.D, lane, false);
+        if (a.lse && lane == 0)
+            a.lse[(int64_t)head * a.Tq + token] =
+                l == 0.0f ? -INFINITY : (m * c + (__log2f(l) - kUp)) * kLn2;
+    }
+}
+
 // Four waves of 32 rows, the same keys for all: K and V tiles of KT keys, two stages.
 template <int DT>
 constexpr int keys_of() {
@@ -545,7 +620,6 @@ att_fwd(const Args a) {
     constexpr int KT = keys_of<DT>();
     using Tl = Tile<DT, DP, KT>;
     __shared__ __attribute__((aligned(16))) T lds[4 * Tl::kElems];
-    __shared__ float scratch[4][32 * 32];
     const Work w(blockIdx.x, a.KV, a.slots);
     const Place pl = place_of(a.slots - 1 - w.slot, a.n, [&](int s) {
         return (int)min(a.qs[s], (uint32_t)a.Tq) * a.G / kRows + s;
@@ -572,6 +646,7 @@ att_fwd(const Args a) {
     const int t0 = (int)((int64_t)tiles * blockIdx.y / a.splits);
     const int t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / a.splits);
 
+    const Lanes<DT, DP> L(lane);
     Rows<DT, DP, KT> st;
     const T *qrow = row < rows ? static_cast<const T *>(a.q) + token * a.ldq +
                                      (int64_t)(w.kv * a.G + g) * a.D
@@ -605,9 +680,13 @@ att_fwd(const Args a) {
         const int key0 = t * KT;
         const T *at = lds + (t & 1) * 2 * Tl::kElems;
         if (key0 <= wave_last)
-            st.step(at, at + Tl::kElems, key0, last, key0 + KT - 1 <= wave_first, c, scratch[wave],
-                    lane);
+            st.step(at, at + Tl::kElems, key0, last, key0 + KT - 1 <= wave_first, c, L);
         if (t + 1 < t1) store(t + 1);
+    }
+    if (__syncthreads_or(st.bad)) {
+        careful_fwd<DT>(a, sq, w.kv, blockIdx.y, m0, min(m0 + kRows, rows), t0 * KT, t1 * KT, wave,
+                        lane);
+        return;
     }
     st.l += __shfl_xor(st.l, 32);
     if (row < rows)
@@ -630,7 +709,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
     constexpr int kWave = kStages * 2 * Tl::kElems;
     static_assert(kWave * sizeof(T) >= 32 * DP * sizeof(float), "room for the sums");
     __shared__ __attribute__((aligned(16))) T lds[4 * kWave];
-    __shared__ float scratch[4][32 * 32];
     __shared__ float ml[4][32][2];
     const Work w(blockIdx.x, a.KV, a.slots);
     const Place pl = place_of(w.slot, a.n, [&](int s) {
@@ -656,6 +734,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
     const int t0 = (int)((int64_t)tiles * blockIdx.y / a.splits) + wave;
     const int t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / a.splits);
 
+    const Lanes<DT, DP> L(lane);
     Rows<DT, DP, KT> st;
     const T *qrow = row < rows ? static_cast<const T *>(a.q) + token * a.ldq +
                                      (int64_t)(w.kv * a.G + g) * a.D
@@ -703,13 +782,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
         }
         const int key0 = t * KT;
         const T *at = mine + stage * 2 * Tl::kElems;
-        st.step(at, at + Tl::kElems, key0, last, key0 + KT - 1 <= first, c, scratch[wave], lane);
+        st.step(at, at + Tl::kElems, key0, last, key0 + KT - 1 <= first, c, L);
         if constexpr (!DMA) {
             __builtin_amdgcn_wave_barrier();
             if (more) store(next);
             __builtin_amdgcn_wave_barrier();
         }
         stage = next;
+    }
+    if (__syncthreads_or(st.bad)) {
+        careful_fwd<DT>(a, sq, w.kv, blockIdx.y, m0, min(m0 + kFewRows, rows), (t0 - wave) * KT,
+                        t1 * KT, wave, lane);
+        return;
     }
     st.l += __shfl_xor(st.l, 32);
     // Join the waves: from their largest m, O scaled by each wave into its own LDS, added
@@ -814,24 +898,90 @@ __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.
 constexpr float kUpDs = 4.0f;  // its power above 1 / the largest |dout|
 constexpr float kUpP = 8.0f;   // fp16: the probabilities' that dV is summed from
 
-// dQ, a tile of rows a workgroup, in the forward's layout; and for the pass over the
+// dQ of rows row0 .. row1 - 1, and dK and dV of keys key0 .. key1 - 1, carefully.
+template <int DT>
+__device__ void careful_bwd_q(const Args &a, const Seq &sq, int kv, int row0, int row1, int wave,
+                              int lane) {
+    using T = typename Type<DT>::T;
+    const float c = a.scale * kLog2e;
+    const T *k = static_cast<const T *>(a.k) + sq.k0 * a.ldk + (int64_t)kv * a.D;
+    const T *v = static_cast<const T *>(a.v) + sq.k0 * a.ldv + (int64_t)kv * a.D;
+    const int64_t n = (int64_t)a.KV * a.Tq * a.G;
+    const float *stats = a.rows + (int64_t)kv * a.Tq * a.G + sq.q0 * a.G;
+    for (int row = row0 + wave; row < row1; row += 4) {
+        const int i = a.group.of(row), head = kv * a.G + row - i * a.G, token = sq.q0 + i;
+        const int end = min(sq.lk, a.causal ? i + sq.lk - sq.lq + 1 : sq.lk);
+        const int64_t col = (int64_t)head * a.D;
+        const T *q = static_cast<const T *>(a.q) + token * a.ldq + col;
+        const T *dout = static_cast<const T *>(a.dout) + token * a.lddo + col;
+        const float lse2 = stats[row], delta = stats[n + row];
+        float acc[2] = {0.0f, 0.0f};
+        for (int j0 = 0; j0 < end; j0 += 64) {
+            const int j = j0 + lane;
+            const float x = dot<DT>(q, k + j * a.ldk, a.D, j < end);
+            const float dp = dot<DT>(dout, v + j * a.ldv, a.D, j < end);
+            const float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -lse2)) * (dp - delta);
+            for (int e = 0; e < min(64, end - j0); ++e)
+                add_row<DT>(acc, __shfl(ds, e), k + (j0 + e) * a.ldk, a.D, lane);
+        }
+        put_row<DT>(static_cast<T *>(a.dq) + token * a.lddq + col, acc, a.scale, a.D, lane,
+                    a.accumulate);
+    }
+}
+template <int DT>
+__device__ void careful_bwd_kv(const Args &a, const Seq &sq, int kv, int key0, int key1, int wave,
+                               int lane) {
+    using T = typename Type<DT>::T;
+    const float c = a.scale * kLog2e;
+    const int rows = sq.lq * a.G, off = sq.lk - sq.lq;
+    const T *q = static_cast<const T *>(a.q) + sq.q0 * a.ldq + (int64_t)kv * a.G * a.D;
+    const T *dout = static_cast<const T *>(a.dout) + sq.q0 * a.lddo + (int64_t)kv * a.G * a.D;
+    const int64_t n = (int64_t)a.KV * a.Tq * a.G, col = (int64_t)kv * a.D;
+    const float *stats = a.rows + (int64_t)kv * a.Tq * a.G + sq.q0 * a.G;
+    auto at = [&](const T *base, int64_t ld, int row) {
+        const int i = a.group.of(row);
+        return base + i * ld + (int64_t)(row - i * a.G) * a.D;
+    };
+    for (int key = key0 + wave; key < key1; key += 4) {
+        const T *k = static_cast<const T *>(a.k) + (sq.k0 + key) * a.ldk + col;
+        const T *v = static_cast<const T *>(a.v) + (sq.k0 + key) * a.ldv + col;
+        float dk[2] = {0.0f, 0.0f}, dv[2] = {0.0f, 0.0f};
+        for (int r0 = a.causal ? max(0, key - off) * a.G : 0; r0 < rows; r0 += 64) {
+            const int row = min(r0 + lane, rows - 1);
+            const bool on = r0 + lane < rows;
+            const float x = dot<DT>(k, at(q, a.ldq, row), a.D, on);
+            const float dp = dot<DT>(v, at(dout, a.lddo, row), a.D, on);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -stats[row]));
+            const float ds = p * (dp - stats[n + row]);
+            for (int e = 0; e < min(64, rows - r0); ++e) {
+                add_row<DT>(dk, __shfl(ds, e), at(q, a.ldq, r0 + e), a.D, lane);
+                add_row<DT>(dv, __shfl(p, e), at(dout, a.lddo, r0 + e), a.D, lane);
+            }
+        }
+        put_row<DT>(static_cast<T *>(a.dk) + (sq.k0 + key) * a.lddk + col, dk, a.scale, a.D, lane,
+                    a.accumulate);
+        put_row<DT>(static_cast<T *>(a.dv) + (sq.k0 + key) * a.lddv + col, dv, 1.0f, a.D, lane,
+                    a.accumulate);
+    }
+}
+
+// dQ, N blocks of 32 rows a wave, in the forward's layout; and for the pass over the
 // keys, in the order of the key head's rows, log2 of their sums, delta and (fp16) their
 // largest |dout|.
-template <int DT, int DP, bool DMA>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
-att_bwd_q(const Args a) {
+template <int DT, int DP, bool DMA, int N>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void att_bwd_q(
+    const Args a) {
     using Ty = Type<DT>;
     using T = typename Ty::T;
-    constexpr int KT = keys_of<DT>(), NB = DP / 32, NK = DP / 16;
+    constexpr int KT = keys_of<DT>(), NB = DP / 32, NK = DP / 16, kWgRows = 128 * N;
     using Tl = Tile<DT, DP, KT>;
     __shared__ __attribute__((aligned(16))) T lds[4 * Tl::kElems];
-    __shared__ float scratch[4][32 * 32];
     const Work w(blockIdx.x, a.KV, a.slots);
     const Place pl = place_of(a.slots - 1 - w.slot, a.n, [&](int s) {
-        return (int)min(a.qs[s], (uint32_t)a.Tq) * a.G / kRows + s;
+        return (int)min(a.qs[s], (uint32_t)a.Tq) * a.G / kWgRows + s;
     });
     const Seq sq(a, pl.seq);
-    const int rows = sq.lq * a.G, m0 = pl.tile * kRows;
+    const int rows = sq.lq * a.G, m0 = pl.tile * kWgRows;
     if (pl.tile < 0 || m0 >= rows) return;  // (a slot of no tile)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, l32 = lane & 31, off = sq.lk - sq.lq;
@@ -841,54 +991,60 @@ att_bwd_q(const Args a) {
     auto last_of = [&](int row) {
         return a.causal ? min(sq.lk - 1, a.group.of(row) + off) : sq.lk - 1;
     };
-    const int w0 = m0 + 32 * wave, row = w0 + l32;
-    const int token = sq.q0 + a.group.of(row), g = row - (token - sq.q0) * a.G;
-    const int head = w.kv * a.G + g;
-    const int last = row < rows ? last_of(row) : -1;
+    const int w0 = m0 + 32 * N * wave;
     const int wave_first = w0 < rows ? last_of(w0) : -1;
-    const int wave_last = w0 < rows ? last_of(min(w0 + 31, rows - 1)) : -1;
-    const int keys = last_of(min(m0 + kRows, rows) - 1) + 1;
+    const int wave_last = w0 < rows ? last_of(min(w0 + 32 * N, rows) - 1) : -1;
+    const int keys = last_of(min(m0 + kWgRows, rows) - 1) + 1;
     const int tiles = keys > 0 ? (keys - 1) / KT + 1 : 0;
 
-    typename Ty::Frag q[NK], dout[NK];
-    const T *qrow = nullptr, *drow = nullptr, *orow = nullptr;
-    if (row < rows) {
-        const int64_t col = (int64_t)head * a.D;
-        qrow = static_cast<const T *>(a.q) + token * a.ldq + col;
-        drow = static_cast<const T *>(a.dout) + token * a.lddo + col;
-        orow = static_cast<const T *>(a.out) + token * a.ldo + col;
-    }
-    float delta = 0.0f, big = 0.0f;
+    typename Ty::Frag q[N][NK], dout[N][NK];
+    int last[N], up[N];
+    float delta[N], from[N];
 #pragma unroll
-    for (int ks = 0; ks < NK; ++ks) {
-        q[ks] = Ty::load8(qrow, 16 * ks + 8 * h, a.D);
-        dout[ks] = Ty::load8(drow, 16 * ks + 8 * h, a.D);
-        const typename Ty::Frag o = Ty::load8(orow, 16 * ks + 8 * h, a.D);
+    for (int i = 0; i < N; ++i) {
+        const int row = w0 + 32 * i + l32;
+        const int token = sq.q0 + a.group.of(row), head = w.kv * a.G + row - (token - sq.q0) * a.G;
+        const T *qrow = nullptr, *drow = nullptr, *orow = nullptr;
+        if (row < rows) {
+            const int64_t col = (int64_t)head * a.D;
+            qrow = static_cast<const T *>(a.q) + token * a.ldq + col;
+            drow = static_cast<const T *>(a.dout) + token * a.lddo + col;
+            orow = static_cast<const T *>(a.out) + token * a.ldo + col;
+        }
+        float sum = 0.0f, big = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float d = Ty::get(dout[ks], j);
-            delta += d * Ty::get(o, j);
-            if constexpr (DT == kF16) big = fmaxf(big, fabsf(d));
+        for (int ks = 0; ks < NK; ++ks) {
+            q[i][ks] = Ty::load8(qrow, 16 * ks + 8 * h, a.D);
+            dout[i][ks] = Ty::load8(drow, 16 * ks + 8 * h, a.D);
+            const typename Ty::Frag o = Ty::load8(orow, 16 * ks + 8 * h, a.D);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = Ty::get(dout[i][ks], j);
+                sum += d * Ty::get(o, j);
+                if constexpr (DT == kF16) big = fmaxf(big, fabsf(d));
+            }
         }
-    }
-    delta += __shfl_xor(delta, 32);
-    if constexpr (DT == kF16) big = fmaxf(big, __shfl_xor(big, 32));
-    // A row of no key (its lse -inf): every probability 0.
-    float lse2 = INFINITY;
-    if (row < rows) {
-        const float x = a.lse[(int64_t)head * a.Tq + token];
-        lse2 = x == -INFINITY ? INFINITY : x * kLog2e;
-        if (x == -INFINITY) delta = 0.0f;
-        if (h == 0) {
-            const int64_t n = (int64_t)a.KV * a.Tq * a.G;
-            const int64_t at = (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G + row;
-            a.rows[at] = lse2;
-            a.rows[n + at] = delta;
-            if constexpr (DT == kF16) a.rows[2 * n + at] = big;
+        sum += __shfl_xor(sum, 32);
+        if constexpr (DT == kF16) big = fmaxf(big, __shfl_xor(big, 32));
+        // A row of no key (its lse -inf): every probability 0.
+        float lse2 = INFINITY;
+        if (row < rows) {
+            const float x = a.lse[(int64_t)head * a.Tq + token];
+            lse2 = x == -INFINITY ? INFINITY : x * kLog2e;
+            if (x == -INFINITY) sum = 0.0f;
+            if (h == 0) {
+                const int64_t n = (int64_t)a.KV * a.Tq * a.G;
+                const int64_t at = (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G + row;
+                a.rows[at] = lse2;
+                a.rows[n + at] = sum;
+                if constexpr (DT == kF16) a.rows[2 * n + at] = big;
+            }
         }
+        last[i] = row < rows ? last_of(row) : -1;
+        delta[i] = sum;
+        up[i] = DT == kF16 ? (int)kUpDs - exponent_above(big) : 0;
+        from[i] = lse2 - (float)up[i];
     }
-    const int up = DT == kF16 ? (int)kUpDs - exponent_above(big) : 0;
-    const float from = lse2 - (float)up;
 
     Mover<DT, DP, KT, 256, DMA> mk, mv;
     auto load = [&](int t) {
@@ -903,8 +1059,11 @@ att_bwd_q(const Args a) {
         mk.store(to, tid);
         mv.store(to + Tl::kElems, tid);
     };
-    f32x16 dq[NB];
-    clear(dq);
+    const Lanes<DT, DP> L(lane);
+    bool bad = false;  // a tile of keys not all visible held an infinity or NaN
+    f32x16 dq[N][NB];
+#pragma unroll
+    for (int i = 0; i < N; ++i) clear(dq[i]);
     if (tiles > 0) {
         load(0);
         store(0);
@@ -917,136 +1076,166 @@ att_bwd_q(const Args a) {
         const T *kt = lds + (t & 1) * 2 * Tl::kElems, *vt = kt + Tl::kElems;
         if (key0 <= wave_last) {
             const bool whole = key0 + KT - 1 <= wave_first;
-            const bool plain = whole || Tl::finite(kt, lane);
+            if (!whole) bad |= !Tl::finite(kt, lane);
 #pragma unroll
             for (int b = 0; b < KT / 32; ++b) {
-                f32x16 s = zero16(), dp = zero16();
+                f32x16 s[N], dp[N];
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks)
-                    s = Ty::mfma(Tl::by_row(kt, 32 * b + l32, ks, h), q[ks], s);
+                for (int i = 0; i < N; ++i) s[i] = dp[i] = zero16();
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks)
-                    dp = Ty::mfma(Tl::by_row(vt, 32 * b + l32, ks, h), dout[ks], dp);
+                for (int ks = 0; ks < NK; ++ks) {
+                    const typename Ty::Frag f = Tl::by_row(kt, b, ks, L);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -from));
-                    s[r] = p * (dp[r] - delta);
+                    for (int i = 0; i < N; ++i) s[i] = Ty::mfma(f, q[i][ks], s[i]);
                 }
-                if (!whole) {
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks) {
+                    const typename Ty::Frag f = Tl::by_row(vt, b, ks, L);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) dp[i] = Ty::mfma(f, dout[i][ks], dp[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int key = key0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
-                        s[r] = key <= last ? s[r] : 0.0f;
+                        const float p =
+                            __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], c, -from[i]));
+                        s[i][r] = p * (dp[i][r] - delta[i]);
                     }
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int key = key0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
+                            s[i][r] = key <= last[i] ? s[i][r] : 0.0f;
+                        }
                 }
-                if (plain) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const typename Ty::Frag ds = Ty::pack(s, u);
+                for (int u = 0; u < 2; ++u) {
+                    typename Ty::Frag ds[N];
 #pragma unroll
-                        for (int d = 0; d < NB; ++d)
-                            dq[d] = Ty::mfma(Tl::by_column(kt, 32 * b + 16 * u, 32 * d, lane), ds,
-                                             dq[d]);
+                    for (int i = 0; i < N; ++i) ds[i] = Ty::pack(s[i], u);
+#pragma unroll
+                    for (int d = 0; d < NB; ++d) {
+                        const typename Ty::Frag f = Tl::by_column(kt, 32 * b + 16 * u, d, L);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) dq[i][d] = Ty::mfma(f, ds[i], dq[i][d]);
                     }
-                } else {
-                    add_careful<DT, DP, KT>(dq, s, kt, 32 * b, 0, last - key0 - 32 * b,
-                                            scratch[wave], lane);
                 }
             }
         }
         if (t + 1 < tiles) store(t + 1);
     }
-    if (row >= rows) return;
-    const float f = a.scale * pow2(-up);
-    T *p = static_cast<T *>(a.dq) + token * a.lddq + (int64_t)head * a.D;
+    if (__syncthreads_or(bad)) {
+        careful_bwd_q<DT>(a, sq, w.kv, m0, min(m0 + kWgRows, rows), wave, lane);
+        return;
+    }
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int i = 0; i < N; ++i) {
+        const int row = w0 + 32 * i + l32;
+        if (row >= rows) continue;
+        const int token = sq.q0 + a.group.of(row), head = w.kv * a.G + row - (token - sq.q0) * a.G;
+        const float f = a.scale * pow2(-up[i]);
+        T *p = static_cast<T *>(a.dq) + token * a.lddq + (int64_t)head * a.D;
 #pragma unroll
-        for (int qd = 0; qd < 4; ++qd)
-            Ty::store4(p, 32 * b + 8 * qd + 4 * h, a.D,
-                       f32x4{dq[b][4 * qd] * f, dq[b][4 * qd + 1] * f, dq[b][4 * qd + 2] * f,
-                             dq[b][4 * qd + 3] * f},
-                       a.accumulate);
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int qd = 0; qd < 4; ++qd)
+                Ty::store4(p, 32 * b + 8 * qd + 4 * h, a.D,
+                           f32x4{dq[i][b][4 * qd] * f, dq[i][b][4 * qd + 1] * f,
+                                 dq[i][b][4 * qd + 2] * f, dq[i][b][4 * qd + 3] * f},
+                           a.accumulate);
+    }
 }
 
-// dK and dV, kKeys keys a workgroup, 32 a wave (one a lane, both halves), over the rows
-// that see them: of all the group's heads, so the sum over a key head's queries is one
+// dK and dV, N blocks of 32 keys a wave (a key a lane, both halves), over the rows that
+// see them: of all the group's heads, so the sum over a key head's queries is one
 // accumulator's.
 template <int DT>
 constexpr int rows_of() {
     return DT == kF32 ? 32 : 64;
 }
-template <int DT, int DP, bool DMA>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
-att_bwd_kv(const Args a) {
+template <int DT, int DP, bool DMA, int N>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void att_bwd_kv(
+    const Args a) {
     using Ty = Type<DT>;
     using T = typename Ty::T;
-    constexpr int RT = rows_of<DT>(), NB = DP / 32, NK = DP / 16;
+    constexpr int RT = rows_of<DT>(), NB = DP / 32, NK = DP / 16, kWgKeys = 128 * N;
     constexpr float kUpV = DT == kF16 ? kUpP : 0.0f;
     using Tl = Tile<DT, DP, RT>;
     __shared__ __attribute__((aligned(16))) T lds[4 * Tl::kElems];
     __shared__ __attribute__((aligned(16))) float stats[2][3][RT];
-    __shared__ float scratch[4][32 * 32];
     const Work w(blockIdx.x, a.KV, a.kslots);
     const Place pl = place_of(w.slot, a.n, [&](int s) {
-        return (int)min(a.ks[s], (uint32_t)a.Tk) / kKeys + s;
+        return (int)min(a.ks[s], (uint32_t)a.Tk) / kWgKeys + s;
     });
     const Seq sq(a, pl.seq);
-    const int n0 = pl.tile * kKeys;
+    const int n0 = pl.tile * kWgKeys;
     if (pl.tile < 0 || n0 >= sq.lk) return;  // (a slot of no tile)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, l32 = lane & 31, off = sq.lk - sq.lq;
     const float c = a.scale * kLog2e;
     const int rows = sq.lq * a.G;
     // The first row that sees a key.
-    auto first_of = [&](int key) { return a.causal ? max(0, key - off) * a.G : 0; };
-    const int kw = n0 + 32 * wave, key = kw + l32;
-    const int first = key < sq.lk ? first_of(key) : rows;
-    const int wave_first = kw < sq.lk ? first_of(kw) : rows;
-    const int wave_last = kw < sq.lk ? first_of(min(kw + 31, sq.lk - 1)) : rows;
+    auto first_of = [&](int key) {
+        return key >= sq.lk ? rows : a.causal ? max(0, key - off) * a.G : 0;
+    };
+    const int kw = n0 + 32 * N * wave;
+    const int wave_first = first_of(kw), wave_last = first_of(kw + 32 * N - 1);
 
-    typename Ty::Frag kf[NK], vf[NK];
-    const T *krow = nullptr, *vrow = nullptr;
-    if (key < sq.lk) {
-        krow = static_cast<const T *>(a.k) + (sq.k0 + key) * a.ldk + (int64_t)w.kv * a.D;
-        vrow = static_cast<const T *>(a.v) + (sq.k0 + key) * a.ldv + (int64_t)w.kv * a.D;
-    }
+    typename Ty::Frag kf[N][NK], vf[N][NK];
+    int first[N];
 #pragma unroll
-    for (int ks = 0; ks < NK; ++ks) {
-        kf[ks] = Ty::load8(krow, 16 * ks + 8 * h, a.D);
-        vf[ks] = Ty::load8(vrow, 16 * ks + 8 * h, a.D);
+    for (int i = 0; i < N; ++i) {
+        const int key = kw + 32 * i + l32;
+        first[i] = first_of(key);
+        const T *krow = nullptr, *vrow = nullptr;
+        if (key < sq.lk) {
+            krow = static_cast<const T *>(a.k) + (sq.k0 + key) * a.ldk + (int64_t)w.kv * a.D;
+            vrow = static_cast<const T *>(a.v) + (sq.k0 + key) * a.ldv + (int64_t)w.kv * a.D;
+        }
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) {
+            kf[i][ks] = Ty::load8(krow, 16 * ks + 8 * h, a.D);
+            vf[i][ks] = Ty::load8(vrow, 16 * ks + 8 * h, a.D);
+        }
     }
     Mover<DT, DP, RT, 256, DMA> mq, md;
     const T *qb = static_cast<const T *>(a.q) + sq.q0 * a.ldq + (int64_t)w.kv * a.G * a.D;
     const T *db = static_cast<const T *>(a.dout) + sq.q0 * a.lddo + (int64_t)w.kv * a.G * a.D;
     const int64_t n = (int64_t)a.KV * a.Tq * a.G;
     const float *rs = a.rows + (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G;
+    constexpr int kStats = DT == kF16 ? 3 : 2;
     float sv = 0.0f;
     auto load = [&](int t) {
         T *to = lds + (t & 1) * 2 * Tl::kElems;
         const int r0 = t * RT, left = rows - r0;
+        const int what = tid / RT, r = tid % RT;
+        if (what < kStats)  // (rows past the last: probability 0)
+            sv = r < left ? rs[what * n + r0 + r] : what == 0 ? INFINITY : 0.0f;
         auto at = [&](const T *base, int64_t ld, int r) {
             const int x = min(r0 + r, rows - 1), i = a.group.of(x);
             return base + i * ld + (int64_t)(x - i * a.G) * a.D;
         };
         mq.load(to, tid, left, a.D, [&](int r) { return at(qb, a.ldq, r); });
         md.load(to + Tl::kElems, tid, left, a.D, [&](int r) { return at(db, a.lddo, r); });
-        const int what = tid / RT, r = tid % RT;
-        if (what < (DT == kF16 ? 3 : 2)) {
-            // (Rows past the last: probability 0.)
-            sv = r < left ? rs[what * n + r0 + r] : what == 0 ? INFINITY : 0.0f;
-        }
     };
     auto store = [&](int t) {
         T *to = lds + (t & 1) * 2 * Tl::kElems;
         mq.store(to, tid);
         md.store(to + Tl::kElems, tid);
         const int what = tid / RT;
-        if (what < (DT == kF16 ? 3 : 2)) stats[t & 1][what][tid % RT] = sv;
+        if (what < kStats) stats[t & 1][what][tid % RT] = sv;
     };
-    f32x16 dk[NB], dv[NB];
-    clear(dk);
-    clear(dv);
+    const Lanes<DT, DP> L(lane);
+    bool bad = false;  // a tile of rows that do not all see every key held an infinity or NaN
+    f32x16 dk[N][NB], dv[N][NB];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        clear(dk[i]);
+        clear(dv[i]);
+    }
     int up = 0;  // fp16: the power of two that dK carries
     bool any = false;
     const int t0 = first_of(n0) / RT, t1 = rows > 0 ? (rows - 1) / RT + 1 : 0;
@@ -1063,7 +1252,7 @@ att_bwd_kv(const Args a) {
         const float *st = stats[t & 1][0];
         if (r0 + RT > wave_first) {
             const bool whole = r0 >= wave_last && r0 + RT <= rows;
-            const bool plain = whole || (Tl::finite(qt, lane) && Tl::finite(dt, lane));
+            if (!whole) bad |= !(Tl::finite(qt, lane) && Tl::finite(dt, lane));
             float fs = 1.0f;
             if constexpr (DT == kF16) {
                 float big = st[2 * RT + lane];
@@ -1074,9 +1263,11 @@ att_bwd_kv(const Args a) {
                     if (any) {
                         const float f = pow2(e - up);
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
+                        for (int i = 0; i < N; ++i)
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) dk[b][r] *= f;
+                            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                                for (int r = 0; r < 16; ++r) dk[i][b][r] *= f;
                     }
                     up = e;
                     any = true;
@@ -1085,79 +1276,105 @@ att_bwd_kv(const Args a) {
             }
 #pragma unroll
             for (int b = 0; b < RT / 32; ++b) {
-                f32x16 p = zero16(), dp = zero16();
+                f32x16 p[N], dp[N];
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks)
-                    p = Ty::mfma(Tl::by_row(qt, 32 * b + l32, ks, h), kf[ks], p);
+                for (int i = 0; i < N; ++i) p[i] = dp[i] = zero16();
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks)
-                    dp = Ty::mfma(Tl::by_row(dt, 32 * b + l32, ks, h), vf[ks], dp);
+                for (int ks = 0; ks < NK; ++ks) {
+                    const typename Ty::Frag f = Tl::by_row(qt, b, ks, L);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) p[i] = Ty::mfma(f, kf[i][ks], p[i]);
+                }
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks) {
+                    const typename Ty::Frag f = Tl::by_row(dt, b, ks, L);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) dp[i] = Ty::mfma(f, vf[i][ks], dp[i]);
+                }
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int at = 32 * b + 8 * q + 4 * h;
                     const f32x4 lse = *reinterpret_cast<const f32x4 *>(st + at);
                     const f32x4 delta = *reinterpret_cast<const f32x4 *>(st + RT + at);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * q + e;
-                        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], c, kUpV - lse[e]));
-                        dp[r] = p[r] * (DT == kF16 ? (dp[r] - delta[e]) * fs : dp[r] - delta[e]);
-                    }
+                    for (int i = 0; i < N; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = 4 * q + e;
+                            const float x = __builtin_amdgcn_exp2f(
+                                __builtin_fmaf(p[i][r], c, kUpV - lse[e]));
+                            const float y = dp[i][r] - delta[e];
+                            p[i][r] = x;
+                            dp[i][r] = x * (DT == kF16 ? y * fs : y);
+                        }
                 }
                 if (!whole) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int x = r0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
-                        const bool on = x >= first && x < rows;
-                        p[r] = on ? p[r] : 0.0f;
-                        dp[r] = on ? dp[r] : 0.0f;
+                    for (int i = 0; i < N; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int x = r0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
+                            const bool on = x >= first[i] && x < rows;
+                            p[i][r] = on ? p[i][r] : 0.0f;
+                            dp[i][r] = on ? dp[i][r] : 0.0f;
+                        }
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    typename Ty::Frag w[N];
+#pragma unroll
+                    for (int i = 0; i < N; ++i) w[i] = Ty::pack(p[i], u);
+#pragma unroll
+                    for (int d = 0; d < NB; ++d) {
+                        const typename Ty::Frag f = Tl::by_column(dt, 32 * b + 16 * u, d, L);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) dv[i][d] = Ty::mfma(f, w[i], dv[i][d]);
                     }
                 }
-                if (plain) {
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const typename Ty::Frag pf = Ty::pack(p, u);
+                for (int u = 0; u < 2; ++u) {
+                    typename Ty::Frag w[N];
 #pragma unroll
-                        for (int d = 0; d < NB; ++d)
-                            dv[d] = Ty::mfma(Tl::by_column(dt, 32 * b + 16 * u, 32 * d, lane), pf,
-                                             dv[d]);
+                    for (int i = 0; i < N; ++i) w[i] = Ty::pack(dp[i], u);
+#pragma unroll
+                    for (int d = 0; d < NB; ++d) {
+                        const typename Ty::Frag f = Tl::by_column(qt, 32 * b + 16 * u, d, L);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) dk[i][d] = Ty::mfma(f, w[i], dk[i][d]);
                     }
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const typename Ty::Frag ds = Ty::pack(dp, u);
-#pragma unroll
-                        for (int d = 0; d < NB; ++d)
-                            dk[d] = Ty::mfma(Tl::by_column(qt, 32 * b + 16 * u, 32 * d, lane), ds,
-                                             dk[d]);
-                    }
-                } else {
-                    const int lo = first - r0 - 32 * b, hi = rows - 1 - r0 - 32 * b;
-                    add_careful<DT, DP, RT>(dv, p, dt, 32 * b, lo, hi, scratch[wave], lane);
-                    add_careful<DT, DP, RT>(dk, dp, qt, 32 * b, lo, hi, scratch[wave], lane);
                 }
             }
         }
         if (t + 1 < t1) store(t + 1);
     }
-    if (key >= sq.lk) return;
+    if (__syncthreads_or(bad)) {
+        careful_bwd_kv<DT>(a, sq, w.kv, n0, min(n0 + kWgKeys, sq.lk), wave, lane);
+        return;
+    }
     const float fk = a.scale * pow2(-up), fv = pow2(-(int)kUpV);
     const int64_t col = (int64_t)w.kv * a.D;
-    T *pk = static_cast<T *>(a.dk) + (sq.k0 + key) * a.lddk + col;
-    T *pv = static_cast<T *>(a.dv) + (sq.k0 + key) * a.lddv + col;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int i = 0; i < N; ++i) {
+        const int key = kw + 32 * i + l32;
+        if (key >= sq.lk) continue;
+        T *pk = static_cast<T *>(a.dk) + (sq.k0 + key) * a.lddk + col;
+        T *pv = static_cast<T *>(a.dv) + (sq.k0 + key) * a.lddv + col;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int d = 32 * b + 8 * q + 4 * h;
-            Ty::store4(pk, d, a.D,
-                       f32x4{dk[b][4 * q] * fk, dk[b][4 * q + 1] * fk, dk[b][4 * q + 2] * fk,
-                             dk[b][4 * q + 3] * fk},
-                       a.accumulate);
-            Ty::store4(pv, d, a.D,
-                       f32x4{dv[b][4 * q] * fv, dv[b][4 * q + 1] * fv, dv[b][4 * q + 2] * fv,
-                             dv[b][4 * q + 3] * fv},
-                       a.accumulate);
-        }
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int d = 32 * b + 8 * q + 4 * h;
+                const f32x16 &x = dk[i][b], &y = dv[i][b];
+                Ty::store4(pk, d, a.D,
+                           f32x4{x[4 * q] * fk, x[4 * q + 1] * fk, x[4 * q + 2] * fk,
+                                 x[4 * q + 3] * fk},
+                           a.accumulate);
+                Ty::store4(pv, d, a.D,
+                           f32x4{y[4 * q] * fv, y[4 * q + 1] * fv, y[4 * q + 2] * fv,
+                                 y[4 * q + 3] * fv},
+                           a.accumulate);
+            }
+    }
 }
 
 // ------------------------------------------------------------------ launches
@@ -1190,8 +1407,9 @@ int combine(hipStream_t st, const Args &a) {
 template <int DT>
 int backward(hipStream_t st, const Args &a, bool dma) {
     with_width<DT>(a.D, dma, [&](auto dp, auto d) {
-        att_bwd_q<DT, dp(), d()><<<a.KV * a.slots, 256, 0, st>>>(a);
-        if (a.kslots) att_bwd_kv<DT, dp(), d()><<<a.KV * a.kslots, 256, 0, st>>>(a);
+        constexpr int N = kBlocks<DT>;
+        att_bwd_q<DT, dp(), d(), N><<<a.KV * a.slots, 256, 0, st>>>(a);
+        if (a.kslots) att_bwd_kv<DT, dp(), d(), N><<<a.KV * a.kslots, 256, 0, st>>>(a);
     });
     return (int)hipGetLastError();
 }
