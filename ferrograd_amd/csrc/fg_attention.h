@@ -7,8 +7,6 @@
 
 #include <cstdint>
 
-#include "fg_half.h"
-
 namespace fg {
 namespace attn {
 
@@ -51,11 +49,9 @@ struct Args {
     int kslots, accumulate;
 };
 
-// Query rows of a workgroup; blocks of 32 rows (keys) a wave of the backward's passes,
-// four waves a workgroup.
-constexpr int kRows = 128, kFewRows = 32;
-template <int DT>
-constexpr int kBlocks = DT == kF32 ? 1 : 2;
+// Rows of a workgroup (of the few rows' one), and keys of one in the backward's pass over
+// the keys.
+constexpr int kRows = 128, kFewRows = 32, kKeys = 128;
 
 // Launches on `st`; 0 or the HIP error.  dma: rows of K and V (and of the other
 // operands) are whole 16-byte chunks at 16-byte boundaries, and D is the tile's width.

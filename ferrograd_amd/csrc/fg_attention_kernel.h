@@ -19,9 +19,11 @@
 // 8 + 4 h + 0..3 of each 16.  Softmax statistics are a lane's own, but for the half of
 // the keys that lane ^ 32 holds.
 //
-// Tiles sit in LDS as rows of DP elements with 16-byte chunk c of row r at c ^ swz(r):
-// read by rows (8 lanes a cycle, the same chunk of 8 rows) and, through the transposing
-// reads, by columns (4 rows of 2 chunks a cycle), both reach distinct banks.
+// Tiles sit in LDS as rows of DP elements, a few chunks apart, with 16-byte chunk c of
+// row r at c ^ swz(r): read by rows (16 lanes a cycle, the same chunk of 16 rows) and,
+// through the transposing reads, by columns (4 rows of 4 chunks a cycle), both reach
+// every bank once.  (With three bits of the row and no gaps, two lanes a bank, half of
+// LDS's time: SQ_LDS_BANK_CONFLICT 5.5e7 of 1.1e8 in dQ's kernel.)
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -51,8 +53,17 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
-// Bits of a chunk's place that its row sets.
-__device__ __forceinline__ int swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+// Bits of a chunk's place that its row sets, and the chunks left free before a row: one
+// every 4 rows, of 8 chunks (128 bytes) two every 8, so that what a wave's direct load
+// writes, 1 KiB, is of one piece.
+template <int CH>
+__device__ __forceinline__ int swz(int row) {
+    return CH == 8 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 1) : (row & 3) << 2;
+}
+template <int CH>
+__device__ __forceinline__ constexpr int gap(int row) {
+    return CH == 8 ? (row >> 3) * 2 : row >> 2;
+}
 
 template <int DT>
 struct Type {
@@ -171,23 +182,27 @@ struct Type {
 
 // ------------------------------------------------------------------ LDS tiles
 // A lane's places in tiles of rows of DP elements, computed once: what the swizzle makes
-// of the low bits of a chunk; everything else of an address is a constant.
+// of a chunk's bits; everything else of an address is a constant.
 template <int DT, int DP>
 struct Lanes {
     static constexpr bool kWide = DT == kF32;
-    int row[4], col[4], lane;
+    static constexpr int E = kWide ? 4 : 8, CH = DP / E;
+    int row[4], col[kWide ? 8 : 4], lane;
+    static __device__ __forceinline__ int place(int r, int c) {
+        return r * DP + (gap<CH>(r) + (c ^ swz<CH>(r))) * E;
+    }
     __device__ __forceinline__ explicit Lanes(int lane_) : lane(lane_) {
         const int h = lane >> 5, l32 = lane & 31;
+        const int e = (lane >> 2) & 3, q = lane & 3;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (kWide) {
-                row[i] = l32 * DP + (((4 * (i >> 1) + 2 * h + (i & 1)) ^ swz(l32)) * 4);
-                col[i] = (4 * h + i) * DP + (((l32 >> 2) ^ swz(4 * h + i)) * 4) + (l32 & 3);
+                row[i] = place(l32, 4 * i + 2 * h);
+                col[i] = place(4 * h + i, l32 >> 2) + (l32 & 3);
+                col[4 + i] = place(4 * h + i, 8 + (l32 >> 2)) + (l32 & 3);
             } else {
-                const int e = (lane >> 2) & 3, q = lane & 3;
-                row[i] = l32 * DP + (((2 * i + h) ^ swz(l32)) * 8);
-                col[i] = (4 * h + e) * DP +
-                         (((4 * (i & 1) + 2 * ((lane >> 4) & 1) + (q >> 1)) ^ swz(4 * h + e)) * 8) +
+                row[i] = place(l32, (4 * i + h) % CH);
+                col[i] = place(4 * h + e, (4 * i + 2 * ((lane >> 4) & 1) + (q >> 1)) % CH) +
                          4 * (q & 1);
             }
         }
@@ -201,24 +216,24 @@ struct Tile {
     using T = typename Ty::T;
     using Frag = typename Ty::Frag;
     static constexpr int E = Ty::E, CH = DP / E;  // chunks of a row
-    static constexpr int kElems = ROWS * DP;
+    static constexpr int kElems = ROWS * DP + gap<CH>(ROWS) * E;
     static constexpr int kChunks = ROWS * CH;
 
     // Rows 32 b + lane % 32, elements 16 ks + 8 h .. + 7: an operand with the tile's rows in
     // lanes.
     static __device__ __forceinline__ Frag by_row(const T *t, int b, int ks,
                                                   const Lanes<DT, DP> &L) {
-        t += 32 * b * DP;
+        t += b * (32 * DP + gap<CH>(32) * E);
         if constexpr (Ty::kWide) {
             Frag f;
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(t + L.row[2 * (ks & 1)] + 32 * (ks >> 1));
-            const f32x4 y =
-                *reinterpret_cast<const f32x4 *>(t + L.row[2 * (ks & 1) + 1] + 32 * (ks >> 1));
+            const T *p = t + L.row[ks & 3] + 64 * (ks >> 2);
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(p);
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(p + 4);
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = j < 4 ? x[j & 3] : y[j & 3];
             return f;
         } else {
-            return *reinterpret_cast<const u32x4 *>(t + L.row[ks & 3] + 64 * (ks >> 2));
+            return *reinterpret_cast<const u32x4 *>(t + L.row[ks >> 1] + 16 * (ks & 1));
         }
     }
     // Columns 32 d + lane % 32, rows r0 + 4 h + 0..3 and r0 + 8 + 4 h + 0..3 (r0 a multiple
@@ -227,17 +242,18 @@ struct Tile {
     // column l's rows.
     static __device__ __forceinline__ Frag by_column(const T *t, int r0, int d,
                                                      const Lanes<DT, DP> &L) {
-        t += r0 * DP;
+        t += r0 / 16 * (16 * DP + gap<CH>(16) * E);
+        constexpr int kHalf = 8 * DP + gap<CH>(8) * E;
         Frag f;
         if constexpr (Ty::kWide) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = t[L.col[j & 3] + 8 * (j >> 2) * DP + 32 * d];
+            for (int j = 0; j < 8; ++j)
+                f[j] = t[L.col[4 * (d & 1) + (j & 3)] + (j >> 2) * kHalf + 64 * (d >> 1)];
         } else {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const v4i16 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) v4i16 *)(t + L.col[d & 1] + 64 * (d >> 1) +
-                                                               8 * half * DP));
+                    (__attribute__((address_space(3))) v4i16 *)(t + L.col[d] + half * kHalf));
                 const u32x2 w = __builtin_bit_cast(u32x2, v);
                 f[2 * half] = w[0];
                 f[2 * half + 1] = w[1];
@@ -251,7 +267,7 @@ struct Tile {
         uint32_t top = 0;
 #pragma unroll 4
         for (int c = lane; c < kChunks; c += 64) {
-            const u32x4 w = *reinterpret_cast<const u32x4 *>(t + c * E);
+            const u32x4 w = *reinterpret_cast<const u32x4 *>(t + (c + gap<CH>(c / CH)) * E);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if constexpr (Ty::kWide) {
@@ -272,41 +288,69 @@ struct Tile {
     }
 };
 
-// Moves a tile's rows from memory, NT threads together (tid among them; wave of them,
-// lane).  DMA: straight into LDS, lane l of a wave load at its 16 l bytes, the source
-// chosen so that the chunks land swizzled; rows past the last are the last again.
-// Otherwise through registers, zeros past the last row and column.
+// Moves a tile's rows from memory, NT threads together.  DMA: straight into LDS, lane l
+// of a wave load at its 16 l bytes, the source chosen so that the chunks land swizzled;
+// rows past the last are the last again.  Otherwise through registers, zeros past the last
+// row and column.
 template <int DT, int DP, int ROWS, int NT, bool DMA>
 struct Mover {
     using Tl = Tile<DT, DP, ROWS>;
     using T = typename Tl::T;
     static constexpr int E = Tl::E, CH = Tl::CH;
     static constexpr int kPer = Tl::kChunks / NT;
+    static constexpr int kLoadRows = 64 / CH;  // rows of a wave load: of one swizzle
     static_assert(Tl::kChunks % NT == 0, "whole chunks a thread");
     u32x4 v[DMA ? 1 : kPer];
 
-    // row_at(r): row r's first element, of the last row for those past it.
+    // DMA: row r at offset_of(r) bytes from the (uniform) base.
     template <class F>
-    __device__ __forceinline__ void load(T *lds, int tid, int rows, int D, F row_at) {
+    static __device__ __forceinline__ void direct(T *lds, int tid, const T *base, F offset_of) {
         const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const uint32_t c = ((lane % CH) ^ swz<CH>(lane / CH)) * 16;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            if constexpr (DMA) {
-                const int li = wave * kPer + i, pos = li * 64 + lane;
-                const int row = pos / CH, c = (pos % CH) ^ swz(row);
-                lds_dma16(row_at(row) + c * E, lds + li * 64 * E);
-            } else {
-                const int pos = i * NT + tid, row = pos / CH, d = (pos % CH) * E;
-                const T *p = row_at(row) + d;
-                if (row < rows && d + E <= D) {
-                    v[i] = *reinterpret_cast<const u32x4_any *>(p);
-                } else {
-                    T e[E];
+            const int row = (wave * kPer + i) * kLoadRows;
+            lds_dma16(base, offset_of(row + lane / CH) + c, lds + row * DP + gap<CH>(row) * E);
+        }
+    }
+    // Otherwise: row r from row_at(r).
+    template <class F>
+    __device__ __forceinline__ void fetch(int tid, int rows, int D, F row_at) {
 #pragma unroll
-                    for (int k = 0; k < E; ++k) e[k] = row < rows && d + k < D ? p[k] : T(0);
-                    v[i] = __builtin_bit_cast(u32x4, e);
-                }
+        for (int i = 0; i < kPer; ++i) {
+            const int pos = i * NT + tid, row = pos / CH, d = (pos % CH) * E;
+            const T *p = row_at(row) + d;
+            if (row < rows && d + E <= D) {
+                v[i] = *reinterpret_cast<const u32x4_any *>(p);
+            } else {
+                T e[E];
+#pragma unroll
+                for (int k = 0; k < E; ++k) e[k] = row < rows && d + k < D ? p[k] : T(0);
+                v[i] = __builtin_bit_cast(u32x4, e);
             }
+        }
+    }
+    // `rows` rows (the tile's, or as many as are left) ld elements apart, from base on.
+    __device__ __forceinline__ void load(T *lds, int tid, const T *base, int64_t ld, int rows,
+                                         int D) {
+        if constexpr (!DMA) {
+            fetch(tid, rows, D, [&](int r) { return base + min(r, rows - 1) * ld; });
+        } else if (rows >= ROWS) {
+            // One offset for all of a lane's loads.
+            const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+            const uint32_t bytes = (uint32_t)ld * sizeof(T);
+            const uint32_t at =
+                lane / CH * bytes + ((lane % CH) ^ swz<CH>(lane / CH)) * 16;
+            const char *from =
+                reinterpret_cast<const char *>(base) + wave * kPer * kLoadRows * bytes;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int row = (wave * kPer + i) * kLoadRows;
+                lds_dma16(from + i * kLoadRows * bytes, at, lds + row * DP + gap<CH>(row) * E);
+            }
+        } else {
+            const uint32_t bytes = (uint32_t)ld * sizeof(T);
+            direct(lds, tid, base, [&](int r) { return (uint32_t)min(r, rows - 1) * bytes; });
         }
     }
     __device__ __forceinline__ void store(T *lds, int tid) const {
@@ -314,7 +358,7 @@ struct Mover {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int pos = i * NT + tid, row = pos / CH, c = pos % CH;
-                *reinterpret_cast<u32x4 *>(lds + row * DP + ((c ^ swz(row)) * E)) = v[i];
+                *reinterpret_cast<u32x4 *>(lds + Lanes<DT, DP>::place(row, c)) = v[i];
             }
         }
     }
@@ -415,10 +459,26 @@ __device__ __forceinline__ void clear(f32x16 (&acc)[NB]) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[b][r] = 0.0f;
 }
-__device__ __forceinline__ f32x16 zero16() {
+__device__ __forceinline__ f32x16 all16(float x) {
     f32x16 z;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+    for (int r = 0; r < 16; ++r) z[r] = x;
+    return z;
+}
+// Keeps a value from being spread over 16 registers once and for all.
+__device__ __forceinline__ float fresh(float x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+// A block's rows' numbers, from those of rows 4 h on.
+__device__ __forceinline__ f32x16 rows16(const float *p) {
+    f32x16 z;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(p + 8 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[4 * q + e] = v[e];
+    }
     return z;
 }
 
@@ -449,7 +509,7 @@ struct Rows {
         f32x16 s[KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-            s[b] = zero16();
+            s[b] = all16(0.0f);
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks)
                 s[b] = Ty::mfma(Tl::by_row(k, b, ks, L), q[ks], s[b]);
@@ -659,9 +719,8 @@ att_fwd(const Args a) {
     auto load = [&](int t) {
         T *to = lds + (t & 1) * 2 * Tl::kElems;
         const int key0 = t * KT, left = sq.lk - key0;
-        mk.load(to, tid, left, a.D, [&](int r) { return k + min(key0 + r, sq.lk - 1) * a.ldk; });
-        mv.load(to + Tl::kElems, tid, left, a.D,
-                [&](int r) { return v + min(key0 + r, sq.lk - 1) * a.ldv; });
+        mk.load(to, tid, k + key0 * a.ldk, a.ldk, left, a.D);
+        mv.load(to + Tl::kElems, tid, v + key0 * a.ldv, a.ldv, left, a.D);
     };
     auto store = [&](int t) {
         T *to = lds + (t & 1) * 2 * Tl::kElems;
@@ -707,7 +766,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
     // A wave's two stages of K and V; at the end its O^T, 32 x DP floats.
     constexpr int kStages = DT == kF32 && DP > 64 ? 1 : 2;
     constexpr int kWave = kStages * 2 * Tl::kElems;
-    static_assert(kWave * sizeof(T) >= 32 * DP * sizeof(float), "room for the sums");
+    static_assert(kWave * sizeof(T) >= 32 * DP * sizeof(float) && kWave % 8 == 0, "room for the sums");
     __shared__ __attribute__((aligned(16))) T lds[4 * kWave];
     __shared__ float ml[4][32][2];
     const Work w(blockIdx.x, a.KV, a.slots);
@@ -748,9 +807,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
     auto load = [&](int t, int stage) {
         T *to = mine + stage * 2 * Tl::kElems;
         const int key0 = t * KT, left = sq.lk - key0;
-        mk.load(to, lane, left, a.D, [&](int r) { return k + min(key0 + r, sq.lk - 1) * a.ldk; });
-        mv.load(to + Tl::kElems, lane, left, a.D,
-                [&](int r) { return v + min(key0 + r, sq.lk - 1) * a.ldv; });
+        mk.load(to, lane, k + key0 * a.ldk, a.ldk, left, a.D);
+        mv.load(to + Tl::kElems, lane, v + key0 * a.ldv, a.ldv, left, a.D);
     };
     auto store = [&](int stage) {
         T *to = mine + stage * 2 * Tl::kElems;
@@ -895,6 +953,11 @@ __device__ __forceinline__ int exponent_above(float x) {
     return max((int)((__float_as_uint(x) & 0x7fffffffu) >> 23) - 126, -100);
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
+// 16 bits: a score's accumulator starts at -lse / c, dP's at -delta, in the units of the
+// products, so that neither is subtracted after them (their roundings, 8 u |lse|, are far
+// below the types').  fp32 would take 64 such roundings of lse.
+template <int DT>
+constexpr bool kFold = DT != kF32;
 constexpr float kUpDs = 4.0f;  // its power above 1 / the largest |dout|
 constexpr float kUpP = 8.0f;   // fp16: the probabilities' that dV is summed from
 
@@ -965,23 +1028,22 @@ __device__ void careful_bwd_kv(const Args &a, const Seq &sq, int kv, int key0, i
     }
 }
 
-// dQ, N blocks of 32 rows a wave, in the forward's layout; and for the pass over the
-// keys, in the order of the key head's rows, log2 of their sums, delta and (fp16) their
-// largest |dout|.
-template <int DT, int DP, bool DMA, int N>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void att_bwd_q(
-    const Args a) {
+// dQ, 32 rows a wave, in the forward's layout; and for the pass over the keys, in the
+// order of the key head's rows, log2 of their sums, delta and (fp16) their largest |dout|.
+template <int DT, int DP, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
+att_bwd_q(const Args a) {
     using Ty = Type<DT>;
     using T = typename Ty::T;
-    constexpr int KT = keys_of<DT>(), NB = DP / 32, NK = DP / 16, kWgRows = 128 * N;
+    constexpr int KT = keys_of<DT>(), NB = DP / 32, NK = DP / 16;
     using Tl = Tile<DT, DP, KT>;
     __shared__ __attribute__((aligned(16))) T lds[4 * Tl::kElems];
     const Work w(blockIdx.x, a.KV, a.slots);
     const Place pl = place_of(a.slots - 1 - w.slot, a.n, [&](int s) {
-        return (int)min(a.qs[s], (uint32_t)a.Tq) * a.G / kWgRows + s;
+        return (int)min(a.qs[s], (uint32_t)a.Tq) * a.G / kRows + s;
     });
     const Seq sq(a, pl.seq);
-    const int rows = sq.lq * a.G, m0 = pl.tile * kWgRows;
+    const int rows = sq.lq * a.G, m0 = pl.tile * kRows;
     if (pl.tile < 0 || m0 >= rows) return;  // (a slot of no tile)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, l32 = lane & 31, off = sq.lk - sq.lq;
@@ -991,68 +1053,61 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
     auto last_of = [&](int row) {
         return a.causal ? min(sq.lk - 1, a.group.of(row) + off) : sq.lk - 1;
     };
-    const int w0 = m0 + 32 * N * wave;
+    const int w0 = m0 + 32 * wave;
     const int wave_first = w0 < rows ? last_of(w0) : -1;
-    const int wave_last = w0 < rows ? last_of(min(w0 + 32 * N, rows) - 1) : -1;
-    const int keys = last_of(min(m0 + kWgRows, rows) - 1) + 1;
+    const int wave_last = w0 < rows ? last_of(min(w0 + 32, rows) - 1) : -1;
+    const int keys = last_of(min(m0 + kRows, rows) - 1) + 1;
     const int tiles = keys > 0 ? (keys - 1) / KT + 1 : 0;
 
-    typename Ty::Frag q[N][NK], dout[N][NK];
-    int last[N], up[N];
-    float delta[N], from[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int row = w0 + 32 * i + l32;
-        const int token = sq.q0 + a.group.of(row), head = w.kv * a.G + row - (token - sq.q0) * a.G;
-        const T *qrow = nullptr, *drow = nullptr, *orow = nullptr;
-        if (row < rows) {
-            const int64_t col = (int64_t)head * a.D;
-            qrow = static_cast<const T *>(a.q) + token * a.ldq + col;
-            drow = static_cast<const T *>(a.dout) + token * a.lddo + col;
-            orow = static_cast<const T *>(a.out) + token * a.ldo + col;
-        }
-        float sum = 0.0f, big = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-            q[i][ks] = Ty::load8(qrow, 16 * ks + 8 * h, a.D);
-            dout[i][ks] = Ty::load8(drow, 16 * ks + 8 * h, a.D);
-            const typename Ty::Frag o = Ty::load8(orow, 16 * ks + 8 * h, a.D);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float d = Ty::get(dout[i][ks], j);
-                sum += d * Ty::get(o, j);
-                if constexpr (DT == kF16) big = fmaxf(big, fabsf(d));
-            }
-        }
-        sum += __shfl_xor(sum, 32);
-        if constexpr (DT == kF16) big = fmaxf(big, __shfl_xor(big, 32));
-        // A row of no key (its lse -inf): every probability 0.
-        float lse2 = INFINITY;
-        if (row < rows) {
-            const float x = a.lse[(int64_t)head * a.Tq + token];
-            lse2 = x == -INFINITY ? INFINITY : x * kLog2e;
-            if (x == -INFINITY) sum = 0.0f;
-            if (h == 0) {
-                const int64_t n = (int64_t)a.KV * a.Tq * a.G;
-                const int64_t at = (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G + row;
-                a.rows[at] = lse2;
-                a.rows[n + at] = sum;
-                if constexpr (DT == kF16) a.rows[2 * n + at] = big;
-            }
-        }
-        last[i] = row < rows ? last_of(row) : -1;
-        delta[i] = sum;
-        up[i] = DT == kF16 ? (int)kUpDs - exponent_above(big) : 0;
-        from[i] = lse2 - (float)up[i];
+    typename Ty::Frag q[NK], dout[NK];
+    const int row = w0 + l32;
+    const int token = sq.q0 + a.group.of(row), head = w.kv * a.G + row - (token - sq.q0) * a.G;
+    const T *qrow = nullptr, *drow = nullptr, *orow = nullptr;
+    if (row < rows) {
+        const int64_t col = (int64_t)head * a.D;
+        qrow = static_cast<const T *>(a.q) + token * a.ldq + col;
+        drow = static_cast<const T *>(a.dout) + token * a.lddo + col;
+        orow = static_cast<const T *>(a.out) + token * a.ldo + col;
     }
+    float delta = 0.0f, big = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < NK; ++ks) {
+        q[ks] = Ty::load8(qrow, 16 * ks + 8 * h, a.D);
+        dout[ks] = Ty::load8(drow, 16 * ks + 8 * h, a.D);
+        const typename Ty::Frag o = Ty::load8(orow, 16 * ks + 8 * h, a.D);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = Ty::get(dout[ks], j);
+            delta += d * Ty::get(o, j);
+            if constexpr (DT == kF16) big = fmaxf(big, fabsf(d));
+        }
+    }
+    delta += __shfl_xor(delta, 32);
+    if constexpr (DT == kF16) big = fmaxf(big, __shfl_xor(big, 32));
+    // A row of no key (its lse -inf): every probability 0.
+    float lse2 = INFINITY;
+    if (row < rows) {
+        const float x = a.lse[(int64_t)head * a.Tq + token];
+        lse2 = x == -INFINITY ? INFINITY : x * kLog2e;
+        if (x == -INFINITY) delta = 0.0f;
+        if (h == 0) {
+            const int64_t n = (int64_t)a.KV * a.Tq * a.G;
+            const int64_t at = (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G + row;
+            a.rows[at] = lse2;
+            a.rows[n + at] = delta;
+            if constexpr (DT == kF16) a.rows[2 * n + at] = big;
+        }
+    }
+    const int last = row < rows ? last_of(row) : -1;
+    const int up = DT == kF16 ? (int)kUpDs - exponent_above(big) : 0;
+    const float from = (lse2 - (float)up) * (kFold<DT> ? 1.0f / c : 1.0f);
 
     Mover<DT, DP, KT, 256, DMA> mk, mv;
     auto load = [&](int t) {
         T *to = lds + (t & 1) * 2 * Tl::kElems;
         const int key0 = t * KT, left = sq.lk - key0;
-        mk.load(to, tid, left, a.D, [&](int r) { return k + min(key0 + r, sq.lk - 1) * a.ldk; });
-        mv.load(to + Tl::kElems, tid, left, a.D,
-                [&](int r) { return v + min(key0 + r, sq.lk - 1) * a.ldv; });
+        mk.load(to, tid, k + key0 * a.ldk, a.ldk, left, a.D);
+        mv.load(to + Tl::kElems, tid, v + key0 * a.ldv, a.ldv, left, a.D);
     };
     auto store = [&](int t) {
         T *to = lds + (t & 1) * 2 * Tl::kElems;
@@ -1061,9 +1116,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
     };
     const Lanes<DT, DP> L(lane);
     bool bad = false;  // a tile of keys not all visible held an infinity or NaN
-    f32x16 dq[N][NB];
-#pragma unroll
-    for (int i = 0; i < N; ++i) clear(dq[i]);
+    f32x16 dq[NB];
+    clear(dq);
     if (tiles > 0) {
         load(0);
         store(0);
@@ -1079,99 +1133,80 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
             if (!whole) bad |= !Tl::finite(kt, lane);
 #pragma unroll
             for (int b = 0; b < KT / 32; ++b) {
-                f32x16 s[N], dp[N];
+                f32x16 s = all16(kFold<DT> ? fresh(-from) : 0.0f);
+                f32x16 dp = all16(kFold<DT> ? fresh(-delta) : 0.0f);
 #pragma unroll
-                for (int i = 0; i < N; ++i) s[i] = dp[i] = zero16();
+                for (int ks = 0; ks < NK; ++ks) s = Ty::mfma(Tl::by_row(kt, b, ks, L), q[ks], s);
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks) {
-                    const typename Ty::Frag f = Tl::by_row(kt, b, ks, L);
+                for (int ks = 0; ks < NK; ++ks)
+                    dp = Ty::mfma(Tl::by_row(vt, b, ks, L), dout[ks], dp);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) s[i] = Ty::mfma(f, q[i][ks], s[i]);
+                for (int r = 0; r < 16; ++r) {
+                    if constexpr (kFold<DT>)
+                        s[r] = __builtin_amdgcn_exp2f(s[r] * c) * dp[r];
+                    else
+                        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -from)) *
+                               (dp[r] - delta);
                 }
-#pragma unroll
-                for (int ks = 0; ks < NK; ++ks) {
-                    const typename Ty::Frag f = Tl::by_row(vt, b, ks, L);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) dp[i] = Ty::mfma(f, dout[i][ks], dp[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float p =
-                            __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], c, -from[i]));
-                        s[i][r] = p * (dp[i][r] - delta[i]);
-                    }
                 if (!whole) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int key = key0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
-                            s[i][r] = key <= last[i] ? s[i][r] : 0.0f;
-                        }
+                    for (int r = 0; r < 16; ++r) {
+                        const int key = key0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
+                        s[r] = key <= last ? s[r] : 0.0f;
+                    }
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    typename Ty::Frag ds[N];
+                    const typename Ty::Frag ds = Ty::pack(s, u);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) ds[i] = Ty::pack(s[i], u);
-#pragma unroll
-                    for (int d = 0; d < NB; ++d) {
-                        const typename Ty::Frag f = Tl::by_column(kt, 32 * b + 16 * u, d, L);
-#pragma unroll
-                        for (int i = 0; i < N; ++i) dq[i][d] = Ty::mfma(f, ds[i], dq[i][d]);
-                    }
+                    for (int d = 0; d < NB; ++d)
+                        dq[d] = Ty::mfma(Tl::by_column(kt, 32 * b + 16 * u, d, L), ds, dq[d]);
                 }
             }
         }
         if (t + 1 < tiles) store(t + 1);
     }
     if (__syncthreads_or(bad)) {
-        careful_bwd_q<DT>(a, sq, w.kv, m0, min(m0 + kWgRows, rows), wave, lane);
+        careful_bwd_q<DT>(a, sq, w.kv, m0, min(m0 + kRows, rows), wave, lane);
         return;
     }
+    if (row >= rows) return;
+    const float f = a.scale * pow2(-up);
+    T *p = static_cast<T *>(a.dq) + token * a.lddq + (int64_t)head * a.D;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int row = w0 + 32 * i + l32;
-        if (row >= rows) continue;
-        const int token = sq.q0 + a.group.of(row), head = w.kv * a.G + row - (token - sq.q0) * a.G;
-        const float f = a.scale * pow2(-up[i]);
-        T *p = static_cast<T *>(a.dq) + token * a.lddq + (int64_t)head * a.D;
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int qd = 0; qd < 4; ++qd)
-                Ty::store4(p, 32 * b + 8 * qd + 4 * h, a.D,
-                           f32x4{dq[i][b][4 * qd] * f, dq[i][b][4 * qd + 1] * f,
-                                 dq[i][b][4 * qd + 2] * f, dq[i][b][4 * qd + 3] * f},
-                           a.accumulate);
-    }
+        for (int qd = 0; qd < 4; ++qd)
+            Ty::store4(p, 32 * b + 8 * qd + 4 * h, a.D,
+                       f32x4{dq[b][4 * qd] * f, dq[b][4 * qd + 1] * f, dq[b][4 * qd + 2] * f,
+                             dq[b][4 * qd + 3] * f},
+                       a.accumulate);
 }
 
-// dK and dV, N blocks of 32 keys a wave (a key a lane, both halves), over the rows that
-// see them: of all the group's heads, so the sum over a key head's queries is one
-// accumulator's.
-template <int DT>
-constexpr int rows_of() {
-    return DT == kF32 ? 32 : 64;
-}
-template <int DT, int DP, bool DMA, int N>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void att_bwd_kv(
-    const Args a) {
+// dK and dV, 32 keys a wave (a key a lane, both halves), over the rows that see them: of
+// all the group's heads, so the sum over a key head's queries is one accumulator's.  K
+// stays in registers and V in LDS: with both in registers there were none left to read
+// ahead into (D 128: each matrix instruction waited for its LDS read, and spilled operands
+// for the next tile's loads in flight; 8 sequences of up to 4096, 32 heads over 8: 2.05 ms
+// and 1.6), and 64 keys a wave, for half the LDS reads, leave one wave a SIMD (2.3 ms).
+template <int DT, int DP, bool DMA>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
+att_bwd_kv(const Args a) {
     using Ty = Type<DT>;
     using T = typename Ty::T;
-    constexpr int RT = rows_of<DT>(), NB = DP / 32, NK = DP / 16, kWgKeys = 128 * N;
+    constexpr int RT = 32, NB = DP / 32, NK = DP / 16;
     constexpr float kUpV = DT == kF16 ? kUpP : 0.0f;
     using Tl = Tile<DT, DP, RT>;
-    __shared__ __attribute__((aligned(16))) T lds[4 * Tl::kElems];
+    using Vt = Tile<DT, DP, kKeys>;
+    __shared__ __attribute__((aligned(16))) T lds[4 * Tl::kElems + Vt::kElems];
+    T *vlds = lds + 4 * Tl::kElems;
     __shared__ __attribute__((aligned(16))) float stats[2][3][RT];
     const Work w(blockIdx.x, a.KV, a.kslots);
     const Place pl = place_of(w.slot, a.n, [&](int s) {
-        return (int)min(a.ks[s], (uint32_t)a.Tk) / kWgKeys + s;
+        return (int)min(a.ks[s], (uint32_t)a.Tk) / kKeys + s;
     });
     const Seq sq(a, pl.seq);
-    const int n0 = pl.tile * kWgKeys;
+    const int n0 = pl.tile * kKeys;
     if (pl.tile < 0 || n0 >= sq.lk) return;  // (a slot of no tile)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, l32 = lane & 31, off = sq.lk - sq.lq;
@@ -1181,26 +1216,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
     auto first_of = [&](int key) {
         return key >= sq.lk ? rows : a.causal ? max(0, key - off) * a.G : 0;
     };
-    const int kw = n0 + 32 * N * wave;
-    const int wave_first = first_of(kw), wave_last = first_of(kw + 32 * N - 1);
+    const int kw = n0 + 32 * wave;
+    const int wave_first = first_of(kw), wave_last = first_of(kw + 31);
 
-    typename Ty::Frag kf[N][NK], vf[N][NK];
-    int first[N];
+    typename Ty::Frag kf[NK];
+    const int key = kw + l32, first = first_of(key);
+    const T *krow = nullptr;
+    if (key < sq.lk)
+        krow = static_cast<const T *>(a.k) + (sq.k0 + key) * a.ldk + (int64_t)w.kv * a.D;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int key = kw + 32 * i + l32;
-        first[i] = first_of(key);
-        const T *krow = nullptr, *vrow = nullptr;
-        if (key < sq.lk) {
-            krow = static_cast<const T *>(a.k) + (sq.k0 + key) * a.ldk + (int64_t)w.kv * a.D;
-            vrow = static_cast<const T *>(a.v) + (sq.k0 + key) * a.ldv + (int64_t)w.kv * a.D;
-        }
-#pragma unroll
-        for (int ks = 0; ks < NK; ++ks) {
-            kf[i][ks] = Ty::load8(krow, 16 * ks + 8 * h, a.D);
-            vf[i][ks] = Ty::load8(vrow, 16 * ks + 8 * h, a.D);
-        }
-    }
+    for (int ks = 0; ks < NK; ++ks) kf[ks] = Ty::load8(krow, 16 * ks + 8 * h, a.D);
     Mover<DT, DP, RT, 256, DMA> mq, md;
     const T *qb = static_cast<const T *>(a.q) + sq.q0 * a.ldq + (int64_t)w.kv * a.G * a.D;
     const T *db = static_cast<const T *>(a.dout) + sq.q0 * a.lddo + (int64_t)w.kv * a.G * a.D;
@@ -1214,32 +1239,50 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
         const int what = tid / RT, r = tid % RT;
         if (what < kStats)  // (rows past the last: probability 0)
             sv = r < left ? rs[what * n + r0 + r] : what == 0 ? INFINITY : 0.0f;
-        auto at = [&](const T *base, int64_t ld, int r) {
-            const int x = min(r0 + r, rows - 1), i = a.group.of(x);
-            return base + i * ld + (int64_t)(x - i * a.G) * a.D;
-        };
-        mq.load(to, tid, left, a.D, [&](int r) { return at(qb, a.ldq, r); });
-        md.load(to + Tl::kElems, tid, left, a.D, [&](int r) { return at(db, a.lddo, r); });
+        // (From the tile's first token on.)
+        const int i0 = a.group.of(r0);
+        const T *qt = qb + i0 * a.ldq, *dt = db + i0 * a.lddo;
+        if constexpr (DMA) {
+            auto at = [&](int64_t ld, int r) {
+                const int x = min(r0 + r, rows - 1), i = a.group.of(x);
+                return ((uint32_t)(i - i0) * (uint32_t)ld + (uint32_t)(x - i * a.G) * a.D) *
+                       (uint32_t)sizeof(T);
+            };
+            mq.direct(to, tid, qt, [&](int r) { return at(a.ldq, r); });
+            md.direct(to + Tl::kElems, tid, dt, [&](int r) { return at(a.lddo, r); });
+        } else {
+            auto at = [&](const T *base, int64_t ld, int r) {
+                const int x = min(r0 + r, rows - 1), i = a.group.of(x);
+                return base + (i - i0) * ld + (int64_t)(x - i * a.G) * a.D;
+            };
+            mq.fetch(tid, left, a.D, [&](int r) { return at(qt, a.ldq, r); });
+            md.fetch(tid, left, a.D, [&](int r) { return at(dt, a.lddo, r); });
+        }
     };
     auto store = [&](int t) {
         T *to = lds + (t & 1) * 2 * Tl::kElems;
         mq.store(to, tid);
         md.store(to + Tl::kElems, tid);
         const int what = tid / RT;
-        if (what < kStats) stats[t & 1][what][tid % RT] = sv;
+        if (what < kStats)
+            stats[t & 1][what][tid % RT] = what == 0 ? (kUpV - sv) * (kFold<DT> ? 1.0f / c : 1.0f)
+                                           : what == 1 ? -sv
+                                                       : sv;
     };
     const Lanes<DT, DP> L(lane);
     bool bad = false;  // a tile of rows that do not all see every key held an infinity or NaN
-    f32x16 dk[N][NB], dv[N][NB];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        clear(dk[i]);
-        clear(dv[i]);
-    }
+    f32x16 dk[NB], dv[NB];
+    clear(dk);
+    clear(dv);
     int up = 0;  // fp16: the power of two that dK carries
     bool any = false;
     const int t0 = first_of(n0) / RT, t1 = rows > 0 ? (rows - 1) / RT + 1 : 0;
     if (t0 < t1) {
+        Mover<DT, DP, kKeys, 256, DMA> mv;
+        mv.load(vlds, tid,
+                static_cast<const T *>(a.v) + (sq.k0 + n0) * a.ldv + (int64_t)w.kv * a.D, a.ldv,
+                sq.lk - n0, a.D);
+        mv.store(vlds, tid);
         load(t0);
         store(t0);
     }
@@ -1255,7 +1298,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
             if (!whole) bad |= !(Tl::finite(qt, lane) && Tl::finite(dt, lane));
             float fs = 1.0f;
             if constexpr (DT == kF16) {
-                float big = st[2 * RT + lane];
+                float big = st[2 * RT + l32];
 #pragma unroll
                 for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o));
                 const int e = __builtin_amdgcn_readfirstlane((int)kUpDs - exponent_above(big));
@@ -1263,118 +1306,86 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
                     if (any) {
                         const float f = pow2(e - up);
 #pragma unroll
-                        for (int i = 0; i < N; ++i)
+                        for (int b = 0; b < NB; ++b)
 #pragma unroll
-                            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                                for (int r = 0; r < 16; ++r) dk[i][b][r] *= f;
+                            for (int r = 0; r < 16; ++r) dk[b][r] *= f;
                     }
                     up = e;
                     any = true;
                 }
                 fs = pow2(up - (int)kUpP);
             }
+            f32x16 p = kFold<DT> ? rows16(st + 4 * h) : all16(0.0f);
+            f32x16 dp = kFold<DT> ? rows16(st + RT + 4 * h) : all16(0.0f);
 #pragma unroll
-            for (int b = 0; b < RT / 32; ++b) {
-                f32x16 p[N], dp[N];
+            for (int ks = 0; ks < NK; ++ks) p = Ty::mfma(Tl::by_row(qt, 0, ks, L), kf[ks], p);
 #pragma unroll
-                for (int i = 0; i < N; ++i) p[i] = dp[i] = zero16();
+            for (int ks = 0; ks < NK; ++ks)
+                dp = Ty::mfma(Tl::by_row(dt, 0, ks, L), Vt::by_row(vlds, wave, ks, L), dp);
+            if constexpr (kFold<DT>) {
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks) {
-                    const typename Ty::Frag f = Tl::by_row(qt, b, ks, L);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) p[i] = Ty::mfma(f, kf[i][ks], p[i]);
+                for (int r = 0; r < 16; ++r) {
+                    p[r] = __builtin_amdgcn_exp2f(p[r] * c);
+                    dp[r] = p[r] * (DT == kF16 ? dp[r] * fs : dp[r]);
                 }
+            } else {
+                const f32x16 lse = rows16(st + 4 * h), delta = rows16(st + RT + 4 * h);
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks) {
-                    const typename Ty::Frag f = Tl::by_row(dt, b, ks, L);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) dp[i] = Ty::mfma(f, vf[i][ks], dp[i]);
+                for (int r = 0; r < 16; ++r) {
+                    p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[r], c, lse[r]));
+                    dp[r] = p[r] * (dp[r] + delta[r]);
                 }
+            }
+            if (!whole) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int at = 32 * b + 8 * q + 4 * h;
-                    const f32x4 lse = *reinterpret_cast<const f32x4 *>(st + at);
-                    const f32x4 delta = *reinterpret_cast<const f32x4 *>(st + RT + at);
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int r = 4 * q + e;
-                            const float x = __builtin_amdgcn_exp2f(
-                                __builtin_fmaf(p[i][r], c, kUpV - lse[e]));
-                            const float y = dp[i][r] - delta[e];
-                            p[i][r] = x;
-                            dp[i][r] = x * (DT == kF16 ? y * fs : y);
-                        }
+                for (int r = 0; r < 16; ++r) {
+                    const int x = r0 + 8 * (r >> 2) + 4 * h + (r & 3);
+                    const bool on = x >= first && x < rows;
+                    p[r] = on ? p[r] : 0.0f;
+                    dp[r] = on ? dp[r] : 0.0f;
                 }
-                if (!whole) {
+            }
 #pragma unroll
-                    for (int i = 0; i < N; ++i)
+            for (int u = 0; u < 2; ++u) {
+                const typename Ty::Frag f = Ty::pack(p, u);
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int x = r0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
-                            const bool on = x >= first[i] && x < rows;
-                            p[i][r] = on ? p[i][r] : 0.0f;
-                            dp[i][r] = on ? dp[i][r] : 0.0f;
-                        }
-                }
+                for (int d = 0; d < NB; ++d)
+                    dv[d] = Ty::mfma(Tl::by_column(dt, 16 * u, d, L), f, dv[d]);
+            }
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    typename Ty::Frag w[N];
+            for (int u = 0; u < 2; ++u) {
+                const typename Ty::Frag f = Ty::pack(dp, u);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) w[i] = Ty::pack(p[i], u);
-#pragma unroll
-                    for (int d = 0; d < NB; ++d) {
-                        const typename Ty::Frag f = Tl::by_column(dt, 32 * b + 16 * u, d, L);
-#pragma unroll
-                        for (int i = 0; i < N; ++i) dv[i][d] = Ty::mfma(f, w[i], dv[i][d]);
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    typename Ty::Frag w[N];
-#pragma unroll
-                    for (int i = 0; i < N; ++i) w[i] = Ty::pack(dp[i], u);
-#pragma unroll
-                    for (int d = 0; d < NB; ++d) {
-                        const typename Ty::Frag f = Tl::by_column(qt, 32 * b + 16 * u, d, L);
-#pragma unroll
-                        for (int i = 0; i < N; ++i) dk[i][d] = Ty::mfma(f, w[i], dk[i][d]);
-                    }
-                }
+                for (int d = 0; d < NB; ++d)
+                    dk[d] = Ty::mfma(Tl::by_column(qt, 16 * u, d, L), f, dk[d]);
             }
         }
         if (t + 1 < t1) store(t + 1);
     }
     if (__syncthreads_or(bad)) {
-        careful_bwd_kv<DT>(a, sq, w.kv, n0, min(n0 + kWgKeys, sq.lk), wave, lane);
+        careful_bwd_kv<DT>(a, sq, w.kv, n0, min(n0 + kKeys, sq.lk), wave, lane);
         return;
     }
     const float fk = a.scale * pow2(-up), fv = pow2(-(int)kUpV);
     const int64_t col = (int64_t)w.kv * a.D;
+    if (key >= sq.lk) return;
+    T *pk = static_cast<T *>(a.dk) + (sq.k0 + key) * a.lddk + col;
+    T *pv = static_cast<T *>(a.dv) + (sq.k0 + key) * a.lddv + col;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int key = kw + 32 * i + l32;
-        if (key >= sq.lk) continue;
-        T *pk = static_cast<T *>(a.dk) + (sq.k0 + key) * a.lddk + col;
-        T *pv = static_cast<T *>(a.dv) + (sq.k0 + key) * a.lddv + col;
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int d = 32 * b + 8 * q + 4 * h;
-                const f32x16 &x = dk[i][b], &y = dv[i][b];
-                Ty::store4(pk, d, a.D,
-                           f32x4{x[4 * q] * fk, x[4 * q + 1] * fk, x[4 * q + 2] * fk,
-                                 x[4 * q + 3] * fk},
-                           a.accumulate);
-                Ty::store4(pv, d, a.D,
-                           f32x4{y[4 * q] * fv, y[4 * q + 1] * fv, y[4 * q + 2] * fv,
-                                 y[4 * q + 3] * fv},
-                           a.accumulate);
-            }
-    }
+        for (int q = 0; q < 4; ++q) {
+            const int d = 32 * b + 8 * q + 4 * h;
+            const f32x16 &x = dk[b], &y = dv[b];
+            Ty::store4(pk, d, a.D,
+                       f32x4{x[4 * q] * fk, x[4 * q + 1] * fk, x[4 * q + 2] * fk,
+                             x[4 * q + 3] * fk},
+                       a.accumulate);
+            Ty::store4(pv, d, a.D,
+                       f32x4{y[4 * q] * fv, y[4 * q + 1] * fv, y[4 * q + 2] * fv,
+                             y[4 * q + 3] * fv},
+                       a.accumulate);
+        }
 }
 
 // ------------------------------------------------------------------ launches
@@ -1407,9 +1418,8 @@ int combine(hipStream_t st, const Args &a) {
 template <int DT>
 int backward(hipStream_t st, const Args &a, bool dma) {
     with_width<DT>(a.D, dma, [&](auto dp, auto d) {
-        constexpr int N = kBlocks<DT>;
-        att_bwd_q<DT, dp(), d(), N><<<a.KV * a.slots, 256, 0, st>>>(a);
-        if (a.kslots) att_bwd_kv<DT, dp(), d(), N><<<a.KV * a.kslots, 256, 0, st>>>(a);
+        att_bwd_q<DT, dp(), d()><<<a.KV * a.slots, 256, 0, st>>>(a);
+        att_bwd_kv<DT, dp(), d()><<<a.KV * a.kslots, 256, 0, st>>>(a);
     });
     return (int)hipGetLastError();
 }

@@ -46,6 +46,19 @@ __device__ __forceinline__ void lds_dma16(const void *src, const void *lds_dst) 
                  : "memory");
 }
 
+// The same from base + offset bytes, base uniform across the wave.
+__device__ __forceinline__ void lds_dma16(const void *base, uint32_t offset, const void *lds_dst) {
+    // (A generic pointer into LDS has the LDS address in its low half.)
+    const uint32_t l = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds_dst);
+    const uintptr_t b = (uintptr_t)base;
+    const uintptr_t from =
+        (uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b) |
+        (uintptr_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32)) << 32;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset),
+                 "s"(from), "s"(l)
+                 : "memory");
+}
+
 // 4x4 transpose within each quad of lanes, for the GEMMs' register
 // epilogues: lane e (of its quad) holds x[q] = M[q][e]; returns M[e][0..3].
 // First an exchange with lane e^1 (DPP quad_perm [1,0,3,2]) that swaps the

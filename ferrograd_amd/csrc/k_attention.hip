@@ -33,8 +33,9 @@ int splits_of(int cus, const Args &a, bool few) {
 
 bool whole_chunks(const Args &a, std::initializer_list<std::pair<const void *, int64_t>> rows) {
     if (a.D != 64 && a.D != 128) return false;
+    // (And a tile's rows are within 32 bits of its first.)
     for (const auto &r : rows)
-        if (((uintptr_t)r.first & 15) || r.second % 8) return false;
+        if (((uintptr_t)r.first & 15) || r.second % 8 || r.second >= 1 << 24) return false;
     return true;
 }
 
@@ -57,7 +58,7 @@ int check(const char *who, int dtype, const Args &a, int heads, int kv_heads) {
                "%s: scale must be positive and finite", who);
     // Rows of a key head are counted in 32 bits, and a grid holds the slots.
     const int64_t slots = (int64_t)a.Tq * (heads / kv_heads) / fg::attn::kFewRows + a.n;
-    const int64_t kslots = (int64_t)a.Tk / fg::attn::kRows + a.n;
+    const int64_t kslots = (int64_t)a.Tk / fg::attn::kKeys + a.n;
     FG_REQUIRE((int64_t)a.Tq * (heads / kv_heads) < INT32_MAX - 256 && a.Tk < INT32_MAX - 256 &&
                    fg::rows::grid_holds(kv_heads * std::max(slots, kslots), 256),
                FG_ERR_OUT_OF_BOUNDS, "%s: %d sequences of %d rows and %d keys with %d heads", who,
@@ -191,10 +192,8 @@ FG_API int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, co
     a.rows = (float *)fg::workspace(ctx, fg::attention_bwd_ws_bytes(Tq, heads));
     if (!a.rows) return FG_ERR_OUT_OF_MEMORY;
     a.splits = 1;
-    const int per = 128 * (dtype == FG_DTYPE_F32 ? fg::attn::kBlocks<fg::kF32>
-                                                 : fg::attn::kBlocks<fg::kBF16>);
-    a.slots = (int)((int64_t)Tq * a.G / per + n);
-    a.kslots = Tk / per + n;
+    a.slots = (int)((int64_t)Tq * a.G / fg::attn::kRows + n);
+    a.kslots = Tk / fg::attn::kKeys + n;
     const bool dma = whole_chunks(a, {{d_q, ldq}, {d_k, ldk}, {d_v, ldv}, {d_dout, lddo}});
     auto launch = dtype == FG_DTYPE_F32    ? fg::attn::backward<fg::kF32>
                   : dtype == FG_DTYPE_BF16 ? fg::attn::backward<fg::kBF16>
