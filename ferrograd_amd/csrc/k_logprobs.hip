@@ -31,7 +31,7 @@ using fg::rows::u32x4;
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 constexpr int kMaxTop = 32;   // alternatives: at most the 64 groups of threads
-constexpr int kCands = 1024;  // candidates for them kept at once
+constexpr int kCands = 512;   // candidates for them kept at once
 
 // A number's place among a row's, as an unsigned integer: -0 as +0, NaN below all.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -52,16 +52,6 @@ struct Stats {
         s *= f;
         m = to;
     }
-    __device__ __forceinline__ void join(float m2, float s2, float w2) {
-        Stats o;
-        o.m = m2;
-        o.s = s2;
-        o.w = w2;
-        raise(m2);
-        o.raise(m);
-        s += o.s;
-        w += o.w;
-    }
     // A value, with from = m (0 before the first number).  exp2 of -inf is 0, and so is
     // that value's share of w; NaN goes into s.
     __device__ __forceinline__ void add(float x, float c, float from) {
@@ -72,6 +62,31 @@ struct Stats {
     __device__ __forceinline__ float from() const { return m == -INFINITY ? 0.0f : m; }
 };
 
+// Largest over a wave's 64 lanes (all active), the same in every lane, NaN left out.
+__device__ __forceinline__ float wave_max(float v) {
+    using namespace fg::smrow;
+    v = fmaxf(v, dpp_f<kDppSwap1>(v));
+    v = fmaxf(v, dpp_f<kDppSwap2>(v));
+    v = fmaxf(v, dpp_f<kDppHalfMirror>(v));
+    v = fmaxf(v, dpp_f<kDppMirror>(v));
+    auto of = [&](int lane) {
+        return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+    };
+    return fmaxf(fmaxf(of(0), of(16)), fmaxf(of(32), of(48)));
+}
+// A value's place among a row's and its column as one number: larger is earlier.
+__device__ __forceinline__ uint64_t place_of(uint32_t key, int col) {
+    return (uint64_t)key << 32 | (uint32_t)~col;
+}
+__device__ __forceinline__ int col_of(uint64_t place) { return (int)~(uint32_t)place; }
+// How many of `all` come before v.
+__device__ __forceinline__ int before_in(const uint64_t *all, int n, uint64_t v) {
+    int before = 0;
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) before += all[k] > v;
+    return before;
+}
+
 struct Fwd {
     const void *x;
     const uint32_t *tokens;
@@ -80,30 +95,61 @@ struct Fwd {
     float *tops;
     float scale;
     int ldx, C, K;
+    // Rows in splits of their columns: [R][splits] of three statistics, and of K places
+    // (place_of) in order.
+    int splits;
+    float *stats;
+    uint64_t *best;
 };
 
-// A row a workgroup of NT threads, read once; for the alternatives the threads that
-// hold one (about as many as there are) read their own chunks again.
+// A row's answers from its statistics, in thread 0.
+__device__ __forceinline__ void write_answers(const Fwd &a, size_t r, const Stats &st, float log_s,
+                                              float xt, bool inside, float c) {
+    if (a.logp)
+        a.logp[r] = inside ? __builtin_fmaf(xt, c, -st.m) * kLn2 - log_s : __builtin_nanf("");
+    if (a.entropy) a.entropy[r] = log_s - kLn2 * (st.w / st.s);
+    if (a.lse) a.lse[r] = __builtin_fmaf(st.m, kLn2, log_s);
+}
+// The alternative at `place`: its column and log probability.
+template <int DT>
+__device__ __forceinline__ void write_top(const Fwd &a, size_t r, int place, int col,
+                                          const typename Io<DT>::T *x, const Stats &st,
+                                          float log_s, float c) {
+    if (a.ids) a.ids[r * a.K + place] = (uint32_t)col;
+    if (a.tops)
+        a.tops[r * a.K + place] =
+            __builtin_fmaf(Io<DT>::load1(x, col), c, -st.m) * kLn2 - log_s;
+}
+
+// A row (or a split of its columns) a workgroup of NT threads, read once; for the
+// alternatives the chunks of the threads that hold one (about as many as there are) are
+// read again, by all threads.
 //   The K-th largest of the maxima of 64 groups of threads is no more than the row's
 // K-th largest value, so every alternative is among the values from it on: about as
 // many as K where the large values lie anyhow.  Where they are more than fit (rows of
 // few different values), the K are taken one after the other, a pass over the row each.
 template <int DT, int NT>
-__global__ __launch_bounds__(NT) void logprobs_fwd(const Fwd a) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void logprobs_fwd(
+    const Fwd a) {
     using IO = Io<DT>;
     constexpr int E = IO::E, NW = NT / 64, kDeep = 4;
     __shared__ float sm[NW][3];
-    __shared__ uint32_t keys[kCands];
-    __shared__ int cols[kCands];
+    __shared__ uint32_t keys[NT];
+    __shared__ uint64_t cand[kCands];
+    __shared__ int hot[NT];
     __shared__ uint32_t bound_s;
-    __shared__ int count_s;
+    __shared__ int count_s, hot_s;
     const size_t r = blockIdx.x;
+    const int split = blockIdx.y;
     const auto *x = static_cast<const typename IO::T *>(a.x) + r * a.ldx;
-    const int t = threadIdx.x, nb = a.C / E;
+    const int t = threadIdx.x, whole = a.C / E;
+    const int j0 = (int)((int64_t)whole * split / a.splits);
+    const int nb = (int)((int64_t)whole * (split + 1) / a.splits);
     const float c = a.scale * kLog2e;
-    const int single = t < a.C - nb * E ? nb * E + t : -1;
+    const int single = split == a.splits - 1 && t < a.C - whole * E ? whole * E + t : -1;
     const uint32_t token = a.tokens[r];
-    const float xt = token < (uint32_t)a.C ? IO::load1(x, (int)token) : 0.0f;
+    const bool inside = token < (uint32_t)a.C;
+    const float xt = inside ? IO::load1(x, (int)token) : 0.0f;
     Stats st;
     float big = -INFINITY;  // the thread's largest value
     auto take = [&](u32x4 w) {
@@ -118,7 +164,7 @@ __global__ __launch_bounds__(NT) void logprobs_fwd(const Fwd a) {
 #pragma unroll
         for (int e = 0; e < E; ++e) st.add(IO::get(w, e), c, from);
     };
-    int j = t;
+    int j = j0 + t;
     for (; j + (kDeep - 1) * NT < nb; j += kDeep * NT) {
         u32x4 w[kDeep];
 #pragma unroll
@@ -133,44 +179,30 @@ __global__ __launch_bounds__(NT) void logprobs_fwd(const Fwd a) {
         st.add(v, c, st.from());
         big = fmaxf(big, v);
     }
-    st.raise(big * c);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        st.join(__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.w, o));
-    if (NW > 1) {
-        if ((t & 63) == 0) {
-            sm[t >> 6][0] = st.m;
-            sm[t >> 6][1] = st.s;
-            sm[t >> 6][2] = st.w;
-        }
-    }
     // (0: no number among the thread's values, or nothing above -inf.)
     const uint32_t mine = big > -INFINITY ? order_key(big) : 0u;
+    const float top = wave_max(big * c);
+    if ((t & 63) == 0) sm[t >> 6][0] = top;
     if (a.K) {
         keys[t] = mine;
-        if (t == 0) count_s = 0;
+        if (t == 0) count_s = hot_s = 0;
     }
-    if (NW > 1 || a.K) __syncthreads();
-    if (NW > 1) {
-        st.m = sm[0][0];
-        st.s = sm[0][1];
-        st.w = sm[0][2];
-        for (int k = 1; k < NW; ++k) st.join(sm[k][0], sm[k][1], sm[k][2]);
+    __syncthreads();
+    float m = sm[0][0];
+#pragma unroll
+    for (int k = 1; k < NW; ++k) m = fmaxf(m, sm[k][0]);
+    st.raise(m);
+    const float s = fg::rows::wave_sum(st.s), w = fg::rows::wave_sum(st.w);
+    if ((t & 63) == 0) {
+        sm[t >> 6][1] = s;
+        sm[t >> 6][2] = w;
     }
-    const float log_s = logf(st.s);
-    if (t == 0) {
-        if (a.logp)
-            a.logp[r] = token < (uint32_t)a.C ? __builtin_fmaf(xt, c, -st.m) * kLn2 - log_s
-                                              : __builtin_nanf("");
-        if (a.entropy) a.entropy[r] = log_s - kLn2 * (st.w / st.s);
-        if (a.lse) a.lse[r] = __builtin_fmaf(st.m, kLn2, log_s);
-    }
-    if (!a.K) return;
-    if (t < 64) {
+    if (a.K && t < 64) {
         uint32_t g = keys[t];
+#pragma unroll
         for (int k = 1; k < NW; ++k) g = max(g, keys[k * 64 + t]);
         int before = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (int k = 0; k < 64; ++k) {
             const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)g, k);
             before += o > g || (o == g && k < t);
@@ -178,67 +210,129 @@ __global__ __launch_bounds__(NT) void logprobs_fwd(const Fwd a) {
         if (before == a.K - 1) bound_s = g;
     }
     __syncthreads();
-    const uint32_t bound = bound_s;
-    auto each = [&](auto f) {  // every (key, column, value) of the thread's
-        for (int i = t; i < nb; i += NT) {
-            const u32x4 w = fg::rows::load<DT>(x, i);
+    st.m = m;
+    st.s = sm[0][1];
+    st.w = sm[0][2];
 #pragma unroll
-            for (int e = 0; e < E; ++e) f(order_key(IO::get(w, e)), i * E + e);
+    for (int k = 1; k < NW; ++k) {
+        st.s += sm[k][1];
+        st.w += sm[k][2];
+    }
+    const float log_s = logf(st.s);
+    const size_t part = r * a.splits + split;
+    if (t == 0) {
+        if (a.splits > 1) {
+            a.stats[3 * part] = st.m;
+            a.stats[3 * part + 1] = st.s;
+            a.stats[3 * part + 2] = st.w;
+        } else {
+            write_answers(a, r, st, log_s, xt, inside, c);
         }
-        if (single >= 0) f(order_key(IO::load1(x, single)), single);
+    }
+    if (!a.K) return;
+    const uint32_t bound = bound_s;
+    auto keep = [&](uint32_t key, int col) {
+        if (key < bound) return;
+        const int at = atomicAdd(&count_s, 1);
+        if (at < kCands) cand[at] = place_of(key, col);
     };
-    auto write = [&](int place, int col) {
-        if (a.ids) a.ids[r * a.K + place] = (uint32_t)col;
-        if (a.tops)
-            a.tops[r * a.K + place] = __builtin_fmaf(IO::load1(x, col), c, -st.m) * kLn2 - log_s;
-    };
-    if (mine >= bound)
-        each([&](uint32_t key, int col) {
-            if (key < bound) return;
-            const int at = atomicAdd(&count_s, 1);
-            if (at < kCands) {
-                keys[at] = key;
-                cols[at] = col;
-            }
-        });
+    if (mine >= bound) hot[atomicAdd(&hot_s, 1)] = t;
+    if (single >= 0) keep(order_key(IO::load1(x, single)), single);
     __syncthreads();
+    const int per = nb > j0 ? (nb - j0 - 1) / NT + 1 : 0;  // chunks of a thread, at most
+    for (int i = t; i < hot_s * per; i += NT) {
+        const int k = i / per, at = j0 + hot[k] + (i - k * per) * NT;
+        if (at >= nb) continue;
+        const u32x4 v = fg::rows::load<DT>(x, at);
+#pragma unroll
+        for (int e = 0; e < E; ++e) keep(order_key(IO::get(v, e)), at * E + e);
+    }
+    __syncthreads();
+    auto write = [&](int at, uint64_t place) {
+        if (a.splits > 1) a.best[part * a.K + at] = place;
+        else write_top<DT>(a, r, at, col_of(place), x, st, log_s, c);
+    };
     const int n = count_s;
     if (n >= a.K && n <= kCands) {
-        // Each at the place that as many come before it.
         for (int i = t; i < n; i += NT) {
-            const uint32_t key = keys[i];
-            const int col = cols[i];
-            int before = 0;
-            for (int k = 0; k < n; ++k)
-                before += keys[k] > key || (keys[k] == key && cols[k] < col);
-            if (before < a.K) write(before, col);
+            const uint64_t v = cand[i];
+            const int before = before_in(cand, n, v);
+            if (before < a.K) write(before, v);
         }
         return;
     }
-    uint64_t last = ~0ull;  // (key, ~column) of the one before
+    uint64_t last = ~0ull;  // the place of the one before
     for (int k = 0; k < a.K; ++k) {
-        uint64_t best = 0;
-        each([&](uint32_t key, int col) {
-            const uint64_t v = (uint64_t)key << 32 | (uint32_t)~col;
-            if (v < last) best = max(best, v);
-        });
+        uint64_t next = 0;
+        auto see = [&](uint32_t key, int col) {
+            const uint64_t v = place_of(key, col);
+            if (v < last) next = max(next, v);
+        };
+        for (int i = j0 + t; i < nb; i += NT) {
+            const u32x4 v = fg::rows::load<DT>(x, i);
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t other = (uint64_t)__shfl_xor((long long)best, o);
-            best = max(best, other);
+            for (int e = 0; e < E; ++e) see(order_key(IO::get(v, e)), i * E + e);
         }
+        if (single >= 0) see(order_key(IO::load1(x, single)), single);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) next = max(next, (uint64_t)__shfl_xor((long long)next, o));
         __syncthreads();
-        if ((t & 63) == 0) {
-            keys[t >> 6] = (uint32_t)(best >> 32);
-            cols[t >> 6] = (int)(uint32_t)best;
-        }
+        if ((t & 63) == 0) cand[t >> 6] = next;
         __syncthreads();
-        for (int q = 0; q < NW; ++q) {
-            const uint64_t v = (uint64_t)keys[q] << 32 | (uint32_t)cols[q];
-            best = max(best, v);
-        }
-        last = best;
-        if (t == 0) write(k, (int)~(uint32_t)best);
+#pragma unroll
+        for (int q = 0; q < NW; ++q) next = max(next, cand[q]);
+        last = next;
+        if (t == 0) write(k, next);
+    }
+}
+
+// A row's splits joined, their numbers all loaded at once: the statistics, and of the
+// alternatives those from the largest of the splits' K-th on.
+constexpr int kMaxSplits = 16, kJoinNT = 256;
+template <int DT>
+__global__ __launch_bounds__(kJoinNT) void logprobs_join(const Fwd a) {
+    constexpr int kPer = kMaxSplits * kMaxTop / kJoinNT;
+    __shared__ uint64_t cand[kMaxSplits * kMaxTop];
+    __shared__ int count_s;
+    const size_t r = blockIdx.x;
+    const auto *x = static_cast<const typename Io<DT>::T *>(a.x) + r * a.ldx;
+    const int t = threadIdx.x, lane = t & 63, all = a.splits * a.K;
+    const float c = a.scale * kLog2e;
+    const uint64_t *best = a.best + r * all;
+    const bool on = lane < a.splits;
+    const float *p = a.stats + 3 * (r * a.splits + (on ? lane : 0));
+    Stats st;
+    st.m = on ? p[0] : -INFINITY;
+    st.s = on ? p[1] : 0.0f;
+    st.w = on ? p[2] : 0.0f;
+    uint64_t mine[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        mine[i] = t + i * kJoinNT < all ? best[t + i * kJoinNT] : 0;
+    uint64_t bound = on && a.K ? best[lane * a.K + a.K - 1] : 0;
+    const uint32_t token = a.tokens[r];
+    const bool inside = token < (uint32_t)a.C;
+    const float xt = inside ? Io<DT>::load1(x, (int)token) : 0.0f;
+    if (t == 0) count_s = 0;
+    st.raise(wave_max(st.m));
+    st.s = fg::rows::wave_sum(st.s);
+    st.w = fg::rows::wave_sum(st.w);
+    st.m = wave_max(st.m);
+    const float log_s = logf(st.s);
+    if (t == 0) write_answers(a, r, st, log_s, xt, inside, c);
+    if (!a.K) return;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) bound = max(bound, (uint64_t)__shfl_xor((long long)bound, o));
+    bound = (uint64_t)__shfl((long long)bound, 0);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (t + i * kJoinNT < all && mine[i] >= bound) cand[atomicAdd(&count_s, 1)] = mine[i];
+    __syncthreads();
+    const int n = count_s;
+    for (int i = t; i < n; i += kJoinNT) {
+        const int before = before_in(cand, n, cand[i]);
+        if (before < a.K) write_top<DT>(a, r, before, col_of(cand[i]), x, st, log_s, c);
     }
 }
 
@@ -312,13 +406,18 @@ __global__ __launch_bounds__(kBwdNT) void logprobs_bwd(const Bwd a) {
     if (single >= 0) IO::store1(dx, single, grad(IO::load1(x, single), token == (uint32_t)single));
 }
 
+// Splits of each row's columns: of few long rows, as many as give every CU two
+// workgroups, of at least 8192 columns.
+int splits_of(int cus, int R, int C) {
+    return std::max(1, std::min({2 * cus / R, C / 8192, kMaxSplits}));
+}
+
 template <int DT>
 void launch_fwd(hipStream_t st, int R, const Fwd &a) {
-    // A wave a row up to 2 chunks a lane, then four waves, then sixteen.
-    const int chunks = a.C / Io<DT>::E;
-    if (chunks <= 128) logprobs_fwd<DT, 64><<<R, 64, 0, st>>>(a);
-    else if (chunks <= 2048) logprobs_fwd<DT, 256><<<R, 256, 0, st>>>(a);
-    else logprobs_fwd<DT, 1024><<<R, 1024, 0, st>>>(a);
+    // A wave a row up to 2 chunks a lane, else four waves.
+    if (a.C / Io<DT>::E <= 128) logprobs_fwd<DT, 64><<<R, 64, 0, st>>>(a);
+    else logprobs_fwd<DT, 256><<<dim3(R, a.splits), 256, 0, st>>>(a);
+    if (a.splits > 1) logprobs_join<DT><<<R, 256, 0, st>>>(a);
 }
 
 template <int DT>
@@ -365,8 +464,14 @@ FG_API int fg_token_logprobs(fg_ctx *ctx, int dtype, const void *d_logits, int l
                FG_ERR_INVALID_ARGUMENT, "%s: an output is another output or an input", who);
     if (R == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
-    const Fwd a{d_logits, d_tokens, d_logp, d_entropy, d_lse, d_top_ids, d_top_logp, scale,
-                ldx, C, top};
+    Fwd a{d_logits, d_tokens, d_logp, d_entropy, d_lse, d_top_ids, d_top_logp, scale,
+          ldx, C, top, splits_of(ctx->cu_count, R, C), nullptr, nullptr};
+    if (a.splits > 1) {
+        const uint64_t parts = (uint64_t)R * a.splits;
+        a.best = (uint64_t *)fg::workspace(ctx, parts * (top * sizeof(uint64_t) + 3 * sizeof(float)));
+        if (!a.best) return FG_ERR_OUT_OF_MEMORY;
+        a.stats = (float *)(a.best + parts * top);
+    }
     if (dtype == FG_DTYPE_F32) launch_fwd<fg::kF32>(ctx->stream, R, a);
     else if (dtype == FG_DTYPE_BF16) launch_fwd<fg::kBF16>(ctx->stream, R, a);
     else launch_fwd<fg::kF16>(ctx->stream, R, a);

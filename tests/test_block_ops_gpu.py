@@ -251,21 +251,22 @@ def test_logprobs(gpu_ctx, dt, R, C, scale, pad, start):
     within(tops, tl, b[:, None] + U * (4 * tl.abs() + 8))
 
 
-def test_logprobs_masked_ties_and_nan(gpu_ctx):
+@pytest.mark.parametrize("C", [3001, 40003])
+def test_logprobs_masked_ties_and_nan(gpu_ctx, C):
     """Masked logits (-inf, or the type's lowest number), rows of one value, tokens
     outside the vocabulary, NaN in one row alone."""
     for dt in ("bf16", "f32"):
-        x = rand((8, 3001), dt, 22, 2.0)
+        x = rand((8, C), dt, 22, 2.0)
         low = torch.finfo(DTS[dt][1]).min
         x[0, 5:] = -math.inf                       # five left
         x[1, ::2] = low
         x[2] = 0.25                                # every one an alternative
         x[3] = torch.where(x[3] > 0, 1.0, 0.0)     # two values
         x[4, 1:] = -math.inf                       # one left: certain
-        x[5, 3000] = 80.0
+        x[5, C - 1] = 80.0
         x[6, :] = -math.inf
-        x[6, 2999:] = 0.0                          # the two past the last chunk's boundary
-        tok = torch.tensor([3, 1, 3000, 7, 0, 3000, 3000, 3001])
+        x[6, C - 2:] = 0.0                          # the two past the last chunk's boundary
+        tok = torch.tensor([3, 1, C - 1, 7, 0, C - 1, C - 1, C])
         want = lp_oracle(x, tok, 1.0)
         got, ids, tops = run_lp(gpu_ctx, x, tok, dt, 32, 1.0)
         for g, (w, b) in zip(got, want):
