@@ -46,7 +46,8 @@ struct Args {
     int64_t lddo, lddq, lddk, lddv;
     void *dq, *dk, *dv;
     float *rows;   // [3][KV Tq G]: log2 of the sum, delta, the largest |dout|
-    int kslots, accumulate;
+    float *kpart;  // ksplits > 1: dK's and dV's sums, [2][ksplits][KV Tk][D] (dQ's: part)
+    int kslots, ksplits, accumulate;
 };
 
 // Rows of a workgroup (of the few rows' one), and keys of one in the backward's pass over

@@ -55,14 +55,16 @@ constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
 // Bits of a chunk's place that its row sets, and the chunks left free before a row: one
 // every 4 rows, of 8 chunks (128 bytes) two every 8, so that what a wave's direct load
-// writes, 1 KiB, is of one piece.
+// writes, 1 KiB, is of one piece.  Rows of 96 elements, which no direct load brings: one a
+// row.
 template <int CH>
 __device__ __forceinline__ int swz(int row) {
+    if (CH == 12 || CH == 24) return 0;
     return CH == 8 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 1) : (row & 3) << 2;
 }
 template <int CH>
 __device__ __forceinline__ constexpr int gap(int row) {
-    return CH == 8 ? (row >> 3) * 2 : row >> 2;
+    return CH == 12 || CH == 24 ? row : CH == 8 ? (row >> 3) * 2 : row >> 2;
 }
 
 template <int DT>
@@ -197,7 +199,7 @@ struct Lanes {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (kWide) {
-                row[i] = place(l32, 4 * i + 2 * h);
+                row[i] = place(l32, (4 * i + 2 * h) % CH);
                 col[i] = place(4 * h + i, l32 >> 2) + (l32 & 3);
                 col[4 + i] = place(4 * h + i, 8 + (l32 >> 2)) + (l32 & 3);
             } else {
@@ -297,9 +299,9 @@ struct Mover {
     using Tl = Tile<DT, DP, ROWS>;
     using T = typename Tl::T;
     static constexpr int E = Tl::E, CH = Tl::CH;
-    static constexpr int kPer = Tl::kChunks / NT;
+    static constexpr int kPer = (Tl::kChunks + NT - 1) / NT;
     static constexpr int kLoadRows = 64 / CH;  // rows of a wave load: of one swizzle
-    static_assert(Tl::kChunks % NT == 0, "whole chunks a thread");
+    static_assert(!DMA || Tl::kChunks % NT == 0, "whole chunks a thread");
     u32x4 v[DMA ? 1 : kPer];
 
     // DMA: row r at offset_of(r) bytes from the (uniform) base.
@@ -319,6 +321,7 @@ struct Mover {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int pos = i * NT + tid, row = pos / CH, d = (pos % CH) * E;
+            if (Tl::kChunks % NT && row >= ROWS) break;
             const T *p = row_at(row) + d;
             if (row < rows && d + E <= D) {
                 v[i] = *reinterpret_cast<const u32x4_any *>(p);
@@ -358,6 +361,7 @@ struct Mover {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int pos = i * NT + tid, row = pos / CH, c = pos % CH;
+                if (Tl::kChunks % NT && row >= ROWS) break;
                 *reinterpret_cast<u32x4 *>(lds + Lanes<DT, DP>::place(row, c)) = v[i];
             }
         }
@@ -961,25 +965,52 @@ constexpr bool kFold = DT != kF32;
 constexpr float kUpDs = 4.0f;  // its power above 1 / the largest |dout|
 constexpr float kUpP = 8.0f;   // fp16: the probabilities' that dV is summed from
 
+// A gradient's row: where it goes, or, in splits, to split blockIdx.y's fp32 rows of
+// `part`, `rows` of them, at place `at`.
+template <int DT, int DP>
+__device__ __forceinline__ void put_grad(const Args &a, float *part, int64_t rows, int64_t at,
+                                         int splits, typename Type<DT>::T *to,
+                                         const f32x16 (&x)[DP / 32], float f, int h) {
+    auto each = [&](auto put) {
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                put(32 * b + 8 * q + 4 * h, f32x4{x[b][4 * q] * f, x[b][4 * q + 1] * f,
+                                                  x[b][4 * q + 2] * f, x[b][4 * q + 3] * f});
+    };
+    if (splits > 1) {
+        float *p = part + (blockIdx.y * rows + at) * a.D;
+        each([&](int d, f32x4 v) { Type<kF32>::store4(p, d, a.D, v, false); });
+    } else {
+        each([&](int d, f32x4 v) { Type<DT>::store4(to, d, a.D, v, a.accumulate); });
+    }
+}
+
 // dQ of rows row0 .. row1 - 1, and dK and dV of keys key0 .. key1 - 1, carefully.
 template <int DT>
-__device__ void careful_bwd_q(const Args &a, const Seq &sq, int kv, int row0, int row1, int wave,
-                              int lane) {
+__device__ void careful_bwd_q(const Args &a, const Seq &sq, int kv, int row0, int row1, int key0,
+                              int key1, int wave, int lane) {
     using T = typename Type<DT>::T;
     const float c = a.scale * kLog2e;
     const T *k = static_cast<const T *>(a.k) + sq.k0 * a.ldk + (int64_t)kv * a.D;
     const T *v = static_cast<const T *>(a.v) + sq.k0 * a.ldv + (int64_t)kv * a.D;
-    const int64_t n = (int64_t)a.KV * a.Tq * a.G;
-    const float *stats = a.rows + (int64_t)kv * a.Tq * a.G + sq.q0 * a.G;
     for (int row = row0 + wave; row < row1; row += 4) {
         const int i = a.group.of(row), head = kv * a.G + row - i * a.G, token = sq.q0 + i;
-        const int end = min(sq.lk, a.causal ? i + sq.lk - sq.lq + 1 : sq.lk);
+        const int end = min(min(key1, sq.lk), a.causal ? i + sq.lk - sq.lq + 1 : sq.lk);
         const int64_t col = (int64_t)head * a.D;
         const T *q = static_cast<const T *>(a.q) + token * a.ldq + col;
         const T *dout = static_cast<const T *>(a.dout) + token * a.lddo + col;
-        const float lse2 = stats[row], delta = stats[n + row];
+        // (Not from a.rows, which another split's workgroup may be writing.)
+        const float lse = a.lse[(int64_t)head * a.Tq + token];
+        const float lse2 = lse * kLog2e;
+        const T *out = static_cast<const T *>(a.out) + token * a.ldo + col;
+        float delta = 0.0f;
+        for (int d = lane; d < a.D; d += 64)
+            delta += Type<DT>::load1(dout + d) * Type<DT>::load1(out + d);
+        delta = wave_add(delta);
         float acc[2] = {0.0f, 0.0f};
-        for (int j0 = 0; j0 < end; j0 += 64) {
+        for (int j0 = key0; j0 < end; j0 += 64) {
             const int j = j0 + lane;
             const float x = dot<DT>(q, k + j * a.ldk, a.D, j < end);
             const float dp = dot<DT>(dout, v + j * a.ldv, a.D, j < end);
@@ -987,16 +1018,21 @@ __device__ void careful_bwd_q(const Args &a, const Seq &sq, int kv, int row0, in
             for (int e = 0; e < min(64, end - j0); ++e)
                 add_row<DT>(acc, __shfl(ds, e), k + (j0 + e) * a.ldk, a.D, lane);
         }
-        put_row<DT>(static_cast<T *>(a.dq) + token * a.lddq + col, acc, a.scale, a.D, lane,
-                    a.accumulate);
+        const int64_t rows = (int64_t)a.KV * a.Tq * a.G;
+        const int64_t at = (int64_t)kv * a.Tq * a.G + sq.q0 * a.G + row;
+        if (a.splits > 1)
+            put_row<kF32>(a.part + (blockIdx.y * rows + at) * a.D, acc, a.scale, a.D, lane, false);
+        else
+            put_row<DT>(static_cast<T *>(a.dq) + token * a.lddq + col, acc, a.scale, a.D, lane,
+                        a.accumulate);
     }
 }
 template <int DT>
-__device__ void careful_bwd_kv(const Args &a, const Seq &sq, int kv, int key0, int key1, int wave,
-                               int lane) {
+__device__ void careful_bwd_kv(const Args &a, const Seq &sq, int kv, int key0, int key1, int row0,
+                               int row1, int wave, int lane) {
     using T = typename Type<DT>::T;
     const float c = a.scale * kLog2e;
-    const int rows = sq.lq * a.G, off = sq.lk - sq.lq;
+    const int rows = min(row1, sq.lq * a.G), off = sq.lk - sq.lq;
     const T *q = static_cast<const T *>(a.q) + sq.q0 * a.ldq + (int64_t)kv * a.G * a.D;
     const T *dout = static_cast<const T *>(a.dout) + sq.q0 * a.lddo + (int64_t)kv * a.G * a.D;
     const int64_t n = (int64_t)a.KV * a.Tq * a.G, col = (int64_t)kv * a.D;
@@ -1009,7 +1045,7 @@ __device__ void careful_bwd_kv(const Args &a, const Seq &sq, int kv, int key0, i
         const T *k = static_cast<const T *>(a.k) + (sq.k0 + key) * a.ldk + col;
         const T *v = static_cast<const T *>(a.v) + (sq.k0 + key) * a.ldv + col;
         float dk[2] = {0.0f, 0.0f}, dv[2] = {0.0f, 0.0f};
-        for (int r0 = a.causal ? max(0, key - off) * a.G : 0; r0 < rows; r0 += 64) {
+        for (int r0 = max(row0, a.causal ? max(0, key - off) * a.G : 0); r0 < rows; r0 += 64) {
             const int row = min(r0 + lane, rows - 1);
             const bool on = r0 + lane < rows;
             const float x = dot<DT>(k, at(q, a.ldq, row), a.D, on);
@@ -1020,6 +1056,13 @@ __device__ void careful_bwd_kv(const Args &a, const Seq &sq, int kv, int key0, i
                 add_row<DT>(dk, __shfl(ds, e), at(q, a.ldq, r0 + e), a.D, lane);
                 add_row<DT>(dv, __shfl(p, e), at(dout, a.lddo, r0 + e), a.D, lane);
             }
+        }
+        if (a.ksplits > 1) {
+            const int64_t keys = (int64_t)a.KV * a.Tk;
+            const int64_t at = blockIdx.y * keys + (int64_t)kv * a.Tk + sq.k0 + key;
+            put_row<kF32>(a.kpart + at * a.D, dk, a.scale, a.D, lane, false);
+            put_row<kF32>(a.kpart + (a.ksplits * keys + at) * a.D, dv, 1.0f, a.D, lane, false);
+            continue;
         }
         put_row<DT>(static_cast<T *>(a.dk) + (sq.k0 + key) * a.lddk + col, dk, a.scale, a.D, lane,
                     a.accumulate);
@@ -1058,6 +1101,8 @@ att_bwd_q(const Args a) {
     const int wave_last = w0 < rows ? last_of(min(w0 + 32, rows) - 1) : -1;
     const int keys = last_of(min(m0 + kRows, rows) - 1) + 1;
     const int tiles = keys > 0 ? (keys - 1) / KT + 1 : 0;
+    const int t0 = (int)((int64_t)tiles * blockIdx.y / a.splits);
+    const int t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / a.splits);
 
     typename Ty::Frag q[NK], dout[NK];
     const int row = w0 + l32;
@@ -1090,7 +1135,7 @@ att_bwd_q(const Args a) {
         const float x = a.lse[(int64_t)head * a.Tq + token];
         lse2 = x == -INFINITY ? INFINITY : x * kLog2e;
         if (x == -INFINITY) delta = 0.0f;
-        if (h == 0) {
+        if (h == 0 && blockIdx.y == 0) {
             const int64_t n = (int64_t)a.KV * a.Tq * a.G;
             const int64_t at = (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G + row;
             a.rows[at] = lse2;
@@ -1118,14 +1163,14 @@ att_bwd_q(const Args a) {
     bool bad = false;  // a tile of keys not all visible held an infinity or NaN
     f32x16 dq[NB];
     clear(dq);
-    if (tiles > 0) {
-        load(0);
-        store(0);
+    if (t0 < t1) {
+        load(t0);
+        store(t0);
     }
-    for (int t = 0; t < tiles; ++t) {
+    for (int t = t0; t < t1; ++t) {
         if constexpr (DMA) landed();
         else __syncthreads();
-        if (t + 1 < tiles) load(t + 1);
+        if (t + 1 < t1) load(t + 1);
         const int key0 = t * KT;
         const T *kt = lds + (t & 1) * 2 * Tl::kElems, *vt = kt + Tl::kElems;
         if (key0 <= wave_last) {
@@ -1164,23 +1209,17 @@ att_bwd_q(const Args a) {
                 }
             }
         }
-        if (t + 1 < tiles) store(t + 1);
+        if (t + 1 < t1) store(t + 1);
     }
     if (__syncthreads_or(bad)) {
-        careful_bwd_q<DT>(a, sq, w.kv, m0, min(m0 + kRows, rows), wave, lane);
+        careful_bwd_q<DT>(a, sq, w.kv, m0, min(m0 + kRows, rows), t0 * KT, t1 * KT, wave, lane);
         return;
     }
     if (row >= rows) return;
-    const float f = a.scale * pow2(-up);
-    T *p = static_cast<T *>(a.dq) + token * a.lddq + (int64_t)head * a.D;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int qd = 0; qd < 4; ++qd)
-            Ty::store4(p, 32 * b + 8 * qd + 4 * h, a.D,
-                       f32x4{dq[b][4 * qd] * f, dq[b][4 * qd + 1] * f, dq[b][4 * qd + 2] * f,
-                             dq[b][4 * qd + 3] * f},
-                       a.accumulate);
+    put_grad<DT, DP>(a, a.part, (int64_t)a.KV * a.Tq * a.G,
+                     (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G + row, a.splits,
+                     static_cast<T *>(a.dq) + token * a.lddq + (int64_t)head * a.D, dq,
+                     a.scale * pow2(-up), h);
 }
 
 // dK and dV, 32 keys a wave (a key a lane, both halves), over the rows that see them: of
@@ -1276,7 +1315,9 @@ att_bwd_kv(const Args a) {
     clear(dv);
     int up = 0;  // fp16: the power of two that dK carries
     bool any = false;
-    const int t0 = first_of(n0) / RT, t1 = rows > 0 ? (rows - 1) / RT + 1 : 0;
+    const int begin = first_of(n0) / RT, tiles = rows > 0 ? (rows - 1) / RT + 1 - begin : 0;
+    const int t0 = begin + (int)((int64_t)max(tiles, 0) * blockIdx.y / a.ksplits);
+    const int t1 = begin + (int)((int64_t)max(tiles, 0) * (blockIdx.y + 1) / a.ksplits);
     if (t0 < t1) {
         Mover<DT, DP, kKeys, 256, DMA> mv;
         mv.load(vlds, tid,
@@ -1363,29 +1404,68 @@ att_bwd_kv(const Args a) {
         if (t + 1 < t1) store(t + 1);
     }
     if (__syncthreads_or(bad)) {
-        careful_bwd_kv<DT>(a, sq, w.kv, n0, min(n0 + kKeys, sq.lk), wave, lane);
+        careful_bwd_kv<DT>(a, sq, w.kv, n0, min(n0 + kKeys, sq.lk), t0 * RT, t1 * RT, wave, lane);
         return;
     }
-    const float fk = a.scale * pow2(-up), fv = pow2(-(int)kUpV);
-    const int64_t col = (int64_t)w.kv * a.D;
     if (key >= sq.lk) return;
-    T *pk = static_cast<T *>(a.dk) + (sq.k0 + key) * a.lddk + col;
-    T *pv = static_cast<T *>(a.dv) + (sq.k0 + key) * a.lddv + col;
+    const int64_t keys = (int64_t)a.KV * a.Tk, at = (int64_t)w.kv * a.Tk + sq.k0 + key;
+    const int64_t col = (int64_t)w.kv * a.D;
+    put_grad<DT, DP>(a, a.kpart, keys, at, a.ksplits,
+                     static_cast<T *>(a.dk) + (sq.k0 + key) * a.lddk + col, dk,
+                     a.scale * pow2(-up), h);
+    put_grad<DT, DP>(a, a.kpart + a.ksplits * keys * a.D, keys, at, a.ksplits,
+                     static_cast<T *>(a.dv) + (sq.k0 + key) * a.lddv + col, dv, pow2(-(int)kUpV),
+                     h);
+}
+
+// The splits' gradients added in order, a wave a row: of dQ, then dK, then dV, those that
+// are in splits.  Rows of no sequence are left.
+template <int DT>
+__global__ __launch_bounds__(256) void att_bwd_combine(const Args a) {
+    using Ty = Type<DT>;
+    using T = typename Ty::T;
+    const int lane = threadIdx.x & 63;
+    const int64_t rows = a.splits > 1 ? (int64_t)a.KV * a.Tq * a.G : 0;
+    const int64_t keys = a.ksplits > 1 ? (int64_t)a.KV * a.Tk : 0;
+    int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at >= rows + 2 * keys) return;
+    const float *p;
+    T *to;
+    int64_t step;
+    int splits;
+    if (at < rows) {
+        const int kv = (int)(at / ((int64_t)a.Tq * a.G));
+        const int row = (int)(at - (int64_t)kv * a.Tq * a.G), token = a.group.of(row);
+        const Place pl =
+            place_of(token, a.n, [&](int s) { return (int)min(a.qs[s], (uint32_t)a.Tq); });
+        const Seq sq(a, pl.seq);
+        if (token < sq.q0 || token >= sq.q0 + sq.lq) return;
+        to = static_cast<T *>(a.dq) + token * a.lddq +
+             (int64_t)(kv * a.G + row - token * a.G) * a.D;
+        p = a.part + at * a.D;
+        step = rows * a.D;
+        splits = a.splits;
+    } else {
+        at -= rows;
+        const bool value = at >= keys;
+        if (value) at -= keys;
+        const int kv = (int)(at / a.Tk), key = (int)(at - (int64_t)kv * a.Tk);
+        const Place pl =
+            place_of(key, a.n, [&](int s) { return (int)min(a.ks[s], (uint32_t)a.Tk); });
+        const Seq sq(a, pl.seq);
+        if (key < sq.k0 || key >= sq.k0 + sq.lk) return;
+        to = (value ? static_cast<T *>(a.dv) + key * a.lddv : static_cast<T *>(a.dk) + key * a.lddk) +
+             (int64_t)kv * a.D;
+        p = a.kpart + ((value ? a.ksplits * keys : 0) + at) * a.D;
+        step = keys * a.D;
+        splits = a.ksplits;
+    }
+    float acc[2] = {0.0f, 0.0f};
+    for (int s = 0; s < splits; ++s)
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int d = 32 * b + 8 * q + 4 * h;
-            const f32x16 &x = dk[b], &y = dv[b];
-            Ty::store4(pk, d, a.D,
-                       f32x4{x[4 * q] * fk, x[4 * q + 1] * fk, x[4 * q + 2] * fk,
-                             x[4 * q + 3] * fk},
-                       a.accumulate);
-            Ty::store4(pv, d, a.D,
-                       f32x4{y[4 * q] * fv, y[4 * q + 1] * fv, y[4 * q + 2] * fv,
-                             y[4 * q + 3] * fv},
-                       a.accumulate);
-        }
+        for (int i = 0; i < 2; ++i)
+            if (lane + 64 * i < a.D) acc[i] += p[s * step + lane + 64 * i];
+    put_row<DT>(to, acc, 1.0f, a.D, lane, a.accumulate);
 }
 
 // ------------------------------------------------------------------ launches
@@ -1398,6 +1478,7 @@ void with_width(int D, bool dma, F f) {
         else f(dp, std::false_type{});
     };
     if (D <= 64) with(integral_constant<int, 64>{});
+    else if (D <= 96) f(integral_constant<int, 96>{}, std::false_type{});
     else with(integral_constant<int, 128>{});
 }
 
@@ -1418,9 +1499,12 @@ int combine(hipStream_t st, const Args &a) {
 template <int DT>
 int backward(hipStream_t st, const Args &a, bool dma) {
     with_width<DT>(a.D, dma, [&](auto dp, auto d) {
-        att_bwd_q<DT, dp(), d()><<<a.KV * a.slots, 256, 0, st>>>(a);
-        att_bwd_kv<DT, dp(), d()><<<a.KV * a.kslots, 256, 0, st>>>(a);
+        att_bwd_q<DT, dp(), d()><<<dim3(a.KV * a.slots, a.splits), 256, 0, st>>>(a);
+        att_bwd_kv<DT, dp(), d()><<<dim3(a.KV * a.kslots, a.ksplits), 256, 0, st>>>(a);
     });
+    const int64_t rows = (a.splits > 1 ? (int64_t)a.KV * a.Tq * a.G : 0) +
+                         (a.ksplits > 1 ? 2 * (int64_t)a.KV * a.Tk : 0);
+    if (rows) att_bwd_combine<DT><<<(rows - 1) / 4 + 1, 256, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 

@@ -142,8 +142,6 @@ uint64_t embedding_bwd_ws_bytes(int dtype, int T, int V, int C);
 // Dispatches of those calls.
 int layer_norm_bwd_dispatches(int cus, int dtype, int R, int C, bool dx, bool weights);
 int embedding_bwd_dispatches(int dtype, int T, int V, int C);
-// Workspace bytes of fg_attention_bwd.
-uint64_t attention_bwd_ws_bytes(int Tq, int heads);
 // The same two of fg_rms_norm_bwd.
 uint64_t rms_norm_bwd_ws_bytes(int cus, int dtype, int R, int C);
 int rms_norm_bwd_dispatches(int cus, int dtype, int R, int C, bool dx, bool weights);

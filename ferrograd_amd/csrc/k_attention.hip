@@ -31,6 +31,33 @@ int splits_of(int cus, const Args &a, bool few) {
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
 }
 
+// Splits of the backward's passes: of `sum` rows (keys) a sequence on average, for one of
+// `tiles` workgroups, 128 at least each, to fill the CUs' twice.
+int bwd_splits(int cus, int64_t tiles, int64_t sum) {
+    const int64_t want = 2 * (int64_t)cus / std::max<int64_t>(tiles, 1);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want, sum / 128, kMaxSplits}));
+}
+
+void set_splits(int cus, Args &a) {
+    const int64_t rows = (int64_t)a.Tq * a.G;
+    const int64_t q_tiles = std::max<int64_t>(a.n, (rows - 1) / fg::attn::kRows + 1) * a.KV;
+    const int64_t k_tiles = std::max<int64_t>(a.n, ((int64_t)a.Tk - 1) / fg::attn::kKeys + 1) * a.KV;
+    a.splits = bwd_splits(cus, q_tiles, a.Tk / a.n);
+    a.ksplits = bwd_splits(cus, k_tiles, rows / a.n);
+}
+
+// Floats of the backward's workspace.
+struct BwdSpace {
+    uint64_t rows, part = 0, kpart = 0;
+    explicit BwdSpace(const Args &a) {
+        const uint64_t all = (uint64_t)std::max(a.Tq, 1) * a.KV * a.G;
+        rows = (3 * all + 3) / 4 * 4;
+        if (a.splits > 1) part = (a.splits * all * a.D + 3) / 4 * 4;
+        if (a.ksplits > 1) kpart = 2 * (uint64_t)a.ksplits * a.KV * a.Tk * a.D;
+    }
+    uint64_t bytes() const { return (rows + part + kpart) * sizeof(float); }
+};
+
 bool whole_chunks(const Args &a, std::initializer_list<std::pair<const void *, int64_t>> rows) {
     if (a.D != 64 && a.D != 128) return false;
     // (And a tile's rows are within 32 bits of its first.)
@@ -67,12 +94,6 @@ int check(const char *who, int dtype, const Args &a, int heads, int kv_heads) {
 }
 
 }  // namespace
-
-namespace fg {
-uint64_t attention_bwd_ws_bytes(int Tq, int heads) {
-    return 3 * (uint64_t)std::max(Tq, 1) * (uint64_t)heads * sizeof(float);
-}
-}  // namespace fg
 
 FG_API int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k, int ldk,
                         const void *d_v, int ldv, const uint32_t *d_q_starts,
@@ -189,9 +210,13 @@ FG_API int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, co
                "%s: an output is another output", who);
     if (n == 0 || (Tq == 0 && Tk == 0)) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
-    a.rows = (float *)fg::workspace(ctx, fg::attention_bwd_ws_bytes(Tq, heads));
-    if (!a.rows) return FG_ERR_OUT_OF_MEMORY;
-    a.splits = 1;
+    set_splits(ctx->cu_count, a);
+    const BwdSpace need(a);
+    float *ws = (float *)fg::workspace(ctx, need.bytes());
+    if (!ws) return FG_ERR_OUT_OF_MEMORY;
+    a.rows = ws;
+    a.part = ws + need.rows;
+    a.kpart = a.part + need.part;
     a.slots = (int)((int64_t)Tq * a.G / fg::attn::kRows + n);
     a.kslots = Tk / fg::attn::kKeys + n;
     const bool dma = whole_chunks(a, {{d_q, ldq}, {d_k, ldk}, {d_v, ldv}, {d_dout, lddo}});

@@ -199,6 +199,8 @@ SETS = [
     ([(77, 77), (65, 65)], 6, 2, 100, False, 1, 1, 0),
     ([(90, 90)], 7, 1, 33, True, 5, 3, 0),
     ([(150, 150)], 8, 1, 128, True, 3, 0, 0),
+    ([(300, 700), (40, 1000)], 2, 1, 96, True, 8, 0, 1),
+    ([(500, 500), (3, 3)], 4, 2, 90, False, 1, 0, 0),
     ([(1, 700), (1, 33), (2, 2), (1, 1)], 8, 2, 128, True, 0, 0, 0),   # single tokens
     ([(1, 129), (3, 64), (1, 0)], 5, 1, 80, True, 1, 1, 1),
 ]
@@ -277,7 +279,7 @@ def test_small_gradients_of_fp16(gpu_ctx):
 
 
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("D,lq,lk", [(64, 100, 100), (128, 70, 140), (40, 65, 65), (128, 1, 90)])
+@pytest.mark.parametrize("D,lq,lk", [(64, 100, 100), (128, 70, 140), (40, 65, 65), (128, 1, 90), (96, 300, 300)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 def test_keys_out_of_sight_do_not_reach_a_row(gpu_ctx, dt, D, lq, lk, bad):
     """The last key (causal: seen by the last row alone) holds NaN or infinity: the other
