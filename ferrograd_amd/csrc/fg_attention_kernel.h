@@ -121,20 +121,22 @@ struct Type {
         if constexpr (kWide) *p = v;
         else *p = f_to_h16(DT, v);
     }
+    static __device__ __forceinline__ Frag load8(const T *p) {
+        Frag f;
+        if constexpr (kWide) {
+            const f32x4 x = *reinterpret_cast<const f32x4_any *>(p);
+            const f32x4 y = *reinterpret_cast<const f32x4_any *>(p + 4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = j < 4 ? x[j & 3] : y[j & 3];
+        } else {
+            f = *reinterpret_cast<const u32x4_any *>(p);
+        }
+        return f;
+    }
     // Elements d .. d + 7 of a row of D (zeros past it; row NULL: zeros).
     static __device__ __forceinline__ Frag load8(const T *row, int d, int D) {
+        if (row && d + 8 <= D) return load8(row + d);
         Frag f;
-        if (row && d + 8 <= D) {
-            if constexpr (kWide) {
-                const f32x4 x = *reinterpret_cast<const f32x4_any *>(row + d);
-                const f32x4 y = *reinterpret_cast<const f32x4_any *>(row + d + 4);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = j < 4 ? x[j & 3] : y[j & 3];
-            } else {
-                f = *reinterpret_cast<const u32x4_any *>(row + d);
-            }
-            return f;
-        }
         T e[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = row && d + j < D ? row[d + j] : T(0);
@@ -315,7 +317,15 @@ struct Mover {
             lds_dma16(base, offset_of(row + lane / CH) + c, lds + row * DP + gap<CH>(row) * E);
         }
     }
-    // Otherwise: row r from row_at(r).
+    // Otherwise: row r from row_at(r); with rows and D, zeros past them.
+    template <class F>
+    __device__ __forceinline__ void fetch(int tid, F row_at) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int pos = i * NT + tid;
+            v[i] = *reinterpret_cast<const u32x4_any *>(row_at(pos / CH) + pos % CH * E);
+        }
+    }
     template <class F>
     __device__ __forceinline__ void fetch(int tid, int rows, int D, F row_at) {
 #pragma unroll
@@ -497,27 +507,18 @@ struct Rows {
     using Ty = Type<DT>;
     using T = typename Ty::T;
     using Tl = Tile<DT, DP, KT>;
-    static constexpr int NB = DP / 32, NK = DP / 16;
+    static constexpr int NB = DP / 32, NK = DP / 16, KB = KT / 32;
     static constexpr float kUp = DT == kF16 ? 8.0f : 0.0f, kRaise = DT == kF16 ? 4.0f : 8.0f;
     typename Ty::Frag q[NK];
     f32x16 o[NB];
     float m = -INFINITY, l = 0.0f;
     bool bad = false;  // a tile of keys not all visible held an infinity or NaN
 
-    // Keys key0 .. key0 + KT - 1 in tiles k and v, up to `last` for the lane's row; whole:
-    // every one is visible to every row of the wave.
-    __device__ __forceinline__ void step(const T *k, const T *v, int key0, int last, bool whole,
-                                         float c, const Lanes<DT, DP> &L) {
-        const int h = L.lane >> 5;
-        constexpr int KB = KT / 32;
-        f32x16 s[KB];
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            s[b] = all16(0.0f);
-#pragma unroll
-            for (int ks = 0; ks < NK; ++ks)
-                s[b] = Ty::mfma(Tl::by_row(k, b, ks, L), q[ks], s[b]);
-        }
+    // Scores of keys key0 .. key0 + KT - 1 (s), the visible of which, up to `last` for the
+    // lane's row, become probabilities; whole: every one is visible to every row of the
+    // wave.
+    __device__ __forceinline__ void weigh(f32x16 (&s)[KB], int key0, int last, bool whole, float c,
+                                          int h) {
         if (!whole) {
 #pragma unroll
             for (int b = 0; b < KB; ++b)
@@ -553,6 +554,10 @@ struct Rows {
                 part[r & 3] += s[b][r];
             }
         l += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    // Their values, from tile v.
+    __device__ __forceinline__ void values(const T *v, const f32x16 (&s)[KB], bool whole,
+                                           const Lanes<DT, DP> &L) {
         if (!whole) bad |= !Tl::finite(v, L.lane);
 #pragma unroll
         for (int b = 0; b < KB; ++b)
@@ -742,8 +747,19 @@ att_fwd(const Args a) {
         if (t + 1 < t1) load(t + 1);
         const int key0 = t * KT;
         const T *at = lds + (t & 1) * 2 * Tl::kElems;
-        if (key0 <= wave_last)
-            st.step(at, at + Tl::kElems, key0, last, key0 + KT - 1 <= wave_first, c, L);
+        if (key0 <= wave_last) {
+            const bool whole = key0 + KT - 1 <= wave_first;
+            f32x16 s[KT / 32];
+#pragma unroll
+            for (int b = 0; b < KT / 32; ++b) {
+                s[b] = all16(0.0f);
+#pragma unroll
+                for (int ks = 0; ks < DP / 16; ++ks)
+                    s[b] = Ty::mfma(Tl::by_row(at, b, ks, L), st.q[ks], s[b]);
+            }
+            st.weigh(s, key0, last, whole, c, h);
+            st.values(at + Tl::kElems, s, whole, L);
+        }
         if (t + 1 < t1) store(t + 1);
     }
     if (__syncthreads_or(st.bad)) {
@@ -757,20 +773,22 @@ att_fwd(const Args a) {
 }
 
 // Few rows (single tokens: a group's heads): 32 rows a workgroup, whose four waves take
-// key tiles in turn, each through LDS of its own, without barriers; their statistics and
-// sums are joined at the end.
+// key tiles in turn without barriers; their statistics and sums are joined at the end.
+// Bound by the keys' and values' bytes: a wave's next keys load into the registers that
+// hold this tile's as soon as its scores are taken, the next values as soon as these have
+// gone to the wave's LDS (for the transposing reads), so that about 16 KiB a wave, 128 a
+// CU, are in flight.  FULL: heads of DP columns.
 constexpr int kFewKeys = 32;
-template <int DT, int DP, bool DMA>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void att_fwd_few(
-    const Args a) {
+template <int DT, int DP, bool FULL>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
+att_fwd_few(const Args a) {
     using Ty = Type<DT>;
     using T = typename Ty::T;
-    constexpr int KT = kFewKeys, NB = DP / 32;
+    constexpr int KT = kFewKeys, NB = DP / 32, NK = DP / 16;
     using Tl = Tile<DT, DP, KT>;
-    // A wave's two stages of K and V; at the end its O^T, 32 x DP floats.
-    constexpr int kStages = DT == kF32 && DP > 64 ? 1 : 2;
-    constexpr int kWave = kStages * 2 * Tl::kElems;
-    static_assert(kWave * sizeof(T) >= 32 * DP * sizeof(float) && kWave % 8 == 0, "room for the sums");
+    // A wave's values; at the end its O^T, 32 x DP floats, of waves 1 to 3.
+    constexpr int kWave = Tl::kElems * (int)sizeof(T) > 32 * DP * 4 ? Tl::kElems
+                                                                   : 32 * DP * 4 / (int)sizeof(T);
     __shared__ __attribute__((aligned(16))) T lds[4 * kWave];
     __shared__ float ml[4][32][2];
     const Work w(blockIdx.x, a.KV, a.slots);
@@ -799,58 +817,46 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) void a
 
     const Lanes<DT, DP> L(lane);
     Rows<DT, DP, KT> st;
+    typename Ty::Frag kf[NK];
+    Mover<DT, DP, KT, 64, false> mv;
+    // (Rows past the sequence's keys: its last again.)
+    auto load_k = [&](int t) {
+        const T *p = k + min(t * KT + l32, sq.lk - 1) * a.ldk;
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks)
+            kf[ks] = FULL ? Ty::load8(p + 16 * ks + 8 * h) : Ty::load8(p, 16 * ks + 8 * h, a.D);
+    };
+    auto load_v = [&](int t) {
+        const int key0 = t * KT, left = sq.lk - key0;
+        const T *p = v + key0 * a.ldv;
+        auto at = [&](int r) { return p + min(r, left - 1) * a.ldv; };
+        if constexpr (FULL) mv.fetch(lane, at);
+        else mv.fetch(lane, left, a.D, at);
+    };
+    if (t0 < t1) {
+        load_k(t0);
+        load_v(t0);
+    }
     const T *qrow = row < rows ? static_cast<const T *>(a.q) + token * a.ldq +
                                      (int64_t)(w.kv * a.G + g) * a.D
                                : nullptr;
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) st.q[ks] = Ty::load8(qrow, 16 * ks + 8 * h, a.D);
+    for (int ks = 0; ks < NK; ++ks) st.q[ks] = Ty::load8(qrow, 16 * ks + 8 * h, a.D);
     clear(st.o);
-
     T *mine = lds + wave * kWave;
-    Mover<DT, DP, KT, 64, DMA> mk, mv;
-    auto load = [&](int t, int stage) {
-        T *to = mine + stage * 2 * Tl::kElems;
-        const int key0 = t * KT, left = sq.lk - key0;
-        mk.load(to, lane, k + key0 * a.ldk, a.ldk, left, a.D);
-        mv.load(to + Tl::kElems, lane, v + key0 * a.ldv, a.ldv, left, a.D);
-    };
-    auto store = [&](int stage) {
-        T *to = mine + stage * 2 * Tl::kElems;
-        mk.store(to, lane);
-        mv.store(to + Tl::kElems, lane);
-    };
-    int stage = 0;
-    if (t0 < t1) {
-        load(t0, 0);
-        store(0);
-    }
     for (int t = t0; t < t1; t += 4) {
-        const int next = kStages > 1 ? stage ^ 1 : 0;
-        const bool more = t + 4 < t1;
-        // DMA: this wave's loads of tile t are done when only the next tile's are left.
-        if constexpr (DMA) {
-            // (The reads of the stage that the next loads fill are done first.)
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (more) {
-                load(t + 4, next);
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * Mover<DT, DP, KT, 64, DMA>::kPer)
-                             : "memory");
-            } else {
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            }
-        } else {
-            __builtin_amdgcn_wave_barrier();
-            if (more) load(t + 4, next);
-        }
         const int key0 = t * KT;
-        const T *at = mine + stage * 2 * Tl::kElems;
-        st.step(at, at + Tl::kElems, key0, last, key0 + KT - 1 <= first, c, L);
-        if constexpr (!DMA) {
-            __builtin_amdgcn_wave_barrier();
-            if (more) store(next);
-            __builtin_amdgcn_wave_barrier();
-        }
-        stage = next;
+        const bool whole = key0 + KT - 1 <= first, more = t + 4 < t1;
+        f32x16 s[1] = {all16(0.0f)};
+#pragma unroll
+        for (int ks = 0; ks < NK; ++ks) s[0] = Ty::mfma(kf[ks], st.q[ks], s[0]);
+        if (more) load_k(t + 4);
+        st.weigh(s, key0, last, whole, c, h);
+        __builtin_amdgcn_wave_barrier();  // (after the reads of the values before)
+        mv.store(mine, lane);
+        __builtin_amdgcn_wave_barrier();
+        if (more) load_v(t + 4);
+        st.values(mine, s, whole, L);
     }
     if (__syncthreads_or(st.bad)) {
         careful_fwd<DT>(a, sq, w.kv, blockIdx.y, m0, min(m0 + kFewRows, rows), (t0 - wave) * KT,
@@ -1482,12 +1488,26 @@ void with_width(int D, bool dma, F f) {
     else with(integral_constant<int, 128>{});
 }
 
+template <int DT, class F>
+void with_few(int D, F f) {
+    using std::integral_constant;
+    auto with = [&](auto dp) {
+        if (D == dp()) f(dp, std::true_type{});
+        else f(dp, std::false_type{});
+    };
+    if (D <= 64) with(integral_constant<int, 64>{});
+    else if (D <= 96) with(integral_constant<int, 96>{});
+    else with(integral_constant<int, 128>{});
+}
+
 template <int DT>
 int forward(hipStream_t st, const Args &a, bool few, bool dma) {
     const dim3 grid(a.KV * a.slots, a.splits);
     with_width<DT>(a.D, dma, [&](auto dp, auto d) {
-        if (few) att_fwd_few<DT, dp(), d()><<<grid, 256, 0, st>>>(a);
-        else att_fwd<DT, dp(), d()><<<grid, 256, 0, st>>>(a);
+        if (!few) att_fwd<DT, dp(), d()><<<grid, 256, 0, st>>>(a);
+    });
+    if (few) with_few<DT>(a.D, [&](auto dp, auto full) {
+        att_fwd_few<DT, dp(), full()><<<grid, 256, 0, st>>>(a);
     });
     return (int)hipGetLastError();
 }

@@ -32,18 +32,20 @@ int splits_of(int cus, const Args &a, bool few) {
 }
 
 // Splits of the backward's passes: of `sum` rows (keys) a sequence on average, for one of
-// `tiles` workgroups, 128 at least each, to fill the CUs' twice.
-int bwd_splits(int cus, int64_t tiles, int64_t sum) {
-    const int64_t want = 2 * (int64_t)cus / std::max<int64_t>(tiles, 1);
+// `tiles` workgroups, 128 at least each, up to `fill` workgroups.
+int bwd_splits(int fill, int64_t tiles, int64_t sum) {
+    const int64_t want = fill / std::max<int64_t>(tiles, 1);
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, sum / 128, kMaxSplits}));
 }
 
-void set_splits(int cus, Args &a) {
+// (A CU holds two workgroups, of fp32 one.)
+void set_splits(int cus, int dtype, Args &a) {
+    const int fill = dtype == FG_DTYPE_F32 ? cus : 2 * cus;
     const int64_t rows = (int64_t)a.Tq * a.G;
     const int64_t q_tiles = std::max<int64_t>(a.n, (rows - 1) / fg::attn::kRows + 1) * a.KV;
     const int64_t k_tiles = std::max<int64_t>(a.n, ((int64_t)a.Tk - 1) / fg::attn::kKeys + 1) * a.KV;
-    a.splits = bwd_splits(cus, q_tiles, a.Tk / a.n);
-    a.ksplits = bwd_splits(cus, k_tiles, rows / a.n);
+    a.splits = bwd_splits(fill, q_tiles, a.Tk / a.n);
+    a.ksplits = bwd_splits(fill, k_tiles, rows / a.n);
 }
 
 // Floats of the backward's workspace.
@@ -210,7 +212,7 @@ FG_API int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, co
                "%s: an output is another output", who);
     if (n == 0 || (Tq == 0 && Tk == 0)) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
-    set_splits(ctx->cu_count, a);
+    set_splits(ctx->cu_count, dtype, a);
     const BwdSpace need(a);
     float *ws = (float *)fg::workspace(ctx, need.bytes());
     if (!ws) return FG_ERR_OUT_OF_MEMORY;
