@@ -333,12 +333,13 @@ struct Mover {
             const int pos = i * NT + tid, row = pos / CH, d = (pos % CH) * E;
             if (Tl::kChunks % NT && row >= ROWS) break;
             const T *p = row_at(row) + d;
+            v[i] = u32x4{0u, 0u, 0u, 0u};
             if (row < rows && d + E <= D) {
                 v[i] = *reinterpret_cast<const u32x4_any *>(p);
-            } else {
+            } else if (row < rows && d < D) {
                 T e[E];
 #pragma unroll
-                for (int k = 0; k < E; ++k) e[k] = row < rows && d + k < D ? p[k] : T(0);
+                for (int k = 0; k < E; ++k) e[k] = d + k < D ? p[k] : T(0);
                 v[i] = __builtin_bit_cast(u32x4, e);
             }
         }
@@ -378,9 +379,26 @@ struct Mover {
     }
 };
 
+// What the scheduler is to send in turn: N LDS reads, or N matrix instructions with R
+// reads after each.  (Left to itself the compiler waits for each pair of reads where
+// registers are few.)
+template <int N>
+__device__ __forceinline__ void reads() {
+    __builtin_amdgcn_sched_group_barrier(0x100, N, 0);
+}
+template <int N, int R>
+__device__ __forceinline__ void products() {
+    each_of<N>([](auto) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (R) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    });
+}
+
 // The wave's direct loads have landed and its LDS reads are done, and every other
-// wave's.
+// wave's.  (The builtin tells the compiler, which otherwise waits for operands loaded
+// before the loop where they are used: for the next tile's loads, just sent, with them.)
 __device__ __forceinline__ void landed() {
+    wait_vmcnt<0>();
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
@@ -1187,10 +1205,14 @@ att_bwd_q(const Args a) {
                 f32x16 s = all16(kFold<DT> ? fresh(-from) : 0.0f);
                 f32x16 dp = all16(kFold<DT> ? fresh(-delta) : 0.0f);
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks) s = Ty::mfma(Tl::by_row(kt, b, ks, L), q[ks], s);
+                for (int ks = 0; ks < NK; ++ks) {
+                    s = Ty::mfma(Tl::by_row(kt, b, ks, L), q[ks], s);
+                    if (Ty::kWide) dp = Ty::mfma(Tl::by_row(vt, b, ks, L), dout[ks], dp);
+                }
+                if (!Ty::kWide)
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks)
-                    dp = Ty::mfma(Tl::by_row(vt, b, ks, L), dout[ks], dp);
+                    for (int ks = 0; ks < NK; ++ks)
+                        dp = Ty::mfma(Tl::by_row(vt, b, ks, L), dout[ks], dp);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     if constexpr (kFold<DT>)
@@ -1365,10 +1387,23 @@ att_bwd_kv(const Args a) {
             f32x16 p = kFold<DT> ? rows16(st + 4 * h) : all16(0.0f);
             f32x16 dp = kFold<DT> ? rows16(st + RT + 4 * h) : all16(0.0f);
 #pragma unroll
-            for (int ks = 0; ks < NK; ++ks) p = Ty::mfma(Tl::by_row(qt, 0, ks, L), kf[ks], p);
+            for (int ks = 0; ks < NK; ++ks) {
+                p = Ty::mfma(Tl::by_row(qt, 0, ks, L), kf[ks], p);
+                if (Ty::kWide)
+                    dp = Ty::mfma(Tl::by_row(dt, 0, ks, L), Vt::by_row(vlds, wave, ks, L), dp);
+            }
+            if (!Ty::kWide)
 #pragma unroll
-            for (int ks = 0; ks < NK; ++ks)
-                dp = Ty::mfma(Tl::by_row(dt, 0, ks, L), Vt::by_row(vlds, wave, ks, L), dp);
+                for (int ks = 0; ks < NK; ++ks)
+                    dp = Ty::mfma(Tl::by_row(dt, 0, ks, L), Vt::by_row(vlds, wave, ks, L), dp);
+            if constexpr (!Ty::kWide) {
+                // Three ahead, after the rows' eight: dP's products take two reads each.
+                // (1.65 -> 1.59 ms; dQ's and the forward's scores gained nothing.)
+                reads<8 + 3>();
+                products<NK - 3, 1>();
+                products<NK, 2>();
+                products<3, 0>();
+            }
             if constexpr (kFold<DT>) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
@@ -1467,6 +1502,7 @@ __global__ __launch_bounds__(256) void att_bwd_combine(const Args a) {
         splits = a.ksplits;
     }
     float acc[2] = {0.0f, 0.0f};
+#pragma unroll 4
     for (int s = 0; s < splits; ++s)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
