@@ -145,6 +145,8 @@ pub const FG_OP_SOFTMAX: c_int = 15;
 pub const FG_OP_BIAS_ADD: c_int = 16;
 pub const FG_OP_LAYER_NORM: c_int = 17;
 pub const FG_OP_EMBEDDING: c_int = 18;
+pub const FG_OP_RMS_NORM: c_int = 19;
+pub const FG_OP_ATTENTION: c_int = 20;
 // input flags
 pub const FG_INPUT_NO_GRAD: u32 = 0x1;
 pub const FG_INPUT_FROZEN: u32 = 0x2;
@@ -864,6 +866,26 @@ extern "C" {
         gamma: u32,
         beta: u32,
         eps: f32,
+        node: *mut u32,
+    ) -> c_int;
+    pub fn fg_graph_rms_norm(
+        g: *mut fg_graph,
+        x: u32,
+        gamma: u32,
+        eps: f32,
+        node: *mut u32,
+    ) -> c_int;
+    pub fn fg_graph_attention(
+        g: *mut fg_graph,
+        q: u32,
+        k: u32,
+        v: u32,
+        q_starts: u32,
+        k_starts: u32,
+        heads: c_int,
+        kv_heads: c_int,
+        scale: f32,
+        causal: c_int,
         node: *mut u32,
     ) -> c_int;
     pub fn fg_graph_embedding(

@@ -261,6 +261,32 @@ impl Graph {
         Ok(id)
     }
 
+    /// RMS norm of `x[..., N]` over its last dimension with `gamma[N]`.
+    pub fn rms_norm(&mut self, x: u32, gamma: u32, eps: f32) -> Result<u32, Error> {
+        let mut id = 0u32;
+        check(unsafe { sys::fg_graph_rms_norm(self.raw, x, gamma, eps, &mut id) })?;
+        Ok(id)
+    }
+
+    /// Attention of packed sequences; `starts` are the `FG_DTYPE_U32` inputs that give each
+    /// one's rows of `q`, and of `k` and `v`; `heads` those of `q`, and of `k` and `v`.
+    pub fn attention(
+        &mut self,
+        [q, k, v]: [u32; 3],
+        [q_starts, k_starts]: [u32; 2],
+        [heads, kv_heads]: [c_int; 2],
+        scale: f32,
+        causal: bool,
+    ) -> Result<u32, Error> {
+        let mut id = 0u32;
+        check(unsafe {
+            sys::fg_graph_attention(
+                self.raw, q, k, v, q_starts, k_starts, heads, kv_heads, scale, causal as c_int, &mut id,
+            )
+        })?;
+        Ok(id)
+    }
+
     /// `scale * table[tokens]`, `tokens` an input of type `FG_DTYPE_U32`.
     pub fn embedding(&mut self, table: u32, tokens: u32, scale: f32) -> Result<u32, Error> {
         let mut id = 0u32;

@@ -66,15 +66,15 @@ bool is_elementwise(int op) { return is_unary(op) || is_binary_elt(op); }
 int arity(int op) {
     if (op == FG_OP_INPUT || op == FG_OP_CONST) return 0;
     if (is_unary(op) || op == FG_OP_SOFTMAX) return 1;
-    return op == FG_OP_LAYER_NORM ? 3 : 2;
+    return op == FG_OP_ATTENTION ? 5 : op == FG_OP_LAYER_NORM ? 3 : 2;
 }
 
 const char *op_name(int op) {
     static const char *names[] = {"input", "const", "add",  "sub", "mul",  "div",
                                   "matmul", "relu", "gelu", "elu", "tanh", "exp",
                                   "log",   "abs",   "neg",  "softmax", "bias_add",
-                                  "layer_norm", "embedding"};
-    return (op >= 0 && op <= FG_OP_EMBEDDING) ? names[op] : "?";
+                                  "layer_norm", "embedding", "rms_norm", "attention"};
+    return (op >= 0 && op <= FG_OP_ATTENTION) ? names[op] : "?";
 }
 
 // SaveIndicator flags (kernel/mod.rs:41-93).
@@ -84,8 +84,10 @@ struct GNode {
     int op = FG_OP_INPUT;
     std::vector<uint32_t> in;
     std::vector<uint32_t> fields;  // Input: meta field per dim
-    float value = 0.0f;            // Const (already rounded to dtype); layer norm: eps;
-                                   // embedding: scale
+    float value = 0.0f;            // Const (already rounded to dtype); norms: eps;
+                                   // embedding, attention: scale
+    int heads = 0, kv_heads = 0;   // attention
+    bool causal = false;
     uint32_t flags = 0;            // Input flags
     bool ckpt8 = false;            // pre-activation kept in 8 bits (fg_graph_set_ckpt8)
     int dtype = FG_DTYPE_F32;      // Input / Const: declared; operations: of their first input
@@ -153,8 +155,11 @@ int infer_shapes(const fg_graph &g, const uint32_t *meta, int n_meta, std::vecto
         for (size_t k = 0; k < nd.in.size(); ++k) {
             const GNode &x = g.nodes[nd.in[k]];
             const bool tokens = x.op == FG_OP_INPUT && x.dtype == FG_DTYPE_U32;
-            FG_REQUIRE(tokens == (nd.op == FG_OP_EMBEDDING && k == 1), FG_ERR_UNSUPPORTED,
-                       "%s %zu: u32 inputs are the tokens of embeddings and nothing else",
+            FG_REQUIRE(tokens == ((nd.op == FG_OP_EMBEDDING && k == 1) ||
+                                  (nd.op == FG_OP_ATTENTION && k >= 3)),
+                       FG_ERR_UNSUPPORTED,
+                       "%s %zu: u32 inputs are the tokens of embeddings and the starts of "
+                       "attention and nothing else",
                        op_name(nd.op), i);
         }
         switch (nd.op) {
@@ -199,6 +204,31 @@ int infer_shapes(const fg_graph &g, const uint32_t *meta, int n_meta, std::vecto
                                be.cols == a.cols,
                            FG_ERR_SHAPE, "layer_norm %zu: needs x[..., N], gamma[N], beta[N]", i);
                 s = a;
+                break;
+            }
+            case FG_OP_RMS_NORM: {
+                const Shape &a = sh[nd.in[0]], &ga = sh[nd.in[1]];
+                FG_REQUIRE(!a.scalar && ga.vector && ga.cols == a.cols, FG_ERR_SHAPE,
+                           "rms_norm %zu: needs x[..., N], gamma[N]", i);
+                s = a;
+                break;
+            }
+            case FG_OP_ATTENTION: {
+                const Shape &q = sh[nd.in[0]], &k = sh[nd.in[1]], &v = sh[nd.in[2]];
+                const Shape &qs = sh[nd.in[3]], &ks = sh[nd.in[4]];
+                for (const Shape *x : {&q, &k, &v})
+                    FG_REQUIRE(!x->scalar && !x->vector && x->rows <= INT32_MAX, FG_ERR_SHAPE,
+                               "attention %zu: q, k and v must be matrices", i);
+                FG_REQUIRE(q.cols % nd.heads == 0 && k.rows == v.rows && k.cols == v.cols &&
+                               k.cols == q.cols / nd.heads * nd.kv_heads,
+                           FG_ERR_SHAPE,
+                           "attention %zu: needs q[Tq, %d D], k[Tk, %d D], v[Tk, %d D]", i,
+                           nd.heads, nd.kv_heads, nd.kv_heads);
+                FG_REQUIRE(qs.vector && ks.vector && qs.cols == ks.cols && qs.cols >= 2 &&
+                               qs.cols <= INT32_MAX,
+                           FG_ERR_SHAPE,
+                           "attention %zu: the starts are n + 1 numbers of n >= 1 sequences", i);
+                s = q;
                 break;
             }
             case FG_OP_EMBEDDING: {
@@ -267,6 +297,10 @@ enum LaunchKind {
     LK_EMB_BWD,
     LK_CKPT_SAVE,
     LK_CKPT_LOAD,
+    LK_RMS,
+    LK_RMS_BWD,
+    LK_ATT,
+    LK_ATT_BWD,
 };
 
 struct Launch {
@@ -280,9 +314,12 @@ struct Launch {
     // statistics, sG / sH dgamma / dbeta (accumulate2 / accumulate3).  Embedding: sA
     // the table (forward), sB tokens, sZ dout, sC out / dtable; K the table's rows.
     // Checkpoints: sA the pre-activation, sB the bytes, sZ the exponents, sC the
-    // activation.
+    // activation.  RMS norm: as layer norm.  Attention: sA q, sB k, sZ v, sBias / sExtra
+    // the starts, sC out, sRstd lse; backward: sMean dout, sG / sH / sProbs dq / dk / dv.
     int sMean = kNone, sRstd = kNone, sG = kNone, sH = kNone, accumulate3 = 0;
     float value = 0.0f;  // eps, scale
+    fg::AttentionShape att{};
+    bool causal = false;
     fg::EltProgram prog{};
     int src_slot[fg::kEltMaxSrc];
     int dst_slot[fg::kEltMaxDst];
@@ -336,7 +373,7 @@ struct fg_plan {
     std::vector<uint32_t> save;
     std::vector<char> needs_grad;
     std::vector<int> val_slot, grad_slot, group_of;
-    std::vector<int> mean_of, rstd_of;  // layer norm statistics, per node
+    std::vector<int> mean_of, rstd_of;  // norms' statistics (attention's lse), per node
     // Activations whose pre-activation is kept in 8 bits: its bytes and exponents,
     // and the shared memory that a backward restores z and act(z) into.
     std::vector<int> ck_q, ck_e, ck_z, ck_h;
@@ -461,6 +498,8 @@ void compute_saved(const fg_graph &g, const std::vector<std::vector<uint32_t>> &
                 for (uint32_t u : users[i]) save[u] |= kDefBwd;
                 break;
             case FG_OP_LAYER_NORM:
+            case FG_OP_RMS_NORM:
+            case FG_OP_ATTENTION:
                 save[i] |= kDefFwd | kDefBwd;
                 for (uint32_t x : nd.in)
                     if (nonleaf(x)) save[x] |= kDefFwd;
@@ -600,6 +639,43 @@ std::string dims_str(int M, int N, int K) {
 }
 
 // ------------------------------------------------------------ lowering
+Launch fill0(const fg_plan &P, int slot, const std::string &desc) {
+    Launch L;
+    L.kind = LK_FILL0;
+    L.sC = slot;
+    L.count = P.slots[slot].bytes / 4;  // words (slot sizes are whole words)
+    L.desc = desc;
+    return L;
+}
+
+// What both directions of an attention node's launch have.
+Launch attention_launch(fg_plan &P, uint32_t n) {
+    const GNode &nd = P.g.nodes[n];
+    Launch L;
+    L.dtype = P.dtype[n];
+    const Shape &q = P.shape[nd.in[0]];
+    L.att = {(int)P.shape[nd.in[3]].cols - 1, (int)q.rows, (int)P.shape[nd.in[1]].rows, nd.heads,
+             nd.kv_heads, (int)(q.cols / nd.heads)};
+    L.causal = nd.causal;
+    L.value = nd.value;
+    L.sA = P.vslot(nd.in[0]);
+    L.sB = P.vslot(nd.in[1]);
+    L.sZ = P.vslot(nd.in[2]);
+    L.sBias = P.vslot(nd.in[3]);
+    L.sExtra = P.vslot(nd.in[4]);
+    L.sC = P.vslot(n);
+    L.sRstd = P.rstd_of[n];
+    return L;
+}
+
+// "n=4 Tq x Tk heads/kv_heads x D"
+std::string att_str(const Launch &L) {
+    return std::to_string(L.att.n) + " sequences " + std::to_string(L.att.Tq) + "x" +
+           std::to_string(L.att.Tk) + " heads " + std::to_string(L.att.heads) + "/" +
+           std::to_string(L.att.kv_heads) + "x" + std::to_string(L.att.D) +
+           (L.causal ? " causal" : "") + dt_suffix(L.dtype);
+}
+
 int lower_forward(fg_plan &P) {
     const fg_graph &g = P.g;
     EltBuilder eb(P);
@@ -651,22 +727,33 @@ int lower_forward(fg_plan &P) {
             }
             continue;
         }
-        if (nd.op == FG_OP_LAYER_NORM) {
+        if (nd.op == FG_OP_LAYER_NORM || nd.op == FG_OP_RMS_NORM) {
+            const bool rms = nd.op == FG_OP_RMS_NORM;
             eb.flush(P.fwd, "forward");
             Launch L;
-            L.kind = LK_LN;
+            L.kind = rms ? LK_RMS : LK_LN;
             L.dtype = P.dtype[n];
             L.M = (int)P.shape[n].rows;
             L.N = (int)P.shape[n].cols;
             L.sA = P.vslot(nd.in[0]);
             L.sZ = P.vslot(nd.in[1]);
-            L.sBias = P.vslot(nd.in[2]);
+            if (!rms) L.sBias = P.vslot(nd.in[2]);
             L.sC = P.vslot(n);
             L.sMean = P.mean_of[n];
             L.sRstd = P.rstd_of[n];
             L.value = nd.value;
-            L.desc = "forward layer_norm " + std::to_string(L.M) + "x" + std::to_string(L.N) +
+            L.desc = std::string("forward ") + op_name(nd.op) + " " + std::to_string(L.M) + "x" + std::to_string(L.N) +
                      dt_suffix(L.dtype) + " -> node " + std::to_string(n);
+            P.fwd.push_back(L);
+            continue;
+        }
+        if (nd.op == FG_OP_ATTENTION) {
+            eb.flush(P.fwd, "forward");
+            P.fwd.push_back(fill0(P, P.vslot(n), "forward zero rows of no sequence of node " +
+                                                     std::to_string(n)));
+            Launch L = attention_launch(P, n);
+            L.kind = LK_ATT;
+            L.desc = "forward attention " + att_str(L) + " -> node " + std::to_string(n);
             P.fwd.push_back(L);
             continue;
         }
@@ -1155,6 +1242,60 @@ int lower_backward(fg_plan &P, bool fused, std::vector<Launch> &out) {
             out.push_back(L);
             continue;
         }
+        if (nd.op == FG_OP_RMS_NORM) {
+            const uint32_t x = nd.in[0], ga = nd.in[1];
+            Launch L;
+            L.kind = LK_RMS_BWD;
+            L.dtype = P.dtype[n];
+            L.M = (int)P.shape[n].rows;
+            L.N = (int)P.shape[n].cols;
+            L.sA = P.vslot(x);
+            L.sB = gs(n);
+            L.sZ = P.vslot(ga);
+            L.sRstd = P.rstd_of[n];
+            L.desc = "backward rms_norm " + std::to_string(L.M) + "x" + std::to_string(L.N) +
+                     " -> grad of node";
+            auto to = [&](uint32_t t, int &slot, int &acc) {
+                if (!P.needs_grad[t]) return;
+                slot = gs(t);
+                acc = ginit[t];
+                ginit[t] = 1;
+                L.desc += " " + std::to_string(t);
+            };
+            to(x, L.sC, L.accumulate);
+            to(ga, L.sG, L.accumulate2);
+            out.push_back(L);
+            continue;
+        }
+        if (nd.op == FG_OP_ATTENTION) {
+            if (!P.needs_grad[nd.in[0]] && !P.needs_grad[nd.in[1]] && !P.needs_grad[nd.in[2]])
+                continue;
+            Launch L = attention_launch(P, n);
+            L.kind = LK_ATT_BWD;
+            L.sMean = gs(n);
+            L.desc = "backward attention " + att_str(L) + " -> grad of node";
+            int *dst[3] = {&L.sG, &L.sH, &L.sProbs};
+            // One of the three that is added to makes all of them so: the call has one
+            // switch for them, and the others start from zeros, as the rows of no
+            // sequence do.
+            for (int k = 0; k < 3; ++k) {
+                const uint32_t t = nd.in[k];
+                if (!P.needs_grad[t]) {  // the call writes all three
+                    *dst[k] = P.new_slot((uint64_t)P.shape[t].numel(), L.dtype);
+                    continue;
+                }
+                *dst[k] = gs(t);
+                L.desc += " " + std::to_string(t);
+                if (ginit[t])
+                    L.accumulate = 1;
+                else
+                    out.push_back(fill0(P, gs(t), "backward zero grad of node " +
+                                                      std::to_string(t)));
+                ginit[t] = 1;
+            }
+            out.push_back(L);
+            continue;
+        }
         if (nd.op == FG_OP_EMBEDDING) {
             const uint32_t x = nd.in[0];
             if (!P.needs_grad[x]) continue;
@@ -1198,12 +1339,7 @@ int lower_backward(fg_plan &P, bool fused, std::vector<Launch> &out) {
     // Inputs no gradient reached get zeros.
     for (uint32_t n : P.inputs) {
         if (!P.needs_grad[n] || ginit[n]) continue;
-        Launch L;
-        L.kind = LK_FILL0;
-        L.sC = gs(n);
-        L.count = P.slots[gs(n)].bytes / 4;  // words (slot sizes are whole words)
-        L.desc = "backward zero grad of node " + std::to_string(n);
-        out.push_back(L);
+        out.push_back(fill0(P, gs(n), "backward zero grad of node " + std::to_string(n)));
     }
     return FG_OK;
 }
@@ -1262,6 +1398,8 @@ int check_launch(const fg_plan &P, const Launch &L) {
             break;
         case LK_LN:
         case LK_LN_BWD:
+        case LK_RMS:
+        case LK_RMS_BWD:
             chk(L.sA, M * N, "x");
             chk(L.sB, M * N, "dy");
             chk(L.sC, M * N, "y");
@@ -1272,6 +1410,23 @@ int check_launch(const fg_plan &P, const Launch &L) {
             chk(L.sG, N, "dgamma");
             chk(L.sH, N, "dbeta");
             break;
+        case LK_ATT:
+        case LK_ATT_BWD: {
+            const uint64_t q = (uint64_t)L.att.Tq * L.att.heads * L.att.D;
+            const uint64_t kv = (uint64_t)L.att.Tk * L.att.kv_heads * L.att.D;
+            chk(L.sA, q, "q");
+            chk(L.sB, kv, "k");
+            chk(L.sZ, kv, "v");
+            chk(L.sBias, (uint64_t)L.att.n + 1, "q's starts");
+            chk(L.sExtra, (uint64_t)L.att.n + 1, "k's starts");
+            chk(L.sC, q, "out");
+            chk(L.sRstd, (uint64_t)L.att.Tq * L.att.heads, "lse");
+            chk(L.sMean, q, "dout");
+            chk(L.sG, q, "dq");
+            chk(L.sH, kv, "dk");
+            chk(L.sProbs, kv, "dv");
+            break;
+        }
         case LK_EMB:
             chk(L.sA, K * N, "table");
             chk(L.sB, M, "tokens");
@@ -1593,6 +1748,37 @@ int run(fg_plan &P, const std::vector<Launch> &list, bool step = false, bool def
                                        L.accumulate, P.ptr(L.sG), L.accumulate2, P.ptr(L.sH),
                                        L.accumulate3);
                 break;
+            case LK_RMS:
+                rc = fg_rms_norm(ctx, L.dtype, P.ptr(L.sA), L.N, nullptr, L.N, P.ptr(L.sZ),
+                                 L.value, L.M, L.N, nullptr, L.N, P.ptr(L.sC), L.N, nullptr, L.N,
+                                 nullptr, L.N, (float *)P.ptr(L.sRstd));
+                break;
+            case LK_RMS_BWD:
+                // (A gradient that is there already enters as ds, in place.)
+                rc = fg_rms_norm_bwd(ctx, L.dtype, P.ptr(L.sA), L.N, P.ptr(L.sB), L.N,
+                                     P.ptr(L.sZ), (const float *)P.ptr(L.sRstd), L.M, L.N,
+                                     L.accumulate ? P.ptr(L.sC) : nullptr, L.N, P.ptr(L.sC), L.N,
+                                     P.ptr(L.sG), L.accumulate2);
+                break;
+            case LK_ATT: {
+                const int qc = L.att.heads * L.att.D, kc = L.att.kv_heads * L.att.D;
+                rc = fg_attention(ctx, L.dtype, P.ptr(L.sA), qc, P.ptr(L.sB), kc, P.ptr(L.sZ), kc,
+                                  (const uint32_t *)P.ptr(L.sBias),
+                                  (const uint32_t *)P.ptr(L.sExtra), nullptr, L.att.n, L.att.Tq,
+                                  L.att.Tk, L.att.heads, L.att.kv_heads, L.att.D, L.value,
+                                  L.causal, P.ptr(L.sC), qc, (float *)P.ptr(L.sRstd));
+                break;
+            }
+            case LK_ATT_BWD: {
+                const int qc = L.att.heads * L.att.D, kc = L.att.kv_heads * L.att.D;
+                rc = fg_attention_bwd(
+                    ctx, L.dtype, P.ptr(L.sA), qc, P.ptr(L.sB), kc, P.ptr(L.sZ), kc, P.ptr(L.sC),
+                    qc, P.ptr(L.sMean), qc, (const float *)P.ptr(L.sRstd),
+                    (const uint32_t *)P.ptr(L.sBias), (const uint32_t *)P.ptr(L.sExtra), L.att.n,
+                    L.att.Tq, L.att.Tk, L.att.heads, L.att.kv_heads, L.att.D, L.value, L.causal,
+                    P.ptr(L.sG), qc, P.ptr(L.sH), kc, P.ptr(L.sProbs), kc, L.accumulate);
+                break;
+            }
             case LK_EMB:
                 rc = fg_embedding(ctx, L.dtype, (const uint32_t *)P.ptr(L.sB), L.M, L.K, L.N,
                                   P.ptr(L.sA), L.N, L.value, P.ptr(L.sC), L.N);
@@ -2006,6 +2192,52 @@ FG_API int fg_graph_layer_norm(fg_graph *g, uint32_t x, uint32_t gamma, uint32_t
     return FG_OK;
 }
 
+FG_API int fg_graph_rms_norm(fg_graph *g, uint32_t x, uint32_t gamma, float eps, uint32_t *node) {
+    FG_REQUIRE(g && node, FG_ERR_INVALID_ARGUMENT, "fg_graph_rms_norm: NULL argument");
+    FG_REQUIRE(eps > 0.0f && eps < INFINITY, FG_ERR_INVALID_ARGUMENT,
+               "fg_graph_rms_norm: eps must be positive and finite");
+    for (uint32_t k : {x, gamma})
+        FG_REQUIRE(k < g->nodes.size(), FG_ERR_GRAPH,
+                   "fg_graph_rms_norm: input node %u does not exist", k);
+    FG_REQUIRE(x != gamma, FG_ERR_UNSUPPORTED,
+               "fg_graph_rms_norm: x and gamma must be different nodes");
+    GNode nd;
+    nd.op = FG_OP_RMS_NORM;
+    nd.in = {x, gamma};
+    nd.value = eps;
+    g->nodes.push_back(nd);
+    *node = (uint32_t)g->nodes.size() - 1;
+    return FG_OK;
+}
+
+FG_API int fg_graph_attention(fg_graph *g, uint32_t q, uint32_t k, uint32_t v, uint32_t q_starts,
+                              uint32_t k_starts, int heads, int kv_heads, float scale, int causal,
+                              uint32_t *node) {
+    FG_REQUIRE(g && node, FG_ERR_INVALID_ARGUMENT, "fg_graph_attention: NULL argument");
+    for (uint32_t x : {q, k, v, q_starts, k_starts})
+        FG_REQUIRE(x < g->nodes.size(), FG_ERR_GRAPH,
+                   "fg_graph_attention: input node %u does not exist", x);
+    for (uint32_t x : {q_starts, k_starts})
+        FG_REQUIRE(g->nodes[x].op == FG_OP_INPUT && g->nodes[x].dtype == FG_DTYPE_U32,
+                   FG_ERR_UNSUPPORTED, "fg_graph_attention: node %u is not a u32 input", x);
+    FG_REQUIRE(q != k && q != v && k != v, FG_ERR_UNSUPPORTED,
+               "fg_graph_attention: q, k and v must be different nodes");
+    FG_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, FG_ERR_INVALID_ARGUMENT,
+               "fg_graph_attention: %d heads are no multiple of %d key heads", heads, kv_heads);
+    FG_REQUIRE(scale > 0.0f && scale < INFINITY, FG_ERR_INVALID_ARGUMENT,
+               "fg_graph_attention: scale must be positive and finite");
+    GNode nd;
+    nd.op = FG_OP_ATTENTION;
+    nd.in = {q, k, v, q_starts, k_starts};
+    nd.heads = heads;
+    nd.kv_heads = kv_heads;
+    nd.value = scale;
+    nd.causal = causal != 0;
+    g->nodes.push_back(nd);
+    *node = (uint32_t)g->nodes.size() - 1;
+    return FG_OK;
+}
+
 FG_API int fg_graph_embedding(fg_graph *g, uint32_t table, uint32_t tokens, float scale,
                               uint32_t *node) {
     FG_REQUIRE(g && node, FG_ERR_INVALID_ARGUMENT, "fg_graph_embedding: NULL argument");
@@ -2151,6 +2383,18 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
                            G.nodes[nd.in[1]].op != FG_OP_CONST && G.nodes[nd.in[2]].op != FG_OP_CONST,
                        FG_ERR_UNSUPPORTED,
                        "layer_norm %u: x, gamma and beta of different element types", i);
+        if (nd.op == FG_OP_RMS_NORM)
+            FG_REQUIRE(P->dtype[nd.in[1]] == P->dtype[i] && G.nodes[nd.in[1]].op != FG_OP_CONST,
+                       FG_ERR_UNSUPPORTED,
+                       "rms_norm %u: x and gamma of different element types", i);
+        if (nd.op == FG_OP_ATTENTION) {
+            FG_REQUIRE(P->dtype[nd.in[1]] == P->dtype[i] && P->dtype[nd.in[2]] == P->dtype[i],
+                       FG_ERR_UNSUPPORTED,
+                       "attention %u: q, k and v of different element types", i);
+            const int64_t D = P->shape[i].cols / nd.heads;
+            FG_REQUIRE(D <= 128, FG_ERR_UNSUPPORTED,
+                       "attention %u: heads of %lld columns, at most 128", i, (long long)D);
+        }
     }
     P->ce_fused_possible = G.loss == FG_LOSS_CE && G.nodes.back().op == FG_OP_SOFTMAX;
 
@@ -2251,11 +2495,13 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
         if (gr.bias_node != kNone) P->val_slot[gr.mm] = P->val_slot[gr.bias_node];
     P->mean_of.assign(nn, kNone);
     P->rstd_of.assign(nn, kNone);
-    for (uint32_t i = 0; i < nn; ++i)
-        if (G.nodes[i].op == FG_OP_LAYER_NORM) {
-            P->mean_of[i] = P->new_slot((uint64_t)P->shape[i].rows);
-            P->rstd_of[i] = P->new_slot((uint64_t)P->shape[i].rows);
-        }
+    for (uint32_t i = 0; i < nn; ++i) {
+        const int op = G.nodes[i].op;
+        const uint64_t rows = (uint64_t)P->shape[i].rows;
+        if (op == FG_OP_LAYER_NORM) P->mean_of[i] = P->new_slot(rows);
+        if (op == FG_OP_LAYER_NORM || op == FG_OP_RMS_NORM) P->rstd_of[i] = P->new_slot(rows);
+        if (op == FG_OP_ATTENTION) P->rstd_of[i] = P->new_slot(rows * G.nodes[i].heads);
+    }
     for (uint32_t i = 0; i < nn; ++i) {
         if (G.nodes[i].op == FG_OP_CONST) continue;
         if (P->needs_grad[i] || (int)i == P->last)
@@ -2328,9 +2574,18 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
                 else if (L.kind == LK_LN_BWD && (L.sG != kNone || L.sH != kNone))
                     ws = std::max<uint64_t>(ws,
                                             fg::layer_norm_bwd_ws_bytes(cus, L.dtype, L.M, L.N));
+                else if (L.kind == LK_RMS_BWD && L.sG != kNone)
+                    ws = std::max<uint64_t>(ws,
+                                            fg::rms_norm_bwd_ws_bytes(cus, L.dtype, L.M, L.N));
+                else if (L.kind == LK_ATT_BWD)
+                    ws = std::max<uint64_t>(ws,
+                                            fg::attention_bwd_ws_bytes(cus, L.dtype, L.att));
                 else if (L.kind == LK_EMB_BWD)
                     ws = std::max<uint64_t>(
                         ws, fg::embedding_bwd_ws_bytes(L.dtype, L.M, L.K, L.N));
+        for (const Launch &L : P->fwd)
+            if (L.kind == LK_ATT)
+                ws = std::max<uint64_t>(ws, fg::attention_ws_bytes(cus, L.att));
         for (auto *list : {&P->fwd, &P->bwd_seed, &P->bwd_fused})
             for (const Launch &L : *list)
                 if ((L.kind == LK_GEMM || L.kind == LK_GEMM_BWD) && L.dtype != FG_DTYPE_F32) {
@@ -2853,6 +3108,13 @@ FG_API int fg_plan_describe(const fg_plan *p, char *buf, size_t len, size_t *nee
             else if (L.kind == LK_LN_BWD)
                 n += fg::layer_norm_bwd_dispatches(wc ? wc->cu_count : 0, L.dtype, L.M, L.N,
                                                    L.sC != kNone, L.sG != kNone || L.sH != kNone);
+            else if (L.kind == LK_RMS_BWD)
+                n += fg::rms_norm_bwd_dispatches(wc ? wc->cu_count : 0, L.dtype, L.M, L.N,
+                                                 L.sC != kNone, L.sG != kNone);
+            else if (L.kind == LK_ATT)
+                n += fg::attention_dispatches(wc ? wc->cu_count : 256, L.att);
+            else if (L.kind == LK_ATT_BWD)
+                n += fg::attention_bwd_dispatches(wc ? wc->cu_count : 256, L.dtype, L.att);
             else if (L.kind == LK_EMB_BWD)
                 n += fg::embedding_bwd_dispatches(L.dtype, L.M, L.K, L.N);
             else

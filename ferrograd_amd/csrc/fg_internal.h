@@ -145,6 +145,14 @@ int embedding_bwd_dispatches(int dtype, int T, int V, int C);
 // The same two of fg_rms_norm_bwd.
 uint64_t rms_norm_bwd_ws_bytes(int cus, int dtype, int R, int C);
 int rms_norm_bwd_dispatches(int cus, int dtype, int R, int C, bool dx, bool weights);
+// And of fg_attention and its backward (the shape as those calls take it).
+struct AttentionShape {
+    int n, Tq, Tk, heads, kv_heads, D;
+};
+uint64_t attention_ws_bytes(int cus, const AttentionShape &s);
+uint64_t attention_bwd_ws_bytes(int cus, int dtype, const AttentionShape &s);
+int attention_dispatches(int cus, const AttentionShape &s);
+int attention_bwd_dispatches(int cus, int dtype, const AttentionShape &s);
 
 // Adam with device-resident step counter / bias-correction scalars
 // (k_optim.hip).  d_state points at adam_dev_state_bytes() zeroed bytes.

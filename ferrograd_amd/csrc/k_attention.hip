@@ -60,6 +60,22 @@ struct BwdSpace {
     uint64_t bytes() const { return (rows + part + kpart) * sizeof(float); }
 };
 
+// Floats of the forward's.
+uint64_t fwd_space(const Args &a) {
+    return a.splits > 1 ? (uint64_t)a.splits * a.Tq * a.KV * a.G * (a.D + 2) : 0;
+}
+
+Args args_of(const fg::AttentionShape &s) {
+    Args a{};
+    a.n = s.n;
+    a.Tq = s.Tq;
+    a.Tk = s.Tk;
+    a.KV = s.kv_heads;
+    a.G = s.heads / s.kv_heads;
+    a.D = s.D;
+    return a;
+}
+
 bool whole_chunks(const Args &a, std::initializer_list<std::pair<const void *, int64_t>> rows) {
     if (a.D != 64 && a.D != 128) return false;
     // (And a tile's rows are within 32 bits of its first.)
@@ -97,6 +113,28 @@ int check(const char *who, int dtype, const Args &a, int heads, int kv_heads) {
 
 }  // namespace
 
+uint64_t fg::attention_ws_bytes(int cus, const AttentionShape &s) {
+    Args a = args_of(s);
+    a.splits = splits_of(cus, a, few_rows(a));
+    return fwd_space(a) * sizeof(float);
+}
+
+uint64_t fg::attention_bwd_ws_bytes(int cus, int dtype, const AttentionShape &s) {
+    Args a = args_of(s);
+    set_splits(cus, dtype, a);
+    return BwdSpace(a).bytes();
+}
+
+int fg::attention_dispatches(int cus, const AttentionShape &s) {
+    return attention_ws_bytes(cus, s) ? 2 : 1;
+}
+
+int fg::attention_bwd_dispatches(int cus, int dtype, const AttentionShape &s) {
+    Args a = args_of(s);
+    set_splits(cus, dtype, a);
+    return a.splits > 1 || a.ksplits > 1 ? 3 : 2;
+}
+
 FG_API int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k, int ldk,
                         const void *d_v, int ldv, const uint32_t *d_q_starts,
                         const uint32_t *d_k_starts, const uint32_t *d_k_lens, int n, int Tq, int Tk,
@@ -127,8 +165,9 @@ FG_API int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const 
     a.ldo = ldo;
     a.lse = d_lse;
     FG_REQUIRE(ldo >= heads * D, FG_ERR_SHAPE, "%s: ldo=%d < %d heads of %d", who, ldo, heads, D);
-    FG_REQUIRE(d_q && d_k && d_v && d_q_starts && d_k_starts && d_out, FG_ERR_INVALID_ARGUMENT,
-               "%s: q, k, v, the starts and out are required", who);
+    // (What has no rows needs no memory.)
+    FG_REQUIRE((Tq == 0 || (d_q && d_out)) && (Tk == 0 || (d_k && d_v)) && d_q_starts && d_k_starts,
+               FG_ERR_INVALID_ARGUMENT, "%s: q, k, v, the starts and out are required", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     FG_REQUIRE(apart(d_out, {d_q, d_k, d_v, d_q_starts, d_k_starts, d_k_lens, d_lse}) &&
                    apart(d_lse, {d_q, d_k, d_v, d_q_starts, d_k_starts, d_k_lens}),
@@ -137,9 +176,8 @@ FG_API int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const 
     FG_HIP(hipSetDevice(ctx->device));
     const bool few = few_rows(a);
     a.splits = splits_of(ctx->cu_count, a, few);
-    const int64_t rows = (int64_t)Tq * heads;
     if (a.splits > 1) {
-        a.part = (float *)fg::workspace(ctx, (uint64_t)a.splits * rows * (D + 2) * sizeof(float));
+        a.part = (float *)fg::workspace(ctx, fwd_space(a) * sizeof(float));
         if (!a.part) return FG_ERR_OUT_OF_MEMORY;
     }
     a.slots = (int)((int64_t)Tq * a.G / (few ? fg::attn::kFewRows : fg::attn::kRows) + n);
@@ -200,15 +238,17 @@ FG_API int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, co
                "%s: ldo=%d, lddo=%d or lddq=%d < %d heads of %d", who, ldo, lddo, lddq, heads, D);
     FG_REQUIRE(lddk >= kv_heads * D && lddv >= kv_heads * D, FG_ERR_SHAPE,
                "%s: lddk=%d or lddv=%d < %d heads of %d", who, lddk, lddv, kv_heads, D);
-    FG_REQUIRE(d_q && d_k && d_v && d_out && d_dout && d_lse && d_q_starts && d_k_starts,
+    FG_REQUIRE((Tq == 0 || (d_q && d_out && d_dout && d_lse)) && (Tk == 0 || (d_k && d_v)) &&
+                   d_q_starts && d_k_starts,
                FG_ERR_INVALID_ARGUMENT, "%s: q, k, v, out, dout, lse and the starts are required",
                who);
-    FG_REQUIRE(d_dq && d_dk && d_dv, FG_ERR_INVALID_ARGUMENT, "%s: dq, dk and dv are required", who);
+    FG_REQUIRE((Tq == 0 || d_dq) && (Tk == 0 || (d_dk && d_dv)), FG_ERR_INVALID_ARGUMENT,
+               "%s: dq, dk and dv are required", who);
     FG_REQUIRE(ctx, FG_ERR_INVALID_ARGUMENT, "%s: ctx is NULL", who);
     for (const void *o : {(const void *)d_dq, (const void *)d_dk, (const void *)d_dv})
         FG_REQUIRE(apart(o, {d_q, d_k, d_v, d_out, d_dout, d_lse, d_q_starts, d_k_starts}),
                    FG_ERR_INVALID_ARGUMENT, "%s: an output is an input", who);
-    FG_REQUIRE(d_dq != d_dk && d_dq != d_dv && d_dk != d_dv, FG_ERR_INVALID_ARGUMENT,
+    FG_REQUIRE(apart(d_dq, {d_dk, d_dv}) && apart(d_dk, {d_dv}), FG_ERR_INVALID_ARGUMENT,
                "%s: an output is another output", who);
     if (n == 0 || (Tq == 0 && Tk == 0)) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));

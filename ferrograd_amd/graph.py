@@ -27,10 +27,10 @@ Differences, all deliberate:
     backend/mod.rs:617-619);
   * `bias_add` (and broadcast in add / sub) exist;
   * `Optim.adam()` exists; `SimpleDType` covers F32, F16 and BF16, and U32 for
-    the tokens of `embedding` (F64 and the other integer types have no op on
-    this path);
-  * `layer_norm`, `embedding` and `ckpt8` (an activation kept in 8 bits for the
-    backward) exist;
+    the tokens of `embedding` and the starts of `attention` (F64 and the other
+    integer types have no op on this path);
+  * `layer_norm`, `rms_norm`, `attention`, `embedding` and `ckpt8` (an activation
+    kept in 8 bits for the backward) exist;
   * after `dispatch_loss` with CROSS_ENTROPY on a final softmax the next
     `dispatch_backward` starts from dlogits = p - onehot (the reference
     pushes that gradient through the softmax Jacobian a second time);
@@ -53,6 +53,7 @@ from ._lib import FgError, call
 OP_INPUT, OP_CONST, OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_MATMUL = 0, 1, 2, 3, 4, 5, 6
 OP_RELU, OP_GELU, OP_ELU, OP_TANH, OP_EXP, OP_LOG, OP_ABS, OP_NEG = 7, 8, 9, 10, 11, 12, 13, 14
 OP_SOFTMAX, OP_BIAS_ADD, OP_LAYER_NORM, OP_EMBEDDING = 15, 16, 17, 18
+OP_RMS_NORM, OP_ATTENTION = 19, 20
 # fg_role
 ROLE_FORWARD_OUT, ROLE_SEED, ROLE_LOSS, ROLE_FORWARD_SAVED, ROLE_GRAD = 0, 1, 2, 3, 4
 ROLE_INPUT, ROLE_STATE, ROLE_MEAN_LOSS, ROLE_TARGET = 5, 6, 7, 8
@@ -157,7 +158,8 @@ class _Node:
     op: int
     inputs: List[int] = field(default_factory=list)
     fields: List[int] = field(default_factory=list)
-    value: float = 0.0  # constant; layer norm: eps; embedding: scale
+    value: float = 0.0  # constant; norms: eps; embedding, attention: scale
+    heads: Sequence[int] = ()  # attention: heads, key heads, causal
     flags: int = 0
     dtype: int = 0  # DTYPE_CODE of an input / constant
     ckpt8: bool = False
@@ -225,6 +227,20 @@ class _DefineOps:
         beta are vectors of its length."""
         return self._push(_Node(OP_LAYER_NORM, inputs=[x, gamma, beta], value=float(eps)))
 
+    def rms_norm(self, x, gamma, eps: float = 1e-5) -> int:
+        """x * rstd * gamma over the last dimension, rstd = 1/sqrt(mean(x^2) + eps);
+        gamma is a vector of its length."""
+        return self._push(_Node(OP_RMS_NORM, inputs=[x, gamma], value=float(eps)))
+
+    def attention(self, q, k, v, starts, heads: int, kv_heads: Optional[int] = None,
+                  scale: float = 1.0, causal: bool = True, k_starts=None) -> int:
+        """softmax(scale * q k^T) v of packed sequences: starts, a U32 input of n + 1
+        numbers, gives each one's rows of q, k_starts (starts) those of k and v."""
+        return self._push(_Node(OP_ATTENTION,
+                                inputs=[q, k, v, starts, starts if k_starts is None else k_starts],
+                                value=float(scale),
+                                heads=(heads, heads if kv_heads is None else kv_heads, int(causal))))
+
     def embedding(self, table, tokens, scale: float = 1.0) -> int:
         """scale * table[tokens]: one row per token of a U32 input."""
         return self._push(_Node(OP_EMBEDDING, inputs=[table, tokens], value=float(scale)))
@@ -277,8 +293,8 @@ class Graph:
                     save[u] |= 2
             elif nd.op == OP_EMBEDDING:
                 save[i] |= 3
-            elif nd.op in (OP_MUL, OP_DIV, OP_LAYER_NORM):
-                if nd.op == OP_LAYER_NORM:
+            elif nd.op in (OP_MUL, OP_DIV, OP_LAYER_NORM, OP_RMS_NORM, OP_ATTENTION):
+                if nd.op not in (OP_MUL, OP_DIV):
                     save[i] |= 3
                 for x in nd.inputs:
                     if nonleaf[x]:
@@ -305,6 +321,12 @@ class Graph:
                     call("fg_graph_constant", h, nd.dtype, nd.value, ctypes.byref(out))
                 elif nd.op == OP_LAYER_NORM:
                     call("fg_graph_layer_norm", h, *nd.inputs, nd.value, ctypes.byref(out))
+                elif nd.op == OP_RMS_NORM:
+                    call("fg_graph_rms_norm", h, *nd.inputs, nd.value, ctypes.byref(out))
+                elif nd.op == OP_ATTENTION:
+                    heads, kv_heads, causal = nd.heads
+                    call("fg_graph_attention", h, *nd.inputs, heads, kv_heads, nd.value, causal,
+                         ctypes.byref(out))
                 elif nd.op == OP_EMBEDDING:
                     call("fg_graph_embedding", h, *nd.inputs, nd.value, ctypes.byref(out))
                 else:

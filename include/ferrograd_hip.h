@@ -196,7 +196,8 @@ typedef enum fg_dtype {
     FG_DTYPE_F32 = 0,
     FG_DTYPE_F16 = 1,
     FG_DTYPE_BF16 = 2,
-    FG_DTYPE_U32 = 3 /* token inputs of a graph only (fg_graph_embedding) */
+    FG_DTYPE_U32 = 3 /* inputs of a graph only: tokens (fg_graph_embedding), starts
+                        (fg_graph_attention) */
 } fg_dtype;
 
 /* 16-bit GEMMs (dtype FG_DTYPE_F16 or FG_DTYPE_BF16 for every operand and
@@ -389,7 +390,8 @@ int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d
  * dk and dv are sums over the group's heads.  P and dS are rounded to dtype for their
  * products, outputs once; no atomics, the order of every sum is fixed.  Rows of dq, and
  * of dk and dv, of no sequence are left as they are.  The workspace takes 12 bytes a row
- * and head. */
+ * and head, and where tiles of 128 rows (or keys) are too few for the CUs, D floats for
+ * each split (at most 32) of every row of dq (of dk and dv). */
 int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k, int ldk,
                      const void *d_v, int ldv, const void *d_out, int ldo, const void *d_dout,
                      int lddo, const float *d_lse, const uint32_t *d_q_starts,
@@ -631,7 +633,9 @@ typedef enum fg_op {
     FG_OP_SOFTMAX = 15,
     FG_OP_BIAS_ADD = 16,
     FG_OP_LAYER_NORM = 17, /* built by fg_graph_layer_norm */
-    FG_OP_EMBEDDING = 18   /* built by fg_graph_embedding  */
+    FG_OP_EMBEDDING = 18,  /* built by fg_graph_embedding  */
+    FG_OP_RMS_NORM = 19,   /* built by fg_graph_rms_norm   */
+    FG_OP_ATTENTION = 20   /* built by fg_graph_attention  */
 } fg_op;
 
 /* Input flags (extension): every Input is trainable in ferrograd
@@ -650,7 +654,7 @@ int fg_graph_new_field(fg_graph *g, uint32_t *field);
 int fg_graph_input(fg_graph *g, const uint32_t *fields, int rank, uint32_t *node);
 /* DefineOps::input(&[fields], SimpleDType) (graph.rs:111, backend/mod.rs:
  * 335-427): an input of element type dtype (FG_DTYPE_F32 / F16 / BF16, or U32
- * for tokens, which take no gradient and no update).  Operations take the type
+ * for tokens and starts, which take no gradient and no update).  Operations take the type
  * of their first input. */
 int fg_graph_input_x(fg_graph *g, const uint32_t *fields, int rank, int dtype,
                      uint32_t *node);
@@ -667,6 +671,17 @@ int fg_graph_op(fg_graph *g, int op, const uint32_t *inputs, int n_inputs, uint3
  * is fg_layer_norm, the backward fg_layer_norm_bwd. */
 int fg_graph_layer_norm(fg_graph *g, uint32_t x, uint32_t gamma, uint32_t beta, float eps,
                         uint32_t *node);
+/* RMS norm over the last dimension of x[..., N] with gamma[N] (two different nodes of
+ * one element type; no reference counterpart): the forward is fg_rms_norm, the backward
+ * fg_rms_norm_bwd. */
+int fg_graph_rms_norm(fg_graph *g, uint32_t x, uint32_t gamma, float eps, uint32_t *node);
+/* Attention over packed sequences (no reference counterpart): fg_attention and
+ * fg_attention_bwd of q[Tq][heads D], k and v[Tk][kv_heads D] (three different nodes of
+ * one element type), with q_starts and k_starts[n + 1] u32 inputs, which may be one
+ * input.  Rows of no sequence are 0, their gradients too. */
+int fg_graph_attention(fg_graph *g, uint32_t q, uint32_t k, uint32_t v, uint32_t q_starts,
+                       uint32_t k_starts, int heads, int kv_heads, float scale, int causal,
+                       uint32_t *node);
 /* The lookup scale * table[tokens] of a u32 input in a table[V][N] (no reference
  * counterpart): a matrix of one row per token.  fg_embedding, and for the
  * table's gradient fg_embedding_bwd.  A table may also feed other nodes (a tied
