@@ -48,6 +48,7 @@ struct Args {
     float *rows;   // [3][KV Tq G]: log2 of the sum, delta, the largest |dout|
     float *kpart;  // ksplits > 1: dK's and dV's sums, [2][ksplits][KV Tk][D] (dQ's: part)
     int kslots, ksplits, accumulate;
+    int fill;  // workgroups that the splits are to come to
 };
 
 // Rows of a workgroup (of the few rows' one), and keys of one in the backward's pass over

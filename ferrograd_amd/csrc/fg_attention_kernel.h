@@ -402,6 +402,18 @@ __device__ __forceinline__ void landed() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// A tile is in LDS.  Through registers the wave's loads had landed before it was stored;
+// the builtin says so to the compiler here too.
+template <bool DMA>
+__device__ __forceinline__ void staged() {
+    if constexpr (DMA) {
+        landed();
+    } else {
+        wait_vmcnt<0>();
+        __syncthreads();
+    }
+}
+
 // ------------------------------------------------------------------ sequences
 // Sequence of work slot `slot` and its tile there: sequence s has the slots from
 // start(s) = first(s) / per + s on (first: its first row, or key), at least as many as
@@ -436,6 +448,44 @@ struct Seq {
         k0 = (int)min(a.ks[s], (uint32_t)a.Tk);
         lk = max(0, (int)min(a.ks[s + 1], (uint32_t)a.Tk) - k0);
         if (a.klens) lk = (int)min((uint32_t)lk, a.klens[s]);
+    }
+};
+
+// Tiles of a split in the backward: the same for all sequences, so that a long one has
+// more splits and no workgroup many times the work of the others.  With w workgroups of t
+// tiles each in a sequence's pass, those of p tiles are at most sum(w t) / p + sum(w):
+// `fill` with this p (128 rows or keys at least).  A wave computes it from the starts.
+// (Five sequences of up to 777 tokens, 6 heads of 72 over 3, fp32: equal splits of every
+// sequence took 200 us in the two passes.)
+template <int KT, bool KEYS>
+__device__ __forceinline__ int split_tiles(const Args &a) {
+    constexpr int kLeast = 128 / KT, kWg = KEYS ? kKeys : kRows;
+    float work = 0.0f, wgs = 0.0f;
+    for (int s = threadIdx.x & 63; s < a.n; s += 64) {
+        const Seq sq(a, s);
+        const int rows = sq.lq * a.G, of = KEYS ? sq.lk : rows, over = KEYS ? rows : sq.lk;
+        const float w = (float)((of + kWg - 1) / kWg);
+        wgs += w;
+        // (Explicitly fused: every kernel that asks gets the same number.)
+        work = __builtin_fmaf(w, (float)((over + KT - 1) / KT), work);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        work += __shfl_xor(work, o);
+        wgs += __shfl_xor(wgs, o);
+    }
+    const float p = (a.causal ? 0.5f : 1.0f) * work * a.KV / fmaxf(1.0f, a.fill - wgs * a.KV);
+    return __builtin_amdgcn_readfirstlane(max(kLeast, (int)fminf(p, 1e6f) + 1));
+}
+
+// Tiles of split y, from the first on; used: splits that have any, or 1.
+struct Share {
+    int t0, t1, used;
+    __device__ __forceinline__ Share(int tiles, int splits, int each, int y) {
+        const int per = max(each, (tiles - 1) / splits + 1);
+        t0 = min(y * per, max(tiles, 0));
+        t1 = min(t0 + per, max(tiles, 0));
+        used = tiles > 0 ? (tiles - 1) / per + 1 : 1;
     }
 };
 
@@ -760,8 +810,7 @@ att_fwd(const Args a) {
     }
     for (int t = t0; t < t1; ++t) {
         // The tile has landed, and every wave is done with the one before it.
-        if constexpr (DMA) landed();
-        else __syncthreads();
+        staged<DMA>();
         if (t + 1 < t1) load(t + 1);
         const int key0 = t * KT;
         const T *at = lds + (t & 1) * 2 * Tl::kElems;
@@ -1125,8 +1174,9 @@ att_bwd_q(const Args a) {
     const int wave_last = w0 < rows ? last_of(min(w0 + 32, rows) - 1) : -1;
     const int keys = last_of(min(m0 + kRows, rows) - 1) + 1;
     const int tiles = keys > 0 ? (keys - 1) / KT + 1 : 0;
-    const int t0 = (int)((int64_t)tiles * blockIdx.y / a.splits);
-    const int t1 = (int)((int64_t)tiles * (blockIdx.y + 1) / a.splits);
+    const Share share(tiles, a.splits, a.splits > 1 ? split_tiles<KT, false>(a) : 1, blockIdx.y);
+    if ((int)blockIdx.y >= share.used) return;
+    const int t0 = share.t0, t1 = share.t1;
 
     typename Ty::Frag q[NK], dout[NK];
     const int row = w0 + l32;
@@ -1192,8 +1242,7 @@ att_bwd_q(const Args a) {
         store(t0);
     }
     for (int t = t0; t < t1; ++t) {
-        if constexpr (DMA) landed();
-        else __syncthreads();
+        staged<DMA>();
         if (t + 1 < t1) load(t + 1);
         const int key0 = t * KT;
         const T *kt = lds + (t & 1) * 2 * Tl::kElems, *vt = kt + Tl::kElems;
@@ -1283,6 +1332,9 @@ att_bwd_kv(const Args a) {
     auto first_of = [&](int key) {
         return key >= sq.lk ? rows : a.causal ? max(0, key - off) * a.G : 0;
     };
+    const int begin = first_of(n0) / RT, tiles = rows > 0 ? (rows - 1) / RT + 1 - begin : 0;
+    const Share share(tiles, a.ksplits, a.ksplits > 1 ? split_tiles<RT, true>(a) : 1, blockIdx.y);
+    if ((int)blockIdx.y >= share.used) return;
     const int kw = n0 + 32 * wave;
     const int wave_first = first_of(kw), wave_last = first_of(kw + 31);
 
@@ -1343,9 +1395,7 @@ att_bwd_kv(const Args a) {
     clear(dv);
     int up = 0;  // fp16: the power of two that dK carries
     bool any = false;
-    const int begin = first_of(n0) / RT, tiles = rows > 0 ? (rows - 1) / RT + 1 - begin : 0;
-    const int t0 = begin + (int)((int64_t)max(tiles, 0) * blockIdx.y / a.ksplits);
-    const int t1 = begin + (int)((int64_t)max(tiles, 0) * (blockIdx.y + 1) / a.ksplits);
+    const int t0 = begin + share.t0, t1 = begin + share.t1;
     if (t0 < t1) {
         Mover<DT, DP, kKeys, 256, DMA> mv;
         mv.load(vlds, tid,
@@ -1356,8 +1406,7 @@ att_bwd_kv(const Args a) {
         store(t0);
     }
     for (int t = t0; t < t1; ++t) {
-        if constexpr (DMA) landed();
-        else __syncthreads();
+        staged<DMA>();
         if (t + 1 < t1) load(t + 1);
         const int r0 = t * RT;
         const T *qt = lds + (t & 1) * 2 * Tl::kElems, *dt = qt + Tl::kElems;
@@ -1485,7 +1534,13 @@ __global__ __launch_bounds__(256) void att_bwd_combine(const Args a) {
              (int64_t)(kv * a.G + row - token * a.G) * a.D;
         p = a.part + at * a.D;
         step = rows * a.D;
-        splits = a.splits;
+        // (The tiles of its workgroup in the pass over the rows.)
+        constexpr int KT = keys_of<DT>();
+        const int all = sq.lq * a.G;
+        const int end = min(((token - sq.q0) * a.G + row - token * a.G) / kRows * kRows + kRows, all);
+        const int keys =
+            a.causal ? min(sq.lk, a.group.of(end - 1) + sq.lk - sq.lq + 1) : sq.lk;
+        splits = Share(keys > 0 ? (keys - 1) / KT + 1 : 0, a.splits, split_tiles<KT, false>(a), 0).used;
     } else {
         at -= rows;
         const bool value = at >= keys;
@@ -1499,7 +1554,11 @@ __global__ __launch_bounds__(256) void att_bwd_combine(const Args a) {
              (int64_t)kv * a.D;
         p = a.kpart + ((value ? a.ksplits * keys : 0) + at) * a.D;
         step = keys * a.D;
-        splits = a.ksplits;
+        const int all = sq.lq * a.G, n0 = (key - sq.k0) / kKeys * kKeys;
+        const int begin = (a.causal ? max(0, n0 - (sq.lk - sq.lq)) * a.G : 0) / 32;
+        splits = Share(all > 0 ? (all - 1) / 32 + 1 - begin : 0, a.ksplits,
+                       split_tiles<32, true>(a), 0)
+                     .used;
     }
     float acc[2] = {0.0f, 0.0f};
 #pragma unroll 4

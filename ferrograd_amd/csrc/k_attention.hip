@@ -31,11 +31,13 @@ int splits_of(int cus, const Args &a, bool few) {
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
 }
 
-// Splits of the backward's passes: of `sum` rows (keys) a sequence on average, for one of
-// `tiles` workgroups, 128 at least each, up to `fill` workgroups.
-int bwd_splits(int fill, int64_t tiles, int64_t sum) {
+// Splits of a backward pass that sums over `all` rows (or keys) of n sequences, with
+// `tiles` workgroups unsplit: for a sequence of average length as many as bring `fill`
+// workgroups, of 128 at least; for the longest up to four times as many.
+void bwd_splits(int fill, int64_t tiles, int64_t all, int n, int &splits) {
     const int64_t want = fill / std::max<int64_t>(tiles, 1);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, sum / 128, kMaxSplits}));
+    const int64_t of = std::min<int64_t>({want, all / n / 128, kMaxSplits});
+    splits = of <= 1 ? 1 : (int)std::min<int64_t>({4 * of, all / 128, kMaxSplits});
 }
 
 // (A CU holds two workgroups, of fp32 one.)
@@ -44,8 +46,11 @@ void set_splits(int cus, int dtype, Args &a) {
     const int64_t rows = (int64_t)a.Tq * a.G;
     const int64_t q_tiles = std::max<int64_t>(a.n, (rows - 1) / fg::attn::kRows + 1) * a.KV;
     const int64_t k_tiles = std::max<int64_t>(a.n, ((int64_t)a.Tk - 1) / fg::attn::kKeys + 1) * a.KV;
-    a.splits = bwd_splits(fill, q_tiles, a.Tk / a.n);
-    a.ksplits = bwd_splits(fill, k_tiles, rows / a.n);
+    bwd_splits(fill, q_tiles, a.Tk, a.n, a.splits);
+    bwd_splits(fill, k_tiles, rows, a.n, a.ksplits);
+    // (Those are not spread over the XCDs evenly: one more than the CUs of one hold is a
+    // second round.  fp32: 162 us where 7 / 8 are filled, 195 where all.)
+    a.fill = fill - fill / 8;
 }
 
 // Floats of the backward's workspace.
