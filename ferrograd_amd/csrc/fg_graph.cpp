@@ -2585,7 +2585,7 @@ FG_API int fg_plan_create(fg_ctx *ctx, const fg_graph *g, const uint32_t *meta, 
                         ws, fg::embedding_bwd_ws_bytes(L.dtype, L.M, L.K, L.N));
         for (const Launch &L : P->fwd)
             if (L.kind == LK_ATT)
-                ws = std::max<uint64_t>(ws, fg::attention_ws_bytes(cus, L.att));
+                ws = std::max<uint64_t>(ws, fg::attention_ws_bytes(cus, L.dtype, L.att));
         for (auto *list : {&P->fwd, &P->bwd_seed, &P->bwd_fused})
             for (const Launch &L : *list)
                 if ((L.kind == LK_GEMM || L.kind == LK_GEMM_BWD) && L.dtype != FG_DTYPE_F32) {
@@ -3112,7 +3112,7 @@ FG_API int fg_plan_describe(const fg_plan *p, char *buf, size_t len, size_t *nee
                 n += fg::rms_norm_bwd_dispatches(wc ? wc->cu_count : 0, L.dtype, L.M, L.N,
                                                  L.sC != kNone, L.sG != kNone);
             else if (L.kind == LK_ATT)
-                n += fg::attention_dispatches(wc ? wc->cu_count : 256, L.att);
+                n += fg::attention_dispatches(wc ? wc->cu_count : 256, L.dtype, L.att);
             else if (L.kind == LK_ATT_BWD)
                 n += fg::attention_bwd_dispatches(wc ? wc->cu_count : 256, L.dtype, L.att);
             else if (L.kind == LK_EMB_BWD)

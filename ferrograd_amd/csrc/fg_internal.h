@@ -149,9 +149,9 @@ int rms_norm_bwd_dispatches(int cus, int dtype, int R, int C, bool dx, bool weig
 struct AttentionShape {
     int n, Tq, Tk, heads, kv_heads, D;
 };
-uint64_t attention_ws_bytes(int cus, const AttentionShape &s);
+uint64_t attention_ws_bytes(int cus, int dtype, const AttentionShape &s);
 uint64_t attention_bwd_ws_bytes(int cus, int dtype, const AttentionShape &s);
-int attention_dispatches(int cus, const AttentionShape &s);
+int attention_dispatches(int cus, int dtype, const AttentionShape &s);
 int attention_bwd_dispatches(int cus, int dtype, const AttentionShape &s);
 
 // Adam with device-resident step counter / bias-correction scalars

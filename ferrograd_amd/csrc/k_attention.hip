@@ -18,25 +18,41 @@ using fg::rows::apart;
 constexpr int kMaxD = 128;      // columns of a head
 constexpr int kMaxSplits = 32;  // of a row's keys
 
-// Few rows a sequence (single tokens): the kernel whose waves share out the keys.
+// Few rows a sequence (single tokens).
 bool few_rows(const Args &a) { return (int64_t)a.Tq * a.G <= (int64_t)a.n * fg::attn::kFewRows; }
 
-// Splits of each sequence's keys, from what the host knows: workgroups for every CU,
-// and no fewer than 512 keys each of a sequence of average length.
-int splits_of(int cus, const Args &a, bool few) {
+// Whether few rows go to the kernel whose waves share out the keys, rather than to the
+// one of 128 rows, of which most are idle.  fp32, always: the idle rows' products are what
+// bounds the other (single tokens over caches of up to 8192, 16 heads of 128 over 4:
+// 1 token 46 us and 96, 8 tokens 79 and 166, 64 tokens 340 and 698).  16 bits, where heads
+// and sequences are few and rows lie on 16-byte boundaries (32 heads of 128 over 8: 1
+// token 24 and 28, 8 tokens 39 and 41); of more the other brings the bytes sooner (64
+// tokens 239 and 200, 8 tokens of 16 heads over 16 82 and 69, 8 rows off the boundaries
+// 62 and 49).
+bool few_kernel(int cus, int dtype, const Args &a, bool aligned) {
+    return few_rows(a) &&
+           (dtype == FG_DTYPE_F32 || (aligned && (int64_t)a.n * a.KV * 4 <= cus));
+}
+
+// Splits of each sequence's keys, from what the host knows: two workgroups for every CU
+// (fp32's few rows, and where few rows have as many workgroups as CUs unsplit, four: the
+// sequences' lengths differ; 64 tokens, 8 heads' keys, one split 242 us, two 200, four
+// 212), and no fewer than 512 keys each of a sequence of average length.
+int splits_of(int cus, int dtype, const Args &a, bool few) {
     const int per = few ? fg::attn::kFewRows : fg::attn::kRows;
     const int64_t tiles = std::max<int64_t>(a.n, ((int64_t)a.Tq * a.G + per - 1) / per) * a.KV;
-    const int64_t want = (few ? 8 : 2) * (int64_t)cus / std::max<int64_t>(tiles, 1);
+    const bool four = few ? dtype == FG_DTYPE_F32 : few_rows(a) && tiles >= cus;
+    const int64_t want = (four ? 4 : 2) * (int64_t)cus / std::max<int64_t>(tiles, 1);
     const int64_t most = (int64_t)a.Tk / a.n / 512;
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
 }
 
 // Splits of a backward pass that sums over `all` rows (or keys) of n sequences, with
 // `tiles` workgroups unsplit: for a sequence of average length as many as bring `fill`
-// workgroups, of 128 at least; for the longest up to four times as many.
-void bwd_splits(int fill, int64_t tiles, int64_t all, int n, int &splits) {
+// workgroups, of `least` at least; for the longest up to four times as many.
+void bwd_splits(int fill, int least, int64_t tiles, int64_t all, int n, int &splits) {
     const int64_t want = fill / std::max<int64_t>(tiles, 1);
-    const int64_t of = std::min<int64_t>({want, all / n / 128, kMaxSplits});
+    const int64_t of = std::min<int64_t>({want, all / n / least, kMaxSplits});
     splits = of <= 1 ? 1 : (int)std::min<int64_t>({4 * of, all / 128, kMaxSplits});
 }
 
@@ -46,8 +62,15 @@ void set_splits(int cus, int dtype, Args &a) {
     const int64_t rows = (int64_t)a.Tq * a.G;
     const int64_t q_tiles = std::max<int64_t>(a.n, (rows - 1) / fg::attn::kRows + 1) * a.KV;
     const int64_t k_tiles = std::max<int64_t>(a.n, ((int64_t)a.Tk - 1) / fg::attn::kKeys + 1) * a.KV;
-    bwd_splits(fill, q_tiles, a.Tk, a.n, a.splits);
-    bwd_splits(fill, k_tiles, rows, a.n, a.ksplits);
+    // Many workgroups' splits pay for their sums' way through memory only where they are
+    // long.  (8 heads of 128, bf16, in splits of 128 and unsplit: one sequence of 512 49 us
+    // and 57, of 1024 67 and 91, four of 512 75 and 58.  fp32, heads of 64: four of 512
+    // 139 and 153.)
+    auto least = [&](int64_t tiles) {
+        return dtype != FG_DTYPE_F32 && tiles * 4 > cus ? 512 : 128;
+    };
+    bwd_splits(fill, least(q_tiles), q_tiles, a.Tk, a.n, a.splits);
+    bwd_splits(fill, least(k_tiles), k_tiles, rows, a.n, a.ksplits);
     // (Those are not spread over the XCDs evenly: one more than the CUs of one hold is a
     // second round.  fp32: 162 us where 7 / 8 are filled, 195 where all.)
     a.fill = fill - fill / 8;
@@ -81,13 +104,13 @@ Args args_of(const fg::AttentionShape &s) {
     return a;
 }
 
-bool whole_chunks(const Args &a, std::initializer_list<std::pair<const void *, int64_t>> rows) {
-    if (a.D != 64 && a.D != 128) return false;
-    // (And a tile's rows are within 32 bits of its first.)
+// Rows of 16-bit elements at 16-byte boundaries, a tile's within 32 bits of its first.
+bool aligned(std::initializer_list<std::pair<const void *, int64_t>> rows) {
     for (const auto &r : rows)
         if (((uintptr_t)r.first & 15) || r.second % 8 || r.second >= 1 << 24) return false;
     return true;
 }
+bool whole_chunks(const Args &a) { return a.D == 64 || a.D == 128; }
 
 // What both directions ask of their arguments.
 int check(const char *who, int dtype, const Args &a, int heads, int kv_heads) {
@@ -118,10 +141,14 @@ int check(const char *who, int dtype, const Args &a, int heads, int kv_heads) {
 
 }  // namespace
 
-uint64_t fg::attention_ws_bytes(int cus, const AttentionShape &s) {
+uint64_t fg::attention_ws_bytes(int cus, int dtype, const AttentionShape &s) {
     Args a = args_of(s);
-    a.splits = splits_of(cus, a, few_rows(a));
-    return fwd_space(a) * sizeof(float);
+    uint64_t most = 0;  // (whatever the rows' alignment)
+    for (bool on : {false, true}) {
+        a.splits = splits_of(cus, dtype, a, few_kernel(cus, dtype, a, on));
+        most = std::max(most, fwd_space(a) * sizeof(float));
+    }
+    return most;
 }
 
 uint64_t fg::attention_bwd_ws_bytes(int cus, int dtype, const AttentionShape &s) {
@@ -130,8 +157,8 @@ uint64_t fg::attention_bwd_ws_bytes(int cus, int dtype, const AttentionShape &s)
     return BwdSpace(a).bytes();
 }
 
-int fg::attention_dispatches(int cus, const AttentionShape &s) {
-    return attention_ws_bytes(cus, s) ? 2 : 1;
+int fg::attention_dispatches(int cus, int dtype, const AttentionShape &s) {
+    return attention_ws_bytes(cus, dtype, s) ? 2 : 1;
 }
 
 int fg::attention_bwd_dispatches(int cus, int dtype, const AttentionShape &s) {
@@ -179,14 +206,14 @@ FG_API int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const 
                FG_ERR_INVALID_ARGUMENT, "%s: an output is another output or an input", who);
     if (n == 0 || Tq == 0) return FG_OK;
     FG_HIP(hipSetDevice(ctx->device));
-    const bool few = few_rows(a);
-    a.splits = splits_of(ctx->cu_count, a, few);
+    const bool on = aligned({{d_k, ldk}, {d_v, ldv}}), dma = on && whole_chunks(a);
+    const bool few = few_kernel(ctx->cu_count, dtype, a, on);
+    a.splits = splits_of(ctx->cu_count, dtype, a, few);
     if (a.splits > 1) {
         a.part = (float *)fg::workspace(ctx, fwd_space(a) * sizeof(float));
         if (!a.part) return FG_ERR_OUT_OF_MEMORY;
     }
     a.slots = (int)((int64_t)Tq * a.G / (few ? fg::attn::kFewRows : fg::attn::kRows) + n);
-    const bool dma = whole_chunks(a, {{d_k, ldk}, {d_v, ldv}});
     auto launch = dtype == FG_DTYPE_F32    ? fg::attn::forward<fg::kF32>
                   : dtype == FG_DTYPE_BF16 ? fg::attn::forward<fg::kBF16>
                                            : fg::attn::forward<fg::kF16>;
@@ -266,7 +293,8 @@ FG_API int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, co
     a.kpart = a.part + need.part;
     a.slots = (int)((int64_t)Tq * a.G / fg::attn::kRows + n);
     a.kslots = Tk / fg::attn::kKeys + n;
-    const bool dma = whole_chunks(a, {{d_q, ldq}, {d_k, ldk}, {d_v, ldv}, {d_dout, lddo}});
+    const bool dma =
+        whole_chunks(a) && aligned({{d_q, ldq}, {d_k, ldk}, {d_v, ldv}, {d_dout, lddo}});
     auto launch = dtype == FG_DTYPE_F32    ? fg::attn::backward<fg::kF32>
                   : dtype == FG_DTYPE_BF16 ? fg::attn::backward<fg::kBF16>
                                            : fg::attn::backward<fg::kF16>;

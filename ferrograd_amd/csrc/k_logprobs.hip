@@ -414,8 +414,9 @@ int splits_of(int cus, int R, int C) {
 
 template <int DT>
 void launch_fwd(hipStream_t st, int R, const Fwd &a) {
-    // A wave a row up to 2 chunks a lane, else four waves.
-    if (a.C / Io<DT>::E <= 128) logprobs_fwd<DT, 64><<<R, 64, 0, st>>>(a);
+    // A wave a row up to 8 chunks a lane, else four waves (8192 rows of bf16, a wave and
+    // four: 2048 columns 8.6 and 13.6 us, 4096 14.6 and 18.1, 16384 44 and 42).
+    if (a.C / Io<DT>::E <= 512) logprobs_fwd<DT, 64><<<R, 64, 0, st>>>(a);
     else logprobs_fwd<DT, 256><<<dim3(R, a.splits), 256, 0, st>>>(a);
     if (a.splits > 1) logprobs_join<DT><<<R, 256, 0, st>>>(a);
 }

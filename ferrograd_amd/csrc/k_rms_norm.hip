@@ -428,8 +428,10 @@ bool fwd_kind(int chunks, F f) {
     return FG_RMS(1, 16, 16) || FG_RMS(1, 64, 4) || FG_RMS(2, 64, 4) || FG_RMS(2, 256, 1) ||
            FG_RMS(4, 256, 1) || FG_RMS(4, 512, 1) || FG_RMS(4, 1024, 1) || FG_RMS(8, 1024, 1);
 }
+// longer: rows of up to 2048 chunks too.  fp32's (4096 x 8192: 103 us, the longer rows'
+// kernels 142); of 16 bits they take two registers a column more (4096 x 16384: 192 and 151).
 template <class F>
-bool bwd_kind(int chunks, F f) {
+bool bwd_kind(int chunks, bool longer, F f) {
     auto with = [&](auto nv, auto l, auto ng) {
         if (chunks > nv() * l()) return false;
         f(nv, l, ng);
@@ -437,7 +439,7 @@ bool bwd_kind(int chunks, F f) {
     };
     using std::integral_constant;
     return FG_RMS(1, 16, 32) || FG_RMS(1, 64, 8) || FG_RMS(1, 128, 4) || FG_RMS(1, 256, 2) ||
-           FG_RMS(1, 512, 1) || FG_RMS(2, 512, 1) || FG_RMS(2, 1024, 1);
+           FG_RMS(1, 512, 1) || FG_RMS(2, 512, 1) || (longer && FG_RMS(2, 1024, 1));
 }
 #undef FG_RMS
 
@@ -452,7 +454,7 @@ struct Split {
 Split split_of(int cus, int dtype, int R, int C) {
     Split s;
     const int chunks = chunks_of(dtype, C);
-    s.held = bwd_kind(chunks, [&](auto, auto l, auto ng) {
+    s.held = bwd_kind(chunks, dtype == FG_DTYPE_F32, [&](auto, auto l, auto ng) {
         const int per_cu = std::max(1, 512 / (l() * ng()));
         s.splits = std::min(R > 0 ? (R - 1) / ng() + 1 : 0, cus * per_cu);
     });
@@ -486,7 +488,7 @@ int launch_bwd(fg_ctx *ctx, const Split &s, Bwd<void> v) {
                    s.rows};
     hipStream_t st = ctx->stream;
     if (s.held) {
-        bwd_kind((a.C - 1) / Io<DT>::E + 1, [&](auto nv, auto l, auto ng) {
+        bwd_kind((a.C - 1) / Io<DT>::E + 1, DT == fg::kF32, [&](auto nv, auto l, auto ng) {
             const size_t lds = ng() > 1 && a.partial ? (size_t)a.C * sizeof(float) : 0;
             rms_bwd<DT, nv(), l(), ng()><<<s.splits, l() * ng(), lds, st>>>(a);
         });
