@@ -743,7 +743,14 @@ __device__ void careful_fwd(const Args &a, const Seq &sq, int kv, int split, int
     }
 }
 
-// Four waves of 32 rows, the same keys for all: K and V tiles of KT keys, two stages.
+// Four waves of 32 rows, the same keys for all: K and V tiles of KT keys, two stages.  (A
+// wave's 32 queries and their sums take half of its registers at D 128 with two waves a
+// SIMD, which 16 bits need to hide the exponentials behind the other wave's products.)
+// bf16, 8 sequences of up to 4096, 32 heads of 128 over 8, causal: 680 us, 860 TFLOP/s,
+// where a square library product reaches 1213: bound by power, at 2.0 GHz (matrix units
+// busy 38 % of the cycles; reads sent further ahead, wave priorities and fewer maxima all
+// left 687 to 694).  Tiles that come through registers (heads of other widths, rows off
+// 16-byte boundaries): 4 sequences of 2048, 175 us and 187.
 template <int DT>
 constexpr int keys_of() {
     return DT == kF32 ? 32 : 64;
@@ -844,7 +851,8 @@ att_fwd(const Args a) {
 // Bound by the keys' and values' bytes: a wave's next keys load into the registers that
 // hold this tile's as soon as its scores are taken, the next values as soon as these have
 // gone to the wave's LDS (for the transposing reads), so that about 16 KiB a wave, 128 a
-// CU, are in flight.  FULL: heads of DP columns.
+// CU, are in flight.  FULL: heads of DP columns.  8 tokens over caches of up to 8192, bf16,
+// 32 heads of 128 over 8: 32 us.
 constexpr int kFewKeys = 32;
 template <int DT, int DP, bool FULL>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
@@ -1146,6 +1154,8 @@ __device__ void careful_bwd_kv(const Args &a, const Seq &sq, int kv, int key0, i
 
 // dQ, 32 rows a wave, in the forward's layout; and for the pass over the keys, in the
 // order of the key head's rows, log2 of their sums, delta and (fp16) their largest |dout|.
+// bf16, 8 sequences of up to 4096, 32 heads of 128 over 8: 0.95 ms, 930 TFLOP/s of its
+// three products.
 template <int DT, int DP, bool DMA>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
 att_bwd_q(const Args a) {
@@ -1305,6 +1315,9 @@ att_bwd_q(const Args a) {
 // ahead into (D 128: each matrix instruction waited for its LDS read, and spilled operands
 // for the next tile's loads in flight; 8 sequences of up to 4096, 32 heads over 8: 2.05 ms
 // and 1.6), and 64 keys a wave, for half the LDS reads, leave one wave a SIMD (2.3 ms).
+// Its four products are 740 TFLOP/s, less than dQ's three by what its LDS reads (five
+// operands of each tile) add beside them.  Through registers at D 128 the tiles' addresses spill (bf16, 4 sequences of 2048:
+// backward 0.66 ms in all, off 16-byte boundaries 1.8).
 template <int DT, int DP, bool DMA>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
 att_bwd_kv(const Args a) {

@@ -26,23 +26,24 @@ bool few_rows(const Args &a) { return (int64_t)a.Tq * a.G <= (int64_t)a.n * fg::
 // bounds the other (single tokens over caches of up to 8192, 16 heads of 128 over 4:
 // 1 token 46 us and 96, 8 tokens 79 and 166, 64 tokens 340 and 698).  16 bits, where heads
 // and sequences are few and rows lie on 16-byte boundaries (32 heads of 128 over 8: 1
-// token 24 and 28, 8 tokens 39 and 41); of more the other brings the bytes sooner (64
-// tokens 239 and 200, 8 tokens of 16 heads over 16 82 and 69, 8 rows off the boundaries
-// 62 and 49).
+// token 24 and 28, 8 tokens 32 and 33, of heads of 64 22 and 25); of more the other brings
+// the bytes sooner (32 tokens 134 and 122, 64 tokens 233 and 224, 8 tokens off the
+// boundaries 51 and 38).
 bool few_kernel(int cus, int dtype, const Args &a, bool aligned) {
     return few_rows(a) &&
            (dtype == FG_DTYPE_F32 || (aligned && (int64_t)a.n * a.KV * 4 <= cus));
 }
 
-// Splits of each sequence's keys, from what the host knows: two workgroups for every CU
-// (fp32's few rows, and where few rows have as many workgroups as CUs unsplit, four: the
-// sequences' lengths differ; 64 tokens, 8 heads' keys, one split 242 us, two 200, four
-// 212), and no fewer than 512 keys each of a sequence of average length.
+// Splits of each sequence's keys, from what the host knows, of no fewer than 512 keys in a
+// sequence of average length: two workgroups for every CU, fp32's few rows four; eight
+// where few rows have as many workgroups as CUs unsplit, since the sequences' lengths
+// differ (up to 8192 at random, 32 heads of 128 over 8, two and eight a CU: 32 tokens 127
+// us and 122, 64 tokens 238 and 224, 8 tokens 33 and 41).
 int splits_of(int cus, int dtype, const Args &a, bool few) {
     const int per = few ? fg::attn::kFewRows : fg::attn::kRows;
     const int64_t tiles = std::max<int64_t>(a.n, ((int64_t)a.Tq * a.G + per - 1) / per) * a.KV;
-    const bool four = few ? dtype == FG_DTYPE_F32 : few_rows(a) && tiles >= cus;
-    const int64_t want = (four ? 4 : 2) * (int64_t)cus / std::max<int64_t>(tiles, 1);
+    const int a_cu = few ? (dtype == FG_DTYPE_F32 ? 4 : 2) : few_rows(a) && tiles >= cus ? 8 : 2;
+    const int64_t want = a_cu * (int64_t)cus / std::max<int64_t>(tiles, 1);
     const int64_t most = (int64_t)a.Tk / a.n / 512;
     return (int)std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits}));
 }

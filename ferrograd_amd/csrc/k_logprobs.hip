@@ -13,7 +13,10 @@
 //
 // Both are bound by HBM, and in 16 bits by the vector unit beside it: the forward reads
 // a row once, with a running maximum and sums a thread that are raised together; the
-// backward reads and writes each logit once.
+// backward reads and writes each logit once.  fp32 4096 x 50257 with 5 alternatives: 155
+// us, 5.3 TB/s (a large copy reaches 4.9); bf16 64 x 131072 with 20: 15, of which the
+// splits' pass is 10.6 and their join 5 (7.5 in all without alternatives); backward, bf16
+// 8192 x 32000, a quarter of the rows padding: 183 us, 5 TB/s.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -407,7 +410,8 @@ __global__ __launch_bounds__(kBwdNT) void logprobs_bwd(const Bwd a) {
 }
 
 // Splits of each row's columns: of few long rows, as many as give every CU two
-// workgroups, of at least 8192 columns.
+// workgroups, of at least 8192 columns (64 x 131072 bf16, 20 alternatives: unsplit 21 us,
+// two a CU 14, four 19; splits of 4096 to 16384 columns alike).
 int splits_of(int cus, int R, int C) {
     return std::max(1, std::min({2 * cus / R, C / 8192, kMaxSplits}));
 }

@@ -13,7 +13,10 @@
 // rounded once.
 //
 // Both directions are bound by HBM: a row is read once, held in registers between its
-// sum and its output, and written once.
+// sum and its output, and written once.  bf16, 16384 x 4096 with a residual: forward 77 us,
+// with the 8 bits 135 (810 MB), backward 96 (537 MB, 5.6 TB/s; a large copy reaches 4.9);
+// fp32 rows of 2051 at odd strides, 4099 of them, backward 31 us.  32 x 4096: 5 us, of
+// which the kernel is 3.6.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -217,7 +220,8 @@ __global__ __launch_bounds__(kLongL) void rms_fwd_long(const Fwd<typename Io<DT>
 
 // ----------------------------------------------------------------- backward
 // The row in registers; dgamma's sums of a lane's columns stay in its registers over
-// the workgroup's rows and go out once, as partial[workgroup][C].
+// the workgroup's rows and go out once, as partial[workgroup][C]: a CU's worth of threads
+// (512), so that the partial sums are a 16th of the rows' bytes at 16384 x 4096.
 template <int DT, int NV, int L, int NG>
 __global__ __launch_bounds__(L *NG) void rms_bwd(const Bwd<typename Io<DT>::T> a) {
     using IO = Io<DT>;
@@ -413,7 +417,10 @@ __global__ __launch_bounds__(1024) void rms_bwd_final(const float *__restrict__ 
 
 // ------------------------------------------------------------------ launches
 // f(chunks a lane, lanes of a row, rows of a workgroup) for rows of `chunks` chunks;
-// false: none holds them.
+// false: none holds them.  The fewest lanes that hold a row: twice as many cost nothing
+// up to 4 chunks a lane (16384 x 4096 bf16 forward, 512 chunks: 256 lanes of two 77 us, of
+// four 78, 512 lanes 88), rows longer than all are read twice (1024 x 65536: held 83 us,
+// read twice 113).
 template <class F>
 bool fwd_kind(int chunks, F f) {
     auto with = [&](auto nv, auto l, auto ng) {

@@ -376,10 +376,11 @@ int fg_rms_norm_bwd(fg_ctx *ctx, int dtype, const void *d_s, int lds, const void
  *   out_i = sum over visible j of softmax(S)_j v_j ;  lse = log sum exp(S)
  * Products and statistics are fp32, probabilities rounded to dtype for the second
  * product, out rounded once.  d_lse [heads][Tq] (fp32, what the backward needs) may be
- * NULL.  A row that sees no key is 0, its lse -inf.  Values of keys that a row does not
- * see do not reach it, infinities and NaN included.  Rows of no sequence are left as
- * they are.  1 <= D <= 128, scale > 0.  Where rows are few and keys many, the keys'
- * splits go to the workspace: D + 2 floats for each of at most 32 a row and head. */
+ * NULL.  A row that sees no key, or none but at scores of -inf, is 0, its lse -inf.
+ * Values of keys that a row does not see do not reach it, infinities and NaN included.
+ * Rows of no sequence are left as they are.  Tensors of no rows may be NULL.  1 <= D <=
+ * 128, scale > 0.  Where rows are few and keys many, the keys' splits go to the
+ * workspace: D + 2 floats for each of at most 32 a row and head. */
 int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k, int ldk,
                  const void *d_v, int ldv, const uint32_t *d_q_starts, const uint32_t *d_k_starts,
                  const uint32_t *d_k_lens, int n, int Tq, int Tk, int heads, int kv_heads, int D,
