@@ -14,7 +14,7 @@
 //
 // Both directions are bound by HBM: a row is read once, held in registers between its
 // sum and its output, and written once.  bf16, 16384 x 4096 with a residual: forward 77 us,
-// with the 8 bits 135 (810 MB), backward 96 (537 MB, 5.6 TB/s; a large copy reaches 4.9);
+// with the 8 bits 95 (606 MB), backward 96 (537 MB, 5.6 TB/s; a large copy reaches 4.9);
 // fp32 rows of 2051 at odd strides, 4099 of them, backward 31 us.  32 x 4096: 5 us, of
 // which the kernel is 3.6.
 #include <hip/hip_runtime.h>
