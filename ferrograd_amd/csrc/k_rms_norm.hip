@@ -221,7 +221,7 @@ __global__ __launch_bounds__(kLongL) void rms_fwd_long(const Fwd<typename Io<DT>
 // ----------------------------------------------------------------- backward
 // The row in registers; dgamma's sums of a lane's columns stay in its registers over
 // the workgroup's rows and go out once, as partial[workgroup][C]: a CU's worth of threads
-// (512), so that the partial sums are a 16th of the rows' bytes at 16384 x 4096.
+// (512), so that the partial sums are few (4 MB beside 537 at 16384 x 4096 of bf16).
 template <int DT, int NV, int L, int NG>
 __global__ __launch_bounds__(L *NG) void rms_bwd(const Bwd<typename Io<DT>::T> a) {
     using IO = Io<DT>;
@@ -417,10 +417,9 @@ __global__ __launch_bounds__(1024) void rms_bwd_final(const float *__restrict__ 
 
 // ------------------------------------------------------------------ launches
 // f(chunks a lane, lanes of a row, rows of a workgroup) for rows of `chunks` chunks;
-// false: none holds them.  The fewest lanes that hold a row: twice as many cost nothing
-// up to 4 chunks a lane (16384 x 4096 bf16 forward, 512 chunks: 256 lanes of two 77 us, of
-// four 78, 512 lanes 88), rows longer than all are read twice (1024 x 65536: held 83 us,
-// read twice 113).
+// false: none holds them.  The first that does: idle lanes cost more than idle chunks
+// (16384 x 4096 bf16 forward, 512 chunks: 256 lanes of two 77 us, of four 78, 512 lanes of
+// four 88); rows longer than all are read twice (1024 x 65536: held 83 us, read twice 113).
 template <class F>
 bool fwd_kind(int chunks, F f) {
     auto with = [&](auto nv, auto l, auto ng) {
@@ -435,18 +434,22 @@ bool fwd_kind(int chunks, F f) {
     return FG_RMS(1, 16, 16) || FG_RMS(1, 64, 4) || FG_RMS(2, 64, 4) || FG_RMS(2, 256, 1) ||
            FG_RMS(4, 256, 1) || FG_RMS(4, 512, 1) || FG_RMS(4, 1024, 1) || FG_RMS(8, 1024, 1);
 }
-// longer: rows of up to 2048 chunks too.  fp32's (4096 x 8192: 103 us, the longer rows'
-// kernels 142); of 16 bits they take two registers a column more (4096 x 16384: 192 and 151).
-template <class F>
-bool bwd_kind(int chunks, bool longer, F f) {
+// LONGER: rows of up to 2048 chunks too, for fp32 (4096 x 8192: 103 us, the longer rows'
+// kernels 142); 16-bit rows of as many chunks have twice the columns' sums (4096 x 16384:
+// 192 us and 151).
+template <bool LONGER, class F>
+bool bwd_kind(int chunks, F f) {
     auto with = [&](auto nv, auto l, auto ng) {
         if (chunks > nv() * l()) return false;
         f(nv, l, ng);
         return true;
     };
     using std::integral_constant;
-    return FG_RMS(1, 16, 32) || FG_RMS(1, 64, 8) || FG_RMS(1, 128, 4) || FG_RMS(1, 256, 2) ||
-           FG_RMS(1, 512, 1) || FG_RMS(2, 512, 1) || (longer && FG_RMS(2, 1024, 1));
+    if (FG_RMS(1, 16, 32) || FG_RMS(1, 64, 8) || FG_RMS(1, 128, 4) || FG_RMS(1, 256, 2) ||
+        FG_RMS(1, 512, 1) || FG_RMS(2, 512, 1))
+        return true;
+    if constexpr (LONGER) return FG_RMS(2, 1024, 1);
+    return false;
 }
 #undef FG_RMS
 
@@ -461,10 +464,11 @@ struct Split {
 Split split_of(int cus, int dtype, int R, int C) {
     Split s;
     const int chunks = chunks_of(dtype, C);
-    s.held = bwd_kind(chunks, dtype == FG_DTYPE_F32, [&](auto, auto l, auto ng) {
+    auto share = [&](auto, auto l, auto ng) {
         const int per_cu = std::max(1, 512 / (l() * ng()));
         s.splits = std::min(R > 0 ? (R - 1) / ng() + 1 : 0, cus * per_cu);
-    });
+    };
+    s.held = dtype == FG_DTYPE_F32 ? bwd_kind<true>(chunks, share) : bwd_kind<false>(chunks, share);
     if (s.held) return s;
     s.strips = (chunks - 1) / kColsNT + 1;
     const int want = std::max(1, std::min((4 * cus - 1) / s.strips + 1, (R + 15) / 16));
@@ -495,7 +499,7 @@ int launch_bwd(fg_ctx *ctx, const Split &s, Bwd<void> v) {
                    s.rows};
     hipStream_t st = ctx->stream;
     if (s.held) {
-        bwd_kind((a.C - 1) / Io<DT>::E + 1, DT == fg::kF32, [&](auto nv, auto l, auto ng) {
+        bwd_kind<DT == fg::kF32>((a.C - 1) / Io<DT>::E + 1, [&](auto nv, auto l, auto ng) {
             const size_t lds = ng() > 1 && a.partial ? (size_t)a.C * sizeof(float) : 0;
             rms_bwd<DT, nv(), l(), ng()><<<s.splits, l() * ng(), lds, st>>>(a);
         });
