@@ -1031,9 +1031,10 @@ __global__ __launch_bounds__(256) void att_combine(const Args a) {
 
 // ------------------------------------------------------------------ backward
 // dS of fp16 tensors carries a power of two that brings it near 1, whatever dout's size:
-// probabilities of long rows times small gradients would be subnormal.  From a number
-// above the largest |dout| of its rows (their V of order 1: what is summed stays within
-// the type up to |V| of some hundreds).
+// probabilities of long rows times small gradients would be subnormal.  It is taken from
+// the largest |dout| (as if V were of order 1) and lowered, the sums with it, where what is
+// carried would pass 2^15: |dS| reaches |dout| |V| D, past the type's range from |V| = 64
+// on.
 __device__ __forceinline__ int exponent_above(float x) {
     return max((int)((__float_as_uint(x) & 0x7fffffffu) >> 23) - 126, -100);
 }
@@ -1044,7 +1045,29 @@ __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.
 template <int DT>
 constexpr bool kFold = DT != kF32;
 constexpr float kUpDs = 4.0f;  // its power above 1 / the largest |dout|
+constexpr int kTopDs = 15;     // and the power of two that nothing carried passes
 constexpr float kUpP = 8.0f;   // fp16: the probabilities' that dV is summed from
+
+// Lowers the power of dS where a lane's number (a row, or a key; both halves) would pass
+// 2^kTopDs: of the block ds and of the sums acc, by `down`, which is returned (0: as they
+// were).  What is not finite stays what it is.
+template <int NB>
+__device__ __forceinline__ int lower(f32x16 &ds, f32x16 (&acc)[NB]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
+    if (!__any(top > pow2(kTopDs))) return 0;
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const int down = top < INFINITY ? max(0, exponent_above(top) - kTopDs) : 0;
+    const float f = pow2(-down);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ds[r] *= f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[b][r] *= f;
+    return down;
+}
 
 // A gradient's row: where it goes, or, in splits, to split blockIdx.y's fp32 rows of
 // `part`, `rows` of them, at place `at`.
@@ -1228,8 +1251,9 @@ att_bwd_q(const Args a) {
         }
     }
     const int last = row < rows ? last_of(row) : -1;
-    const int up = DT == kF16 ? (int)kUpDs - exponent_above(big) : 0;
-    const float from = (lse2 - (float)up) * (kFold<DT> ? 1.0f / c : 1.0f);
+    int up = DT == kF16 ? (int)kUpDs - exponent_above(big) : 0;
+    auto power = [&] { return (lse2 - (float)up) * (kFold<DT> ? 1.0f / c : 1.0f); };
+    float from = power();
 
     Mover<DT, DP, KT, 256, DMA> mk, mv;
     auto load = [&](int t) {
@@ -1285,6 +1309,12 @@ att_bwd_q(const Args a) {
                     for (int r = 0; r < 16; ++r) {
                         const int key = key0 + 32 * b + 8 * (r >> 2) + 4 * h + (r & 3);
                         s[r] = key <= last ? s[r] : 0.0f;
+                    }
+                }
+                if constexpr (DT == kF16) {
+                    if (const int down = lower(s, dq)) {
+                        up -= down;
+                        from = power();
                     }
                 }
 #pragma unroll
@@ -1406,7 +1436,7 @@ att_bwd_kv(const Args a) {
     f32x16 dk[NB], dv[NB];
     clear(dk);
     clear(dv);
-    int up = 0;  // fp16: the power of two that dK carries
+    int up = 0;  // fp16: the power of two that the lane's key's dK carries
     bool any = false;
     const int t0 = begin + share.t0, t1 = begin + share.t1;
     if (t0 < t1) {
@@ -1433,17 +1463,16 @@ att_bwd_kv(const Args a) {
 #pragma unroll
                 for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o));
                 const int e = __builtin_amdgcn_readfirstlane((int)kUpDs - exponent_above(big));
-                if (!any || e < up) {
-                    if (any) {
-                        const float f = pow2(e - up);
+                if (!any) up = e;
+                if (__any(e < up)) {
+                    const float f = pow2(min(e - up, 0));
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
+                    for (int b = 0; b < NB; ++b)
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) dk[b][r] *= f;
-                    }
-                    up = e;
-                    any = true;
+                        for (int r = 0; r < 16; ++r) dk[b][r] *= f;
+                    up = min(e, up);
                 }
+                any = true;
                 fs = pow2(up - (int)kUpP);
             }
             f32x16 p = kFold<DT> ? rows16(st + 4 * h) : all16(0.0f);
@@ -1496,6 +1525,7 @@ att_bwd_kv(const Args a) {
                 for (int d = 0; d < NB; ++d)
                     dv[d] = Ty::mfma(Tl::by_column(dt, 16 * u, d, L), f, dv[d]);
             }
+            if constexpr (DT == kF16) up -= lower(dp, dk);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const typename Ty::Frag f = Ty::pack(dp, u);
