@@ -1107,12 +1107,14 @@ __device__ void careful_bwd_q(const Args &a, const Seq &sq, int kv, int row0, in
         const T *dout = static_cast<const T *>(a.dout) + token * a.lddo + col;
         // (Not from a.rows, which another split's workgroup may be writing.)
         const float lse = a.lse[(int64_t)head * a.Tq + token];
-        const float lse2 = lse * kLog2e;
+        // (As in att_bwd_q: a row of no key, or of none but scores of -inf.)
+        const bool none = lse == -INFINITY;
+        const float lse2 = none ? INFINITY : lse * kLog2e;
         const T *out = static_cast<const T *>(a.out) + token * a.ldo + col;
         float delta = 0.0f;
         for (int d = lane; d < a.D; d += 64)
             delta += Type<DT>::load1(dout + d) * Type<DT>::load1(out + d);
-        delta = wave_add(delta);
+        delta = none ? 0.0f : wave_add(delta);
         float acc[2] = {0.0f, 0.0f};
         for (int j0 = key0; j0 < end; j0 += 64) {
             const int j = j0 + lane;

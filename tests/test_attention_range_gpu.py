@@ -142,3 +142,30 @@ def test_one_query_between_two_values(gpu_ctx, D, pad, value):
     dout = torch.full((1, D), 1.9, dtype=torch.float16, device="cuda")
     out, lse = b.forward(gpu_ctx)
     check(b, b.backward(gpu_ctx, out, lse, dout), out, lse, dout)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,pad", [(64, 0), (128, 0), (128, 1), (40, 0)])
+@pytest.mark.parametrize("lq,lk,bad", [(2, 2, math.inf), (70, 90, math.nan), (70, 90, math.inf),
+                                       (6, 3000, math.nan)])
+def test_rows_of_minus_infinity_beside_keys_out_of_sight(gpu_ctx, dt, D, pad, lq, lk, bad):
+    """Rows that see keys at scores of -inf alone have a dq of 0, whatever a key holds that
+    they do not see."""
+    note("-inf beside", dt, D, pad, lq, lk, bad)
+    b = Batch([(lq, lk)], 2, 1, D, dt, True, pad)
+    rows = list(range(0, lq - 1, 3))  # (the last row sees the last key)
+    b.k[:, 0] = b.k[:, 0].abs() + 0.5
+    for head in range(2):
+        b.q[rows, head * D] = -math.inf
+    dout = rand((b.Tq, 2 * D), dt, 9, 1.0, 0.0, pad)
+    out, lse = b.forward(gpu_ctx)
+    assert (out[rows] == 0).all() and (lse[:, rows] == -math.inf).all()
+    want = b.backward(gpu_ctx, out, lse, dout)[0]
+    assert (want[rows] == 0).all()
+    for t in (b.k, b.v):
+        t[lk - 1] = bad
+    again, again_lse = b.forward(gpu_ctx)
+    assert (again[rows] == 0).all() and (again_lse[:, rows] == -math.inf).all()
+    got = b.backward(gpu_ctx, out, lse, dout)[0]
+    assert (got[rows] == 0).all()
+    assert torch.isfinite(got[:lq - 1].float()).all()
