@@ -378,18 +378,12 @@ __global__ __launch_bounds__(kBwdNT) void logprobs_bwd(const Bwd a) {
     }
     const float lse = a.lse[row], h = gb != 0.0f ? a.entropy[row] : 0.0f;
     const uint32_t token = a.tokens[row];
-    const float c = a.scale * kLog2e, from = lse * kLog2e;
-    const float k1 = -gb * a.scale, k0 = -(ga + gb * (h - lse));
     auto grad = [&](float v, bool hot) {
-        v = fmaxf(v, -1e30f);  // (a masked logit: -inf times its probability, 0)
-        float o;
-        if constexpr (DT == fg::kF32) {
-            // z - lse rounded once; `from` would be off by 2^-24 of lse itself.
-            const float d = __builtin_fmaf(v, a.scale, -lse);
-            o = -__builtin_amdgcn_exp2f(d * kLog2e) * __builtin_fmaf(gb, d + h, ga);
-        } else {
-            o = __builtin_amdgcn_exp2f(__builtin_fmaf(v, c, -from)) * __builtin_fmaf(v, k1, k0);
-        }
+        // (z - lse rounded once; a masked logit's, which may be -inf, as its probability is 0
+        // long before: the formula's products stay finite.  NaN stays NaN.)
+        float d = __builtin_fmaf(v, a.scale, -lse);
+        d = d < -1000.0f ? -1000.0f : d;
+        const float o = -__builtin_amdgcn_exp2f(d * kLog2e) * __builtin_fmaf(gb, d + h, ga);
         return hot ? o + ga : o;
     };
     u32x4 w[kBwdDeep];
