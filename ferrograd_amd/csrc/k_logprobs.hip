@@ -65,6 +65,24 @@ struct Stats {
     __device__ __forceinline__ float from() const { return m == -INFINITY ? 0.0f : m; }
 };
 
+// What a row's log probabilities are taken from: its maximum m times c, or where that
+// product is past fp32 (a row of nothing but the type's lowest number) the maximum
+// logit itself, `raw`.
+struct Base {
+    float m;
+    bool raw;
+    // scale (x - max x)
+    __device__ __forceinline__ float from_max(float x, float scale, float c) const {
+        if (raw) return (x - m) * scale;
+        const float d = __builtin_fmaf(x, c, -m) * kLn2;
+        // (A finite logit so low that its product with c alone is past fp32.)
+        return d == -INFINITY ? __builtin_fmaf(x, scale, -m * kLn2) : d;
+    }
+    __device__ __forceinline__ float lse(float scale, float log_s) const {
+        return __builtin_fmaf(m, raw ? scale : kLn2, log_s);
+    }
+};
+
 // Largest over a wave's 64 lanes (all active), the same in every lane, NaN left out.
 __device__ __forceinline__ float wave_max(float v) {
     using namespace fg::smrow;
@@ -98,30 +116,29 @@ struct Fwd {
     float *tops;
     float scale;
     int ldx, C, K;
-    // Rows in splits of their columns: [R][splits] of three statistics, and of K places
-    // (place_of) in order.
+    // Rows in splits of their columns: [R][splits] of four statistics (Stats, and a raw
+    // Base's maximum or -inf), and of K places (place_of) in order.
     int splits;
     float *stats;
     uint64_t *best;
 };
 
 // A row's answers from its statistics, in thread 0.
-__device__ __forceinline__ void write_answers(const Fwd &a, size_t r, const Stats &st, float log_s,
-                                              float xt, bool inside, float c) {
+__device__ __forceinline__ void write_answers(const Fwd &a, size_t r, const Stats &st, Base base,
+                                              float log_s, float xt, bool inside, float c) {
     if (a.logp)
-        a.logp[r] = inside ? __builtin_fmaf(xt, c, -st.m) * kLn2 - log_s : __builtin_nanf("");
+        a.logp[r] = inside ? base.from_max(xt, a.scale, c) - log_s : __builtin_nanf("");
     if (a.entropy) a.entropy[r] = log_s - kLn2 * (st.w / st.s);
-    if (a.lse) a.lse[r] = __builtin_fmaf(st.m, kLn2, log_s);
+    if (a.lse) a.lse[r] = base.lse(a.scale, log_s);
 }
 // The alternative at `place`: its column and log probability.
 template <int DT>
 __device__ __forceinline__ void write_top(const Fwd &a, size_t r, int place, int col,
-                                          const typename Io<DT>::T *x, const Stats &st,
-                                          float log_s, float c) {
+                                          const typename Io<DT>::T *x, Base base, float log_s,
+                                          float c) {
     if (a.ids) a.ids[r * a.K + place] = (uint32_t)col;
     if (a.tops)
-        a.tops[r * a.K + place] =
-            __builtin_fmaf(Io<DT>::load1(x, col), c, -st.m) * kLn2 - log_s;
+        a.tops[r * a.K + place] = base.from_max(Io<DT>::load1(x, col), a.scale, c) - log_s;
 }
 
 // A row (or a split of its columns) a workgroup of NT threads, read once; for the
@@ -221,15 +238,50 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lo
         st.s += sm[k][1];
         st.w += sm[k][2];
     }
+    Base base{m, false};
+    if (fabsf(m) == INFINITY) {
+        // The sums again from the largest logit, if that is finite.
+        const float of_wave = wave_max(big);
+        __syncthreads();
+        if ((t & 63) == 0) sm[t >> 6][0] = of_wave;
+        __syncthreads();
+        float most = sm[0][0];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) most = fmaxf(most, sm[k][0]);
+        if (fabsf(most) < INFINITY) {
+            base = {most, true};
+            Stats again;
+            for (int i = j0 + t; i < nb; i += NT) {
+                const u32x4 v = fg::rows::load<DT>(x, i);
+#pragma unroll
+                for (int e = 0; e < E; ++e) again.add(IO::get(v, e) - most, c, 0.0f);
+            }
+            if (single >= 0) again.add(IO::load1(x, single) - most, c, 0.0f);
+            const float s2 = fg::rows::wave_sum(again.s), w2 = fg::rows::wave_sum(again.w);
+            if ((t & 63) == 0) {
+                sm[t >> 6][1] = s2;
+                sm[t >> 6][2] = w2;
+            }
+            __syncthreads();
+            st.s = sm[0][1];
+            st.w = sm[0][2];
+#pragma unroll
+            for (int k = 1; k < NW; ++k) {
+                st.s += sm[k][1];
+                st.w += sm[k][2];
+            }
+        }
+    }
     const float log_s = logf(st.s);
     const size_t part = r * a.splits + split;
     if (t == 0) {
         if (a.splits > 1) {
-            a.stats[3 * part] = st.m;
-            a.stats[3 * part + 1] = st.s;
-            a.stats[3 * part + 2] = st.w;
+            a.stats[4 * part] = st.m;
+            a.stats[4 * part + 1] = st.s;
+            a.stats[4 * part + 2] = st.w;
+            a.stats[4 * part + 3] = base.raw ? base.m : -INFINITY;
         } else {
-            write_answers(a, r, st, log_s, xt, inside, c);
+            write_answers(a, r, st, base, log_s, xt, inside, c);
         }
     }
     if (!a.K) return;
@@ -253,7 +305,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lo
     __syncthreads();
     auto write = [&](int at, uint64_t place) {
         if (a.splits > 1) a.best[part * a.K + at] = place;
-        else write_top<DT>(a, r, at, col_of(place), x, st, log_s, c);
+        else write_top<DT>(a, r, at, col_of(place), x, base, log_s, c);
     };
     const int n = count_s;
     if (n >= a.K && n <= kCands) {
@@ -303,11 +355,12 @@ __global__ __launch_bounds__(kJoinNT) void logprobs_join(const Fwd a) {
     const float c = a.scale * kLog2e;
     const uint64_t *best = a.best + r * all;
     const bool on = lane < a.splits;
-    const float *p = a.stats + 3 * (r * a.splits + (on ? lane : 0));
+    const float *p = a.stats + 4 * (r * a.splits + (on ? lane : 0));
     Stats st;
     st.m = on ? p[0] : -INFINITY;
     st.s = on ? p[1] : 0.0f;
     st.w = on ? p[2] : 0.0f;
+    const float raw = on ? p[3] : -INFINITY;
     uint64_t mine[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
@@ -317,12 +370,25 @@ __global__ __launch_bounds__(kJoinNT) void logprobs_join(const Fwd a) {
     const bool inside = token < (uint32_t)a.C;
     const float xt = inside ? Io<DT>::load1(x, (int)token) : 0.0f;
     if (t == 0) count_s = 0;
-    st.raise(wave_max(st.m));
+    // Where the row's maximum is raw, so are the splits that count: the others are far below
+    // it.  Where it is not, raw splits are far below.
+    Base base{wave_max(st.m), false};
+    if (fabsf(base.m) == INFINITY) {
+        const float most = wave_max(raw);
+        if (most > -INFINITY) {
+            base = {most, true};
+            const float d = (raw - most) * c, f = __builtin_amdgcn_exp2f(d);
+            st.w = raw > -INFINITY && f > 0.0f ? f * (st.w + st.s * d) : 0.0f;
+            st.s = st.s == st.s ? (raw > -INFINITY ? st.s * f : 0.0f) : st.s;
+        }
+    } else {
+        if (raw > -INFINITY) st.s = st.s == st.s ? 0.0f : st.s, st.w = 0.0f;
+        st.raise(base.m);
+    }
     st.s = fg::rows::wave_sum(st.s);
     st.w = fg::rows::wave_sum(st.w);
-    st.m = wave_max(st.m);
     const float log_s = logf(st.s);
-    if (t == 0) write_answers(a, r, st, log_s, xt, inside, c);
+    if (t == 0) write_answers(a, r, st, base, log_s, xt, inside, c);
     if (!a.K) return;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) bound = max(bound, (uint64_t)__shfl_xor((long long)bound, o));
@@ -335,7 +401,7 @@ __global__ __launch_bounds__(kJoinNT) void logprobs_join(const Fwd a) {
     const int n = count_s;
     for (int i = t; i < n; i += kJoinNT) {
         const int before = before_in(cand, n, cand[i]);
-        if (before < a.K) write_top<DT>(a, r, before, col_of(cand[i]), x, st, log_s, c);
+        if (before < a.K) write_top<DT>(a, r, before, col_of(cand[i]), x, base, log_s, c);
     }
 }
 
@@ -467,7 +533,7 @@ FG_API int fg_token_logprobs(fg_ctx *ctx, int dtype, const void *d_logits, int l
           ldx, C, top, splits_of(ctx->cu_count, R, C), nullptr, nullptr};
     if (a.splits > 1) {
         const uint64_t parts = (uint64_t)R * a.splits;
-        a.best = (uint64_t *)fg::workspace(ctx, parts * (top * sizeof(uint64_t) + 3 * sizeof(float)));
+        a.best = (uint64_t *)fg::workspace(ctx, parts * (top * sizeof(uint64_t) + 4 * sizeof(float)));
         if (!a.best) return FG_ERR_OUT_OF_MEMORY;
         a.stats = (float *)(a.best + parts * top);
     }

@@ -409,7 +409,7 @@ int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const voi
  * Outputs are fp32 (top_ids u32, both [R][top]); any may be NULL.  top is at most 32
  * and C.  A token outside [0, C) gives a NaN logp; logits of -inf (masked) have
  * probability 0.  scale > 0 (an inverse temperature).  Few rows of many columns are split:
- * 12 bytes and 8 an alternative for each of at most 16 splits a row go to the workspace. */
+ * 16 bytes and 8 an alternative for each of at most 16 splits a row go to the workspace. */
 int fg_token_logprobs(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
                       const uint32_t *d_tokens, int R, int C, float scale, float *d_logp,
                       float *d_entropy, float *d_lse, int top, uint32_t *d_top_ids,

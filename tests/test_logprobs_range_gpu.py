@@ -68,3 +68,77 @@ def test_gradient_of_nan_logits_is_nan(gpu_ctx, dt):
                                    ld(out), entropy=h.float().cuda(), dlogp=one, dentropy=gb,
                                    dtype=DTS[dt][0])
         assert torch.isnan(out[1]).all() and torch.isfinite(out[[0, 2]].float()).all()
+
+
+# A wave a row, four waves, rows in splits.
+WIDTHS = [1, 5, 100, 3001, 40003, 131072]
+
+
+def of_one_value(ctx, x, dt, scale, value, live, note_):
+    """Rows whose `live` columns hold `value`, the largest there is: a uniform answer."""
+    note(*note_)
+    R, C = x.shape
+    n = live.sum().item()
+    cols = live.nonzero().flatten()
+    tok = torch.stack([cols[0], cols[-1], cols[n // 2]]).cpu()
+    top = min(C, 32)
+    (logp, h, lse), ids, tops = run_lp(ctx, x, tok, dt, top, scale)
+    # The sum is a whole number below 2^24; a logarithm and a subtraction.
+    tol = torch.full((R,), 8 * U * (1.0 + math.log(n)))
+    want = torch.full((R,), math.log(n)).double()
+    within(logp.cpu(), -want, tol)
+    within(h.cpu(), want, tol)
+    z = value * scale
+    within(lse.cpu(), z + want, tol + 4 * U * abs(z))
+    assert torch.equal(ids.long(), tops_oracle(x, top))
+    some = min(n, top)
+    within(tops[:, :some], -want[:, None].expand(-1, some), tol[:, None])
+    return tops
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("C", WIDTHS)
+@pytest.mark.parametrize("scale", [1.0, 0.7])
+def test_rows_of_the_types_lowest_number(gpu_ctx, dt, C, scale):
+    """A mask of the type's lowest number that leaves nothing is a row of equal logits; among
+    logits of -inf too, and at the type's largest."""
+    scale = float(np.float32(scale))
+    info = torch.finfo(DTS[dt][1])
+    every = torch.ones(C, dtype=torch.bool, device="cuda")
+    for value in (info.min, info.max):
+        x = torch.full((3, C), value, dtype=DTS[dt][1], device="cuda")
+        of_one_value(gpu_ctx, x, dt, scale, value, every, ("lowest", dt, C, value))
+    if C < 5:
+        return
+    some = every.clone()
+    some[1::2] = False
+    x = torch.full((3, C), info.min, dtype=DTS[dt][1], device="cuda")
+    x[:, 1::2] = -math.inf
+    tops = of_one_value(gpu_ctx, x, dt, scale, info.min, some, ("lowest and -inf", dt, C))
+    assert (tops[:, int(some.sum()):] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("C", [100, 3001, 40003, 131072])
+def test_masked_tokens_of_the_lowest_number(gpu_ctx, dt, C):
+    """Beside ordinary logits the lowest number is itself as a log probability, to rounding; a
+    few large logits at one end of a row leave the rest without probability."""
+    note("masked tokens", dt, C)
+    low = torch.finfo(DTS[dt][1]).min
+    x = torch.full((3, C), low, dtype=DTS[dt][1], device="cuda")
+    x[0, 7:12] = 1.0
+    x[1, C - 5:] = 2.0
+    x[2, :] = low
+    x[2, C // 2] = 3e38
+    tok = torch.tensor([C - 1, 0, C // 2])
+    (logp, h, lse), ids, tops = run_lp(gpu_ctx, x, tok, dt, 20, 1.0)
+    five = math.log(5)
+    within(logp.cpu(), torch.tensor([low, low, 0.0]).double(),
+           torch.tensor([-low * U * 4, -low * U * 4, 1e-30]))
+    within(h.cpu(), torch.tensor([five, five, 0.0]).double(), torch.tensor([1.0] * 3) * 32 * U)
+    top = x[2, C // 2].item()
+    within(lse.cpu(), torch.tensor([1.0 + five, 2.0 + five, top]).double(),
+           torch.tensor([16 * U, 16 * U, 4 * U * top]))
+    assert torch.equal(ids.long(), tops_oracle(x, 20))
+    within(tops[:2, :5], torch.full((2, 5), -five).double(), torch.full((2, 5), 16 * U))
+    within(tops[:2, 5:], torch.full((2, 15), low).double(), torch.full((2, 15), -low * U * 4))
