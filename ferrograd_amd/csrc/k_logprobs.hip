@@ -66,8 +66,12 @@ struct Stats {
 };
 
 // What a row's log probabilities are taken from: its maximum m times c, or where that
-// product is past fp32 (a row of nothing but the type's lowest number) the maximum
-// logit itself, `raw`.
+// product's rounding is not far below 1 or the product past fp32 (a row of nothing but
+// masks of -1e10, or of the type's lowest number) the maximum logit itself, `raw`.
+constexpr float kFar = 0x1p20f;
+__device__ __forceinline__ bool is_raw(float m, float most) {
+    return fabsf(m) >= kFar && fabsf(most) < INFINITY;
+}
 struct Base {
     float m;
     bool raw;
@@ -116,8 +120,8 @@ struct Fwd {
     float *tops;
     float scale;
     int ldx, C, K;
-    // Rows in splits of their columns: [R][splits] of four statistics (Stats, and a raw
-    // Base's maximum or -inf), and of K places (place_of) in order.
+    // Rows in splits of their columns: [R][splits] of four statistics (Stats and the largest
+    // logit), and of K places (place_of) in order.
     int splits;
     float *stats;
     uint64_t *best;
@@ -201,16 +205,17 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lo
     }
     // (0: no number among the thread's values, or nothing above -inf.)
     const uint32_t mine = big > -INFINITY ? order_key(big) : 0u;
-    const float top = wave_max(big * c);
+    const float top = wave_max(big);
     if ((t & 63) == 0) sm[t >> 6][0] = top;
     if (a.K) {
         keys[t] = mine;
         if (t == 0) count_s = hot_s = 0;
     }
     __syncthreads();
-    float m = sm[0][0];
+    float most = sm[0][0];
 #pragma unroll
-    for (int k = 1; k < NW; ++k) m = fmaxf(m, sm[k][0]);
+    for (int k = 1; k < NW; ++k) most = fmaxf(most, sm[k][0]);
+    const float m = most * c;
     st.raise(m);
     const float s = fg::rows::wave_sum(st.s), w = fg::rows::wave_sum(st.w);
     if ((t & 63) == 0) {
@@ -239,37 +244,29 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lo
         st.w += sm[k][2];
     }
     Base base{m, false};
-    if (fabsf(m) == INFINITY) {
-        // The sums again from the largest logit, if that is finite.
-        const float of_wave = wave_max(big);
+    if (is_raw(m, most)) {
+        // The sums again from the largest logit.
+        base = {most, true};
+        Stats again;
+        for (int i = j0 + t; i < nb; i += NT) {
+            const u32x4 v = fg::rows::load<DT>(x, i);
+#pragma unroll
+            for (int e = 0; e < E; ++e) again.add(IO::get(v, e) - most, c, 0.0f);
+        }
+        if (single >= 0) again.add(IO::load1(x, single) - most, c, 0.0f);
+        const float s2 = fg::rows::wave_sum(again.s), w2 = fg::rows::wave_sum(again.w);
         __syncthreads();
-        if ((t & 63) == 0) sm[t >> 6][0] = of_wave;
+        if ((t & 63) == 0) {
+            sm[t >> 6][1] = s2;
+            sm[t >> 6][2] = w2;
+        }
         __syncthreads();
-        float most = sm[0][0];
+        st.s = sm[0][1];
+        st.w = sm[0][2];
 #pragma unroll
-        for (int k = 1; k < NW; ++k) most = fmaxf(most, sm[k][0]);
-        if (fabsf(most) < INFINITY) {
-            base = {most, true};
-            Stats again;
-            for (int i = j0 + t; i < nb; i += NT) {
-                const u32x4 v = fg::rows::load<DT>(x, i);
-#pragma unroll
-                for (int e = 0; e < E; ++e) again.add(IO::get(v, e) - most, c, 0.0f);
-            }
-            if (single >= 0) again.add(IO::load1(x, single) - most, c, 0.0f);
-            const float s2 = fg::rows::wave_sum(again.s), w2 = fg::rows::wave_sum(again.w);
-            if ((t & 63) == 0) {
-                sm[t >> 6][1] = s2;
-                sm[t >> 6][2] = w2;
-            }
-            __syncthreads();
-            st.s = sm[0][1];
-            st.w = sm[0][2];
-#pragma unroll
-            for (int k = 1; k < NW; ++k) {
-                st.s += sm[k][1];
-                st.w += sm[k][2];
-            }
+        for (int k = 1; k < NW; ++k) {
+            st.s += sm[k][1];
+            st.w += sm[k][2];
         }
     }
     const float log_s = logf(st.s);
@@ -279,7 +276,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void lo
             a.stats[4 * part] = st.m;
             a.stats[4 * part + 1] = st.s;
             a.stats[4 * part + 2] = st.w;
-            a.stats[4 * part + 3] = base.raw ? base.m : -INFINITY;
+            a.stats[4 * part + 3] = most;
         } else {
             write_answers(a, r, st, base, log_s, xt, inside, c);
         }
@@ -360,7 +357,7 @@ __global__ __launch_bounds__(kJoinNT) void logprobs_join(const Fwd a) {
     st.m = on ? p[0] : -INFINITY;
     st.s = on ? p[1] : 0.0f;
     st.w = on ? p[2] : 0.0f;
-    const float raw = on ? p[3] : -INFINITY;
+    const float largest = on ? p[3] : -INFINITY;
     uint64_t mine[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
@@ -370,19 +367,16 @@ __global__ __launch_bounds__(kJoinNT) void logprobs_join(const Fwd a) {
     const bool inside = token < (uint32_t)a.C;
     const float xt = inside ? Io<DT>::load1(x, (int)token) : 0.0f;
     if (t == 0) count_s = 0;
-    // Where the row's maximum is raw, so are the splits that count: the others are far below
-    // it.  Where it is not, raw splits are far below.
     Base base{wave_max(st.m), false};
-    if (fabsf(base.m) == INFINITY) {
-        const float most = wave_max(raw);
-        if (most > -INFINITY) {
-            base = {most, true};
-            const float d = (raw - most) * c, f = __builtin_amdgcn_exp2f(d);
-            st.w = raw > -INFINITY && f > 0.0f ? f * (st.w + st.s * d) : 0.0f;
-            st.s = st.s == st.s ? (raw > -INFINITY ? st.s * f : 0.0f) : st.s;
-        }
+    const bool raw = is_raw(st.m, largest);
+    if (__any(raw)) {
+        // All from the largest logits: the others' sums by the rounding of theirs times c.
+        base = {wave_max(largest), true};
+        const float r = raw || largest == -INFINITY ? 0.0f : __builtin_fmaf(largest, c, -st.m);
+        const float d = (largest - base.m) * c - r, f = __builtin_amdgcn_exp2f(d);
+        st.w = f > 0.0f ? f * (st.w + st.s * d) : 0.0f;
+        st.s *= f;
     } else {
-        if (raw > -INFINITY) st.s = st.s == st.s ? 0.0f : st.s, st.w = 0.0f;
         st.raise(base.m);
     }
     st.s = fg::rows::wave_sum(st.s);
@@ -444,12 +438,13 @@ __global__ __launch_bounds__(kBwdNT) void logprobs_bwd(const Bwd a) {
     }
     const float lse = a.lse[row], h = gb != 0.0f ? a.entropy[row] : 0.0f;
     const uint32_t token = a.tokens[row];
+    // (A row with NaN, or of -inf alone, has no gradients.)
+    const float gn = fabsf(lse) < INFINITY ? ga : __builtin_nanf("");
     auto grad = [&](float v, bool hot) {
-        // (z - lse rounded once; a masked logit's, which may be -inf, as its probability is 0
-        // long before: the formula's products stay finite.  NaN stays NaN.)
-        float d = __builtin_fmaf(v, a.scale, -lse);
-        d = d < -1000.0f ? -1000.0f : d;
-        const float o = -__builtin_amdgcn_exp2f(d * kLog2e) * __builtin_fmaf(gb, d + h, ga);
+        // z - lse rounded once, kept where its exponential is one of a probability: a masked
+        // logit's may be -inf, and lse's own rounding may lie between it and the largest z.
+        const float d = __builtin_amdgcn_fmed3f(__builtin_fmaf(v, a.scale, -lse), -1000.0f, 0.0f);
+        const float o = -__builtin_amdgcn_exp2f(d * kLog2e) * __builtin_fmaf(gb, d + h, gn);
         return hot ? o + ga : o;
     };
     u32x4 w[kBwdDeep];

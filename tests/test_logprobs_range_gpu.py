@@ -142,3 +142,55 @@ def test_masked_tokens_of_the_lowest_number(gpu_ctx, dt, C):
     assert torch.equal(ids.long(), tops_oracle(x, 20))
     within(tops[:2, :5], torch.full((2, 5), -five).double(), torch.full((2, 5), 16 * U))
     within(tops[:2, 5:], torch.full((2, 15), low).double(), torch.full((2, 15), -low * U * 4))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [-1e10, -1e20, 3e20, "lowest"])
+@pytest.mark.parametrize("scale", [1.0, 0.7, 0.37])
+def test_gradient_of_rows_far_from_zero(gpu_ctx, dt, value, scale):
+    """An lse so large that fp32 rounds it by more than the logits' spread: probabilities
+    stay between 0 and 1."""
+    note("far", dt, value, scale)
+    ty, scale = DTS[dt][1], float(np.float32(scale))
+    for C in (5, 1000):
+        x = torch.full((2, C), torch.finfo(ty).min if value == "lowest" else value, dtype=ty,
+                       device="cuda")
+        tok = torch.tensor([1, C - 1])
+        (_, h, lse), _, _ = run_lp(gpu_ctx, x, tok, dt, 0, scale)
+        assert torch.isfinite(lse).all() and torch.isfinite(h).all()
+        out, (a, b) = torch.zeros_like(x), (torch.tensor(t, device="cuda") for t in ([2.0, -1.0],
+                                                                                     [0.5, 1.0]))
+        gpu_ctx.token_logprobs_bwd(x, C, tok.int().cuda(), 2, C, lse, out, C, entropy=h, dlogp=a,
+                                   dentropy=b, scale=scale, dtype=DTS[dt][0])
+        # p (d + h), d <= 0, is at most h, and at least -1 / e.
+        most = scale * (a.abs() + b.abs() * (h + 0.4)) * (1.0 + 2.0 ** -7)
+        assert (out.float().abs() <= most[:, None]).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("C", WIDTHS)
+@pytest.mark.parametrize("value", [-1e4, -1e7, -1e10, 1e9])
+def test_rows_of_one_large_number(gpu_ctx, dt, C, value):
+    """A mask that leaves nothing, and a product with the scale that fp32 rounds by more than
+    1: a row of equal logits all the same."""
+    value = torch.tensor(value).to(DTS[dt][1]).item()
+    x = torch.full((3, C), value, dtype=DTS[dt][1], device="cuda")
+    every = torch.ones(C, dtype=torch.bool, device="cuda")
+    of_one_value(gpu_ctx, x, dt, float(np.float32(0.7)), value, every, ("one", dt, C, value))
+
+
+@pytest.mark.parametrize("C", [3000, 40003, 131072])
+@pytest.mark.parametrize("at", [726817.0, -726817.0])
+def test_rows_on_both_sides_of_the_large_numbers(gpu_ctx, C, at):
+    """Parts of a row whose maximum counts as large, and parts whose does not, one row (2^20 over
+    log2(e) is 726817)."""
+    note("both sides", C, at)
+    x = torch.full((2, C), at - 2.0, device="cuda")
+    x[0, C // 2:] = at + 2.0
+    x[1, :C // 2] = at + 2.0
+    tok = torch.tensor([0, 0])
+    (logp, h, lse), _, _ = run_lp(gpu_ctx, x, tok, "f32", 0, 1.0)
+    want = lp_oracle(x, tok, 1.0)
+    # The differences are exact; a product's rounding at 2^20 is up to 2^-4 in the exponent.
+    for g, (w, _) in zip((logp, h, lse), want):
+        within(g.cpu(), w, torch.full((2,), 0.1))
