@@ -52,6 +52,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+constexpr float kFar = 0x1p20f;  // a score, in units of log 2, whose rounding is 2^-4
 
 // Bits of a chunk's place that its row sets, and the chunks left free before a row: one
 // every 4 rows, of 8 chunks (128 bytes) two every 8, so that what a wave's direct load
@@ -504,7 +505,7 @@ struct Work {
 
 // Where a tile in which not every key is visible to every row holds an infinity or NaN,
 // the matrix instructions would bring it, times 0, to rows that do not see it.  A
-// workgroup that meets such a tile does its work over, a wave an output row, lanes over
+// workgroup that meets such a tile (or, forward, scores past kFar) does its work over, a wave an output row, lanes over
 // 64 of the summed index and then over the row's columns, what is not visible left out.
 // Sum over a row's D columns of x y, x the wave's row, y the lane's (lanes that are on).
 template <int DT>
@@ -580,7 +581,7 @@ struct Rows {
     typename Ty::Frag q[NK];
     f32x16 o[NB];
     float m = -INFINITY, l = 0.0f;
-    bool bad = false;  // a tile of keys not all visible held an infinity or NaN
+    bool bad = false;  // a tile of keys not all visible held an infinity or NaN, or m is far
 
     // Scores of keys key0 .. key0 + KT - 1 (s), the visible of which, up to `last` for the
     // lane's row, become probabilities; whole: every one is visible to every row of the
@@ -606,6 +607,8 @@ struct Rows {
             const float to = fmaxf(m, top);
             const float f = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - to) * c);
             m = to;
+            // (Exponentials from a rounded m c: past kFar the rounding would be in them.)
+            bad |= fabsf(to) * c > kFar && fabsf(to) < INFINITY;
             l *= f;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -714,9 +717,8 @@ __device__ void careful_fwd(const Args &a, const Seq &sq, int kv, int split, int
             const float to = fmaxf(m, wave_max(j < end ? x : -INFINITY));
             const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - to) * c);
             m = to;
-            const float from = (m == -INFINITY ? 0.0f : m * c) - kUp;
-            const float p =
-                j < end ? __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -from)) : 0.0f;
+            const float from = m == -INFINITY ? 0.0f : m;
+            const float p = j < end ? __builtin_amdgcn_exp2f((x - from) * c + kUp) : 0.0f;
             l = (l == 0.0f ? 0.0f : l * f) + wave_add(p);
 #pragma unroll
             for (int e = 0; e < 2; ++e) acc[e] = acc[e] == 0.0f ? 0.0f : acc[e] * f;

@@ -169,3 +169,33 @@ def test_rows_of_minus_infinity_beside_keys_out_of_sight(gpu_ctx, dt, D, pad, lq
     got = b.backward(gpu_ctx, out, lse, dout)[0]
     assert (got[rows] == 0).all()
     assert torch.isfinite(got[:lq - 1].float()).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,pad", [(64, 0), (128, 0), (100, 1)])
+@pytest.mark.parametrize("lq,lk", [(1, 40), (70, 90), (300, 300), (1, 5000), (40, 4000)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_that_fp32_rounds_by_more_than_one(gpu_ctx, dt, D, pad, lq, lk, sign):
+    """Equal scores of some 1e9: every visible key counts alike.  And one key's a little larger:
+    it takes all."""
+    note("large scores", dt, D, pad, lq, lk, sign)
+    b = Batch([(lq, lk)], 2, 1, D, dt, True, pad)
+    b.q.fill_(19000.0)
+    b.k.fill_(19000.0 * sign)
+    h = DTS[dt][2]
+
+    def rows(want):
+        # Weights are equal to rounding: sums of as many terms, in any order, and P's rounding.
+        out, lse = b.forward(gpu_ctx)
+        bound = (h + U * (lk + 64)) * b.v.double().abs().cpu().max() * torch.ones(lq, D)
+        for head in range(2):
+            within(out[:, head * D:head * D + D].cpu(), want, bound, dt)
+        z = b.scale * D * (b.q[0, 0].double() * b.k[:, 0].double().max()).item()
+        assert (lse.double().cpu() - z).abs().max() <= 1e-4 * abs(z)
+
+    v = b.v.double().cpu()
+    seen = torch.arange(lk)[None] <= torch.arange(lq)[:, None] + lk - lq
+    rows((seen.double() @ v) / seen.sum(1)[:, None])
+    last = lk - lq  # (the last key that every row sees)
+    b.k[last] += 1024.0
+    rows(v[last].expand(lq, D))
