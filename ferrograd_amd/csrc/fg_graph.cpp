@@ -377,6 +377,9 @@ struct fg_plan {
     // Activations whose pre-activation is kept in 8 bits: its bytes and exponents,
     // and the shared memory that a backward restores z and act(z) into.
     std::vector<int> ck_q, ck_e, ck_z, ck_h;
+    // What attention's backward writes of operands that need no gradient: two tensors at
+    // most, one memory each for all launches (nothing reads it).
+    int unread[2] = {kNone, kNone};
     std::vector<Group> groups;
     std::vector<Slot> slots;
     char *arena = nullptr;
@@ -1274,14 +1277,16 @@ int lower_backward(fg_plan &P, bool fused, std::vector<Launch> &out) {
             L.kind = LK_ATT_BWD;
             L.sMean = gs(n);
             L.desc = "backward attention " + att_str(L) + " -> grad of node";
-            int *dst[3] = {&L.sG, &L.sH, &L.sProbs};
+            int *dst[3] = {&L.sG, &L.sH, &L.sProbs}, unread = 0;
             // One of the three that is added to makes all of them so: the call has one
             // switch for them, and the others start from zeros, as the rows of no
             // sequence do.
             for (int k = 0; k < 3; ++k) {
                 const uint32_t t = nd.in[k];
                 if (!P.needs_grad[t]) {  // the call writes all three
-                    *dst[k] = P.new_slot((uint64_t)P.shape[t].numel(), L.dtype);
+                    int &base = P.unread[unread++];
+                    if (base == kNone) base = P.new_slot(0);
+                    *dst[k] = P.new_shared(base, (uint64_t)P.shape[t].numel(), L.dtype);
                     continue;
                 }
                 *dst[k] = gs(t);
