@@ -158,7 +158,7 @@ class _Node:
     op: int
     inputs: List[int] = field(default_factory=list)
     fields: List[int] = field(default_factory=list)
-    value: float = 0.0  # constant; norms: eps; embedding, attention: scale
+    value: Optional[float] = 0.0  # constant; norms: eps; embedding, attention: scale
     heads: Sequence[int] = ()  # attention: heads, key heads, causal
     flags: int = 0
     dtype: int = 0  # DTYPE_CODE of an input / constant
@@ -233,12 +233,13 @@ class _DefineOps:
         return self._push(_Node(OP_RMS_NORM, inputs=[x, gamma], value=float(eps)))
 
     def attention(self, q, k, v, starts, heads: int, kv_heads: Optional[int] = None,
-                  scale: float = 1.0, causal: bool = True, k_starts=None) -> int:
+                  scale: Optional[float] = None, causal: bool = True, k_starts=None) -> int:
         """softmax(scale * q k^T) v of packed sequences: starts, a U32 input of n + 1
-        numbers, gives each one's rows of q, k_starts (starts) those of k and v."""
+        numbers, gives each one's rows of q, k_starts (starts) those of k and v.
+        scale None: 1/sqrt(columns of a head)."""
         return self._push(_Node(OP_ATTENTION,
                                 inputs=[q, k, v, starts, starts if k_starts is None else k_starts],
-                                value=float(scale),
+                                value=None if scale is None else float(scale),
                                 heads=(heads, heads if kv_heads is None else kv_heads, int(causal))))
 
     def embedding(self, table, tokens, scale: float = 1.0) -> int:
@@ -303,7 +304,23 @@ class Graph:
                 save[nd.inputs[0]] |= 1
         return save
 
-    def _c_graph(self, nfields: int):
+    def _columns(self, binding: Sequence[int]) -> List[int]:
+        """Columns of each node's value for a meta binding (1: a constant)."""
+        cols: List[int] = []
+        for nd in self.nodes:
+            of = [cols[x] if 0 <= x < len(cols) else 1 for x in nd.inputs]
+            if nd.op == OP_INPUT and nd.fields and nd.fields[-1] < len(binding):
+                cols.append(binding[nd.fields[-1]])
+            elif nd.op == OP_MATMUL:
+                cols.append(of[1])
+            elif nd.op in (OP_ADD, OP_SUB, OP_MUL, OP_DIV):
+                cols.append(max(of))
+            else:
+                cols.append(of[0] if of else 1)
+        return cols
+
+    def _c_graph(self, nfields: int, binding: Sequence[int]):
+        cols = self._columns(binding)
         h = ctypes.c_void_p()
         call("fg_graph_create", self.loss.code, self.optim.code, ctypes.byref(h))
         try:
@@ -325,7 +342,11 @@ class Graph:
                     call("fg_graph_rms_norm", h, *nd.inputs, nd.value, ctypes.byref(out))
                 elif nd.op == OP_ATTENTION:
                     heads, kv_heads, causal = nd.heads
-                    call("fg_graph_attention", h, *nd.inputs, heads, kv_heads, nd.value, causal,
+                    scale = nd.value
+                    if scale is None:  # (a q that there is not is the call's to refuse)
+                        of = cols[nd.inputs[0]] if nd.inputs[0] < len(cols) else 1
+                        scale = (max(heads, 1) / max(of, 1)) ** 0.5
+                    call("fg_graph_attention", h, *nd.inputs, heads, kv_heads, scale, causal,
                          ctypes.byref(out))
                 elif nd.op == OP_EMBEDDING:
                     call("fg_graph_embedding", h, *nd.inputs, nd.value, ctypes.byref(out))
@@ -347,7 +368,7 @@ class Graph:
         meta binding is given (or default dims of 16 otherwise)."""
         nf = max(meta.fields, self._nfields())
         b = list(binding) if binding is not None else [0] + [16] * nf
-        h = self._c_graph(nf)
+        h = self._c_graph(nf, b)
         try:
             arr = (ctypes.c_uint32 * len(b))(*b)
             call("fg_graph_validate", h, arr, len(b))
@@ -361,7 +382,7 @@ class Graph:
         """The fused launch list the planner builds for a meta binding (no
         device needed)."""
         nf = max(len(binding) - 1, self._nfields())
-        h = self._c_graph(nf)
+        h = self._c_graph(nf, binding)
         p = ctypes.c_void_p()
         try:
             arr = (ctypes.c_uint32 * len(binding))(*binding)
@@ -430,7 +451,7 @@ class Plan:
     def __init__(self, ctx: "GpuContext", graph: Graph, binding: Sequence[int]):
         self.ctx = ctx
         nf = max(len(binding) - 1, graph._nfields())
-        h = graph._c_graph(nf)
+        h = graph._c_graph(nf, binding)
         p = ctypes.c_void_p()
         try:
             arr = (ctypes.c_uint32 * len(binding))(*binding)
