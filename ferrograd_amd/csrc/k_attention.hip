@@ -251,6 +251,9 @@ FG_API int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, co
     a.D = D;
     a.scale = scale;
     if (int rc = check(who, dtype, a, heads, kv_heads)) return rc;
+    // (16 bits: lse enters the products' sums in units of 1 / scale.)
+    FG_REQUIRE(dtype == FG_DTYPE_F32 || scale >= 0x1p-120f, FG_ERR_UNSUPPORTED,
+               "%s: a scale of %g, in 16 bits at least 2^-120", who, (double)scale);
     a.KV = kv_heads;
     a.G = heads / kv_heads;
     a.group = fg::attn::Div((uint32_t)a.G);

@@ -389,7 +389,9 @@ int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d
  *   delta = dout_i . out_i ;  dS = P * (dout_i . v_j - delta)
  *   dq (=|+=) scale * dS k ;  dk (=|+=) scale * dS^T q ;  dv (=|+=) P^T dout
  * dk and dv are sums over the group's heads.  P and dS are rounded to dtype for their
- * products, outputs once; no atomics, the order of every sum is fixed.  Rows of dq, and
+ * products (fp16: dS with a power of two that keeps it within the type), outputs once; P is
+ * as exact as fp32 holds S and lse (2^-24 of either in its exponent); no atomics, the order
+ * of every sum is fixed.  In 16 bits scale is at least 2^-120.  Rows of dq, and
  * of dk and dv, of no sequence are left as they are.  The workspace takes 12 bytes a row
  * and head, and where tiles of 128 rows (or keys) are too few for the CUs, D floats for
  * each split (at most 32) of every row of dq (of dk and dv). */

@@ -199,3 +199,19 @@ def test_scores_that_fp32_rounds_by_more_than_one(gpu_ctx, dt, D, pad, lq, lk, s
     last = lk - lq  # (the last key that every row sees)
     b.k[last] += 1024.0
     rows(v[last].expand(lq, D))
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("scale", [2.0 ** -120, 1e-30, 1e-10])
+@pytest.mark.parametrize("D,pad", [(64, 0), (100, 1)])
+def test_small_scales(gpu_ctx, dt, scale, D, pad):
+    """Scales that leave every visible key the same weight."""
+    note("small scale", dt, scale, D, pad)
+    b = Batch([(70, 90), (1, 300)], 2, 1, D, dt, True, pad)
+    b.scale = float(scale)
+    out, lse = b.forward(gpu_ctx)
+    b.check_forward(out, lse)
+    dout = rand((b.Tq, 2 * D), dt, 9, 1.0, 0.0, pad)
+    grads = b.backward(gpu_ctx, out, lse, dout)
+    b.check_backward(grads, out, lse, dout)
+    assert bool((grads[2] != 0).any())

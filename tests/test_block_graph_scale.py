@@ -1,8 +1,10 @@
-"""CPU tests of the scale that attention nodes have where none is given: that of the direct
-call, 1/sqrt(columns of a head)."""
+"""CPU tests of attention's scale: the one that a node has where none is given, that of the direct
+call, 1/sqrt(columns of a head), and the smallest that a backward takes."""
 import pytest
 
+from ferrograd_amd import FgError, _lib
 from ferrograd_amd import graph as G
+from test_block_ops import CALLS, NO_DEVICE, UNSUPPORTED
 
 U32 = G.SimpleDType.U32
 
@@ -78,3 +80,19 @@ def test_columns_of_a_long_chain_of_sums(monkeypatch):
         o.attention(q, k, v, starts, 4)
 
     assert scales_of(monkeypatch, build, (32, 64, 3)) == [0.25]
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_backward_in_16_bits_refuses_scales_whose_reciprocal_is_past_fp32(dtype):
+    """The rows' log-sums enter its products in units of the scale."""
+    args = dict(CALLS["fg_attention_bwd"], dtype=dtype, ctx=NO_DEVICE, n=0)
+    for scale, refused in ((2.0 ** -120, False), (2.0 ** -121, dtype != 0), (1e-44, dtype != 0)):
+        args["scale"] = scale
+        if refused:
+            with pytest.raises(FgError) as e:
+                _lib.call("fg_attention_bwd", *args.values())
+            assert e.value.code == UNSUPPORTED and "scale" in str(e.value)
+        else:
+            _lib.call("fg_attention_bwd", *args.values())
+    fwd = dict(CALLS["fg_attention"], dtype=dtype, ctx=NO_DEVICE, n=0, scale=1e-44)
+    _lib.call("fg_attention", *fwd.values())
