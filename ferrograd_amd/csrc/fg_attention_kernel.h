@@ -19,6 +19,12 @@
 // 8 + 4 h + 0..3 of each 16.  Softmax statistics are a lane's own, but for the half of
 // the keys that lane ^ 32 holds.
 //
+// In 16 bits P and dS are rounded to the type between their two products, since a matrix
+// instruction takes both operands in one type: bf16 outputs are then off by 0.0018 to
+// 0.0022 of their norm, gradients by 0.0024, where their own rounding alone is 0.0015 to
+// 0.0017.  What the rounding leaves, as an operand of its own, would take half as many
+// matrix instructions again.
+//
 // Tiles sit in LDS as rows of DP elements, a few chunks apart, with 16-byte chunk c of
 // row r at c ^ swz(r): read by rows (16 lanes a cycle, the same chunk of 16 rows) and,
 // through the transposing reads, by columns (4 rows of 4 chunks a cycle), both reach
@@ -749,10 +755,13 @@ __device__ void careful_fwd(const Args &a, const Seq &sq, int kv, int split, int
 // wave's 32 queries and their sums take half of its registers at D 128 with two waves a
 // SIMD, which 16 bits need to hide the exponentials behind the other wave's products.)
 // bf16, 8 sequences of up to 4096, 32 heads of 128 over 8, causal: 680 us, 860 TFLOP/s,
-// where a square library product reaches 1213: bound by power, at 2.0 GHz (matrix units
-// busy 38 % of the cycles; reads sent further ahead, wave priorities and fewer maxima all
-// left 687 to 694).  Tiles that come through registers (heads of other widths, rows off
-// 16-byte boundaries): 4 sequences of 2048, 175 us and 187.
+// where a square library product reaches 1213 (fp16 705 us): the matrix units are busy 40 %
+// of the cycles and the vector unit about 47 %, LDS 21 %, at 2.2 GHz, where that product
+// keeps the matrix units busy 70 %, at 2.0.  Two waves a SIMD take turns at the two units;
+// reads sent further ahead, wave priorities and fewer maxima all left 687 to 694.  Tiles
+// that come through registers (heads of other widths, rows off 16-byte boundaries): 4
+// sequences of 2048, 175 us and 187.  fp32, one wave a SIMD: 8 sequences of up to 4096, 8
+// heads of 128 over 2, 1.67 ms, 88 TFLOP/s of 144.
 template <int DT>
 constexpr int keys_of() {
     return DT == kF32 ? 32 : 64;
@@ -1052,7 +1061,9 @@ constexpr float kUpP = 8.0f;   // fp16: the probabilities' that dV is summed fro
 
 // Lowers the power of dS where a lane's number (a row, or a key; both halves) would pass
 // 2^kTopDs: of the block ds and of the sums acc, by `down`, which is returned (0: as they
-// were).  What is not finite stays what it is.
+// were).  What is not finite stays what it is.  (Looking costs 8 maxima a block: backward of
+// 4 sequences of 2048, 16 heads of 64, 276 us and 287; of 8 of up to 4096, 32 heads of 128,
+// nothing.)
 template <int NB>
 __device__ __forceinline__ int lower(f32x16 &ds, f32x16 (&acc)[NB]) {
     float top = 0.0f;

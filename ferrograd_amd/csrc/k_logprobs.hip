@@ -15,8 +15,11 @@
 // a row once, with a running maximum and sums a thread that are raised together; the
 // backward reads and writes each logit once.  fp32 4096 x 50257 with 5 alternatives: 155
 // us, 5.3 TB/s (a large copy reaches 4.9); bf16 64 x 131072 with 20: 15, of which the
-// splits' pass is 10.6 and their join 5 (7.5 in all without alternatives); backward, bf16
+// splits' pass is 10.6 and their join 5 (8 in all without alternatives); backward, bf16
 // 8192 x 32000, a quarter of the rows padding: 183 us, 5 TB/s.
+//   Rows that have fewer logits above the others than alternatives are asked for take a
+// pass an alternative: masked to 10 of their columns, with 20 alternatives, 64 x 131072 114
+// us (15 with 1000 left) and 8192 x 32000 2.2 ms (0.12).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

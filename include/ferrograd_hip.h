@@ -378,6 +378,7 @@ int fg_rms_norm_bwd(fg_ctx *ctx, int dtype, const void *d_s, int lds, const void
  * product, out rounded once.  d_lse [heads][Tq] (fp32, what the backward needs) may be
  * NULL.  A row that sees no key, or none but at scores of -inf, is 0, its lse -inf.
  * Values of keys that a row does not see do not reach it, infinities and NaN included.
+ * Workgroups that meet such, or scores past 2^20 / log2(e), take a slower way.
  * Rows of no sequence are left as they are.  Tensors of no rows may be NULL.  1 <= D <=
  * 128, scale > 0.  Where rows are few and keys many, the keys' splits go to the
  * workspace: D + 2 floats for each of at most 32 a row and head. */
@@ -410,7 +411,7 @@ int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const voi
  *   probability, k < top, the lower column first among equals (NaN below all)
  * Outputs are fp32 (top_ids u32, both [R][top]); any may be NULL.  top is at most 32
  * and C.  A token outside [0, C) gives a NaN logp; logits of -inf (masked) have
- * probability 0.  scale > 0 (an inverse temperature).  Few rows of many columns are split:
+ * probability 0 (of nothing else: NaN, lse -inf).  scale > 0 (an inverse temperature).  Few rows of many columns are split:
  * 16 bytes and 8 an alternative for each of at most 16 splits a row go to the workspace. */
 int fg_token_logprobs(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
                       const uint32_t *d_tokens, int R, int C, float scale, float *d_logp,
@@ -419,8 +420,8 @@ int fg_token_logprobs(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
 /* Its backward from lse and entropy [R], with the gradients dlogp and dentropy [R]
  * (either may be NULL: 0; entropy is read where dentropy is given):
  *   dlogits[c] = scale * (dlogp * ([c = token] - p_c)
- *                         - dentropy * p_c * (z_c - lse + entropy))
- * rounded to dtype once.  dlogits may be logits (ldd = ldx).  A row whose two
+ *                         - dentropy * p_c * (z_c - lse + entropy)), p_c = exp(z_c - lse)
+ * rounded to dtype once; p_c is at most 1, however lse is rounded.  dlogits may be logits (ldd = ldx).  A row whose two
  * gradients are 0 is zeros, whatever its logits; a token outside [0, C) is no column. */
 int fg_token_logprobs_bwd(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
                           const uint32_t *d_tokens, int R, int C, float scale,

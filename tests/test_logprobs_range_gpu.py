@@ -194,3 +194,26 @@ def test_rows_on_both_sides_of_the_large_numbers(gpu_ctx, C, at):
     # The differences are exact; a product's rounding at 2^20 is up to 2^-4 in the exponent.
     for g, (w, _) in zip((logp, h, lse), want):
         within(g.cpu(), w, torch.full((2,), 0.1))
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("C", WIDTHS)
+def test_rows_of_minus_infinity_alone(gpu_ctx, dt, C):
+    """No log probabilities, and no gradients but of rows whose own are 0."""
+    note("-inf alone", dt, C)
+    x = torch.full((3, C), -math.inf, dtype=DTS[dt][1], device="cuda")
+    x[1] = 0.5
+    tok = torch.tensor([0, C - 1, C // 2])
+    top = min(C, 5)
+    (logp, h, lse), ids, tops = run_lp(gpu_ctx, x, tok, dt, top, 1.0)
+    for t in (logp, h):
+        assert torch.isnan(t).tolist() == [True, False, True]
+    assert (lse == -math.inf).tolist() == [True, False, True]
+    assert torch.equal(ids, torch.arange(top, dtype=torch.int32).expand(3, -1))
+    assert torch.isnan(tops[0]).all() and torch.isfinite(tops[1]).all()
+    out = torch.full_like(x, 7.0)
+    gpu_ctx.token_logprobs_bwd(x, C, tok.int().cuda(), 3, C, lse, out, C, entropy=h,
+                               dlogp=torch.tensor([1.0, 1.0, 0.0], device="cuda"),
+                               dtype=DTS[dt][0])
+    assert torch.isnan(out[0]).all() and torch.isfinite(out[1].float()).all()
+    assert (out[2] == 0).all()
