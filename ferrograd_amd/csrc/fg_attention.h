@@ -45,7 +45,10 @@ struct Args {
     const void *dout;
     int64_t lddo, lddq, lddk, lddv;
     void *dq, *dk, *dv;
-    float *rows;   // [3][KV Tq G]: log2 of the sum, delta, the largest |dout|
+    float *rows;   // [3][KV Tq G]: log2 of the sum, delta; of a row of large scores, the
+                   // maximum's and beside it the sum's (otherwise 0)
+    float *tiles;  // [KV][slots][4][4]: of a wave's 32 rows the largest |dout| and |delta|
+                   // (fp16), and whether one has large scores
     float *kpart;  // ksplits > 1: dK's and dV's sums, [2][ksplits][KV Tk][D] (dQ's: part)
     int kslots, ksplits, accumulate;
     int fill;  // workgroups that the splits are to come to

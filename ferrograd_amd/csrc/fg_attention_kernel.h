@@ -58,7 +58,11 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
-constexpr float kFar = 0x1p20f;  // a score, in units of log 2, whose rounding is 2^-4
+// A score, or a row's log-sum, in units of log 2, whose rounding is 2^-4 and more.
+constexpr float kFar = 0x1p20f;
+__device__ __forceinline__ bool is_far(float x, float from = kFar) {
+    return fabsf(x) > from && fabsf(x) < INFINITY;
+}
 
 // Bits of a chunk's place that its row sets, and the chunks left free before a row: one
 // every 4 rows, of 8 chunks (128 bytes) two every 8, so that what a wave's direct load
@@ -511,7 +515,7 @@ struct Work {
 
 // Where a tile in which not every key is visible to every row holds an infinity or NaN,
 // the matrix instructions would bring it, times 0, to rows that do not see it.  A
-// workgroup that meets such a tile (or, forward, scores past kFar) does its work over, a wave an output row, lanes over
+// workgroup that meets such a tile (or scores or log-sums past kFar) does its work over, a wave an output row, lanes over
 // 64 of the summed index and then over the row's columns, what is not visible left out.
 // Sum over a row's D columns of x y, x the wave's row, y the lane's (lanes that are on).
 template <int DT>
@@ -1045,7 +1049,10 @@ __global__ __launch_bounds__(256) void att_combine(const Args a) {
 // probabilities of long rows times small gradients would be subnormal.  It is taken from
 // the largest |dout| (as if V were of order 1) and lowered, the sums with it, where what is
 // carried would pass 2^15: |dS| reaches |dout| |V| D, past the type's range from |V| = 64
-// on.
+// on.  The pass over rows looks at what it carries, a power a row; the pass over keys, which
+// knows its keys' V, at what that can be, |dout| sum |V| + |delta|, a power a key.  (4
+// sequences of 2048, 16 heads of 64 over 8: 266 us for both; 297 where the second looked at
+// what it carries too.)
 __device__ __forceinline__ int exponent_above(float x) {
     return max((int)((__float_as_uint(x) & 0x7fffffffu) >> 23) - 126, -100);
 }
@@ -1059,11 +1066,9 @@ constexpr float kUpDs = 4.0f;  // its power above 1 / the largest |dout|
 constexpr int kTopDs = 15;     // and the power of two that nothing carried passes
 constexpr float kUpP = 8.0f;   // fp16: the probabilities' that dV is summed from
 
-// Lowers the power of dS where a lane's number (a row, or a key; both halves) would pass
+// Lowers the power of dS where a lane's number (of its row; both halves) would pass
 // 2^kTopDs: of the block ds and of the sums acc, by `down`, which is returned (0: as they
-// were).  What is not finite stays what it is.  (Looking costs 8 maxima a block: backward of
-// 4 sequences of 2048, 16 heads of 64, 276 us and 287; of 8 of up to 4096, 32 heads of 128,
-// nothing.)
+// were).  What is not finite stays what it is.
 template <int NB>
 __device__ __forceinline__ int lower(f32x16 &ds, f32x16 (&acc)[NB]) {
     float top = 0.0f;
@@ -1122,7 +1127,30 @@ __device__ void careful_bwd_q(const Args &a, const Seq &sq, int kv, int row0, in
         const float lse = a.lse[(int64_t)head * a.Tq + token];
         // (As in att_bwd_q: a row of no key, or of none but scores of -inf.)
         const bool none = lse == -INFINITY;
-        const float lse2 = none ? INFINITY : lse * kLog2e;
+        const int64_t rows = (int64_t)a.KV * a.Tq * a.G;
+        const int64_t at = (int64_t)kv * a.Tq * a.G + sq.q0 * a.G + row;
+        // A far row's lse is its maximum rounded, and little of its sum: both again, the sum
+        // beside the maximum (and what the product with c rounds off).
+        float lse2 = none ? INFINITY : lse * kLog2e, rest = 0.0f;
+        if (is_far(lse2)) {
+            const int all = a.causal ? min(sq.lk, i + sq.lk - sq.lq + 1) : sq.lk;
+            float m = -INFINITY, l = 0.0f;
+            for (int j0 = 0; j0 < all; j0 += 64) {
+                const bool on = j0 + lane < all;
+                const float x = dot<DT>(q, k + (j0 + lane) * a.ldk, a.D, on);
+                const float to = fmaxf(m, wave_max(on ? x : -INFINITY));
+                const float from = to == -INFINITY ? 0.0f : to;
+                l = (l == 0.0f ? 0.0f : l * __builtin_amdgcn_exp2f((m - to) * c)) +
+                    wave_add(on ? __builtin_amdgcn_exp2f((x - from) * c) : 0.0f);
+                m = to;
+            }
+            lse2 = m == -INFINITY ? INFINITY : m * c;
+            rest = m == -INFINITY ? 0.0f : __builtin_fmaf(m, c, -lse2) + __log2f(l);
+            if (blockIdx.y == 0 && lane == 0) {
+                a.rows[at] = lse2;
+                a.rows[2 * rows + at] = rest;
+            }
+        }
         const T *out = static_cast<const T *>(a.out) + token * a.ldo + col;
         float delta = 0.0f;
         for (int d = lane; d < a.D; d += 64)
@@ -1133,12 +1161,11 @@ __device__ void careful_bwd_q(const Args &a, const Seq &sq, int kv, int row0, in
             const int j = j0 + lane;
             const float x = dot<DT>(q, k + j * a.ldk, a.D, j < end);
             const float dp = dot<DT>(dout, v + j * a.ldv, a.D, j < end);
-            const float ds = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -lse2)) * (dp - delta);
+            const float ds =
+                __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -lse2) - rest) * (dp - delta);
             for (int e = 0; e < min(64, end - j0); ++e)
                 add_row<DT>(acc, __shfl(ds, e), k + (j0 + e) * a.ldk, a.D, lane);
         }
-        const int64_t rows = (int64_t)a.KV * a.Tq * a.G;
-        const int64_t at = (int64_t)kv * a.Tq * a.G + sq.q0 * a.G + row;
         if (a.splits > 1)
             put_row<kF32>(a.part + (blockIdx.y * rows + at) * a.D, acc, a.scale, a.D, lane, false);
         else
@@ -1169,7 +1196,8 @@ __device__ void careful_bwd_kv(const Args &a, const Seq &sq, int kv, int key0, i
             const bool on = r0 + lane < rows;
             const float x = dot<DT>(k, at(q, a.ldq, row), a.D, on);
             const float dp = dot<DT>(v, at(dout, a.lddo, row), a.D, on);
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -stats[row]));
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -stats[row]) -
+                                                   stats[2 * n + row]);
             const float ds = p * (dp - stats[n + row]);
             for (int e = 0; e < min(64, rows - r0); ++e) {
                 add_row<DT>(dk, __shfl(ds, e), at(q, a.ldq, r0 + e), a.D, lane);
@@ -1190,12 +1218,25 @@ __device__ void careful_bwd_kv(const Args &a, const Seq &sq, int kv, int key0, i
     }
 }
 
+// Of a sequence's rows, 32 at a time, the record that its pass over rows leaves.
+enum { kBig, kDelta, kIsFar, kRecord = 4 };
+__device__ __forceinline__ float *records(const Args &a, int seq, int kv, int q0) {
+    static_assert(kRows == 4 * 32, "a record a wave");
+    return a.tiles + ((int64_t)kv * a.slots + q0 * a.G / kRows + seq) * (4 * kRecord);
+}
+
+// Waves that a SIMD is to hold.
+template <int DT, int DP>
+constexpr int bwd_waves() {
+    return DT == kF32 ? 1 : DP == 64 ? 3 : 2;
+}
+
 // dQ, 32 rows a wave, in the forward's layout; and for the pass over the keys, in the
 // order of the key head's rows, log2 of their sums, delta and (fp16) their largest |dout|.
 // bf16, 8 sequences of up to 4096, 32 heads of 128 over 8: 0.95 ms, 930 TFLOP/s of its
 // three products.
 template <int DT, int DP, bool DMA>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<DT, DP>()))) void
 att_bwd_q(const Args a) {
     using Ty = Type<DT>;
     using T = typename Ty::T;
@@ -1253,17 +1294,26 @@ att_bwd_q(const Args a) {
     if constexpr (DT == kF16) big = fmaxf(big, __shfl_xor(big, 32));
     // A row of no key (its lse -inf): every probability 0.
     float lse2 = INFINITY;
+    bool far = false;
     if (row < rows) {
         const float x = a.lse[(int64_t)head * a.Tq + token];
         lse2 = x == -INFINITY ? INFINITY : x * kLog2e;
+        far = is_far(lse2);
         if (x == -INFINITY) delta = 0.0f;
         if (h == 0 && blockIdx.y == 0) {
             const int64_t n = (int64_t)a.KV * a.Tq * a.G;
             const int64_t at = (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G + row;
-            a.rows[at] = lse2;
+            if (!far) {  // (else the careful way's)
+                a.rows[at] = lse2;
+                a.rows[2 * n + at] = 0.0f;
+            }
             a.rows[n + at] = delta;
-            if constexpr (DT == kF16) a.rows[2 * n + at] = big;
         }
+    }
+    float tile_big = 0.0f, tile_delta = 0.0f;
+    if constexpr (DT == kF16) {
+        tile_big = wave_max(big);
+        tile_delta = wave_max(fabsf(delta));
     }
     const int last = row < rows ? last_of(row) : -1;
     int up = DT == kF16 ? (int)kUpDs - exponent_above(big) : 0;
@@ -1283,12 +1333,19 @@ att_bwd_q(const Args a) {
         mv.store(to + Tl::kElems, tid);
     };
     const Lanes<DT, DP> L(lane);
-    bool bad = false;  // a tile of keys not all visible held an infinity or NaN
+    bool bad = far;  // or a tile of keys not all visible held an infinity or NaN
     f32x16 dq[NB];
     clear(dq);
     if (t0 < t1) {
         load(t0);
         store(t0);
+    }
+    const bool any_far = __any(far);
+    if (lane == 0 && blockIdx.y == 0) {
+        float *p = records(a, pl.seq, w.kv, sq.q0) + (4 * pl.tile + wave) * kRecord;
+        p[kBig] = tile_big;
+        p[kDelta] = tile_delta;
+        p[kIsFar] = any_far;
     }
     for (int t = t0; t < t1; ++t) {
         staged<DMA>();
@@ -1364,7 +1421,7 @@ att_bwd_q(const Args a) {
 // operands of each tile) add beside them.  Through registers at D 128 the tiles' addresses spill (bf16, 4 sequences of 2048:
 // backward 0.66 ms in all, off 16-byte boundaries 1.8).
 template <int DT, int DP, bool DMA>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DT == kF32 ? 1 : 2))) void
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<DT, DP>()))) void
 att_bwd_kv(const Args a) {
     using Ty = Type<DT>;
     using T = typename Ty::T;
@@ -1408,14 +1465,17 @@ att_bwd_kv(const Args a) {
     const T *db = static_cast<const T *>(a.dout) + sq.q0 * a.lddo + (int64_t)w.kv * a.G * a.D;
     const int64_t n = (int64_t)a.KV * a.Tq * a.G;
     const float *rs = a.rows + (int64_t)w.kv * a.Tq * a.G + sq.q0 * a.G;
-    constexpr int kStats = DT == kF16 ? 3 : 2;
+    const float *tile_at = records(a, pl.seq, w.kv, sq.q0);
+    constexpr int kStats = DT == kF16 ? 3 : 2;  // fp16: a record's first two numbers too
     float sv = 0.0f;
     auto load = [&](int t) {
         T *to = lds + (t & 1) * 2 * Tl::kElems;
         const int r0 = t * RT, left = rows - r0;
         const int what = tid / RT, r = tid % RT;
-        if (what < kStats)  // (rows past the last: probability 0)
+        if (what < 2)  // (rows past the last: probability 0)
             sv = r < left ? rs[what * n + r0 + r] : what == 0 ? INFINITY : 0.0f;
+        else if (what < kStats && r < 2)
+            sv = tile_at[t * kRecord + r];
         // (From the tile's first token on.)
         const int i0 = a.group.of(r0);
         const T *qt = qb + i0 * a.ldq, *dt = db + i0 * a.lddo;
@@ -1451,10 +1511,13 @@ att_bwd_kv(const Args a) {
     f32x16 dk[NB], dv[NB];
     clear(dk);
     clear(dv);
-    int up = 0;  // fp16: the power of two that the lane's key's dK carries
-    bool any = false;
+    int up = DT == kF16 ? 100 : 0;  // fp16: the power of two that the lane's key's dK carries
+    float values = 0.0f;            // and the sum of its |V|
     const int t0 = begin + share.t0, t1 = begin + share.t1;
+    float far = 0.0f;  // (not looked at before the loop's end: nothing waits for it)
     if (t0 < t1) {
+        if (t0 + tid < t1) far = tile_at[(t0 + tid) * kRecord + kIsFar];
+        for (int t = t0 + tid + 256; t < t1; t += 256) far += tile_at[t * kRecord + kIsFar];
         Mover<DT, DP, kKeys, 256, DMA> mv;
         mv.load(vlds, tid,
                 static_cast<const T *>(a.v) + (sq.k0 + n0) * a.ldv + (int64_t)w.kv * a.D, a.ldv,
@@ -1462,6 +1525,16 @@ att_bwd_kv(const Args a) {
         mv.store(vlds, tid);
         load(t0);
         store(t0);
+        if constexpr (DT == kF16) {
+            staged<DMA>();
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) {
+                const typename Ty::Frag f = Vt::by_row(vlds, wave, ks, L);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) values += fabsf(Ty::get(f, j));
+            }
+            values += __shfl_xor(values, 32);
+        }
     }
     for (int t = t0; t < t1; ++t) {
         staged<DMA>();
@@ -1474,11 +1547,9 @@ att_bwd_kv(const Args a) {
             if (!whole) bad |= !(Tl::finite(qt, lane) && Tl::finite(dt, lane));
             float fs = 1.0f;
             if constexpr (DT == kF16) {
-                float big = st[2 * RT + l32];
-#pragma unroll
-                for (int o = 32; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o));
-                const int e = __builtin_amdgcn_readfirstlane((int)kUpDs - exponent_above(big));
-                if (!any) up = e;
+                const float big = st[2 * RT + kBig];
+                const int e = min((int)kUpDs - exponent_above(big),
+                                  kTopDs - exponent_above(big * values + st[2 * RT + kDelta]));
                 if (__any(e < up)) {
                     const float f = pow2(min(e - up, 0));
 #pragma unroll
@@ -1487,7 +1558,6 @@ att_bwd_kv(const Args a) {
                         for (int r = 0; r < 16; ++r) dk[b][r] *= f;
                     up = min(e, up);
                 }
-                any = true;
                 fs = pow2(up - (int)kUpP);
             }
             f32x16 p = kFold<DT> ? rows16(st + 4 * h) : all16(0.0f);
@@ -1540,7 +1610,6 @@ att_bwd_kv(const Args a) {
                 for (int d = 0; d < NB; ++d)
                     dv[d] = Ty::mfma(Tl::by_column(dt, 16 * u, d, L), f, dv[d]);
             }
-            if constexpr (DT == kF16) up -= lower(dp, dk);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const typename Ty::Frag f = Ty::pack(dp, u);
@@ -1551,7 +1620,7 @@ att_bwd_kv(const Args a) {
         }
         if (t + 1 < t1) store(t + 1);
     }
-    if (__syncthreads_or(bad)) {
+    if (__syncthreads_or(bad || far != 0.0f)) {
         careful_bwd_kv<DT>(a, sq, w.kv, n0, min(n0 + kKeys, sq.lk), t0 * RT, t1 * RT, wave, lane);
         return;
     }

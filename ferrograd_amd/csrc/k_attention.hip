@@ -77,16 +77,20 @@ void set_splits(int cus, int dtype, Args &a) {
     a.fill = fill - fill / 8;
 }
 
+// Work slots of the passes over rows, 128 a workgroup.
+int q_slots(const Args &a) { return (int)((int64_t)a.Tq * a.G / fg::attn::kRows + a.n); }
+
 // Floats of the backward's workspace.
 struct BwdSpace {
-    uint64_t rows, part = 0, kpart = 0;
+    uint64_t rows, tiles, part = 0, kpart = 0;
     explicit BwdSpace(const Args &a) {
         const uint64_t all = (uint64_t)std::max(a.Tq, 1) * a.KV * a.G;
         rows = (3 * all + 3) / 4 * 4;
+        tiles = 16 * (uint64_t)a.KV * q_slots(a);
         if (a.splits > 1) part = (a.splits * all * a.D + 3) / 4 * 4;
         if (a.ksplits > 1) kpart = 2 * (uint64_t)a.ksplits * a.KV * a.Tk * a.D;
     }
-    uint64_t bytes() const { return (rows + part + kpart) * sizeof(float); }
+    uint64_t bytes() const { return (rows + tiles + part + kpart) * sizeof(float); }
 };
 
 // Floats of the forward's.
@@ -293,9 +297,10 @@ FG_API int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, co
     float *ws = (float *)fg::workspace(ctx, need.bytes());
     if (!ws) return FG_ERR_OUT_OF_MEMORY;
     a.rows = ws;
-    a.part = ws + need.rows;
+    a.tiles = ws + need.rows;
+    a.part = a.tiles + need.tiles;
     a.kpart = a.part + need.part;
-    a.slots = (int)((int64_t)Tq * a.G / fg::attn::kRows + n);
+    a.slots = q_slots(a);
     a.kslots = Tk / fg::attn::kKeys + n;
     const bool dma =
         whole_chunks(a) && aligned({{d_q, ldq}, {d_k, ldk}, {d_v, ldv}, {d_dout, lddo}});

@@ -391,10 +391,11 @@ int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d
  *   dq (=|+=) scale * dS k ;  dk (=|+=) scale * dS^T q ;  dv (=|+=) P^T dout
  * dk and dv are sums over the group's heads.  P and dS are rounded to dtype for their
  * products (fp16: dS with a power of two that keeps it within the type), outputs once; P is
- * as exact as fp32 holds S and lse (2^-24 of either in its exponent); no atomics, the order
+ * as exact as fp32 holds S and lse (2^-24 of either in its exponent; of rows whose lse
+ * passes 2^20 / log2(e) the sum is taken again, a much slower way); no atomics, the order
  * of every sum is fixed.  In 16 bits scale is at least 2^-120.  Rows of dq, and
- * of dk and dv, of no sequence are left as they are.  The workspace takes 12 bytes a row
- * and head, and where tiles of 128 rows (or keys) are too few for the CUs, D floats for
+ * of dk and dv, of no sequence are left as they are.  The workspace takes 13 bytes a row
+ * and head (64 a key head and sequence), and where tiles of 128 rows (or keys) are too few for the CUs, D floats for
  * each split (at most 32) of every row of dq (of dk and dv). */
 int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k, int ldk,
                      const void *d_v, int ldv, const void *d_out, int ldo, const void *d_dout,

@@ -2,9 +2,10 @@
 gradients of any size.
 
 Tolerances are the bounds of test_attention_gpu.py, and for fp16 one term more: dS carries a
-power of two.  It brings the largest |dout| to 2^3 at least, unless the largest |dS| would pass
-2^15 with it; then it brings that above 2^14.  fp16's half step below its normal numbers, 2^-25,
-so stands for at most 2^-28 of the largest |dout| or 2^-39 of the largest |dS|.
+power of two.  It brings the largest |dout| to 2^3 at least, unless something would pass 2^15 with
+it, which it then brings to 2^14 at least: for dq the largest |dS|, for dk the largest |dout| times
+the sum of the key's |V| and the largest |delta|, which bound dS.  fp16's half step below its
+normal numbers, 2^-25, so stands for at most 2^-28 of the largest |dout| or 2^-39 of those.
 """
 import math
 
@@ -24,7 +25,7 @@ def check(b, grads, out, lse, dout):
     for s, (lq, lk) in enumerate(b.seqs):
         rq, rk = slice(b.qs[s], b.qs[s] + lq), slice(b.ks[s], b.ks[s] + lk)
         for c in range(b.kv):
-            work = []
+            work, far = [], 0.0
             for head in range(c * G, c * G + G):
                 cols = slice(head * D, head * D + D)
                 q, k, v, see, z, err = b.parts(s, head)
@@ -32,24 +33,30 @@ def check(b, grads, out, lse, dout):
                 do, o = dout[rq, cols].double().cpu(), out[rq, cols].double().cpu()
                 p = torch.where(see, torch.exp(z - L), 0.0)
                 ep = torch.where(see, 2 * err + U * (8 * L.abs() + 16), 0.0)
-                part = do @ v.t() - (do * o).sum(1)[:, None]
+                delta = (do * o).sum(1)[:, None]
+                part = do @ v.t() - delta
                 ed = U * (D + 8) * (do.abs() @ v.abs().t() + (do * o).abs().sum(1)[:, None])
                 work.append((head, cols, q, k, do, see, p, ep, p * part,
                              p * (part.abs() * ep + ed) + see * FLUSH * part.abs()))
+                far = max(far, delta.abs().max().item())
             most = max((w[8].abs() + w[9]).max().item() for w in work)
             big = max(w[4].abs().max().item() for w in work)
-            low = (2.0 ** -28 * big + 2.0 ** -39 * most) if b.dt == "f16" else 0.0
+            low, low_k = 0.0, 0.0
+            if b.dt == "f16":
+                low = 2.0 ** -28 * big + 2.0 ** -39 * most
+                low_k = 2.0 ** -28 * big + 2.0 ** -39 * 1.001 * (big * v.abs().sum(1) + far)
             tp = 2.0 ** -33 if b.dt == "f16" else FLUSH
             dk, dv, bk, bv = (torch.zeros(lk, D).double() for _ in range(4))
             for head, cols, q, k, do, see, p, ep, ds, es in work:
-                es = es + h * ds.abs() + low * see
+                es = es + h * ds.abs()
+                ek, es = es + low_k * see, es + low * see
                 dq = b.scale * (ds @ k)
                 bq = b.scale * (es @ k.abs() + U * (lk + 64) * (ds.abs() @ k.abs()))
                 assert dq.abs().max() < 6e4
                 within(got[0][rq, cols], dq, bq + 8 * U * dq.abs(), b.dt)
                 dk += b.scale * (ds.t() @ q)
                 n = lq * G
-                bk += b.scale * (es.t() @ q.abs() + U * (n + 64) * (ds.abs().t() @ q.abs()))
+                bk += b.scale * (ek.t() @ q.abs() + U * (n + 64) * (ds.abs().t() @ q.abs()))
                 dv += p.t() @ do
                 bv += (p * (h + ep)).t() @ do.abs() + (U * (n + 64) * p + tp * see).t() @ do.abs()
             cols = slice(c * D, c * D + D)
@@ -215,3 +222,54 @@ def test_small_scales(gpu_ctx, dt, scale, D, pad):
     grads = b.backward(gpu_ctx, out, lse, dout)
     b.check_backward(grads, out, lse, dout)
     assert bool((grads[2] != 0).any())
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,pad", [(64, 0), (128, 0), (100, 1)])
+@pytest.mark.parametrize("lq,lk", [(1, 40), (70, 90), (300, 300), (8, 3000)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("one", [False, True])
+def test_gradients_of_scores_that_fp32_rounds_by_more_than_one(gpu_ctx, dt, D, pad, lq, lk, sign, one):
+    """lse alone no longer holds such rows' probabilities.  Equal scores: P is 1 / n; one key's
+    larger: 1 and 0.  Beside a sequence of ordinary scores."""
+    note("gradients of large scores", dt, D, pad, lq, lk, sign, one)
+    b = Batch([(lq, lk), (40, 50)], 2, 1, D, dt, True, pad)
+    far_q, far_k = slice(0, lq), slice(0, lk)
+    b.q[far_q] = 19000.0
+    b.k[far_k] = 19000.0 * sign
+    see = torch.arange(lk)[None] <= torch.arange(lq)[:, None] + lk - lq
+    p = see.double() / see.sum(1)[:, None]
+    if one:
+        last = lk - lq  # (the last key that every row sees)
+        b.k[last] += 1024.0
+        p = torch.zeros(lq, lk).double()
+        p[:, last] = 1.0
+    out, lse = b.forward(gpu_ctx)
+    dout = rand((b.Tq, 2 * D), dt, 9, 2.0 ** -6, 0.0, pad)
+    grads = b.backward(gpu_ctx, out, lse, dout)
+    assert all(torch.equal(x, y) for x, y in zip(grads, b.backward(gpu_ctx, out, lse, dout)))
+    # The ordinary sequence, as ever.
+    near = [g.clone() for g in grads]
+    seqs, qs, ks = b.seqs, b.qs, b.ks
+    b.seqs, b.qs, b.ks = seqs[1:], qs[1:], ks[1:]
+    check(b, near, out, lse, dout)
+    b.seqs, b.qs, b.ks = seqs, qs, ks
+    # The other: everything is fp32; P is off by its sum's rounding.
+    k, v = b.k[far_k].double().cpu(), b.v[far_k].double().cpu()
+    dk, dv, bk, bv = (torch.zeros(lk, D).double() for _ in range(4))
+    for head in range(2):
+        cols = slice(head * D, head * D + D)
+        q, do, o = (t[far_q, cols].double().cpu() for t in (b.q, dout, out))
+        part = do @ v.t() - (do * o).sum(1)[:, None]
+        ds, rel = p * part, U * (lk + 64)
+        es = p * (part.abs() * rel + U * (D + 8) * (do.abs() @ v.abs().t()
+                                                    + (do * o).abs().sum(1)[:, None]))
+        dq = b.scale * (ds @ k)
+        within(grads[0][far_q, cols].cpu(), dq,
+               b.scale * ((es + ds.abs() * U * (lk + 64)) @ k.abs()) + 8 * U * dq.abs(), dt)
+        dk += b.scale * (ds.t() @ q)
+        bk += b.scale * ((es + ds.abs() * U * (2 * lq + 64)).t() @ q.abs())
+        dv += p.t() @ do
+        bv += (p * (rel + U * (2 * lq + 64))).t() @ do.abs()
+    within(grads[1][far_k].cpu(), dk, bk + 8 * U * dk.abs(), dt)
+    within(grads[2][far_k].cpu(), dv, bv + 8 * U * dv.abs(), dt)
