@@ -515,8 +515,9 @@ struct Work {
 
 // Where a tile in which not every key is visible to every row holds an infinity or NaN,
 // the matrix instructions would bring it, times 0, to rows that do not see it.  A
-// workgroup that meets such a tile (or scores or log-sums past kFar) does its work over, a wave an output row, lanes over
-// 64 of the summed index and then over the row's columns, what is not visible left out.
+// workgroup that meets such a tile (or scores or log-sums past kFar) does its work over, a
+// wave an output row, lanes over 64 of the summed index and then over the row's columns,
+// what is not visible left out.
 // Sum over a row's D columns of x y, x the wave's row, y the lane's (lanes that are on).
 template <int DT>
 __device__ __forceinline__ float dot(const typename Type<DT>::T *x, const typename Type<DT>::T *y,
@@ -1225,7 +1226,8 @@ __device__ __forceinline__ float *records(const Args &a, int seq, int kv, int q0
     return a.tiles + ((int64_t)kv * a.slots + q0 * a.G / kRows + seq) * (4 * kRecord);
 }
 
-// Waves that a SIMD is to hold.
+// Waves that a SIMD is to hold: three of tiles of 64 columns fit, left to itself the
+// compiler takes a few registers more than that for the careful way.
 template <int DT, int DP>
 constexpr int bwd_waves() {
     return DT == kF32 ? 1 : DP == 64 ? 3 : 2;
@@ -1418,8 +1420,8 @@ att_bwd_q(const Args a) {
 // for the next tile's loads in flight; 8 sequences of up to 4096, 32 heads over 8: 2.05 ms
 // and 1.6), and 64 keys a wave, for half the LDS reads, leave one wave a SIMD (2.3 ms).
 // Its four products are 740 TFLOP/s, less than dQ's three by what its LDS reads (five
-// operands of each tile) add beside them.  Through registers at D 128 the tiles' addresses spill (bf16, 4 sequences of 2048:
-// backward 0.66 ms in all, off 16-byte boundaries 1.8).
+// operands of each tile) add beside them.  Through registers at D 128 the tiles' addresses
+// spill (bf16, 4 sequences of 2048: backward 0.66 ms in all, off 16-byte boundaries 1.8).
 template <int DT, int DP, bool DMA>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(bwd_waves<DT, DP>()))) void
 att_bwd_kv(const Args a) {

@@ -393,10 +393,10 @@ int fg_attention(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d
  * products (fp16: dS with a power of two that keeps it within the type), outputs once; P is
  * as exact as fp32 holds S and lse (2^-24 of either in its exponent; of rows whose lse
  * passes 2^20 / log2(e) the sum is taken again, a much slower way); no atomics, the order
- * of every sum is fixed.  In 16 bits scale is at least 2^-120.  Rows of dq, and
- * of dk and dv, of no sequence are left as they are.  The workspace takes 13 bytes a row
- * and head (64 a key head and sequence), and where tiles of 128 rows (or keys) are too few for the CUs, D floats for
- * each split (at most 32) of every row of dq (of dk and dv). */
+ * of every sum is fixed.  In 16 bits scale is at least 2^-120.  Rows of dq, and of dk and
+ * dv, of no sequence are left as they are.  The workspace takes 13 bytes a row and head and
+ * 64 a sequence and key head, and where tiles of 128 rows (or keys) are too few for the
+ * CUs, D floats for each split (at most 32) of every row of dq (of dk and dv). */
 int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const void *d_k, int ldk,
                      const void *d_v, int ldv, const void *d_out, int ldo, const void *d_dout,
                      int lddo, const float *d_lse, const uint32_t *d_q_starts,
@@ -412,8 +412,9 @@ int fg_attention_bwd(fg_ctx *ctx, int dtype, const void *d_q, int ldq, const voi
  *   probability, k < top, the lower column first among equals (NaN below all)
  * Outputs are fp32 (top_ids u32, both [R][top]); any may be NULL.  top is at most 32
  * and C.  A token outside [0, C) gives a NaN logp; logits of -inf (masked) have
- * probability 0 (of nothing else: NaN, lse -inf).  scale > 0 (an inverse temperature).  Few rows of many columns are split:
- * 16 bytes and 8 an alternative for each of at most 16 splits a row go to the workspace. */
+ * probability 0 (of nothing else: NaN, lse -inf).  scale > 0 (an inverse temperature).  Few
+ * rows of many columns are split: 16 bytes and 8 an alternative for each of at most 16
+ * splits a row go to the workspace. */
 int fg_token_logprobs(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
                       const uint32_t *d_tokens, int R, int C, float scale, float *d_logp,
                       float *d_entropy, float *d_lse, int top, uint32_t *d_top_ids,
@@ -422,8 +423,9 @@ int fg_token_logprobs(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
  * (either may be NULL: 0; entropy is read where dentropy is given):
  *   dlogits[c] = scale * (dlogp * ([c = token] - p_c)
  *                         - dentropy * p_c * (z_c - lse + entropy)), p_c = exp(z_c - lse)
- * rounded to dtype once; p_c is at most 1, however lse is rounded.  dlogits may be logits (ldd = ldx).  A row whose two
- * gradients are 0 is zeros, whatever its logits; a token outside [0, C) is no column. */
+ * rounded to dtype once; p_c is at most 1, however lse is rounded.  dlogits may be logits
+ * (ldd = ldx).  A row whose two gradients are 0 is zeros, whatever its logits; a token
+ * outside [0, C) is no column. */
 int fg_token_logprobs_bwd(fg_ctx *ctx, int dtype, const void *d_logits, int ldx,
                           const uint32_t *d_tokens, int R, int C, float scale,
                           const float *d_lse, const float *d_entropy, const float *d_dlogp,
