@@ -682,15 +682,17 @@ __device__ __forceinline__ void write_row(const Args &a, int kv, int split, int 
         return;
     }
     const int head = kv * a.G + g;
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    const float f = 1.0f / l;
     T *p = static_cast<T *>(a.out) + token * a.ldo + (int64_t)head * a.D;
+    // (Without a sum 0, also where a value that counts nothing was infinite.)
+    auto of = [&](float x) { return l == 0.0f ? 0.0f : x * f; };
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             Ty::store4(p, 32 * b + 8 * q + 4 * h, a.D,
-                       f32x4{o[b][4 * q] * f, o[b][4 * q + 1] * f, o[b][4 * q + 2] * f,
-                             o[b][4 * q + 3] * f},
+                       f32x4{of(o[b][4 * q]), of(o[b][4 * q + 1]), of(o[b][4 * q + 2]),
+                             of(o[b][4 * q + 3])},
                        false);
     if (a.lse && h == 0)
         a.lse[(int64_t)head * a.Tq + token] =
@@ -736,6 +738,7 @@ __device__ void careful_fwd(const Args &a, const Seq &sq, int kv, int split, int
             for (int n = 0; n < min(64, end - j0); ++n)
                 add_row<DT>(acc, __shfl(p, n), v + (j0 + n) * a.ldv, a.D, lane);
         }
+        if (l == 0.0f) acc[0] = acc[1] = 0.0f;
         if (a.splits > 1) {
             const int64_t rows = (int64_t)a.KV * a.Tq * a.G;
             const int64_t at =

@@ -273,3 +273,23 @@ def test_gradients_of_scores_that_fp32_rounds_by_more_than_one(gpu_ctx, dt, D, p
         bv += (p * (rel + U * (2 * lq + 64))).t() @ do.abs()
     within(grads[1][far_k].cpu(), dk, bk + 8 * U * dk.abs(), dt)
     within(grads[2][far_k].cpu(), dv, bv + 8 * U * dv.abs(), dt)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D,pad", [(64, 0), (128, 0), (100, 1)])
+@pytest.mark.parametrize("lq,lk,hidden", [(1, 40, False), (70, 90, False), (70, 90, True),
+                                          (1, 5000, False), (200, 4000, False), (200, 4000, True)])
+def test_rows_of_minus_infinity_are_0_whatever_the_values(gpu_ctx, dt, D, pad, lq, lk, hidden):
+    """A row of none but scores of -inf is 0 also where a value that it sees is infinite (in
+    splits and not, beside an infinite key out of sight and not)."""
+    note("-inf and infinite values", dt, D, pad, lq, lk, hidden)
+    b = Batch([(lq, lk)], 2, 1, D, dt, True, pad)
+    rows = list(range(0, max(1, lq - 1), 2))
+    b.k[:, 0] = b.k[:, 0].abs() + 0.5
+    for head in range(2):
+        b.q[rows, head * D] = -math.inf
+    b.v[0] = math.inf
+    if hidden:
+        b.k[lk - 1], b.v[lk - 1] = math.inf, math.nan
+    out, lse = b.forward(gpu_ctx)
+    assert (out[rows] == 0).all() and (lse[:, rows] == -math.inf).all()
